@@ -255,6 +255,56 @@ TQ_API int tq_gqa_prefill(tq_ctx* ctx, const void* q_dev, const void* k_cache_de
                           const int* cache_start_dev, size_t batch, size_t q_len, size_t n_heads, size_t n_kv_heads,
                           size_t head_dim, size_t seq_stride, void* out_dev, int out_dtype);
 
+/* ---- log probabilities -------------------------------------------------------------------------
+ * No counterpart in the reference (its Sampler keeps the chosen token only, crates/tang-infer/src/sampling.rs:86-158).  Rows of
+ * logits x as for tq_argmax_rows, [slices][rows][ld] f32 or bf16 (ld = 0: cols), V = slices * cols of them, are a distribution
+ * p = exp(x) / sum exp(x):
+ *   logprob_out [rows][n_tokens]   log p of the given tokens [rows][n_tokens] (a negative one is padding: 0; one that does not exist: NaN)
+ *   entropy_out [rows]             -sum p log p (NULL: not wanted)
+ *   top_ids_out, top_logprob_out [rows][top]   the `top` (0 to 64, at most V) largest, largest first, the lower index among equals; -1 and
+ *                                  NaN where a row has fewer numbers
+ * A token with logit -infinity has log p = -infinity; a row that has nothing else has the entropy 0.  A NaN or an infinite logit makes
+ * its row's results NaN, but for top_ids, among which a NaN never is.  Sums are f32. */
+TQ_API int tq_token_logprobs(tq_ctx* ctx, const void* logits_dev, int dtype, size_t ld, size_t slices, size_t rows, size_t cols,
+                             const int* tokens_dev_or_null, size_t n_tokens, size_t top, float* logprob_out_dev, float* entropy_out_dev_or_null,
+                             int* top_ids_out_dev, float* top_logprob_out_dev);
+
+/* ---- pages of a cache ----------------------------------------------------------------------------
+ * No counterpart in the reference, whose KVCache holds one sequence (crates/tang-infer/src/kv_cache.rs:12-160).  A pool cuts caches of
+ * n_pages * page_rows rows (page_rows 16, 32, .. 1024) into pages that several sequences may hold: position j of sequence s is row
+ * j % page_rows of page tables[s][j / page_rows].  Its state is in device memory, the caller's or (all three NULL) the library's, which
+ * starts empty: refs [n_pages], how many sequences hold a page (0: free); tables [n_seqs][table_ld], -1 behind a sequence's pages; lens [n_seqs].
+ *
+ * All calls are asynchronous and may be recorded in a graph.  Lists are device arrays of 1 to 1024 sequence numbers, each number once
+ * (src of tq_pages_fork aside).  A call is all or nothing: with a list that breaks a rule (tq_sync: TQ_EINVAL) or without enough free pages or table
+ * entries (TQ_ENOMEM) it changes nothing.  Pages are handed out lowest number first, in the order of the list. */
+typedef struct tq_pages tq_pages;
+TQ_API int tq_pages_create(tq_ctx* ctx, size_t n_pages, size_t page_rows, size_t n_seqs, size_t table_ld, int* refs_dev_or_null,
+                           int* tables_dev_or_null, int* lens_dev_or_null, tq_pages** out);
+TQ_API int tq_pages_destroy(tq_pages* pages);
+/* The caches whose rows the pages are (keys and values of every layer): n_arrays device addresses, 16-byte aligned, of n_pages * page_rows rows
+ * of row_bytes (a multiple of 16).  Needed by the calls that copy. */
+TQ_API int tq_pages_arrays(tq_pages* pages, void* const* bases_host, size_t n_arrays, size_t row_bytes);
+TQ_API int tq_pages_data(const tq_pages* pages, int** refs_dev, int** tables_dev, int** lens_dev);
+/* Room for the next counts[i] positions (NULL: one) of each sequence, and its length that much larger.  A partly filled last page that has
+ * other holders is copied first (its rows in every array); of several listed sequences that are its only holders the last one keeps it. */
+TQ_API int tq_pages_extend(tq_pages* pages, const int* seqs_dev, const int* counts_dev_or_null, size_t n);
+/* dst[i], which must be empty, gets the positions of src[i] (the first keep[i] of them) in the same pages. */
+TQ_API int tq_pages_fork(tq_pages* pages, const int* src_dev, const int* dst_dev, const int* keep_dev_or_null, size_t n);
+TQ_API int tq_pages_free(tq_pages* pages, const int* seqs_dev, size_t n);
+/* The u pages in use become pages 0 .. u-1: those numbered u and above move, in order, to the free ones below.  u goes to *used_out. */
+TQ_API int tq_pages_compact(tq_pages* pages, int* used_out_dev_or_null);
+/* tq_gqa_decode over pages: one new token for each of `batch` sequences (seqs [batch] of the pool; NULL: b), q [batch, n_heads*128] bf16, pages
+ * bf16 [n_pages][page_rows][n_kv_heads*128], lengths from the pool (the new token's position included; 0: the result is 0).  max_len bounds
+ * them: what lies behind it is not attended.
+ * Groups (NULL: none): group g is sequences group_starts[g] .. group_starts[g+1]-1 of the batch (the last group's end is the batch's; starts
+ * ascend from 0) and shares its first shared[g] positions (at most max_shared), which are read from its first sequence's pages, once for all.
+ * out [batch, n_heads*128] bf16 or f32; all four 16-byte aligned.  A page that does not exist is skipped and reported by tq_sync. */
+TQ_API int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k_pages_dev, const void* v_pages_dev, const tq_pages* pages,
+                               const int* seqs_dev_or_null, size_t batch, const int* group_starts_dev_or_null, const int* shared_dev_or_null,
+                               size_t n_groups, size_t max_shared, size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t max_len,
+                               void* out_dev, int out_dtype);
+
 /* ---- collectives -----------------------------------------------------------------------------
  * NCCL over NVLink at the shard boundaries (the reference's only collective is a star sum over
  * QUIC, crates/tang-mesh/src/allreduce.rs:43-70).  One communicator per context; calls are

@@ -474,6 +474,16 @@ extern "C" {
     pub fn tq_gqa_decode(ctx: *mut tq_ctx, q_dev: *const c_void, k_cache_dev: *const c_void, v_cache_dev: *const c_void, lens_dev: *const c_int, batch: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, seq_stride: usize, max_len: usize, out_dev: *mut c_void, out_dtype: c_int) -> c_int;
     pub fn tq_gqa_decode_noalloc(ctx: *mut tq_ctx, q_dev: *const c_void, k_cache_dev: *const c_void, v_cache_dev: *const c_void, lens_dev: *const c_int, batch: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, seq_stride: usize, max_len: usize, out_dev: *mut c_void, out_dtype: c_int) -> c_int;
     pub fn tq_gqa_prefill(ctx: *mut tq_ctx, q_dev: *const c_void, k_cache_dev: *const c_void, v_cache_dev: *const c_void, cache_start_dev: *const c_int, batch: usize, q_len: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, seq_stride: usize, out_dev: *mut c_void, out_dtype: c_int) -> c_int;
+    pub fn tq_token_logprobs(ctx: *mut tq_ctx, logits_dev: *const c_void, dtype: c_int, ld: usize, slices: usize, rows: usize, cols: usize, tokens_dev_or_null: *const c_int, n_tokens: usize, top: usize, logprob_out_dev: *mut f32, entropy_out_dev_or_null: *mut f32, top_ids_out_dev: *mut c_int, top_logprob_out_dev: *mut f32) -> c_int;
+    pub fn tq_pages_create(ctx: *mut tq_ctx, n_pages: usize, page_rows: usize, n_seqs: usize, table_ld: usize, refs_dev_or_null: *mut c_int, tables_dev_or_null: *mut c_int, lens_dev_or_null: *mut c_int, out: *mut *mut tq_pages) -> c_int;
+    pub fn tq_pages_destroy(pages: *mut tq_pages) -> c_int;
+    pub fn tq_pages_arrays(pages: *mut tq_pages, bases_host: *const *mut c_void, n_arrays: usize, row_bytes: usize) -> c_int;
+    pub fn tq_pages_data(pages: *const tq_pages, refs_dev: *mut *mut c_int, tables_dev: *mut *mut c_int, lens_dev: *mut *mut c_int) -> c_int;
+    pub fn tq_pages_extend(pages: *mut tq_pages, seqs_dev: *const c_int, counts_dev_or_null: *const c_int, n: usize) -> c_int;
+    pub fn tq_pages_fork(pages: *mut tq_pages, src_dev: *const c_int, dst_dev: *const c_int, keep_dev_or_null: *const c_int, n: usize) -> c_int;
+    pub fn tq_pages_free(pages: *mut tq_pages, seqs_dev: *const c_int, n: usize) -> c_int;
+    pub fn tq_pages_compact(pages: *mut tq_pages, used_out_dev_or_null: *mut c_int) -> c_int;
+    pub fn tq_gqa_decode_paged(ctx: *mut tq_ctx, q_dev: *const c_void, k_pages_dev: *const c_void, v_pages_dev: *const c_void, pages: *const tq_pages, seqs_dev_or_null: *const c_int, batch: usize, group_starts_dev_or_null: *const c_int, shared_dev_or_null: *const c_int, n_groups: usize, max_shared: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, max_len: usize, out_dev: *mut c_void, out_dtype: c_int) -> c_int;
     pub fn tq_comm_unique_id(id_out128: *mut c_void) -> c_int;
     pub fn tq_comm_create(ctx: *mut tq_ctx, id128: *const c_void, rank: c_int, world: c_int, out: *mut *mut tq_comm) -> c_int;
     pub fn tq_comm_destroy(ctx: *mut tq_ctx, comm: *mut tq_comm) -> c_int;

@@ -64,6 +64,16 @@ PROTOTYPES = {
     "tq_gqa_decode": (_i, [_p, _p, _p, _p, _p, _sz, _sz, _sz, _sz, _sz, _sz, _p, _i]),
     "tq_gqa_prefill": (_i, [_p, _p, _p, _p, _p, _sz, _sz, _sz, _sz, _sz, _sz, _p, _i]),
     "tq_gqa_decode_noalloc": (_i, [_p, _p, _p, _p, _p, _sz, _sz, _sz, _sz, _sz, _sz, _p, _i]),
+    "tq_token_logprobs": (_i, [_p, _p, _i, _sz, _sz, _sz, _sz, _p, _sz, _sz, _p, _p, _p, _p]),
+    "tq_pages_create": (_i, [_p, _sz, _sz, _sz, _sz, _p, _p, _p, _pp]),
+    "tq_pages_destroy": (_i, [_p]),
+    "tq_pages_arrays": (_i, [_p, _pp, _sz, _sz]),
+    "tq_pages_data": (_i, [_p, _pp, _pp, _pp]),
+    "tq_pages_extend": (_i, [_p, _p, _p, _sz]),
+    "tq_pages_fork": (_i, [_p, _p, _p, _p, _sz]),
+    "tq_pages_free": (_i, [_p, _p, _sz]),
+    "tq_pages_compact": (_i, [_p, _p]),
+    "tq_gqa_decode_paged": (_i, [_p, _p, _p, _p, _p, _p, _sz, _p, _p, _sz, _sz, _sz, _sz, _sz, _sz, _p, _i]),
     "tq_comm_unique_id": (_i, [_p]),
     "tq_comm_create": (_i, [_p, _p, _i, _i, _pp]),
     "tq_comm_destroy": (_i, [_p, _p]),

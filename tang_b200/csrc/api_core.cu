@@ -201,6 +201,10 @@ int tq_sync(tq_ctx* ctx) {
     if (ctx->gemm_ws2) cudaMemset(ctx->gemm_ws2, 0, ctx->gemm_ws2_bytes);   // ... or parked partial sums
     if (code == 6)   // DERR_POSITION
       return fail(ctx, TQ_EINVAL, "a sequence position outside the KV cache reached a kernel (the access was skipped): positions must stay below max_seq");
+    if (code == 7)   // DERR_PAGES
+      return fail(ctx, TQ_ENOMEM, "not enough free pages, or a sequence's table is full: the call changed nothing");
+    if (code == 8)   // DERR_PAGE_LIST
+      return fail(ctx, TQ_EINVAL, "a list of sequences names one that does not exist, is not in the state that the call needs, or stands in it twice, or a table names a page that does not exist");
     return fail(ctx, TQ_ETIMEOUT, "a kernel gave up a bounded wait (device code %d)", code);
   }
   return TQ_OK;

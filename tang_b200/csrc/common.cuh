@@ -19,6 +19,8 @@ enum DeviceErr : int {
   DERR_PEER_WAIT = 4,    // gave up waiting for a peer rank's flag
   DERR_TMEM = 5,         // tensor-memory allocation / MMA completion wait gave up
   DERR_POSITION = 6,     // a sequence position outside the cache (or the RoPE tables): the access was skipped
+  DERR_PAGES = 7,        // a pool of pages ran out, or a sequence's table did: the call changed nothing
+  DERR_PAGE_LIST = 8,    // a list of sequences with one that does not exist, or twice the same, or a table with such a page
 };
 
 // Upper bound on polls of one barrier before a kernel records an error and moves on.  Each poll

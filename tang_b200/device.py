@@ -180,6 +180,24 @@ class QuantComputeDevice:
                                       _opt_ptr(rng_states), _opt_ptr(past), _opt_ptr(past_lens), past_ld, C.c_void_p(out.ptr)))
         return out
 
+    def token_logprobs(self, logits: Buffer, rows: int, cols: int, tokens: Buffer | None = None, n_tokens: int = 1, top: int = 0, slices: int = 1,
+                       ld: int = 0, entropy: bool = True, out: TokenLogprobs | None = None) -> TokenLogprobs:
+        """Log probabilities of the given tokens (int32 [rows, n_tokens]) under rows of f32 or bf16 logits, the rows' entropies and their `top` most
+        likely tokens (``tq_token_logprobs``).  `out`: buffers of an earlier call to write to."""
+        n_tokens = 0 if tokens is None else n_tokens
+        if logits.n < ((slices * rows - 1) * (ld or cols) + cols if rows else 0) or (tokens is not None and tokens.n != rows * n_tokens):
+            raise TangqError(_lib.TQ_EINVAL, f"token_logprobs: {logits.n} logits or {0 if tokens is None else tokens.n} tokens do not match the shapes")
+        if out is None:
+            out = TokenLogprobs(self.alloc(rows * n_tokens) if n_tokens else None, self.alloc(rows) if entropy else None,
+                                self.alloc(rows * top, _lib.I32) if top else None, self.alloc(rows * top) if top else None)
+        for b, n in ((out.logprobs, rows * n_tokens), (out.entropy, rows if entropy else 0), (out.top_ids, rows * top), (out.top_logprobs, rows * top)):
+            if n and (b is None or b.n < n):
+                raise TangqError(_lib.TQ_EINVAL, f"token_logprobs: a result needs room for {n} values")
+        self._check(self._L.tq_token_logprobs(self._ctx, C.c_void_p(logits.ptr), logits.dtype, ld, slices, rows, cols, _opt_ptr(tokens), n_tokens, top,
+                                              _opt_ptr(out.logprobs), _opt_ptr(out.entropy if entropy else None), _opt_ptr(out.top_ids),
+                                              _opt_ptr(out.top_logprobs)))
+        return out
+
     def upload_bf16(self, data_f32) -> Buffer:
         """Uploads f32 data and narrows it to bf16 on the device (round to nearest even)."""
         tmp = self.upload(data_f32, F32)
@@ -335,6 +353,15 @@ class SamplerConfig(C.Structure):
     _fields_ = [("temperature", C.c_double), ("top_k", C.c_uint64), ("top_p", C.c_double), ("repetition_penalty", C.c_double)]
 
 
+@dataclass
+class TokenLogprobs:
+    """What ``token_logprobs`` writes: f32 [rows, n_tokens], f32 [rows], int32 and f32 [rows, top] (None: not wanted)."""
+    logprobs: Buffer | None = None
+    entropy: Buffer | None = None
+    top_ids: Buffer | None = None
+    top_logprobs: Buffer | None = None
+
+
 class Graph:
     def __init__(self, dev: QuantComputeDevice, handle: int):
         self.dev, self.handle = dev, handle
@@ -436,6 +463,26 @@ def _add_ops(cls):
         out._keep = cb
         return out
 
+    def gqa_decode_paged(self, q: Buffer, k_pages: Buffer, v_pages: Buffer, pool, batch: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int,
+                         seqs: Buffer | None = None, group_starts: Buffer | None = None, shared: Buffer | None = None, n_groups: int = 0,
+                         max_shared: int = 0, out: Buffer | None = None, out_dtype: int = BF16) -> Buffer:
+        """``gqa_decode`` over the pages of a ``PagePool`` (``tq_gqa_decode_paged``): one new token for each of `batch` sequences `seqs` (0 .. batch-1
+        unless given) of the pool.  Group g is sequences group_starts[g] .. group_starts[g+1]-1 of the batch and shares its first shared[g] <= max_shared
+        positions."""
+        rows = pool.n_pages * pool.page_rows * n_kv_heads * head_dim
+        if q.n != batch * n_heads * head_dim or k_pages.n != rows or v_pages.n != rows or (seqs is not None and seqs.n < batch):
+            raise TangqError(_lib.TQ_EINVAL, "gqa_decode_paged: buffer sizes do not match the shapes")
+        if group_starts is not None and (group_starts.n < n_groups or shared is None or shared.n < n_groups):
+            raise TangqError(_lib.TQ_EINVAL, "gqa_decode_paged: fewer starts or shared lengths than groups")
+        if out is None:
+            out = self.alloc(q.n, out_dtype)
+        elif out.n != q.n:
+            raise TangqError(_lib.TQ_EINVAL, "gqa_decode_paged: the output has another size than the queries")
+        self._check(self._L.tq_gqa_decode_paged(self._ctx, C.c_void_p(q.ptr), C.c_void_p(k_pages.ptr), C.c_void_p(v_pages.ptr), C.c_void_p(pool.handle),
+                                                _opt_ptr(seqs), batch, _opt_ptr(group_starts), _opt_ptr(shared), n_groups, max_shared, n_heads, n_kv_heads,
+                                                head_dim, max_len, C.c_void_p(out.ptr), out.dtype))
+        return out
+
     def concat_rows(self, parts) -> QBuffer:
         arr = (C.c_void_p * len(parts))(*[p.handle for p in parts])
         h = C.c_void_p()
@@ -453,7 +500,7 @@ def _add_ops(cls):
         return out
 
     for f in (rms_norm, rms_norm_residual, rope_tables, rope_forward, swiglu_fused, embedding, kv_attention, gqa_decode,
-              gqa_prefill, concat_rows, interleave_gate_up):
+              gqa_prefill, gqa_decode_paged, concat_rows, interleave_gate_up):
         setattr(cls, f.__name__, f)
 
 

@@ -1,0 +1,313 @@
+"""Decode attention over pages (tq_gqa_decode_paged) against 64 bits: lengths from nothing to long ones, groups that share a prefix, every page
+size and group of heads, rows behind a sequence's end that hold NaN, pages that do not exist, refusals."""
+import numpy as np
+import pytest
+
+from util import bf16_round
+
+pytestmark = pytest.mark.gpu
+HD = 128
+NAN = 0x7FC0
+
+
+@pytest.fixture(scope="module")
+def dev():
+    import tang_b200
+
+    d = tang_b200.QuantComputeDevice(0)
+    yield d
+    d.close()
+
+
+class Setup:
+    """Sequences in a pool: `groups` is a list of (shared positions, lengths of the members); every row that nobody holds is NaN."""
+
+    def __init__(self, nh, nkv, P, groups, seed, extra=3, q_std=1.5, order=None):
+        rng = np.random.default_rng(seed)
+        self.nh, self.nkv, self.P = nh, nkv, P
+        lens = np.array([n for _, m in groups for n in m])
+        self.B, self.lens = len(lens), lens
+        held = -(-lens // P)
+        self.ld = max(1, int(held.max())) + 1
+        self.starts = np.cumsum([0] + [len(m) for _, m in groups]).astype(np.int32)
+        self.shared = np.array([s for s, _ in groups], np.int32)
+        n_pages = int(held.sum()) + extra
+        free = rng.permutation(n_pages).tolist()
+        self.tables = np.full((self.B, self.ld), -1, np.int32)
+        for g, (s, m) in enumerate(groups):
+            first = int(self.starts[g])
+            whole = s // P
+            for b in range(first, first + len(m)):
+                for j in range(held[b]):
+                    share = b > first and j < whole and j < held[first]
+                    self.tables[b, j] = self.tables[first, j] if share else free.pop()
+        self.n_pages = n_pages
+        self.q_bits, self.q = bf16_round((rng.standard_normal((self.B, nh, HD)) * q_std).astype(np.float32))
+        self.kv_bits = np.full((2, n_pages, P, nkv, HD), NAN, np.uint16)
+        self.kv = np.zeros((2, n_pages, P, nkv, HD), np.float32)
+        for b in range(self.B):
+            for j in range(held[b]):
+                rows = min(P, int(lens[b]) - j * P)
+                bits, f = bf16_round(rng.standard_normal((2, rows, nkv, HD)).astype(np.float32))
+                page = self.tables[b, j]
+                self.kv_bits[:, page, :rows], self.kv[:, page, :rows] = bits.reshape(f.shape), f
+        # the part of the shared positions that is no whole page is the same in every member's own page
+        for g, (s, m) in enumerate(groups):
+            first, whole, rest = int(self.starts[g]), s // P, s % P
+            for b in range(first + 1, first + len(m)):
+                n = min(rest, int(lens[b]) - whole * P, int(lens[first]) - whole * P)
+                if n > 0:
+                    for a in (self.kv_bits, self.kv):
+                        a[:, self.tables[b, whole], :n] = a[:, self.tables[first, whole], :n]
+
+    def put(self, dev, seqs=None):
+        import tang_b200 as tb
+
+        self.dev = dev
+        refs = np.zeros(self.n_pages, np.int32)
+        np.add.at(refs, self.tables[self.tables >= 0], 1)
+        tables, lens = self.tables, self.lens.astype(np.int32)
+        n = self.B
+        self.seqs = None
+        if seqs is not None:           # the batch is these sequences of a larger pool
+            n = int(max(seqs)) + 1
+            t, l = np.full((n, self.ld), -1, np.int32), np.zeros(n, np.int32)
+            t[seqs], l[seqs] = tables, lens
+            tables, lens = t, l
+            self.seqs = dev.upload(np.array(seqs, np.int32), tb.I32)
+        self.state = [dev.upload(a, tb.I32) for a in (refs, tables, lens)]
+        self.pool = tb.PagePool(dev, self.n_pages, self.P, n, self.ld, None, *self.state)
+        self.qb, self.kb, self.vb = (dev.upload(a.reshape(-1), tb.BF16) for a in (self.q_bits, self.kv_bits[0], self.kv_bits[1]))
+        self.gb, self.sb = dev.upload(self.starts, tb.I32), dev.upload(self.shared, tb.I32)
+        return self
+
+    def run(self, f32, grouped=True, max_len=None, out=None):
+        import tang_b200 as tb
+
+        kw = {"group_starts": self.gb, "shared": self.sb, "n_groups": len(self.shared), "max_shared": int(self.shared.max())} if grouped else {}
+        return self.dev.gqa_decode_paged(self.qb, self.kb, self.vb, self.pool, self.B, self.nh, self.nkv, HD, max_len or max(1, int(self.lens.max())), seqs=self.seqs,
+                                         out=out, out_dtype=tb.F32 if f32 else tb.BF16, **kw)
+
+    def reference(self):
+        """(result, sum of the weights times the values' sizes), 64 bits."""
+        out, size = np.zeros((self.B, self.nh, HD)), np.zeros((self.B, self.nh, HD))
+        for b in range(self.B):
+            n = int(self.lens[b])
+            if not n:
+                continue
+            pages = self.tables[b, :-(-n // self.P)]
+            k, v = (self.kv[i, pages].reshape(-1, self.nkv, HD)[:n].astype(np.float64).transpose(1, 0, 2) for i in (0, 1))
+            q = self.q[b].astype(np.float64).reshape(self.nkv, -1, HD)
+            s = q @ k.transpose(0, 2, 1) / np.sqrt(HD)
+            e = np.exp(s - s.max(-1, keepdims=True))
+            w = e / e.sum(-1, keepdims=True)
+            out[b], size[b] = (w @ v).reshape(self.nh, HD), (w @ np.abs(v)).reshape(self.nh, HD)
+        return out, size
+
+    def check(self, got, f32, rows=slice(None)):
+        """f32: the weights are two bf16 terms (2^-16 of themselves) and the scores, sums of 128 exact products in f32, are off by 2^-23 of their parts' sum
+        per step of 16 (at most 2^-17 here), every sum of up to 2^12 steps likewise: 2^-14 of the sum of |weight value|.  bf16: one term of the weights
+        (2^-9) and the result's rounding (2^-9) more."""
+        want, size = self.reference()
+        got = got.astype(np.float64) if f32 else (got.astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+        got = got.reshape(want.shape)
+        tol = (2.0 ** -14 if f32 else 2.0 ** -14 + 2.0 ** -8) * size + 1e-30
+        assert np.isfinite(got[rows]).all()
+        err = np.abs(got - want)[rows] / tol[rows]
+        assert err.max() <= 1, (err.max(), np.unravel_index(err.argmax(), err.shape))
+
+
+CASES = {
+    "one": (8, 2, 16, [(0, [1])]),
+    "nothing": (8, 2, 16, [(0, [0])]),
+    "lengths": (8, 2, 16, [(0, [0]), (0, [1]), (0, [15]), (0, [16]), (0, [17]), (0, [63]), (0, [64]), (0, [65]), (0, [127]), (0, [128]), (0, [129]), (0, [700])]),
+    "samples": (8, 2, 16, [(64, [65, 70, 64, 100])]),
+    "odd prefix": (32, 8, 32, [(135, [136, 300, 135, 140, 136, 190])]),
+    "groups": (16, 4, 16, [(0, [5]), (130, [131, 260]), (1, [1, 2, 3]), (600, [601, 640, 700, 601, 601]), (0, [33])]),
+    "one to one": (8, 8, 64, [(256, [257, 300, 511]), (129, [129, 129])]),
+    "one kv head": (8, 1, 128, [(1024, [1025, 1100] + [1030] * 15)]),
+    "three to one": (6, 2, 256, [(700, [701, 900, 777]), (0, [255])]),
+    "five to one": (5, 1, 16, [(384, [400] * 30)]),
+    "many": (32, 8, 64, [(512, [513 + 7 * i for i in range(64)])]),
+    "long": (8, 2, 16, [(0, [9001]), (4096, [4097, 4500]), (0, [3])]),
+    "short members": (16, 4, 16, [(512, [600, 100, 0, 513, 511])]),
+    "empty first": (16, 4, 16, [(512, [0, 0, 0])]),
+    "pages of 1024": (8, 2, 1024, [(1500, [1501, 1600, 2049]), (0, [1024])]),
+    "two hundred": (4, 4, 32, [(256, [257 + i % 40 for i in range(200)])]),
+}
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("name", list(CASES))
+def test_against_64_bits(dev, name, f32):
+    s = Setup(*CASES[name], seed=len(name)).put(dev)
+    got = s.run(f32).to_vec()
+    dev.sync()
+    s.check(got, f32)
+    alone = s.run(f32, grouped=False).to_vec()
+    dev.sync()
+    s.check(alone, f32)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("P", [16, 32, 64, 128, 256, 512, 1024])
+def test_every_page_size(dev, P, f32):
+    s = Setup(8, 2, P, [(3 * P // 2 + 130, [3 * P // 2 + 131, 2 * P + 200, 3 * P + 300])], seed=P).put(dev)
+    got = s.run(f32).to_vec()
+    dev.sync()
+    s.check(got, f32)
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_drawn_batches(dev, seed):
+    rng = np.random.default_rng(seed + 500)
+    nkv, group, P = int(rng.choice([1, 2, 3, 8])), int(rng.integers(1, 9)), int(rng.choice([16, 32, 64, 128]))
+    groups = []
+    for _ in range(rng.integers(1, 7)):
+        shared = int(rng.choice([0, 5, 128, 200, 1000]))
+        groups.append((shared, [shared + int(rng.integers(0, 400)) + 1 for _ in range(rng.integers(1, 12))]))
+    s = Setup(nkv * group, nkv, P, groups, seed)
+    s.put(dev, rng.permutation(s.B + 9)[:s.B].tolist())
+    for f32 in (False, True):
+        got = s.run(f32).to_vec()
+        dev.sync()
+        s.check(got, f32)
+
+
+def test_sharp_and_flat_scores(dev):
+    for std in (0.0, 40.0):
+        s = Setup(8, 2, 16, [(256, [300, 290, 400]), (0, [77])], seed=3, q_std=std).put(dev)
+        got = s.run(True).to_vec()
+        dev.sync()
+        want, size = s.reference()
+        # scores of size 40 * 128 / sqrt(128): 2^-23 of each of eight steps
+        assert (np.abs(got.reshape(want.shape) - want) <= (2.0 ** -14 + std * 40 * 2.0 ** -20) * size + 1e-30).all()
+
+
+def test_max_len_cuts_and_rows_behind_the_batch_stay(dev):
+    import tang_b200 as tb
+
+    s = Setup(8, 2, 16, [(128, [300, 200, 150])], seed=8).put(dev)
+    out = dev.upload(np.full((s.B + 1) * 8 * HD, 5, np.float32))
+    part = tb.Buffer(dev, out.ptr, s.B * 8 * HD, tb.F32, owns=False)
+    s.run(True, max_len=180, out=part)
+    dev.sync()
+    s.lens = np.minimum(s.lens, 180)
+    got = out.to_vec()
+    s.check(got[:-8 * HD], True)
+    assert (got[-8 * HD:] == 5).all()
+
+
+def test_infinities_reach_only_those_who_see_them(dev):
+    s = Setup(8, 2, 16, [(256, [300, 257, 400]), (0, [40])], seed=9)
+    bits = [0x7F80, NAN]
+    s.kv_bits[1, s.tables[0, 290 // 16], 290 % 16, :, 3] = bits[0]          # sequence 0 alone
+    s.kv_bits[1, s.tables[2, 390 // 16], 390 % 16, :, 4] = bits[1]          # sequence 2 alone
+    s.put(dev)
+    for f32 in (False, True):
+        got = s.run(f32).to_vec()
+        dev.sync()
+        g = got.reshape(4, 8, HD).astype(np.float64) if f32 else (got.astype(np.uint32) << 16).view(np.float32).astype(np.float64).reshape(4, 8, HD)
+        assert (g[0, :, 3] == np.inf).all() and np.isnan(g[2, :, 4]).all()
+        mask = np.isfinite(g)
+        mask[0, :, 3] = mask[2, :, 4] = True
+        assert mask.all()
+        want, size = s.reference()
+        ok = np.isfinite(g)
+        assert (np.abs(g - want)[ok] <= (2.0 ** -14 + 2.0 ** -8) * size[ok]).all()
+
+
+def test_pages_and_sequences_that_do_not_exist_are_reported(dev):
+    import tang_b200 as tb
+
+    for page in (-1, 10 ** 6, -2 ** 31):
+        s = Setup(8, 2, 16, [(256, [300, 290]), (0, [77]), (0, [200])], seed=10)
+        s.tables[0, 2] = s.tables[1, 2] = s.tables[3, 4] = page
+        refs = s.tables.copy()
+        s.tables = np.where((refs < 0) | (refs >= s.n_pages), -1, refs)      # (for the reference counts)
+        s.put(dev)
+        dev.upload_into(s.pool.tables, refs)
+        got = s.run(True).to_vec()
+        with pytest.raises(tb.TangqError) as e:
+            dev.sync()
+        assert e.value.status == tb._lib.TQ_EINVAL
+        dev.sync()
+        s.check(got, True, rows=slice(2, 3))                  # the sequence whose pages exist
+    s = Setup(8, 2, 16, [(0, [77]), (0, [20])], seed=11).put(dev, [3, 1])
+    dev.upload_into(s.seqs, np.array([3, 99], np.int32))
+    got = s.run(True).to_vec()
+    with pytest.raises(tb.TangqError):
+        dev.sync()
+    s.check(got, True, rows=slice(0, 1))
+    assert (got.reshape(2, -1)[1] == 0).all()
+    dev.sync()
+
+
+def test_the_same_bits_again_from_a_graph_and_beside_another_handle(dev):
+    import tang_b200 as tb
+
+    s = Setup(32, 8, 32, [(640, [700 + 9 * i for i in range(20)]), (0, [1500])], seed=12).put(dev)
+    out = s.run(True)
+    first = out.to_vec()
+    dev.sync()
+    other = tb.QuantComputeDevice(0)
+    z = Setup(8, 2, 16, [(256, [600] * 9)], seed=13).put(other)
+    dev.begin_capture()
+    s.run(True, out=out)
+    g = dev.end_capture()
+    for _ in range(3):
+        dev.memset(out, 1)
+        g.launch()
+        second = z.run(True)
+        dev.sync()
+        other.sync()
+        assert np.array_equal(out.to_vec(), first)
+        z.check(second.to_vec(), True)
+    # a longer cache under the same graph: the lengths are the device's
+    g.free()
+    del second
+    for b in (z.pool, z.qb, z.kb, z.vb, z.gb, z.sb, *z.state):
+        b.destroy() if hasattr(b, "destroy") else b.free()
+    other.close()
+
+
+def test_pages_behind_32_bits(dev):
+    """Rows whose offset in elements is larger than 2^32."""
+    import tang_b200 as tb
+
+    nh, nkv, P, n_pages = 8, 8, 1024, 4200                    # 1024 elements a row, 2^20 a page
+    k, v = (dev.alloc(n_pages * P * nkv * HD, tb.BF16) for _ in range(2))
+    s = Setup(nh, nkv, P, [(1024, [1030, 1100])], seed=14)
+    far = {int(p): n_pages - 1 - i for i, p in enumerate(sorted(set(s.tables[s.tables >= 0].tolist())))}
+    for buf, src in ((k, s.kv_bits[0]), (v, s.kv_bits[1])):
+        for p, to in far.items():
+            dev.upload_into(tb.Buffer(dev, buf.ptr + to * P * nkv * HD * 2, P * nkv * HD, tb.BF16, owns=False), src[p])
+    tables = np.array([[far.get(int(p), -1) for p in row] for row in s.tables], np.int32)
+    refs = np.zeros(n_pages, np.int32)
+    pool = tb.PagePool(dev, n_pages, P, 2, s.ld, None, dev.upload(refs, tb.I32), dev.upload(tables, tb.I32), dev.upload(s.lens.astype(np.int32), tb.I32))
+    q = dev.upload(s.q_bits.reshape(-1), tb.BF16)
+    for grouped in (False, True):
+        kw = {"group_starts": dev.upload(s.starts, tb.I32), "shared": dev.upload(s.shared, tb.I32), "n_groups": 1, "max_shared": 1024} if grouped else {}
+        got = dev.gqa_decode_paged(q, k, v, pool, 2, nh, nkv, HD, 1100, out_dtype=tb.F32, **kw).to_vec()
+        dev.sync()
+        s.check(got, True)
+
+
+def test_refusals(dev):
+    import tang_b200 as tb
+
+    s = Setup(8, 2, 16, [(16, [20, 30])], seed=15).put(dev)
+    call = dev.gqa_decode_paged
+    base = dict(q=s.qb, k_pages=s.kb, v_pages=s.vb, pool=s.pool, batch=2, n_heads=8, n_kv_heads=2, head_dim=HD, max_len=30)
+    wide = dev.alloc(2 * 18 * HD, tb.BF16)
+    for kw in ({"batch": 3}, {"n_heads": 4}, {"max_len": 0}, {"n_kv_heads": 4}, {"group_starts": s.gb}, {"group_starts": s.gb, "shared": s.sb, "n_groups": 2},
+               {"group_starts": s.gb, "shared": s.sb, "n_groups": 0}, {"head_dim": 64, "q": dev.alloc(2 * 8 * 64, tb.BF16), "k_pages": dev.alloc(s.n_pages * 16 * 128, tb.BF16),
+                                                                      "v_pages": dev.alloc(s.n_pages * 16 * 128, tb.BF16)},
+               {"n_heads": 18, "q": wide}, {"out": dev.alloc(2 * 8 * HD, tb.I32)}, {"out": dev.alloc(8, tb.F32)}, {"seqs": dev.alloc(1, tb.I32)}):
+        with pytest.raises(tb.TangqError):
+            call(**{**base, **kw})
+    off = tb.Buffer(dev, s.qb.ptr + 2, s.qb.n, tb.BF16, owns=False)
+    with pytest.raises(tb.TangqError):
+        call(**{**base, "q": off})
+    call(**base)
+    dev.sync()

@@ -1,0 +1,217 @@
+"""Pages of a cache (tq_pages_*) against their definition in plain Python: state, rows copied, refusals, graphs."""
+import numpy as np
+import pytest
+
+from pages_util import Pool, Refused
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    import tang_b200
+
+    d = tang_b200.QuantComputeDevice(0)
+    yield d
+    d.close()
+
+
+class Both:
+    """A pool on the device and its definition, with caches whose rows carry their first place."""
+
+    def __init__(self, dev, n_pages, P, n_seqs, ld, n_arrays=3, row=8):
+        import tang_b200 as tb
+
+        self.dev, self.want, self.P = dev, Pool(n_pages, P, n_seqs, ld), P
+        rng = np.random.default_rng(n_pages)
+        self.data = rng.integers(0, 1 << 16, (n_arrays, n_pages, P, row)).astype(np.uint16)
+        self.bufs = [dev.upload(a, tb.BF16) for a in self.data]
+        self.pool = tb.PagePool(dev, n_pages, P, n_seqs, ld, self.bufs)
+
+    def copy(self, copies):
+        for a, b, n in copies:
+            self.data[:, b, :n] = self.data[:, a, :n]
+
+    def check(self):
+        self.dev.sync()
+        refs, tables, lens = self.pool.state()
+        assert np.array_equal(refs, self.want.refs) and np.array_equal(tables, self.want.tables) and np.array_equal(lens, self.want.lens)
+        self.want.sound()
+        for b, d in zip(self.bufs, self.data):
+            assert np.array_equal(b.to_vec().reshape(d.shape), d)
+
+    def extend(self, seqs, counts=None):
+        self.pool.extend(seqs, counts=counts)
+        self.copy(self.want.extend(list(seqs), counts))
+
+    def fork(self, src, dst, keep=None):
+        self.pool.fork(src, dst, keep=keep)
+        self.want.fork(list(src), list(dst), keep)
+
+    def free(self, seqs):
+        self.pool.free(seqs)
+        self.want.free(list(seqs))
+
+    def compact(self):
+        self.pool.compact()
+        self.copy(self.want.compact()[0])
+
+
+def test_samples_of_one_prompt(dev):
+    b = Both(dev, 40, 16, 6, 8)
+    b.extend([0], [37])
+    b.check()
+    b.fork([0, 0, 0], [1, 2, 3])
+    b.check()
+    b.extend([1, 3, 2])                # three copies: the prompt keeps its own last page
+    b.check()
+    b.free([0])
+    b.fork([1], [0])
+    b.extend([1, 0])                   # the only two holders: the second keeps the page
+    b.check()
+    b.extend([0, 1, 2, 3], [0, 11, 16, 64])
+    b.check()
+    b.free([2])
+    b.compact()
+    b.check()
+    b.extend([4], [1])
+    b.fork([4, 1], [5, 2], keep=[0, 20])
+    b.check()
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("n_pages,P,n_seqs,ld,n_arrays,row", [(50, 16, 9, 12, 2, 8), (300, 32, 40, 20, 5, 24), (9000, 16, 70, 200, 1, 8), (33, 256, 5, 9, 2, 64)])
+def test_any_order_of_calls(dev, n_pages, P, n_seqs, ld, n_arrays, row, seed):
+    rng = np.random.default_rng(seed * 1000 + n_pages)
+    b = Both(dev, n_pages, P, n_seqs, ld, n_arrays, row)
+    for _ in range(25):
+        what = rng.choice(["extend", "extend", "extend", "fork", "free", "compact"])
+        seqs = rng.permutation(n_seqs)[:rng.integers(1, n_seqs + 1)].tolist()
+        if what == "extend":
+            counts = (rng.integers(0, 3, len(seqs)) * rng.integers(1, 2 * P, len(seqs))).tolist()
+            trial = Pool(n_pages, P, n_seqs, ld)
+            trial.refs, trial.tables, trial.lens = b.want.refs, b.want.tables, b.want.lens
+            try:
+                trial.extend(seqs, counts)
+            except Refused:
+                continue
+            b.extend(seqs, counts)
+        elif what == "fork":
+            empty, held = [s for s in seqs if not b.want.lens[s]], [s for s in range(n_seqs) if b.want.lens[s]]
+            if empty and held:
+                src = rng.choice(held, len(empty)).tolist()
+                b.fork(src, empty, None if rng.random() < 0.5 else rng.integers(0, P * 4, len(empty)).tolist())
+        elif what == "free":
+            b.free(seqs[:max(1, len(seqs) // 2)])
+        else:
+            b.compact()
+    b.check()
+
+
+def test_a_thousand_sequences(dev):
+    b = Both(dev, 5000, 16, 1024, 6, 1, 8)
+    every = np.random.default_rng(0).permutation(1024).tolist()
+    b.extend([3], [40])
+    b.fork([3] * 1023, [s for s in every if s != 3])
+    b.extend(every)
+    b.check()
+    b.extend(every, [(7 * s) % 33 for s in every])
+    b.free(every[:1000])
+    b.compact()
+    b.check()
+
+
+def test_large_rows_and_offsets_behind_32_bits(dev):
+    """Pages further than 2^32 bytes from the array's start."""
+    import tang_b200 as tb
+
+    n_pages, P, row = 3000, 64, 2048 * 8                     # 1 MiB a page in two arrays, 2 GiB behind page 2048
+    bufs = [dev.alloc(n_pages * P * row, tb.U8) for _ in range(2)]
+    for buf in bufs:
+        dev.memset(buf, 1)
+    refs = np.zeros(n_pages, np.int32)
+    tables = np.full((2, 4), -1, np.int32)
+    tables[0, :2], refs[[n_pages - 1, 5]] = [n_pages - 1, 5], 1
+    refs[:5] = refs[6:n_pages - 9] = 1                       # (only the last few are free)
+    state = [dev.upload(a, tb.I32) for a in (refs, tables, np.array([70, 0], np.int32))]
+    pool = tb.PagePool(dev, n_pages, P, 2, 4, bufs, *state)
+    pages = [tb.Buffer(dev, buf.ptr + (n_pages - 1) * P * row, P * row, tb.U8, owns=False) for buf in bufs]
+    for i, page in enumerate(pages):
+        dev.memset(page, 7 + i)
+    pool.fork([0], [1], keep=[33])                           # page n_pages - 1, partly filled
+    pool.extend([1])
+    dev.sync()
+    refs, tables, lens = pool.state()
+    to = n_pages - 9
+    assert tables[1].tolist() == [to, -1, -1, -1] and lens.tolist() == [70, 34] and refs[to] == 1 and refs[n_pages - 1] == 1
+    for i, buf in enumerate(bufs):
+        got = tb.Buffer(dev, buf.ptr + to * P * row, P * row, tb.U8, owns=False).to_vec().reshape(P, row)
+        assert (got[:33] == 7 + i).all() and (got[33:] == 1).all()
+    pool.destroy()
+
+
+def test_refused_calls_change_nothing(dev):
+    import tang_b200 as tb
+
+    b = Both(dev, 12, 16, 4, 6)
+    b.extend([0, 1], [40, 16])
+    b.fork([0], [2])
+    b.check()
+
+    def refused(call, status):
+        call()
+        with pytest.raises(tb.TangqError) as e:
+            dev.sync()
+        assert e.value.status == status
+        b.check()
+
+    bad, full = tb._lib.TQ_EINVAL, tb._lib.TQ_ENOMEM
+    refused(lambda: b.pool.extend([0, 4]), bad)
+    refused(lambda: b.pool.extend([-1]), bad)
+    refused(lambda: b.pool.extend([1, 0, 1]), bad)
+    refused(lambda: b.pool.extend([0], counts=[-1]), bad)
+    refused(lambda: b.pool.extend([1], counts=[81]), full)                   # the table has six entries
+    refused(lambda: b.pool.extend([1], counts=[2 ** 31 - 1]), full)
+    refused(lambda: b.pool.extend([3, 1, 0, 2], counts=[64, 48, 16, 16]), full)
+    refused(lambda: b.pool.fork([0], [1]), bad)                              # not empty
+    refused(lambda: b.pool.fork([0, 0], [3, 3]), bad)
+    refused(lambda: b.pool.fork([3], [3]), bad)
+    refused(lambda: b.pool.fork([0, 3], [3, 3]), bad)
+    refused(lambda: b.pool.fork([7], [3]), bad)
+    refused(lambda: b.pool.fork([0], [3], keep=[-5]), bad)
+    refused(lambda: b.pool.free([0, 0]), bad)
+    refused(lambda: b.pool.free([2, 9]), bad)
+    b.free([2])
+    b.extend([1], [1])
+    b.check()
+    for args in ((0, 16, 1, 1), (4, 24, 1, 1), (4, 8, 1, 1), (4, 2048, 1, 1), (4, 16, 0, 1), (4, 16, 1, 0)):
+        with pytest.raises(tb.TangqError):
+            tb.PagePool(dev, *args)
+    bare = tb.PagePool(dev, 4, 16, 2, 2)
+    for call in (lambda: bare.extend([0]), bare.compact, lambda: bare.set_arrays([]), lambda: bare.set_arrays([dev.alloc(4 * 16 * 4, tb.BF16)]),
+                 lambda: b.pool.free(list(range(1025)))):
+        with pytest.raises(tb.TangqError):
+            call()
+    bare.free([0, 1])
+    dev.sync()
+
+
+def test_calls_recorded_in_a_graph(dev):
+    """Forty tokens for three samples: one recorded step, replayed."""
+    import tang_b200 as tb
+
+    b = Both(dev, 40, 16, 4, 8)
+    b.extend([0], [21])
+    b.fork([0, 0], [1, 2])
+    seqs = dev.upload(np.array([2, 0, 1], np.int32), tb.I32)
+    b.pool.extend(seqs)
+    b.copy(b.want.extend([2, 0, 1]))
+    dev.sync()
+    dev.begin_capture()
+    b.pool.extend(seqs)
+    g = dev.end_capture()
+    for _ in range(40):
+        g.launch()
+        b.copy(b.want.extend([2, 0, 1]))
+    b.check()
+    g.free()
