@@ -35,8 +35,9 @@ def reference(x, tokens, top):
 
 def close(got, want, rest, V):
     """A log probability is (x - m) - log S: a rounding of each difference, and log S as exact as the sum of the other terms, in which a thread adds
-    at most V / 64 terms one after the other, each with four roundings of its own."""
-    tol = 4 * STEP * np.abs(want) + (V / 64 + 64) * STEP * rest[:, None] + 1e-38
+    at most V / 64 terms one after the other, each with four roundings of its own.  An exponential below 2^-126, the smallest normal f32, counts as zero:
+    V of them are less than V 2^-126."""
+    tol = 4 * STEP * np.abs(want) + (V / 64 + 64) * STEP * rest[:, None] + V * 2.0 ** -126
     fin = np.isfinite(want)
     assert np.array_equal(np.isneginf(got), np.isneginf(want))
     assert (np.abs(got - want)[fin] <= tol[fin]).all(), (np.abs(got - want)[fin] / tol[fin]).max()
@@ -70,8 +71,9 @@ def check(dev, x, tokens, top, **how):
     want_lp, want_h, want_ids, want_top, rest = reference(x64, tokens, top)
     close(lp, want_lp, rest, V)
     if h is not None:
-        # every term of the entropy is positive: its relative error is that of the sums
-        assert (np.abs(h - want_h) <= (V / 64 + 64) * STEP * want_h + 1e-38).all()
+        # every term of the entropy is positive: its relative error is that of the sums; and (m - x) exp(x - m) falls with m - x behind 1: the terms whose
+        # exponential is below 2^-126, m - x > 87, and so counts as zero are below 88 * 2^-126 each
+        assert (np.abs(h - want_h) <= (V / 64 + 64) * STEP * want_h + V * 88 * 2.0 ** -126).all()
     assert np.array_equal(ids, want_ids)
     close(top_lp, want_top, rest, V)
 
