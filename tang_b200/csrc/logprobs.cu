@@ -16,11 +16,11 @@ namespace tq {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256, kLpPerSm = 4;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 64;
 constexpr int kLpLoads = 4;            // 16-byte loads of a thread in flight, twice
-constexpr int kLpGroups = kLpThreads / 4;
+constexpr int kLpGroups = 128;         // of neighbouring threads; four warps sort their maxima
 constexpr int kLpList = 512;           // candidates that a CTA sorts
 constexpr int kLpMaxCluster = 8;
 constexpr float kLpLog2e = 1.4426950408889634f;
@@ -65,14 +65,24 @@ __device__ __forceinline__ void lp_unpack(const uint4& v, float (&x)[8], __nv_bf
     x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
   }
 }
+__device__ __forceinline__ void lp_set(uint32_t& w, float v) { w = __float_as_uint(v); }
+__device__ __forceinline__ void lp_set(uint32_t& w, __nv_bfloat16 v) { w = (w & 0xFFFF0000u) | __bfloat16_as_ushort(v); }
 __device__ __forceinline__ float lp_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-// (larger value, else lower index)
-__device__ __forceinline__ bool lp_before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+// Larger for a larger logit and, among equals (the zeros too), for a lower index; 0 is nobody's.
+__device__ __forceinline__ unsigned long long lp_key(float v, int i) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return (unsigned long long)(b >> 31 ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - (uint32_t)i);
+}
+__device__ __forceinline__ float lp_key_value(unsigned long long k) {
+  const uint32_t o = (uint32_t)(k >> 32);
+  return __uint_as_float(o >> 31 ? o & 0x7FFFFFFFu : ~o);
+}
+__device__ __forceinline__ int lp_key_index(unsigned long long k) { return (int)(0xFFFFFFFFu - (uint32_t)k); }
 
 // Part of a row: its largest logit m, how many equal it, the sum of exp(x - m) over the others, and sum (m - x) exp(x - m).
 struct LpState {
@@ -87,16 +97,105 @@ struct LpState {
       m = to;
     }
   }
-  template <bool ENT, int N>
-  __device__ __forceinline__ void add(const float (&x)[N]) {
-    const float base = m == -INFINITY ? 0.f : m;
+};
+
+// What a thread has read.  Exponents are fma(x, log2 e, -base), one instruction instead of the two of (x - b) log2 e, with base = b log2 e rounded and
+// b the largest logit of the warp's first batch: it only moves where a batch goes kLpSlack beyond it, so that the loop needs no maximum but the
+// thread's own.  What the rounding of base adds to every exponent alike, `off`, is taken out at the end (it would be too large from |b| = 2^20 on:
+// there, and before anything but -infinity was seen, the two instructions are used).
+// The 16 bytes with the thread's largest logit are held back: the row's largest must not be added before it is known (the sum of the others would be
+// lost against it where a model is sure).  Where another vector has the same one, that is among s, which is no loss there.
+constexpr float kLpSlack = 20.f;
+template <typename T, bool ENT>
+struct LpRunning {
+  static constexpr int N = 16 / (int)sizeof(T);
+  static constexpr uint32_t kNone = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;        // -infinity
+  float b = -INFINITY, base = 0.f, off = 0.f, s = 0.f, u = 0.f;        // u: sum of exponent * exponential
+  float mine = -INFINITY, second = -INFINITY;                      // the largest of `held` and of all other vectors
+  uint4 held = make_uint4(kNone, kNone, kNone, kNone);
+  int where = -1;                                       // the row's place of its first logit (-1: not 16 bytes of the row)
+
+  static __device__ __forceinline__ uint4 none() { return make_uint4(kNone, kNone, kNone, kNone); }
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    float x[N];
+    lp_unpack(v, x, T());
+    float mx = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
+    return mx;
+  }
+  __device__ __forceinline__ bool far() const { return !(fabsf(b) <= 1048576.f); }
+  __device__ __forceinline__ void take(float a) {
+    const float e = lp_ex2(a);
+    s += e;
+    if (ENT) u = fmaf(fmaxf(a, -1e4f), e, u);           // (e is 0 there, and -infinity times that is not)
+  }
+  // K vectors, the first of them at place `at` of the row and the others `step` apart (-1: nowhere)
+  template <int K>
+  __device__ __forceinline__ void add(uint4 (&v)[K], int at, int step) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float mx = largest(v[k]);
+      top = fmaxf(top, mx);
+      second = fmaxf(second, fminf(mx, mine));
+      if (mx > mine) {                                  // (selects, no branch)
+        const uint4 w = held;
+        held = v[k];
+        v[k] = w;
+        mine = mx;
+        where = at < 0 ? -1 : at + k * step;
+      }
+    }
+    if (__any_sync(0xffffffffu, top > b + kLpSlack)) {
+      const float was = b, off_was = off;
+      b = fmaxf(b, warp_max(top));
+      base = far() ? 0.f : b * kLpLog2e;
+      off = far() ? 0.f : fmaf(b, kLpLog2e, -base);
+      if (was != -INFINITY) {
+        const float by = fmaxf((was - b) * kLpLog2e - off_was + off, -1e4f), f = lp_ex2(by);
+        if (ENT) u = fmaf(by, s, u) * f;
+        s *= f;
+      }
+    }
+    if (!far()) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float x[N];
+        lp_unpack(v[k], x, T());
+#pragma unroll
+        for (int i = 0; i < N; ++i) take(fmaf(x[i], kLpLog2e, -base));
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float x[N];
+        lp_unpack(v[k], x, T());
+#pragma unroll
+        for (int i = 0; i < N; ++i) take(x[i] == -INFINITY ? -INFINITY : (x[i] - b) * kLpLog2e);
+      }
+    }
+  }
+  // All of it relative to m, the largest logit of the CTA.
+  __device__ __forceinline__ LpState state(float m) const {
+    LpState r;
+    r.m = m;
+    const float by = b == -INFINITY ? 0.f : fmaxf((b - m) * kLpLog2e - off, -1e4f), f = lp_ex2(by);
+    r.s = s * f;
+    if (ENT) r.u = -fmaf(by, s, u) * f * 0.693147180559945309f;
+    float x[N];
+    lp_unpack(held, x, T());
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float d = x[i] - base, e = lp_ex2(d * kLpLog2e);
-      if (x[i] == m) c += 1.f;
-      else s += e;
-      if (ENT) u = fmaf(fmaxf(d, -1e4f), -e, u);        // (e is 0 there, and -infinity times that is not)
+      const float d = x[i] - m, e = lp_ex2(d * kLpLog2e);
+      if (x[i] == m) {
+        r.c += 1.f;
+      } else if (x[i] != -INFINITY) {
+        r.s += e;
+        if (ENT) r.u = fmaf(fmaxf(d, -1e4f), -e, r.u);
+      }
     }
+    return r;
   }
 };
 
@@ -115,19 +214,19 @@ struct LpSegment {
 };
 
 template <typename T, bool ENT>
-__global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(const LogprobParams p) {
   constexpr int N = LpSegment<T>::N;
   __shared__ float red[4][kLpWarps];
   __shared__ float4 part;              // this CTA's state
   __shared__ __align__(16) float group_max[kLpGroups];
   __shared__ float thr_s;
   __shared__ int n_above, n_equal;
-  __shared__ float list_v[kLpList];    // above the threshold
-  __shared__ int list_i[kLpList], equal_i[kLpList];
-  __shared__ float top_v[kLpMaxTop];   // this CTA's largest, in order
-  __shared__ int top_i[kLpMaxTop];
-  __shared__ float all_v[kLpMaxCluster * kLpMaxTop];
-  __shared__ int all_i[kLpMaxCluster * kLpMaxTop];
+  __shared__ __align__(16) unsigned long long list[kLpList];           // above the threshold
+  __shared__ unsigned long long equal_list[kLpList];
+  __shared__ int scan[kLpThreads];     // threads that have any of them
+  __shared__ int n_scan;
+  __shared__ unsigned long long top_k[kLpMaxTop];                      // this CTA's largest, in order
+  __shared__ __align__(16) unsigned long long all_k[kLpMaxCluster * kLpMaxTop];
   pdl_wait();
   pdl_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
@@ -142,125 +241,145 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
   }
 
   // ---- one pass: maximum and sums of this thread's elements
-  LpState a;
+  LpRunning<T, ENT> sums;
   for (int at = lo; at < hi;) {
     const int sl = at / p.cols, in = at - sl * p.cols, n = min(hi - at, p.cols - in);
     const LpSegment<T> g(lp_slice<T>(p, row, sl) + in, n);
-    const uint4 none = sizeof(T) == 4 ? make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u) : make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
     uint4 v[kLpLoads];
     auto fetch = [&](int first) {
 #pragma unroll
       for (int k = 0; k < kLpLoads; ++k) {
         const int i = first + k * kLpThreads + t;
-        v[k] = i < g.vecs ? lp_load(g.base + g.head + i * N) : none;
+        v[k] = i < g.vecs ? lp_load(g.base + g.head + i * N) : sums.none();
       }
     };
     fetch(0);
-    if (t < g.head || g.tail0 + t < n) {               // (both at most 7 elements)
-      float x[2] = {-INFINITY, -INFINITY};
-      if (t < g.head) x[0] = lp_float(g.base[t]);
-      if (g.tail0 + t < n) x[1] = lp_float(g.base[g.tail0 + t]);
-      a.rise(fmaxf(a.m, fmaxf(x[0], x[1])));
-      a.template add<ENT>(x);
+    if (g.head > 0 || g.tail0 < n) {                   // (at most 7 elements each)
+      uint4 x[1] = {sums.none()};
+      if (t < g.head) lp_set(x[0].x, g.base[t]);
+      if (g.tail0 + t < n) lp_set(x[0].y, g.base[g.tail0 + t]);
+      sums.add(x, -1, 0);
     }
     for (int first = 0; first < g.vecs; first += kLpLoads * kLpThreads) {
       uint4 w[kLpLoads];
 #pragma unroll
       for (int k = 0; k < kLpLoads; ++k) w[k] = v[k];
       if (first + kLpLoads * kLpThreads < g.vecs) fetch(first + kLpLoads * kLpThreads);
-#pragma unroll
-      for (int k = 0; k < kLpLoads; ++k) {
-        float x[N];
-        lp_unpack(w[k], x, T());
-        float mx = x[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
-        a.rise(fmaxf(a.m, mx));
-        a.template add<ENT>(x);
-      }
+      sums.add(w, at + g.head + (first + t) * N, kLpThreads * N);
     }
     at += n;
   }
-  const float mine = a.m;
 
-  // ---- the CTA's state: lanes, then warps
-  auto meet_warp = [&](LpState& st) {
-    const float m = warp_max(st.m);
-    st.rise(m);
-    st.c = warp_sum(st.c);
-    st.s = warp_sum(st.s);
-    if (ENT) st.u = warp_sum(st.u);
-  };
-  meet_warp(a);
-  if (lane == 0) {
-    red[0][warp] = a.m;
-    red[1][warp] = a.c;
-    red[2][warp] = a.s;
-    red[3][warp] = a.u;
+  // ---- the CTA's state
+  const float mine = sums.mine;
+  {
+    const float m = warp_max(mine);
+    if (lane == 0) red[0][warp] = m;
   }
   if (top) {
-    const float g2 = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 1)), g4 = fmaxf(g2, __shfl_xor_sync(0xffffffffu, g2, 2));
-    if ((t & 3) == 0) group_max[t >> 2] = g4;
-    if (t == 0) n_above = n_equal = 0;
-    if (t < kLpMaxTop) top_i[t] = 0x7fffffff;
+    float g = mine;
+#pragma unroll
+    for (int o = 1; o < kLpThreads / kLpGroups; o *= 2) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (t % (kLpThreads / kLpGroups) == 0) group_max[t / (kLpThreads / kLpGroups)] = g;
+    if (t == 0) n_above = n_equal = n_scan = 0;
+    if (t < kLpMaxTop) top_k[t] = 0ull;
   }
   __syncthreads();
-  if (warp == 0) {
-    LpState b;
-    if (lane < kLpWarps) {
-      b.m = red[0][lane];
-      b.c = red[1][lane];
-      b.s = red[2][lane];
-      b.u = red[3][lane];
+  {
+    float m = red[0][0];
+#pragma unroll
+    for (int w = 1; w < kLpWarps; ++w) m = fmaxf(m, red[0][w]);
+    LpState a = sums.state(m);
+    a.c = warp_sum(a.c);
+    a.s = warp_sum(a.s);
+    if (ENT) a.u = warp_sum(a.u);
+    if (lane == 0) {
+      red[1][warp] = a.c;
+      red[2][warp] = a.s;
+      red[3][warp] = a.u;
     }
-    meet_warp(b);
-    if (lane == 0) part = make_float4(b.m, b.c, b.s, b.u);
   }
 
   // ---- the CTA's `top` largest.  The top-th largest of the 128 groups' maxima is a lower bound of the top-th largest element: few elements are above
   // it, and only the threads whose own maximum reaches it have any.
   if (top) {
     if (t >= kLpThreads - kLpGroups) {
-      const int me = t - (kLpThreads - kLpGroups);
-      const float v = group_max[me];
-      int before = 0;
-#pragma unroll 8
-      for (int j = 0; j < kLpGroups / 4; ++j) {
-        const float4 w = reinterpret_cast<const float4*>(group_max)[j];
-        before += lp_before(w.x, 4 * j, v, me) + lp_before(w.y, 4 * j + 1, v, me) + lp_before(w.z, 4 * j + 2, v, me) + lp_before(w.w, 4 * j + 3, v, me);
+      // every warp sorts 32 maxima, largest first; a maximum's rank is its place there and how many of the other three lists are before it
+      const int me = t - (kLpThreads - kLpGroups), w = me >> 5;
+      float v = group_max[me];
+#pragma unroll
+      for (int k = 2; k <= 32; k *= 2)
+#pragma unroll
+        for (int j = k / 2; j > 0; j /= 2) {
+          const float o = __shfl_xor_sync(0xffffffffu, v, j);
+          v = ((lane & k) == 0) == ((lane & j) == 0) ? fmaxf(v, o) : fminf(v, o);
+        }
+      group_max[me] = v;
+      asm volatile("bar.sync 1, %0;" ::"n"(kLpGroups) : "memory");
+      int before = lane;
+#pragma unroll
+      for (int q = 1; q < 4; ++q) {
+        const int other = (w + q) & 3;
+        const bool first = other < w;                  // (among equals, the lower list's)
+        int n = 0;
+#pragma unroll
+        for (int half = 16; half > 0; half /= 2) {
+          const float o = group_max[32 * other + n + half - 1];
+          if (first ? o >= v : o > v) n += half;
+        }
+        if (n == 31 && (first ? group_max[32 * other + 31] >= v : group_max[32 * other + 31] > v)) n = 32;
+        before += n;
       }
       if (before == top - 1) thr_s = v;
     }
     __syncthreads();
     const float thr = thr_s;
-    if (mine >= thr) {
-      auto offer = [&](float x, int i) {
-        if (x > thr) {
-          const int k = atomicAdd(&n_above, 1);
-          if (k < kLpList) {
-            list_v[k] = x;
-            list_i[k] = i;
-          }
-        } else if (x == thr) {
-          const int k = atomicAdd(&n_equal, 1);
-          if (k < kLpList) equal_i[k] = i;
-        }
-      };
+    auto offer = [&](float x, int i) {
+      if (x > thr) {
+        const int k = atomicAdd(&n_above, 1);
+        if (k < kLpList) list[k] = lp_key(x, i);
+      } else if (x == thr) {
+        const int k = thr == -INFINITY ? kLpList : atomicAdd(&n_equal, 1);
+        if (k < kLpList) equal_list[k] = lp_key(x, i);
+      }
+    };
+    if (t == 0 && thr == -INFINITY) n_equal = kLpList + 1;            // (any number of them: see below)
+    if (mine == -INFINITY) {
+    } else if (sums.second >= thr || (mine >= thr && sums.where < 0)) {
+      scan[atomicAdd(&n_scan, 1)] = t;
+    } else if (mine >= thr) {
+      float x[N];
+      lp_unpack(sums.held, x, T());
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (x[j] >= thr) offer(x[j], sums.where + j);
+    }
+    __syncthreads();
+    // (few) threads with more than one such vector: eight lanes read all of one's again, eight 16-byte loads each at a time
+    for (int q = t >> 3; q < n_scan; q += kLpThreads / 8) {
+      const int owner = scan[q], o8 = t & 7;
       for (int at = lo; at < hi;) {
         const int sl = at / p.cols, in = at - sl * p.cols, n = min(hi - at, p.cols - in);
         const LpSegment<T> g(lp_slice<T>(p, row, sl) + in, n);
-        if (t < g.head) offer(lp_float(g.base[t]), at + t);
-        if (g.tail0 + t < n) offer(lp_float(g.base[g.tail0 + t]), at + g.tail0 + t);
-#pragma unroll 4
-        for (int i = t; i < g.vecs; i += kLpThreads) {
-          float x[N];
-          lp_unpack(lp_load(g.base + g.head + i * N), x, T());
-          float mx = x[0];
+        if (o8 == 0 && owner < g.head) offer(lp_float(g.base[owner]), at + owner);
+        if (o8 == 0 && g.tail0 + owner < n) offer(lp_float(g.base[g.tail0 + owner]), at + g.tail0 + owner);
+        for (int first = owner + o8 * kLpThreads; first < g.vecs; first += 64 * kLpThreads) {
+          uint4 v[8];
 #pragma unroll
-          for (int j = 1; j < N; ++j) mx = fmaxf(mx, x[j]);
-          if (mx >= thr)
+          for (int k = 0; k < 8; ++k)
+            if (first + 8 * k * kLpThreads < g.vecs) v[k] = lp_load(g.base + g.head + (first + 8 * k * kLpThreads) * N);
 #pragma unroll
-            for (int j = 0; j < N; ++j) offer(x[j], at + g.head + i * N + j);
+          for (int k = 0; k < 8; ++k) {
+            if (first + 8 * k * kLpThreads >= g.vecs) break;
+            float x[N];
+            lp_unpack(v[k], x, T());
+            float mx = x[0];
+#pragma unroll
+            for (int j = 1; j < N; ++j) mx = fmaxf(mx, x[j]);
+            if (mx >= thr)
+#pragma unroll
+              for (int j = 0; j < N; ++j) offer(x[j], at + g.head + (first + 8 * k * kLpThreads) * N + j);
+          }
         }
         at += n;
       }
@@ -269,25 +388,20 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
     const int above = n_above, equal = n_equal;
     if (above <= kLpList) {
       for (int i = t; i < above; i += kLpThreads) {
-        const float v = list_v[i];
-        const int id = list_i[i];
+        const unsigned long long me = list[i];
         int before = 0;
-        for (int j = 0; j < above; ++j) before += lp_before(list_v[j], list_i[j], v, id);
-        if (before < top) {
-          top_v[before] = v;
-          top_i[before] = id;
-        }
+#pragma unroll 4
+        for (int j = 0; j < above; ++j) before += list[j] > me;
+        if (before < top) top_k[before] = me;
       }
       const int want = top - above;
       if (want > 0 && equal <= kLpList) {
         for (int i = t; i < equal; i += kLpThreads) {
-          const int id = equal_i[i];
+          const unsigned long long me = equal_list[i];
           int before = 0;
-          for (int j = 0; j < equal; ++j) before += equal_i[j] < id;
-          if (before < want) {
-            top_v[above + before] = thr;
-            top_i[above + before] = id;
-          }
+#pragma unroll 4
+          for (int j = 0; j < equal; ++j) before += equal_list[j] > me;
+          if (before < want) top_k[above + before] = me;
         }
       } else if (want > 0) {
         // many equal ones: the first of them in the order of the row
@@ -296,59 +410,53 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
           const bool hit = base + t < hi && lp_at<T>(p, row, base + t) == thr;
           const unsigned ballot = __ballot_sync(0xffffffffu, hit);
           __syncthreads();
-          if (lane == 0) list_i[warp] = __popc(ballot);
+          if (lane == 0) scan[warp] = __popc(ballot);
           __syncthreads();
           int at = found + __popc(ballot & ((1u << lane) - 1u));
           for (int w = 0; w < kLpWarps; ++w) {
-            at += w < warp ? list_i[w] : 0;
-            found += list_i[w];
+            at += w < warp ? scan[w] : 0;
+            found += scan[w];
           }
-          if (hit && at < want) {
-            top_v[above + at] = thr;
-            top_i[above + at] = base + t;
-          }
+          if (hit && at < want) top_k[above + at] = lp_key(thr, base + t);
         }
       }
     } else {
       // more above the bound than the list holds (they sit in few threads' elements): the next in order, one after the other
-      float last_v = INFINITY;
-      int last_i = -1;
+      unsigned long long last = ~0ull;
       for (int k = 0; k < top; ++k) {
-        float bv = -INFINITY;
-        int bi = 0x7fffffff;
-        auto meet = [&](float v, int i) {
-          if (i != 0x7fffffff && (bi == 0x7fffffff || lp_before(v, i, bv, bi))) {
-            bv = v;
-            bi = i;
-          }
-        };
+        unsigned long long best = 0ull;
         for (int i = lo + t; i < hi; i += kLpThreads) {
           const float v = lp_at<T>(p, row, i);
-          if (v == v && lp_before(last_v, last_i, v, i)) meet(v, i);
+          const unsigned long long key = lp_key(v, i);
+          if (v == v && key < last && key > best) best = key;
         }
         for (int o = 16; o > 0; o >>= 1) {
-          const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-          const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-          meet(ov, oi);
+          const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
+          best = other > best ? other : best;
         }
         __syncthreads();
-        if (lane == 0) {
-          list_v[warp] = bv;
-          list_i[warp] = bi;
-        }
+        if (lane == 0) list[warp] = best;
         __syncthreads();
-        for (int w = 0; w < kLpWarps; ++w) meet(list_v[w], list_i[w]);
-        if (t == 0) {
-          top_v[k] = bv;
-          top_i[k] = bi;
-        }
-        last_v = bv;
-        last_i = bi;
+        for (int w = 0; w < kLpWarps; ++w) best = list[w] > best ? list[w] : best;
+        if (t == 0) top_k[k] = best;
+        last = best;
       }
     }
   }
 
   // ---- the row: the first CTA of the cluster reads the others' states and lists
+  __syncthreads();
+  if (t == 0) {
+    LpState r;
+#pragma unroll
+    for (int w = 0; w < kLpWarps; ++w) {
+      r.m = fmaxf(r.m, red[0][w]);
+      r.c += red[1][w];
+      r.s += red[2][w];
+      if (ENT) r.u += red[3][w];
+    }
+    part = make_float4(r.m, r.c, r.s, r.u);
+  }
   if (C > 1) cluster.sync();
   else __syncthreads();
   if (rank == 0) {
@@ -387,41 +495,27 @@ __global__ void __launch_bounds__(kLpThreads, 2) token_logprobs_kernel(const Log
       p.logprob[(size_t)row * p.n_tokens + j] = tok < 0 ? 0.f : tok >= V ? NAN : logprob(lp_at<T>(p, row, tok));
     }
     if (top) {
+      // place k of the row, a key or nobody's
+      auto put = [&](int k, unsigned long long key) {
+        p.top_ids[(size_t)row * top + k] = key ? lp_key_index(key) : -1;
+        p.top_logprob[(size_t)row * top + k] = key ? logprob(lp_key_value(key)) : NAN;
+      };
       if (C == 1) {
-        if (t < top) {
-          const int id = top_i[t];
-          p.top_ids[(size_t)row * top + t] = id == 0x7fffffff ? -1 : id;
-          p.top_logprob[(size_t)row * top + t] = id == 0x7fffffff ? NAN : logprob(top_v[t]);
-        }
+        if (t < top) put(t, top_k[t]);
       } else {
         const int all = C * top;
-        for (int i = t; i < all; i += kLpThreads) {
-          const int k = i / top, j = i - k * top;
-          all_i[i] = *cluster.map_shared_rank(&top_i[j], k);
-          all_v[i] = *cluster.map_shared_rank(&top_v[j], k);
-        }
-        __syncthreads();
+        for (int i = t; i < all; i += kLpThreads) all_k[i] = *cluster.map_shared_rank(&top_k[i % top], i / top);
         int have = 0;
+        for (int i = t; i - t < all; i += kLpThreads) have += __syncthreads_count(i < all && all_k[i] != 0ull);   // (a thread counts the keys that it wrote)
         for (int i = t; i < all; i += kLpThreads) {
-          const int id = all_i[i];
-          if (id == 0x7fffffff) continue;
-          const float v = all_v[i];
+          const unsigned long long me = all_k[i];
+          if (!me) continue;
           int before = 0;
-          for (int j = 0; j < all; ++j) before += all_i[j] != 0x7fffffff && lp_before(all_v[j], all_i[j], v, id);
-          if (before < top) {
-            p.top_ids[(size_t)row * top + before] = id;
-            p.top_logprob[(size_t)row * top + before] = logprob(v);
-          }
-          ++have;
+#pragma unroll 8
+          for (int j = 0; j < all; ++j) before += all_k[j] > me;
+          if (before < top) put(before, me);
         }
-        if (t < top) {                                 // (fewer numbers than places)
-          have = 0;
-          for (int j = 0; j < all; ++j) have += all_i[j] != 0x7fffffff;
-          if (t >= have) {
-            p.top_ids[(size_t)row * top + t] = -1;
-            p.top_logprob[(size_t)row * top + t] = NAN;
-          }
-        }
+        if (t >= have && t < top) put(t, 0ull);        // (fewer numbers than places)
       }
     }
   }
@@ -459,10 +553,12 @@ extern "C" int tq_token_logprobs(tq_ctx* ctx, const void* logits_dev, int dtype,
   p.entropy = entropy_out_dev;
   p.top_ids = top_ids_out_dev;
   p.top_logprob = top_logprob_out_dev;
-  // CTAs of a row (a cluster): as many as keep the GPU's CTA slots (two an SM) filled, none with less than 2048 logits.
-  const size_t V = slices * cols;
-  int C = 1;
-  while (C < kLpMaxCluster && rows * C < 4 * (size_t)ctx->sm_count && V / (2 * C) >= 2048) C *= 2;
+  // CTAs of a row (a cluster): as many as fit the GPU at once (four an SM), none with less than 2048 logits.  More, smaller ones cost more than they
+  // balance, fewer leave SMs idle; us for one, two, four, eight: 64 rows of 128256 f32 23.7, 14.8, 10.6, 10.2, 256 rows 28.0, 23.7, 27.5, 33.9,
+  // one row of 32000 6.7, 5.5, 4.6, 4.4.
+  const size_t V = slices * cols, slots = (size_t)ctx->sm_count * kLpPerSm;
+  size_t C = slots / rows < V / 2048 ? slots / rows : V / 2048;
+  C = C < 1 ? 1 : C > (size_t)kLpMaxCluster ? (size_t)kLpMaxCluster : C;
   const bool ent = entropy_out_dev != nullptr;
   auto kern = dtype == TQ_BF16 ? (ent ? token_logprobs_kernel<__nv_bfloat16, true> : token_logprobs_kernel<__nv_bfloat16, false>)
                                : (ent ? token_logprobs_kernel<float, true> : token_logprobs_kernel<float, false>);

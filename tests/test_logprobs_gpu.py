@@ -29,6 +29,8 @@ def reference(x, tokens, top):
     with np.errstate(invalid="ignore"):
         h = log_s - np.where(e > 0, d * e, 0).sum(1) / (lead + rest)
     lp = d - log_s[:, None]
+    with np.errstate(over="ignore"):
+        lp[np.isneginf(lp.astype(np.float32))] = -np.inf      # (too far from zero for an f32)
     ids = np.argsort(-x, axis=1, kind="stable")[:, :top]
     return np.take_along_axis(lp, tokens, 1), h, ids, np.take_along_axis(lp, ids, 1), rest / (lead + rest)
 
@@ -90,7 +92,7 @@ def test_against_64_bits(dev, rows, V, slices, pad, top, n_tokens, bf16):
     check(dev, x, rng.integers(0, V, (rows, n_tokens)), top, slices=slices, bf16=bf16, pad=pad)
 
 
-@pytest.mark.parametrize("kind", ["equal", "two values", "ascending", "descending", "one finite", "few finite", "far apart", "large", "signed zeros", "sure", "blocks"])
+@pytest.mark.parametrize("kind", ["equal", "two values", "ascending", "descending", "one finite", "few finite", "far apart", "large", "signed zeros", "sure", "blocks", "lowest", "mostly lowest", "millions", "huge"])
 @pytest.mark.parametrize("V,slices", [(90, 1), (5000, 1), (4 * 5003, 4), (128256, 1)])
 def test_rows_that_are_hard_to_order_or_to_add(dev, kind, V, slices):
     rng = np.random.default_rng(V)
@@ -118,6 +120,18 @@ def test_rows_that_are_hard_to_order_or_to_add(dev, kind, V, slices):
         x[:] = np.where(rng.random((rows, V)) < 0.5, 0.0, -0.0)
     elif kind == "sure":
         x[np.arange(rows), rng.integers(0, V, rows)] = 40
+    elif kind == "lowest":             # what masks are made of
+        x[:] = np.finfo(np.float32).min
+        x[1, :V // 2] = -np.inf
+        x[2, 1::2] = 2e30
+    elif kind == "mostly lowest":
+        x[rng.random((rows, V)) < 1 - 12 / V] = np.finfo(np.float32).min
+        x[0, V // 2] = np.finfo(np.float32).max
+        x[3, V // 3:] = -np.inf
+    elif kind == "millions":           # steps of 1/8 between neighbours
+        x += np.array([2 ** 20 - 2, 2 ** 20 + 5, -2 ** 20, -2 ** 20 - 3, 2 ** 23])[:, None]
+    elif kind == "huge":
+        x *= 1e37
     elif kind == "blocks":             # the largest ones side by side, over and over the same
         x[:, V // 3:V // 3 + min(3000, V // 3)] = 7.5
         x[:, V - 2] = 7.5
