@@ -299,7 +299,8 @@ TQ_API int tq_pages_compact(tq_pages* pages, int* used_out_dev_or_null);
  * them: what lies behind it is not attended.
  * Groups (NULL: none): group g is sequences group_starts[g] .. group_starts[g+1]-1 of the batch (the last group's end is the batch's; starts
  * ascend from 0) and shares its first shared[g] positions (at most max_shared), which are read from its first sequence's pages, once for all.
- * out [batch, n_heads*128] bf16 or f32; all four 16-byte aligned.  A page that does not exist is skipped and reported by tq_sync. */
+ * out [batch, n_heads*128] bf16 or f32; all four 16-byte aligned.  A page or sequence that does not exist is reported by tq_sync, and the results
+ * of the sequences (and the group) that hold it are not defined.  At most 1024 sequences; max_len at most 2^30. */
 TQ_API int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k_pages_dev, const void* v_pages_dev, const tq_pages* pages,
                                const int* seqs_dev_or_null, size_t batch, const int* group_starts_dev_or_null, const int* shared_dev_or_null,
                                size_t n_groups, size_t max_shared, size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t max_len,
