@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 
 #include <cfloat>
+#include <type_traits>
 
 #include "attn_mma.cuh"
 #include "attn_umma.cuh"
@@ -32,29 +33,32 @@ __device__ __forceinline__ int paged_row_of(const PagedParams& p, int b) {
 }
 // ---------------------------------------------------------------------------------------------
 // Units, tiles, pieces.  A unit is what meets the same keys: the rows (member, query head of one KV head) of up to 128 / group members of a group over
-// the group's shared positions, in whole tiles of 128, or one sequence's query heads over the rest.  All tiles of all units stand in one list, shared ones
-// first, and CTA c of N takes tiles T c / N .. T (c + 1) / N - 1: the same number each, whatever the lengths.  Odd and even tiles of the list belong
-// to different softmax groups, which keep maximum, sum and products of their own: a piece (unit, CTA, parity) leaves one partial result.
+// the group's shared positions, in whole tiles of 128, or one sequence's query heads over the rest.  The tiles of all units of a KV head stand in one list,
+// shared ones first, and CTA j of the J that a KV head has takes tiles T j / J .. T (j + 1) / J - 1: the same number each, whatever the lengths.
+// (CTAs of all KV heads walk their lists at the same pace: a cache row holds all of them, and its 256 bytes a head are fetched at the same time.)  Odd and
+// even tiles of the list belong to different softmax groups, which keep maximum, sum and products of their own: a piece (unit, CTA, parity) leaves
+// one partial result.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPuThreads = 384;
 constexpr int kPuTile = 4 * kPfBox / 2;               // bytes of 128 rows of keys or values
 constexpr int kPuRing = 5;
-constexpr int kPuStageLd = 17;                        // words between rows of a group's staging
-constexpr int kPuStage = 128 * kPuStageLd * 4;
-constexpr int kPuHeader = 512;
+constexpr int kPuWeights = 2 * 32 * 128;              // a parity's weights where keys are the lanes: 32 rows of 128 keys, in two halves
+constexpr int kPuMeet = 2 * 2 * 4 * 32 * 4;           // [parity][maxima, sums][warp][row]
+constexpr float kPuLargest = 7.9228162514264338e28f;  // 2^96: a weight above it is too far from its reference
+constexpr int kPuHeader = 256;                        // barriers
 constexpr int kPuBatch = 1024;                        // sequences of a call
-constexpr size_t kPuFixed = kPuHeader + 1024 + 2 * (size_t)kPfBox + kPuRing * (size_t)kPuTile + 2 * (size_t)kPuStage;
+constexpr size_t kPuFixed = 2 * (size_t)kPfBox + kPuRing * (size_t)kPuTile + 2 * (size_t)kPuWeights + kPuMeet + kPuHeader;
 
 // In shared memory, behind the buffers.
 struct PuPlan {
   int *own, *last, *pre, *eff;                        // [batch + 1] own tiles of the sequences before; [batch] shared tiles << 8 | keys of the last tile - 1;
-                                                      // [groups + 1] shared tiles of the groups before; [groups] tiles that a group shares
-  int batch, groups, n_kv, group, per_tile, pre_tiles, total;
+                                                      // [groups + 1] units' shared tiles of the groups before; [groups] tiles that a group shares
+  int batch, groups, group, per_tile, pre_tiles, total;
 };
 struct PuUnit {
   bool pre;
-  int b0, kv, rows, tiles, tile, shared_tiles, last;  // b0: (first) sequence of the batch; tile: the asked one; last: keys of the last tile
-  int slot;                                           // first row of its partial results at CTA 0
+  int b0, rows, tiles, tile, shared_tiles, last;      // b0: (first) sequence of the batch; tile: the asked one; last: keys of the last tile
+  int slot;                                           // first row of its partial results, without what the KV head and the CTA add
   int q_slot;
 };
 
@@ -74,44 +78,60 @@ __device__ __forceinline__ PuUnit pu_locate(const PagedParams& p, const PuPlan& 
   u.pre = f < l.pre_tiles;
   if (u.pre) {
     const int g = pu_last_not_above(l.pre, l.groups, f), start = pu_group_start(p, g), members = pu_group_end(p, g, start) - start;
-    const int row_tiles = (members + l.per_tile - 1) / l.per_tile;
     u.tiles = l.eff[g];
-    const int rest = f - l.pre[g], unit = rest / u.tiles, rt = unit % row_tiles;
-    u.tile = rest - unit * u.tiles;
-    u.kv = unit / row_tiles;
+    const int rest = f - l.pre[g], rt = rest / u.tiles;
+    u.tile = rest - rt * u.tiles;
     u.b0 = start + rt * l.per_tile;
     u.rows = min(l.per_tile, members - rt * l.per_tile) * l.group;
     u.shared_tiles = 0;
     u.last = kPfTile;
-    u.slot = (start * l.n_kv + u.kv * members + rt * l.per_tile) * l.group;
+    u.slot = u.b0 * l.group;
     u.q_slot = 0;
   } else {
-    const int h = f - l.pre_tiles, b = pu_last_not_above(l.own, l.batch, h / l.n_kv);
+    const int h = f - l.pre_tiles, b = pu_last_not_above(l.own, l.batch, h);
     u.tiles = l.own[b + 1] - l.own[b];
-    const int rest = h - l.own[b] * l.n_kv;
-    u.kv = rest / u.tiles;
-    u.tile = rest - u.kv * u.tiles;
+    u.tile = h - l.own[b];
     u.b0 = b;
     u.rows = l.group;
     u.shared_tiles = l.last[b] >> 8;
     u.last = (l.last[b] & 255) + 1;
-    u.slot = (b * l.n_kv + u.kv) * l.group;
-    u.q_slot = (b * l.n_kv + u.kv) & 3;
+    u.slot = b * l.group;
+    u.q_slot = b & 3;
   }
   return u;
 }
 
-// What the kernel that joins the pieces has to know of a sequence, and the total behind them all.
+// From a tile of the list to the next one, f, which exists.
+__device__ __forceinline__ void pu_step(const PagedParams& p, const PuPlan& l, PuUnit& u, int f) {
+  if (++u.tile < u.tiles) return;
+  if (u.pre) {
+    u = pu_locate(p, l, f);
+    return;
+  }
+  int b = u.b0 + 1;
+  while (l.own[b + 1] == l.own[b]) ++b;
+  u.tiles = l.own[b + 1] - l.own[b];
+  u.tile = 0;
+  u.b0 = b;
+  u.shared_tiles = l.last[b] >> 8;
+  u.last = (l.last[b] & 255) + 1;
+  u.slot = b * l.group;
+  u.q_slot = b & 3;
+}
+// Rows that are laid out for a unit whose keys are the tensor memory's lanes (0: its rows are), each as two terms but for the 32 of bf16 results.
+template <int TERMS>
+__device__ __forceinline__ int pu_wide(const PuUnit& u) { return u.rows <= 8 ? 8 : u.rows <= 16 ? 16 : u.rows <= 32 && TERMS == 1 ? 32 : 0; }
+__device__ __forceinline__ int pu_keys(const PuUnit& u) { return u.tile == u.tiles - 1 ? u.last : kPfTile; }
+
+// What the kernel that joins the pieces has to know of a sequence: where its tiles stand in a KV head's list.
 struct PuSeqPlan {
-  int own_f, own_tiles;                               // first tile of (sequence, KV head 0) in the list, tiles per KV head
-  int pre_f, pre_kv, pre_tiles;                       // first tile of its row tile's unit for KV head 0, tiles between KV heads, tiles of the unit
-  int pre_row, pre_row_kv;                            // its first row among the partial results, rows between KV heads
-  int pad;
+  int own_f, own_tiles, pre_f, pre_tiles;
 };
 
 struct PuParams {
   PagedParams a;
   int per_tile, per_quarter;                          // members of a row tile; of a row tile that fits 32 rows
+  int per_head;                                       // CTAs of a KV head
   float *own_o, *own_ml, *pre_o, *pre_ml;             // partial results: [row][parity][128], [row][parity][2]
   PuSeqPlan* plan;
   int* plan_total;
@@ -133,13 +153,26 @@ __device__ __forceinline__ void pu_scan(int* a, int n, int lane) {      // a[0 .
   if (lane == 0) a[n] = sum;
 }
 
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 template <int TERMS>
 __global__ void __launch_bounds__(kPuThreads, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_constant__ CUtensorMap q_quarter, const __grid_constant__ CUtensorMap q_whole,
                     const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PuParams pp) {
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];   // (the swizzled buffers come first)
   const PagedParams& p = pp.a;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem_raw);            // [4]
+  uint8_t *q_s = smem_raw, *kv_s = q_s + 2 * kPfBox;
+  uint8_t* w_s = kv_s + kPuRing * kPuTile;            // [parity]
+  float* meet_s = reinterpret_cast<float*>(w_s + 2 * kPuWeights);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(meet_s + kPuMeet / 4);  // [4]
   uint64_t* q_empty = q_full + 4;                     // [4]
   uint64_t* kv_full = q_empty + 4;                    // [ring]
   uint64_t* kv_empty = kv_full + kPuRing;
@@ -149,17 +182,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   uint64_t* o_done = p_full + 2;
   uint64_t* o_free = o_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 2);
-  uint8_t* q_s = smem_raw + kPuHeader + ((1024 - ((smem_u32(smem_raw) + kPuHeader) & 1023)) & 1023);
-  uint8_t* kv_s = q_s + 2 * kPfBox;
-  float* stage_s = reinterpret_cast<float*>(kv_s + kPuRing * kPuTile);
   PuPlan l;
-  l.own = reinterpret_cast<int*>(stage_s) + 2 * kPuStage / 4;
+  l.own = reinterpret_cast<int*>(q_full) + kPuHeader / 4;
   l.last = l.own + p.batch + 1;
   l.pre = l.last + p.batch;
   l.eff = l.pre + p.n_groups + 1;
   l.batch = p.batch;
   l.groups = p.n_groups;
-  l.n_kv = p.n_kv;
   l.group = p.group;
   l.per_tile = pp.per_tile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -184,7 +213,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     }
   } else if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
-  } else if (warp == 2 && lane == 0) {
+  } else if (warp == 3 && lane == 0) {
     prefetch_map(&q_own);
     prefetch_map(&k_map);
     prefetch_map(&v_map);
@@ -193,6 +222,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   pdl_wait();
   pdl_launch_dependents();
   auto give_up = [&](int code) { atomicCAS(p.err, 0, code); };
+  if (threadIdx.x == 0 && (smem_u32(smem_raw) & 1023)) give_up(DERR_TMEM);
 
   // ---- the plan: every CTA makes it for itself
   for (int b = threadIdx.x; b < p.batch; b += kPuThreads) {
@@ -212,7 +242,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     for (int b = start + lane; b < end; b += 32) l.last[b] = tiles << 8;
     if (lane == 0) {
       l.eff[g] = tiles;
-      l.pre[g] = tiles * ((end - start + pp.per_tile - 1) / pp.per_tile) * p.n_kv;
+      l.pre[g] = tiles * ((end - start + pp.per_tile - 1) / pp.per_tile);
     }
   }
   __syncthreads();
@@ -228,98 +258,86 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   l.pre_tiles = l.pre[p.n_groups];
-  l.total = l.pre_tiles + l.own[p.batch] * p.n_kv;
-  const int f0 = (int)((long long)l.total * blockIdx.x / gridDim.x), f1 = (int)((long long)l.total * (blockIdx.x + 1) / gridDim.x), n = f1 - f0;
+  l.total = l.pre_tiles + l.own[p.batch];
+  const int kvh = (int)(blockIdx.x % p.n_kv), part = (int)(blockIdx.x / p.n_kv);
+  const int f0 = (int)((long long)l.total * part / pp.per_head), f1 = (int)((long long)l.total * (part + 1) / pp.per_head), n = f1 - f0;
   if (blockIdx.x == 0) {               // for the kernel that joins the pieces
     for (int b = threadIdx.x; b < p.batch; b += kPuThreads) {
-      PuSeqPlan q;
-      q.own_tiles = l.own[b + 1] - l.own[b];
-      q.own_f = l.pre_tiles + l.own[b] * p.n_kv;
-      q.pre_tiles = l.last[b] >> 8;
-      q.pre_f = q.pre_kv = q.pre_row = q.pre_row_kv = q.pad = 0;
-      pp.plan[b] = q;
-    }
-    __syncthreads();
-    for (int g = warp; g < p.n_groups; g += kPuThreads / 32) {
-      const int start = pu_group_start(p, g), end = pu_group_end(p, g, start), members = end - start, row_tiles = (members + pp.per_tile - 1) / pp.per_tile;
-      for (int b = start + lane; b < end; b += 32) {
-        const int rt = (b - start) / pp.per_tile;
-        PuSeqPlan* q = &pp.plan[b];
-        q->pre_f = l.pre[g] + rt * l.eff[g];
-        q->pre_kv = row_tiles * l.eff[g];
-        q->pre_row = (start * p.n_kv + b - start) * p.group;
-        q->pre_row_kv = members * p.group;
+      int pre_f = 0;
+      const int shared = l.last[b] >> 8;
+      if (shared) {
+        int lo = 0, hi = p.n_groups;   // the group with b: the last that starts there or before
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (pu_group_start(p, mid) <= b) lo = mid;
+          else hi = mid;
+        }
+        pre_f = l.pre[lo] + (b - pu_group_start(p, lo)) / pp.per_tile * l.eff[lo];
       }
+      pp.plan[b] = PuSeqPlan{l.pre_tiles + l.own[b], l.own[b + 1] - l.own[b], pre_f, shared};
     }
     if (threadIdx.x == 0) *pp.plan_total = l.total;
   }
 
-  if (warp == 0) {
-    // ---- copies: queries of every unit, keys and values of every tile; a lane per box
+  if (warp == 0 || warp == 2) {
+    // ---- copies: the keys of every tile (warp 0); the queries of every unit and the values of every tile (warp 2).  A lane per box: a page's rows, half
+    // their columns.  The page of the next tile is asked for before the wait of this one.
+    const bool values = warp == 2;
+    const int box_rows = min(1 << p.page_shift, kPfTile), boxes = kPfTile / box_rows, j = lane >> 1, c = lane & 1;
     uint32_t q_used = 0;               // phases of the query slots
-    PuUnit u;
-    int page_next = 0;
-    const int* table = p.tables;
-    const int box_rows = min(1 << p.page_shift, kPfTile), boxes = kPfTile / box_rows;
     bool ok = true;
-    // the page of box `lane / 2` of a tile (the boxes' halves are the lanes' parity)
-    auto page_of = [&](const PuUnit& w, const int* t, int tile, int keys) {
-      const int j = lane >> 1, at = tile * kPfTile + j * box_rows;
-      if (j >= boxes || j * box_rows >= keys) return -1;
-      int page = t[at >> p.page_shift];
-      if (page < 0 || page >= p.n_pages) {
+    const int* table = nullptr;
+    auto table_of = [&](const PuUnit& w, int f) {
+      const int s = paged_row_of(p, w.pre ? pu_group_start(p, pu_last_not_above(l.pre, l.groups, f)) : w.b0);
+      return p.tables + (size_t)max(s, 0) * p.table_ld;
+    };
+    auto page_of = [&](const PuUnit& w) {
+      return j < boxes && j * box_rows < pu_keys(w) ? table[((w.shared_tiles + w.tile) * kPfTile + j * box_rows) >> p.page_shift] : 0;
+    };
+    PuUnit u, next;
+    int page = 0, page_next = 0;
+    if (n > 0) {
+      next = pu_locate(p, l, f0);
+      table = table_of(next, f0);
+      page_next = page_of(next);
+    }
+    for (int i = 0; i < n && ok; ++i) {
+      const bool fresh = i == 0 || u.tile == u.tiles - 1;
+      u = next;
+      page = page_next;
+      if (i + 1 < n) {
+        pu_step(p, l, next, f0 + i + 1);
+        if (next.tile == 0) table = table_of(next, f0 + i + 1);
+        page_next = page_of(next);
+      }
+      if (values && fresh) {
+        const int slot = u.q_slot;
+        for (int k = 0; k < 4; ++k)
+          if (ok && (u.pre || k == slot)) {
+            ok = mbar_wait_spin(&q_empty[k], ((q_used >> k) & 1u) ^ 1u);
+            q_used ^= 1u << k;
+          }
+        if (!ok) break;
+        const bool whole = pu_wide<TERMS>(u) == 0;
+        const uint32_t rows = (uint32_t)((whole ? pp.per_tile : u.pre ? pp.per_quarter : 1) * p.group);
+        if (lane == 0) mbar_arrive_expect_tx(&q_full[slot], 2u * rows * 128u);
+        __syncwarp();
+        if (lane < 2) tma_load_3d(q_s + c * kPfBox + 16 * slot * 128, whole ? &q_whole : u.pre ? &q_quarter : &q_own, 64 * c, kvh * p.group, u.b0, &q_full[slot]);
+        __syncwarp();
+      }
+      const int keys = pu_keys(u), used = (keys + box_rows - 1) / box_rows, r = 2 * i + (values ? 1 : 0), slot = r % kPuRing;
+      if (j < used && (page < 0 || page >= p.n_pages)) {
         give_up(DERR_POSITION);
         page = 0;
       }
-      return page;
-    };
-    for (int i = 0; i < n && ok; ++i) {
-      if (i == 0 || ++u.tile == u.tiles) {
-        u = pu_locate(p, l, f0 + i);
-        const int first = u.pre ? pu_group_start(p, pu_last_not_above(l.pre, l.groups, f0 + i)) : u.b0, s = paged_row_of(p, first);
-        table = p.tables + (size_t)max(s, 0) * p.table_ld;
-        page_next = page_of(u, table, u.shared_tiles + u.tile, u.tile == u.tiles - 1 ? u.last : kPfTile);
-        if (u.pre) {
-          for (int j = 0; j < 4 && ok; ++j) ok = mbar_wait_spin(&q_empty[j], ((q_used >> j) & 1u) ^ 1u);
-          q_used ^= 15u;
-          if (!ok) break;
-          if (lane == 0) {
-            if (u.rows <= 32) {
-              mbar_arrive_expect_tx(&q_full[0], 8u * (uint32_t)(pp.per_quarter * p.group) * 128u);
-              for (int j = 0; j < 8; ++j) tma_load_3d(q_s + (j & 1) * kPfBox + (j >> 1) * 32 * 128, &q_quarter, 64 * (j & 1), u.kv * p.group, u.b0, &q_full[0]);
-            } else {
-              mbar_arrive_expect_tx(&q_full[0], 2u * (uint32_t)(pp.per_tile * p.group) * 128u);
-              for (int j = 0; j < 2; ++j) tma_load_3d(q_s + j * kPfBox, &q_whole, 64 * j, u.kv * p.group, u.b0, &q_full[0]);
-            }
-          }
-        } else {
-          ok = mbar_wait_spin(&q_empty[u.q_slot], ((q_used >> u.q_slot) & 1u) ^ 1u);
-          q_used ^= 1u << u.q_slot;
-          if (!ok) break;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&q_full[u.q_slot], 8u * (uint32_t)p.group * 128u);
-            for (int j = 0; j < 8; ++j)
-              tma_load_3d(q_s + (j & 1) * kPfBox + ((j >> 1) * 32 + 8 * u.q_slot) * 128, &q_own, 64 * (j & 1), u.kv * p.group, u.b0, &q_full[u.q_slot]);
-          }
-        }
-        __syncwarp();
-      }
-      const bool is_last = u.tile == u.tiles - 1;
-      const int keys = is_last ? u.last : kPfTile, page = page_next, tile = u.shared_tiles + u.tile;
-      if (!is_last) page_next = page_of(u, table, tile + 1, u.tile + 1 == u.tiles - 1 ? u.last : kPfTile);
-      const int used = (keys + box_rows - 1) / box_rows, j = lane >> 1, c = lane & 1;
-      const int row = (page << p.page_shift) + ((tile * kPfTile) & ((1 << p.page_shift) - 1) & ~(box_rows - 1));
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int r = 2 * i + kv, slot = r % kPuRing;
-        ok = ok && mbar_wait_spin(&kv_empty[slot], (uint32_t)((r / kPuRing) & 1) ^ 1u);
-        if (!ok) break;
-        uint64_t* bar = kv && (keys & 15) ? &v_raw[slot] : &kv_full[slot];
-        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(used * box_rows) * 256u);
-        __syncwarp();
-        if (j < used) tma_load_2d(kv_s + slot * kPuTile + c * kPfBox + j * box_rows * 128, kv ? &v_map : &k_map, u.kv * kPaDim + 64 * c, row, bar);
-        __syncwarp();
-      }
+      const int row = (page << p.page_shift) + (((u.shared_tiles + u.tile) * kPfTile) & ((1 << p.page_shift) - 1) & ~(box_rows - 1));
+      ok = mbar_wait_spin(&kv_empty[slot], (uint32_t)((r / kPuRing) & 1) ^ 1u);
+      if (!ok) break;
+      uint64_t* bar = values && (keys & 15) ? &v_raw[slot] : &kv_full[slot];
+      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(used * box_rows) * 256u);
+      __syncwarp();
+      if (j < used) tma_load_2d(kv_s + slot * kPuTile + c * kPfBox + j * box_rows * 128, values ? &v_map : &k_map, kvh * kPaDim + 64 * c, row, bar);
+      __syncwarp();
     }
     if (!ok) give_up(DERR_EMPTY_WAIT);
   } else if (warp == 3) {
@@ -328,7 +346,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     uint32_t used = 0;                 // phases of v_raw
     bool ok = true;
     for (int i = 0; i < n && ok;) {
-      u = pu_locate(p, l, f0 + i);
+      if (i == 0) {
+        u = pu_locate(p, l, f0);
+      } else {
+        u.tile = u.tiles - 1;
+        pu_step(p, l, u, f0 + i);
+      }
       const int end = i + u.tiles - u.tile;           // behind the unit's last tile
       if (end <= n && (u.last & 15)) {
         const int r = 2 * (end - 1) + 1, slot = r % kPuRing;
@@ -352,8 +375,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   } else if (warp == 1) {
     // ---- products: the scores of a tile, then the weighted values of the tile before
     const bool leader = elect_one();
-    const uint32_t idesc_o = umma_idesc_bf16(kPaDim) | (1u << 16);     // (bit 16: B is N-major)
-    const uint64_t qd = umma_desc_sw128(q_s), kd = umma_desc_sw128(kv_s), vd = pf_desc_mn(kv_s);
+    const uint32_t idesc_o = umma_idesc_bf16(kPaDim) | (1u << 16);     // (bit 16: B is N-major; bit 15: A is M-major)
+    const uint64_t qd = umma_desc_sw128(q_s), kd = umma_desc_sw128(kv_s), vd = pf_desc_mn(kv_s), wd = umma_desc_sw128(w_s);
     uint32_t q_seen = 0;
     int made[2] = {0, 0}, freed[2] = {0, 0};          // tiles of a parity so far, results read
     bool ok = true;
@@ -371,11 +394,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
       if (!good) return false;
       tc_fence_after();
       if (leader) {
-        const int steps = w.tile == w.tiles - 1 ? (w.last + 15) >> 4 : 8;
+        const int steps = (pu_keys(w) + 15) >> 4, wide = pu_wide<TERMS>(w);
         const uint64_t at = vd + (uint64_t)(slot * (kPuTile >> 4));
-        for (int k = 0; k < steps; ++k) umma_f16_ts(o_t, s_t + 8u * k, at + (uint64_t)(k * (2048 >> 4)), idesc_o, !first || k != 0);
-        if (TERMS == 2 || w.rows <= 32)
-          for (int k = 0; k < steps; ++k) umma_f16_ts(o_t, s_t + 64u + 8u * k, at + (uint64_t)(k * (2048 >> 4)), idesc_o, 1u);
+        if (wide) {
+          const uint32_t idesc = umma_idesc_bf16(wide == 8 ? 16 : 32) | (1u << 15);
+          for (int k = 0; k < steps; ++k)
+            umma_f16(o_t, at + (uint64_t)(k * (2048 >> 4)), wd + (uint64_t)(x * (kPuWeights >> 4) + (k >> 2) * (kPuWeights >> 5) + 2 * (k & 3)), idesc, !first || k != 0);
+        } else {
+          for (int k = 0; k < steps; ++k) umma_f16_ts(o_t, s_t + 8u * k, at + (uint64_t)(k * (2048 >> 4)), idesc_o, !first || k != 0);
+          if (TERMS == 2)
+            for (int k = 0; k < steps; ++k) umma_f16_ts(o_t, s_t + 64u + 8u * k, at + (uint64_t)(k * (2048 >> 4)), idesc_o, 1u);
+        }
         umma_commit(&o_done[x]);
         umma_commit(&kv_empty[slot]);
       }
@@ -384,8 +413,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     };
     for (int i = 0; i < n && ok; ++i) {
       const int x = (f0 + i) & 1, r = 2 * i, slot = r % kPuRing;
-      if (i == 0 || ++u.tile == u.tiles) {
-        u = pu_locate(p, l, f0 + i);
+      if (i == 0) u = pu_locate(p, l, f0);
+      else pu_step(p, l, u, f0 + i);
+      if (i == 0 || u.tile == 0) {
         fresh[0] = fresh[1] = true;
         ok = mbar_wait_spin(&q_full[u.q_slot], (q_seen >> u.q_slot) & 1u);
         q_seen ^= 1u << u.q_slot;
@@ -396,11 +426,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
       tc_fence_after();
       if (leader) {
         const uint32_t s_t = tmem + (uint32_t)(x * 256);
-        const uint32_t idesc_s = umma_idesc_bf16(u.tile == u.tiles - 1 ? (u.last + 15) & ~15 : kPfTile);
+        const int wide = pu_wide<TERMS>(u);
+        const uint32_t idesc = umma_idesc_bf16(wide ? (wide == 32 ? 32 : 16) : kPfTile);
+        const uint64_t keys = kd + (uint64_t)(slot * (kPuTile >> 4)), queries = qd + (uint64_t)(u.q_slot * (16 * 128 >> 4));
+        const uint64_t da = wide ? keys : queries, db = wide ? queries : keys;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const uint32_t off = (uint32_t)((k >> 2) * (kPfBox >> 4) + 2 * (k & 3));
-          umma_f16(s_t, qd + off, kd + (uint32_t)(slot * (kPuTile >> 4)) + off, idesc_s, k != 0);
+          const uint64_t off = (uint64_t)((k >> 2) * (kPfBox >> 4) + 2 * (k & 3));
+          umma_f16(s_t, da + off, db + off, idesc, k != 0);
         }
         umma_commit(&s_full[x]);
         umma_commit(&kv_empty[slot]);
@@ -418,95 +451,144 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     if (ok && n > 0) ok = values(n - 1, before, before_fresh);
     if (!ok) give_up(DERR_FULL_WAIT);
   } else if (warp >= 4) {
-    // ---- softmax of the tiles of a parity.  More than 32 rows: a thread per row.  Up to 32: the queries stand in all four quarters of the tensor
-    // memory's lanes, and a warp takes 32 of the tile's keys for them (weights of zero for the others), so that a thread has 32 scores instead of 128.
+    // ---- softmax of the tiles of a parity.  More than 32 rows: S = Q K^T, a thread per row, the weights over the scores' columns.  Up to 32: the keys are
+    // the tensor memory's lanes, S^T = K Q^T and O^T = V^T P, with as many columns as there are rows (a product of 128 x 128 x 16 takes 84 cycles for four
+    // rows too, one of 128 x 16 x 16 a fraction): a thread per key, whose weights go to shared memory, each as two bf16 terms in rows of their own.
+    // The reference that scores are taken from is their maximum in the unit's first tile: a bf16 weight may be as large as an f32 one, so that
+    // nothing is rescaled; a weight above 2^96 leaves a sum that is no number, and the joining kernel goes through the row's keys one by one.
     const int x = (warp - 4) >> 2, q4 = warp & 3;
     const uint32_t s_t = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)(x * 256), o_t = s_t + 128u;
-    float* stage = stage_s + x * (kPuStage / 4);
-    float m = -FLT_MAX, l_sum = 0.f;
+    float *max_s = meet_s + x * 256, *sum_s = max_s + 128;             // [warp][32 rows]
+    auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory"); };
+    float ref[16], sums[32], largest = 0.f;            // (32 rows: the references stay in max_s)
     bool ok = true, first = true;
     int done = 0;                      // tiles of this parity
     PuUnit u;
     int unit_end = 0;                  // the tile behind the unit's last, or the CTA's
-    for (int i = (f0 & 1) == x ? 0 : 1; i < n && ok; i += 2) {
-      if (i >= unit_end) {
-        u = pu_locate(p, l, f0 + i);
+    // a tile whose lanes are keys
+    auto keyed = [&](auto rows_c) {
+      constexpr int NR = decltype(rows_c)::value;
+      constexpr bool kTwo = NR < 32;
+      float v[NR];
+      if constexpr (NR == 8) tmem_ld8(s_t, v);
+      else if constexpr (NR == 16) tmem_ld16(s_t, v);
+      else pf_ld32(s_t, v);
+      const int key = 32 * q4 + lane;
+      const bool seen = key < pu_keys(u);
+      if (first) {
+        float mine = -FLT_MAX;
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+          if (r < u.rows) {
+            const float mx = warp_max(seen ? v[r] : -FLT_MAX);
+            if (lane == r) mine = mx;
+          }
+        max_s[32 * q4 + lane] = mine;
+        meet();
+        if constexpr (NR == 32) {
+          const float mx = fmaxf(fmaxf(max_s[lane], max_s[32 + lane]), fmaxf(max_s[64 + lane], max_s[96 + lane]));
+          meet();                                      // (everyone has read: a warp's own 32 become the references)
+          max_s[32 * q4 + lane] = mx;
+          __syncwarp();
+        } else {
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            ref[r] = fmaxf(fmaxf(max_s[r], max_s[32 + r]), fmaxf(max_s[64 + r], max_s[96 + r]));
+            ref[r] = ref[r] == -FLT_MAX ? ref[r] : ref[r] * p.scale_log2;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < NR; ++r) sums[r] = 0.f;
+      }
+      uint8_t* at = w_s + x * kPuWeights + (key >> 6) * (kPuWeights / 2) + 2 * (key & 7);
+      const int chunk = (key & 63) >> 3;
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+        if (r < u.rows) {
+          float from;
+          if constexpr (NR == 32) from = max_s[32 * q4 + r] == -FLT_MAX ? -FLT_MAX : max_s[32 * q4 + r] * p.scale_log2;
+          else from = ref[r];
+          const float w = seen ? ex2(fmaf(v[r], p.scale_log2, -from)) : 0.f;
+          sums[r] += w;
+          largest = fmaxf(largest, w);
+          const __nv_bfloat16 hi = __float2bfloat16_rn(w);
+          *reinterpret_cast<__nv_bfloat16*>(at + r * 128 + ((chunk ^ (r & 7)) << 4)) = hi;
+          if constexpr (kTwo) *reinterpret_cast<__nv_bfloat16*>(at + (NR + r) * 128 + ((chunk ^ (r & 7)) << 4)) = __float2bfloat16_rn(w - __bfloat162float(hi));
+        }
+      tc_fence_before();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    };
+    auto keyed_out = [&](auto rows_c, float* to_o, float* to_ml) {
+      constexpr int NR = decltype(rows_c)::value;
+      constexpr bool kTwo = NR < 32;
+      float o[32];
+      if constexpr (NR == 8) {
+        float w[16];
+        tmem_ld16(o_t, w);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) o[r] = w[r] + w[8 + r];
+      } else {
+        pf_ld32(o_t, o);
+        if constexpr (kTwo)
+#pragma unroll
+          for (int r = 0; r < NR; ++r) o[r] += o[NR + r];
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_free[x]);          // (the next unit's products may begin)
+      float mine = 0.f;
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+        if (r < u.rows) {
+          to_o[(size_t)r * 2 * kPaDim + 32 * q4 + lane] = o[r];
+          const float sum = warp_sum(largest > kPuLargest ? NAN : sums[r]);
+          if (lane == r) mine = sum;
+        }
+      sum_s[32 * q4 + lane] = mine;
+      meet();
+      if (q4 == 0 && lane < u.rows) {
+        const float mx = fmaxf(fmaxf(max_s[lane], max_s[32 + lane]), fmaxf(max_s[64 + lane], max_s[96 + lane]));
+        *reinterpret_cast<float2*>(to_ml + lane * 4) =
+            make_float2(mx == -FLT_MAX ? mx : mx * p.scale_log2, (sum_s[lane] + sum_s[32 + lane]) + (sum_s[64 + lane] + sum_s[96 + lane]));
+      }
+      meet();                                          // (the next unit's maxima go where these were)
+    };
+    using R8 = std::integral_constant<int, 8>;
+    using R16 = std::integral_constant<int, 16>;
+    using R32 = std::integral_constant<int, 32>;
+    for (int i = 0; i < n && ok; ++i) {
+      if (i == 0) u = pu_locate(p, l, f0);
+      else pu_step(p, l, u, f0 + i);
+      if (i == 0 || u.tile == 0) {
         unit_end = min(n, i + u.tiles - u.tile);
         first = true;
-        m = -FLT_MAX;
-        l_sum = 0.f;
-      } else {
-        u.tile += 2;
+        largest = 0.f;
       }
-      const bool quarter = u.rows <= 32;
-      const int r = quarter ? lane - (u.pre ? 0 : 8 * u.q_slot) : 32 * q4 + lane;
-      const bool live = r >= 0 && r < u.rows;
+      if (((f0 + i) & 1) != x) continue;
+      const int wide = pu_wide<TERMS>(u), r = 32 * q4 + lane;
+      const bool live = r < u.rows;
       ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[x], (uint32_t)(done & 1)));
       if (!ok) break;
       tc_fence_after();
-      auto rescale = [&](float mx) {                   // (the products so far are done: these scores were asked for after them)
-        const bool grown = live && mx > m;
-        if (first) {
-          m = mx;
-        } else if (__any_sync(0xffffffffu, grown)) {
-          const float to = grown ? mx : m, f = ex2(m - to);
-#pragma unroll 1
-          for (int c = 0; c < kPaDim; c += 32) {
-            float o[32];
-            pf_ld32(o_t + (uint32_t)c, o);
-            uint32_t w0[16], w1[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              w0[j] = __float_as_uint(o[j] * f);
-              w1[j] = __float_as_uint(o[16 + j] * f);
-            }
-            tmem_st16(o_t + (uint32_t)c, w0);
-            tmem_st16(o_t + (uint32_t)c + 16u, w1);
-          }
-          l_sum *= f;
-          m = to;
-        }
-      };
-      if (quarter) {
-        const int keys = min(max((u.tile == u.tiles - 1 ? u.last : kPfTile) - 32 * q4, 0), 32);
-        float v[32];
-        pf_ld32(s_t + 32u * q4, v);
-        float mx = -FLT_MAX;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) mx = fmaxf(mx, j < keys ? v[j] : -FLT_MAX);
-        rescale(mx == -FLT_MAX ? mx : mx * p.scale_log2);
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t hi[16], lo[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float w0 = 2 * j < keys ? ex2(fmaf(v[2 * j], p.scale_log2, -m)) : 0.f, w1 = 2 * j + 1 < keys ? ex2(fmaf(v[2 * j + 1], p.scale_log2, -m)) : 0.f;
-          sum[j & 3] += w0 + w1;
-          split_bf16(w0, w1, hi[j], lo[j]);
-        }
-        l_sum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        uint32_t zero[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) zero[j] = 0u;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (q == q4) {
-            tmem_st16(s_t + 16u * q, hi);
-            tmem_st16(s_t + 64u + 16u * q, lo);
-          } else {
-            tmem_st16(s_t + 16u * q, zero);
-            tmem_st16(s_t + 64u + 16u * q, zero);
-          }
-        }
+      if (wide == 8) {
+        keyed(R8());
+      } else if (wide == 16) {
+        keyed(R16());
+      } else if (TERMS == 1 && wide == 32) {
+        keyed(R32());
       } else {
-        float mx = -FLT_MAX;
+        if (first) {
+          float mx = -FLT_MAX;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v[32];
-          pf_ld32(s_t + 32u * c, v);
+          for (int c = 0; c < 4; ++c) {
+            float v[32];
+            pf_ld32(s_t + 32u * c, v);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[j]);
+            for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[j]);
+          }
+          ref[0] = mx == -FLT_MAX ? mx : mx * p.scale_log2;
+          sums[0] = 0.f;
         }
-        rescale(mx == -FLT_MAX ? mx : mx * p.scale_log2);
         uint32_t low[TERMS == 2 ? 64 : 1];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -516,14 +598,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const float w0 = ex2(fmaf(v[2 * j], p.scale_log2, -m)), w1 = ex2(fmaf(v[2 * j + 1], p.scale_log2, -m));
+            const float w0 = ex2(fmaf(v[2 * j], p.scale_log2, -ref[0])), w1 = ex2(fmaf(v[2 * j + 1], p.scale_log2, -ref[0]));
             sum[j & 3] += w0 + w1;
             if constexpr (TERMS == 2) split_bf16(w0, w1, w[j], low[16 * c + j]);
             else w[j] = pack_bf16(w0, w1);
           }
-          l_sum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          sums[0] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_st16(s_t + 16u * c, w);                 // over scores that this thread has read
         }
+        largest = sums[0];
         if constexpr (TERMS == 2)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -532,10 +615,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
             for (int j = 0; j < 16; ++j) w[j] = low[16 * c + j];
             tmem_st16(s_t + 64u + 16u * c, w);
           }
+        tmem_st_wait();
+        tc_fence_before();
       }
       first = false;
-      tmem_st_wait();
-      tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[x]);
       ++done;
@@ -545,83 +628,31 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
       ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[x], (uint32_t)((done - 1) & 1)));
       if (!ok) break;
       tc_fence_after();
-      const size_t row0 = (size_t)u.slot + (size_t)(u.pre ? 128 : 8) * blockIdx.x;
-      float *to_o = u.pre ? pp.pre_o : pp.own_o, *to_ml = u.pre ? pp.pre_ml : pp.own_ml;
-      if (!quarter) {
-        float* o_row = to_o + ((row0 + r) * 2 + x) * kPaDim;
+      const int apart = u.pre ? 128 : 8;
+      const size_t row0 = (size_t)kvh * (p.batch * p.group + apart * pp.per_head) + u.slot + apart * part;
+      float *to_o = (u.pre ? pp.pre_o : pp.own_o) + (row0 * 2 + x) * kPaDim, *to_ml = (u.pre ? pp.pre_ml : pp.own_ml) + (row0 * 2 + x) * 2;
+      if (wide == 8) {
+        keyed_out(R8(), to_o, to_ml);
+      } else if (wide == 16) {
+        keyed_out(R16(), to_o, to_ml);
+      } else if (TERMS == 1 && wide == 32) {
+        keyed_out(R32(), to_o, to_ml);
+      } else {
 #pragma unroll 1
         for (int c = 0; c < kPaDim; c += 32) {
           float o[32];
           pf_ld32(o_t + (uint32_t)c, o);
+          float4* o_row = reinterpret_cast<float4*>(to_o + (size_t)r * 2 * kPaDim + c);
           if (live)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) reinterpret_cast<float4*>(o_row + c)[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            for (int j = 0; j < 8; ++j) o_row[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
         }
-        if (live) *reinterpret_cast<float2*>(to_ml + ((row0 + r) * 2 + x) * 2) = make_float2(m, l_sum);
-      } else {
-        // the four warps' parts of a row meet here: their maxima and sums, then 16 or 64 columns at a time
-        auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory"); };
-        if (live) {
-          stage[(4 * r + q4) * 2] = m;
-          stage[(4 * r + q4) * 2 + 1] = l_sum;
-        }
-        meet();
-        float top = -FLT_MAX, all = 0.f;
-        if (live) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) top = fmaxf(top, stage[(4 * r + w) * 2]);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) all += stage[(4 * r + w) * 2 + 1] * ex2(stage[(4 * r + w) * 2] - top);
-          if (q4 == 0) *reinterpret_cast<float2*>(to_ml + ((row0 + r) * 2 + x) * 2) = make_float2(top, all);
-        }
-        const float f = ex2(m - top);
-        const int t = (int)(threadIdx.x & 127);
-        meet();
-        if (u.rows <= 8) {
-          constexpr int kLd = 65;                      // [warp][8 rows][64 columns]
-#pragma unroll 1
-          for (int c = 0; c < kPaDim; c += 64) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float o[32];
-              pf_ld32(o_t + (uint32_t)(c + 32 * h), o);
-              if (live)
-#pragma unroll
-                for (int j = 0; j < 32; ++j) stage[(q4 * 8 + r) * kLd + 32 * h + j] = o[j] * f;
-            }
-            meet();
-            for (int k = t; k < u.rows * 64; k += 128) {
-              const int row = k >> 6, col = k & 63;
-              float sum = 0.f;
-#pragma unroll
-              for (int w = 0; w < 4; ++w) sum += stage[(w * 8 + row) * kLd + col];
-              to_o[((row0 + row) * 2 + x) * kPaDim + c + col] = sum;
-            }
-            meet();
-          }
-        } else {
-#pragma unroll 1
-          for (int c = 0; c < kPaDim; c += 16) {
-            float o[16];
-            tmem_ld16(o_t + (uint32_t)c, o);
-            if (live)
-#pragma unroll
-              for (int j = 0; j < 16; ++j) stage[(q4 * 32 + r) * kPuStageLd + j] = o[j] * f;
-            meet();
-            for (int k = t; k < u.rows * 16; k += 128) {
-              const int row = k >> 4, col = k & 15;
-              float sum = 0.f;
-#pragma unroll
-              for (int w = 0; w < 4; ++w) sum += stage[(w * 32 + row) * kPuStageLd + col];
-              to_o[((row0 + row) * 2 + x) * kPaDim + c + col] = sum;
-            }
-            meet();
-          }
-        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[x]);
+        if (live)
+          *reinterpret_cast<float2*>(to_ml + r * 4) = make_float2(ref[0], largest > kPuLargest ? NAN : sums[0]);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&o_free[x]);
     }
     if (!ok) give_up(DERR_TMEM);
   }
@@ -631,65 +662,64 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
 }
 
 // Joins the pieces of a query head: a warp per head, four columns a lane.
-__global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp, int n_ctas) {
+__global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
   pdl_wait();
   pdl_launch_dependents();
   const PagedParams& p = pp.a;
-  const int b = blockIdx.x, lane = threadIdx.x & 31;
+  const int b = blockIdx.x, lane = threadIdx.x & 31, J = pp.per_head;
   const PuSeqPlan q = pp.plan[b];
   const int total = *pp.plan_total;
-  for (int head = (int)(blockIdx.y * 4 + (threadIdx.x >> 5)); head < p.n_heads; head += gridDim.y * 4) {
+  const int head = (int)(blockIdx.y * 4 + (threadIdx.x >> 5));
+  if (head < p.n_heads) {
     const int kv = head / p.group, h = head - kv * p.group;
     // tiles of the list, first CTA and number of (CTA, parity) places of the own and of the shared part
-    int f[2], e[2], c[2], places[2];
-    f[0] = q.own_f + kv * q.own_tiles;
-    e[0] = f[0] + q.own_tiles;
-    f[1] = q.pre_f + kv * q.pre_kv;
-    e[1] = f[1] + q.pre_tiles;
+    const int f[2] = {q.own_f, q.pre_f}, e[2] = {q.own_f + q.own_tiles, q.pre_f + q.pre_tiles}, wide[2] = {8, 128};
+    int c[2] = {0, 0}, places[2] = {0, 0};
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      c[k] = places[k] = 0;
+    for (int k = 0; k < 2; ++k)
       if (e[k] > f[k]) {
-        c[k] = (int)(((long long)(f[k] + 1) * n_ctas - 1) / total);
-        places[k] = 2 * ((int)(((long long)e[k] * n_ctas - 1) / total) - c[k] + 1);
+        c[k] = (int)(((long long)(f[k] + 1) * J - 1) / total);
+        places[k] = 2 * ((int)(((long long)e[k] * J - 1) / total) - c[k] + 1);
+      }
+    const int all = places[0] + places[1];
+    float top = -FLT_MAX, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int base = 0; base < all; base += 32) {
+      // a lane per place: its row of the partial results (none where the CTA has no tile of the parity), maximum and sum
+      const int i = base + lane;
+      const float *row = nullptr, *ml = nullptr;
+      if (i < all) {
+        const int k = i >= places[0], j = k ? i - places[0] : i, cta = c[k] + (j >> 1), x = j & 1;
+        const int lo = max(f[k], (int)((long long)total * cta / J)), hi = min(e[k], (int)((long long)total * (cta + 1) / J));
+        if (hi - lo > 1 || (hi - lo == 1 && (lo & 1) == x)) {
+          const size_t r = ((size_t)kv * (p.batch * p.group + wide[k] * J) + b * p.group + h + (size_t)wide[k] * cta) * 2 + x;
+          row = (k ? pp.pre_o : pp.own_o) + r * kPaDim;
+          ml = (k ? pp.pre_ml : pp.own_ml) + r * 2;
+        }
+      }
+      float2 mine = make_float2(-FLT_MAX, 0.f);
+      if (ml) mine = *reinterpret_cast<const float2*>(ml);
+      const float to = fmaxf(top, warp_max(mine.x)), f0 = ex2(top - to), w = ex2(mine.x - to);
+      top = to;
+      l = l * f0 + warp_sum(mine.y * w);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] *= f0;
+      const int count = min(32, all - base);
+#pragma unroll 8
+      for (int k = 0; k < count; ++k) {
+        const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)row, k));
+        const float wk = __shfl_sync(0xffffffffu, w, k);
+        if (from) {
+          const float4 v = *reinterpret_cast<const float4*>(from + 4 * lane);
+          o[0] = fmaf(v.x, wk, o[0]);
+          o[1] = fmaf(v.y, wk, o[1]);
+          o[2] = fmaf(v.z, wk, o[2]);
+          o[3] = fmaf(v.w, wk, o[3]);
+        }
       }
     }
-    const size_t own_row = (size_t)(b * p.n_kv + kv) * p.group + h, pre_row = (size_t)q.pre_row + (size_t)kv * q.pre_row_kv + h;
-    const int all = places[0] + places[1];
-    // place i: its row of the partial results, or none
-    auto row_of = [&](int i, bool& pre) -> long long {
-      pre = i >= places[0];
-      const int k = pre, j = pre ? i - places[0] : i, cta = c[k] + (j >> 1), x = j & 1;
-      const int lo = max(f[k], (int)((long long)total * cta / n_ctas)), hi = min(e[k], (int)((long long)total * (cta + 1) / n_ctas));
-      if (hi - lo < 1 || (hi - lo == 1 && (lo & 1) != x)) return -1;
-      return (long long)(((pre ? pre_row : own_row) + (size_t)(pre ? 128 : 8) * cta) * 2 + x);
-    };
-    float top = -FLT_MAX;
-    for (int i = lane; i < all; i += 32) {
-      bool pre;
-      const long long r = row_of(i, pre);
-      if (r >= 0) top = fmaxf(top, (pre ? pp.pre_ml : pp.own_ml)[2 * r]);
-    }
-    top = warp_max(top);
-    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int i = 0; i < all; ++i) {
-      bool pre;
-      const long long r = row_of(i, pre);
-      if (r < 0) continue;
-      const float2 ml = *reinterpret_cast<const float2*>((pre ? pp.pre_ml : pp.own_ml) + 2 * r);
-      const float4 v = *reinterpret_cast<const float4*>((pre ? pp.pre_o : pp.own_o) + r * kPaDim + 4 * lane);
-      const float w = ex2(ml.x - top);
-      l += ml.y * w;
-      o[0] = fmaf(v.x, w, o[0]);
-      o[1] = fmaf(v.y, w, o[1]);
-      o[2] = fmaf(v.z, w, o[2]);
-      o[3] = fmaf(v.w, w, o[3]);
-    }
     const size_t at = ((size_t)b * p.n_heads + head) * kPaDim + 4 * lane;
-    if (__any_sync(0xffffffffu, o[0] != o[0] || o[1] != o[1] || o[2] != o[2] || o[3] != o[3])) {
-      // An infinite value times a weight of zero, in the quarters that do not have its key, is no number, though the sum may be infinite: once more,
-      // key by key.
+    if (__any_sync(0xffffffffu, l != l || o[0] != o[0] || o[1] != o[1] || o[2] != o[2] || o[3] != o[3])) {
+      // A score far above those of its unit's first tile, or an infinite value beside a weight that is zero as a second term: once more, key by key.
       const int s = paged_row_of(p, b), len = s < 0 ? 0 : min(max(p.lens[s], 0), p.max_len);
       float m = -FLT_MAX, x[4];
       l = o[0] = o[1] = o[2] = o[3] = 0.f;
@@ -770,7 +800,10 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   pp.per_quarter = 32 / p.group;
   const size_t tiles = batch * (((size_t)p.max_len + kPfTile - 1) / kPfTile) * n_kv_heads;
   TQ_REQUIRE(ctx, tiles < (1ull << 30) && (size_t)p.n_pages * pages->page_rows < (1ull << 31), "tq_gqa_decode_paged: too many positions");
-  const size_t n_ctas = tiles < (size_t)ctx->sm_count ? tiles : (size_t)ctx->sm_count;
+  // as many CTAs for every KV head, one an SM
+  const size_t per_kv = tiles / n_kv_heads, fit = (size_t)ctx->sm_count / n_kv_heads;
+  pp.per_head = (int)(per_kv < fit ? per_kv : fit < 1 ? 1 : fit);
+  const size_t n_ctas = n_kv_heads * (size_t)pp.per_head;
   // partial results, the sequences' plans
   const size_t own_rows = (batch * n_heads + 8 * n_ctas) * 2, pre_rows = p.n_groups ? (batch * n_heads + 128 * n_ctas) * 2 : 0;
   const size_t floats = (own_rows + pre_rows) * (kPaDim + 2);
@@ -793,6 +826,6 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   auto kern = p.out_f32 ? paged_decode_kernel<2> : paged_decode_kernel<1>;
   TQ_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kPuFixed + (4 * kPuBatch + 2) * sizeof(int))));
   TQ_CUDA(ctx, launch_k(ctx, kern, dim3((unsigned)n_ctas), dim3(kPuThreads), smem, qo, qq, qw, km, vm, pp));
-  TQ_CUDA(ctx, launch_k(ctx, paged_join_kernel, dim3((unsigned)batch, (unsigned)((n_heads + 3) / 4)), dim3(128), 0, pp, (int)n_ctas));
+  TQ_CUDA(ctx, launch_k(ctx, paged_join_kernel, dim3((unsigned)batch, (unsigned)((n_heads + 3) / 4)), dim3(128), 0, pp));
   return TQ_OK;
 }
