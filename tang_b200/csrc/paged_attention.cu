@@ -32,12 +32,12 @@ __device__ __forceinline__ int paged_row_of(const PagedParams& p, int b) {
   return s >= 0 && s < p.n_seqs ? s : -1;
 }
 // ---------------------------------------------------------------------------------------------
-// Units, tiles, pieces.  A unit is what meets the same keys: the rows (member, query head of one KV head) of up to 128 / group members of a group over
-// the group's shared positions, in whole tiles of 128, or one sequence's query heads over the rest.  The tiles of all units of a KV head stand in one list,
-// shared ones first, and CTA j of the J that a KV head has takes tiles T j / J .. T (j + 1) / J - 1: the same number each, whatever the lengths.
-// (CTAs of all KV heads walk their lists at the same pace: a cache row holds all of them, and its 256 bytes a head are fetched at the same time.)  Odd and
-// even tiles of the list belong to different softmax groups, which keep maximum, sum and products of their own: a piece (unit, CTA, parity) leaves
-// one partial result.
+// Units, tiles, items, pieces.  A unit is what meets the same keys: the rows (member, query head of one KV head) of up to 128 / group members of a group
+// over the group's shared positions, in whole tiles of 128, or one sequence's query heads over the rest.  The tiles of all units of a KV head stand in one
+// list, shared ones first, and are cut into items of equal length; CTAs, one an SM, take two items each and then the next one that nobody has, whatever
+// the lengths of the sequences and the speeds of the SMs.  (Items of all KV heads that stand at the same place of their lists follow one another: a cache
+// row holds all heads, and its 256 bytes a head are fetched at the same time.)  A piece is what an item has of a unit.  Its odd and its even tiles belong
+// to different softmax groups, which keep sums and products of their own and leave a partial result each.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPuThreads = 384;
 constexpr int kPuTile = 4 * kPfBox / 2;               // bytes of 128 rows of keys or values
@@ -45,7 +45,8 @@ constexpr int kPuRing = 5;
 constexpr int kPuWeights = 2 * 32 * 128;              // a parity's weights where keys are the lanes: 32 rows of 128 keys, in two halves
 constexpr int kPuMeet = 2 * 2 * 4 * 32 * 4;           // [parity][maxima, sums][warp][row]
 constexpr float kPuLargest = 7.9228162514264338e28f;  // 2^96: a weight above it is too far from its reference
-constexpr int kPuHeader = 256;                        // barriers
+constexpr int kPuHeader = 384;                        // barriers, items
+constexpr int kPuReaders = 11;                        // warps that are told the items
 constexpr int kPuBatch = 1024;                        // sequences of a call
 constexpr size_t kPuFixed = 2 * (size_t)kPfBox + kPuRing * (size_t)kPuTile + 2 * (size_t)kPuWeights + kPuMeet + kPuHeader;
 
@@ -54,12 +55,12 @@ struct PuPlan {
   int *own, *last, *pre, *eff;                        // [batch + 1] own tiles of the sequences before; [batch] shared tiles << 8 | keys of the last tile - 1;
                                                       // [groups + 1] units' shared tiles of the groups before; [groups] tiles that a group shares
   int batch, groups, group, per_tile, pre_tiles, total;
+  int n_kv, pre_len, own_len, pre_items, items;       // tiles of an item, items of a KV head
 };
 struct PuUnit {
   bool pre;
   int b0, rows, tiles, tile, shared_tiles, last;      // b0: (first) sequence of the batch; tile: the asked one; last: keys of the last tile
-  int slot;                                           // first row of its partial results, without what the KV head and the CTA add
-  int q_slot;
+  int slot;                                           // first row of its partial results, without what KV head and item add
 };
 
 __device__ __forceinline__ int pu_group_start(const PagedParams& p, int g) { return min(max(p.group_starts[g], 0), p.batch); }
@@ -86,7 +87,6 @@ __device__ __forceinline__ PuUnit pu_locate(const PagedParams& p, const PuPlan& 
     u.shared_tiles = 0;
     u.last = kPfTile;
     u.slot = u.b0 * l.group;
-    u.q_slot = 0;
   } else {
     const int h = f - l.pre_tiles, b = pu_last_not_above(l.own, l.batch, h);
     u.tiles = l.own[b + 1] - l.own[b];
@@ -96,7 +96,6 @@ __device__ __forceinline__ PuUnit pu_locate(const PagedParams& p, const PuPlan& 
     u.shared_tiles = l.last[b] >> 8;
     u.last = (l.last[b] & 255) + 1;
     u.slot = b * l.group;
-    u.q_slot = b & 3;
   }
   return u;
 }
@@ -116,25 +115,52 @@ __device__ __forceinline__ void pu_step(const PagedParams& p, const PuPlan& l, P
   u.shared_tiles = l.last[b] >> 8;
   u.last = (l.last[b] & 255) + 1;
   u.slot = b * l.group;
-  u.q_slot = b & 3;
 }
 // Rows that are laid out for a unit whose keys are the tensor memory's lanes (0: its rows are), each as two terms but for the 32 of bf16 results.
 template <int TERMS>
 __device__ __forceinline__ int pu_wide(const PuUnit& u) { return u.rows <= 8 ? 8 : u.rows <= 16 ? 16 : u.rows <= 32 && TERMS == 1 ? 32 : 0; }
 __device__ __forceinline__ int pu_keys(const PuUnit& u) { return u.tile == u.tiles - 1 ? u.last : kPfTile; }
 
-// What the kernel that joins the pieces has to know of a sequence: where its tiles stand in a KV head's list.
+// A role's place in the CTA's items.
+struct PuCursor {
+  PuUnit u;
+  int f, end, kv, item;                               // tile of the list, the item's end; item: its number among the KV head's shared or own ones
+  int piece;                                          // first tile of the piece
+};
+__device__ __forceinline__ void pu_begin(const PagedParams& p, const PuPlan& l, PuCursor& c, int item) {
+  const int k = item / l.n_kv;
+  c.kv = item - k * l.n_kv;
+  const bool pre = k < l.pre_items;
+  c.item = pre ? k : k - l.pre_items;
+  c.f = pre ? c.item * l.pre_len : l.pre_tiles + c.item * l.own_len;
+  c.end = pre ? min(c.f + l.pre_len, l.pre_tiles) : min(c.f + l.own_len, l.total);
+  c.piece = c.f;
+  c.u = pu_locate(p, l, c.f);
+}
+// Within an item: to the next tile, which exists.
+__device__ __forceinline__ void pu_next(const PagedParams& p, const PuPlan& l, PuCursor& c) {
+  ++c.f;
+  pu_step(p, l, c.u, c.f);
+  if (c.u.tile == 0) c.piece = c.f;
+}
+__device__ __forceinline__ int pu_piece_end(const PuCursor& c) { return min(c.end, c.f + c.u.tiles - c.u.tile); }
+// Places in the ring, in the order in which they are needed: keys 0, keys 1, values 0, keys 2, values 1 ..
+__device__ __forceinline__ int pu_keys_at(int t) { return t == 0 ? 0 : 2 * t - 1; }
+__device__ __forceinline__ int pu_values_at(int t) { return 2 * t + 2; }
+
+// What the kernel that joins the pieces has to know: where a sequence's tiles stand in a KV head's list, and how the list is cut.
 struct PuSeqPlan {
-  int own_f, own_tiles, pre_f, pre_tiles;
+  int own_f, own_tiles, pre_f, pre_tiles;             // (the place among the own, the shared tiles)
 };
 
 struct PuParams {
   PagedParams a;
   int per_tile, per_quarter;                          // members of a row tile; of a row tile that fits 32 rows
-  int per_head;                                       // CTAs of a KV head
-  float *own_o, *own_ml, *pre_o, *pre_ml;             // partial results: [row][parity][128], [row][parity][2]
+  int max_pre, max_own;                               // items of a KV head at most
+  float *own_o, *own_ml, *pre_o, *pre_ml;             // partial results: [row][2][128], [row][2][2]
   PuSeqPlan* plan;
-  int* plan_total;
+  int* plan_cut;                                      // [2] tiles of a shared, an own item
+  int* counter;                                       // items handed out beyond the first two of every CTA; zero between calls
 };
 
 __device__ __forceinline__ void pu_scan(int* a, int n, int lane) {      // a[0 .. n-1] become the sums before them, a[n] the sum; one warp
@@ -181,7 +207,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   uint64_t* p_full = s_full + 2;
   uint64_t* o_done = p_full + 2;
   uint64_t* o_free = o_done + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 2);
+  uint64_t* item_full = o_free + 2;                   // [4]
+  uint64_t* item_empty = item_full + 4;
+  uint64_t* met = item_empty + 4;                     // [parity] the four warps of a softmax group
+  int* item_s = reinterpret_cast<int*>(met + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(item_s + 4);
   PuPlan l;
   l.own = reinterpret_cast<int*>(q_full) + kPuHeader / 4;
   l.last = l.own + p.batch + 1;
@@ -191,12 +221,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   l.groups = p.n_groups;
   l.group = p.group;
   l.per_tile = pp.per_tile;
+  l.n_kv = p.n_kv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < 4; ++i) {
         mbar_init(&q_full[i], 1);
         mbar_init(&q_empty[i], 1);
+        mbar_init(&item_full[i], 1);
+        mbar_init(&item_empty[i], kPuReaders);
       }
       for (int i = 0; i < kPuRing; ++i) {
         mbar_init(&kv_full[i], 1);
@@ -208,6 +241,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         mbar_init(&p_full[x], 4);
         mbar_init(&o_done[x], 1);
         mbar_init(&o_free[x], 4);
+        mbar_init(&met[x], 4);
       }
       mbar_init_fence();
     }
@@ -259,8 +293,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   const uint32_t tmem = *tmem_slot;
   l.pre_tiles = l.pre[p.n_groups];
   l.total = l.pre_tiles + l.own[p.batch];
-  const int kvh = (int)(blockIdx.x % p.n_kv), part = (int)(blockIdx.x / p.n_kv);
-  const int f0 = (int)((long long)l.total * part / pp.per_head), f1 = (int)((long long)l.total * (part + 1) / pp.per_head), n = f1 - f0;
+  const int own_tiles = l.own[p.batch];
+  l.pre_len = max(1, (l.pre_tiles + pp.max_pre - 1) / pp.max_pre);
+  // (as many turns of the CTAs as leave items of about four tiles, up to eight: shorter ones cost more than they balance)
+  const int turns = max(1, min(pp.max_own / pp.max_pre, own_tiles / (4 * pp.max_pre)));
+  l.own_len = max(1, (own_tiles + pp.max_pre * turns - 1) / (pp.max_pre * turns));
+  l.pre_items = (l.pre_tiles + l.pre_len - 1) / l.pre_len;
+  l.items = (l.pre_items + (own_tiles + l.own_len - 1) / l.own_len) * p.n_kv;
   if (blockIdx.x == 0) {               // for the kernel that joins the pieces
     for (int b = threadIdx.x; b < p.batch; b += kPuThreads) {
       int pre_f = 0;
@@ -274,10 +313,29 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         }
         pre_f = l.pre[lo] + (b - pu_group_start(p, lo)) / pp.per_tile * l.eff[lo];
       }
-      pp.plan[b] = PuSeqPlan{l.pre_tiles + l.own[b], l.own[b + 1] - l.own[b], pre_f, shared};
+      pp.plan[b] = PuSeqPlan{l.own[b], l.own[b + 1] - l.own[b], pre_f, shared};
     }
-    if (threadIdx.x == 0) *pp.plan_total = l.total;
+    if (threadIdx.x == 0) {
+      pp.plan_cut[0] = l.pre_len;
+      pp.plan_cut[1] = l.own_len;
+    }
   }
+  // One arrival for the warp.  The lanes meet before it and behind it: none may wait for what the arrival lets happen before it is made.
+  auto arrive = [&](uint64_t* bar) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+    __syncwarp();
+  };
+  // ---- items: warp 0 hands them on to the others (-1: there are no more)
+  int it = 0;
+  auto take = [&](bool& ok) {
+    const int slot = it & 3;
+    ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(&item_full[slot], (uint32_t)((it >> 2) & 1)));
+    const int item = __shfl_sync(0xffffffffu, ok ? item_s[slot] : -1, 0);
+    arrive(&item_empty[slot]);
+    ++it;
+    return item;
+  };
 
   if (warp == 0 || warp == 2) {
     // ---- copies: the keys of every tile (warp 0); the queries of every unit and the values of every tile (warp 2).  A lane per box: a page's rows, half
@@ -285,33 +343,58 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     const bool values = warp == 2;
     const int box_rows = min(1 << p.page_shift, kPfTile), boxes = kPfTile / box_rows, j = lane >> 1, c = lane & 1;
     uint32_t q_used = 0;               // phases of the query slots
+    int own_pieces = 0;
     bool ok = true;
     const int* table = nullptr;
-    auto table_of = [&](const PuUnit& w, int f) {
-      const int s = paged_row_of(p, w.pre ? pu_group_start(p, pu_last_not_above(l.pre, l.groups, f)) : w.b0);
-      return p.tables + (size_t)max(s, 0) * p.table_ld;
-    };
-    auto page_of = [&](const PuUnit& w) {
-      return j < boxes && j * box_rows < pu_keys(w) ? table[((w.shared_tiles + w.tile) * kPfTile + j * box_rows) >> p.page_shift] : 0;
-    };
-    PuUnit u, next;
-    int page = 0, page_next = 0;
-    if (n > 0) {
-      next = pu_locate(p, l, f0);
-      table = table_of(next, f0);
-      page_next = page_of(next);
-    }
-    for (int i = 0; i < n && ok; ++i) {
-      const bool fresh = i == 0 || u.tile == u.tiles - 1;
-      u = next;
-      page = page_next;
-      if (i + 1 < n) {
-        pu_step(p, l, next, f0 + i + 1);
-        if (next.tile == 0) table = table_of(next, f0 + i + 1);
-        page_next = page_of(next);
+    auto page_of = [&](const PuCursor& w, bool fresh) {
+      if (fresh) {
+        const int s = paged_row_of(p, w.u.pre ? pu_group_start(p, pu_last_not_above(l.pre, l.groups, w.f)) : w.u.b0);
+        table = p.tables + (size_t)max(s, 0) * p.table_ld;
       }
+      return j < boxes && j * box_rows < pu_keys(w.u) ? table[((w.u.shared_tiles + w.u.tile) * kPfTile + j * box_rows) >> p.page_shift] : 0;
+    };
+    // the items that come: the next one, and the one behind it, which is on its way
+    const int n_ctas = (int)gridDim.x;
+    int coming = (int)blockIdx.x, behind = (int)blockIdx.x + n_ctas;
+    auto next_item = [&]() {
+      if (values) return take(ok);
+      const int item = coming < l.items ? coming : -1, slot = it & 3;
+      coming = __shfl_sync(0xffffffffu, behind, 0);
+      if (coming < l.items && lane == 0) behind = 2 * n_ctas + atomicAdd(pp.counter, 1);
+      ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(&item_empty[slot], (uint32_t)((it >> 2) & 1) ^ 1u));
+      if (lane == 0) {
+        item_s[slot] = item;
+        mbar_arrive(&item_full[slot]);
+      }
+      __syncwarp();
+      ++it;
+      return ok ? item : -1;
+    };
+    PuCursor cur, next;
+    int page = 0, page_next = 0, item = next_item();
+    bool more = item >= 0, fresh_next = true;
+    if (more) {
+      pu_begin(p, l, next, item);
+      page_next = page_of(next, true);
+    }
+    for (int t = 0; more && ok; ++t) {
+      cur = next;
+      page = page_next;
+      const bool fresh = fresh_next;
+      if (next.f + 1 < next.end) {
+        pu_next(p, l, next);
+      } else {
+        item = next_item();
+        more = item >= 0;
+        if (more) pu_begin(p, l, next, item);
+      }
+      if (more) {
+        fresh_next = next.piece == next.f;
+        page_next = page_of(next, fresh_next);
+      }
+      const PuUnit& u = cur.u;
       if (values && fresh) {
-        const int slot = u.q_slot;
+        const int slot = u.pre ? 0 : own_pieces++ & 3;
         for (int k = 0; k < 4; ++k)
           if (ok && (u.pre || k == slot)) {
             ok = mbar_wait_spin(&q_empty[k], ((q_used >> k) & 1u) ^ 1u);
@@ -322,53 +405,55 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         const uint32_t rows = (uint32_t)((whole ? pp.per_tile : u.pre ? pp.per_quarter : 1) * p.group);
         if (lane == 0) mbar_arrive_expect_tx(&q_full[slot], 2u * rows * 128u);
         __syncwarp();
-        if (lane < 2) tma_load_3d(q_s + c * kPfBox + 16 * slot * 128, whole ? &q_whole : u.pre ? &q_quarter : &q_own, 64 * c, kvh * p.group, u.b0, &q_full[slot]);
+        if (lane < 2) tma_load_3d(q_s + c * kPfBox + 16 * slot * 128, whole ? &q_whole : u.pre ? &q_quarter : &q_own, 64 * c, cur.kv * p.group, u.b0, &q_full[slot]);
         __syncwarp();
       }
-      const int keys = pu_keys(u), used = (keys + box_rows - 1) / box_rows, r = 2 * i + (values ? 1 : 0), slot = r % kPuRing;
+      const int keys = pu_keys(u), used = (keys + box_rows - 1) / box_rows, r = values ? pu_values_at(t) : pu_keys_at(t), slot = r % kPuRing;
       if (j < used && (page < 0 || page >= p.n_pages)) {
         give_up(DERR_POSITION);
         page = 0;
       }
       const int row = (page << p.page_shift) + (((u.shared_tiles + u.tile) * kPfTile) & ((1 << p.page_shift) - 1) & ~(box_rows - 1));
-      ok = mbar_wait_spin(&kv_empty[slot], (uint32_t)((r / kPuRing) & 1) ^ 1u);
+      ok = ok && mbar_wait_spin(&kv_empty[slot], (uint32_t)((r / kPuRing) & 1) ^ 1u);
       if (!ok) break;
       uint64_t* bar = values && (keys & 15) ? &v_raw[slot] : &kv_full[slot];
       if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(used * box_rows) * 256u);
       __syncwarp();
-      if (j < used) tma_load_2d(kv_s + slot * kPuTile + c * kPfBox + j * box_rows * 128, values ? &v_map : &k_map, kvh * kPaDim + 64 * c, row, bar);
+      if (j < used) tma_load_2d(kv_s + slot * kPuTile + c * kPfBox + j * box_rows * 128, values ? &v_map : &k_map, cur.kv * kPaDim + 64 * c, row, bar);
       __syncwarp();
     }
     if (!ok) give_up(DERR_EMPTY_WAIT);
   } else if (warp == 3) {
     // ---- value rows between the last key and the next multiple of 16: whatever the cache holds there must not meet a weight of zero
-    PuUnit u;
     uint32_t used = 0;                 // phases of v_raw
     bool ok = true;
-    for (int i = 0; i < n && ok;) {
-      if (i == 0) {
-        u = pu_locate(p, l, f0);
-      } else {
-        u.tile = u.tiles - 1;
-        pu_step(p, l, u, f0 + i);
-      }
-      const int end = i + u.tiles - u.tile;           // behind the unit's last tile
-      if (end <= n && (u.last & 15)) {
-        const int r = 2 * (end - 1) + 1, slot = r % kPuRing;
-        ok = mbar_wait_spin(&v_raw[slot], (used >> slot) & 1u);
-        used ^= 1u << slot;
-        if (!ok) break;
-        uint8_t* at = kv_s + slot * kPuTile;
-        const int rows = 16 - (u.last & 15);
-        for (int k = lane; k < 2 * rows * 8; k += 32) {               // (a row's 128 bytes of either box, whatever their order)
-          const int box = (k >> 3) & 1, row = u.last + (k >> 4);
-          *reinterpret_cast<uint4*>(at + box * kPfBox + row * 128 + 16 * (k & 7)) = make_uint4(0u, 0u, 0u, 0u);
+    int t = 0;                         // tiles before the piece
+    for (int item = take(ok); item >= 0 && ok; item = take(ok)) {
+      PuCursor c;
+      pu_begin(p, l, c, item);
+      while (ok) {
+        const int end = pu_piece_end(c);
+        t += end - c.f;
+        const PuUnit& u = c.u;
+        if (u.tile + end - c.f == u.tiles && (u.last & 15)) {
+          const int slot = pu_values_at(t - 1) % kPuRing;
+          ok = mbar_wait_spin(&v_raw[slot], (used >> slot) & 1u);
+          used ^= 1u << slot;
+          if (!ok) break;
+          uint8_t* at = kv_s + slot * kPuTile;
+          const int rows = 16 - (u.last & 15);
+          for (int k = lane; k < 2 * rows * 8; k += 32) {             // (a row's 128 bytes of either box, whatever their order)
+            const int box = (k >> 3) & 1, row = u.last + (k >> 4);
+            *reinterpret_cast<uint4*>(at + box * kPfBox + row * 128 + 16 * (k & 7)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          arrive(&kv_full[slot]);
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&kv_full[slot]);
+        if (end == c.end) break;
+        c.u.tile += end - 1 - c.f;
+        c.f = end - 1;
+        pu_next(p, l, c);
       }
-      i = end;
     }
     if (!ok) give_up(DERR_EMPTY_WAIT);
     __syncwarp();
@@ -380,30 +465,31 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     uint32_t q_seen = 0;
     int made[2] = {0, 0}, freed[2] = {0, 0};          // tiles of a parity so far, results read
     bool ok = true;
-    PuUnit u, before;
-    bool fresh[2] = {true, true}, before_fresh = false;                // the parity's next tile is its first of the unit
-    auto values = [&](int i, const PuUnit& w, bool first) {
-      const int x = (f0 + i) & 1, r = 2 * i + 1, slot = r % kPuRing;
+    struct Tile {
+      int steps, wide;                                // 16-key steps, layout
+      bool first;                                     // of its parity in the piece
+    };
+    auto values = [&](int t, const Tile& w) {
+      const int x = t & 1, r = pu_values_at(t), slot = r % kPuRing;
       const uint32_t s_t = tmem + (uint32_t)(x * 256), o_t = s_t + 128u;
       bool good = mbar_wait_spin(&kv_full[slot], (uint32_t)((r / kPuRing) & 1)) && mbar_wait_spin(&p_full[x], (uint32_t)(made[x] & 1));
       ++made[x];
-      if (good && first) {
+      if (good && w.first) {
         good = freed[x] == 0 || mbar_wait_spin(&o_free[x], (uint32_t)((freed[x] - 1) & 1));
         ++freed[x];
       }
       if (!good) return false;
       tc_fence_after();
       if (leader) {
-        const int steps = (pu_keys(w) + 15) >> 4, wide = pu_wide<TERMS>(w);
         const uint64_t at = vd + (uint64_t)(slot * (kPuTile >> 4));
-        if (wide) {
-          const uint32_t idesc = umma_idesc_bf16(wide == 8 ? 16 : 32) | (1u << 15);
-          for (int k = 0; k < steps; ++k)
-            umma_f16(o_t, at + (uint64_t)(k * (2048 >> 4)), wd + (uint64_t)(x * (kPuWeights >> 4) + (k >> 2) * (kPuWeights >> 5) + 2 * (k & 3)), idesc, !first || k != 0);
+        if (w.wide) {
+          const uint32_t idesc = umma_idesc_bf16(w.wide == 8 ? 16 : 32) | (1u << 15);
+          for (int k = 0; k < w.steps; ++k)
+            umma_f16(o_t, at + (uint64_t)(k * (2048 >> 4)), wd + (uint64_t)(x * (kPuWeights >> 4) + (k >> 2) * (kPuWeights >> 5) + 2 * (k & 3)), idesc, !w.first || k != 0);
         } else {
-          for (int k = 0; k < steps; ++k) umma_f16_ts(o_t, s_t + 8u * k, at + (uint64_t)(k * (2048 >> 4)), idesc_o, !first || k != 0);
+          for (int k = 0; k < w.steps; ++k) umma_f16_ts(o_t, s_t + 8u * k, at + (uint64_t)(k * (2048 >> 4)), idesc_o, !w.first || k != 0);
           if (TERMS == 2)
-            for (int k = 0; k < steps; ++k) umma_f16_ts(o_t, s_t + 64u + 8u * k, at + (uint64_t)(k * (2048 >> 4)), idesc_o, 1u);
+            for (int k = 0; k < w.steps; ++k) umma_f16_ts(o_t, s_t + 64u + 8u * k, at + (uint64_t)(k * (2048 >> 4)), idesc_o, 1u);
         }
         umma_commit(&o_done[x]);
         umma_commit(&kv_empty[slot]);
@@ -411,25 +497,32 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
       __syncwarp();
       return true;
     };
-    for (int i = 0; i < n && ok; ++i) {
-      const int x = (f0 + i) & 1, r = 2 * i, slot = r % kPuRing;
-      if (i == 0) u = pu_locate(p, l, f0);
-      else pu_step(p, l, u, f0 + i);
-      if (i == 0 || u.tile == 0) {
+    PuCursor c;
+    Tile before{};
+    bool fresh[2] = {true, true};
+    int own_pieces = 0, q_slot = 0, t = 0, item = take(ok);
+    if (item >= 0) pu_begin(p, l, c, item);
+    while (item >= 0 && ok) {
+      const int x = t & 1, r = pu_keys_at(t), slot = r % kPuRing;
+      const PuUnit& u = c.u;
+      if (c.f == c.piece) {
         fresh[0] = fresh[1] = true;
-        ok = mbar_wait_spin(&q_full[u.q_slot], (q_seen >> u.q_slot) & 1u);
-        q_seen ^= 1u << u.q_slot;
+        q_slot = u.pre ? 0 : own_pieces++ & 3;
+        ok = mbar_wait_spin(&q_full[q_slot], (q_seen >> q_slot) & 1u);
+        q_seen ^= 1u << q_slot;
       }
       // (the scores' columns hold the weights of the parity's tile before until its products are done)
       ok = ok && mbar_wait_spin(&kv_full[slot], (uint32_t)((r / kPuRing) & 1)) && (made[x] == 0 || mbar_wait_spin(&o_done[x], (uint32_t)((made[x] - 1) & 1)));
       if (!ok) break;
       tc_fence_after();
+      const int keys = pu_keys(u);
+      const Tile now{(keys + 15) >> 4, pu_wide<TERMS>(u), fresh[x]};
+      fresh[x] = false;
       if (leader) {
         const uint32_t s_t = tmem + (uint32_t)(x * 256);
-        const int wide = pu_wide<TERMS>(u);
-        const uint32_t idesc = umma_idesc_bf16(wide ? (wide == 32 ? 32 : 16) : kPfTile);
-        const uint64_t keys = kd + (uint64_t)(slot * (kPuTile >> 4)), queries = qd + (uint64_t)(u.q_slot * (16 * 128 >> 4));
-        const uint64_t da = wide ? keys : queries, db = wide ? queries : keys;
+        const uint32_t idesc = umma_idesc_bf16(now.wide ? (now.wide == 32 ? 32 : 16) : kPfTile);
+        const uint64_t kt = kd + (uint64_t)(slot * (kPuTile >> 4)), qt = qd + (uint64_t)(q_slot * (16 * 128 >> 4));
+        const uint64_t da = now.wide ? kt : qt, db = now.wide ? qt : kt;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint64_t off = (uint64_t)((k >> 2) * (kPfBox >> 4) + 2 * (k & 3));
@@ -437,18 +530,22 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         }
         umma_commit(&s_full[x]);
         umma_commit(&kv_empty[slot]);
-        if (i == n - 1 || u.tile == u.tiles - 1)
-          for (int j = 0; j < 4; ++j)
-            if (u.pre || j == u.q_slot) umma_commit(&q_empty[j]);
+        if (c.f + 1 == pu_piece_end(c))
+          for (int k = 0; k < 4; ++k)
+            if (u.pre || k == q_slot) umma_commit(&q_empty[k]);
       }
       __syncwarp();
-      const bool first = fresh[x];
-      fresh[x] = false;
-      if (i > 0) ok = values(i - 1, before, before_fresh);
-      before = u;
-      before_fresh = first;
+      if (t > 0) ok = values(t - 1, before);
+      before = now;
+      ++t;
+      if (c.f + 1 < c.end) {
+        pu_next(p, l, c);
+      } else {
+        item = take(ok);
+        if (item >= 0) pu_begin(p, l, c, item);
+      }
     }
-    if (ok && n > 0) ok = values(n - 1, before, before_fresh);
+    if (ok && t > 0) ok = values(t - 1, before);
     if (!ok) give_up(DERR_FULL_WAIT);
   } else if (warp >= 4) {
     // ---- softmax of the tiles of a parity.  More than 32 rows: S = Q K^T, a thread per row, the weights over the scores' columns.  Up to 32: the keys are
@@ -459,17 +556,23 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     const int x = (warp - 4) >> 2, q4 = warp & 3;
     const uint32_t s_t = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)(x * 256), o_t = s_t + 128u;
     float *max_s = meet_s + x * 256, *sum_s = max_s + 128;             // [warp][32 rows]
-    auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory"); };
-    float ref[16], sums[32], largest = 0.f;            // (32 rows: the references stay in max_s)
+    int meetings = 0;
     bool ok = true, first = true;
+    auto meet = [&]() {                // (a barrier of the group whose wait ends, as every other's)
+      arrive(&met[x]);
+      ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(&met[x], (uint32_t)(meetings++ & 1)));
+    };
+    float ref[16], sums[32], largest = 0.f;            // (32 rows: the references stay in max_s)
     int done = 0;                      // tiles of this parity
-    PuUnit u;
-    int unit_end = 0;                  // the tile behind the unit's last, or the CTA's
+    PuCursor cur;
+    const PuUnit& u = cur.u;
+    int place = 0;                     // the group's first tile of the piece is the piece's first or second: its partial result's place
     // a tile whose lanes are keys
     auto keyed = [&](auto rows_c) {
       constexpr int NR = decltype(rows_c)::value;
       constexpr bool kTwo = NR < 32;
       float v[NR];
+      __syncwarp();
       if constexpr (NR == 8) tmem_ld8(s_t, v);
       else if constexpr (NR == 16) tmem_ld16(s_t, v);
       else pf_ld32(s_t, v);
@@ -522,6 +625,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
       constexpr int NR = decltype(rows_c)::value;
       constexpr bool kTwo = NR < 32;
       float o[32];
+      __syncwarp();
       if constexpr (NR == 8) {
         float w[16];
         tmem_ld16(o_t, w);
@@ -534,8 +638,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
           for (int r = 0; r < NR; ++r) o[r] += o[NR + r];
       }
       tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&o_free[x]);          // (the next unit's products may begin)
+      arrive(&o_free[x]);                              // (the next unit's products may begin)
       float mine = 0.f;
 #pragma unroll
       for (int r = 0; r < NR; ++r)
@@ -556,15 +659,27 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     using R8 = std::integral_constant<int, 8>;
     using R16 = std::integral_constant<int, 16>;
     using R32 = std::integral_constant<int, 32>;
-    for (int i = 0; i < n && ok; ++i) {
-      if (i == 0) u = pu_locate(p, l, f0);
-      else pu_step(p, l, u, f0 + i);
-      if (i == 0 || u.tile == 0) {
-        unit_end = min(n, i + u.tiles - u.tile);
-        first = true;
+    int item = take(ok);
+    if (item >= 0) pu_begin(p, l, cur, item);
+    bool begun = false;                // the group has had a tile of the piece
+    for (int t = 0; item >= 0 && ok; ++t) {
+      if (t > 0) {
+        if (cur.f + 1 < cur.end) {
+          pu_next(p, l, cur);
+        } else {
+          item = take(ok);
+          if (item < 0) break;
+          pu_begin(p, l, cur, item);
+        }
+      }
+      if (cur.f == cur.piece) begun = false;
+      if ((t & 1) != x) continue;
+      first = !begun;
+      if (first) {
+        begun = true;
+        place = (cur.f - cur.piece) & 1;
         largest = 0.f;
       }
-      if (((f0 + i) & 1) != x) continue;
       const int wide = pu_wide<TERMS>(u), r = 32 * q4 + lane;
       const bool live = r < u.rows;
       ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[x], (uint32_t)(done & 1)));
@@ -577,6 +692,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
       } else if (TERMS == 1 && wide == 32) {
         keyed(R32());
       } else {
+        __syncwarp();
         if (first) {
           float mx = -FLT_MAX;
 #pragma unroll
@@ -589,6 +705,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
           ref[0] = mx == -FLT_MAX ? mx : mx * p.scale_log2;
           sums[0] = 0.f;
         }
+        __syncwarp();
         uint32_t low[TERMS == 2 ? 64 : 1];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -618,19 +735,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         tmem_st_wait();
         tc_fence_before();
       }
-      first = false;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[x]);
+      arrive(&p_full[x]);
       ++done;
-      if (i + 2 < unit_end) continue;
+      if (cur.f + 2 < pu_piece_end(cur)) continue;
 
       // ---- the piece's result
       ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[x], (uint32_t)((done - 1) & 1)));
       if (!ok) break;
       tc_fence_after();
       const int apart = u.pre ? 128 : 8;
-      const size_t row0 = (size_t)kvh * (p.batch * p.group + apart * pp.per_head) + u.slot + apart * part;
-      float *to_o = (u.pre ? pp.pre_o : pp.own_o) + (row0 * 2 + x) * kPaDim, *to_ml = (u.pre ? pp.pre_ml : pp.own_ml) + (row0 * 2 + x) * 2;
+      const size_t row0 = (size_t)cur.kv * (p.batch * p.group + apart * (u.pre ? pp.max_pre : pp.max_own)) + u.slot + apart * cur.item;
+      float *to_o = (u.pre ? pp.pre_o : pp.own_o) + (row0 * 2 + place) * kPaDim, *to_ml = (u.pre ? pp.pre_ml : pp.own_ml) + (row0 * 2 + place) * 2;
       if (wide == 8) {
         keyed_out(R8(), to_o, to_ml);
       } else if (wide == 16) {
@@ -641,6 +756,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
 #pragma unroll 1
         for (int c = 0; c < kPaDim; c += 32) {
           float o[32];
+          __syncwarp();
           pf_ld32(o_t + (uint32_t)c, o);
           float4* o_row = reinterpret_cast<float4*>(to_o + (size_t)r * 2 * kPaDim + c);
           if (live)
@@ -648,8 +764,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
             for (int j = 0; j < 8; ++j) o_row[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
         }
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&o_free[x]);
+        arrive(&o_free[x]);
         if (live)
           *reinterpret_cast<float2*>(to_ml + r * 4) = make_float2(ref[0], largest > kPuLargest ? NAN : sums[0]);
       }
@@ -658,6 +773,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   }
   tc_fence_before();
   __syncthreads();
+  __syncwarp();                        // (the release is one instruction of the whole warp)
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
@@ -666,32 +782,33 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
   pdl_wait();
   pdl_launch_dependents();
   const PagedParams& p = pp.a;
-  const int b = blockIdx.x, lane = threadIdx.x & 31, J = pp.per_head;
+  const int b = blockIdx.x, lane = threadIdx.x & 31;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *pp.counter = 0;
   const PuSeqPlan q = pp.plan[b];
-  const int total = *pp.plan_total;
+  const int cut[2] = {pp.plan_cut[1], pp.plan_cut[0]};
   const int head = (int)(blockIdx.y * 4 + (threadIdx.x >> 5));
   if (head < p.n_heads) {
     const int kv = head / p.group, h = head - kv * p.group;
-    // tiles of the list, first CTA and number of (CTA, parity) places of the own and of the shared part
-    const int f[2] = {q.own_f, q.pre_f}, e[2] = {q.own_f + q.own_tiles, q.pre_f + q.pre_tiles}, wide[2] = {8, 128};
+    // tiles of the own and of the shared part, first item and number of (item, place)s
+    const int f[2] = {q.own_f, q.pre_f}, e[2] = {q.own_f + q.own_tiles, q.pre_f + q.pre_tiles}, apart[2] = {8, 128}, most[2] = {pp.max_own, pp.max_pre};
     int c[2] = {0, 0}, places[2] = {0, 0};
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       if (e[k] > f[k]) {
-        c[k] = (int)(((long long)(f[k] + 1) * J - 1) / total);
-        places[k] = 2 * ((int)(((long long)e[k] * J - 1) / total) - c[k] + 1);
+        c[k] = f[k] / cut[k];
+        places[k] = 2 * ((e[k] - 1) / cut[k] - c[k] + 1);
       }
     const int all = places[0] + places[1];
     float top = -FLT_MAX, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
     for (int base = 0; base < all; base += 32) {
-      // a lane per place: its row of the partial results (none where the CTA has no tile of the parity), maximum and sum
+      // a lane per place: its row of the partial results (the second one of a piece of one tile is none), maximum and sum
       const int i = base + lane;
       const float *row = nullptr, *ml = nullptr;
       if (i < all) {
-        const int k = i >= places[0], j = k ? i - places[0] : i, cta = c[k] + (j >> 1), x = j & 1;
-        const int lo = max(f[k], (int)((long long)total * cta / J)), hi = min(e[k], (int)((long long)total * (cta + 1) / J));
-        if (hi - lo > 1 || (hi - lo == 1 && (lo & 1) == x)) {
-          const size_t r = ((size_t)kv * (p.batch * p.group + wide[k] * J) + b * p.group + h + (size_t)wide[k] * cta) * 2 + x;
+        const int k = i >= places[0], j = k ? i - places[0] : i, item = c[k] + (j >> 1), x = j & 1;
+        const int lo = max(f[k], item * cut[k]), hi = min(e[k], (item + 1) * cut[k]);
+        if (hi - lo > x) {
+          const size_t r = ((size_t)kv * (p.batch * p.group + apart[k] * most[k]) + b * p.group + h + (size_t)apart[k] * item) * 2 + x;
           row = (k ? pp.pre_o : pp.own_o) + r * kPaDim;
           ml = (k ? pp.pre_ml : pp.own_ml) + r * 2;
         }
@@ -781,7 +898,7 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   p.group_starts = group_starts_dev;
   p.shared = shared_dev;
   p.batch = (int)batch;
-  p.n_groups = (int)n_groups;
+  p.n_groups = group_starts_dev ? (int)n_groups : 0;
   p.max_len = (int)(max_len < most ? max_len : most);
   p.max_shared = (int)(max_shared < (size_t)p.max_len ? max_shared : (size_t)p.max_len);
   p.n_pages = pages->n_pages;
@@ -800,12 +917,13 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   pp.per_quarter = 32 / p.group;
   const size_t tiles = batch * (((size_t)p.max_len + kPfTile - 1) / kPfTile) * n_kv_heads;
   TQ_REQUIRE(ctx, tiles < (1ull << 30) && (size_t)p.n_pages * pages->page_rows < (1ull << 31), "tq_gqa_decode_paged: too many positions");
-  // as many CTAs for every KV head, one an SM
-  const size_t per_kv = tiles / n_kv_heads, fit = (size_t)ctx->sm_count / n_kv_heads;
-  pp.per_head = (int)(per_kv < fit ? per_kv : fit < 1 ? 1 : fit);
-  const size_t n_ctas = n_kv_heads * (size_t)pp.per_head;
+  const size_t n_ctas = tiles < (size_t)ctx->sm_count ? tiles : (size_t)ctx->sm_count;
+  // A CTA takes one item of shared tiles (whose partial results are many rows) and eight of the others, if there are as many tiles.
+  const size_t per_kv = ((size_t)ctx->sm_count + n_kv_heads - 1) / n_kv_heads;
+  pp.max_pre = (int)per_kv;
+  pp.max_own = (int)(8 * per_kv);
   // partial results, the sequences' plans
-  const size_t own_rows = (batch * n_heads + 8 * n_ctas) * 2, pre_rows = p.n_groups ? (batch * n_heads + 128 * n_ctas) * 2 : 0;
+  const size_t own_rows = (batch * n_heads + 8 * n_kv_heads * pp.max_own) * 2, pre_rows = p.n_groups ? (batch * n_heads + 128 * n_kv_heads * pp.max_pre) * 2 : 0;
   const size_t floats = (own_rows + pre_rows) * (kPaDim + 2);
   if (int st = ensure_scratch(ctx, floats * sizeof(float) + (batch + 1) * sizeof(PuSeqPlan))) return st;
   pp.own_o = static_cast<float*>(ctx->scratch);
@@ -813,7 +931,8 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   pp.own_ml = pp.pre_o + pre_rows * kPaDim;
   pp.pre_ml = pp.own_ml + own_rows * 2;
   pp.plan = reinterpret_cast<PuSeqPlan*>(pp.pre_ml + pre_rows * 2);
-  pp.plan_total = reinterpret_cast<int*>(pp.plan + batch);
+  pp.plan_cut = reinterpret_cast<int*>(pp.plan + batch);
+  pp.counter = ctx->dev_err + kTileCounters;          // (the last of the counters)
   pp.a = p;
   CUtensorMap qo, qq, qw, km, vm;
   const size_t row = n_kv_heads * kPaDim, rows = (size_t)p.n_pages * pages->page_rows;
