@@ -184,6 +184,28 @@ def test_sharp_and_flat_scores(dev):
         assert (np.abs(got.reshape(want.shape) - want) <= (2.0 ** -14 + std * 40 * 2.0 ** -20) * size + 1e-30).all()
 
 
+@pytest.mark.parametrize("group", [4, 1])
+def test_scores_that_leave_their_reference_far_behind(dev, group):
+    """Scores that grow along the sequence by more than an f32 exponent: the last keys have all the weight."""
+    s = Setup(8, 8 // group, 16, [(256, [700, 400] + [300] * 40), (0, [500])], seed=21)
+    for b in range(s.B):
+        n = int(s.lens[b])
+        for j in range(n):
+            page, r = s.tables[b, j // 16], j % 16
+            bits, f = bf16_round(np.full((8 // group, HD), (j // 64) * 4.0 + (j % 64) / 64, np.float32))
+            s.kv_bits[0, page, r], s.kv[0, page, r] = bits.reshape(f.shape), f
+    s.q_bits, s.q = bf16_round(np.full(s.q.shape, 1.5, np.float32))
+    s.q_bits, s.q = s.q_bits.reshape(s.B, 8, HD), s.q.reshape(s.B, 8, HD)
+    s.put(dev)
+    for f32 in (False, True):
+        got = s.run(f32).to_vec()
+        dev.sync()
+        # scores up to 45 * 1.5 * 128 / sqrt(128): off by 2^-23 of that per step of 16, 2^-10 in all
+        want, size = s.reference()
+        g = got.astype(np.float64) if f32 else (got.astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+        assert (np.abs(g.reshape(want.shape) - want) <= (2.0 ** -10 + (0 if f32 else 2.0 ** -8)) * size + 1e-30).all()
+
+
 def test_max_len_cuts_and_rows_behind_the_batch_stay(dev):
     import tang_b200 as tb
 
@@ -233,6 +255,17 @@ def test_pages_and_sequences_that_do_not_exist_are_reported(dev):
         assert e.value.status == tb._lib.TQ_EINVAL
         dev.sync()
         s.check(got, True, rows=slice(2, 3))                  # the sequence whose pages exist
+    s = Setup(8, 2, 16, [(256, [300, 290]), (128, [177, 150, 140])], seed=16).put(dev)
+    for starts in ([1, 2], [0, -1], [0, 6], [3, 2]):          # starts that do not ascend from 0: reported, and nothing is shared
+        dev.upload_into(s.gb, np.array(starts + [0], np.int32))
+        got = s.run(True).to_vec()
+        with pytest.raises(tb.TangqError):
+            dev.sync()
+        s.check(got, True)
+    dev.upload_into(s.gb, s.starts)
+    got = s.run(True).to_vec()
+    dev.sync()
+    s.check(got, True)
     s = Setup(8, 2, 16, [(0, [77]), (0, [20])], seed=11).put(dev, [3, 1])
     dev.upload_into(s.seqs, np.array([3, 99], np.int32))
     got = s.run(True).to_vec()
