@@ -49,7 +49,7 @@ constexpr float kPuLargest = 7.9228162514264338e28f;  // 2^96: a weight above it
 constexpr int kPuHeader = 640;                        // barriers, pieces
 constexpr int kPuReaders = 12;                        // warps that are told the pieces
 constexpr int kPuPieces = 4;                          // pieces that are told ahead
-constexpr int kPuLong = 6, kPuShort = 8;              // a CTA's items of own tiles: long ones, then short ones for the last quarter
+constexpr int kPuLong = 3, kPuShort = 8;              // a CTA's items of own tiles: long ones, then short ones for the last quarter
 constexpr int kPuBatch = 1024;                        // sequences of a call
 constexpr size_t kPuFixed = 2 * (size_t)kPfBox + kPuRing * (size_t)kPuTile + 2 * (size_t)kPuWeights + kPuOnes + kPuMeet + kPuHeader;
 
@@ -155,6 +155,11 @@ __device__ __forceinline__ void pu_scan(int* a, int n, int lane) {      // a[0 .
   if (lane == 0) a[n] = sum;
 }
 
+__device__ __forceinline__ float redux_max(float v) {                  // of the warp's values; NaN is none of them
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
 __device__ __forceinline__ void st_global8(float* to, const float* v) {
   asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
                : "memory");
@@ -568,7 +573,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
           tmem_ld8(s_t + 8u * i, v);
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
-            const float mx = warp_max(seen ? v[r] : -FLT_MAX);
+            const float mx = redux_max(seen ? v[r] : -FLT_MAX);
             if (lane == 8 * i + r) mine = mx;
           }
         }
@@ -587,15 +592,22 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         tmem_ld8(s_t + 8u * i, v);
         const float4 f0 = *reinterpret_cast<const float4*>(&ref_s[8 * i]), f1 = *reinterpret_cast<const float4*>(&ref_s[8 * i + 4]);
         const float from[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+        // (rows behind the last one have columns and places too, which nobody reads: without branches the eight go side by side)
+        float w[8];
+        __nv_bfloat16 hi[8];
+        uint8_t* row = at + i * 1024;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          if (8 * i + r >= u.rows) break;
-          float w = seen ? ex2(fmaf(v[r], p.scale_log2, -from[r])) : 0.f;
-          if (w > kPuLargest) w = NAN;
-          const __nv_bfloat16 hi = __float2bfloat16_rn(w);
-          uint8_t* to = at + (8 * i + r) * 128 + ((chunk ^ r) << 4);
-          *reinterpret_cast<__nv_bfloat16*>(to) = hi;
-          if (wide < 32) *reinterpret_cast<__nv_bfloat16*>(to + wide * 128) = __float2bfloat16_rn(w - __bfloat162float(hi));
+          const float e = ex2(fmaf(v[r], p.scale_log2, -from[r]));
+          w[r] = !seen ? 0.f : e > kPuLargest ? NAN : e;
+          hi[r] = __float2bfloat16_rn(w[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) *reinterpret_cast<__nv_bfloat16*>(row + r * 128 + ((chunk ^ r) << 4)) = hi[r];
+        if (wide < 32) {
+          row += wide * 128;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) *reinterpret_cast<__nv_bfloat16*>(row + r * 128 + ((chunk ^ r) << 4)) = __float2bfloat16_rn(w[r] - __bfloat162float(hi[r]));
         }
       }
       tc_fence_before();
@@ -619,10 +631,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         }
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          if (8 * i + r >= u.rows) break;
-          to_o[(size_t)(8 * i + r) * 2 * kPaDim + t128] = o[r];
-          if (t128 == r) *reinterpret_cast<float2*>(to_ml + (8 * i + r) * 4) = make_float2(ref_s[8 * i + r], l8[r]);
+          if (8 * i + r < u.rows) to_o[(size_t)(8 * i + r) * 2 * kPaDim + t128] = o[r];
         }
+        float sum = l8[0];
+#pragma unroll
+        for (int r = 1; r < 8; ++r) sum = lane == r ? l8[r] : sum;
+        if (q4 == 0 && lane < 8 && 8 * i + lane < u.rows) *reinterpret_cast<float2*>(to_ml + (8 * i + lane) * 4) = make_float2(ref_s[8 * i + lane], sum);
       }
       tc_fence_before();
       arrive(&o_free[x]);                              // (the next piece's products may begin)
@@ -757,7 +771,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
       const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)row, 4 * k + warp));
       v[k] = from ? *reinterpret_cast<const float4*>(from + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const float to = fmaxf(top, warp_max(mine.x)), f0 = ex2(top - to), w = ex2(mine.x - to);
+    const float to = fmaxf(top, redux_max(mine.x)), f0 = ex2(top - to), w = ex2(mine.x - to);
     top = to;
     l = l * f0 + warp_sum(mine.y * w);
 #pragma unroll
