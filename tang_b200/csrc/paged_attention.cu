@@ -364,19 +364,20 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     if (!ok) give_up(DERR_EMPTY_WAIT);
   } else if (warp == 0 || warp == 2) {
     // ---- copies: the keys of every tile (warp 0); the queries of every piece and the values of every tile (warp 2).  A lane per box: a page's rows, half
-    // their columns.  The page of the next tile is asked for before the wait of this one.
+    // their columns.  The warp holds the pages of the next 32 boxes' rows (four tiles or more), and has asked for those behind them.
     const bool values = warp == 2;
     const int box_rows = min(1 << p.page_shift, kPfTile), boxes = kPfTile / box_rows, j = lane >> 1, c = lane & 1;
     uint32_t q_used = 0;               // phases of the query slots
     int own_pieces = 0;
     bool ok = true;
-    auto page_of = [&](const PuPiece& w, int i) {
-      const int keys = i == w.n - 1 ? w.last : kPfTile;
-      return j < boxes && j * box_rows < keys ? p.tables[(size_t)w.seq * p.table_ld + (((w.tile + i) * kPfTile + j * box_rows) >> p.page_shift)] : 0;
+    const int tiles_ahead = 32 / boxes;
+    auto pages_from = [&](const PuPiece& w, int i0) {
+      const int i = i0 + lane / boxes, row = lane % boxes * box_rows;
+      return i < w.n && row < (i == w.n - 1 ? w.last : kPfTile) ? p.tables[(size_t)w.seq * p.table_ld + (((w.tile + i) * kPfTile + row) >> p.page_shift)] : 0;
     };
     PuPiece w, next;
     take(ok, next);
-    int page_next = next.n ? page_of(next, 0) : 0;
+    int pages = 0, ahead = next.n ? pages_from(next, 0) : 0;
     for (int t = 0; next.n && ok;) {
       w = next;
       if (values) {
@@ -395,13 +396,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         __syncwarp();
       }
       for (int i = 0; i < w.n && ok; ++i, ++t) {
-        int page = page_next;
-        if (i + 1 < w.n) {
-          page_next = page_of(w, i + 1);
-        } else {
-          take(ok, next);
-          page_next = next.n ? page_of(next, 0) : 0;
-        }
+        const int k = i % tiles_ahead;
+        if (k == 0) pages = ahead;
+        int page = __shfl_sync(0xffffffffu, pages, k * boxes + min(j, boxes - 1));
         const int keys = i == w.n - 1 ? w.last : kPfTile, used = (keys + box_rows - 1) / box_rows, r = values ? pu_values_at(t) : pu_keys_at(t), slot = r % kPuRing;
         if (j < used && (page < 0 || page >= p.n_pages)) {
           give_up(DERR_POSITION);
@@ -415,6 +412,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         __syncwarp();
         if (j < used) tma_load_2d(kv_s + slot * kPuTile + c * kPfBox + j * box_rows * 128, values ? &v_map : &k_map, w.kv * kPaDim + 64 * c, row, bar);
         __syncwarp();
+        if (k == 0) {
+          if (i + tiles_ahead < w.n) {
+            ahead = pages_from(w, i + tiles_ahead);
+          } else {
+            take(ok, next);
+            ahead = next.n ? pages_from(next, 0) : 0;
+          }
+        }
       }
     }
     if (!ok) give_up(DERR_EMPTY_WAIT);
