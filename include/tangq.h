@@ -392,6 +392,12 @@ TQ_API int tq_llama_decode(tq_llama* model, const int* token_ids_dev, const int*
  * tq_llama_decode. */
 TQ_API int tq_llama_decode_at(tq_llama* model, const int* token_ids_dev, const int* positions_dev, const int* rope_positions_dev,
                               size_t batch, size_t max_len, float* logits_dev);
+/* The same step over a pool whose pages are rows of the model's caches (at most max_batch*max_seq rows of every layer: page p's are rows
+ * p*page_rows .. of the cache seen as one, so that sequence b's own rows are the pages from b*max_seq/page_rows on).  tq_pages_extend has made
+ * room for the new tokens: each is its sequence's last position, below max_len.  Sequences and groups as in tq_gqa_decode_paged, batch at most max_batch. */
+TQ_API int tq_llama_decode_paged(tq_llama* model, const int* token_ids_dev, const tq_pages* pages, const int* seqs_dev_or_null, size_t batch,
+                                 const int* group_starts_dev_or_null, const int* shared_dev_or_null, size_t n_groups, size_t max_shared,
+                                 size_t max_len, float* logits_dev);
 /* The same step for a chunk of q_len new tokens per sequence (prompt processing): token_ids [batch][q_len],
  * sequence b's chunk starts at position cache_start[b] (its earlier positions are in the cache already).
  * Appends the chunk's K/V rows, runs causal attention over cache + chunk (tq_gqa_prefill) and the linear layers

@@ -93,6 +93,7 @@ PROTOTYPES = {
     "tq_llama_set_head": (_i, [_p, _p, _p, _p]),
     "tq_llama_kv_cache": (_i, [_p, _sz, _pp, _pp, C.POINTER(_sz)]),
     "tq_llama_decode_at": (_i, [_p, _p, _p, _p, _sz, _sz, _p]),
+    "tq_llama_decode_paged": (_i, [_p, _p, _p, _p, _sz, _p, _p, _sz, _sz, _sz, _p]),
     "tq_llama_kv_trim": (_i, [_p, _p, _sz, _sz]),
     "tq_llama_hidden": (_i, [_p, _pp]),
     "tq_llama_decode": (_i, [_p, _p, _p, _sz, _sz, _p]),

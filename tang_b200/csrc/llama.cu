@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "internal.h"
+#include "pages.h"
 #include "qlayout.cuh"
 
 struct tq_comm;
@@ -41,6 +42,25 @@ __global__ void lens_kernel(const int* positions, int* lens, int n, int max_seq)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i < n) lens[i] = min(max(positions[i] + 1, 0), max_seq);
+}
+
+// The same for a cache of pages, whose pool has counted the new tokens already: a sequence's new token is its last position, and goes to that
+// position's row of its page.  Whatever does not exist gives row -1, which the kernel that appends K/V reports.
+__global__ void paged_rows_kernel(const int* tables, const int* lens, const int* seqs, int n, int n_seqs, int table_ld, int n_pages, int page_rows,
+                                  int max_len, int* rows, int* positions) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int s = seqs ? seqs[i] : i;
+  int row = -1, pos = 0;
+  if (s >= 0 && s < n_seqs && lens[s] > 0 && lens[s] <= max_len) {
+    pos = lens[s] - 1;
+    const int page = tables[(size_t)s * table_ld + pos / page_rows];
+    if (page >= 0 && page < n_pages) row = page * page_rows + pos % page_rows;
+  }
+  rows[i] = row;
+  positions[i] = pos;
 }
 
 // KVCache::trim_to (crates/tang-infer/src/kv_cache.rs:138-149) for one layer's K and V caches: a sequence that
@@ -97,7 +117,7 @@ struct tq_llama {
   float* h_last = nullptr;   // which of h / h2 holds the residual stream after the last decode step
   float* ss = nullptr;       // [8][d_model / 16]: row sums of squares handed from a projection to the next pre-norm
   __nv_bfloat16 *xn = nullptr, *qb = nullptr, *attn = nullptr, *act = nullptr;
-  int* lens = nullptr;
+  int *lens = nullptr, *rope = nullptr;   // rope: positions of the new tokens where their rows are places in pages
   // prefill workspaces (rows = sequences x chunk length), grown on demand by tq_llama_prefill
   size_t pre_rows = 0;
   float *p_h = nullptr, *p_delta = nullptr, *p_qkv = nullptr, *p_gu = nullptr;
@@ -112,6 +132,15 @@ static int dev_alloc(tq_llama* m, void** p, size_t bytes) {
   m->owned.push_back(*p);
   return TQ_OK;
 }
+
+// How the sequences of a step over pages are told (tq_gqa_decode_paged).
+struct PagedStep {
+  const tq_pages* pages;
+  const int *seqs, *group_starts, *shared;
+  size_t n_groups, max_shared;
+};
+static int decode_step(tq_llama* m, const int* token_ids_dev, const int* positions_dev, const int* rope_positions_dev, const PagedStep* paged,
+                       size_t batch, size_t max_len, float* logits_dev);
 
 extern "C" {
 
@@ -202,6 +231,7 @@ int tq_llama_create(tq_ctx* ctx, const tq_llama_config* cfg, tq_comm* comm, tq_l
   A((void**)&m->attn, B * q_dim * 2);
   A((void**)&m->act, B * m->ffn_l * 2);
   A((void**)&m->lens, B * 4);
+  A((void**)&m->rope, B * 4);
   for (auto& L : m->layers) {
     A((void**)&L.k_cache, B * cfg->max_seq * kv_dim * 2);
     A((void**)&L.v_cache, B * cfg->max_seq * kv_dim * 2);
@@ -309,106 +339,28 @@ int tq_llama_decode_at(tq_llama* m, const int* token_ids_dev, const int* positio
   if (!m) return TQ_EINVAL;
   tq_ctx* ctx = m->ctx;
   if (int st = bind(ctx)) return st;
-  const tq_llama_config& c = m->cfg;
-  TQ_REQUIRE(ctx, batch > 0 && batch <= c.max_batch, "tq_llama_decode: batch must be 1..%u", c.max_batch);
+  TQ_REQUIRE(ctx, batch > 0 && batch <= m->cfg.max_batch, "tq_llama_decode: batch must be 1..%u", m->cfg.max_batch);
   TQ_REQUIRE(ctx, token_ids_dev && positions_dev && logits_dev, "tq_llama_decode: null pointer");
-  TQ_REQUIRE(ctx, max_len > 0 && max_len <= c.max_seq, "tq_llama_decode: max_len must be 1..max_seq");
-  TQ_REQUIRE(ctx, m->lm_head != nullptr, "tq_llama_decode: head weights not set");
-  for (auto& L : m->layers) TQ_REQUIRE(ctx, L.wqkv != nullptr, "tq_llama_decode: a layer has no weights");
-  const int B = (int)batch;
-  const size_t d = c.d_model, hd = c.head_dim;
-  const size_t q_dim = (size_t)m->heads_l * hd, kv_dim = (size_t)m->kv_l * hd;
-  const size_t seq_stride = (size_t)c.max_seq * kv_dim;
-  int st;
-#define TQ_STEP(expr) \
-  if ((st = (expr)) != TQ_OK) return st;
+  return decode_step(m, token_ids_dev, positions_dev, rope_positions_dev, nullptr, batch, max_len, logits_dev);
+}
 
-  TQ_CUDA(ctx, launch_k(ctx, lens_kernel, dim3((B + 63) / 64), dim3(64), 0, positions_dev, m->lens, B, (int)c.max_seq));
-  TQ_STEP(tq_embedding(ctx, m->embed, TQ_BF16, token_ids_dev, B, d, c.vocab, m->h, TQ_F32));
-
-  // The residual stream alternates between two buffers, and every pre-norm is fused into the projection that follows
-  // it; with a gate/up weight in the interleaved row order the SwiGLU is that projection's epilogue.  Per layer: qkv
-  // (+norm), RoPE/append, attention, merge, o, gate/up (+norm, +SwiGLU), down.  Batches above eight rows take the
-  // same path through the separate operators.
-  //   * One GPU, up to eight rows: o and down add the residual themselves (y = h_next, residual = h) and, from four
-  //     rows on, leave the rows' sums of squares per 16-row block, so that the pre-norm that follows reads only its
-  //     slab of the stream.
-  //   * Tensor parallel, or more than eight rows: o and down write this rank's partial sums to `delta`, which is all-reduced; each CTA of the
-  //     next projection forms rms_norm(h + delta) itself and its first CTA writes h + delta to the OTHER buffer while
-  //     its siblings still read the old one.
-  float *h_cur = m->h, *h_nxt = m->h2;
-  const bool fold = m->comm == nullptr && B <= 8;   // (the tensor-memory GEMM of the larger batches takes no residual)
-  // (measured per decode step against the plain prologue: -1.3 % at four rows, -5.3 % at eight, nothing below)
-  const int ss_min = 4;
-  const int n_ss = (int)((d + 15) / 16);
-  struct SsGuard {   // (no request outlives this call, whichever way it returns)
-    tq_ctx* c;
-    ~SsGuard() { c->ss_req = nullptr; }
-  } ss_guard{ctx};
-  bool have_delta = false;  // true once `delta` holds a projection output not yet added to h
-  bool have_ss = false;     // true while `ss` describes h_cur
-  // y = h_nxt = h_cur + W x (one GPU), or delta = W x, all-reduced
-  auto project_back = [&](const tq_qweight* w, const void* x, size_t cols) -> int {
-    if (!fold) {
-      if (int e = tq_qlinear(ctx, w, x, TQ_BF16, cols, B, m->delta, TQ_F32, d, nullptr)) return e;
-      have_delta = true;
-      return tq_all_reduce_f32(ctx, m->comm, m->delta, (size_t)B * d);
-    }
-    ctx->ss_req = B >= ss_min ? m->ss : nullptr;
-    ctx->ss_written = false;
-    const int e = tq_qlinear(ctx, w, x, TQ_BF16, cols, B, h_nxt, TQ_F32, d, h_cur);
-    ctx->ss_req = nullptr;
-    have_ss = e == TQ_OK && ctx->ss_written;
-    std::swap(h_cur, h_nxt);
-    return e;
-  };
-  auto pre_norm = [&](const void* gain) {
-    QlinearNorm n;
-    n.h = h_cur;
-    n.delta = have_delta ? m->delta : nullptr;
-    n.gain_bf16 = gain;
-    n.h_out = fold ? nullptr : h_nxt;
-    n.eps = c.eps;
-    n.xn_tmp = m->xn;
-    n.sumsq = have_ss ? m->ss : nullptr;
-    n.n_sumsq = have_ss ? n_ss : 0;
-    return n;
-  };
-  for (size_t l = 0; l < m->layers.size(); ++l) {
-    const LlamaLayerW& L = m->layers[l];
-    const QlinearNorm n1 = pre_norm(L.attn_norm);
-    TQ_STEP(qlinear_fused(ctx, L.wqkv, nullptr, &n1, B, m->qkv, TQ_F32, q_dim + 2 * kv_dim, false, nullptr));
-    if (!fold) std::swap(h_cur, h_nxt);
-    TQ_STEP(launch_qkv_post(ctx, m->qkv, m->cos_t, m->sin_t, positions_dev, rope_positions_dev, B, m->heads_l, m->kv_l, (int)hd, (int)c.max_seq,
-                            m->qb, L.k_cache, L.v_cache, seq_stride, 1));
-    TQ_STEP(launch_gqa_decode(ctx, m->qb, L.k_cache, L.v_cache, m->lens, B, m->heads_l, m->kv_l, (int)hd, seq_stride,
-                              (int)max_len, m->attn, TQ_BF16));
-    TQ_STEP(project_back(L.wo, m->attn, q_dim));
-    // h += attention output; pre-norm of the MLP; gate/up; SwiGLU
-    const QlinearNorm n2 = pre_norm(L.ffn_norm);
-    if (L.wgu->gate_up_interleaved) {
-      TQ_STEP(qlinear_fused(ctx, L.wgu, nullptr, &n2, B, m->act, TQ_BF16, m->ffn_l, true, m->gu));
-    } else {
-      TQ_STEP(qlinear_fused(ctx, L.wgu, nullptr, &n2, B, m->gu, TQ_F32, 2 * (size_t)m->ffn_l, false, nullptr));
-      TQ_STEP(tq_swiglu(ctx, m->gu, m->gu + m->ffn_l, TQ_F32, 2 * (size_t)m->ffn_l, B, m->ffn_l, m->act, TQ_BF16));
-    }
-    if (!fold) std::swap(h_cur, h_nxt);
-    TQ_STEP(project_back(L.wdown, m->act, m->ffn_l));
-  }
-  // final norm (under tensor parallelism it adds the last MLP output) fused into the LM head, which sees every row
-  // (each is a sequence's last token)
-  const QlinearNorm nf = pre_norm(m->final_norm);
-  m->h_last = fold ? h_cur : h_nxt;   // (tensor parallel: the head kernel writes h + the last MLP output there)
-  if (m->tp == 1) {
-    TQ_STEP(qlinear_fused(ctx, m->lm_head, nullptr, &nf, B, logits_dev, TQ_F32, c.vocab, false, nullptr));
-  } else {
-    // column-parallel head: this rank's vocabulary slice, gathered rank-major: logits_dev is
-    // [tp][B][vocab/tp]
-    TQ_STEP(qlinear_fused(ctx, m->lm_head, nullptr, &nf, B, m->logits_l, TQ_F32, m->vocab_l, false, nullptr));
-    TQ_STEP(tq_all_gather(ctx, m->comm, m->logits_l, logits_dev, (size_t)B * m->vocab_l * sizeof(float)));
-  }
-#undef TQ_STEP
-  return TQ_OK;
+int tq_llama_decode_paged(tq_llama* m, const int* token_ids_dev, const tq_pages* pages, const int* seqs_dev, size_t batch, const int* group_starts_dev,
+                          const int* shared_dev, size_t n_groups, size_t max_shared, size_t max_len, float* logits_dev) {
+  if (!m) return TQ_EINVAL;
+  tq_ctx* ctx = m->ctx;
+  if (int st = bind(ctx)) return st;
+  const tq_llama_config& c = m->cfg;
+  TQ_REQUIRE(ctx, batch > 0 && batch <= c.max_batch, "tq_llama_decode_paged: batch must be 1..%u", c.max_batch);
+  TQ_REQUIRE(ctx, token_ids_dev && pages && logits_dev, "tq_llama_decode_paged: null pointer");
+  TQ_REQUIRE(ctx, pages->ctx->device == ctx->device, "tq_llama_decode_paged: the pool belongs to another device");
+  TQ_REQUIRE(ctx, seqs_dev || batch <= (size_t)pages->n_seqs, "tq_llama_decode_paged: the pool has %d sequences", pages->n_seqs);
+  const size_t rows = (size_t)pages->n_pages * pages->page_rows;
+  TQ_REQUIRE(ctx, rows <= (size_t)c.max_batch * c.max_seq && rows < (1ull << 31), "tq_llama_decode_paged: the cache has %zu rows, the pool's pages %zu",
+             (size_t)c.max_batch * c.max_seq, rows);
+  TQ_REQUIRE(ctx, (group_starts_dev != nullptr) == (shared_dev != nullptr) && (group_starts_dev == nullptr || (n_groups > 0 && n_groups <= batch)),
+             "tq_llama_decode_paged: groups have starts and shared lengths, at most one per sequence");
+  const PagedStep paged{pages, seqs_dev, group_starts_dev, shared_dev, n_groups, max_shared};
+  return decode_step(m, token_ids_dev, m->lens, m->rope, &paged, batch, max_len, logits_dev);
 }
 
 int tq_llama_prefill(tq_llama* m, const int* token_ids_dev, const int* cache_start_dev, size_t batch, size_t q_len,
@@ -487,3 +439,120 @@ int tq_llama_prefill(tq_llama* m, const int* token_ids_dev, const int* cache_sta
 }
 
 }  // extern "C"
+
+// One new token for each of `batch` sequences.  With pages, `positions` and `rope_positions` are the model's own arrays, filled here.
+static int decode_step(tq_llama* m, const int* token_ids_dev, const int* positions_dev, const int* rope_positions_dev, const PagedStep* paged,
+                       size_t batch, size_t max_len, float* logits_dev) {
+  tq_ctx* ctx = m->ctx;
+  const tq_llama_config& c = m->cfg;
+  TQ_REQUIRE(ctx, max_len > 0 && max_len <= c.max_seq, "tq_llama_decode: max_len must be 1..max_seq");
+  TQ_REQUIRE(ctx, m->lm_head != nullptr, "tq_llama_decode: head weights not set");
+  for (auto& L : m->layers) TQ_REQUIRE(ctx, L.wqkv != nullptr, "tq_llama_decode: a layer has no weights");
+  const int B = (int)batch;
+  const size_t d = c.d_model, hd = c.head_dim;
+  const size_t q_dim = (size_t)m->heads_l * hd, kv_dim = (size_t)m->kv_l * hd;
+  const size_t seq_stride = (size_t)c.max_seq * kv_dim;
+  int st;
+#define TQ_STEP(expr) \
+  if ((st = (expr)) != TQ_OK) return st;
+
+  if (paged) {
+    const tq_pages* pg = paged->pages;
+    const size_t most = (size_t)pg->table_ld * pg->page_rows;
+    TQ_CUDA(ctx, launch_k(ctx, paged_rows_kernel, dim3((B + 63) / 64), dim3(64), 0, (const int*)pg->tables, (const int*)pg->lens, paged->seqs, B, pg->n_seqs,
+                          pg->table_ld, pg->n_pages, pg->page_rows, (int)(max_len < most ? max_len : most), m->lens, m->rope));
+  } else {
+    TQ_CUDA(ctx, launch_k(ctx, lens_kernel, dim3((B + 63) / 64), dim3(64), 0, positions_dev, m->lens, B, (int)c.max_seq));
+  }
+  TQ_STEP(tq_embedding(ctx, m->embed, TQ_BF16, token_ids_dev, B, d, c.vocab, m->h, TQ_F32));
+
+  // The residual stream alternates between two buffers, and every pre-norm is fused into the projection that follows
+  // it; with a gate/up weight in the interleaved row order the SwiGLU is that projection's epilogue.  Per layer: qkv
+  // (+norm), RoPE/append, attention, merge, o, gate/up (+norm, +SwiGLU), down.  Batches above eight rows take the
+  // same path through the separate operators.
+  //   * One GPU, up to eight rows: o and down add the residual themselves (y = h_next, residual = h) and, from four
+  //     rows on, leave the rows' sums of squares per 16-row block, so that the pre-norm that follows reads only its
+  //     slab of the stream.
+  //   * Tensor parallel, or more than eight rows: o and down write this rank's partial sums to `delta`, which is all-reduced; each CTA of the
+  //     next projection forms rms_norm(h + delta) itself and its first CTA writes h + delta to the OTHER buffer while
+  //     its siblings still read the old one.
+  float *h_cur = m->h, *h_nxt = m->h2;
+  const bool fold = m->comm == nullptr && B <= 8;   // (the tensor-memory GEMM of the larger batches takes no residual)
+  // (measured per decode step against the plain prologue: -1.3 % at four rows, -5.3 % at eight, nothing below)
+  const int ss_min = 4;
+  const int n_ss = (int)((d + 15) / 16);
+  struct SsGuard {   // (no request outlives this call, whichever way it returns)
+    tq_ctx* c;
+    ~SsGuard() { c->ss_req = nullptr; }
+  } ss_guard{ctx};
+  bool have_delta = false;  // true once `delta` holds a projection output not yet added to h
+  bool have_ss = false;     // true while `ss` describes h_cur
+  // y = h_nxt = h_cur + W x (one GPU), or delta = W x, all-reduced
+  auto project_back = [&](const tq_qweight* w, const void* x, size_t cols) -> int {
+    if (!fold) {
+      if (int e = tq_qlinear(ctx, w, x, TQ_BF16, cols, B, m->delta, TQ_F32, d, nullptr)) return e;
+      have_delta = true;
+      return tq_all_reduce_f32(ctx, m->comm, m->delta, (size_t)B * d);
+    }
+    ctx->ss_req = B >= ss_min ? m->ss : nullptr;
+    ctx->ss_written = false;
+    const int e = tq_qlinear(ctx, w, x, TQ_BF16, cols, B, h_nxt, TQ_F32, d, h_cur);
+    ctx->ss_req = nullptr;
+    have_ss = e == TQ_OK && ctx->ss_written;
+    std::swap(h_cur, h_nxt);
+    return e;
+  };
+  auto pre_norm = [&](const void* gain) {
+    QlinearNorm n;
+    n.h = h_cur;
+    n.delta = have_delta ? m->delta : nullptr;
+    n.gain_bf16 = gain;
+    n.h_out = fold ? nullptr : h_nxt;
+    n.eps = c.eps;
+    n.xn_tmp = m->xn;
+    n.sumsq = have_ss ? m->ss : nullptr;
+    n.n_sumsq = have_ss ? n_ss : 0;
+    return n;
+  };
+  for (size_t l = 0; l < m->layers.size(); ++l) {
+    const LlamaLayerW& L = m->layers[l];
+    const QlinearNorm n1 = pre_norm(L.attn_norm);
+    TQ_STEP(qlinear_fused(ctx, L.wqkv, nullptr, &n1, B, m->qkv, TQ_F32, q_dim + 2 * kv_dim, false, nullptr));
+    if (!fold) std::swap(h_cur, h_nxt);
+    // (over pages: rows of one long cache, and positions for the rotation that are below max_seq already)
+    TQ_STEP(launch_qkv_post(ctx, m->qkv, m->cos_t, m->sin_t, positions_dev, rope_positions_dev, B, m->heads_l, m->kv_l, (int)hd,
+                            paged ? paged->pages->n_pages * paged->pages->page_rows : (int)c.max_seq, m->qb, L.k_cache, L.v_cache, paged ? 0 : seq_stride, 1));
+    if (paged) {
+      TQ_STEP(tq_gqa_decode_paged(ctx, m->qb, L.k_cache, L.v_cache, paged->pages, paged->seqs, batch, paged->group_starts, paged->shared, paged->n_groups,
+                                  paged->max_shared, m->heads_l, m->kv_l, hd, max_len, m->attn, TQ_BF16));
+    } else {
+      TQ_STEP(launch_gqa_decode(ctx, m->qb, L.k_cache, L.v_cache, m->lens, B, m->heads_l, m->kv_l, (int)hd, seq_stride,
+                                (int)max_len, m->attn, TQ_BF16));
+    }
+    TQ_STEP(project_back(L.wo, m->attn, q_dim));
+    // h += attention output; pre-norm of the MLP; gate/up; SwiGLU
+    const QlinearNorm n2 = pre_norm(L.ffn_norm);
+    if (L.wgu->gate_up_interleaved) {
+      TQ_STEP(qlinear_fused(ctx, L.wgu, nullptr, &n2, B, m->act, TQ_BF16, m->ffn_l, true, m->gu));
+    } else {
+      TQ_STEP(qlinear_fused(ctx, L.wgu, nullptr, &n2, B, m->gu, TQ_F32, 2 * (size_t)m->ffn_l, false, nullptr));
+      TQ_STEP(tq_swiglu(ctx, m->gu, m->gu + m->ffn_l, TQ_F32, 2 * (size_t)m->ffn_l, B, m->ffn_l, m->act, TQ_BF16));
+    }
+    if (!fold) std::swap(h_cur, h_nxt);
+    TQ_STEP(project_back(L.wdown, m->act, m->ffn_l));
+  }
+  // final norm (under tensor parallelism it adds the last MLP output) fused into the LM head, which sees every row
+  // (each is a sequence's last token)
+  const QlinearNorm nf = pre_norm(m->final_norm);
+  m->h_last = fold ? h_cur : h_nxt;   // (tensor parallel: the head kernel writes h + the last MLP output there)
+  if (m->tp == 1) {
+    TQ_STEP(qlinear_fused(ctx, m->lm_head, nullptr, &nf, B, logits_dev, TQ_F32, c.vocab, false, nullptr));
+  } else {
+    // column-parallel head: this rank's vocabulary slice, gathered rank-major: logits_dev is
+    // [tp][B][vocab/tp]
+    TQ_STEP(qlinear_fused(ctx, m->lm_head, nullptr, &nf, B, m->logits_l, TQ_F32, m->vocab_l, false, nullptr));
+    TQ_STEP(tq_all_gather(ctx, m->comm, m->logits_l, logits_dev, (size_t)B * m->vocab_l * sizeof(float)));
+  }
+#undef TQ_STEP
+  return TQ_OK;
+}

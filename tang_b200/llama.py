@@ -11,6 +11,7 @@ import numpy as np
 from . import _lib
 from .device import Buffer, QBuffer, QuantComputeDevice
 from .generation import check_lengths, decode_loop
+from .pages import PagePool
 
 
 class LlamaConfig(C.Structure):
@@ -76,6 +77,15 @@ class LlamaLayerWeights:
     ffn_norm: Buffer    # bf16 [d_model]
 
 
+@dataclass
+class Samples:
+    """What ``LlamaModel.sample`` draws: int32 and f32 [prompts, samples, n_new], and for every prompt its samples' numbers from the
+    likeliest (largest sum of log probabilities) to the least."""
+    tokens: np.ndarray
+    logprobs: np.ndarray
+    order: np.ndarray
+
+
 class LlamaModel:
     def __init__(self, dev: QuantComputeDevice, cfg: LlamaConfig, comm: Comm | None = None):
         self.dev, self.cfg, self.comm = dev, cfg, comm
@@ -128,14 +138,82 @@ class LlamaModel:
         self.dev._check(self.dev._L.tq_llama_prefill(C.c_void_p(self.handle), C.c_void_p(token_ids.ptr), C.c_void_p(cache_start.ptr),
                                                      batch, q_len, C.c_void_p(logits.ptr)))
 
-    def generate(self, prompts, n_new: int, sampling=None, seed: int = 42, comm_world: int = 1) -> np.ndarray:
+    def page_pool(self, n_seqs: int, page_rows: int | None = None, **state) -> PagePool:
+        """A ``PagePool`` over the caches of all layers, seen as max_batch * max_seq / page_rows pages: the rows that ``prefill`` and ``decode``
+        give sequence b are the pages from b * max_seq / page_rows on.  `page_rows`: the largest of 64, 32 and 16 that divides max_seq unless
+        given.  `state`: refs, tables, lens of ``PagePool``."""
+        c = self.cfg
+        if page_rows is None:
+            page_rows = next((p for p in (64, 32, 16) if c.max_seq % p == 0), 0)
+        if page_rows < 1 or c.max_seq % page_rows:
+            raise _lib.TangqError(_lib.TQ_EINVAL, f"page_pool: max_seq {c.max_seq} is not a multiple of the pages' rows (16 or more)")
+        arrays = [b for layer in range(c.n_layers) for b in self.kv_buffers(layer)[:2]]
+        return PagePool(self.dev, c.max_batch * c.max_seq // page_rows, page_rows, n_seqs, c.max_seq // page_rows, arrays, **state)
+
+    def decode_paged(self, token_ids: Buffer, pool: PagePool, batch: int, max_len: int, logits: Buffer, seqs: Buffer | None = None,
+                     group_starts: Buffer | None = None, shared: Buffer | None = None, n_groups: int = 0, max_shared: int = 0) -> None:
+        """``decode`` over a ``page_pool``: the last position of each sequence, for which ``PagePool.extend`` has made room, is its new token's
+        (``tq_llama_decode_paged``); sequences and groups as in ``gqa_decode_paged``."""
+        if token_ids.n < batch or logits.n < batch * self.cfg.vocab or (seqs is not None and seqs.n < batch):
+            raise _lib.TangqError(_lib.TQ_EINVAL, "decode_paged: buffer sizes do not match the batch")
+        if group_starts is not None and (group_starts.n < n_groups or shared is None or shared.n < n_groups):
+            raise _lib.TangqError(_lib.TQ_EINVAL, "decode_paged: fewer starts or shared lengths than groups")
+        ptr = lambda b: C.c_void_p(b.ptr if b is not None else 0)
+        self.dev._check(self.dev._L.tq_llama_decode_paged(C.c_void_p(self.handle), ptr(token_ids), C.c_void_p(pool.handle), ptr(seqs), batch,
+                                                          ptr(group_starts), ptr(shared), n_groups, max_shared, max_len, ptr(logits)))
+
+    def sample(self, prompts, n_new: int, samples: int, sampling=None, seed: int = 42, comm_world: int = 1) -> Samples:
+        """`samples` continuations of each prompt (equal lengths), each with its log probability.  A prompt is run through the model and kept in
+        the cache once: its samples are forked from it, share its pages and attend them as one group.  Sample j draws as ``generate`` with
+        seed + j does.  Uses the whole cache; prompts * samples are at most max_batch."""
+        prompts = np.asarray(prompts, np.int32)
+        check_lengths(prompts, n_new, self.cfg.max_seq)
+        dev, c = self.dev, self.cfg
+        B, P = prompts.shape
+        if samples < 1 or B * samples > c.max_batch:
+            raise _lib.TangqError(_lib.TQ_EINVAL, f"sample: {B} prompts with {samples} samples each need a model of that many sequences")
+        N, first = B * samples, np.arange(B, dtype=np.int32) * samples
+        pool = self.page_pool(N)
+        try:
+            if P > 1:
+                scratch = dev.alloc(B * c.vocab, _lib.F32)
+                self.prefill(dev.upload(np.ascontiguousarray(prompts[:, :P - 1]), _lib.I32), dev.upload(np.zeros(B, np.int32), _lib.I32), B, P - 1,
+                             scratch)
+                # the first sample of prompt i takes over the pages of the rows that prefill gave prompt i
+                refs, tables, lens = np.zeros(pool.n_pages, np.int32), np.full((N, pool.max_pages), -1, np.int32), np.zeros(N, np.int32)
+                used = -(-(P - 1) // pool.page_rows)
+                for i, s in enumerate(first):
+                    tables[s, :used] = i * pool.max_pages + np.arange(used)
+                    refs[tables[s, :used]] = 1
+                    lens[s] = P - 1
+                for buf, v in ((pool.refs, refs), (pool.tables, tables), (pool.lens, lens)):
+                    dev.upload_into(buf, v)
+                if samples > 1:
+                    pool.fork(np.repeat(first, samples - 1), [s + j for s in first for j in range(1, samples)])
+            every, starts = dev.upload(np.arange(N, dtype=np.int32), _lib.I32), dev.upload(first, _lib.I32)
+            shared = dev.upload(np.full(B, P - 1, np.int32), _lib.I32)
+
+            def step(tok, pos, logits):
+                pool.extend(every, N)
+                self.decode_paged(tok, pool, N, P + n_new, logits, group_starts=starts, shared=shared, n_groups=B, max_shared=P - 1)
+
+            tokens, logprobs = decode_loop(dev, step, np.repeat(prompts, samples, 0), n_new, c.vocab, sampling,
+                                           np.tile(seed + np.arange(samples, dtype=np.uint64), B), comm_world, logprobs=True)
+        finally:
+            dev.sync()
+            pool.destroy()
+        tokens, logprobs = tokens.reshape(B, samples, n_new), logprobs.reshape(B, samples, n_new)
+        return Samples(tokens, logprobs, np.argsort(-logprobs.sum(2, dtype=np.float64), axis=1, kind="stable"))
+
+    def generate(self, prompts, n_new: int, sampling=None, seed: int = 42, comm_world: int = 1, logprobs: bool = False):
         """``generate`` (crates/tang-infer/src/sampling.rs:229-256) for a batch of equal-length prompts.  The prompt
         goes through one prefill chunk (all tokens but the last); then decode -> ``Sampler::sample`` -> advance is captured
         once as a CUDA graph and replayed `n_new` times, the logits never leaving the device.  `sampling` is a
         ``SamplerConfig`` (None or temperature 0: greedy, the first maximum); every sequence owns an LCG seeded
         with `seed` (as ``Sampler::with_seed`` per call of ``generate``); the repetition penalty sees the prompt and
         everything generated so far.  Returns int32 [batch, n_new]; the caller cuts at its stop token (what is
-        drawn before a stop token does not depend on what follows)."""
+        drawn before a stop token does not depend on what follows); with `logprobs` also the tokens' log probabilities,
+        f32 [batch, n_new]."""
         prompts = np.asarray(prompts, np.int32)
         check_lengths(prompts, n_new, self.cfg.max_seq)
         dev = self.dev
@@ -145,7 +223,7 @@ class LlamaModel:
             self.prefill(dev.upload(np.ascontiguousarray(prompts[:, :P - 1]), _lib.I32), dev.upload(np.zeros(B, np.int32), _lib.I32),
                          B, P - 1, scratch)
         return decode_loop(dev, lambda tok, pos, logits: self.decode(tok, pos, B, P + n_new, logits), prompts, n_new,
-                           self.cfg.vocab, sampling, seed, comm_world)
+                           self.cfg.vocab, sampling, seed, comm_world, logprobs)
 
     def generate_greedy(self, prompts, n_new: int, comm_world: int = 1) -> np.ndarray:
         """``generate`` with ``SamplingConfig::greedy()``."""

@@ -58,9 +58,10 @@ class StepModel:
         """While set, every step leaves the f32 stream after each layer in `streams` [layers, rows, width]."""
         self._call("trace", C.c_void_p(streams.ptr if streams is not None else 0))
 
-    def generate(self, prompts, n_new: int, sampling=None, seed: int = 42) -> np.ndarray:
+    def generate(self, prompts, n_new: int, sampling=None, seed: int = 42, logprobs: bool = False):
         """``generate`` for a batch of prompts of any lengths: the prompts run as one ragged batch (all tokens but the
-        last of each), then decode -> sample -> advance as one replayed graph.  Returns int32 [batch, n_new]."""
+        last of each), then decode -> sample -> advance as one replayed graph.  Returns int32 [batch, n_new]; with `logprobs` also the tokens'
+        log probabilities, f32 [batch, n_new]."""
         from .engine import Engine
 
         prompts = [np.asarray(p, np.int32) for p in prompts]
@@ -73,7 +74,7 @@ class StepModel:
         B, longest = len(prompts), max(len(p) for p in prompts)
         slot_buf = self.dev.upload(np.array(slots, np.int32), _lib.I32)
         return decode_loop(self.dev, lambda tok, pos, logits: self.decode(tok, pos, B, longest + n_new, logits, slot_buf), prompts, n_new,
-                           self.cfg.vocab, sampling, seed)
+                           self.cfg.vocab, sampling, seed, logprobs=logprobs)
 
     def generate_greedy(self, prompts, n_new: int) -> np.ndarray:
         return self.generate(prompts, n_new, None)
