@@ -74,7 +74,7 @@ struct PuSeqPlan {
 };
 struct PuUnit {
   bool pre;
-  int b0, rows, tiles, tile, shared_tiles, last;      // b0: (first) sequence of the batch; tile: the asked one; last: keys of the last tile
+  int b0, head, rows, tiles, tile, shared_tiles, last;  // b0: (first) sequence of the batch; head: whose pages; tile: the asked one; last: keys of the last
   int slot;                                           // first row of its partial results, without what KV head and item add
 };
 
@@ -98,6 +98,7 @@ __device__ __forceinline__ PuUnit pu_locate(const PagedParams& p, const PuPlan& 
     const int rest = f - l.pre[g], rt = rest / u.tiles;
     u.tile = rest - rt * u.tiles;
     u.b0 = start + rt * l.per_tile;
+    u.head = start;                    // the group's first member
     u.rows = min(l.per_tile, members - rt * l.per_tile) * l.group;
     u.shared_tiles = 0;
     u.last = kPfTile;
@@ -106,7 +107,7 @@ __device__ __forceinline__ PuUnit pu_locate(const PagedParams& p, const PuPlan& 
     const int h = f - l.pre_tiles, b = pu_last_not_above(l.own, l.batch, h);
     u.tiles = l.own[b + 1] - l.own[b];
     u.tile = h - l.own[b];
-    u.b0 = b;
+    u.b0 = u.head = b;
     u.rows = l.group;
     u.shared_tiles = l.last[b] >> 8;
     u.last = (l.last[b] & 255) + 1;
@@ -139,10 +140,11 @@ struct PuParams {
   int* counter;                                       // items handed out beyond the first two of every CTA; zero between calls
 };
 
-__device__ __forceinline__ void pu_scan(int* a, int n, int lane) {      // a[0 .. n-1] become the sums before them, a[n] the sum; one warp
+template <typename F>
+__device__ __forceinline__ void pu_scan(int* a, int n, int lane, F value) {      // a[i] becomes the sum of the values before i, a[n] the whole; one warp
   int sum = 0;
   for (int base = 0; base < n; base += 32) {
-    const int v = base + lane < n ? a[base + lane] : 0;
+    const int v = base + lane < n ? value(base + lane) : 0;
     int incl = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -249,41 +251,40 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   if (threadIdx.x == 0 && (smem_u32(smem_raw) & 1023)) give_up(DERR_TMEM);
 
   // ---- the plan: every CTA makes it for itself
+  // (what is read of the groups is on its way before the sequences' lengths, which two loads in a row bring)
+  bool bad = false;                    // starts that do not ascend from 0: nothing is shared, and the status word says why
+  for (int g = threadIdx.x; g < p.n_groups; g += kPuThreads) {
+    const int start = p.group_starts[g], next = g + 1 < p.n_groups ? p.group_starts[g + 1] : p.batch;
+    l.pre[g] = min(max(p.shared[g], 0), p.max_shared);
+    bad = bad || start < 0 || start > next || next > p.batch || (g == 0 && start != 0);
+  }
   for (int b = threadIdx.x; b < p.batch; b += kPuThreads) {
     const int s = paged_row_of(p, b);
     if (s < 0 && blockIdx.x == 0) give_up(DERR_PAGE_LIST);
     l.own[b] = s < 0 ? 0 : min(max(p.lens[s], 0), p.max_len);
     l.last[b] = 0;
   }
-  bool bad = false;                    // starts that do not ascend from 0: nothing is shared, and the status word says why
-  for (int g = threadIdx.x; g < p.n_groups; g += kPuThreads) {
-    const int start = p.group_starts[g], next = g + 1 < p.n_groups ? p.group_starts[g + 1] : p.batch;
-    bad = bad || start < 0 || start > next || next > p.batch || (g == 0 && start != 0);
-  }
   bad = __syncthreads_or(bad);
   if (bad && threadIdx.x == 0 && blockIdx.x == 0) give_up(DERR_PAGE_LIST);
   l.groups = bad ? 0 : p.n_groups;
   for (int g = warp; g < l.groups; g += kPuThreads / 32) {
     // no more than the shortest member has, in whole tiles
-    const int start = pu_group_start(p, g), end = pu_group_end(p, g, start);
-    int least = min(max(p.shared[g], 0), p.max_shared);
+    const int start = pu_group_start(p, g), end = pu_group_end(p, g, start), members = end - start;
+    int least = l.pre[g];
     for (int b = start + lane; b < end; b += 32) least = min(least, l.own[b]);
-    for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-    const int tiles = end - start > 1 ? least / kPfTile : 0;
+    least = __reduce_min_sync(0xffffffffu, least);
+    const int tiles = members > 1 ? least / kPfTile : 0;
     for (int b = start + lane; b < end; b += 32) l.last[b] = tiles << 8;
-    if (lane == 0) {
-      l.pre[g] = tiles * ((end - start + pp.per_tile - 1) / pp.per_tile);
-    }
+    if (lane == 0) l.pre[g] = members <= pp.per_tile ? tiles : tiles * ((members + pp.per_tile - 1) / pp.per_tile);
   }
-  __syncthreads();
-  for (int b = threadIdx.x; b < p.batch; b += kPuThreads) {
-    const int len = l.own[b], shared = l.last[b] >> 8, tiles = (len + kPfTile - 1) / kPfTile;
-    l.own[b] = tiles - shared;
-    l.last[b] |= tiles > shared ? len - 1 - (tiles - 1) * kPfTile : 0;
-  }
-  __syncthreads();
-  if (warp == 0) pu_scan(l.own, p.batch, lane);
-  if (warp == 1) pu_scan(l.pre, l.groups, lane);
+  if (l.groups) __syncthreads();
+  if (warp == 0)
+    pu_scan(l.own, p.batch, lane, [&](int b) {
+      const int len = l.own[b], shared = l.last[b] >> 8, tiles = (len + kPfTile - 1) / kPfTile;
+      l.last[b] |= tiles > shared ? len - 1 - (tiles - 1) * kPfTile : 0;
+      return tiles - shared;
+    });
+  if (warp == 1) pu_scan(l.pre, l.groups, lane, [&](int g) { return l.pre[g]; });
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
@@ -350,8 +351,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         w.last = u.tile + w.n == u.tiles ? u.last : kPfTile;
         w.rows = u.rows;
         w.b0 = u.b0;
-        // (shared tiles: the pages of the group's first member)
-        w.seq = max(paged_row_of(p, w.pre ? pu_group_start(p, pu_last_not_above(l.pre, l.groups, f)) : u.b0), 0);
+        w.seq = max(paged_row_of(p, u.head), 0);
         w.wide = pu_wide<TERMS>(u);
         w.out = w.kv * (p.batch * p.group + apart * (w.pre ? pp.max_pre : pp.max_own)) + u.slot + apart * i;
         tell(w);
