@@ -44,7 +44,7 @@ constexpr int kPuTile = 4 * kPfBox / 2;               // bytes of 128 rows of ke
 constexpr int kPuRing = 5;
 constexpr int kPuWeights = 2 * 32 * 128;              // a parity's weights where keys are the lanes: 32 rows of 128 keys, in two halves
 constexpr int kPuOnes = 1024;                         // eight rows of 64 ones
-constexpr int kPuMeet = 2 * 2 * 4 * 32 * 4;           // [parity][maxima, references][warp][row]
+constexpr int kPuMeet = (2 + 2) * 128 * 4;            // maxima [parity][warp][row], references [piece's parity][row, or warp and row]
 constexpr float kPuLargest = 7.9228162514264338e28f;  // 2^96: a weight above it is too far from its reference
 constexpr int kPuHeader = 640;                        // barriers, pieces
 constexpr int kPuReaders = 12;                        // warps that are told the pieces
@@ -198,7 +198,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   uint64_t* piece_full = o_free + 2;                  // [kPuPieces]
   uint64_t* piece_empty = piece_full + kPuPieces;
   uint64_t* met = piece_empty + kPuPieces;            // [parity] the four warps of a softmax group
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(met + 2);
+  uint64_t* ref_full = met + 2;                       // [piece's parity]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ref_full + 2);
   PuPiece* piece_s = reinterpret_cast<PuPiece*>(q_full) + (kPuHeader / sizeof(PuPiece) - kPuPieces);
   PuPlan l;
   l.own = reinterpret_cast<int*>(q_full) + kPuHeader / 4;
@@ -230,6 +231,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         mbar_init(&o_done[x], 1);
         mbar_init(&o_free[x], 4);
         mbar_init(&met[x], 4);
+        mbar_init(&ref_full[x], 4);
       }
       mbar_init_fence();
     }
@@ -472,20 +474,21 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     const uint64_t qd = umma_desc_sw128(q_s), kd = umma_desc_sw128(kv_s), vd = pf_desc_mn(kv_s), wd = umma_desc_sw128(w_s);
     const uint64_t od = umma_desc_sw128(ones_s) & ~((uint64_t)0x3FFF << 32);      // (all groups of eight rows are the same one)
     uint32_t q_seen = 0;
-    int made[2] = {0, 0}, freed[2] = {0, 0};          // tiles of a parity so far, results read
+    int made[2] = {0, 0}, freed[2] = {0, 0};          // tiles of a parity so far, pieces of a parity
     bool ok = true;
     struct Tile {
       int steps, wide;                                // 16-key steps, layout
-      bool first;                                     // of its parity in the piece
+      bool first;                                     // of the piece
+      int piece;                                      // its parity
     };
     auto values = [&](int t, const Tile& w) {
       const int x = t & 1, r = pu_values_at(t), slot = r % kPuRing;
-      const uint32_t s_t = tmem + (uint32_t)(x * 256), o_t = s_t + 128u;
+      const uint32_t s_t = tmem + (uint32_t)(x * 128), o_t = tmem + 256u + (uint32_t)(w.piece * 128);
       bool good = __all_sync(0xffffffffu, mbar_wait_spin(&kv_full[slot], (uint32_t)((r / kPuRing) & 1)) && mbar_wait_spin(&p_full[x], (uint32_t)(made[x] & 1)));
       ++made[x];
       if (good && w.first) {
-        good = __all_sync(0xffffffffu, freed[x] == 0 || mbar_wait_spin(&o_free[x], (uint32_t)((freed[x] - 1) & 1)));
-        ++freed[x];
+        good = __all_sync(0xffffffffu, freed[w.piece] == 0 || mbar_wait_spin(&o_free[w.piece], (uint32_t)((freed[w.piece] - 1) & 1)));
+        ++freed[w.piece];
       }
       if (!good) return false;
       tc_fence_after();
@@ -511,8 +514,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     };
     Tile before{};
     PuPiece w;
-    int own_pieces = 0, t = 0;
-    for (take(ok, w); w.n && ok; take(ok, w)) {
+    int own_pieces = 0, t = 0, piece = 0;
+    for (take(ok, w); w.n && ok; piece ^= 1, take(ok, w)) {
       const int q_slot = w.pre ? 0 : own_pieces++ & 3;
       ok = __all_sync(0xffffffffu, mbar_wait_spin(&q_full[q_slot], (q_seen >> q_slot) & 1u));
       q_seen ^= 1u << q_slot;
@@ -524,9 +527,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         if (!ok) break;
         tc_fence_after();
         const int keys = i == w.n - 1 ? w.last : kPfTile;
-        const Tile now{(keys + 15) >> 4, w.wide, i < 2};
+        const Tile now{(keys + 15) >> 4, w.wide, i == 0, piece};
         if (leader) {
-          const uint32_t s_t = tmem + (uint32_t)(x * 256);
+          const uint32_t s_t = tmem + (uint32_t)(x * 128);
           const uint32_t idesc = umma_idesc_bf16(now.wide ? (now.wide == 32 ? 32 : 16) : kPfTile);
           const uint64_t kt = kd + (uint64_t)(slot * (kPuTile >> 4)), qt = qd + (uint64_t)(q_slot * (16 * 128 >> 4));
           const uint64_t da = now.wide ? kt : qt, db = now.wide ? qt : kt;
@@ -556,10 +559,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     // The reference that scores are taken from is their maximum in the piece's first tile: a bf16 weight may be as large as an f32 one, so that
     // nothing is rescaled; a weight above 2^96 becomes no number, and the joining kernel goes through the row's keys one by one.
     const int x = (warp - 4) >> 2, q4 = warp & 3, t128 = 32 * q4 + lane;
-    const uint32_t s_t = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)(x * 256), o_t = s_t + 128u;
-    float *max_s = meet_s + x * 256, *ref_s = max_s + 128 + 32 * q4;   // [warp][32 rows]; this warp's [32 rows]
+    const uint32_t s_t = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)(x * 128);
+    uint32_t o_t = 0;                  // of the piece
+    float *max_s = meet_s + x * 128, *ref_s = nullptr;                 // [warp][32 rows]; the piece's references
     int meetings = 0;
-    bool ok = true, first = true;
+    bool ok = true, first = true, leads = true;      // the group's first tile of the piece; it is the piece's first
+    int slot = 0;                      // the piece's parity
     auto meet = [&]() {                // (a barrier of the group whose wait ends, as every other's)
       arrive(&met[x]);
       ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(&met[x], (uint32_t)(meetings++ & 1)));
@@ -569,7 +574,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     PuPiece u{};
     // a tile whose lanes are keys
     auto keyed = [&](int wide, bool seen) {
-      if (first) {
+      if (first && leads) {
         float mine = -FLT_MAX;
 #pragma unroll 1
         for (int i = 0; 8 * i < u.rows; ++i) {
@@ -585,9 +590,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         max_s[t128] = mine;
         meet();
         const float mx = fmaxf(fmaxf(max_s[lane], max_s[32 + lane]), fmaxf(max_s[64 + lane], max_s[96 + lane]));
-        ref_s[lane] = mx == -FLT_MAX ? mx : mx * p.scale_log2;
-        __syncwarp();
+        ref_s[t128] = mx == -FLT_MAX ? mx : mx * p.scale_log2;         // (a copy for every warp)
+        arrive(&ref_full[slot]);
       }
+      if (first) ref = ref_s[t128];
+      const float* refs = ref_s + 32 * q4;
       uint8_t* at = w_s + x * kPuWeights + (t128 >> 6) * (kPuWeights / 2) + 2 * (t128 & 7);
       const int chunk = (t128 & 63) >> 3;
 #pragma unroll 1
@@ -595,7 +602,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         float v[8];
         __syncwarp();
         tmem_ld8(s_t + 8u * i, v);
-        const float4 f0 = *reinterpret_cast<const float4*>(&ref_s[8 * i]), f1 = *reinterpret_cast<const float4*>(&ref_s[8 * i + 4]);
+        const float4 f0 = *reinterpret_cast<const float4*>(&refs[8 * i]), f1 = *reinterpret_cast<const float4*>(&refs[8 * i + 4]);
         const float from[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
         // (rows behind the last one have columns and places too, which nobody reads: without branches the eight go side by side)
         float w[8];
@@ -636,31 +643,37 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         }
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          if (8 * i + r < u.rows) to_o[(size_t)(8 * i + r) * 2 * kPaDim + t128] = o[r];
+          if (8 * i + r < u.rows) to_o[(size_t)(8 * i + r) * kPaDim + t128] = o[r];
         }
         float sum = l8[0];
 #pragma unroll
-        for (int r = 1; r < 8; ++r) sum = lane == r ? l8[r] : sum;
-        if (q4 == 0 && lane < 8 && 8 * i + lane < u.rows) *reinterpret_cast<float2*>(to_ml + (8 * i + lane) * 4) = make_float2(ref_s[8 * i + lane], sum);
+        for (int r = 1; r < 8; ++r) sum = (lane & 7) == r ? l8[r] : sum;
+        // (a row's reference is in the lane of its number)
+        if (q4 == 0 && (lane >> 3) == i && lane < u.rows) *reinterpret_cast<float4*>(to_ml + lane * 4) = make_float4(ref, sum, ref, 0.f);
       }
       tc_fence_before();
-      arrive(&o_free[x]);                              // (the next piece's products may begin)
+      arrive(&o_free[slot]);                           // (the products of the piece after the next may begin)
     };
-    int t0 = 0;                        // tiles before the piece
-    for (take(ok, u); u.n && ok; t0 += u.n, take(ok, u)) {
-      const int place = (x - t0) & 1;   // the group's first tile is the piece's first or second: its partial result's place
+    int t0 = 0, piece = 0;             // tiles and pieces before the piece
+    for (take(ok, u); u.n && ok; t0 += u.n, ++piece, take(ok, u)) {
+      const int place = (x - t0) & 1;  // the group's first tile is the piece's first or second
+      leads = place == 0;
+      slot = piece & 1;
+      o_t = tmem + ((uint32_t)(32 * q4) << 16) + 256u + (uint32_t)(slot * 128);
+      ref_s = meet_s + 256 + slot * 128;
+      float *to_o = (u.pre ? pp.pre_o : pp.own_o) + (size_t)u.out * kPaDim, *to_ml = (u.pre ? pp.pre_ml : pp.own_ml) + (size_t)u.out * 4;
       for (int i = place; i < u.n && ok; i += 2) {
         first = i == place;
         const int wide = u.wide, r = 32 * q4 + lane;
         const bool live = r < u.rows;
-        ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[x], (uint32_t)(done & 1)));
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[x], (uint32_t)(done & 1)) && (!first || leads || mbar_wait_spin(&ref_full[slot], (uint32_t)((piece >> 1) & 1))));
         if (!ok) break;
         tc_fence_after();
         if (wide) {
           keyed(wide, t128 < (i == u.n - 1 ? u.last : kPfTile));
         } else {
           __syncwarp();
-          if (first) {
+          if (first && leads) {
             float mx = -FLT_MAX;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -669,7 +682,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
 #pragma unroll
               for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[j]);
             }
-            ref = mx == -FLT_MAX ? mx : mx * p.scale_log2;
+            ref_s[r] = mx == -FLT_MAX ? mx : mx * p.scale_log2;
+            arrive(&ref_full[slot]);
+          }
+          if (first) {
+            ref = ref_s[r];
             sum_all = 0.f;
           }
           __syncwarp();
@@ -703,13 +720,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         }
         arrive(&p_full[x]);
         ++done;
-        if (i + 2 < u.n) continue;
+        // (a sum each of the two groups; a piece of one tile has one)
+        if (!wide && live && i + 2 >= u.n) {
+          const float2 ml = make_float2(ref, sum_all > kPuLargest ? NAN : sum_all);
+          if (u.n > 1) *reinterpret_cast<float2*>(to_ml + r * 4 + 2 * place) = ml;
+          else *reinterpret_cast<float4*>(to_ml + r * 4) = make_float4(ml.x, ml.y, ml.x, 0.f);
+        }
+        if (i + 1 < u.n) continue;
 
-        // ---- the piece's result
+        // ---- the piece's result, by the group that has its last tile
         ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[x], (uint32_t)((done - 1) & 1)));
         if (!ok) break;
         tc_fence_after();
-        float *to_o = (u.pre ? pp.pre_o : pp.own_o) + ((size_t)u.out * 2 + place) * kPaDim, *to_ml = (u.pre ? pp.pre_ml : pp.own_ml) + ((size_t)u.out * 2 + place) * 2;
         if (wide) {
           keyed_out(wide, to_o, to_ml);
         } else {
@@ -719,14 +741,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
             __syncwarp();
             pf_ld32(o_t + (uint32_t)c, o);
             if (live) {
-              float* o_row = to_o + (size_t)r * 2 * kPaDim + c;          // (whole sectors: 32 bytes a store)
+              float* o_row = to_o + (size_t)r * kPaDim + c;          // (whole sectors: 32 bytes a store)
 #pragma unroll
               for (int j = 0; j < 32; j += 8) st_global8(o_row + j, &o[j]);
             }
           }
           tc_fence_before();
-          arrive(&o_free[x]);
-          if (live) *reinterpret_cast<float2*>(to_ml + r * 4) = make_float2(ref, sum_all > kPuLargest ? NAN : sum_all);
+          arrive(&o_free[slot]);
         }
       }
     }
@@ -751,24 +772,19 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *pp.counter = 0;
   const int kv = head / p.group, h = head - kv * p.group;
   const int own_e = q.own_f + q.own_tiles, pre_e = q.pre_f + q.pre_tiles, own_c = pu_own_item(cut, q.own_f), pre_c = q.pre_f / cut.pre;
-  const int own = q.own_tiles ? 2 * (pu_own_item(cut, own_e - 1) - own_c + 1) : 0, pre = q.pre_tiles ? 2 * ((pre_e - 1) / cut.pre - pre_c + 1) : 0;
+  const int own = q.own_tiles ? pu_own_item(cut, own_e - 1) - own_c + 1 : 0, pre = q.pre_tiles ? (pre_e - 1) / cut.pre - pre_c + 1 : 0;
   float top = -FLT_MAX, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int base = 0; base < own + pre; base += 32) {
-    // a lane per place: its row of the partial results (the second one of a piece of one tile is none), maximum and sum
+    // a lane per partial result: its row, reference and sums
     const int i = base + lane;
     const float* row = nullptr;
-    float2 mine = make_float2(-FLT_MAX, 0.f);
+    float4 mine = make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
     if (i < own + pre) {
       const bool k = i >= own;
-      const int j = k ? i - own : i, item = (k ? pre_c : own_c) + (j >> 1), x = j & 1;
-      const int lo = k ? max(q.pre_f, item * cut.pre) : max(q.own_f, pu_own_first(cut, item));
-      const int hi = k ? min(pre_e, (item + 1) * cut.pre) : min(own_e, pu_own_first(cut, item + 1));
-      if (hi - lo > x) {
-        const int apart = k ? 128 : 8, most = k ? pp.max_pre : pp.max_own;
-        const size_t r = ((size_t)kv * (p.batch * p.group + apart * most) + b * p.group + h + (size_t)apart * item) * 2 + x;
-        row = (k ? pp.pre_o : pp.own_o) + r * kPaDim;
-        mine = *reinterpret_cast<const float2*>((k ? pp.pre_ml : pp.own_ml) + r * 2);
-      }
+      const int item = k ? pre_c + i - own : own_c + i, apart = k ? 128 : 8, most = k ? pp.max_pre : pp.max_own;
+      const size_t r = (size_t)kv * (p.batch * p.group + apart * most) + b * p.group + h + (size_t)apart * item;
+      row = (k ? pp.pre_o : pp.own_o) + r * kPaDim;
+      mine = *reinterpret_cast<const float4*>((k ? pp.pre_ml : pp.own_ml) + r * 4);
     }
     float4 v[8];
 #pragma unroll
@@ -778,7 +794,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
     }
     const float to = fmaxf(top, redux_max(mine.x)), f0 = ex2(top - to), w = ex2(mine.x - to);
     top = to;
-    l = l * f0 + warp_sum(mine.y * w);
+    l = l * f0 + warp_sum((mine.y + mine.w) * w);
 #pragma unroll
     for (int k = 0; k < 4; ++k) o[k] *= f0;
 #pragma unroll
@@ -889,14 +905,14 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   pp.max_pre = (int)per_kv;
   pp.max_own = (int)((kPuLong + kPuShort) * per_kv + 8);
   // partial results, the sequences' plans
-  const size_t own_rows = (batch * n_heads + 8 * n_kv_heads * pp.max_own) * 2, pre_rows = p.n_groups ? (batch * n_heads + 128 * n_kv_heads * pp.max_pre) * 2 : 0;
-  const size_t floats = (own_rows + pre_rows) * (kPaDim + 2);
+  const size_t own_rows = batch * n_heads + 8 * n_kv_heads * pp.max_own, pre_rows = p.n_groups ? batch * n_heads + 128 * n_kv_heads * pp.max_pre : 0;
+  const size_t floats = (own_rows + pre_rows) * (kPaDim + 4);
   if (int st = ensure_scratch(ctx, floats * sizeof(float) + (batch + 1) * sizeof(PuSeqPlan))) return st;
   pp.own_o = static_cast<float*>(ctx->scratch);
   pp.pre_o = pp.own_o + own_rows * kPaDim;
   pp.own_ml = pp.pre_o + pre_rows * kPaDim;
-  pp.pre_ml = pp.own_ml + own_rows * 2;
-  pp.plan = reinterpret_cast<PuSeqPlan*>(pp.pre_ml + pre_rows * 2);
+  pp.pre_ml = pp.own_ml + own_rows * 4;
+  pp.plan = reinterpret_cast<PuSeqPlan*>(pp.pre_ml + pre_rows * 4);
   pp.cut = reinterpret_cast<PuCut*>(pp.plan + batch);
   pp.counter = ctx->dev_err + kTileCounters;          // (the last of the counters)
   pp.a = p;
