@@ -33,11 +33,11 @@ __device__ __forceinline__ int paged_row_of(const PagedParams& p, int b) {
 // ---------------------------------------------------------------------------------------------
 // Units, tiles, items, pieces.  A unit is what meets the same keys: the rows (member, query head of one KV head) of up to 128 / group members of a group
 // over the group's shared positions, in whole tiles of 128, or one sequence's query heads over the rest.  The tiles of all units of a KV head stand in one
-// list, shared ones first, and are cut into items of equal length; CTAs, one an SM, take two items each and then the next one that nobody has, whatever
+// list, shared ones first, and are cut into items; CTAs, one an SM, take two items each and then the next one that nobody has, whatever
 // the lengths of the sequences and the speeds of the SMs.  (Items of all KV heads that stand at the same place of their lists follow one another: a cache
 // row holds all heads, and its 256 bytes a head are fetched at the same time.)  A piece is what an item has of a unit.  Its odd and its even tiles belong
-// to different softmax groups, which keep sums and products of their own and leave a partial result each; a second kernel joins them, in the
-// order of the list.
+// to different softmax groups, which take scores from the same reference, so that the products of both go to the same columns (two sets of columns, for
+// pieces that follow one another).  It leaves a partial result; a second kernel joins those of a row, in the order of the list.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPuThreads = 416;
 constexpr int kPuTile = 4 * kPfBox / 2;               // bytes of 128 rows of keys or values
@@ -134,7 +134,7 @@ struct PuParams {
   PagedParams a;
   int per_tile, per_quarter;                          // members of a row tile; of a row tile that fits 32 rows
   int max_pre, max_own;                               // items of a KV head at most (own ones: what the plan's rule can make, which rounds up a few)
-  float *own_o, *own_ml, *pre_o, *pre_ml;             // partial results: [row][2][128], [row][2][2]
+  float *own_o, *own_ml, *pre_o, *pre_ml;             // partial results: [row][128], [row][2] references and sums (of the groups)
   PuSeqPlan* plan;                                    // [batch]
   PuCut* cut;
   int* counter;                                       // items handed out beyond the first two of every CTA; zero between calls
@@ -556,7 +556,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     // the tensor memory's lanes, S^T = K Q^T and O^T = V^T P, with as many columns as there are rows (a product of 128 x 128 x 16 takes 84 cycles for four
     // rows too, one of 128 x 16 x 16 a fraction): a thread per key, whose weights go to shared memory, each as two bf16 terms in rows of their own.
     // The weights' sums come from a product with ones.
-    // The reference that scores are taken from is their maximum in the piece's first tile: a bf16 weight may be as large as an f32 one, so that
+    // The reference that scores are taken from is their maximum in the piece's first tile, which the group with that tile tells the other one: a bf16 weight may be as large as an f32 one, so that
     // nothing is rescaled; a weight above 2^96 becomes no number, and the joining kernel goes through the row's keys one by one.
     const int x = (warp - 4) >> 2, q4 = warp & 3, t128 = 32 * q4 + lane;
     const uint32_t s_t = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)(x * 128);
@@ -690,31 +690,44 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
             sum_all = 0.f;
           }
           __syncwarp();
-          uint32_t low[TERMS == 2 ? 64 : 1];
+          // Weights take the first half of the scores' columns.  Second terms take the other half: quarters in the order 0, 2, 1, 3, so that only three
+          // sixteens wait in registers for columns that are read.
+          uint32_t keep[TERMS == 2 ? 3 : 1][16];                       // second terms of quarter 0; weights and second terms of quarter 2
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int step = 0; step < 4; ++step) {
+            const int c = TERMS == 1 ? step : step == 1 ? 2 : step == 2 ? 1 : step;
             float v[32];
             pf_ld32(s_t + 32u * c, v);
-            uint32_t w[16];
+            uint32_t w[16], low[TERMS == 2 ? 16 : 1];
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const float w0 = ex2(fmaf(v[2 * j], p.scale_log2, -ref)), w1 = ex2(fmaf(v[2 * j + 1], p.scale_log2, -ref));
               sum[j & 3] += w0 + w1;
-              if constexpr (TERMS == 2) split_bf16(w0, w1, w[j], low[16 * c + j]);
+              if constexpr (TERMS == 2) split_bf16(w0, w1, w[j], low[j]);
               else w[j] = pack_bf16(w0, w1);
             }
             sum_all += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_st16(s_t + 16u * c, w);                 // over scores that this thread has read
-          }
-          if constexpr (TERMS == 2)
+            if constexpr (TERMS == 1) {
+              tmem_st16(s_t + 16u * c, w);                 // over scores that this thread has read
+            } else if (step == 0) {
+              tmem_st16(s_t, w);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t w[16];
+              for (int j = 0; j < 16; ++j) keep[0][j] = low[j];
+            } else if (step == 1) {
+              tmem_st16(s_t + 64u, keep[0]);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) w[j] = low[16 * c + j];
-              tmem_st16(s_t + 64u + 16u * c, w);
+              for (int j = 0; j < 16; ++j) {
+                keep[1][j] = w[j];
+                keep[2][j] = low[j];
+              }
+            } else {
+              tmem_st16(s_t + 16u * c, w);
+              tmem_st16(s_t + 64u + 16u * c, low);
+              if (step == 2) tmem_st16(s_t + 32u, keep[1]);
+              else tmem_st16(s_t + 96u, keep[2]);
             }
+          }
           tmem_st_wait();
           tc_fence_before();
         }
