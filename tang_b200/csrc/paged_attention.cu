@@ -32,40 +32,39 @@ __device__ __forceinline__ int paged_row_of(const PagedParams& p, int b) {
 }
 // ---------------------------------------------------------------------------------------------
 // Units, tiles, items, pieces.  A unit is what meets the same keys: the rows (member, query head of one KV head) of up to 128 / group members of a group
-// over the group's shared positions, in whole tiles of 128, or one sequence's query heads over the rest.  The tiles of all units of a KV head stand in one
-// list, shared ones first, and are cut into items; CTAs, one an SM, take two items each and then the next one that nobody has, whatever
-// the lengths of the sequences and the speeds of the SMs.  (Items of all KV heads that stand at the same place of their lists follow one another: a cache
-// row holds all heads, and its 256 bytes a head are fetched at the same time.)  A piece is what an item has of a unit.  Its odd and its even tiles belong
-// to different softmax groups, which take scores from the same reference, so that the products of both go to the same columns (two sets of columns, for
-// pieces that follow one another).  It leaves a partial result; a second kernel joins those of a row, in the order of the list.
+// over the group's shared positions, in whole tiles of 128, or one sequence's query heads over the rest.  The tiles of all units of a KV head stand in
+// two lists, one of shared and one of own tiles, and every CTA, one an SM, takes an item of either: as many tiles of the one and of the other as everybody
+// else.  CTAs that stand at the same place of the KV heads' lists are neighbours: a cache row holds all heads, and its 256 bytes a head are fetched at the
+// same time.  A piece is what an item has of a unit.  Its odd and its even tiles belong to different softmax groups, which take scores from the same reference,
+// so that the products of both go to the same columns (two sets of columns, for pieces that follow one another).  It leaves a partial result; a second
+// kernel joins those of a row, in the order of the list.
+// (64 sequences of 4096 positions and 8 KV heads take PERF_ALONE.  One list of all heads' tiles, cut for 148 CTAs rather than 144, took 98 us.  Shorter items,
+// handed out as CTAs get to them because SMs differ in speed by a fifth, took 102: they make more partial results than they balance.)
 // ---------------------------------------------------------------------------------------------
 constexpr int kPuThreads = 416;
 constexpr int kPuTile = 4 * kPfBox / 2;               // bytes of 128 rows of keys or values
 constexpr int kPuRing = 5;
-constexpr int kPuWeights = 2 * 32 * 128;              // a parity's weights where keys are the lanes: 32 rows of 128 keys, in two halves
+constexpr int kPuWeights = 2 * 16 * 128;              // a parity's weights where keys are the lanes: two terms of eight rows of 128 keys, in two halves
 constexpr int kPuOnes = 1024;                         // eight rows of 64 ones
 constexpr int kPuMeet = (2 + 2) * 128 * 4;            // maxima [parity][warp][row], references [piece's parity][row, or warp and row]
 constexpr float kPuLargest = 7.9228162514264338e28f;  // 2^96: a weight above it is too far from its reference
 constexpr int kPuHeader = 640;                        // barriers, pieces
 constexpr int kPuReaders = 12;                        // warps that are told the pieces
 constexpr int kPuPieces = 4;                          // pieces that are told ahead
-constexpr int kPuLong = 3, kPuShort = 8;              // a CTA's items of own tiles: long ones, then short ones for the last quarter
+
 constexpr int kPuBatch = 1024;                        // sequences of a call
 constexpr size_t kPuFixed = 2 * (size_t)kPfBox + kPuRing * (size_t)kPuTile + 2 * (size_t)kPuWeights + kPuOnes + kPuMeet + kPuHeader;
 
-// How the tiles of a KV head's list are cut into items: shared ones in items of `pre`, own ones in `n_long` items of `len`, the rest in items of `tail`.
+// How many tiles of the lists an item has.
 struct PuCut {
-  int pre, len, n_long, tail;
+  int pre, own;
 };
-__device__ __forceinline__ int pu_own_item(const PuCut& c, int f) { return f < c.n_long * c.len ? f / c.len : c.n_long + (f - c.n_long * c.len) / c.tail; }
-__device__ __forceinline__ int pu_own_first(const PuCut& c, int item) { return item < c.n_long ? item * c.len : c.n_long * c.len + (item - c.n_long) * c.tail; }
 
 // In shared memory, behind the buffers.
 struct PuPlan {
   int *own, *last, *pre;                              // [batch + 1] own tiles of the sequences before; [batch] shared tiles << 8 | keys of the last tile - 1;
                                                       // [groups + 1] units' shared tiles of the groups before
-  int batch, groups, group, per_tile, pre_tiles, total;
-  int n_kv, pre_items, items;                         // items of shared tiles of a KV head, of all KV heads
+  int batch, groups, group, per_tile;
   PuCut cut;
 };
 // What the kernel that joins the pieces has to know: where a sequence's tiles stand in a KV head's list.
@@ -73,9 +72,7 @@ struct PuSeqPlan {
   int own_f, own_tiles, pre_f, pre_tiles;
 };
 struct PuUnit {
-  bool pre;
   int b0, head, rows, tiles, tile, shared_tiles, last;  // b0: (first) sequence of the batch; head: whose pages; tile: the asked one; last: keys of the last
-  int slot;                                           // first row of its partial results, without what KV head and item add
 };
 
 __device__ __forceinline__ int pu_group_start(const PagedParams& p, int g) { return min(max(p.group_starts[g], 0), p.batch); }
@@ -89,42 +86,35 @@ __device__ __forceinline__ int pu_last_not_above(const int* a, int n, int v) {  
   }
   return lo;
 }
-__device__ __forceinline__ PuUnit pu_locate(const PagedParams& p, const PuPlan& l, int f) {
+// Tile f of a KV head's shared (pre) or own tiles.
+__device__ __forceinline__ PuUnit pu_locate(const PagedParams& p, const PuPlan& l, bool pre, int f) {
   PuUnit u;
-  u.pre = f < l.pre_tiles;
-  if (u.pre) {
+  if (pre) {
     const int g = pu_last_not_above(l.pre, l.groups, f), start = pu_group_start(p, g), members = pu_group_end(p, g, start) - start;
     u.tiles = l.last[start] >> 8;
-    const int rest = f - l.pre[g], rt = rest / u.tiles;
+    const int rest = f - l.pre[g], rt = rest < u.tiles ? 0 : rest / u.tiles;
     u.tile = rest - rt * u.tiles;
     u.b0 = start + rt * l.per_tile;
     u.head = start;                    // the group's first member
     u.rows = min(l.per_tile, members - rt * l.per_tile) * l.group;
     u.shared_tiles = 0;
     u.last = kPfTile;
-    u.slot = u.b0 * l.group;
   } else {
-    const int h = f - l.pre_tiles, b = pu_last_not_above(l.own, l.batch, h);
+    const int b = pu_last_not_above(l.own, l.batch, f);
     u.tiles = l.own[b + 1] - l.own[b];
-    u.tile = h - l.own[b];
+    u.tile = f - l.own[b];
     u.b0 = u.head = b;
     u.rows = l.group;
     u.shared_tiles = l.last[b] >> 8;
     u.last = (l.last[b] & 255) + 1;
-    u.slot = b * l.group;
   }
   return u;
 }
-
-// Rows that are laid out for a unit whose keys are the tensor memory's lanes (0: its rows are), each as two terms but for the 32 of bf16 results.
-template <int TERMS>
-__device__ __forceinline__ int pu_wide(const PuUnit& u) { return u.rows <= 8 ? 8 : u.rows <= 16 ? 16 : u.rows <= 32 && TERMS == 1 ? 32 : 0; }
-
 // A piece as the roles are told of it, in shared memory.
 struct __align__(16) PuPiece {
   int n, tile, last, rows;                            // tiles (0: there are no more pieces), the first one's place in the sequence, keys of the last one, rows
   int kv, b0, seq, pre;                               // KV head, (first) sequence of the batch, its row of the tables, shared or not
-  int wide, out, pad[2];                              // layout, first row of its partial results
+  int keyed, out, pad[2];                             // the keys are the lanes; first row of its partial results
 };
 // Places in the ring, in the order in which they are needed: keys 0, keys 1, values 0, keys 2, values 1 ..
 __device__ __forceinline__ int pu_keys_at(int t) { return t == 0 ? 0 : 2 * t - 1; }
@@ -132,12 +122,10 @@ __device__ __forceinline__ int pu_values_at(int t) { return 2 * t + 2; }
 
 struct PuParams {
   PagedParams a;
-  int per_tile, per_quarter;                          // members of a row tile; of a row tile that fits 32 rows
-  int max_pre, max_own;                               // items of a KV head at most (own ones: what the plan's rule can make, which rounds up a few)
+  int per_tile, per_eight, n_items;                   // members of a row tile; of eight rows; items of a KV head's list
   float *own_o, *own_ml, *pre_o, *pre_ml;             // partial results: [row][128], [row][2] references and sums (of the groups)
   PuSeqPlan* plan;                                    // [batch]
   PuCut* cut;
-  int* counter;                                       // items handed out beyond the first two of every CTA; zero between calls
 };
 
 template <typename F>
@@ -178,7 +166,7 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
 
 template <int TERMS>
 __global__ void __launch_bounds__(kPuThreads, 1)
-paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_constant__ CUtensorMap q_quarter, const __grid_constant__ CUtensorMap q_whole,
+paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_constant__ CUtensorMap q_whole,
                     const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PuParams pp) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];   // (the swizzled buffers come first)
   const PagedParams& p = pp.a;
@@ -208,7 +196,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   l.batch = p.batch;
   l.group = p.group;
   l.per_tile = pp.per_tile;
-  l.n_kv = p.n_kv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
     if (lane == 0) {
@@ -239,7 +226,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     tmem_alloc(tmem_slot, 512);
   } else if (warp == 3) {
     if (lane == 0) {
-      prefetch_map(&q_own);
+      prefetch_map(&q_eight);
       prefetch_map(&k_map);
       prefetch_map(&v_map);
     }
@@ -290,19 +277,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  l.pre_tiles = l.pre[l.groups];
-  l.total = l.pre_tiles + l.own[p.batch];
-  const int own_tiles = l.own[p.batch];
-  l.cut.pre = max(1, (l.pre_tiles + pp.max_pre - 1) / pp.max_pre);
-  // Own tiles: one item a CTA where there are few.  Otherwise items of eight or more for three quarters, which keep partial results few, and items of two or
-  // more for the rest, which make up for the different speeds of the SMs (a fifth apart: their paths to memory differ).
-  const int share = (own_tiles + pp.max_pre - 1) / pp.max_pre;
-  l.cut.len = share < 12 ? max(1, share) : max(8, (3 * share + 4 * kPuLong - 1) / (4 * kPuLong));
-  l.cut.tail = max(2, (share + 4 * kPuShort - 1) / (4 * kPuShort));
-  l.cut.n_long = share < 12 ? (own_tiles + l.cut.len - 1) / l.cut.len : (int)(3ll * own_tiles / 4) / l.cut.len;
-  l.pre_items = (l.pre_tiles + l.cut.pre - 1) / l.cut.pre;
-  l.items = own_tiles - l.cut.n_long * l.cut.len;
-  l.items = (l.pre_items + l.cut.n_long + (l.items > 0 ? (l.items + l.cut.tail - 1) / l.cut.tail : 0)) * p.n_kv;
+  const int pre_tiles = l.pre[l.groups], own_tiles = l.own[p.batch];
+  l.cut.pre = max(1, (pre_tiles + pp.n_items - 1) / pp.n_items);
+  l.cut.own = max(1, (own_tiles + pp.n_items - 1) / pp.n_items);
   // One arrival for the warp.  The lanes meet before it and behind it: none may wait for what the arrival lets happen before it is made.
   auto arrive = [&](uint64_t* bar) {
     __syncwarp();
@@ -321,9 +298,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
   };
 
   if (warp == 12) {
-    // ---- what to do: the CTA's items, two that it has by its number, then the next one that nobody has (asked for while the one before is told), in pieces
-    const int n_ctas = (int)gridDim.x;
-    int item = (int)blockIdx.x, behind = item + n_ctas;
+    // ---- what to do: the CTA's two items, in pieces
     bool ok = true;
     auto tell = [&](const PuPiece& w) {
       const int slot = told % kPuPieces;
@@ -335,31 +310,28 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
       __syncwarp();
       ++told;
     };
+    const int item = (int)blockIdx.x / p.n_kv;
     PuPiece w{};
-    while (item < l.items && ok) {
-      const int coming = __shfl_sync(0xffffffffu, behind, 0);
-      if (coming < l.items && lane == 0) behind = 2 * n_ctas + atomicAdd(pp.counter, 1);
-      const int k = item / l.n_kv;
-      w.kv = item - k * l.n_kv;
-      w.pre = k < l.pre_items;
-      const int i = w.pre ? k : k - l.pre_items, own_f = w.pre ? 0 : pu_own_first(l.cut, i);
-      int f = w.pre ? i * l.cut.pre : l.pre_tiles + own_f;
-      const int end = w.pre ? min(f + l.cut.pre, l.pre_tiles) : min(f + (i < l.cut.n_long ? l.cut.len : l.cut.tail), l.total);
-      const int apart = w.pre ? 128 : 8;
+    w.kv = (int)blockIdx.x - item * p.n_kv;
+#pragma unroll 1
+    for (int k = 1; k >= 0 && ok; --k) {
+      const int len = k ? l.cut.pre : l.cut.own, apart = k ? 128 : 8;
+      int f = len * item;
+      const int end = min(f + len, k ? pre_tiles : own_tiles);
+      w.pre = k;
       while (f < end && ok) {
-        const PuUnit u = pu_locate(p, l, f);
+        const PuUnit u = pu_locate(p, l, k, f);
         w.n = min(end - f, u.tiles - u.tile);
         w.tile = u.shared_tiles + u.tile;
         w.last = u.tile + w.n == u.tiles ? u.last : kPfTile;
         w.rows = u.rows;
         w.b0 = u.b0;
         w.seq = max(paged_row_of(p, u.head), 0);
-        w.wide = pu_wide<TERMS>(u);
-        w.out = w.kv * (p.batch * p.group + apart * (w.pre ? pp.max_pre : pp.max_own)) + u.slot + apart * i;
+        w.keyed = u.rows <= 8;
+        w.out = w.kv * (p.batch * p.group + apart * pp.n_items) + u.b0 * p.group + apart * item;
         tell(w);
         f += w.n;
       }
-      item = coming;
     }
     w.n = 0;
     if (ok) tell(w);
@@ -390,11 +362,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
             q_used ^= 1u << k;
           }
         if (!ok) break;
-        const bool whole = w.wide == 0;
-        const uint32_t rows = (uint32_t)((whole ? pp.per_tile : w.pre ? pp.per_quarter : 1) * p.group);
+        const bool whole = !w.keyed;
+        const uint32_t rows = (uint32_t)((whole ? pp.per_tile : pp.per_eight) * p.group);
         if (lane == 0) mbar_arrive_expect_tx(&q_full[slot], 2u * rows * 128u);
         __syncwarp();
-        if (lane < 2) tma_load_3d(q_s + c * kPfBox + 16 * slot * 128, whole ? &q_whole : w.pre ? &q_quarter : &q_own, 64 * c, w.kv * p.group, w.b0, &q_full[slot]);
+        if (lane < 2) tma_load_3d(q_s + c * kPfBox + 16 * slot * 128, whole ? &q_whole : &q_eight, 64 * c, w.kv * p.group, w.b0, &q_full[slot]);
         __syncwarp();
       }
       for (int i = 0; i < w.n && ok; ++i, ++t) {
@@ -477,8 +449,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     int made[2] = {0, 0}, freed[2] = {0, 0};          // tiles of a parity so far, pieces of a parity
     bool ok = true;
     struct Tile {
-      int steps, wide;                                // 16-key steps, layout
-      bool first;                                     // of the piece
+      int steps;                                      // of 16 keys
+      bool keyed, first;                                     // of the piece
       int piece;                                      // its parity
     };
     auto values = [&](int t, const Tile& w) {
@@ -494,8 +466,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
       tc_fence_after();
       if (leader) {
         const uint64_t at = vd + (uint64_t)(slot * (kPuTile >> 4));
-        if (w.wide) {
-          const uint32_t idesc = umma_idesc_bf16(w.wide == 8 ? 16 : 32);
+        if (w.keyed) {
+          const uint32_t idesc = umma_idesc_bf16(16);
           for (int k = 0; k < w.steps; ++k) {
             const uint64_t wk = wd + (uint64_t)(x * (kPuWeights >> 4) + (k >> 2) * (kPuWeights >> 5) + 2 * (k & 3));
             umma_f16(o_t, at + (uint64_t)(k * (2048 >> 4)), wk, idesc | (1u << 15), !w.first || k != 0);
@@ -527,12 +499,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         if (!ok) break;
         tc_fence_after();
         const int keys = i == w.n - 1 ? w.last : kPfTile;
-        const Tile now{(keys + 15) >> 4, w.wide, i == 0, piece};
+        const Tile now{(keys + 15) >> 4, w.keyed != 0, i == 0, piece};
         if (leader) {
           const uint32_t s_t = tmem + (uint32_t)(x * 128);
-          const uint32_t idesc = umma_idesc_bf16(now.wide ? (now.wide == 32 ? 32 : 16) : kPfTile);
+          const uint32_t idesc = umma_idesc_bf16(now.keyed ? 16 : kPfTile);
           const uint64_t kt = kd + (uint64_t)(slot * (kPuTile >> 4)), qt = qd + (uint64_t)(q_slot * (16 * 128 >> 4));
-          const uint64_t da = now.wide ? kt : qt, db = now.wide ? qt : kt;
+          const uint64_t da = now.keyed ? kt : qt, db = now.keyed ? qt : kt;
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint64_t off = (uint64_t)((k >> 2) * (kPfBox >> 4) + 2 * (k & 3));
@@ -573,86 +545,57 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
     int done = 0;                      // tiles of this parity
     PuPiece u{};
     // a tile whose lanes are keys
-    auto keyed = [&](int wide, bool seen) {
+    auto keyed = [&](bool seen) {
+      float v[8];
+      __syncwarp();
+      tmem_ld8(s_t, v);
       if (first && leads) {
         float mine = -FLT_MAX;
-#pragma unroll 1
-        for (int i = 0; 8 * i < u.rows; ++i) {
-          float v[8];
-          __syncwarp();
-          tmem_ld8(s_t + 8u * i, v);
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            const float mx = redux_max(seen ? v[r] : -FLT_MAX);
-            if (lane == 8 * i + r) mine = mx;
-          }
-        }
-        max_s[t128] = mine;
-        meet();
-        const float mx = fmaxf(fmaxf(max_s[lane], max_s[32 + lane]), fmaxf(max_s[64 + lane], max_s[96 + lane]));
-        ref_s[t128] = mx == -FLT_MAX ? mx : mx * p.scale_log2;         // (a copy for every warp)
-        arrive(&ref_full[slot]);
-      }
-      if (first) ref = ref_s[t128];
-      const float* refs = ref_s + 32 * q4;
-      uint8_t* at = w_s + x * kPuWeights + (t128 >> 6) * (kPuWeights / 2) + 2 * (t128 & 7);
-      const int chunk = (t128 & 63) >> 3;
-#pragma unroll 1
-      for (int i = 0; 8 * i < u.rows; ++i) {
-        float v[8];
-        __syncwarp();
-        tmem_ld8(s_t + 8u * i, v);
-        const float4 f0 = *reinterpret_cast<const float4*>(&refs[8 * i]), f1 = *reinterpret_cast<const float4*>(&refs[8 * i + 4]);
-        const float from[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
-        // (rows behind the last one have columns and places too, which nobody reads: without branches the eight go side by side)
-        float w[8];
-        __nv_bfloat16 hi[8];
-        uint8_t* row = at + i * 1024;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          const float e = ex2(fmaf(v[r], p.scale_log2, -from[r]));
-          w[r] = !seen ? 0.f : e > kPuLargest ? NAN : e;
-          hi[r] = __float2bfloat16_rn(w[r]);
+          const float mx = redux_max(seen ? v[r] : -FLT_MAX);
+          if (lane == r) mine = mx;
         }
+        if (lane < 8) max_s[8 * q4 + lane] = mine;
+        meet();
+        const int r = lane & 7;
+        const float mx = fmaxf(fmaxf(max_s[r], max_s[8 + r]), fmaxf(max_s[16 + r], max_s[24 + r]));
+        if (lane < 8) ref_s[8 * q4 + lane] = mx == -FLT_MAX ? mx : mx * p.scale_log2;      // (a copy for every warp)
+        arrive(&ref_full[slot]);
+      }
+      const float4 f0 = *reinterpret_cast<const float4*>(&ref_s[8 * q4]), f1 = *reinterpret_cast<const float4*>(&ref_s[8 * q4 + 4]);
+      if (first) ref = ref_s[8 * q4 + (lane & 7)];
+      const float from[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+      // (rows behind the last one have columns and places too, which nobody reads: without branches the eight go side by side)
+      uint8_t* at = w_s + x * kPuWeights + (t128 >> 6) * (kPuWeights / 2) + 2 * (t128 & 7);
+      const int chunk = (t128 & 63) >> 3;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) *reinterpret_cast<__nv_bfloat16*>(row + r * 128 + ((chunk ^ r) << 4)) = hi[r];
-        if (wide < 32) {
-          row += wide * 128;
-#pragma unroll
-          for (int r = 0; r < 8; ++r) *reinterpret_cast<__nv_bfloat16*>(row + r * 128 + ((chunk ^ r) << 4)) = __float2bfloat16_rn(w[r] - __bfloat162float(hi[r]));
-        }
+      for (int r = 0; r < 8; ++r) {
+        const float e = ex2(fmaf(v[r], p.scale_log2, -from[r])), w = !seen ? 0.f : e > kPuLargest ? NAN : e;
+        const __nv_bfloat16 hi = __float2bfloat16_rn(w);
+        uint8_t* to = at + r * 128 + ((chunk ^ r) << 4);
+        *reinterpret_cast<__nv_bfloat16*>(to) = hi;
+        *reinterpret_cast<__nv_bfloat16*>(to + 1024) = __float2bfloat16_rn(w - __bfloat162float(hi));
       }
       tc_fence_before();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     };
-    auto keyed_out = [&](int wide, float* to_o, float* to_ml) {
-#pragma unroll 1
-      for (int i = 0; 8 * i < u.rows; ++i) {
-        float o[8], l8[8];
-        __syncwarp();
-        tmem_ld8(o_t + 8u * i, o);
-        tmem_ld8(o_t + 64u + 8u * i, l8);
-        if (wide < 32) {
-          float w[8];
-          tmem_ld8(o_t + (uint32_t)wide + 8u * i, w);
-#pragma unroll
-          for (int r = 0; r < 8; ++r) o[r] += w[r];
-          tmem_ld8(o_t + 64u + (uint32_t)wide + 8u * i, w);
-#pragma unroll
-          for (int r = 0; r < 8; ++r) l8[r] += w[r];
-        }
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          if (8 * i + r < u.rows) to_o[(size_t)(8 * i + r) * kPaDim + t128] = o[r];
-        }
-        float sum = l8[0];
-#pragma unroll
-        for (int r = 1; r < 8; ++r) sum = (lane & 7) == r ? l8[r] : sum;
-        // (a row's reference is in the lane of its number)
-        if (q4 == 0 && (lane >> 3) == i && lane < u.rows) *reinterpret_cast<float4*>(to_ml + lane * 4) = make_float4(ref, sum, ref, 0.f);
-      }
+    auto keyed_out = [&](float* to_o, float* to_ml) {
+      float o[8], low[8], sum[8], sum_low[8];
+      __syncwarp();
+      tmem_ld8(o_t, o);
+      tmem_ld8(o_t + 8u, low);
+      tmem_ld8(o_t + 64u, sum);
+      tmem_ld8(o_t + 72u, sum_low);
       tc_fence_before();
       arrive(&o_free[slot]);                           // (the products of the piece after the next may begin)
+      float l = 0.f;                                   // of the lane's row
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        if (r < u.rows) to_o[r * kPaDim + t128] = o[r] + low[r];
+        if (lane == r) l = sum[r] + sum_low[r];
+      }
+      if (q4 == 0 && lane < u.rows) *reinterpret_cast<float4*>(to_ml + lane * 4) = make_float4(ref, l, ref, 0.f);
     };
     int t0 = 0, piece = 0;             // tiles and pieces before the piece
     for (take(ok, u); u.n && ok; t0 += u.n, ++piece, take(ok, u)) {
@@ -664,13 +607,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
       float *to_o = (u.pre ? pp.pre_o : pp.own_o) + (size_t)u.out * kPaDim, *to_ml = (u.pre ? pp.pre_ml : pp.own_ml) + (size_t)u.out * 4;
       for (int i = place; i < u.n && ok; i += 2) {
         first = i == place;
-        const int wide = u.wide, r = 32 * q4 + lane;
+        const int r = 32 * q4 + lane;
         const bool live = r < u.rows;
         ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[x], (uint32_t)(done & 1)) && (!first || leads || mbar_wait_spin(&ref_full[slot], (uint32_t)((piece >> 1) & 1))));
         if (!ok) break;
         tc_fence_after();
-        if (wide) {
-          keyed(wide, t128 < (i == u.n - 1 ? u.last : kPfTile));
+        if (u.keyed) {
+          keyed(t128 < (i == u.n - 1 ? u.last : kPfTile));
         } else {
           __syncwarp();
           if (first && leads) {
@@ -734,7 +677,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         arrive(&p_full[x]);
         ++done;
         // (a sum each of the two groups; a piece of one tile has one)
-        if (!wide && live && i + 2 >= u.n) {
+        if (!u.keyed && live && i + 2 >= u.n) {
           const float2 ml = make_float2(ref, sum_all > kPuLargest ? NAN : sum_all);
           if (u.n > 1) *reinterpret_cast<float2*>(to_ml + r * 4 + 2 * place) = ml;
           else *reinterpret_cast<float4*>(to_ml + r * 4) = make_float4(ml.x, ml.y, ml.x, 0.f);
@@ -745,8 +688,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_own, const __grid_cons
         ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[x], (uint32_t)((done - 1) & 1)));
         if (!ok) break;
         tc_fence_after();
-        if (wide) {
-          keyed_out(wide, to_o, to_ml);
+        if (u.keyed) {
+          keyed_out(to_o, to_ml);
         } else {
 #pragma unroll 1
           for (int c = 0; c < kPaDim; c += 32) {
@@ -782,10 +725,10 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
   const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const PuSeqPlan q = pp.plan[b];
   const PuCut cut = *pp.cut;
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *pp.counter = 0;
   const int kv = head / p.group, h = head - kv * p.group;
-  const int own_e = q.own_f + q.own_tiles, pre_e = q.pre_f + q.pre_tiles, own_c = pu_own_item(cut, q.own_f), pre_c = q.pre_f / cut.pre;
-  const int own = q.own_tiles ? pu_own_item(cut, own_e - 1) - own_c + 1 : 0, pre = q.pre_tiles ? (pre_e - 1) / cut.pre - pre_c + 1 : 0;
+  // items of the row's own and shared tiles
+  const int own_c = q.own_f / cut.own, pre_c = q.pre_f / cut.pre;
+  const int own = q.own_tiles ? (q.own_f + q.own_tiles - 1) / cut.own - own_c + 1 : 0, pre = q.pre_tiles ? (q.pre_f + q.pre_tiles - 1) / cut.pre - pre_c + 1 : 0;
   float top = -FLT_MAX, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int base = 0; base < own + pre; base += 32) {
     // a lane per partial result: its row, reference and sums
@@ -794,8 +737,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
     float4 mine = make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
     if (i < own + pre) {
       const bool k = i >= own;
-      const int item = k ? pre_c + i - own : own_c + i, apart = k ? 128 : 8, most = k ? pp.max_pre : pp.max_own;
-      const size_t r = (size_t)kv * (p.batch * p.group + apart * most) + b * p.group + h + (size_t)apart * item;
+      const int item = k ? pre_c + i - own : own_c + i, apart = k ? 128 : 8;
+      const size_t r = (size_t)kv * (p.batch * p.group + apart * pp.n_items) + b * p.group + h + (size_t)apart * item;
       row = (k ? pp.pre_o : pp.own_o) + r * kPaDim;
       mine = *reinterpret_cast<const float4*>((k ? pp.pre_ml : pp.own_ml) + r * 4);
     }
@@ -909,16 +852,14 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   p.err = ctx->dev_err;
   PuParams pp;
   pp.per_tile = 128 / p.group;
-  pp.per_quarter = 32 / p.group;
+  pp.per_eight = 8 / p.group;
   const size_t tiles = batch * (((size_t)p.max_len + kPfTile - 1) / kPfTile) * n_kv_heads;
   TQ_REQUIRE(ctx, tiles < (1ull << 30) && (size_t)p.n_pages * pages->page_rows < (1ull << 31), "tq_gqa_decode_paged: too many positions");
-  const size_t n_ctas = tiles < (size_t)ctx->sm_count ? tiles : (size_t)ctx->sm_count;
-  // A CTA takes one item of shared tiles (whose partial results are many rows) and several of the others, if there are as many tiles.
-  const size_t per_kv = (size_t)ctx->sm_count / n_kv_heads > 0 ? (size_t)ctx->sm_count / n_kv_heads : 1;
-  pp.max_pre = (int)per_kv;
-  pp.max_own = (int)((kPuLong + kPuShort) * per_kv + 8);
+  const size_t most_ctas = tiles < (size_t)ctx->sm_count ? tiles : (size_t)ctx->sm_count;
+  pp.n_items = (int)(most_ctas > n_kv_heads ? most_ctas / n_kv_heads : 1);
+  const size_t n_ctas = pp.n_items * n_kv_heads;
   // partial results, the sequences' plans
-  const size_t own_rows = batch * n_heads + 8 * n_kv_heads * pp.max_own, pre_rows = p.n_groups ? batch * n_heads + 128 * n_kv_heads * pp.max_pre : 0;
+  const size_t own_rows = batch * n_heads + 8 * n_ctas, pre_rows = p.n_groups ? batch * n_heads + 128 * n_ctas : 0;
   const size_t floats = (own_rows + pre_rows) * (kPaDim + 4);
   if (int st = ensure_scratch(ctx, floats * sizeof(float) + (batch + 1) * sizeof(PuSeqPlan))) return st;
   pp.own_o = static_cast<float*>(ctx->scratch);
@@ -927,19 +868,18 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   pp.pre_ml = pp.own_ml + own_rows * 4;
   pp.plan = reinterpret_cast<PuSeqPlan*>(pp.pre_ml + pre_rows * 4);
   pp.cut = reinterpret_cast<PuCut*>(pp.plan + batch);
-  pp.counter = ctx->dev_err + kTileCounters;          // (the last of the counters)
   pp.a = p;
-  CUtensorMap qo, qq, qw, km, vm;
+  CUtensorMap qe, qw, km, vm;
   const size_t row = n_kv_heads * kPaDim, rows = (size_t)p.n_pages * pages->page_rows;
   const unsigned g = (unsigned)p.group, box = pages->page_rows < kPfTile ? (unsigned)pages->page_rows : (unsigned)kPfTile;
   auto q_map = [&](CUtensorMap* m, int members) { return encode_bf16_boxes(m, q_dev, kPaDim, n_heads, batch, kPaDim * 2, n_heads * kPaDim * 2, g, (unsigned)members); };
-  if (!q_map(&qo, 1) || !q_map(&qq, pp.per_quarter) || !q_map(&qw, pp.per_tile) || !encode_pages(&km, k_pages_dev, row, rows, box) ||
+  if (!q_map(&qe, pp.per_eight) || !q_map(&qw, pp.per_tile) || !encode_pages(&km, k_pages_dev, row, rows, box) ||
       !encode_pages(&vm, v_pages_dev, row, rows, box))
     return fail(ctx, TQ_ECUDA, "cuTensorMapEncodeTiled failed");
   const size_t smem = kPuFixed + (2 * batch + 1 + (size_t)p.n_groups + 1) * sizeof(int);
   auto kern = p.out_f32 ? paged_decode_kernel<2> : paged_decode_kernel<1>;
   TQ_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kPuFixed + (3 * kPuBatch + 2) * sizeof(int))));
-  TQ_CUDA(ctx, launch_k(ctx, kern, dim3((unsigned)n_ctas), dim3(kPuThreads), smem, qo, qq, qw, km, vm, pp));
+  TQ_CUDA(ctx, launch_k(ctx, kern, dim3((unsigned)n_ctas), dim3(kPuThreads), smem, qe, qw, km, vm, pp));
   TQ_CUDA(ctx, launch_k(ctx, paged_join_kernel, dim3((unsigned)n_heads, (unsigned)batch), dim3(128), 0, pp));
   return TQ_OK;
 }
