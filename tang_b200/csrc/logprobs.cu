@@ -73,6 +73,38 @@ __device__ __forceinline__ float lp_ex2(float x) {
   return y;
 }
 
+// Two f32 operations of one instruction.
+__device__ __forceinline__ unsigned long long lp_pair(float x, float y) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1,%2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 lp_split(unsigned long long v) {
+  float2 r;
+  asm("mov.b64 {%0,%1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ unsigned long long lp_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long lp_add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// The largest of 16 bytes of logits (NaN is none of them); bf16 by pairs.
+__device__ __forceinline__ float lp_largest(const uint4& v, float) {
+  return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+}
+__device__ __forceinline__ float lp_largest(const uint4& v, __nv_bfloat16) {
+  const __nv_bfloat162 a = __hmax2(__hmax2(reinterpret_cast<const __nv_bfloat162&>(v.x), reinterpret_cast<const __nv_bfloat162&>(v.y)),
+                                   __hmax2(reinterpret_cast<const __nv_bfloat162&>(v.z), reinterpret_cast<const __nv_bfloat162&>(v.w)));
+  return fmaxf(__low2float(a), __high2float(a));
+}
+
 // Larger for a larger logit and, among equals (the zeros too), for a lower index; 0 is nobody's.
 __device__ __forceinline__ unsigned long long lp_key(float v, int i) {
   const uint32_t b = __float_as_uint(v + 0.f);
@@ -106,29 +138,22 @@ struct LpState {
 // The 16 bytes with the thread's largest logit are held back: the row's largest must not be added before it is known (the sum of the others would be
 // lost against it where a model is sure).  Where another vector has the same one, that is among s, which is no loss there.
 constexpr float kLpSlack = 20.f;
-template <typename T, bool ENT>
+template <typename T, bool ENT, bool TOP>
 struct LpRunning {
   static constexpr int N = 16 / (int)sizeof(T);
   static constexpr uint32_t kNone = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;        // -infinity
-  float b = -INFINITY, base = 0.f, off = 0.f, s = 0.f, u = 0.f;        // u: sum of exponent * exponential
+  float b = -INFINITY, base = 0.f, off = 0.f;
+  unsigned long long s = 0, u = 0;                      // two sums each, of even and of odd places; u: of exponent * exponential
   float mine = -INFINITY, second = -INFINITY;                      // the largest of `held` and of all other vectors
   uint4 held = make_uint4(kNone, kNone, kNone, kNone);
   int where = -1;                                       // the row's place of its first logit (-1: not 16 bytes of the row)
 
   static __device__ __forceinline__ uint4 none() { return make_uint4(kNone, kNone, kNone, kNone); }
-  static __device__ __forceinline__ float largest(const uint4& v) {
-    float x[N];
-    lp_unpack(v, x, T());
-    float mx = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
-    return mx;
-  }
   __device__ __forceinline__ bool far() const { return !(fabsf(b) <= 1048576.f); }
-  __device__ __forceinline__ void take(float a) {
-    const float e = lp_ex2(a);
-    s += e;
-    if (ENT) u = fmaf(fmaxf(a, -1e4f), e, u);           // (e is 0 there, and -infinity times that is not)
+  __device__ __forceinline__ void take(float a0, float a1) {
+    const unsigned long long e = lp_pair(lp_ex2(a0), lp_ex2(a1));
+    s = lp_add2(s, e);
+    if (ENT) u = lp_fma2(lp_pair(fmaxf(a0, -1e4f), fmaxf(a1, -1e4f)), e, u);             // (e is 0 there, and -infinity times that is not)
   }
   // K vectors, the first of them at place `at` of the row and the others `step` apart (-1: nowhere)
   template <int K>
@@ -136,15 +161,15 @@ struct LpRunning {
     float top = -INFINITY;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const float mx = largest(v[k]);
+      const float mx = lp_largest(v[k], T());
       top = fmaxf(top, mx);
-      second = fmaxf(second, fminf(mx, mine));
+      if (TOP) second = fmaxf(second, fminf(mx, mine));
       if (mx > mine) {                                  // (selects, no branch)
         const uint4 w = held;
         held = v[k];
         v[k] = w;
         mine = mx;
-        where = at < 0 ? -1 : at + k * step;
+        if (TOP) where = at < 0 ? -1 : at + k * step;
       }
     }
     if (__any_sync(0xffffffffu, top > b + kLpSlack)) {
@@ -154,8 +179,9 @@ struct LpRunning {
       off = far() ? 0.f : fmaf(b, kLpLog2e, -base);
       if (was != -INFINITY) {
         const float by = fmaxf((was - b) * kLpLog2e - off_was + off, -1e4f), f = lp_ex2(by);
-        if (ENT) u = fmaf(by, s, u) * f;
-        s *= f;
+        const unsigned long long f2 = lp_pair(f, f);
+        if (ENT) u = lp_fma2(lp_fma2(lp_pair(by, by), s, u), f2, 0ull);
+        s = lp_fma2(s, f2, 0ull);
       }
     }
     if (!far()) {
@@ -164,7 +190,10 @@ struct LpRunning {
         float x[N];
         lp_unpack(v[k], x, T());
 #pragma unroll
-        for (int i = 0; i < N; ++i) take(fmaf(x[i], kLpLog2e, -base));
+        for (int i = 0; i < N; i += 2) {
+          const float2 a = lp_split(lp_fma2(lp_pair(x[i], x[i + 1]), lp_pair(kLpLog2e, kLpLog2e), lp_pair(-base, -base)));
+          take(a.x, a.y);
+        }
       }
     } else {
 #pragma unroll
@@ -172,7 +201,8 @@ struct LpRunning {
         float x[N];
         lp_unpack(v[k], x, T());
 #pragma unroll
-        for (int i = 0; i < N; ++i) take(x[i] == -INFINITY ? -INFINITY : (x[i] - b) * kLpLog2e);
+        for (int i = 0; i < N; i += 2)
+          take(x[i] == -INFINITY ? -INFINITY : (x[i] - b) * kLpLog2e, x[i + 1] == -INFINITY ? -INFINITY : (x[i + 1] - b) * kLpLog2e);
       }
     }
   }
@@ -181,8 +211,10 @@ struct LpRunning {
     LpState r;
     r.m = m;
     const float by = b == -INFINITY ? 0.f : fmaxf((b - m) * kLpLog2e - off, -1e4f), f = lp_ex2(by);
-    r.s = s * f;
-    if (ENT) r.u = -fmaf(by, s, u) * f * 0.693147180559945309f;
+    const float2 s2 = lp_split(s), u2 = lp_split(u);
+    const float sum = s2.x + s2.y;
+    r.s = sum * f;
+    if (ENT) r.u = -fmaf(by, sum, u2.x + u2.y) * f * 0.693147180559945309f;
     float x[N];
     lp_unpack(held, x, T());
 #pragma unroll
@@ -213,7 +245,7 @@ struct LpSegment {
   }
 };
 
-template <typename T, bool ENT>
+template <typename T, bool ENT, bool TOP>
 __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(const LogprobParams p) {
   constexpr int N = LpSegment<T>::N;
   __shared__ float red[4][kLpWarps];
@@ -231,7 +263,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
   pdl_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int row = (int)(blockIdx.x / C), t = threadIdx.x, warp = t >> 5, lane = t & 31, V = p.slices * p.cols, top = p.top;
+  const int row = (int)(blockIdx.x / C), t = threadIdx.x, warp = t >> 5, lane = t & 31, V = p.slices * p.cols, top = TOP ? p.top : 0;
   const int lo = (int)((long long)V * rank / C) & ~63, hi = rank == C - 1 ? V : (int)((long long)V * (rank + 1) / C) & ~63;
   int token = -1;
   float token_x = 0.f;
@@ -241,7 +273,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
   }
 
   // ---- one pass: maximum and sums of this thread's elements
-  LpRunning<T, ENT> sums;
+  LpRunning<T, ENT, TOP> sums;
   for (int at = lo; at < hi;) {
     const int sl = at / p.cols, in = at - sl * p.cols, n = min(hi - at, p.cols - in);
     const LpSegment<T> g(lp_slice<T>(p, row, sl) + in, n);
@@ -560,8 +592,12 @@ extern "C" int tq_token_logprobs(tq_ctx* ctx, const void* logits_dev, int dtype,
   size_t C = slots / rows < V / 2048 ? slots / rows : V / 2048;
   C = C < 1 ? 1 : C > (size_t)kLpMaxCluster ? (size_t)kLpMaxCluster : C;
   const bool ent = entropy_out_dev != nullptr;
-  auto kern = dtype == TQ_BF16 ? (ent ? token_logprobs_kernel<__nv_bfloat16, true> : token_logprobs_kernel<__nv_bfloat16, false>)
-                               : (ent ? token_logprobs_kernel<float, true> : token_logprobs_kernel<float, false>);
+  using bf = __nv_bfloat16;
+  void (*kern)(LogprobParams);
+  if (top) kern = dtype == TQ_BF16 ? (ent ? token_logprobs_kernel<bf, true, true> : token_logprobs_kernel<bf, false, true>)
+                                   : (ent ? token_logprobs_kernel<float, true, true> : token_logprobs_kernel<float, false, true>);
+  else kern = dtype == TQ_BF16 ? (ent ? token_logprobs_kernel<bf, true, false> : token_logprobs_kernel<bf, false, false>)
+                               : (ent ? token_logprobs_kernel<float, true, false> : token_logprobs_kernel<float, false, false>);
   TQ_REQUIRE(ctx, rows < (size_t)(0x7fffffff / kLpMaxCluster), "tq_token_logprobs: too many rows");
   TQ_CUDA(ctx, launch_k_cluster(ctx, kern, dim3((unsigned)(rows * C)), dim3(kLpThreads), 0, dim3((unsigned)C), p));
   return TQ_OK;

@@ -38,8 +38,14 @@ __device__ __forceinline__ int paged_row_of(const PagedParams& p, int b) {
 // same time.  A piece is what an item has of a unit.  Its odd and its even tiles belong to different softmax groups, which take scores from the same reference,
 // so that the products of both go to the same columns (two sets of columns, for pieces that follow one another).  It leaves a partial result; a second
 // kernel joins those of a row, in the order of the list.
-// (64 sequences of 4096 positions and 8 KV heads take PERF_ALONE.  One list of all heads' tiles, cut for 148 CTAs rather than 144, took 98 us.  Shorter items,
+// (64 sequences of 2048 positions and 8 KV heads take 97 us.  One list of all heads' tiles, cut for 148 CTAs rather than 144, took 98 us.  Shorter items,
 // handed out as CTAs get to them because SMs differ in speed by a fifth, took 102: they make more partial results than they balance.)
+//
+// What bounds it: the bytes of the cache, once, where sequences are long (537 MB in 97 us, 5.5 TB/s; the steady state is 2800 cycles for a tile of 64 KB,
+// which is an SM's share of the memory's rate); beside them a start of 5 us (lengths, plan, first pages, first tile: six loads in a row) and 4 us until the
+// second kernel is through, which are most of a small call (one sequence of 700 positions 8.9 us, 8 samples of a prompt of 2040 16.7).  A shared tile of
+// 128 rows is 2000 cycles: two products of 670 each, of two softmax groups in turn, and 64 KB from L2 (64 samples of a prompt of 8192: 42 us, of which the
+// shared part is 11).
 // ---------------------------------------------------------------------------------------------
 constexpr int kPuThreads = 416;
 constexpr int kPuTile = 4 * kPfBox / 2;               // bytes of 128 rows of keys or values
@@ -51,7 +57,6 @@ constexpr float kPuLargest = 7.9228162514264338e28f;  // 2^96: a weight above it
 constexpr int kPuHeader = 640;                        // barriers, pieces
 constexpr int kPuReaders = 12;                        // warps that are told the pieces
 constexpr int kPuPieces = 4;                          // pieces that are told ahead
-
 constexpr int kPuBatch = 1024;                        // sequences of a call
 constexpr size_t kPuFixed = 2 * (size_t)kPfBox + kPuRing * (size_t)kPuTile + 2 * (size_t)kPuWeights + kPuOnes + kPuMeet + kPuHeader;
 
@@ -524,16 +529,20 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
     if (ok && t > 0) ok = values(t - 1, before);
     if (!ok) give_up(DERR_FULL_WAIT);
   } else if (warp >= 4) {
-    // ---- softmax of the tiles of a parity.  More than 32 rows: S = Q K^T, a thread per row, the weights over the scores' columns.  Up to 32: the keys are
-    // the tensor memory's lanes, S^T = K Q^T and O^T = V^T P, with as many columns as there are rows (a product of 128 x 128 x 16 takes 84 cycles for four
-    // rows too, one of 128 x 16 x 16 a fraction): a thread per key, whose weights go to shared memory, each as two bf16 terms in rows of their own.
-    // The weights' sums come from a product with ones.
-    // The reference that scores are taken from is their maximum in the piece's first tile, which the group with that tile tells the other one: a bf16 weight may be as large as an f32 one, so that
-    // nothing is rescaled; a weight above 2^96 becomes no number, and the joining kernel goes through the row's keys one by one.
+    // ---- softmax of the tiles of a parity.  More than eight rows: S = Q K^T, a thread per row, the weights over the scores' columns.  Up to eight: the keys
+    // are the tensor memory's lanes, S^T = K Q^T and O^T = V^T P with 16 columns (a product of 128 x 128 x 16 takes 84 cycles for four rows too, one of
+    // 128 x 16 x 16 a fraction): a thread per key, whose weights go to shared memory, and the weights' sums come from a product with ones.  (Both ways for 9
+    // to 32 rows: 16 groups of four samples 41.8 us with keys as lanes and 42.4 with rows, 64 samples by fours 71.6 and 70.4.)
+    // A weight is two bf16 terms, hi + lo, where keys are the lanes and where results are f32: within 2^-18 of it.  (Three would be nearer to f32 results,
+    // whose error from 64 bits is 2e-6 so and 8e-7 by f32 arithmetic, but tensor memory has no columns for them.)  One term, within 2^-9 like the rounding
+    // of the result, where rows are the lanes and results are bf16.
+    // The reference that scores are taken from is their maximum in the piece's first tile, which the group with that tile tells the other one: a bf16 weight
+    // may be as large as an f32 one, so that nothing is rescaled; a weight above 2^96 becomes no number, and the joining kernel goes through the row's keys
+    // one by one.
     const int x = (warp - 4) >> 2, q4 = warp & 3, t128 = 32 * q4 + lane;
     const uint32_t s_t = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)(x * 128);
     uint32_t o_t = 0;                  // of the piece
-    float *max_s = meet_s + x * 128, *ref_s = nullptr;                 // [warp][32 rows]; the piece's references
+    float *max_s = meet_s + x * 128, *ref_s = nullptr;                 // [warp][8 rows]; the piece's references
     int meetings = 0;
     bool ok = true, first = true, leads = true;      // the group's first tile of the piece; it is the piece's first
     int slot = 0;                      // the piece's parity
