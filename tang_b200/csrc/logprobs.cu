@@ -4,6 +4,10 @@
 // With m the largest logit, c how many logits equal it and s the sum of exp(x - m) over the others,
 //     log sum exp x = m + log c + log1p(s / c),      H = log c + log1p(s / c) + sum (m - x) exp(x - m) / (c + s),
 // so that a model that is sure of a token (log probability and entropy near zero) loses nothing to the addition of the leading one.
+//
+// What bounds it: the logits' bytes where rows are many (1024 x 128256 f32 79.5 us, 6.6 TB/s; as many bytes of bf16 91 us, 5.8 TB/s, with four fifths of
+// the issue slots taken: an exponential, a share of a maximum and half an addition and multiplication for every logit); the latency of the launch, the
+// cluster's meeting and, with alternatives, of sorting 128 maxima where they are few (one row of 32000 4.3 us, 7.1 with five alternatives).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -231,7 +235,7 @@ struct LpRunning {
   }
 };
 
-// The elements first .. end-1 of a segment that this thread takes: up to one before the first 16-byte boundary, every 512th 16 bytes, up to one
+// The elements first .. end-1 of a segment that this thread takes: up to one before the first 16-byte boundary, every 256th 16 bytes, up to one
 // behind the last.
 template <typename T>
 struct LpSegment {
@@ -308,7 +312,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
     const float m = warp_max(mine);
     if (lane == 0) red[0][warp] = m;
   }
-  if (top) {
+  if constexpr (TOP) {
     float g = mine;
 #pragma unroll
     for (int o = 1; o < kLpThreads / kLpGroups; o *= 2) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
@@ -334,7 +338,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
 
   // ---- the CTA's `top` largest.  The top-th largest of the 128 groups' maxima is a lower bound of the top-th largest element: few elements are above
   // it, and only the threads whose own maximum reaches it have any.
-  if (top) {
+  if constexpr (TOP) {
     if (t >= kLpThreads - kLpGroups) {
       // every warp sorts 32 maxima, largest first; a maximum's rank is its place there and how many of the other three lists are before it
       const int me = t - (kLpThreads - kLpGroups), w = me >> 5;
@@ -526,7 +530,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
       const int tok = p.tokens[(size_t)row * p.n_tokens + j];
       p.logprob[(size_t)row * p.n_tokens + j] = tok < 0 ? 0.f : tok >= V ? NAN : logprob(lp_at<T>(p, row, tok));
     }
-    if (top) {
+    if constexpr (TOP) {
       // place k of the row, a key or nobody's
       auto put = [&](int k, unsigned long long key) {
         p.top_ids[(size_t)row * top + k] = key ? lp_key_index(key) : -1;
@@ -586,8 +590,9 @@ extern "C" int tq_token_logprobs(tq_ctx* ctx, const void* logits_dev, int dtype,
   p.top_ids = top_ids_out_dev;
   p.top_logprob = top_logprob_out_dev;
   // CTAs of a row (a cluster): as many as fit the GPU at once (four an SM), none with less than 2048 logits.  More, smaller ones cost more than they
-  // balance, fewer leave SMs idle; us for one, two, four, eight: 64 rows of 128256 f32 23.7, 14.8, 10.6, 10.2, 256 rows 28.0, 23.7, 27.5, 33.9,
-  // one row of 32000 6.7, 5.5, 4.6, 4.4.
+  // balance, fewer leave SMs idle; us for one, two, four, eight: 64 rows of 128256 f32 23.7, 14.6, 10.3, 9.8, 256 rows 27.5, 22.3, 26.1, 33.0,
+  // one row of 32000 6.5, 5.2, 4.6, 4.3.  Forms without alternatives or entropies leave their bookkeeping out of the loop: 2048 rows of 128256 bf16
+  // 91 us, 98 with entropies, 108 with 20 alternatives, 122 with both.
   const size_t V = slices * cols, slots = (size_t)ctx->sm_count * kLpPerSm;
   size_t C = slots / rows < V / 2048 ? slots / rows : V / 2048;
   C = C < 1 ? 1 : C > (size_t)kLpMaxCluster ? (size_t)kLpMaxCluster : C;
