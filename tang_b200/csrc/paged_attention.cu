@@ -33,8 +33,8 @@ __device__ __forceinline__ int paged_row_of(const PagedParams& p, int b) {
 // ---------------------------------------------------------------------------------------------
 // Units, tiles, items, pieces.  A unit is what meets the same keys: the rows (member, query head of one KV head) of up to 128 / group members of a group
 // over the group's shared positions, in whole tiles of 128, or one sequence's query heads over the rest.  The tiles of all units of a KV head stand in
-// two lists, one of shared and one of own tiles, and every CTA, one an SM, takes an item of either: as many tiles of the one and of the other as everybody
-// else.  CTAs that stand at the same place of the KV heads' lists are neighbours: a cache row holds all heads, and its 256 bytes a head are fetched at the
+// two lists, one of shared and one of own tiles, and every CTA, one an SM, takes a share of either: as many tiles of the one and of the other as everybody
+// else.  A long share is cut into items (kPuWindow).  CTAs that stand at the same place of the KV heads' lists are neighbours: a cache row holds all heads, and its 256 bytes a head are fetched at the
 // same time.  A piece is what an item has of a unit.  Its odd and its even tiles belong to different softmax groups, which take scores from the same reference,
 // so that the products of both go to the same columns (two sets of columns, for pieces that follow one another).  It leaves a partial result; a second
 // kernel joins those of a row, in the order of the list.
@@ -57,12 +57,21 @@ constexpr float kPuLargest = 7.9228162514264338e28f;  // 2^96: a weight above it
 constexpr int kPuHeader = 640;                        // barriers, pieces
 constexpr int kPuReaders = 12;                        // warps that are told the pieces
 constexpr int kPuPieces = 4;                          // pieces that are told ahead
+// Tiles of an item at most, for f32 and for bf16 results: the tensor core truncates what it adds up, about 4e-9 of a sum for a position (64 sequences of 16384
+// positions in one piece each, with values of one sign, were off by 7e-5, in pieces of 2048 by 4e-6).
+constexpr int kPuWindow[2] = {16, 128};
+constexpr size_t kPuPartials = 256u << 20;            // bytes of partial results that shares are not cut further for
 constexpr int kPuBatch = 1024;                        // sequences of a call
 constexpr size_t kPuFixed = 2 * (size_t)kPfBox + kPuRing * (size_t)kPuTile + 2 * (size_t)kPuWeights + kPuOnes + kPuMeet + kPuHeader;
 
-// How many tiles of the lists an item has.
+// How a KV head's list is cut: CTAs' shares of `share` tiles, each in `parts` items of equal length but for a tile.
 struct PuCut {
-  int pre, own;
+  int share, parts;
+  __device__ __forceinline__ int item(int f) const {                   // with tile f
+    const int cta = f / share;
+    return parts == 1 ? cta : cta * parts + (int)((long long)(f - cta * share) * parts / share);
+  }
+  __device__ __forceinline__ int first(int part) const { return parts == 1 ? part * share : (int)(((long long)part * share + parts - 1) / parts); }
 };
 
 // In shared memory, behind the buffers.
@@ -70,7 +79,7 @@ struct PuPlan {
   int *own, *last, *pre;                              // [batch + 1] own tiles of the sequences before; [batch] shared tiles << 8 | keys of the last tile - 1;
                                                       // [groups + 1] units' shared tiles of the groups before
   int batch, groups, group, per_tile;
-  PuCut cut;
+  PuCut cut[2];                                       // own, shared tiles
 };
 // What the kernel that joins the pieces has to know: where a sequence's tiles stand in a KV head's list.
 struct PuSeqPlan {
@@ -127,10 +136,11 @@ __device__ __forceinline__ int pu_values_at(int t) { return 2 * t + 2; }
 
 struct PuParams {
   PagedParams a;
-  int per_tile, per_eight, n_items;                   // members of a row tile; of eight rows; items of a KV head's list
+  int per_tile, per_eight, n_shares;                  // members of a row tile; of eight rows; CTAs of a KV head
+  int window[2], most[2];                             // own, shared tiles: of an item, and items of a KV head, at most
   float *own_o, *own_ml, *pre_o, *pre_ml;             // partial results: [row][128], [row][2] references and sums (of the groups)
   PuSeqPlan* plan;                                    // [batch]
-  PuCut* cut;
+  PuCut* cut;                                         // [2]
 };
 
 template <typename F>
@@ -283,8 +293,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int pre_tiles = l.pre[l.groups], own_tiles = l.own[p.batch];
-  l.cut.pre = max(1, (pre_tiles + pp.n_items - 1) / pp.n_items);
-  l.cut.own = max(1, (own_tiles + pp.n_items - 1) / pp.n_items);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    l.cut[k].share = max(1, ((k ? pre_tiles : own_tiles) + pp.n_shares - 1) / pp.n_shares);
+    l.cut[k].parts = l.cut[k].share <= pp.window[k] ? 1 : (l.cut[k].share + pp.window[k] - 1) / pp.window[k];
+  }
   // One arrival for the warp.  The lanes meet before it and behind it: none may wait for what the arrival lets happen before it is made.
   auto arrive = [&](uint64_t* bar) {
     __syncwarp();
@@ -315,16 +328,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
       __syncwarp();
       ++told;
     };
-    const int item = (int)blockIdx.x / p.n_kv;
+    const int cta = (int)blockIdx.x / p.n_kv;            // of the KV head
     PuPiece w{};
-    w.kv = (int)blockIdx.x - item * p.n_kv;
+    w.kv = (int)blockIdx.x - cta * p.n_kv;
 #pragma unroll 1
     for (int k = 1; k >= 0 && ok; --k) {
-      const int len = k ? l.cut.pre : l.cut.own, apart = k ? 128 : 8;
-      int f = len * item;
-      const int end = min(f + len, k ? pre_tiles : own_tiles);
+      const PuCut cut = k ? l.cut[1] : l.cut[0];
+      const int from = cut.share * cta, most = min(from + cut.share, k ? pre_tiles : own_tiles), apart = k ? 128 : 8;
+      int part = 0, end = min(from + cut.first(1), most);
       w.pre = k;
-      while (f < end && ok) {
+      for (int f = from; f < most && ok; f += w.n) {
+        if (f == end) end = min(from + cut.first(++part + 1), most);
         const PuUnit u = pu_locate(p, l, k, f);
         w.n = min(end - f, u.tiles - u.tile);
         w.tile = u.shared_tiles + u.tile;
@@ -333,9 +347,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
         w.b0 = u.b0;
         w.seq = max(paged_row_of(p, u.head), 0);
         w.keyed = u.rows <= 8;
-        w.out = w.kv * (p.batch * p.group + apart * pp.n_items) + u.b0 * p.group + apart * item;
+        w.out = w.kv * (p.batch * p.group + apart * pp.most[k]) + u.b0 * p.group + apart * (cta * cut.parts + part);
         tell(w);
-        f += w.n;
       }
     }
     w.n = 0;
@@ -419,7 +432,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
         }
         pp.plan[b] = PuSeqPlan{l.own[b], l.own[b + 1] - l.own[b], pre_f, shared};
       }
-      if (lane == 0) *pp.cut = l.cut;
+      if (lane == 0) {
+        pp.cut[0] = l.cut[0];
+        pp.cut[1] = l.cut[1];
+      }
       __syncwarp();
     }
     uint32_t used = 0;                 // phases of v_raw
@@ -733,11 +749,11 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
   const PagedParams& p = pp.a;
   const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const PuSeqPlan q = pp.plan[b];
-  const PuCut cut = *pp.cut;
+  const PuCut cut[2] = {pp.cut[0], pp.cut[1]};
   const int kv = head / p.group, h = head - kv * p.group;
   // items of the row's own and shared tiles
-  const int own_c = q.own_f / cut.own, pre_c = q.pre_f / cut.pre;
-  const int own = q.own_tiles ? (q.own_f + q.own_tiles - 1) / cut.own - own_c + 1 : 0, pre = q.pre_tiles ? (q.pre_f + q.pre_tiles - 1) / cut.pre - pre_c + 1 : 0;
+  const int own_c = cut[0].item(q.own_f), pre_c = cut[1].item(q.pre_f);
+  const int own = q.own_tiles ? cut[0].item(q.own_f + q.own_tiles - 1) - own_c + 1 : 0, pre = q.pre_tiles ? cut[1].item(q.pre_f + q.pre_tiles - 1) - pre_c + 1 : 0;
   float top = -FLT_MAX, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int base = 0; base < own + pre; base += 32) {
     // a lane per partial result: its row, reference and sums
@@ -747,7 +763,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
     if (i < own + pre) {
       const bool k = i >= own;
       const int item = k ? pre_c + i - own : own_c + i, apart = k ? 128 : 8;
-      const size_t r = (size_t)kv * (p.batch * p.group + apart * pp.n_items) + b * p.group + h + (size_t)apart * item;
+      const size_t r = (size_t)kv * (p.batch * p.group + apart * pp.most[k]) + b * p.group + h + (size_t)apart * item;
       row = (k ? pp.pre_o : pp.own_o) + r * kPaDim;
       mine = *reinterpret_cast<const float4*>((k ? pp.pre_ml : pp.own_ml) + r * 4);
     }
@@ -865,11 +881,20 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   const size_t tiles = batch * (((size_t)p.max_len + kPfTile - 1) / kPfTile) * n_kv_heads;
   TQ_REQUIRE(ctx, tiles < (1ull << 30) && (size_t)p.n_pages * pages->page_rows < (1ull << 31), "tq_gqa_decode_paged: too many positions");
   const size_t most_ctas = tiles < (size_t)ctx->sm_count ? tiles : (size_t)ctx->sm_count;
-  pp.n_items = (int)(most_ctas > n_kv_heads ? most_ctas / n_kv_heads : 1);
-  const size_t n_ctas = pp.n_items * n_kv_heads;
-  // partial results, the sequences' plans
-  const size_t own_rows = batch * n_heads + 8 * n_ctas, pre_rows = p.n_groups ? batch * n_heads + 128 * n_ctas : 0;
-  const size_t floats = (own_rows + pre_rows) * (kPaDim + 4);
+  pp.n_shares = (int)(most_ctas > n_kv_heads ? most_ctas / n_kv_heads : 1);
+  const size_t n_ctas = pp.n_shares * n_kv_heads;
+  // partial results (rows of either kind: the list's, and what an item adds), the sequences' plans
+  size_t part_rows[2];
+  for (int k = 0; k < 2; ++k) {
+    const size_t len = k ? (size_t)p.max_shared / kPfTile : ((size_t)p.max_len + kPfTile - 1) / kPfTile, units = k ? p.n_groups + batch / pp.per_tile : batch;
+    const size_t share = (units * len + pp.n_shares - 1) / pp.n_shares;
+    for (pp.window[k] = kPuWindow[!p.out_f32];; pp.window[k] *= 2) {
+      pp.most[k] = (int)(pp.n_shares * (share / pp.window[k] + 1));
+      part_rows[k] = k && !p.n_groups ? 0 : batch * n_heads + (k ? 128 : 8) * n_kv_heads * pp.most[k];
+      if (share <= (size_t)pp.window[k] || part_rows[k] * (kPaDim + 4) * sizeof(float) <= kPuPartials) break;
+    }
+  }
+  const size_t own_rows = part_rows[0], pre_rows = part_rows[1], floats = (own_rows + pre_rows) * (kPaDim + 4);
   if (int st = ensure_scratch(ctx, floats * sizeof(float) + (batch + 1) * sizeof(PuSeqPlan))) return st;
   pp.own_o = static_cast<float*>(ctx->scratch);
   pp.pre_o = pp.own_o + own_rows * kPaDim;

@@ -344,3 +344,27 @@ def test_refusals(dev):
         call(**{**base, "q": off})
     call(**base)
     dev.sync()
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_long_sums_keep_the_precision_of_f32(dev, shared):
+    """64 sequences of 16384 positions in the same pages, values of one sign: what the tensor core truncates must not add up over a long sequence.  An error
+    of 2^-17 for weights of two bf16 terms (2^-18 each, of a weight and of the sum) and of 6e-9 for each of the 2048 positions that are added up at once."""
+    import tang_b200 as tb
+
+    rng, L, P, B, nh, nkv = np.random.default_rng(8), 16384, 64, 64, 8, 2
+    n_pages = L // P
+    k_bits, k = bf16_round(rng.standard_normal((L, nkv, HD)).astype(np.float32))
+    v_bits, v = bf16_round((1 + 0.1 * rng.standard_normal((L, nkv, HD))).astype(np.float32))
+    q_bits, q = bf16_round(rng.standard_normal((B, nh, HD)).astype(np.float32))
+    pool = tb.PagePool(dev, n_pages, P, B, n_pages, None, dev.upload(np.full(n_pages, B, np.int32), tb.I32),
+                       dev.upload(np.tile(np.arange(n_pages, dtype=np.int32), (B, 1)), tb.I32), dev.upload(np.full(B, L, np.int32), tb.I32))
+    kw = dict(group_starts=dev.upload(np.zeros(1, np.int32), tb.I32), shared=dev.upload(np.full(1, L, np.int32), tb.I32), n_groups=1, max_shared=L) if shared else {}
+    got = dev.gqa_decode_paged(dev.upload(q_bits.reshape(-1), tb.BF16), dev.upload(k_bits.reshape(-1), tb.BF16), dev.upload(v_bits.reshape(-1), tb.BF16), pool, B, nh, nkv,
+                               HD, L, out_dtype=tb.F32, **kw).to_vec().reshape(B, nh, HD)
+    for b, h in ((0, 0), (31, 5), (63, 7)):
+        s = k[:, h // 4].reshape(L, HD).astype(np.float64) @ q[b, h].reshape(HD).astype(np.float64) / np.sqrt(HD)
+        w = np.exp(s - s.max())
+        want = w @ v[:, h // 4].reshape(L, HD).astype(np.float64) / w.sum()
+        assert np.abs(got[b, h] / want - 1).max() <= 2.0 ** -17 + 2048 * 6e-9, (b, h)
+    pool.destroy()
