@@ -203,6 +203,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
   uint64_t* met = piece_empty + kPuPieces;            // [parity] the four warps of a softmax group
   uint64_t* ref_full = met + 2;                       // [piece's parity]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ref_full + 2);
+  volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
   PuPiece* piece_s = reinterpret_cast<PuPiece*>(q_full) + (kPuHeader / sizeof(PuPiece) - kPuPieces);
   PuPlan l;
   l.own = reinterpret_cast<int*>(q_full) + kPuHeader / 4;
@@ -235,6 +236,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
         mbar_init(&met[x], 4);
         mbar_init(&ref_full[x], 4);
       }
+      *failed = 0;
       mbar_init_fence();
     }
   } else if (warp == 1) {
@@ -252,6 +254,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
   pdl_wait();
   pdl_launch_dependents();
   auto give_up = [&](int code) { atomicCAS(p.err, 0, code); };
+  auto abandon = [&](int code) {
+    give_up(code);
+    *failed = 1;
+  };
   if (threadIdx.x == 0 && (smem_u32(smem_raw) & 1023)) give_up(DERR_TMEM);
 
   // ---- the plan: every CTA makes it for itself
@@ -353,7 +359,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
     }
     w.n = 0;
     if (ok) tell(w);
-    if (!ok) give_up(DERR_EMPTY_WAIT);
+    if (!ok) abandon(DERR_EMPTY_WAIT);
   } else if (warp == 0 || warp == 2) {
     // ---- copies: the keys of every tile (warp 0); the queries of every piece and the values of every tile (warp 2).  A lane per box: a page's rows, half
     // their columns.  The warp holds the pages of the next 32 boxes' rows (four tiles or more), and has asked for those behind them.
@@ -414,7 +420,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
         }
       }
     }
-    if (!ok) give_up(DERR_EMPTY_WAIT);
+    if (!ok) abandon(DERR_EMPTY_WAIT);
   } else if (warp == 3) {
     // ---- value rows between the last key and the next multiple of 16: whatever the cache holds there must not meet a weight of zero
     if (blockIdx.x == 0) {             // (before that: what the kernel that joins the pieces has to know)
@@ -458,7 +464,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       arrive(&kv_full[slot]);
     }
-    if (!ok) give_up(DERR_EMPTY_WAIT);
+    if (!ok) abandon(DERR_EMPTY_WAIT);
     __syncwarp();
   } else if (warp == 1) {
     // ---- products: the scores of a tile, then the weighted values of the tile before
@@ -543,7 +549,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
       }
     }
     if (ok && t > 0) ok = values(t - 1, before);
-    if (!ok) give_up(DERR_FULL_WAIT);
+    if (!ok) abandon(DERR_FULL_WAIT);
   } else if (warp >= 4) {
     // ---- softmax of the tiles of a parity.  More than eight rows: S = Q K^T, a thread per row, the weights over the scores' columns.  Up to eight: the keys
     // are the tensor memory's lanes, S^T = K Q^T and O^T = V^T P with 16 columns (a product of 128 x 128 x 16 takes 84 cycles for four rows too, one of
@@ -732,9 +738,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
         }
       }
     }
-    if (!ok) give_up(DERR_TMEM);
+    if (!ok) abandon(DERR_TMEM);
   }
   tc_fence_before();
+  __syncthreads();
+  if (*failed && threadIdx.x == 0) {
+    // copies and products that are still in flight target this CTA's memories: give them time to land before leaving
+    for (int i = 0; i < 10000; ++i) __nanosleep(1000);
+  }
   __syncthreads();
   __syncwarp();                        // (the release is one instruction of the whole warp)
   if (warp == 1) tmem_dealloc(tmem, 512);

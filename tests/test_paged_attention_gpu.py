@@ -368,3 +368,28 @@ def test_long_sums_keep_the_precision_of_f32(dev, shared):
         want = w @ v[:, h // 4].reshape(L, HD).astype(np.float64) / w.sum()
         assert np.abs(got[b, h] / want - 1).max() <= 2.0 ** -17 + 2048 * 6e-9, (b, h)
     pool.destroy()
+
+
+def test_the_largest_batch_many_kv_heads_and_a_loose_bound(dev):
+    import tang_b200 as tb
+
+    # 1024 sequences, a group each or all in one
+    s = Setup(8, 1, 16, [(0, [i % 37]) for i in range(1024)], seed=31).put(dev)
+    for f32 in (False, True):
+        s.check(s.run(f32).to_vec(), f32)
+    s = Setup(2, 2, 16, [(200, [200 + i % 9 for i in range(1024)])], seed=32).put(dev)
+    s.check(s.run(True).to_vec(), True)
+    with pytest.raises(tb.TangqError):
+        dev.gqa_decode_paged(dev.alloc(1025 * 2 * HD, tb.BF16), s.kb, s.vb, s.pool, 1025, 2, 2, HD, 209, seqs=dev.alloc(1025, tb.I32))
+    # more KV heads than SMs
+    s = Setup(320, 160, 16, [(130, [131, 150, 140]), (0, [33])], seed=33).put(dev)
+    for f32 in (False, True):
+        s.check(s.run(f32).to_vec(), f32)
+    # tables for a million positions, of which sequences have few
+    s = Setup(8, 2, 16, [(256, [300, 400, 290]), (0, [5000])], seed=34)
+    s.tables = np.concatenate([s.tables, np.full((s.B, 65536 - s.ld), -1, np.int32)], 1)
+    s.ld = 65536
+    s.put(dev)
+    for f32 in (False, True):
+        s.check(s.run(f32, max_len=1 << 20).to_vec(), f32)
+    dev.sync()
