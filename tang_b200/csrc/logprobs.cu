@@ -5,8 +5,8 @@
 //     log sum exp x = m + log c + log1p(s / c),      H = log c + log1p(s / c) + sum (m - x) exp(x - m) / (c + s),
 // so that a model that is sure of a token (log probability and entropy near zero) loses nothing to the addition of the leading one.
 //
-// What bounds it: the logits' bytes where rows are many (1024 x 128256 f32 79.5 us, 6.6 TB/s; as many bytes of bf16 91 us, 5.8 TB/s, with four fifths of
-// the issue slots taken: an exponential, a share of a maximum and half an addition and multiplication for every logit); the latency of the launch, the
+// What bounds it: the logits' bytes where rows are many (1024 x 128256 f32 79.5 us, 6.6 TB/s; as many bytes of bf16 86 us, 6.1 TB/s, where
+// every logit costs an exponential, a share of a maximum and half an addition and multiplication); the latency of the launch, the
 // cluster's meeting and, with alternatives, of sorting 128 maxima where they are few (one row of 32000 4.3 us, 7.1 with five alternatives).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -103,10 +103,27 @@ __device__ __forceinline__ unsigned long long lp_add2(unsigned long long a, unsi
 __device__ __forceinline__ float lp_largest(const uint4& v, float) {
   return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
 }
+__device__ __forceinline__ __nv_bfloat162 lp_largest2(const uint4& v) {
+  return __hmax2(__hmax2(reinterpret_cast<const __nv_bfloat162&>(v.x), reinterpret_cast<const __nv_bfloat162&>(v.y)),
+                 __hmax2(reinterpret_cast<const __nv_bfloat162&>(v.z), reinterpret_cast<const __nv_bfloat162&>(v.w)));
+}
 __device__ __forceinline__ float lp_largest(const uint4& v, __nv_bfloat16) {
-  const __nv_bfloat162 a = __hmax2(__hmax2(reinterpret_cast<const __nv_bfloat162&>(v.x), reinterpret_cast<const __nv_bfloat162&>(v.y)),
-                                   __hmax2(reinterpret_cast<const __nv_bfloat162&>(v.z), reinterpret_cast<const __nv_bfloat162&>(v.w)));
-  return fmaxf(__low2float(a), __high2float(a));
+  const __nv_bfloat162 m = lp_largest2(v);
+  return fmaxf(__low2float(m), __high2float(m));
+}
+template <int K>
+__device__ __forceinline__ float lp_largest(const uint4 (&v)[K], float) {
+  float m = lp_largest(v[0], 0.f);
+#pragma unroll
+  for (int k = 1; k < K; ++k) m = fmaxf(m, lp_largest(v[k], 0.f));
+  return m;
+}
+template <int K>
+__device__ __forceinline__ float lp_largest(const uint4 (&v)[K], __nv_bfloat16) {
+  __nv_bfloat162 m = lp_largest2(v[0]);
+#pragma unroll
+  for (int k = 1; k < K; ++k) m = __hmax2(m, lp_largest2(v[k]));
+  return fmaxf(__low2float(m), __high2float(m));
 }
 
 // Larger for a larger logit and, among equals (the zeros too), for a lower index; 0 is nobody's.
@@ -140,15 +157,19 @@ struct LpState {
 // thread's own.  What the rounding of base adds to every exponent alike, `off`, is taken out at the end (it would be too large from |b| = 2^20 on:
 // there, and before anything but -infinity was seen, the two instructions are used).
 // The 16 bytes with the thread's largest logit are held back: the row's largest must not be added before it is known (the sum of the others would be
-// lost against it where a model is sure).  Where another vector has the same one, that is among s, which is no loss there.
+// lost against it where a model is sure).  Where another vector has the same one, that is among s, which is no loss there.  Without alternatives it is
+// enough to do so where a batch goes beyond what the warp has seen (2048 rows of 128256 bf16 91 -> 86 us, with entropies 98 -> 94); f32 with entropies has
+// each thread look after its own all the same (256 rows 23.2 us, the other way 24.0).
 constexpr float kLpSlack = 20.f;
 template <typename T, bool ENT, bool TOP>
 struct LpRunning {
   static constexpr int N = 16 / (int)sizeof(T);
+  static constexpr bool EACH = TOP || (ENT && sizeof(T) == 4);
   static constexpr uint32_t kNone = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;        // -infinity
   float b = -INFINITY, base = 0.f, off = 0.f;
   unsigned long long s = 0, u = 0;                      // two sums each, of even and of odd places; u: of exponent * exponential
-  float mine = -INFINITY, second = -INFINITY;                      // the largest of `held` and of all other vectors
+  float warps = -INFINITY;                              // the largest that the warp has read
+  float mine = -INFINITY, second = -INFINITY;           // the largest of `held` and of all other vectors
   uint4 held = make_uint4(kNone, kNone, kNone, kNone);
   int where = -1;                                       // the row's place of its first logit (-1: not 16 bytes of the row)
 
@@ -163,11 +184,7 @@ struct LpRunning {
   template <int K>
   __device__ __forceinline__ void add(uint4 (&v)[K], int at, int step) {
     float top = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const float mx = lp_largest(v[k], T());
-      top = fmaxf(top, mx);
-      if (TOP) second = fmaxf(second, fminf(mx, mine));
+    auto hold = [&](int k, float mx) {
       if (mx > mine) {                                  // (selects, no branch)
         const uint4 w = held;
         held = v[k];
@@ -175,17 +192,35 @@ struct LpRunning {
         mine = mx;
         if (TOP) where = at < 0 ? -1 : at + k * step;
       }
+    };
+    if constexpr (EACH) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const float mx = lp_largest(v[k], T());
+        top = fmaxf(top, mx);
+        if (TOP) second = fmaxf(second, fminf(mx, mine));
+        hold(k, mx);
+      }
+    } else {
+      top = lp_largest(v, T());
     }
-    if (__any_sync(0xffffffffu, top > b + kLpSlack)) {
-      const float was = b, off_was = off;
-      b = fmaxf(b, warp_max(top));
-      base = far() ? 0.f : b * kLpLog2e;
-      off = far() ? 0.f : fmaf(b, kLpLog2e, -base);
-      if (was != -INFINITY) {
-        const float by = fmaxf((was - b) * kLpLog2e - off_was + off, -1e4f), f = lp_ex2(by);
-        const unsigned long long f2 = lp_pair(f, f);
-        if (ENT) u = lp_fma2(lp_fma2(lp_pair(by, by), s, u), f2, 0ull);
-        s = lp_fma2(s, f2, 0ull);
+    // (the warp's largest rises a few times in a row: 3.4 of 16 batches)
+    if (__any_sync(0xffffffffu, top > (EACH ? b + kLpSlack : warps))) {
+      if constexpr (!EACH)
+#pragma unroll
+        for (int k = 0; k < K; ++k) hold(k, lp_largest(v[k], T()));
+      warps = fmaxf(warps, warp_max(top));
+      if (warps > b + kLpSlack) {
+        const float was = b, off_was = off;
+        b = warps;
+        base = far() ? 0.f : b * kLpLog2e;
+        off = far() ? 0.f : fmaf(b, kLpLog2e, -base);
+        if (was != -INFINITY) {
+          const float by = fmaxf((was - b) * kLpLog2e - off_was + off, -1e4f), f = lp_ex2(by);
+          const unsigned long long f2 = lp_pair(f, f);
+          if (ENT) u = lp_fma2(lp_fma2(lp_pair(by, by), s, u), f2, 0ull);
+          s = lp_fma2(s, f2, 0ull);
+        }
       }
     }
     if (!far()) {
@@ -592,7 +627,7 @@ extern "C" int tq_token_logprobs(tq_ctx* ctx, const void* logits_dev, int dtype,
   // CTAs of a row (a cluster): as many as fit the GPU at once (four an SM), none with less than 2048 logits.  More, smaller ones cost more than they
   // balance, fewer leave SMs idle; us for one, two, four, eight: 64 rows of 128256 f32 23.7, 14.6, 10.3, 9.8, 256 rows 27.5, 22.3, 26.1, 33.0,
   // one row of 32000 6.5, 5.2, 4.6, 4.3.  Forms without alternatives or entropies leave their bookkeeping out of the loop: 2048 rows of 128256 bf16
-  // 91 us, 98 with entropies, 108 with 20 alternatives, 122 with both.
+  // 86 us, 95 with entropies, 108 with 20 alternatives, 122 with both.
   const size_t V = slices * cols, slots = (size_t)ctx->sm_count * kLpPerSm;
   size_t C = slots / rows < V / 2048 ? slots / rows : V / 2048;
   C = C < 1 ? 1 : C > (size_t)kLpMaxCluster ? (size_t)kLpMaxCluster : C;
