@@ -34,16 +34,16 @@ __device__ __forceinline__ int paged_row_of(const PagedParams& p, int b) {
 // Units, tiles, items, pieces.  A unit is what meets the same keys: the rows (member, query head of one KV head) of up to 128 / group members of a group
 // over the group's shared positions, in whole tiles of 128, or one sequence's query heads over the rest.  The tiles of all units of a KV head stand in
 // two lists, one of shared and one of own tiles, and every CTA, one an SM, takes a share of either: as many tiles of the one and of the other as everybody
-// else.  A long share is cut into items (kPuWindow).  CTAs that stand at the same place of the KV heads' lists are neighbours: a cache row holds all heads, and its 256 bytes a head are fetched at the
-// same time.  A piece is what an item has of a unit.  Its odd and its even tiles belong to different softmax groups, which take scores from the same reference,
-// so that the products of both go to the same columns (two sets of columns, for pieces that follow one another).  It leaves a partial result; a second
-// kernel joins those of a row, in the order of the list.
+// else.  A long share is cut into items (kPuWindow).  CTAs that stand at the same place of the KV heads' lists are neighbours: a cache row holds all heads,
+// and its 256 bytes a head are fetched at the same time.  A piece is what an item has of a unit.  Its odd and its even tiles belong to different softmax
+// groups, which take scores from the same reference, so that the products of both go to the same columns (two sets of columns, for pieces that follow one
+// another).  It leaves a partial result; a second kernel joins those of a row, in the order of the list.
 // (64 sequences of 2048 positions and 8 KV heads take 97 us.  One list of all heads' tiles, cut for 148 CTAs rather than 144, took 98 us.  Shorter items,
 // handed out as CTAs get to them because SMs differ in speed by a fifth, took 102: they make more partial results than they balance.)
 //
 // What bounds it: the bytes of the cache, once, where sequences are long (537 MB in 97 us, 5.5 TB/s; the steady state is 2800 cycles for a tile of 64 KB,
 // which is an SM's share of the memory's rate); beside them a start of 5 us (lengths, plan, first pages, first tile: six loads in a row) and 4 us until the
-// second kernel is through, which are most of a small call (one sequence of 700 positions 8.9 us, 8 samples of a prompt of 2040 16.7).  A shared tile of
+// second kernel is through, which are most of a small call (one sequence of 700 positions 8.8 us, 8 samples of a prompt of 2040 16.3).  A shared tile of
 // 128 rows is 2000 cycles: two products of 670 each, of two softmax groups in turn, and 64 KB from L2 (64 samples of a prompt of 8192: 42 us, of which the
 // shared part is 11).
 // ---------------------------------------------------------------------------------------------
@@ -645,7 +645,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
         first = i == place;
         const int r = 32 * q4 + lane;
         const bool live = r < u.rows;
-        ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[x], (uint32_t)(done & 1)) && (!first || leads || mbar_wait_spin(&ref_full[slot], (uint32_t)((piece >> 1) & 1))));
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[x], (uint32_t)(done & 1)) &&
+                                         (!first || leads || mbar_wait_spin(&ref_full[slot], (uint32_t)((piece >> 1) & 1))));
         if (!ok) break;
         tc_fence_after();
         if (u.keyed) {
