@@ -7,7 +7,7 @@
 //
 // What bounds it: the logits' bytes where rows are many (1024 x 128256 f32 79.5 us, 6.6 TB/s; as many bytes of bf16 86 us, 6.1 TB/s, where
 // every logit costs an exponential, a share of a maximum and half an addition and multiplication); the latency of the launch, the
-// cluster's meeting and, with alternatives, of sorting 128 maxima where they are few (one row of 32000 4.3 us, 7.1 with five alternatives).
+// cluster's meeting and, with alternatives, of sorting 128 maxima where they are few (one row of 32000 4.0 us, 6.6 with five alternatives).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -288,7 +288,7 @@ template <typename T, bool ENT, bool TOP>
 __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(const LogprobParams p) {
   constexpr int N = LpSegment<T>::N;
   __shared__ float red[4][kLpWarps];
-  __shared__ float4 part;              // this CTA's state
+  __shared__ float4 parts[kLpMaxCluster];              // the CTAs' states, and
   __shared__ __align__(16) float group_max[kLpGroups];
   __shared__ float thr_s;
   __shared__ int n_above, n_equal;
@@ -296,14 +296,15 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
   __shared__ unsigned long long equal_list[kLpList];
   __shared__ int scan[kLpThreads];     // threads that have any of them
   __shared__ int n_scan;
+  __shared__ __align__(16) unsigned long long all_k[kLpMaxCluster * kLpMaxTop + 2];        // their largest, each in order, in the first CTA
   __shared__ unsigned long long top_k[kLpMaxTop];                      // this CTA's largest, in order
-  __shared__ __align__(16) unsigned long long all_k[kLpMaxCluster * kLpMaxTop];
   pdl_wait();
   pdl_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = (int)(blockIdx.x / C), t = threadIdx.x, warp = t >> 5, lane = t & 31, V = p.slices * p.cols, top = TOP ? p.top : 0;
   const int lo = (int)((long long)V * rank / C) & ~63, hi = rank == C - 1 ? V : (int)((long long)V * (rank + 1) / C) & ~63;
+  if (C > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");              // (this CTA runs: the others may write to its memory)
   int token = -1;
   float token_x = 0.f;
   if (rank == 0 && t < p.n_tokens) {   // (on their way while the row is read)
@@ -515,7 +516,8 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
     }
   }
 
-  // ---- the row: the first CTA of the cluster reads the others' states and lists
+  // ---- the row: every CTA of the cluster writes its state and its list to the first one's memory
+  if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   __syncthreads();
   if (t == 0) {
     LpState r;
@@ -526,29 +528,28 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
       r.s += red[2][w];
       if (ENT) r.u += red[3][w];
     }
-    part = make_float4(r.m, r.c, r.s, r.u);
+    *(C > 1 ? cluster.map_shared_rank(&parts[rank], 0) : parts) = make_float4(r.m, r.c, r.s, r.u);
   }
+  if (TOP && C > 1 && t < top) *cluster.map_shared_rank(&all_k[rank * top + t], 0) = top_k[t];
   if (C > 1) cluster.sync();
   else __syncthreads();
   if (rank == 0) {
     LpState r;
     {
-      float4 q[kLpMaxCluster];
+      float m = -INFINITY;
 #pragma unroll
       for (int k = 0; k < kLpMaxCluster; ++k)
-        if (k < C) q[k] = C > 1 ? *cluster.map_shared_rank(&part, k) : part;
-#pragma unroll
-      for (int k = 0; k < kLpMaxCluster; ++k)
-        if (k < C) r.m = fmaxf(r.m, q[k].x);
-      const float m = r.m;
+        if (k < C) m = fmaxf(m, parts[k].x);
+      r.m = m;
 #pragma unroll
       for (int k = 0; k < kLpMaxCluster; ++k) {
         if (k >= C) break;
+        const float4 q = parts[k];
         LpState b;
-        b.m = q[k].x;
-        b.c = q[k].y;
-        b.s = q[k].z;
-        b.u = q[k].w;
+        b.m = q.x;
+        b.c = q.y;
+        b.s = q.z;
+        b.u = q.w;
         b.rise(m);
         r.c += b.c;
         r.s += b.s;
@@ -574,23 +575,26 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
       if (C == 1) {
         if (t < top) put(t, top_k[t]);
       } else {
+        // (a key's place is how many are before it; searching the lists, which are in order, is more code and was 1 us slower)
         const int all = C * top;
-        for (int i = t; i < all; i += kLpThreads) all_k[i] = *cluster.map_shared_rank(&top_k[i % top], i / top);
+        if (t == 0 && (all & 1)) all_k[all] = 0ull;    // (read as the second of two)
         int have = 0;
-        for (int i = t; i - t < all; i += kLpThreads) have += __syncthreads_count(i < all && all_k[i] != 0ull);   // (a thread counts the keys that it wrote)
-        for (int i = t; i < all; i += kLpThreads) {
-          const unsigned long long me = all_k[i];
+        for (int i = t; i - t < all; i += kLpThreads) {
+          const unsigned long long me = i < all ? all_k[i] : 0ull;
+          have += __syncthreads_count(me != 0ull);
           if (!me) continue;
           int before = 0;
 #pragma unroll 8
-          for (int j = 0; j < all; ++j) before += all_k[j] > me;
+          for (int j = 0; j < all; j += 2) {
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&all_k[j]);
+            before += (two.x > me) + (two.y > me);
+          }
           if (before < top) put(before, me);
         }
         if (t >= have && t < top) put(t, 0ull);        // (fewer numbers than places)
       }
     }
   }
-  if (C > 1) cluster.sync();           // (nobody leaves while its memory is read)
 }
 
 }  // namespace tq
