@@ -179,7 +179,6 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-template <int TERMS>
 __global__ void __launch_bounds__(kPuThreads, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_constant__ CUtensorMap q_whole,
                     const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PuParams pp) {
@@ -507,8 +506,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
           }
         } else {
           for (int k = 0; k < w.steps; ++k) umma_f16_ts(o_t, s_t + 8u * k, at + (uint64_t)(k * (2048 >> 4)), idesc_o, !w.first || k != 0);
-          if (TERMS == 2)
-            for (int k = 0; k < w.steps; ++k) umma_f16_ts(o_t, s_t + 64u + 8u * k, at + (uint64_t)(k * (2048 >> 4)), idesc_o, 1u);
+          for (int k = 0; k < w.steps; ++k) umma_f16_ts(o_t, s_t + 64u + 8u * k, at + (uint64_t)(k * (2048 >> 4)), idesc_o, 1u);
         }
         umma_commit(&o_done[x]);
         umma_commit(&kv_empty[slot]);
@@ -560,9 +558,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
     // are the tensor memory's lanes, S^T = K Q^T and O^T = V^T P with 16 columns (a product of 128 x 128 x 16 takes 84 cycles for four rows too, one of
     // 128 x 16 x 16 a fraction): a thread per key, whose weights go to shared memory, and the weights' sums come from a product with ones.  (Both ways for 9
     // to 32 rows: 16 groups of four samples 41.8 us with keys as lanes and 42.4 with rows, 64 samples by fours 71.6 and 70.4.)
-    // A weight is two bf16 terms, hi + lo, where keys are the lanes and where results are f32: within 2^-18 of it.  (Three would be nearer to f32 results,
-    // whose error from 64 bits is 2e-6 so and 8e-7 by f32 arithmetic, but tensor memory has no columns for them.)  One term, within 2^-9 like the rounding
-    // of the result, where rows are the lanes and results are bf16.
+    // A weight is two bf16 terms, hi + lo, within 2^-16 of it, as in the attention over slots.  (Three would be nearer to f32 results, whose error from
+    // 64 bits is 2e-6 so and 8e-7 by f32 arithmetic, but tensor memory has no columns for them.  One, within 2^-8, would be as far off as the rounding of a
+    // bf16 result.)
     // The reference that scores are taken from is their maximum in the piece's first tile, which the group with that tile tells the other one: a bf16 weight
     // may be as large as an f32 one, so that nothing is rescaled; a weight above 2^96 becomes no number, and the joining kernel goes through the row's keys
     // one by one.
@@ -672,25 +670,22 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
           __syncwarp();
           // Weights take the first half of the scores' columns.  Second terms take the other half: quarters in the order 0, 2, 1, 3, so that only three
           // sixteens wait in registers for columns that are read.
-          uint32_t keep[TERMS == 2 ? 3 : 1][16];                       // second terms of quarter 0; weights and second terms of quarter 2
+          uint32_t keep[3][16];                       // second terms of quarter 0; weights and second terms of quarter 2
 #pragma unroll
           for (int step = 0; step < 4; ++step) {
-            const int c = TERMS == 1 ? step : step == 1 ? 2 : step == 2 ? 1 : step;
+            const int c = step == 1 ? 2 : step == 2 ? 1 : step;
             float v[32];
             pf_ld32(s_t + 32u * c, v);
-            uint32_t w[16], low[TERMS == 2 ? 16 : 1];
+            uint32_t w[16], low[16];
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const float w0 = ex2(fmaf(v[2 * j], p.scale_log2, -ref)), w1 = ex2(fmaf(v[2 * j + 1], p.scale_log2, -ref));
               sum[j & 3] += w0 + w1;
-              if constexpr (TERMS == 2) split_bf16(w0, w1, w[j], low[j]);
-              else w[j] = pack_bf16(w0, w1);
+              split_bf16(w0, w1, w[j], low[j]);
             }
             sum_all += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            if constexpr (TERMS == 1) {
-              tmem_st16(s_t + 16u * c, w);                 // over scores that this thread has read
-            } else if (step == 0) {
+            if (step == 0) {                               // (over scores that this thread has read)
               tmem_st16(s_t, w);
 #pragma unroll
               for (int j = 0; j < 16; ++j) keep[0][j] = low[j];
@@ -929,9 +924,8 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
       !encode_pages(&vm, v_pages_dev, row, rows, box))
     return fail(ctx, TQ_ECUDA, "cuTensorMapEncodeTiled failed");
   const size_t smem = kPuFixed + (2 * batch + 1 + (size_t)p.n_groups + 1) * sizeof(int);
-  auto kern = p.out_f32 ? paged_decode_kernel<2> : paged_decode_kernel<1>;
-  TQ_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kPuFixed + (3 * kPuBatch + 2) * sizeof(int))));
-  TQ_CUDA(ctx, launch_k(ctx, kern, dim3((unsigned)n_ctas), dim3(kPuThreads), smem, qe, qw, km, vm, pp));
+  TQ_CUDA(ctx, cudaFuncSetAttribute(paged_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kPuFixed + (3 * kPuBatch + 2) * sizeof(int))));
+  TQ_CUDA(ctx, launch_k(ctx, paged_decode_kernel, dim3((unsigned)n_ctas), dim3(kPuThreads), smem, qe, qw, km, vm, pp));
   TQ_CUDA(ctx, launch_k(ctx, paged_join_kernel, dim3((unsigned)n_heads, (unsigned)batch), dim3(128), 0, pp));
   return TQ_OK;
 }

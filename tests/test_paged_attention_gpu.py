@@ -393,3 +393,16 @@ def test_the_largest_batch_many_kv_heads_and_a_loose_bound(dev):
     for f32 in (False, True):
         s.check(s.run(f32, max_len=1 << 20).to_vec(), f32)
     dev.sync()
+
+
+@pytest.mark.parametrize("name", ["samples", "groups", "many", "one kv head", "five to one", "two hundred"])
+def test_bf16_results_are_off_by_their_own_rounding(dev, name):
+    """Shared tiles too, whatever number of rows meets them: 2^-14 of the sum of |weight value| for what f32 results may be off (``Setup.check``), and the
+    rounding to bf16 of what that gives, 2^-8 of it."""
+    s = Setup(*CASES[name], seed=40 + len(name)).put(dev)
+    got = (s.run(False).to_vec().astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+    dev.sync()
+    want, size = s.reference()
+    off = 2.0 ** -14 * size
+    err = np.abs(got.reshape(want.shape) - want) / (off + 2.0 ** -8 * (np.abs(want) + off) + 1e-30)
+    assert err.max() <= 1, (err.max(), np.unravel_index(err.argmax(), err.shape))
