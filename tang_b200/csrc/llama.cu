@@ -17,6 +17,7 @@
 #include <utility>
 #include <vector>
 
+#include "common.cuh"
 #include "internal.h"
 #include "pages.h"
 #include "qlayout.cuh"
@@ -45,9 +46,10 @@ __global__ void lens_kernel(const int* positions, int* lens, int n, int max_seq)
 }
 
 // The same for a cache of pages, whose pool has counted the new tokens already: a sequence's new token is its last position, and goes to that
-// position's row of its page.  Whatever does not exist gives row -1, which the kernel that appends K/V reports.
-__global__ void paged_rows_kernel(const int* tables, const int* lens, const int* seqs, int n, int n_seqs, int table_ld, int n_pages, int page_rows,
-                                  int max_len, int* rows, int* positions) {
+// position's row of its page.  Whatever does not exist gives row -1, which the kernel that appends K/V reports.  So does a last position that is not the
+// sequence's to write: the pool was asked for room and refused (`refused`), or the page has other holders (it was forked and not extended).
+__global__ void paged_rows_kernel(const int* tables, const int* lens, const int* refs, const int* refused, const int* seqs, int n, int n_seqs, int table_ld,
+                                  int n_pages, int page_rows, int max_len, int* rows, int* positions, int* err) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
@@ -57,7 +59,10 @@ __global__ void paged_rows_kernel(const int* tables, const int* lens, const int*
   if (s >= 0 && s < n_seqs && lens[s] > 0 && lens[s] <= max_len) {
     pos = lens[s] - 1;
     const int page = tables[(size_t)s * table_ld + pos / page_rows];
-    if (page >= 0 && page < n_pages) row = page * page_rows + pos % page_rows;
+    if (page >= 0 && page < n_pages) {
+      if (refused[s] == 0 && refs[page] == 1) row = page * page_rows + pos % page_rows;
+      else atomicCAS(err, 0, (int)DERR_PAGE_LIST);
+    }
   }
   rows[i] = row;
   positions[i] = pos;
@@ -459,8 +464,9 @@ static int decode_step(tq_llama* m, const int* token_ids_dev, const int* positio
   if (paged) {
     const tq_pages* pg = paged->pages;
     const size_t most = (size_t)pg->table_ld * pg->page_rows;
-    TQ_CUDA(ctx, launch_k(ctx, paged_rows_kernel, dim3((B + 63) / 64), dim3(64), 0, (const int*)pg->tables, (const int*)pg->lens, paged->seqs, B, pg->n_seqs,
-                          pg->table_ld, pg->n_pages, pg->page_rows, (int)(max_len < most ? max_len : most), m->lens, m->rope));
+    TQ_CUDA(ctx, launch_k(ctx, paged_rows_kernel, dim3((B + 63) / 64), dim3(64), 0, (const int*)pg->tables, (const int*)pg->lens, (const int*)pg->refs,
+                          (const int*)pages_refused(pg), paged->seqs, B, pg->n_seqs, pg->table_ld, pg->n_pages, pg->page_rows,
+                          (int)(max_len < most ? max_len : most), m->lens, m->rope, ctx->dev_err));
   } else {
     TQ_CUDA(ctx, launch_k(ctx, lens_kernel, dim3((B + 63) / 64), dim3(64), 0, positions_dev, m->lens, B, (int)c.max_seq));
   }

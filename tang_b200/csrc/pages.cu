@@ -23,7 +23,7 @@ constexpr int kCopyChunk = kCopyThreads * 4 * 16;   // bytes that a CTA moves pe
 struct PagesParams {
   int *refs, *tables, *lens;
   int n_pages, page_rows, n_seqs, table_ld;
-  int *n_copies, *from, *to, *rows, *list, *marks;
+  int *n_copies, *from, *to, *rows, *list, *marks, *refused;
   int* err;
 };
 
@@ -125,6 +125,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_extend_kernel(const PagesP
   if (!bad && !full && total > 0) full = find_pages(p.refs, 0, p.n_pages, true, total, p.list, warp_sums) < total;
   if (bad || full) {
     if (t == 0) atomicCAS(p.err, 0, bad ? (int)DERR_PAGE_LIST : (int)DERR_PAGES);
+    if (s >= 0 && s < p.n_seqs) p.refused[s] = 1;      // (the step that stands behind this call in a graph runs all the same)
     return;
   }
   first_s[t] = first;
@@ -137,7 +138,10 @@ __global__ void __launch_bounds__(kBookThreads) pages_extend_kernel(const PagesP
     p.rows[copy_at] = len % P;
     atomicSub(&p.refs[last], 1);
   }
-  if (t < n) p.lens[s] = len + c;
+  if (t < n) {
+    p.lens[s] = len + c;
+    if (c > 0) p.refused[s] = 0;
+  }
   if (t == 0) *p.n_copies = n_copies;
   for (int i = t; i < total; i += kBookThreads) {
     int lo = 0, hi = n;                // the last sequence whose first page is at most i
@@ -323,6 +327,7 @@ static PagesParams params_of(const tq_pages* p) {
   k.rows = k.to + m;
   k.list = pages_list(p);
   k.marks = pages_marks(p);
+  k.refused = pages_refused(p);
   k.err = p->ctx->dev_err;
   return k;
 }

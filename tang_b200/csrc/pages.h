@@ -10,7 +10,7 @@ struct tq_pages {
   void** arrays = nullptr;      // device: the caches' base pointers
   int n_arrays = 0;
   size_t row_bytes = 0;
-  int* ws = nullptr;            // [0] copies to make; then their from, to and rows, a list of pages, a mark per sequence (zero between calls)
+  int* ws = nullptr;            // [0] copies to make; then their from, to and rows, a list of pages, a mark per sequence (zero between calls), refusals
   bool owns = false;
 };
 
@@ -21,6 +21,9 @@ inline size_t pages_max_copies(const tq_pages* p) { return p->n_pages > kPageCal
 inline int* pages_copies(const tq_pages* p) { return p->ws + 4; }
 inline int* pages_list(const tq_pages* p) { return pages_copies(p) + 3 * pages_max_copies(p); }
 inline int* pages_marks(const tq_pages* p) { return pages_list(p) + p->n_pages; }
-inline size_t pages_ws_ints(const tq_pages* p) { return 4 + 3 * pages_max_copies(p) + p->n_pages + p->n_seqs; }
+// Per sequence: not zero from a refused tq_pages_extend on until one that gives it new positions.  Its last position is then an old one, which a step must
+// not write.
+inline int* pages_refused(const tq_pages* p) { return pages_marks(p) + p->n_seqs; }
+inline size_t pages_ws_ints(const tq_pages* p) { return 4 + 3 * pages_max_copies(p) + p->n_pages + 2 * (size_t)p->n_seqs; }
 
 }  // namespace tq

@@ -279,3 +279,102 @@ def test_refusals(dev):
         odd.sample([[1, 2]], 4, 2)
     for x in (big, pool, model, odd):
         x.destroy()
+
+
+def caches(model):
+    return [b.to_vec() for layer in range(model.cfg.n_layers) for b in model.kv_buffers(layer)[:2]]
+
+
+def test_a_step_behind_a_refused_call_writes_nothing(dev):
+    """A recorded step (extend, decode) whose pool runs out: caches and pool stay as they are to the byte, and the same step goes on once there is room."""
+    import tang_b200 as tb
+
+    host = host_model(23)
+    V, max_seq, n = host.vocab, 64, 4
+    a, b = host.to_device(dev, max_seq, n), host.to_device(dev, max_seq, n)
+    prompt = np.random.default_rng(4).integers(0, V, 20).astype(np.int32)
+    ints = lambda v: dev.upload(np.asarray(v, np.int32), tb.I32)
+    lg = dev.alloc(n * V)
+    pool = b.page_pool(6, 16)                          # 16 pages
+    one = ints([0])
+    for t in prompt:
+        pool.extend(one)
+        b.decode_paged(ints([t]), pool, 1, max_seq, lg, seqs=one)
+    pool.fork([0, 0, 0], [1, 2, 3])
+    pool.extend([4, 5], counts=[64, 64])               # 2 + 8 pages held, 6 free: three copies, and then one too few for four new pages
+    seqs, tok = ints(np.arange(n)), ints(np.arange(n) + 7)
+
+    def step():
+        pool.extend(seqs, n)
+        b.decode_paged(tok, pool, n, max_seq, lg)
+
+    step()
+    dev.sync()
+    dev.begin_capture()
+    step()
+    graph = dev.end_capture()
+    for _ in range(21, 32):
+        graph.launch()
+    dev.sync()
+    assert pool.state()[2].tolist() == [32] * 4 + [64] * 2
+    before, state = caches(b), pool.state()
+    dev.upload_into(tok, np.arange(n) + 90)            # (the tokens of the step before would give the rows that are there)
+    for _ in range(2):
+        graph.launch()
+        with pytest.raises(tb.TangqError) as e:
+            dev.sync()
+        assert e.value.status == tb._lib.TQ_ENOMEM
+        assert all(np.array_equal(x, y) for x, y in zip(before, caches(b))) and all(np.array_equal(x, y) for x, y in zip(state, pool.state()))
+    b.decode_paged(tok, pool, 2, max_seq, lg, seqs=ints([2, 0]))       # and without asking once more
+    with pytest.raises(tb.TangqError) as e:
+        dev.sync()
+    assert e.value.status == tb._lib.TQ_EINVAL and all(np.array_equal(x, y) for x, y in zip(before, caches(b)))
+    pool.extend([2, 0], counts=[0, 0])                 # (no new position: still not)
+    b.decode_paged(tok, pool, 2, max_seq, lg, seqs=ints([2, 0]))
+    with pytest.raises(tb.TangqError):
+        dev.sync()
+    assert all(np.array_equal(x, y) for x, y in zip(before, caches(b)))
+    pool.free([5])
+    dev.upload_into(tok, np.arange(n) + 7)
+    graph.launch()
+    dev.sync()
+    got = dev.download(lg).reshape(n, V)
+    assert pool.state()[2].tolist() == [33] * 4 + [64, 0]
+    for j in range(n):                                 # as over slots
+        for p, t in enumerate([*prompt, *[j + 7] * 13]):
+            a.decode(ints([t]), ints([p]), 1, max_seq, lg)
+        want = dev.download(lg)[:V]
+        assert np.abs(got[j] - want).max() <= 2 * BAR * np.sqrt(np.mean(want.astype(np.float64) ** 2)), j
+    graph.free()
+    pool.destroy()
+    a.destroy()
+    b.destroy()
+
+
+def test_a_forked_sequence_is_not_stepped_before_it_is_extended(dev):
+    import tang_b200 as tb
+
+    host = host_model(24)
+    model = host.to_device(dev, 64, 4)
+    ints = lambda v: dev.upload(np.asarray(v, np.int32), tb.I32)
+    lg = dev.alloc(4 * host.vocab)
+    for n in (5, 16):
+        pool = model.page_pool(4, 16)
+        for t in range(n):
+            pool.extend([0])
+            model.decode_paged(ints([t]), pool, 1, 64, lg)
+        pool.fork([0], [2])
+        dev.sync()
+        before = caches(model)
+        for seqs in ([2], [0], [2, 0]):
+            model.decode_paged(ints([3, 4]), pool, len(seqs), 64, lg, seqs=ints(seqs))
+            with pytest.raises(tb.TangqError) as e:
+                dev.sync()
+            assert e.value.status == tb._lib.TQ_EINVAL
+            assert all(np.array_equal(x, y) for x, y in zip(before, caches(model)))
+        pool.extend([2, 0])
+        model.decode_paged(ints([3, 4]), pool, 2, 64, lg, seqs=ints([2, 0]))
+        dev.sync()
+        assert not all(np.array_equal(x, y) for x, y in zip(before, caches(model)))
+        pool.destroy()
+    model.destroy()
