@@ -31,14 +31,14 @@ __device__ __forceinline__ int paged_row_of(const PagedParams& p, int b) {
   return s >= 0 && s < p.n_seqs ? s : -1;
 }
 // ---------------------------------------------------------------------------------------------
-// Units, tiles, items, pieces.  A unit is what meets the same keys: the rows (member, query head of one KV head) of up to 128 / group members of a group
+// Units, tiles, runs, pieces.  A unit is what meets the same keys: the rows (member, query head of one KV head) of up to 128 / group members of a group
 // over the group's shared positions, in whole tiles of 128, or one sequence's query heads over the rest.  The tiles of all units of a KV head stand in
 // two lists, one of shared and one of own tiles, and every CTA, one an SM, takes a share of either: as many tiles of the one and of the other as everybody
-// else.  A long share is cut into items (kPuWindow).  CTAs that stand at the same place of the KV heads' lists are neighbours: a cache row holds all heads,
-// and its 256 bytes a head are fetched at the same time.  A piece is what an item has of a unit.  Its odd and its even tiles belong to different softmax
-// groups, which take scores from the same reference, so that the products of both go to the same columns (two sets of columns, for pieces that follow one
-// another).  It leaves a partial result; a second kernel joins those of a row, in the order of the list.
-// (64 sequences of 2048 positions and 8 KV heads take 97 us.  One list of all heads' tiles, cut for 148 CTAs rather than 144, took 98 us.  Shorter items,
+// else.  CTAs that stand at the same place of the KV heads' lists are neighbours: a cache row holds all heads, and its 256 bytes a head are fetched at the
+// same time.  A run is what a share has of a unit; a long one is cut into pieces (kPuWindow).  A piece's odd and even tiles belong to different softmax
+// groups, which take scores from the run's one reference, so that the products of both go to the same columns (two sets of columns, for pieces that follow
+// one another).  A run leaves a partial result, to which each of its pieces adds; a second kernel joins those of a row, in the order of the list.
+// (64 sequences of 2048 positions and 8 KV heads take 97 us.  One list of all heads' tiles, cut for 148 CTAs rather than 144, took 98 us.  Shorter shares,
 // handed out as CTAs get to them because SMs differ in speed by a fifth, took 102: they make more partial results than they balance.)
 //
 // What bounds it: the bytes of the cache, once, where sequences are long (537 MB in 97 us, 5.5 TB/s; the steady state is 2800 cycles for a tile of 64 KB,
@@ -52,34 +52,26 @@ constexpr int kPuTile = 4 * kPfBox / 2;               // bytes of 128 rows of ke
 constexpr int kPuRing = 5;
 constexpr int kPuWeights = 2 * 16 * 128;              // a parity's weights where keys are the lanes: two terms of eight rows of 128 keys, in two halves
 constexpr int kPuOnes = 1024;                         // eight rows of 64 ones
-constexpr int kPuMeet = (2 + 2) * 128 * 4;            // maxima [parity][warp][row], references [piece's parity][row, or warp and row]
+constexpr int kPuMeet = (2 + 2) * 128 * 4;            // maxima [parity][warp][row], references [run's parity][row, or warp and row]
 constexpr float kPuLargest = 7.9228162514264338e28f;  // 2^96: a weight above it is too far from its reference
 constexpr int kPuHeader = 640;                        // barriers, pieces
 constexpr int kPuReaders = 12;                        // warps that are told the pieces
 constexpr int kPuPieces = 4;                          // pieces that are told ahead
-// Tiles of an item at most, for f32 and for bf16 results: the tensor core truncates what it adds up, about 4e-9 of a sum for a position (64 sequences of 16384
-// positions in one piece each, with values of one sign, were off by 7e-5, in pieces of 2048 by 4e-6).
+// Tiles of a piece, for f32 and for bf16 results: the tensor core truncates what it adds up, about 4e-9 of a sum for a position (64 sequences of 16384
+// positions in one piece each, with values of one sign, were off by 7e-5, in pieces of 2048 by 4e-6).  Powers of two; only a run's first piece has another
+// number, 1 more at most and 2 at least: so the last tiles of a run's pieces have the same parity, and a thread that adds to a partial result adds to what
+// it wrote itself.
 constexpr int kPuWindow[2] = {16, 128};
-constexpr size_t kPuPartials = 256u << 20;            // bytes of partial results that shares are not cut further for
+__device__ __forceinline__ int pu_piece(int left, int window) { return left <= window + 1 ? left : ((left - 2) & (window - 1)) + 2; }
 constexpr int kPuBatch = 1024;                        // sequences of a call
 constexpr size_t kPuFixed = 2 * (size_t)kPfBox + kPuRing * (size_t)kPuTile + 2 * (size_t)kPuWeights + kPuOnes + kPuMeet + kPuHeader;
-
-// How a KV head's list is cut: CTAs' shares of `share` tiles, each in `parts` items of equal length but for a tile.
-struct PuCut {
-  int share, parts;
-  __device__ __forceinline__ int item(int f) const {                   // with tile f
-    const int cta = f / share;
-    return parts == 1 ? cta : cta * parts + (int)((long long)(f - cta * share) * parts / share);
-  }
-  __device__ __forceinline__ int first(int part) const { return parts == 1 ? part * share : (int)(((long long)part * share + parts - 1) / parts); }
-};
 
 // In shared memory, behind the buffers.
 struct PuPlan {
   int *own, *last, *pre;                              // [batch + 1] own tiles of the sequences before; [batch] shared tiles << 8 | keys of the last tile - 1;
                                                       // [groups + 1] units' shared tiles of the groups before
   int batch, groups, group, per_tile;
-  PuCut cut[2];                                       // own, shared tiles
+  int share[2];                                       // own, shared tiles of a CTA
 };
 // What the kernel that joins the pieces has to know: where a sequence's tiles stand in a KV head's list.
 struct PuSeqPlan {
@@ -127,8 +119,14 @@ __device__ __forceinline__ PuUnit pu_locate(const PagedParams& p, const PuPlan& 
 // A piece as the roles are told of it, in shared memory.
 struct __align__(16) PuPiece {
   int n, tile, last, rows;                            // tiles (0: there are no more pieces), the first one's place in the sequence, keys of the last one, rows
-  int kv, b0, seq, pre;                               // KV head, (first) sequence of the batch, its row of the tables, shared or not
-  int keyed, out, pad[2];                             // the keys are the lanes; first row of its partial results
+  int kv, b0, seq, out;                               // KV head, (first) sequence of the batch, its row of the tables; first row of its run's partial results
+  int what, pad[3];                                   // bits: see below
+  __device__ __forceinline__ bool pre() const { return what & 1; }                 // of shared tiles
+  __device__ __forceinline__ bool keyed() const { return what & 2; }               // the keys are the lanes
+  __device__ __forceinline__ bool later() const { return what & 4; }               // not its run's first piece
+  __device__ __forceinline__ bool more() const { return what & 8; }                // not its run's last piece
+  __device__ __forceinline__ int run() const { return (what >> 4) & 1; }           // the run's parity
+  __device__ __forceinline__ uint32_t phase() const { return (uint32_t)what >> 5; }       // and that of the runs before with the same
 };
 // Places in the ring, in the order in which they are needed: keys 0, keys 1, values 0, keys 2, values 1 ..
 __device__ __forceinline__ int pu_keys_at(int t) { return t == 0 ? 0 : 2 * t - 1; }
@@ -137,10 +135,10 @@ __device__ __forceinline__ int pu_values_at(int t) { return 2 * t + 2; }
 struct PuParams {
   PagedParams a;
   int per_tile, per_eight, n_shares;                  // members of a row tile; of eight rows; CTAs of a KV head
-  int window[2], most[2];                             // own, shared tiles: of an item, and items of a KV head, at most
+  int window;                                         // tiles of a piece
   float *own_o, *own_ml, *pre_o, *pre_ml;             // partial results: [row][128], [row][2] references and sums (of the groups)
   PuSeqPlan* plan;                                    // [batch]
-  PuCut* cut;                                         // [2]
+  int* share;                                         // [2]
 };
 
 template <typename F>
@@ -179,6 +177,8 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// LONG: there may be runs of several pieces.
+template <bool LONG>
 __global__ void __launch_bounds__(kPuThreads, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_constant__ CUtensorMap q_whole,
                     const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PuParams pp) {
@@ -200,7 +200,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
   uint64_t* piece_full = o_free + 2;                  // [kPuPieces]
   uint64_t* piece_empty = piece_full + kPuPieces;
   uint64_t* met = piece_empty + kPuPieces;            // [parity] the four warps of a softmax group
-  uint64_t* ref_full = met + 2;                       // [piece's parity]
+  uint64_t* ref_full = met + 2;                       // [run's parity]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ref_full + 2);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
   PuPiece* piece_s = reinterpret_cast<PuPiece*>(q_full) + (kPuHeader / sizeof(PuPiece) - kPuPieces);
@@ -299,10 +299,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
   const uint32_t tmem = *tmem_slot;
   const int pre_tiles = l.pre[l.groups], own_tiles = l.own[p.batch];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    l.cut[k].share = max(1, ((k ? pre_tiles : own_tiles) + pp.n_shares - 1) / pp.n_shares);
-    l.cut[k].parts = l.cut[k].share <= pp.window[k] ? 1 : (l.cut[k].share + pp.window[k] - 1) / pp.window[k];
-  }
+  for (int k = 0; k < 2; ++k) l.share[k] = max(1, ((k ? pre_tiles : own_tiles) + pp.n_shares - 1) / pp.n_shares);
   // One arrival for the warp.  The lanes meet before it and behind it: none may wait for what the arrival lets happen before it is made.
   auto arrive = [&](uint64_t* bar) {
     __syncwarp();
@@ -321,7 +318,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
   };
 
   if (warp == 12) {
-    // ---- what to do: the CTA's two items, in pieces
+    // ---- what to do: the CTA's two shares, in pieces
     bool ok = true;
     auto tell = [&](const PuPiece& w) {
       const int slot = told % kPuPieces;
@@ -339,26 +336,30 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
     // Own tiles first where there are several shared ones: the first burst of copies is the own tiles', which only one CTA reads, and shared ones find the
     // other heads' rows in L2 by the time they are needed (64 samples by fours 69.0 us, the other way 71.8; one prefix 41.5 and 42.2; but 8 samples with a
     // shared tile a CTA 16.9 and 16.4).
-    const bool own_first = l.cut[1].share > 1;
+    const bool own_first = l.share[1] > 1;
+    int run = 0;
 #pragma unroll 1
     for (int turn = 0; turn < 2 && ok; ++turn) {
       const int k = (turn == 0) != own_first;            // 1: shared tiles
-      const PuCut cut = k ? l.cut[1] : l.cut[0];
-      const int from = cut.share * cta, most = min(from + cut.share, k ? pre_tiles : own_tiles), apart = k ? 128 : 8;
-      int part = 0, end = min(from + cut.first(1), most);
-      w.pre = k;
-      for (int f = from; f < most && ok; f += w.n) {
-        if (f == end) end = min(from + cut.first(++part + 1), most);
+      const int share = k ? l.share[1] : l.share[0], from = share * cta, most = min(from + share, k ? pre_tiles : own_tiles), apart = k ? 128 : 8;
+      for (int f = from; f < most && ok;) {
         const PuUnit u = pu_locate(p, l, k, f);
-        w.n = min(end - f, u.tiles - u.tile);
+        int left = min(most - f, u.tiles - u.tile);
+        f += left;
+        const int last = u.tile + left == u.tiles ? u.last : kPfTile;
         w.tile = u.shared_tiles + u.tile;
-        w.last = u.tile + w.n == u.tiles ? u.last : kPfTile;
         w.rows = u.rows;
         w.b0 = u.b0;
         w.seq = max(paged_row_of(p, u.head), 0);
-        w.keyed = u.rows <= 8;
-        w.out = w.kv * (p.batch * p.group + apart * pp.most[k]) + u.b0 * p.group + apart * (cta * cut.parts + part);
-        tell(w);
+        w.out = w.kv * (p.batch * p.group + apart * pp.n_shares) + u.b0 * p.group + apart * cta;
+        w.what = k | (u.rows <= 8) << 1 | (run & 3) << 4;
+        for (++run; left > 0 && ok; w.what |= 4, w.tile += w.n) {
+          w.n = LONG ? pu_piece(left, pp.window) : left;
+          left -= w.n;
+          w.what = left > 0 ? w.what | 8 : w.what & ~8;
+          w.last = left > 0 ? kPfTile : last;
+          tell(w);
+        }
       }
     }
     w.n = 0;
@@ -383,14 +384,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
     for (int t = 0; next.n && ok;) {
       w = next;
       if (values) {
-        const int slot = w.pre ? 0 : own_pieces++ & 3;
+        const int slot = w.pre() ? 0 : own_pieces++ & 3;
         for (int k = 0; k < 4; ++k)
-          if (ok && (w.pre || k == slot)) {
+          if (ok && (w.pre() || k == slot)) {
             ok = __all_sync(0xffffffffu, mbar_wait_spin(&q_empty[k], ((q_used >> k) & 1u) ^ 1u));
             q_used ^= 1u << k;
           }
         if (!ok) break;
-        const bool whole = !w.keyed;
+        const bool whole = !w.keyed();
         const uint32_t rows = (uint32_t)((whole ? pp.per_tile : pp.per_eight) * p.group);
         if (lane == 0) mbar_arrive_expect_tx(&q_full[slot], 2u * rows * 128u);
         __syncwarp();
@@ -442,10 +443,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
         }
         pp.plan[b] = PuSeqPlan{l.own[b], l.own[b + 1] - l.own[b], pre_f, shared};
       }
-      if (lane == 0) {
-        pp.cut[0] = l.cut[0];
-        pp.cut[1] = l.cut[1];
-      }
+      if (lane < 2) pp.share[lane] = lane ? l.share[1] : l.share[0];
       __syncwarp();
     }
     uint32_t used = 0;                 // phases of v_raw
@@ -518,7 +516,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
     PuPiece w;
     int own_pieces = 0, t = 0, piece = 0;
     for (take(ok, w); w.n && ok; piece ^= 1, take(ok, w)) {
-      const int q_slot = w.pre ? 0 : own_pieces++ & 3;
+      const int q_slot = w.pre() ? 0 : own_pieces++ & 3;
       ok = __all_sync(0xffffffffu, mbar_wait_spin(&q_full[q_slot], (q_seen >> q_slot) & 1u));
       q_seen ^= 1u << q_slot;
       for (int i = 0; i < w.n && ok; ++i, ++t) {
@@ -529,7 +527,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
         if (!ok) break;
         tc_fence_after();
         const int keys = i == w.n - 1 ? w.last : kPfTile;
-        const Tile now{(keys + 15) >> 4, w.keyed != 0, i == 0, piece};
+        const Tile now{(keys + 15) >> 4, w.keyed(), i == 0, piece};
         if (leader) {
           const uint32_t s_t = tmem + (uint32_t)(x * 128);
           const uint32_t idesc = umma_idesc_bf16(now.keyed ? 16 : kPfTile);
@@ -544,7 +542,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
           umma_commit(&kv_empty[slot]);
           if (i == w.n - 1)
             for (int k = 0; k < 4; ++k)
-              if (w.pre || k == q_slot) umma_commit(&q_empty[k]);
+              if (w.pre() || k == q_slot) umma_commit(&q_empty[k]);
         }
         __syncwarp();
         if (t > 0) ok = values(t - 1, before);
@@ -561,21 +559,21 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
     // A weight is two bf16 terms, hi + lo, within 2^-16 of it, as in the attention over slots.  (Three would be nearer to f32 results, whose error from
     // 64 bits is 2e-6 so and 8e-7 by f32 arithmetic, but tensor memory has no columns for them.  One, within 2^-8, would be as far off as the rounding of a
     // bf16 result.)
-    // The reference that scores are taken from is their maximum in the piece's first tile, which the group with that tile tells the other one: a bf16 weight
+    // The reference that scores are taken from is their maximum in the run's first tile, which the group with that tile tells the other one: a bf16 weight
     // may be as large as an f32 one, so that nothing is rescaled; a weight above 2^96 becomes no number, and the joining kernel goes through the row's keys
     // one by one.
     const int x = (warp - 4) >> 2, q4 = warp & 3, t128 = 32 * q4 + lane;
     const uint32_t s_t = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)(x * 128);
     uint32_t o_t = 0;                  // of the piece
-    float *max_s = meet_s + x * 128, *ref_s = nullptr;                 // [warp][8 rows]; the piece's references
+    float *max_s = meet_s + x * 128, *ref_s = nullptr;                 // [warp][8 rows]; the run's references
     int meetings = 0;
-    bool ok = true, first = true, leads = true;      // the group's first tile of the piece; it is the piece's first
+    bool ok = true, first = true, leads = true;      // the group's first tile of the run; it is the piece's first
     int slot = 0;                      // the piece's parity
     auto meet = [&]() {                // (a barrier of the group whose wait ends, as every other's)
       arrive(&met[x]);
       ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(&met[x], (uint32_t)(meetings++ & 1)));
     };
-    float ref = 0.f, sum_all = 0.f;    // of the thread's row, where rows are the lanes
+    float ref = 0.f, sum_all = 0.f;    // of the thread's row, and its weights' sum in the run
     int done = 0;                      // tiles of this parity
     PuPiece u{};
     // a tile whose lanes are keys
@@ -595,7 +593,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
         const int r = lane & 7;
         const float mx = fmaxf(fmaxf(max_s[r], max_s[8 + r]), fmaxf(max_s[16 + r], max_s[24 + r]));
         if (lane < 8) ref_s[8 * q4 + lane] = mx == -FLT_MAX ? mx : mx * p.scale_log2;      // (a copy for every warp)
-        arrive(&ref_full[slot]);
+        arrive(&ref_full[u.run()]);
       }
       const float4 f0 = *reinterpret_cast<const float4*>(&ref_s[8 * q4]), f1 = *reinterpret_cast<const float4*>(&ref_s[8 * q4 + 4]);
       if (first) ref = ref_s[8 * q4 + (lane & 7)];
@@ -615,7 +613,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     };
     auto keyed_out = [&](float* to_o, float* to_ml) {
-      float o[8], low[8], sum[8], sum_low[8];
+      float o[8], low[8], sum[8], sum_low[8], was[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) was[r] = LONG && u.later() && r < u.rows ? to_o[r * kPaDim + t128] : 0.f;
       __syncwarp();
       tmem_ld8(o_t, o);
       tmem_ld8(o_t + 8u, low);
@@ -626,10 +626,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
       float l = 0.f;                                   // of the lane's row
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        if (r < u.rows) to_o[r * kPaDim + t128] = o[r] + low[r];
+        if (r < u.rows) to_o[r * kPaDim + t128] = was[r] + (o[r] + low[r]);
         if (lane == r) l = sum[r] + sum_low[r];
       }
-      if (q4 == 0 && lane < u.rows) *reinterpret_cast<float4*>(to_ml + lane * 4) = make_float4(ref, l, ref, 0.f);
+      sum_all = LONG && u.later() ? sum_all + l : l;
+      if (!(LONG && u.more()) && q4 == 0 && lane < u.rows) *reinterpret_cast<float4*>(to_ml + lane * 4) = make_float4(ref, sum_all, ref, 0.f);
     };
     int t0 = 0, piece = 0;             // tiles and pieces before the piece
     for (take(ok, u); u.n && ok; t0 += u.n, ++piece, take(ok, u)) {
@@ -637,17 +638,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
       leads = place == 0;
       slot = piece & 1;
       o_t = tmem + ((uint32_t)(32 * q4) << 16) + 256u + (uint32_t)(slot * 128);
-      ref_s = meet_s + 256 + slot * 128;
-      float *to_o = (u.pre ? pp.pre_o : pp.own_o) + (size_t)u.out * kPaDim, *to_ml = (u.pre ? pp.pre_ml : pp.own_ml) + (size_t)u.out * 4;
+      ref_s = meet_s + 256 + u.run() * 128;
+      float *to_o = (u.pre() ? pp.pre_o : pp.own_o) + (size_t)u.out * kPaDim, *to_ml = (u.pre() ? pp.pre_ml : pp.own_ml) + (size_t)u.out * 4;
       for (int i = place; i < u.n && ok; i += 2) {
-        first = i == place;
+        first = i == place && !(LONG && u.later());
         const int r = 32 * q4 + lane;
         const bool live = r < u.rows;
         ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[x], (uint32_t)(done & 1)) &&
-                                         (!first || leads || mbar_wait_spin(&ref_full[slot], (uint32_t)((piece >> 1) & 1))));
+                                         (!first || leads || mbar_wait_spin(&ref_full[u.run()], u.phase())));
         if (!ok) break;
         tc_fence_after();
-        if (u.keyed) {
+        if (u.keyed()) {
           keyed(t128 < (i == u.n - 1 ? u.last : kPfTile));
         } else {
           __syncwarp();
@@ -661,7 +662,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
               for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[j]);
             }
             ref_s[r] = mx == -FLT_MAX ? mx : mx * p.scale_log2;
-            arrive(&ref_full[slot]);
+            arrive(&ref_full[u.run()]);
           }
           if (first) {
             ref = ref_s[r];
@@ -708,19 +709,19 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
         }
         arrive(&p_full[x]);
         ++done;
-        // (a sum each of the two groups; a piece of one tile has one)
-        if (!u.keyed && live && i + 2 >= u.n) {
+        // (a sum each of the two groups; a run of one tile has one)
+        if (!u.keyed() && live && i + 2 >= u.n && !(LONG && u.more())) {
           const float2 ml = make_float2(ref, sum_all > kPuLargest ? NAN : sum_all);
           if (u.n > 1) *reinterpret_cast<float2*>(to_ml + r * 4 + 2 * place) = ml;
           else *reinterpret_cast<float4*>(to_ml + r * 4) = make_float4(ml.x, ml.y, ml.x, 0.f);
         }
         if (i + 1 < u.n) continue;
 
-        // ---- the piece's result, by the group that has its last tile
+        // ---- the piece's result, by the group that has its last tile (the same for all pieces of a run)
         ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[x], (uint32_t)((done - 1) & 1)));
         if (!ok) break;
         tc_fence_after();
-        if (u.keyed) {
+        if (u.keyed()) {
           keyed_out(to_o, to_ml);
         } else {
 #pragma unroll 1
@@ -730,6 +731,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
             pf_ld32(o_t + (uint32_t)c, o);
             if (live) {
               float* o_row = to_o + (size_t)r * kPaDim + c;          // (whole sectors: 32 bytes a store)
+              if (LONG && u.later())
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                  const float4 was = *reinterpret_cast<const float4*>(o_row + j);
+                  o[j] += was.x;
+                  o[j + 1] += was.y;
+                  o[j + 2] += was.z;
+                  o[j + 3] += was.w;
+                }
 #pragma unroll
               for (int j = 0; j < 32; j += 8) st_global8(o_row + j, &o[j]);
             }
@@ -761,11 +771,11 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
   const PagedParams& p = pp.a;
   const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const PuSeqPlan q = pp.plan[b];
-  const PuCut cut[2] = {pp.cut[0], pp.cut[1]};
+  const int own_share = pp.share[0], pre_share = pp.share[1];
   const int kv = head / p.group, h = head - kv * p.group;
-  // items of the row's own and shared tiles
-  const int own_c = cut[0].item(q.own_f), pre_c = cut[1].item(q.pre_f);
-  const int own = q.own_tiles ? cut[0].item(q.own_f + q.own_tiles - 1) - own_c + 1 : 0, pre = q.pre_tiles ? cut[1].item(q.pre_f + q.pre_tiles - 1) - pre_c + 1 : 0;
+  // CTAs (of the KV head) with the row's own and shared tiles
+  const int own_c = q.own_f / own_share, pre_c = q.pre_f / pre_share;
+  const int own = q.own_tiles ? (q.own_f + q.own_tiles - 1) / own_share - own_c + 1 : 0, pre = q.pre_tiles ? (q.pre_f + q.pre_tiles - 1) / pre_share - pre_c + 1 : 0;
   float top = -FLT_MAX, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int base = 0; base < own + pre; base += 32) {
     // a lane per partial result: its row, reference and sums
@@ -774,8 +784,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
     float4 mine = make_float4(-FLT_MAX, 0.f, 0.f, 0.f);
     if (i < own + pre) {
       const bool k = i >= own;
-      const int item = k ? pre_c + i - own : own_c + i, apart = k ? 128 : 8;
-      const size_t r = (size_t)kv * (p.batch * p.group + apart * pp.most[k]) + b * p.group + h + (size_t)apart * item;
+      const int cta = k ? pre_c + i - own : own_c + i, apart = k ? 128 : 8;
+      const size_t r = (size_t)kv * (p.batch * p.group + apart * pp.n_shares) + b * p.group + h + (size_t)apart * cta;
       row = (k ? pp.pre_o : pp.own_o) + r * kPaDim;
       mine = *reinterpret_cast<const float4*>((k ? pp.pre_ml : pp.own_ml) + r * 4);
     }
@@ -896,25 +906,19 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   const size_t most_ctas = tiles < (size_t)ctx->sm_count ? tiles : (size_t)ctx->sm_count;
   pp.n_shares = (int)(most_ctas > n_kv_heads ? most_ctas / n_kv_heads : 1);
   const size_t n_ctas = pp.n_shares * n_kv_heads;
-  // partial results (rows of either kind: the list's, and what an item adds), the sequences' plans
-  size_t part_rows[2];
-  for (int k = 0; k < 2; ++k) {
-    const size_t len = k ? (size_t)p.max_shared / kPfTile : ((size_t)p.max_len + kPfTile - 1) / kPfTile, units = k ? p.n_groups + batch / pp.per_tile : batch;
-    const size_t share = (units * len + pp.n_shares - 1) / pp.n_shares;
-    for (pp.window[k] = kPuWindow[!p.out_f32];; pp.window[k] *= 2) {
-      pp.most[k] = (int)(pp.n_shares * (share / pp.window[k] + 1));
-      part_rows[k] = k && !p.n_groups ? 0 : batch * n_heads + (k ? 128 : 8) * n_kv_heads * pp.most[k];
-      if (share <= (size_t)pp.window[k] || part_rows[k] * (kPaDim + 4) * sizeof(float) <= kPuPartials) break;
-    }
-  }
-  const size_t own_rows = part_rows[0], pre_rows = part_rows[1], floats = (own_rows + pre_rows) * (kPaDim + 4);
+  // partial results (rows of either kind: the list's, and what a CTA adds), the sequences' plans
+  // (The form without LONG has less code to fetch: one sequence of 700 positions 9.3 us, with it 9.8; 16 groups of four samples 40.5 and 41.6.)
+  pp.window = kPuWindow[!p.out_f32];
+  const size_t longest = ((size_t)p.max_len + kPfTile - 1) / kPfTile;      // (tiles of a run: no more than a sequence has)
+  auto kern = longest > (size_t)pp.window + 1 ? paged_decode_kernel<true> : paged_decode_kernel<false>;
+  const size_t own_rows = batch * n_heads + 8 * n_ctas, pre_rows = p.n_groups ? batch * n_heads + 128 * n_ctas : 0, floats = (own_rows + pre_rows) * (kPaDim + 4);
   if (int st = ensure_scratch(ctx, floats * sizeof(float) + (batch + 1) * sizeof(PuSeqPlan))) return st;
   pp.own_o = static_cast<float*>(ctx->scratch);
   pp.pre_o = pp.own_o + own_rows * kPaDim;
   pp.own_ml = pp.pre_o + pre_rows * kPaDim;
   pp.pre_ml = pp.own_ml + own_rows * 4;
   pp.plan = reinterpret_cast<PuSeqPlan*>(pp.pre_ml + pre_rows * 4);
-  pp.cut = reinterpret_cast<PuCut*>(pp.plan + batch);
+  pp.share = reinterpret_cast<int*>(pp.plan + batch);
   pp.a = p;
   CUtensorMap qe, qw, km, vm;
   const size_t row = n_kv_heads * kPaDim, rows = (size_t)p.n_pages * pages->page_rows;
@@ -924,8 +928,8 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
       !encode_pages(&vm, v_pages_dev, row, rows, box))
     return fail(ctx, TQ_ECUDA, "cuTensorMapEncodeTiled failed");
   const size_t smem = kPuFixed + (2 * batch + 1 + (size_t)p.n_groups + 1) * sizeof(int);
-  TQ_CUDA(ctx, cudaFuncSetAttribute(paged_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kPuFixed + (3 * kPuBatch + 2) * sizeof(int))));
-  TQ_CUDA(ctx, launch_k(ctx, paged_decode_kernel, dim3((unsigned)n_ctas), dim3(kPuThreads), smem, qe, qw, km, vm, pp));
+  TQ_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kPuFixed + (3 * kPuBatch + 2) * sizeof(int))));
+  TQ_CUDA(ctx, launch_k(ctx, kern, dim3((unsigned)n_ctas), dim3(kPuThreads), smem, qe, qw, km, vm, pp));
   TQ_CUDA(ctx, launch_k(ctx, paged_join_kernel, dim3((unsigned)n_heads, (unsigned)batch), dim3(128), 0, pp));
   return TQ_OK;
 }

@@ -406,3 +406,46 @@ def test_bf16_results_are_off_by_their_own_rounding(dev, name):
     off = 2.0 ** -14 * size
     err = np.abs(got.reshape(want.shape) - want) / (off + 2.0 ** -8 * (np.abs(want) + off) + 1e-30)
     assert err.max() <= 1, (err.max(), np.unravel_index(err.argmax(), err.shape))
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_a_loose_bound_costs_no_precision(dev, shared):
+    """As ``test_long_sums_keep_the_precision_of_f32``, with the bounds of a caller who has recorded a graph for any length: eight KV heads, tables for a
+    million positions.  A piece has 2176 positions at most."""
+    import tang_b200 as tb
+
+    rng, L, P, B, nh, nkv, ld = np.random.default_rng(28), 16384, 128, 64, 32, 8, 8192
+    n_pages, most = L // P, ld * P
+    k_bits, k = bf16_round(rng.standard_normal((L, nkv, HD)).astype(np.float32))
+    v_bits, v = bf16_round((1 + 0.1 * rng.standard_normal((L, nkv, HD))).astype(np.float32))
+    q_bits, q = bf16_round(rng.standard_normal((B, nh, HD)).astype(np.float32))
+    tables = np.full((B, ld), -1, np.int32)
+    tables[:, :n_pages] = np.arange(n_pages)
+    pool = tb.PagePool(dev, n_pages, P, B, ld, None, dev.upload(np.full(n_pages, B, np.int32), tb.I32), dev.upload(tables, tb.I32),
+                       dev.upload(np.full(B, L, np.int32), tb.I32))
+    kw = dict(group_starts=dev.upload(np.zeros(1, np.int32), tb.I32), shared=dev.upload(np.full(1, L, np.int32), tb.I32), n_groups=1, max_shared=most) if shared else {}
+    got = dev.gqa_decode_paged(dev.upload(q_bits.reshape(-1), tb.BF16), dev.upload(k_bits.reshape(-1), tb.BF16), dev.upload(v_bits.reshape(-1), tb.BF16), pool, B, nh, nkv,
+                               HD, most, out_dtype=tb.F32, **kw).to_vec().reshape(B, nh, HD)
+    dev.sync()
+    for b, h in ((0, 0), (31, 17), (63, 31)):
+        s = k[:, h // 4].reshape(L, HD).astype(np.float64) @ q[b, h].reshape(HD).astype(np.float64) / np.sqrt(HD)
+        w = np.exp(s - s.max())
+        want = w @ v[:, h // 4].reshape(L, HD).astype(np.float64) / w.sum()
+        assert np.abs(got[b, h] / want - 1).max() <= 2.0 ** -17 + 2176 * 6e-9, (b, h)
+    pool.destroy()
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_runs_of_several_pieces(dev, f32):
+    """One CTA for each of 75 KV heads: runs that end at, before and behind the tiles of a piece, of three rows and of nine."""
+    if f32:
+        groups = [(0, [n]) for n in (1, 2048, 2049, 2177, 2305, 4225)] + [(2500, [2500, 2540, 2600]), (2176, [2180, 2177, 2300])]
+    else:
+        groups = [(0, [16513]), (0, [300]), (16900, [16901, 16900, 17000])]
+    s = Setup(225, 75, 128, groups, seed=51).put(dev)
+    want = s.reference()
+    s.reference = lambda: want
+    for grouped in (True, False):
+        got = s.run(f32, grouped=grouped).to_vec()
+        dev.sync()
+        s.check(got, f32)
