@@ -821,8 +821,10 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
     o[3] += v.w;
   }
   const size_t at = ((size_t)b * p.n_heads + head) * kPaDim + 4 * lane;
-  if (__any_sync(0xffffffffu, l != l || o[0] != o[0] || o[1] != o[1] || o[2] != o[2] || o[3] != o[3])) {
-    // A score far above those of its unit's first tile, or an infinite value beside a weight that is zero as a second term: once more, key by key.
+  const float largest = fmaxf(fmaxf(fabsf(o[0]), fabsf(o[1])), fmaxf(fabsf(o[2]), fabsf(o[3])));
+  if (__any_sync(0xffffffffu, !(l + largest <= FLT_MAX) || o[0] != o[0] || o[1] != o[1] || o[2] != o[2] || o[3] != o[3])) {
+    // A score far above those of its run's first tile, whose weight, or weight times value, is no f32 number any more, or an infinite value beside a weight
+    // that is zero as a second term: once more, key by key.
     const int s = paged_row_of(p, b), len = s < 0 ? 0 : min(max(p.lens[s], 0), p.max_len);
     float m = -FLT_MAX, x[4];
     l = o[0] = o[1] = o[2] = o[3] = 0.f;

@@ -449,3 +449,33 @@ def test_runs_of_several_pieces(dev, f32):
         got = s.run(f32, grouped=grouped).to_vec()
         dev.sync()
         s.check(got, f32)
+
+
+def later_keys_weigh_more(s, factor):
+    """Makes the scores of a set-up grow along each sequence: `factor` (natural logarithm) for every 128 positions, q . k / sqrt(128) = 1.5 * sqrt(128) * k."""
+    for b in range(s.B):
+        for j in range(int(s.lens[b])):
+            page, r = s.tables[b, j // s.P], j % s.P
+            bits, f = bf16_round(np.full((s.nkv, HD), factor * (j // 128) / (1.5 * np.sqrt(HD)), np.float32))
+            s.kv_bits[0, page, r], s.kv[0, page, r] = bits.reshape(f.shape), f
+    s.q_bits, s.q = (a.reshape(s.q.shape) for a in bf16_round(np.full(s.q.shape, 1.5, np.float32)))
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_large_values_under_weights_far_above_their_reference(dev, f32):
+    """Weights of 2^64 against the first tile's, which are f32 numbers, and values of 1e18, whose weighted sum is none: the result is one."""
+    s = Setup(225, 75, 16, [(256, [300, 270, 290]), (0, [200]), (256, [256] * 3), (0, [256])], seed=61)       # (a CTA for each KV head)
+    later_keys_weigh_more(s, 44.4)                                     # 2^64 for each tile
+    s.kv_bits[1], s.kv[1] = (a.reshape(s.kv[1].shape) for a in bf16_round((1 + 0.1 * s.kv[1]) * np.float32(1e18)))
+    for b in range(s.B):
+        if s.lens[b] % 16:
+            s.kv_bits[1, s.tables[b, s.lens[b] // 16], s.lens[b] % 16:] = NAN
+    s.put(dev)
+    want, size = s.reference()
+    for grouped in (True, False):
+        got = s.run(f32, grouped=grouped).to_vec()
+        dev.sync()
+        g = (got.astype(np.float64) if f32 else (got.astype(np.uint32) << 16).view(np.float32).astype(np.float64)).reshape(want.shape)
+        # scores up to 3 * 44.4, a sum of 128 products: off by 2^-24 of it a product
+        off = (2.0 ** -14 + 128 * 133 * 2.0 ** -24) * size
+        assert np.isfinite(g).all() and (np.abs(g - want) <= off + (0 if f32 else 2.0 ** -8) * (np.abs(want) + off)).all()
