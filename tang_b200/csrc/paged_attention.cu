@@ -824,14 +824,21 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
   const float largest = fmaxf(fmaxf(fabsf(o[0]), fabsf(o[1])), fmaxf(fabsf(o[2]), fabsf(o[3])));
   if (__any_sync(0xffffffffu, !(l + largest <= FLT_MAX) || o[0] != o[0] || o[1] != o[1] || o[2] != o[2] || o[3] != o[3])) {
     // A score far above those of its run's first tile, whose weight, or weight times value, is no f32 number any more, or an infinite value beside a weight
-    // that is zero as a second term: once more, key by key.
+    // that is zero as a second term: once more, key by key, the shared tiles' from the group's first sequence.
     const int s = paged_row_of(p, b), len = s < 0 ? 0 : min(max(p.lens[s], 0), p.max_len);
     float m = -FLT_MAX, x[4];
     l = o[0] = o[1] = o[2] = o[3] = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(p.q[at + i]);
+    int head_s = s;                    // whose pages
+    if (q.pre_tiles) {
+      int g = p.n_groups - 1;          // the last group that starts there or before
+      while (g > 0 && pu_group_start(p, g) > b) --g;
+      head_s = max(paged_row_of(p, pu_group_start(p, g)), 0);
+    }
     for (int j = 0; j < len; ++j) {
-      const int page = min(max(p.tables[(size_t)s * p.table_ld + (j >> p.page_shift)], 0), p.n_pages - 1);
+      const int from = j < q.pre_tiles * kPfTile ? head_s : s;
+      const int page = min(max(p.tables[(size_t)from * p.table_ld + (j >> p.page_shift)], 0), p.n_pages - 1);
       const size_t r = (((size_t)page << p.page_shift) + (j & ((1 << p.page_shift) - 1))) * p.n_kv * kPaDim + (size_t)kv * kPaDim;
       attend_row(p.k + r, 0, p.v + r, 0, 0, 1, x, p.scale_log2, lane, m, l, o);
     }

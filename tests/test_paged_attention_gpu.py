@@ -479,3 +479,19 @@ def test_large_values_under_weights_far_above_their_reference(dev, f32):
         # scores up to 3 * 44.4, a sum of 128 products: off by 2^-24 of it a product
         off = (2.0 ** -14 + 128 * 133 * 2.0 ** -24) * size
         assert np.isfinite(g).all() and (np.abs(g - want) <= off + (0 if f32 else 2.0 ** -8) * (np.abs(want) + off)).all()
+
+
+def test_shared_positions_are_the_first_sequences_whatever_the_scores(dev):
+    """What the other members' tables say of the shared positions counts as little for a row that is attended key by key."""
+    for factor in (0.0, 80.0):
+        s = Setup(225, 75, 16, [(256, [300, 270, 290]), (0, [500])], seed=62)               # (a CTA for each KV head)
+        later_keys_weigh_more(s, factor)
+        true = s.tables.copy()
+        s.put(dev)
+        other = true.copy()
+        other[1, :16], other[2, :16] = true[3, 1:17], true[3, 15::-1]  # pages of the sequence behind the group
+        dev.upload_into(s.pool.tables, other)
+        got = s.run(True).to_vec().reshape(s.B, 225, HD)
+        dev.sync()
+        want, size = s.reference()
+        assert (np.abs(got - want) <= (2.0 ** -14 + 128 * 4 * factor * 2.0 ** -24) * size).all(), factor
