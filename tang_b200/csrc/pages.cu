@@ -74,6 +74,20 @@ __device__ __forceinline__ int find_pages(const int* refs, int from, int end, bo
   return found;
 }
 
+// Whether tables name a page that does not exist (this library did not write them): of sequences seqs[i] the first pages_of(lens[i]) entries, a warp per
+// sequence, and for the whole CTA.
+__device__ __forceinline__ bool names_no_page(const PagesParams& p, const int* seqs, const int* lens, int n) {
+  bool none = false;
+  for (int i = threadIdx.x >> 5; i < n; i += kBookThreads / 32) {
+    const int pages = pages_of(lens[i], p.page_rows);
+    for (int j = threadIdx.x & 31; j < pages; j += 32) {
+      const int page = p.tables[(size_t)seqs[i] * p.table_ld + j];
+      none = none || page < 0 || page >= p.n_pages;
+    }
+  }
+  return __syncthreads_or(none);
+}
+
 // One sequence per thread: valid, and in the list once.  (The mark is taken back by the threads that set it.)
 __device__ __forceinline__ bool mark_once(const PagesParams& p, int s) {
   return s >= 0 && s < p.n_seqs && atomicExch(&p.marks[s], 1) == 0;
@@ -184,14 +198,11 @@ __global__ void __launch_bounds__(kBookThreads) pages_fork_kernel(const PagesPar
   len_s[t] = len;
   bad = __syncthreads_or(bad);
   if (marked) p.marks[d] = 0;
+  if (!bad) bad = names_no_page(p, src_s, len_s, n);
   for (int i = t >> 5; i < n && !bad; i += kBookThreads / 32) {      // a warp per pair
     const int pages = pages_of(len_s[i], p.page_rows);
     for (int j = t & 31; j < pages; j += 32) {
       const int page = p.tables[(size_t)src_s[i] * p.table_ld + j];
-      if (page < 0 || page >= p.n_pages) {             // (a table that this library did not write)
-        atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
-        continue;
-      }
       atomicAdd(&p.refs[page], 1);
       p.tables[(size_t)dst_s[i] * p.table_ld + j] = page;
     }
@@ -223,14 +234,14 @@ __global__ void __launch_bounds__(kBookThreads) pages_free_kernel(const PagesPar
   len_s[t] = len;
   bad = __syncthreads_or(bad);
   if (marked) p.marks[s] = 0;
+  if (!bad) bad = names_no_page(p, seq_s, len_s, n);
   for (int i = t >> 5; i < n && !bad; i += kBookThreads / 32) {
     const int pages = pages_of(len_s[i], p.page_rows);
     for (int j = t & 31; j < pages; j += 32) {
       int* at = &p.tables[(size_t)seq_s[i] * p.table_ld + j];
       const int page = *at;
       *at = -1;
-      if (page < 0 || page >= p.n_pages) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
-      else atomicSub(&p.refs[page], 1);
+      atomicSub(&p.refs[page], 1);
     }
   }
   if (bad) {

@@ -215,3 +215,27 @@ def test_calls_recorded_in_a_graph(dev):
         b.copy(b.want.extend([2, 0, 1]))
     b.check()
     g.free()
+
+
+@pytest.mark.parametrize("page", [-1, 12, 2 ** 31 - 1, -2 ** 31])
+def test_a_table_with_a_page_that_does_not_exist_changes_nothing(dev, page):
+    """Of a caller's tables: the second of three sequences names such a page behind good ones."""
+    import tang_b200 as tb
+
+    refs, tables, lens = np.zeros(12, np.int32), np.full((6, 4), -1, np.int32), np.array([40, 33, 5, 0, 0, 0], np.int32)
+    tables[0, :3], tables[1, :3], tables[2, 0] = [7, 1, 3], [2, 0, page], 9
+    refs[[7, 1, 3, 2, 0, 9]] = 1
+    data = np.random.default_rng(0).integers(0, 1 << 16, (12, 16, 8)).astype(np.uint16)
+    caches = dev.upload(data, tb.BF16)
+    pool = tb.PagePool(dev, 12, 16, 6, 4, [caches], *(dev.upload(a, tb.I32) for a in (refs, tables, lens)))
+    for call in (lambda: pool.fork([0, 1, 2], [3, 4, 5]), lambda: pool.fork([1], [4], keep=[33]), lambda: pool.free([0, 1, 2]), lambda: pool.extend([0, 1, 2])):
+        call()
+        with pytest.raises(tb.TangqError) as e:
+            dev.sync()
+        assert e.value.status == tb._lib.TQ_EINVAL
+        assert all(np.array_equal(a, b) for a, b in zip(pool.state(), (refs, tables, lens))) and np.array_equal(caches.to_vec().reshape(data.shape), data)
+    pool.fork([0, 1], [3, 4], keep=[40, 32])           # (the page is not among these)
+    pool.free([0, 3, 4, 2])
+    dev.sync()
+    assert pool.state()[2].tolist() == [0, 33, 0, 0, 0, 0] and pool.state()[0].tolist() == [1, 0, 1] + [0] * 9
+    pool.destroy()
