@@ -765,7 +765,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
 // Joins the partial results of a query head, in their order: a CTA, every fourth result a warp, four columns a lane.  It is launched while the kernel
 // above runs and fits beside it (that one is held to 128 registers a thread), so that nothing but loads stands between the last piece and the result.
 __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
-  __shared__ float4 part[3][32];
+  __shared__ float4 part[4][32];
+  __shared__ float2 part_ml[4];
+  __shared__ bool again;
   pdl_wait();
   pdl_launch_dependents();
   const PagedParams& p = pp.a;
@@ -809,40 +811,97 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PuParams pp) {
       o[3] = fmaf(v[k].w, wk, o[3]);
     }
   }
-  if (warp) part[warp - 1][lane] = make_float4(o[0], o[1], o[2], o[3]);
+  if (warp) part[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
   __syncthreads();
-  if (warp) return;
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    const float4 v = part[k][lane];
-    o[0] += v.x;
-    o[1] += v.y;
-    o[2] += v.z;
-    o[3] += v.w;
-  }
   const size_t at = ((size_t)b * p.n_heads + head) * kPaDim + 4 * lane;
-  const float largest = fmaxf(fmaxf(fabsf(o[0]), fabsf(o[1])), fmaxf(fabsf(o[2]), fabsf(o[3])));
-  if (__any_sync(0xffffffffu, !(l + largest <= FLT_MAX) || o[0] != o[0] || o[1] != o[1] || o[2] != o[2] || o[3] != o[3])) {
-    // A score far above those of its run's first tile, whose weight, or weight times value, is no f32 number any more, or an infinite value beside a weight
-    // that is zero as a second term: once more, key by key, the shared tiles' from the group's first sequence.
-    const int s = paged_row_of(p, b), len = s < 0 ? 0 : min(max(p.lens[s], 0), p.max_len);
-    float m = -FLT_MAX, x[4];
-    l = o[0] = o[1] = o[2] = o[3] = 0.f;
+  if (warp == 0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(p.q[at + i]);
+    for (int k = 1; k < 4; ++k) {
+      const float4 v = part[k][lane];
+      o[0] += v.x;
+      o[1] += v.y;
+      o[2] += v.z;
+      o[3] += v.w;
+    }
+    const float largest = fmaxf(fmaxf(fabsf(o[0]), fabsf(o[1])), fmaxf(fabsf(o[2]), fabsf(o[3])));
+    const bool bad = __any_sync(0xffffffffu, !(l + largest <= FLT_MAX) || o[0] != o[0] || o[1] != o[1] || o[2] != o[2] || o[3] != o[3]);
+    if (lane == 0) again = bad;
+  }
+  __syncthreads();
+  if (again) {
+    // A score far above those of its run's first tile, whose weight, or weight times value, is no f32 number any more, or an infinite value beside a weight
+    // that is zero as a second term: once more, four keys a warp at a time, the shared tiles' from the group's first sequence.  (One sequence of 100000
+    // positions 14 ms, 105 by one warp and key by key; 0.1 where no row is attended again.)
+    const int s = paged_row_of(p, b), len = s < 0 ? 0 : min(max(p.lens[s], 0), p.max_len);
     int head_s = s;                    // whose pages
     if (q.pre_tiles) {
       int g = p.n_groups - 1;          // the last group that starts there or before
       while (g > 0 && pu_group_start(p, g) > b) --g;
       head_s = max(paged_row_of(p, pu_group_start(p, g)), 0);
     }
-    for (int j = 0; j < len; ++j) {
-      const int from = j < q.pre_tiles * kPfTile ? head_s : s;
-      const int page = min(max(p.tables[(size_t)from * p.table_ld + (j >> p.page_shift)], 0), p.n_pages - 1);
-      const size_t r = (((size_t)page << p.page_shift) + (j & ((1 << p.page_shift) - 1))) * p.n_kv * kPaDim + (size_t)kv * kPaDim;
-      attend_row(p.k + r, 0, p.v + r, 0, 0, 1, x, p.scale_log2, lane, m, l, o);
+    float m = -FLT_MAX, x[4];
+    l = o[0] = o[1] = o[2] = o[3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(p.q[at + i]);
+    auto four = [](const __nv_bfloat16* from, float (&to)[4]) {
+      const uint2 w = *reinterpret_cast<const uint2*>(from);
+      to[0] = __uint_as_float(w.x << 16);
+      to[1] = __uint_as_float(w.x & 0xFFFF0000u);
+      to[2] = __uint_as_float(w.y << 16);
+      to[3] = __uint_as_float(w.y & 0xFFFF0000u);
+    };
+    for (int j0 = 4 * warp; j0 < len; j0 += 16) {      // (of one page: a page has 16 rows or more)
+      const int from = j0 < q.pre_tiles * kPfTile ? head_s : s;
+      const int page = min(max(p.tables[(size_t)from * p.table_ld + (j0 >> p.page_shift)], 0), p.n_pages - 1);
+      const size_t row = ((size_t)page << p.page_shift) + (j0 & ((1 << p.page_shift) - 1));
+      float sc[4], v[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const size_t r = ((row + i) * p.n_kv + kv) * kPaDim + 4 * lane;
+        float k[4];
+        four(p.k + r, k);
+        four(p.v + r, v[i]);
+        sc[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sc[i] = fmaf(x[c], k[c], sc[i]);
+      }
+      float mn = m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[i] = warp_sum(sc[i]) * p.scale_log2;
+        if (j0 + i < len) mn = fmaxf(mn, sc[i]);
+      }
+      const float f = ex2(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j0 + i < len) {
+          const float w = ex2(sc[i] - mn);
+          l += w;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[c] += w * v[i][c];
+        }
+    }
+    part[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
+    if (lane == 0) part_ml[warp] = make_float2(m, l);
+    __syncthreads();
+    m = fmaxf(fmaxf(part_ml[0].x, part_ml[1].x), fmaxf(part_ml[2].x, part_ml[3].x));
+    l = o[0] = o[1] = o[2] = o[3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float4 v = part[k][lane];
+      const float f = ex2(part_ml[k].x - m);
+      l += part_ml[k].y * f;
+      o[0] += v.x * f;
+      o[1] += v.y * f;
+      o[2] += v.z * f;
+      o[3] += v.w * f;
     }
   }
+  if (warp) return;
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;                // (a NaN stays one)
   if (p.out_f32) {
     *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);

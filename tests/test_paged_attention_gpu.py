@@ -495,3 +495,26 @@ def test_shared_positions_are_the_first_sequences_whatever_the_scores(dev):
         dev.sync()
         want, size = s.reference()
         assert (np.abs(got - want) <= (2.0 ** -14 + 128 * 4 * factor * 2.0 ** -24) * size).all(), factor
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("P", [16, 1024])
+def test_rows_that_are_attended_again(dev, P, f32):
+    """Every number of keys that the last turn of four keys and four warps can have, beside a NaN in another element; scores that start at -infinity too."""
+    s = Setup(8, 2, P, [(256, [256 + i for i in range(1, 18)])] + [(0, [i]) for i in range(1, 18)], seed=63)
+    s.kv_bits[1, :, :, :, 5] = NAN
+    for b in range(s.B):
+        s.kv_bits[0, s.tables[b, 0], 0], s.kv[0, s.tables[b, 0], 0] = bf16_round(np.full((2, HD), -3e38, np.float32))
+    s.q_bits, s.q = (a.reshape(s.q.shape) for a in bf16_round(np.abs(s.q) + 1))        # (the first key's score is -infinity)
+    s.put(dev)
+    got = s.run(f32).to_vec()
+    dev.sync()
+    with np.errstate(over="ignore"):
+        want, size = s.reference()
+    g = (got.astype(np.float64) if f32 else (got.astype(np.uint32) << 16).view(np.float32).astype(np.float64)).reshape(want.shape)
+    ok = np.ones(want.shape, bool)
+    ok[:, :, 5] = False
+    ok[np.array(s.lens) == 1] = False                  # (nothing but the first key: 0 over 0 in 32 bits)
+    assert np.isnan(g[s.lens > 1][:, :, 5]).all()
+    off = (2.0 ** -14 + 128 * 2.0 ** -24 * 8 * 12) * size              # scores up to 8 * 12 here, sums of 128 products
+    assert (np.abs(g - want)[ok] <= (off + (0 if f32 else 2.0 ** -8) * (np.abs(want) + off))[ok]).all()
