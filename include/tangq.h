@@ -277,7 +277,8 @@ TQ_API int tq_token_logprobs(tq_ctx* ctx, const void* logits_dev, int dtype, siz
  *
  * All calls are asynchronous and may be recorded in a graph.  Lists are device arrays of 1 to 1024 sequence numbers, each number once
  * (src of tq_pages_fork aside).  A call is all or nothing: with a list that breaks a rule (tq_sync: TQ_EINVAL) or without enough free pages or table
- * entries (TQ_ENOMEM) it changes nothing.  Pages are handed out lowest number first, in the order of the list. */
+ * entries (TQ_ENOMEM) it changes nothing.  Pages are handed out lowest number first, in the order of the list.  A graph that was recorded over a pool is
+ * refused (tq_graph_launch: TQ_EINVAL) once the pool is destroyed or has other arrays. */
 typedef struct tq_pages tq_pages;
 TQ_API int tq_pages_create(tq_ctx* ctx, size_t n_pages, size_t page_rows, size_t n_seqs, size_t table_ld, int* refs_dev_or_null,
                            int* tables_dev_or_null, int* lens_dev_or_null, tq_pages** out);

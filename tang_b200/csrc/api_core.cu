@@ -162,6 +162,7 @@ int tq_ctx_destroy(tq_ctx* ctx) {
   if (ctx->side_begin) cudaEventDestroy(ctx->side_begin);
   if (ctx->side_done) cudaEventDestroy(ctx->side_done);
   if (ctx->owns_stream) cudaStreamDestroy(ctx->stream);
+  free(ctx->recorded_pools);
   delete ctx;
   return TQ_OK;
 }

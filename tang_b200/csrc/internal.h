@@ -80,6 +80,12 @@ struct tq_ctx {
   bool hostx_epoch_pending = false;  // a capture is open and has not bumped the word yet
   unsigned long long ws_generation = 0;        // bumped whenever a workspace is freed and reallocated: graphs recorded
                                                // before that hold the old addresses and refuse to launch
+  // Pools of pages (pages.h): those that live, and the numbers of those that the open capture has used, which tq_graph_end hands to the graph.
+  // A graph whose pool is gone holds the addresses of freed memory and refuses to launch.
+  struct tq_pages* pools = nullptr;
+  unsigned long long pool_ids = 0;
+  unsigned long long* recorded_pools = nullptr;
+  size_t n_recorded_pools = 0, recorded_pools_room = 0;
   unsigned long long launches = 0;             // kernels launched through this context
   bool pdl = true;                             // programmatic dependent launch for the decode-path kernels
   bool capturing = false;                      // between tq_graph_begin and tq_graph_end

@@ -464,6 +464,7 @@ static int decode_step(tq_llama* m, const int* token_ids_dev, const int* positio
   if (paged) {
     const tq_pages* pg = paged->pages;
     const size_t most = (size_t)pg->table_ld * pg->page_rows;
+    if (int use = pages_use(ctx, pg)) return use;
     TQ_CUDA(ctx, launch_k(ctx, paged_rows_kernel, dim3((B + 63) / 64), dim3(64), 0, (const int*)pg->tables, (const int*)pg->lens, (const int*)pg->refs,
                           (const int*)pages_refused(pg), paged->seqs, B, pg->n_seqs, pg->table_ld, pg->n_pages, pg->page_rows,
                           (int)(max_len < most ? max_len : most), m->lens, m->rope, ctx->dev_err));

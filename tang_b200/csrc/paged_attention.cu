@@ -996,6 +996,7 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
       !encode_pages(&vm, v_pages_dev, row, rows, box))
     return fail(ctx, TQ_ECUDA, "cuTensorMapEncodeTiled failed");
   const size_t smem = kPuFixed + (2 * batch + 1 + (size_t)p.n_groups + 1) * sizeof(int);
+  if (int st = pages_use(ctx, pages)) return st;
   TQ_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kPuFixed + (3 * kPuBatch + 2) * sizeof(int))));
   TQ_CUDA(ctx, launch_k(ctx, kern, dim3((unsigned)n_ctas), dim3(kPuThreads), smem, qe, qw, km, vm, pp));
   TQ_CUDA(ctx, launch_k(ctx, paged_join_kernel, dim3((unsigned)n_heads, (unsigned)batch), dim3(128), 0, pp));

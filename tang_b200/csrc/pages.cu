@@ -422,6 +422,9 @@ int tq_pages_create(tq_ctx* ctx, size_t n_pages, size_t page_rows, size_t n_seqs
     cudaGetLastError();
     return fail(ctx, e == cudaErrorMemoryAllocation ? TQ_ENOMEM : TQ_ECUDA, "tq_pages_create: %s", cudaGetErrorString(e));
   }
+  p->id = ++ctx->pool_ids;
+  p->next = ctx->pools;
+  ctx->pools = p;
   *out = p;
   return TQ_OK;
 }
@@ -430,6 +433,11 @@ int tq_pages_destroy(tq_pages* p) {
   if (!p) return TQ_OK;
   bind(p->ctx);
   cudaStreamSynchronize(p->ctx->stream);
+  for (tq_pages** at = &p->ctx->pools; *at; at = &(*at)->next)
+    if (*at == p) {
+      *at = p->next;
+      break;
+    }
   release(p);
   return TQ_OK;
 }
@@ -453,7 +461,7 @@ int tq_pages_arrays(tq_pages* p, void* const* bases_host, size_t n_arrays, size_
   }
   if (p->arrays) {
     cudaFree(p->arrays);
-    ctx->ws_generation++;              // (recorded graphs hold the old list)
+    p->id = ++ctx->pool_ids;
   }
   p->arrays = fresh;
   p->n_arrays = (int)n_arrays;
@@ -478,6 +486,7 @@ int tq_pages_extend(tq_pages* p, const int* seqs_dev, const int* counts_dev, siz
   TQ_REQUIRE(ctx, n <= (size_t)kPageCalls, "tq_pages_extend: at most %d sequences in a call", kPageCalls);
   TQ_REQUIRE(ctx, p->arrays != nullptr, "tq_pages_extend: a shared page cannot be copied before tq_pages_arrays names the caches");
   const PagesParams k = params_of(p);
+  if (int st = pages_use(ctx, p)) return st;
   TQ_CUDA(ctx, launch_k(ctx, pages_extend_kernel, dim3(1), dim3(kBookThreads), 0, k, seqs_dev, counts_dev, (int)n));
   return launch_copies(p, k, false);
 }
@@ -489,6 +498,7 @@ int tq_pages_fork(tq_pages* p, const int* src_dev, const int* dst_dev, const int
   if (n == 0) return TQ_OK;
   TQ_REQUIRE(ctx, src_dev && dst_dev, "tq_pages_fork: null list");
   TQ_REQUIRE(ctx, n <= (size_t)kPageCalls, "tq_pages_fork: at most %d sequences in a call", kPageCalls);
+  if (int st = pages_use(ctx, p)) return st;
   TQ_CUDA(ctx, launch_k(ctx, pages_fork_kernel, dim3(1), dim3(kBookThreads), 0, params_of(p), src_dev, dst_dev, keep_dev, (int)n));
   return TQ_OK;
 }
@@ -500,6 +510,7 @@ int tq_pages_free(tq_pages* p, const int* seqs_dev, size_t n) {
   if (n == 0) return TQ_OK;
   TQ_REQUIRE(ctx, seqs_dev != nullptr, "tq_pages_free: null list");
   TQ_REQUIRE(ctx, n <= (size_t)kPageCalls, "tq_pages_free: at most %d sequences in a call", kPageCalls);
+  if (int st = pages_use(ctx, p)) return st;
   TQ_CUDA(ctx, launch_k(ctx, pages_free_kernel, dim3(1), dim3(kBookThreads), 0, params_of(p), seqs_dev, (int)n));
   return TQ_OK;
 }
@@ -510,6 +521,7 @@ int tq_pages_compact(tq_pages* p, int* used_out_dev) {
   if (int st = bind(ctx)) return st;
   TQ_REQUIRE(ctx, p->arrays != nullptr, "tq_pages_compact: pages cannot be moved before tq_pages_arrays names the caches");
   const PagesParams k = params_of(p);
+  if (int st = pages_use(ctx, p)) return st;
   TQ_CUDA(ctx, launch_k(ctx, pages_compact_kernel, dim3(1), dim3(kBookThreads), 0, k, used_out_dev));
   return launch_copies(p, k, true);
 }

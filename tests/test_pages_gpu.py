@@ -239,3 +239,50 @@ def test_a_table_with_a_page_that_does_not_exist_changes_nothing(dev, page):
     dev.sync()
     assert pool.state()[2].tolist() == [0, 33, 0, 0, 0, 0] and pool.state()[0].tolist() == [1, 0, 1] + [0] * 9
     pool.destroy()
+
+
+def test_a_graph_over_a_pool_that_is_gone_is_refused(dev):
+    """Destroyed, or with other arrays; graphs over other pools and over none go on."""
+    import tang_b200 as tb
+
+    seqs, x = dev.upload(np.array([0], np.int32), tb.I32), dev.alloc(16 * 128, tb.BF16)
+    pools = [tb.PagePool(dev, 4, 16, 2, 4, [dev.alloc(4 * 16 * 8, tb.BF16)]) for _ in range(7)]
+    kv, out = dev.alloc(4 * 16 * 128, tb.BF16), dev.alloc(128, tb.BF16)
+    dev.memset(kv, 0)
+    dev.memset(x, 0)
+    q = tb.Buffer(dev, x.ptr, 128, tb.BF16, owns=False)
+    attend = lambda p: dev.gqa_decode_paged(q, kv, kv, p, 1, 1, 1, 128, 16, out=out)
+    uses = [lambda p: p.extend(seqs), lambda p: p.fork(seqs, seqs, 1), lambda p: p.free(seqs), lambda p: p.compact(), attend,
+            lambda p: (p.free(seqs), attend(p), attend(pools[6]))]
+    attend(pools[0])                                   # (workspaces)
+    dev.sync()
+
+    def record(call):
+        dev.begin_capture()
+        call()
+        return dev.end_capture()
+
+    graphs = [record(lambda: use(p)) for use, p in zip(uses, pools)]
+    both, none = record(lambda: [p.free(seqs) for p in pools[:6]]), record(lambda: dev.memset(out, 0))
+    last = record(lambda: pools[6].free(seqs))
+    for i, p in enumerate(pools[:6]):
+        if i % 2:
+            p.set_arrays([dev.alloc(4 * 16 * 8, tb.BF16)])
+        else:
+            p.destroy()
+        with pytest.raises(tb.TangqError, match="pool of pages"):
+            graphs[i].launch()
+        with pytest.raises(tb.TangqError, match="pool of pages"):
+            both.launch()
+        last.launch()
+        none.launch()
+        if i < 5:
+            fresh = tb.PagePool(dev, 4, 16, 2, 4)      # (one that may stand where the old one stood)
+            with pytest.raises(tb.TangqError, match="pool of pages"):
+                graphs[i].launch()
+            fresh.destroy()
+        dev.sync()
+    for g in (*graphs, both, none, last):
+        g.free()
+    for p in pools:
+        p.destroy()
