@@ -296,8 +296,8 @@ TQ_API int tq_pages_free(tq_pages* pages, const int* seqs_dev, size_t n);
 /* The u pages in use become pages 0 .. u-1: those numbered u and above move, in order, to the free ones below.  u goes to *used_out. */
 TQ_API int tq_pages_compact(tq_pages* pages, int* used_out_dev_or_null);
 /* tq_gqa_decode over pages: one new token for each of `batch` sequences (seqs [batch] of the pool; NULL: b), q [batch, n_heads*128] bf16, pages
- * bf16 [n_pages][page_rows][n_kv_heads*128], lengths from the pool (the new token's position included; 0: the result is 0).  max_len bounds
- * them: what lies behind it is not attended.
+ * bf16 [n_pages][page_rows][n_kv_heads*128], lengths from the pool, which is one of the same context (the new token's position included; 0: the result
+ * is 0).  max_len bounds them: what lies behind it is not attended.
  * Groups (NULL: none): group g is sequences group_starts[g] .. group_starts[g+1]-1 of the batch (the last group's end is the batch's; starts
  * ascend from 0) and shares its first shared[g] positions (at most max_shared), which are read from its first sequence's pages, once for all.
  * out [batch, n_heads*128] bf16 or f32; all four 16-byte aligned.  A page or sequence that does not exist is reported by tq_sync, and the results

@@ -357,7 +357,7 @@ int tq_llama_decode_paged(tq_llama* m, const int* token_ids_dev, const tq_pages*
   const tq_llama_config& c = m->cfg;
   TQ_REQUIRE(ctx, batch > 0 && batch <= c.max_batch, "tq_llama_decode_paged: batch must be 1..%u", c.max_batch);
   TQ_REQUIRE(ctx, token_ids_dev && pages && logits_dev, "tq_llama_decode_paged: null pointer");
-  TQ_REQUIRE(ctx, pages->ctx->device == ctx->device, "tq_llama_decode_paged: the pool belongs to another device");
+  TQ_REQUIRE(ctx, pages->ctx == ctx, "tq_llama_decode_paged: the pool belongs to another context");
   TQ_REQUIRE(ctx, seqs_dev || batch <= (size_t)pages->n_seqs, "tq_llama_decode_paged: the pool has %d sequences", pages->n_seqs);
   const size_t rows = (size_t)pages->n_pages * pages->page_rows;
   TQ_REQUIRE(ctx, rows <= (size_t)c.max_batch * c.max_seq && rows < (1ull << 31), "tq_llama_decode_paged: the cache has %zu rows, the pool's pages %zu",

@@ -929,7 +929,7 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   if (int st = bind(ctx)) return st;
   if (batch == 0) return TQ_OK;
   TQ_REQUIRE(ctx, q_dev && k_pages_dev && v_pages_dev && pages && out_dev, "tq_gqa_decode_paged: null pointer");
-  TQ_REQUIRE(ctx, pages->ctx->device == ctx->device, "tq_gqa_decode_paged: the pool belongs to another device");
+  TQ_REQUIRE(ctx, pages->ctx == ctx, "tq_gqa_decode_paged: the pool belongs to another context");
   TQ_REQUIRE(ctx, head_dim == (size_t)kPaDim, "tq_gqa_decode_paged: head_dim must be %d", kPaDim);
   TQ_REQUIRE(ctx, n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_heads / n_kv_heads >= 1 && n_heads / n_kv_heads <= 8 && n_heads <= 65535,
              "tq_gqa_decode_paged: n_heads/n_kv_heads must be 1..8");

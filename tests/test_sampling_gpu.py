@@ -378,3 +378,21 @@ def test_a_forked_sequence_is_not_stepped_before_it_is_extended(dev):
         assert not all(np.array_equal(x, y) for x, y in zip(before, caches(model)))
         pool.destroy()
     model.destroy()
+
+
+def test_a_pool_of_another_handle_is_refused(dev):
+    """Its calls run on another stream, with nothing to order them."""
+    import tang_b200 as tb
+
+    host = host_model(25)
+    model, other = host.to_device(dev, 64, 2), tb.QuantComputeDevice(0)
+    pool = tb.PagePool(other, 8, 16, 2, 4)
+    tok, lg = dev.upload(np.zeros(2, np.int32), tb.I32), dev.alloc(2 * host.vocab)
+    with pytest.raises(tb.TangqError, match="context"):
+        model.decode_paged(tok, pool, 2, 64, lg)
+    kv = dev.alloc(8 * 16 * 256, tb.BF16)
+    with pytest.raises(tb.TangqError, match="context"):
+        dev.gqa_decode_paged(dev.alloc(2 * 512, tb.BF16), kv, kv, pool, 2, 4, 2, 128, 64)
+    pool.destroy()
+    other.close()
+    model.destroy()
