@@ -6,6 +6,7 @@
 #include <new>
 
 #include "internal.h"
+#include "pages.h"
 
 namespace tq {
 
@@ -163,6 +164,7 @@ int tq_ctx_destroy(tq_ctx* ctx) {
   if (ctx->side_done) cudaEventDestroy(ctx->side_done);
   if (ctx->owns_stream) cudaStreamDestroy(ctx->stream);
   free(ctx->recorded_pools);
+  for (tq_pages* p = ctx->pools; p; p = p->next) p->ctx = nullptr;     // (tq_pages_destroy is all that is left for them)
   delete ctx;
   return TQ_OK;
 }

@@ -431,13 +431,15 @@ int tq_pages_create(tq_ctx* ctx, size_t n_pages, size_t page_rows, size_t n_seqs
 
 int tq_pages_destroy(tq_pages* p) {
   if (!p) return TQ_OK;
-  bind(p->ctx);
-  cudaStreamSynchronize(p->ctx->stream);
-  for (tq_pages** at = &p->ctx->pools; *at; at = &(*at)->next)
-    if (*at == p) {
-      *at = p->next;
-      break;
-    }
+  if (tq_ctx* ctx = p->ctx) {          // (null: the context went first, and its stream was waited for)
+    bind(ctx);
+    cudaStreamSynchronize(ctx->stream);
+    for (tq_pages** at = &ctx->pools; *at; at = &(*at)->next)
+      if (*at == p) {
+        *at = p->next;
+        break;
+      }
+  }
   release(p);
   return TQ_OK;
 }

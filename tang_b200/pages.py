@@ -89,7 +89,6 @@ class PagePool:
 
     def __del__(self):
         try:
-            if self.dev._ctx:
-                self.destroy()
+            self.destroy()
         except Exception:
             pass

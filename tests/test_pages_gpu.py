@@ -286,3 +286,22 @@ def test_a_graph_over_a_pool_that_is_gone_is_refused(dev):
         g.free()
     for p in pools:
         p.destroy()
+
+
+def test_a_pool_that_outlives_its_handle():
+    """Calls are refused, and it can still be destroyed."""
+    import tang_b200 as tb
+
+    d = tb.QuantComputeDevice(0)
+    pools = [tb.PagePool(d, 4, 16, 2, 4) for _ in range(3)]
+    seqs = d.upload(np.array([0], np.int32), tb.I32)
+    pools[1].destroy()
+    handles, L = [tb._lib.C.c_void_p(p.handle) for p in pools], d._L
+    d.close()
+    z = tb._lib.C.c_void_p(seqs.ptr)
+    for h in (handles[0], handles[2]):
+        assert L.tq_pages_extend(h, z, None, 1) == L.tq_pages_fork(h, z, z, None, 1) == L.tq_pages_free(h, z, 1) == L.tq_pages_compact(h, None) == tb._lib.TQ_EINVAL
+        assert L.tq_pages_arrays(h, None, 1, 16) == tb._lib.TQ_EINVAL
+    for p in pools:
+        p.destroy()
+        p.destroy()
