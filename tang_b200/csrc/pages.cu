@@ -30,18 +30,19 @@ struct PagesParams {
 __device__ __forceinline__ int pages_of(int positions, int page_rows) { return (positions + page_rows - 1) / page_rows; }
 
 // Sum of v over the lower threads of the CTA and, in *total, over all of them.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T* warp_sums, T* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = v;
+  T incl = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, incl, o);
+    const T u = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += u;
   }
   __syncthreads();                     // (the sums of the call before have been read)
   if (lane == 31) warp_sums[warp] = incl;
   __syncthreads();
-  int base = 0, all = 0;
+  T base = 0, all = 0;
 #pragma unroll 8
   for (int w = 0; w < kBookThreads / 32; ++w) {
     base += w < warp ? warp_sums[w] : 0;
@@ -96,6 +97,7 @@ __device__ __forceinline__ bool mark_once(const PagesParams& p, int s) {
 __device__ __forceinline__ bool sound(const PagesParams& p, int len) { return len >= 0 && len <= 0x7fffffff - p.page_rows && pages_of(len, p.page_rows) <= p.table_ld; }
 
 __global__ void __launch_bounds__(kBookThreads) pages_extend_kernel(const PagesParams p, const int* seqs, const int* counts, int n) {
+  __shared__ long long warp_needs[kBookThreads / 32];
   __shared__ int warp_sums[kBookThreads / 32], first_s[kBookThreads + 1], last_s[kBookThreads], seq_s[kBookThreads], at_s[kBookThreads];
   pdl_wait();
   pdl_launch_dependents();
@@ -134,8 +136,11 @@ __global__ void __launch_bounds__(kBookThreads) pages_extend_kernel(const PagesP
   }
   if (marked) p.marks[s] = 0;
   full = __syncthreads_or(full);
-  int total = 0, n_copies = 0;
-  const int first = block_scan(need, warp_sums, &total), copy_at = block_scan(cow ? 1 : 0, warp_sums, &n_copies);
+  long long needs = 0;                 // (1024 sequences of 2^24 pages each are more than 32 bits)
+  int n_copies = 0;
+  const int first = (int)block_scan<long long>(need, warp_needs, &needs), copy_at = block_scan(cow ? 1 : 0, warp_sums, &n_copies);
+  full = full || needs > p.n_pages;
+  const int total = (int)needs;
   if (!bad && !full && total > 0) full = find_pages(p.refs, 0, p.n_pages, true, total, p.list, warp_sums) < total;
   if (bad || full) {
     if (t == 0) atomicCAS(p.err, 0, bad ? (int)DERR_PAGE_LIST : (int)DERR_PAGES);

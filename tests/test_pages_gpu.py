@@ -305,3 +305,31 @@ def test_a_pool_that_outlives_its_handle():
     for p in pools:
         p.destroy()
         p.destroy()
+
+
+def test_more_pages_than_32_bits_count(dev):
+    """What 1024 sequences ask for together: 2^31, 2^32 and 2^32 + 1 pages, of tables that are large enough."""
+    import tang_b200 as tb
+
+    ld, n = (1 << 22) + 1, 1024
+    pool = tb.PagePool(dev, 64, 16, n, ld, [dev.alloc(64 * 16 * 8, tb.BF16)])
+    seqs, small = dev.upload(np.arange(n, dtype=np.int32), tb.I32), [3, 5]
+    pool.extend(small, counts=[20, 7])
+    pool.fork([3], [9])                                # (a partly filled page that would be copied)
+    dev.sync()
+    refs, lens = pool.refs.to_vec(), pool.lens.to_vec()
+    row = lambda s: tb.Buffer(dev, pool.tables.ptr + 4 * s * ld, 4, tb.I32, owns=False).to_vec().tolist()
+    rows = [row(s) for s in (0, 3, 5, 9, n - 1)]
+    for pages, more in ((1 << 21, 0), (1 << 22, 0), (1 << 22, 1)):
+        counts = np.full(n, 16 * pages, np.int32)
+        counts[[3, 5, 9]] -= 32                        # (with what they have, and one copy: five pages too few, which five others ask for)
+        counts[10:15 + more] += 16
+        pool.extend(seqs, n, counts=dev.upload(counts, tb.I32))
+        with pytest.raises(tb.TangqError) as e:
+            dev.sync()
+        assert e.value.status == tb._lib.TQ_ENOMEM
+        assert np.array_equal(pool.refs.to_vec(), refs) and np.array_equal(pool.lens.to_vec(), lens) and [row(s) for s in (0, 3, 5, 9, n - 1)] == rows
+    pool.extend([9])
+    dev.sync()
+    assert pool.lens.to_vec()[9] == 21
+    pool.destroy()
