@@ -187,12 +187,15 @@ class QuantComputeDevice:
         n_tokens = 0 if tokens is None else n_tokens
         if logits.n < ((slices * rows - 1) * (ld or cols) + cols if rows else 0) or (tokens is not None and tokens.n != rows * n_tokens):
             raise TangqError(_lib.TQ_EINVAL, f"token_logprobs: {logits.n} logits or {0 if tokens is None else tokens.n} tokens do not match the shapes")
+        _check_types("token_logprobs", _lib.I32, tokens=tokens)
         if out is None:
             out = TokenLogprobs(self.alloc(rows * n_tokens) if n_tokens else None, self.alloc(rows) if entropy else None,
                                 self.alloc(rows * top, _lib.I32) if top else None, self.alloc(rows * top) if top else None)
         for b, n in ((out.logprobs, rows * n_tokens), (out.entropy, rows if entropy else 0), (out.top_ids, rows * top), (out.top_logprobs, rows * top)):
             if n and (b is None or b.n < n):
                 raise TangqError(_lib.TQ_EINVAL, f"token_logprobs: a result needs room for {n} values")
+        _check_types("token_logprobs", F32, logprobs=out.logprobs, entropy=out.entropy, top_logprobs=out.top_logprobs)
+        _check_types("token_logprobs", _lib.I32, top_ids=out.top_ids)
         self._check(self._L.tq_token_logprobs(self._ctx, C.c_void_p(logits.ptr), logits.dtype, ld, slices, rows, cols, _opt_ptr(tokens), n_tokens, top,
                                               _opt_ptr(out.logprobs), _opt_ptr(out.entropy if entropy else None), _opt_ptr(out.top_ids),
                                               _opt_ptr(out.top_logprobs)))
@@ -376,6 +379,13 @@ class Graph:
 
 
 # ---------------------------------------------------------------------- operators of the decode step
+def _check_types(call: str, dtype: int, **buffers) -> None:
+    """A kernel takes a buffer's elements as what it needs: of another type they would be other values, or fewer bytes."""
+    for name, b in buffers.items():
+        if b is not None and b.dtype != dtype:
+            raise TangqError(_lib.TQ_EINVAL, f"{call}: {name} has elements of another type than the call takes")
+
+
 def _opt_ptr(buf) -> C.c_void_p:
     return C.c_void_p(buf.ptr if buf is not None else 0)
 
@@ -474,6 +484,8 @@ def _add_ops(cls):
             raise TangqError(_lib.TQ_EINVAL, "gqa_decode_paged: buffer sizes do not match the shapes")
         if group_starts is not None and (group_starts.n < n_groups or shared is None or shared.n < n_groups):
             raise TangqError(_lib.TQ_EINVAL, "gqa_decode_paged: fewer starts or shared lengths than groups")
+        _check_types("gqa_decode_paged", BF16, q=q, k_pages=k_pages, v_pages=v_pages)
+        _check_types("gqa_decode_paged", _lib.I32, seqs=seqs, group_starts=group_starts, shared=shared)
         if out is None:
             out = self.alloc(q.n, out_dtype)
         elif out.n != q.n:

@@ -9,7 +9,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib
-from .device import Buffer, QBuffer, QuantComputeDevice
+from .device import Buffer, QBuffer, QuantComputeDevice, _check_types
 from .generation import check_lengths, decode_loop
 from .pages import PagePool
 
@@ -158,6 +158,8 @@ class LlamaModel:
             raise _lib.TangqError(_lib.TQ_EINVAL, "decode_paged: buffer sizes do not match the batch")
         if group_starts is not None and (group_starts.n < n_groups or shared is None or shared.n < n_groups):
             raise _lib.TangqError(_lib.TQ_EINVAL, "decode_paged: fewer starts or shared lengths than groups")
+        _check_types("decode_paged", _lib.I32, token_ids=token_ids, seqs=seqs, group_starts=group_starts, shared=shared)
+        _check_types("decode_paged", _lib.F32, logits=logits)
         ptr = lambda b: C.c_void_p(b.ptr if b is not None else 0)
         self.dev._check(self.dev._L.tq_llama_decode_paged(C.c_void_p(self.handle), ptr(token_ids), C.c_void_p(pool.handle), ptr(seqs), batch,
                                                           ptr(group_starts), ptr(shared), n_groups, max_shared, max_len, ptr(logits)))

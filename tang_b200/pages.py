@@ -76,6 +76,8 @@ class PagePool:
 
     def compact(self, used: Buffer | None = None) -> None:
         """Moves the pages in use to the front of the pool; `used` receives how many there are."""
+        if used is not None and (used.dtype != _lib.I32 or used.n < 1):
+            raise TangqError(TQ_EINVAL, "PagePool: the number of pages in use needs an int32")
         self.dev._check(self.dev._L.tq_pages_compact(C.c_void_p(self.handle), _opt_ptr(used)))
 
     def state(self):

@@ -72,3 +72,33 @@ def test_the_definition_keeps_its_counts():
             except Refused:
                 assert all(np.array_equal(a, b) for a, b in zip(before, (p.refs, p.tables, p.lens)))
             p.sound()
+
+
+def test_types_are_checked_before_the_call(tb):
+    """A buffer with enough elements of a smaller type has too few bytes."""
+    dev = tb.QuantComputeDevice.__new__(tb.QuantComputeDevice)
+    dev._ctx, dev._L = None, NoDevice()
+    dev.alloc = dev.upload = NoDevice
+    buf = lambda n, dt=tb.I32: tb.Buffer(dev, 64, n, dt, owns=False)
+    logits, out = buf(12, tb.F32), lambda **kw: tb.TokenLogprobs(**{**dict(logprobs=buf(2, tb.F32), entropy=buf(2, tb.F32), top_ids=buf(6), top_logprobs=buf(6, tb.F32)), **kw})
+    for kw in (dict(tokens=buf(2, tb.U8)), dict(tokens=buf(2, tb.F64)), dict(out=out(logprobs=buf(2, tb.BF16))), dict(out=out(entropy=buf(2, tb.U8))),
+               dict(out=out(top_ids=buf(6, tb.I8))), dict(out=out(top_logprobs=buf(6, tb.BF16)))):
+        with pytest.raises(tb.TangqError, match="type"):
+            dev.token_logprobs(**{**dict(logits=logits, rows=2, cols=6, tokens=buf(2), top=3, out=out()), **kw})
+    pool = tb.PagePool.__new__(tb.PagePool)
+    pool.dev, pool.n_pages, pool.page_rows, pool.handle = dev, 2, 16, 0
+    ok = dict(q=buf(8 * 128, tb.BF16), k_pages=buf(2 * 16 * 256, tb.BF16), v_pages=buf(2 * 16 * 256, tb.BF16), pool=pool, batch=1, n_heads=8, n_kv_heads=2, head_dim=128,
+              max_len=5, seqs=buf(1), group_starts=buf(1), shared=buf(1), n_groups=1, max_shared=1, out=buf(8 * 128, tb.BF16))
+    for kw in ({"q": buf(8 * 128, tb.U8)}, {"k_pages": buf(2 * 16 * 256, tb.U8)}, {"v_pages": buf(2 * 16 * 256, tb.F32)}, {"seqs": buf(1, tb.U8)}, {"group_starts": buf(1, tb.I8)},
+               {"shared": buf(1, tb.BF16)}):
+        with pytest.raises(tb.TangqError, match="type"):
+            dev.gqa_decode_paged(**{**ok, **kw})
+    model = tb.LlamaModel.__new__(tb.LlamaModel)
+    model.dev, model.handle, model.cfg = dev, 0, tb.LlamaConfig(vocab=6)
+    ok = dict(token_ids=buf(1), pool=pool, batch=1, max_len=5, logits=logits, seqs=buf(1), group_starts=buf(1), shared=buf(1), n_groups=1)
+    for kw in ({"token_ids": buf(1, tb.U8)}, {"logits": buf(12, tb.BF16)}, {"seqs": buf(1, tb.U8)}, {"group_starts": buf(1, tb.F64)}, {"shared": buf(1, tb.U8)}):
+        with pytest.raises(tb.TangqError, match="type"):
+            model.decode_paged(**{**ok, **kw})
+    for used in (buf(1, tb.U8), buf(0)):
+        with pytest.raises(tb.TangqError):
+            pool.compact(used)
