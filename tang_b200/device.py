@@ -112,6 +112,7 @@ def _host(a, dtype) -> np.ndarray:
 
 class QuantComputeDevice:
     """One GPU, one stream (``CudaComputeDevice::new``, crates/tang-compute/src/cuda.rs:151-179)."""
+    capturing = False     # between begin_capture and end_capture
 
     def __init__(self, device: int = 0, stream: int | None = None):
         self._L = _lib.load()
@@ -338,10 +339,12 @@ class QuantComputeDevice:
     def begin_capture(self) -> None:
         """``begin_capture`` (crates/tang-compute/src/cuda.rs:344)."""
         self._check(self._L.tq_graph_begin(self._ctx))
+        self.capturing = True
 
     def end_capture(self) -> "Graph":
         """``end_capture`` (cuda.rs:350): returns a replayable graph."""
         g = C.c_void_p()
+        self.capturing = False
         self._check(self._L.tq_graph_end(self._ctx, C.byref(g)))
         return Graph(self, g.value)
 

@@ -1,6 +1,6 @@
 """Pages of a KV cache that several sequences hold at once (``tq_pages_*`` in include/tangq.h): forked sequences share their
 pages, and a shared page is copied when one of them is about to write it.  All bookkeeping happens on the device, so that the
-calls can be recorded in a graph; ``state()`` is the only one that waits."""
+calls can be recorded in a graph (with lists that are Buffers); ``state()`` is the only one that waits."""
 from __future__ import annotations
 
 import ctypes as C
@@ -50,6 +50,8 @@ class PagePool:
         if v is None:
             return None, n
         if not isinstance(v, Buffer):
+            if self.dev.capturing:
+                raise TangqError(TQ_EINVAL, "PagePool: a recorded call reads its lists when it is replayed: they have to be Buffers that live as long")
             v = self.dev.upload(np.asarray(v, np.int32), _lib.I32)
         if v.dtype != _lib.I32 or (n is not None and v.n < n):
             raise TangqError(TQ_EINVAL, f"PagePool: a list of {v.n} values where {n} of int32 are needed")

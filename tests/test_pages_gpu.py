@@ -333,3 +333,26 @@ def test_more_pages_than_32_bits_count(dev):
     dev.sync()
     assert pool.lens.to_vec()[9] == 21
     pool.destroy()
+
+
+def test_a_recorded_call_takes_its_lists_from_the_device(dev):
+    """A list of the host's is refused while a graph is recorded, and the recording goes on."""
+    import tang_b200 as tb
+
+    b = Both(dev, 20, 16, 3, 8)
+    b.extend([0], [5])
+    seqs = dev.upload(np.array([0], np.int32), tb.I32)
+    dev.sync()
+    dev.begin_capture()
+    for call in (lambda: b.pool.extend([0]), lambda: b.pool.extend(seqs, counts=[1]), lambda: b.pool.fork(seqs, [1]), lambda: b.pool.free([0])):
+        with pytest.raises(tb.TangqError, match="recorded"):
+            call()
+    b.pool.extend(seqs)
+    g = dev.end_capture()
+    for _ in range(3):
+        g.launch()
+        b.copy(b.want.extend([0]))
+    b.check()
+    g.free()
+    b.extend([0])
+    b.check()
