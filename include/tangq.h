@@ -257,7 +257,7 @@ TQ_API int tq_gqa_prefill(tq_ctx* ctx, const void* q_dev, const void* k_cache_de
 
 /* ---- log probabilities -------------------------------------------------------------------------
  * No counterpart in the reference (its Sampler keeps the chosen token only, crates/tang-infer/src/sampling.rs:86-158).  Rows of
- * logits x as for tq_argmax_rows, [slices][rows][ld] f32 or bf16 (ld = 0: cols), V = slices * cols of them, are a distribution
+ * logits x as for tq_argmax_rows, [slices][rows][ld] f32 or bf16 (ld = 0: cols), V = slices * cols <= 2^31 - 2^16 of them, are a distribution
  * p = exp(x) / sum exp(x):
  *   logprob_out [rows][n_tokens]   log p of the given tokens [rows][n_tokens] (a negative one is padding: 0; one that does not exist: NaN)
  *   entropy_out [rows]             -sum p log p (NULL: not wanted)

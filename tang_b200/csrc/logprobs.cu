@@ -608,7 +608,9 @@ extern "C" int tq_token_logprobs(tq_ctx* ctx, const void* logits_dev, int dtype,
   if (rows == 0) return TQ_OK;
   TQ_REQUIRE(ctx, logits_dev != nullptr && slices > 0 && cols > 0, "tq_token_logprobs: null pointer or empty vocabulary");
   TQ_REQUIRE(ctx, dtype == TQ_F32 || dtype == TQ_BF16, "tq_token_logprobs: logits must be f32 or bf16");
-  TQ_REQUIRE(ctx, slices < (1u << 16) && cols < (1ull << 31) && slices * cols < (1ull << 31) && rows < (1ull << 31), "tq_token_logprobs: vocabulary or rows too large");
+  // (32-bit places: a thread's next one may lie up to a turn of 1024 vectors behind the row's end)
+  TQ_REQUIRE(ctx, slices < (1u << 16) && cols < (1ull << 31) && slices * cols <= (1ull << 31) - (1u << 16) && rows < (1ull << 31),
+             "tq_token_logprobs: vocabulary or rows too large");
   if (ld == 0) ld = cols;
   TQ_REQUIRE(ctx, ld >= cols, "tq_token_logprobs: rows overlap");
   TQ_REQUIRE(ctx, ((uintptr_t)logits_dev & (dtype == TQ_F32 ? 3 : 1)) == 0, "tq_token_logprobs: logits are not aligned to their type");

@@ -248,3 +248,16 @@ def test_refusals(dev):
     assert L.tq_token_logprobs(dev._ctx, C.c_void_p(x.ptr), tb.F32, 0, 1, 1, 10, None, 0, 1, None, None, None, None) == tb._lib.TQ_EINVAL
     assert L.tq_token_logprobs(dev._ctx, None, tb.F32, 0, 1, 0, 10, None, 0, 0, None, None, None, None) == tb._lib.TQ_OK     # no rows
     dev.sync()
+
+
+def test_vocabularies_whose_places_pass_32_bits_are_refused(dev):
+    """Before anything is launched: there is no such row here."""
+    import ctypes as C
+
+    import tang_b200 as tb
+
+    x, out = dev.upload(np.zeros(16, np.float32)), dev.alloc(1)
+    for slices, cols in ((1, 2 ** 31 - 1), (1, 2 ** 31 - 2 ** 16 + 1), (2, 2 ** 30), (3, 715806038), (65535, 32768), (1, 2 ** 31), (2 ** 16, 1)):
+        assert slices * cols > 2 ** 31 - 2 ** 16 or slices == 2 ** 16
+        assert dev._L.tq_token_logprobs(dev._ctx, C.c_void_p(x.ptr), tb.BF16, 0, slices, 1, cols, None, 0, 0, None, C.c_void_p(out.ptr), None, None) == tb._lib.TQ_EINVAL
+    dev.sync()
