@@ -99,6 +99,10 @@ __device__ __forceinline__ unsigned long long lp_add2(unsigned long long a, unsi
   return r;
 }
 
+// The cluster's barrier, in the forms that ask nothing of where a warp's lanes are: they come from branches.
+__device__ __forceinline__ void lp_cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void lp_cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
 // The largest of 16 bytes of logits (NaN is none of them); bf16 by pairs.
 __device__ __forceinline__ float lp_largest(const uint4& v, float) {
   return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
@@ -304,7 +308,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = (int)(blockIdx.x / C), t = threadIdx.x, warp = t >> 5, lane = t & 31, V = p.slices * p.cols, top = TOP ? p.top : 0;
   const int lo = (int)((long long)V * rank / C) & ~63, hi = rank == C - 1 ? V : (int)((long long)V * (rank + 1) / C) & ~63;
-  if (C > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");              // (this CTA runs: the others may write to its memory)
+  if (C > 1) lp_cluster_arrive();      // (this CTA runs: the others may write to its memory)
   int token = -1;
   float token_x = 0.f;
   if (rank == 0 && t < p.n_tokens) {   // (on their way while the row is read)
@@ -517,7 +521,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
   }
 
   // ---- the row: every CTA of the cluster writes its state and its list to the first one's memory
-  if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (C > 1) lp_cluster_wait();
   __syncthreads();
   if (t == 0) {
     LpState r;
@@ -531,8 +535,12 @@ __global__ void __launch_bounds__(kLpThreads, kLpPerSm) token_logprobs_kernel(co
     *(C > 1 ? cluster.map_shared_rank(&parts[rank], 0) : parts) = make_float4(r.m, r.c, r.s, r.u);
   }
   if (TOP && C > 1 && t < top) *cluster.map_shared_rank(&all_k[rank * top + t], 0) = top_k[t];
-  if (C > 1) cluster.sync();
-  else __syncthreads();
+  if (C > 1) {
+    lp_cluster_arrive();
+    lp_cluster_wait();
+  } else {
+    __syncthreads();
+  }
   if (rank == 0) {
     LpState r;
     {
