@@ -274,6 +274,8 @@ TQ_API int tq_token_logprobs(tq_ctx* ctx, const void* logits_dev, int dtype, siz
  * n_pages * page_rows rows (page_rows 16, 32, .. 1024) into pages that several sequences may hold: position j of sequence s is row
  * j % page_rows of page tables[s][j / page_rows].  Its state is in device memory, the caller's or (all three NULL) the library's, which
  * starts empty: refs [n_pages], how many sequences hold a page (0: free); tables [n_seqs][table_ld], -1 behind a sequence's pages; lens [n_seqs].
+ * A pool does not know what other calls (tq_llama_prefill) wrote to the caches: whoever wants such rows to be a sequence's writes the three arrays
+ * (tq_pages_data) to say so.
  *
  * All calls are asynchronous and may be recorded in a graph.  Lists are device arrays of 1 to 1024 sequence numbers, each number once
  * (src of tq_pages_fork aside).  A call is all or nothing: with a list that breaks a rule (tq_sync: TQ_EINVAL) or without enough free pages or table
@@ -284,13 +286,13 @@ TQ_API int tq_pages_create(tq_ctx* ctx, size_t n_pages, size_t page_rows, size_t
                            int* tables_dev_or_null, int* lens_dev_or_null, tq_pages** out);
 TQ_API int tq_pages_destroy(tq_pages* pages);
 /* The caches whose rows the pages are (keys and values of every layer): n_arrays device addresses, 16-byte aligned, of n_pages * page_rows rows
- * of row_bytes (a multiple of 16).  Needed by the calls that copy. */
+ * of row_bytes (a multiple of 16).  Needed by the calls that copy, which they have to outlive. */
 TQ_API int tq_pages_arrays(tq_pages* pages, void* const* bases_host, size_t n_arrays, size_t row_bytes);
 TQ_API int tq_pages_data(const tq_pages* pages, int** refs_dev, int** tables_dev, int** lens_dev);
 /* Room for the next counts[i] positions (NULL: one) of each sequence, and its length that much larger.  A partly filled last page that has
  * other holders is copied first (its rows in every array); of several listed sequences that are its only holders the last one keeps it. */
 TQ_API int tq_pages_extend(tq_pages* pages, const int* seqs_dev, const int* counts_dev_or_null, size_t n);
-/* dst[i], which must be empty, gets the positions of src[i] (the first keep[i] of them) in the same pages. */
+/* dst[i], which must be empty, gets the positions of src[i] (the first keep[i] of them) in the same pages; none if src[i] is empty. */
 TQ_API int tq_pages_fork(tq_pages* pages, const int* src_dev, const int* dst_dev, const int* keep_dev_or_null, size_t n);
 TQ_API int tq_pages_free(tq_pages* pages, const int* seqs_dev, size_t n);
 /* The u pages in use become pages 0 .. u-1: those numbered u and above move, in order, to the free ones below.  u goes to *used_out. */

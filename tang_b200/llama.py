@@ -141,7 +141,8 @@ class LlamaModel:
     def page_pool(self, n_seqs: int, page_rows: int | None = None, **state) -> PagePool:
         """A ``PagePool`` over the caches of all layers, seen as max_batch * max_seq / page_rows pages: the rows that ``prefill`` and ``decode``
         give sequence b are the pages from b * max_seq / page_rows on.  `page_rows`: the largest of 64, 32 and 16 that divides max_seq unless
-        given.  `state`: refs, tables, lens of ``PagePool``."""
+        given.  `state`: refs, tables, lens of ``PagePool``.  The pool starts empty: rows that ``prefill`` wrote become a sequence's when its state
+        says so (see ``sample``).  It must not be used once the model is destroyed."""
         c = self.cfg
         if page_rows is None:
             page_rows = next((p for p in (64, 32, 16) if c.max_seq % p == 0), 0)

@@ -396,3 +396,73 @@ def test_a_pool_of_another_handle_is_refused(dev):
     pool.destroy()
     other.close()
     model.destroy()
+
+
+def test_the_calls_of_the_integration_guide(dev):
+    """Prefill, the pool's state, fork, one step as it is, the rest from a graph: through the C interface, and the same tokens as ``sample``."""
+    import ctypes as C
+
+    import tang_b200 as tb
+
+    host = host_model(27)
+    V, max_seq, n, n_new, length = host.vocab, 256, 3, 9, 150
+    model = host.to_device(dev, max_seq, n)
+    prompt = np.random.default_rng(27).integers(0, V, length).astype(np.int32)
+    cfg = tb.SamplerConfig(0.9, 0, 1.0, 1.0)
+    want = model.sample(prompt[None], n_new, n, cfg, seed=5)
+
+    L, ctx, m, vp = dev._L, dev._ctx, C.c_void_p(model.handle), C.c_void_p
+    ok = lambda st: dev._check(st)
+    keep = []
+
+    def ints(v):
+        keep.append(dev.upload(np.asarray(v, np.int32), tb.I32))
+        return vp(keep[-1].ptr)
+
+    def room(k, dtype=tb.F32):
+        keep.append(dev.alloc(k, dtype))
+        return vp(keep[-1].ptr)
+
+    page_rows = 64
+    n_pages, table_ld = n * max_seq // page_rows, max_seq // page_rows
+    pool, arrays = vp(), [b for layer in range(host.n_layers) for b in model.kv_buffers(layer)[:2]]
+    for b in arrays:
+        dev.memset(b, 0xFF)                            # (NaN wherever these calls do not write)
+    ok(L.tq_pages_create(ctx, n_pages, page_rows, n, table_ld, None, None, None, C.byref(pool)))
+    ok(L.tq_pages_arrays(pool, (vp * len(arrays))(*[b.ptr for b in arrays]), len(arrays), host.n_kv * host.hd * 2))
+    held = length - 1
+    used = -(-held // page_rows)
+    refs, tables, lens = np.zeros(n_pages, np.int32), np.full((n, table_ld), -1, np.int32), np.zeros(n, np.int32)
+    refs[:used], tables[0, :used], lens[0] = 1, np.arange(used), held
+    logits, rates, chosen = room(n * V), room(n), room(n, tb.I32)
+    ok(L.tq_llama_prefill(m, ints(prompt[:held]), ints([0]), 1, held, logits))
+    state = [vp() for _ in range(3)]
+    ok(L.tq_pages_data(pool, *(C.byref(p) for p in state)))
+    for p, a in zip(state, (refs, tables, lens)):
+        ok(L.tq_upload(ctx, p, vp(a.ctypes.data), a.nbytes))
+    ok(L.tq_pages_fork(pool, ints([0] * (n - 1)), ints(range(1, n)), None, n - 1))
+    tokens, positions, out_tokens, step_no = ints([prompt[-1]] * n), ints([held] * n), ints(np.zeros((n, n_new))), ints([0])
+    seqs, starts, shared = ints(range(n)), ints([0]), ints([held])
+    keep.append(dev.upload((5 + np.arange(n, dtype=np.uint64)).view(np.float64), tb.F64))
+    rng = vp(keep[-1].ptr)
+
+    def step():
+        ok(L.tq_pages_extend(pool, seqs, None, n))
+        ok(L.tq_llama_decode_paged(m, tokens, pool, seqs, n, starts, shared, 1, held, length + n_new, logits))
+        ok(L.tq_sample(ctx, logits, 1, n, V, C.byref(cfg), rng, None, None, 0, chosen))
+        ok(L.tq_token_logprobs(ctx, logits, tb.F32, 0, 1, n, V, chosen, 1, 0, rates, None, None, None))
+        ok(L.tq_generate_advance(ctx, chosen, n, tokens, positions, out_tokens, n_new, step_no, None))
+
+    step()
+    ok(L.tq_graph_begin(ctx))
+    step()
+    g = vp()
+    ok(L.tq_graph_end(ctx, C.byref(g)))
+    for _ in range(1, n_new):
+        ok(L.tq_graph_launch(ctx, g))
+    dev.sync()
+    read = lambda p: next(b for b in keep if b.ptr == p.value).to_vec()
+    assert np.array_equal(read(out_tokens).reshape(n, n_new), want.tokens[0]) and np.array_equal(read(rates), want.logprobs[0, :, -1])
+    ok(L.tq_graph_free(ctx, g))
+    L.tq_pages_destroy(pool)
+    model.destroy()
