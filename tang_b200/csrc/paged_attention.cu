@@ -50,18 +50,20 @@ __device__ __forceinline__ int paged_row_of(const PagedParams& p, int b) {
 constexpr int kPuThreads = 416;
 constexpr int kPuTile = 4 * kPfBox / 2;               // bytes of 128 rows of keys or values
 constexpr int kPuRing = 5;
-constexpr int kPuWeights = 2 * 16 * 128;              // a parity's weights where keys are the lanes: two terms of eight rows of 128 keys, in two halves
+constexpr int kPuWeights = 2 * 32 * 128;              // a parity's weights where keys are the lanes: three terms of eight rows (32 columns) of 128 keys, in two halves
 constexpr int kPuOnes = 1024;                         // eight rows of 64 ones
 constexpr int kPuMeet = (2 + 2) * 128 * 4;            // maxima [parity][warp][row], references [run's parity][row, or warp and row]
 constexpr float kPuLargest = 7.9228162514264338e28f;  // 2^96: a weight above it is too far from its reference
 constexpr int kPuHeader = 640;                        // barriers, pieces
 constexpr int kPuReaders = 12;                        // warps that are told the pieces
 constexpr int kPuPieces = 4;                          // pieces that are told ahead
-// Tiles of a piece, for f32 and for bf16 results: the tensor core truncates what it adds up, about 4e-9 of a sum for a position (64 sequences of 16384
-// positions in one piece each, with values of one sign, were off by 7e-5, in pieces of 2048 by 4e-6).  Powers of two; only a run's first piece has another
-// number, 1 more at most and 2 at least: so the last tiles of a run's pieces have the same parity, and a thread that adds to a partial result adds to what
-// it wrote itself.
-constexpr int kPuWindow[2] = {16, 128};
+// Tiles of a piece, own and shared ones, for f32 and for bf16 results: the tensor core truncates what it adds up, about 4e-9 of a sum for a position (64
+// sequences of 16384 positions in one piece each, with values of one sign, were off by 7e-5).  f32 results of 64 sequences of up to 2048 positions: error
+// from 64 bits 1.9e-6 in pieces of 16 tiles, 1.2e-6 in pieces of 8 (the attention over slots 1.4e-6, f32 arithmetic 0.9e-6), 56.6 and 57.8 us; 64 samples of a
+// prompt of 8192, whose shared tiles add both terms of a weight to the same sums, 3.6e-6 in pieces of 8 tiles, 2.8e-6 in pieces of 4, 36.9 and 42.5 us.
+// Powers of two; only a run's first piece has another number, 1 more at most and 2 at least: so the last tiles of a run's pieces have the same parity, and
+// a thread that adds to a partial result adds to what it wrote itself.
+constexpr int kPuWindow[2][2] = {{8, 4}, {128, 128}};
 __device__ __forceinline__ int pu_piece(int left, int window) { return left <= window + 1 ? left : ((left - 2) & (window - 1)) + 2; }
 constexpr int kPuBatch = 1024;                        // sequences of a call
 constexpr size_t kPuFixed = 2 * (size_t)kPfBox + kPuRing * (size_t)kPuTile + 2 * (size_t)kPuWeights + kPuOnes + kPuMeet + kPuHeader;
@@ -135,7 +137,7 @@ __device__ __forceinline__ int pu_values_at(int t) { return 2 * t + 2; }
 struct PuParams {
   PagedParams a;
   int per_tile, per_eight, n_shares;                  // members of a row tile; of eight rows; CTAs of a KV head
-  int window;                                         // tiles of a piece
+  int window[2];                                      // own, shared tiles of a piece
   float *own_o, *own_ml, *pre_o, *pre_ml;             // partial results: [row][128], [row][2] references and sums (of the groups)
   PuSeqPlan* plan;                                    // [batch]
   int* share;                                         // [2]
@@ -177,7 +179,7 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// LONG: there may be runs of several pieces.
+// LONG: there may be runs of several pieces.  (The form without has less code to fetch: one sequence of 700 positions 9.4 us, with it 9.8.)
 template <bool LONG>
 __global__ void __launch_bounds__(kPuThreads, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_constant__ CUtensorMap q_whole,
@@ -354,7 +356,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
         w.out = w.kv * (p.batch * p.group + apart * pp.n_shares) + u.b0 * p.group + apart * cta;
         w.what = k | (u.rows <= 8) << 1 | (run & 3) << 4;
         for (++run; left > 0 && ok; w.what |= 4, w.tile += w.n) {
-          w.n = LONG ? pu_piece(left, pp.window) : left;
+          w.n = LONG ? pu_piece(left, pp.window[k]) : left;
           left -= w.n;
           w.what = left > 0 ? w.what | 8 : w.what & ~8;
           w.last = left > 0 ? kPfTile : last;
@@ -496,7 +498,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
       if (leader) {
         const uint64_t at = vd + (uint64_t)(slot * (kPuTile >> 4));
         if (w.keyed) {
-          const uint32_t idesc = umma_idesc_bf16(16);
+          const uint32_t idesc = umma_idesc_bf16(32);
           for (int k = 0; k < w.steps; ++k) {
             const uint64_t wk = wd + (uint64_t)(x * (kPuWeights >> 4) + (k >> 2) * (kPuWeights >> 5) + 2 * (k & 3));
             umma_f16(o_t, at + (uint64_t)(k * (2048 >> 4)), wk, idesc | (1u << 15), !w.first || k != 0);
@@ -556,9 +558,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
     // are the tensor memory's lanes, S^T = K Q^T and O^T = V^T P with 16 columns (a product of 128 x 128 x 16 takes 84 cycles for four rows too, one of
     // 128 x 16 x 16 a fraction): a thread per key, whose weights go to shared memory, and the weights' sums come from a product with ones.  (Both ways for 9
     // to 32 rows: 16 groups of four samples 41.8 us with keys as lanes and 42.4 with rows, 64 samples by fours 71.6 and 70.4.)
-    // A weight is two bf16 terms, hi + lo, within 2^-16 of it, as in the attention over slots.  (Three would be nearer to f32 results, whose error from
-    // 64 bits is 2e-6 so and 8e-7 by f32 arithmetic, but tensor memory has no columns for them.  One, within 2^-8, would be as far off as the rounding of a
-    // bf16 result.)
+    // A weight is bf16 terms, each the rounding of what those before leave.  Two, within 2^-16 of it as in the attention over slots, where rows are the lanes
+    // (one, within 2^-8, would be as far off as the rounding of a bf16 result).  Three, an f32 number's bits, where keys are: their columns are there and cost
+    // nothing (8 sequences of up to 700 positions, f32 results: error from 64 bits 1.9e-6 with two, 0.5e-6 with three, 14.2 us both), while a third product of
+    // 128 rows does (16 groups of four samples 39 -> 46 us for 2.0e-6 -> 1.6e-6).
     // The reference that scores are taken from is their maximum in the run's first tile, which the group with that tile tells the other one: a bf16 weight
     // may be as large as an f32 one, so that nothing is rescaled; a weight above 2^96 becomes no number, and the joining kernel goes through the row's keys
     // one by one.
@@ -606,28 +609,33 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
         const float e = ex2(fmaf(v[r], p.scale_log2, -from[r])), w = !seen ? 0.f : e > kPuLargest ? NAN : e;
         const __nv_bfloat16 hi = __float2bfloat16_rn(w);
         uint8_t* to = at + r * 128 + ((chunk ^ r) << 4);
+        const float rest = w - __bfloat162float(hi);
+        const __nv_bfloat16 second = __float2bfloat16_rn(rest);
         *reinterpret_cast<__nv_bfloat16*>(to) = hi;
-        *reinterpret_cast<__nv_bfloat16*>(to + 1024) = __float2bfloat16_rn(w - __bfloat162float(hi));
+        *reinterpret_cast<__nv_bfloat16*>(to + 1024) = second;
+        *reinterpret_cast<__nv_bfloat16*>(to + 2048) = __float2bfloat16_rn(rest - __bfloat162float(second));
       }
       tc_fence_before();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     };
     auto keyed_out = [&](float* to_o, float* to_ml) {
-      float o[8], low[8], sum[8], sum_low[8], was[8];
+      float o[8], low[2][8], sum[8], sum_low[2][8], was[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) was[r] = LONG && u.later() && r < u.rows ? to_o[r * kPaDim + t128] : 0.f;
       __syncwarp();
       tmem_ld8(o_t, o);
-      tmem_ld8(o_t + 8u, low);
+      tmem_ld8(o_t + 8u, low[0]);
+      tmem_ld8(o_t + 16u, low[1]);
       tmem_ld8(o_t + 64u, sum);
-      tmem_ld8(o_t + 72u, sum_low);
+      tmem_ld8(o_t + 72u, sum_low[0]);
+      tmem_ld8(o_t + 80u, sum_low[1]);
       tc_fence_before();
       arrive(&o_free[slot]);                           // (the products of the piece after the next may begin)
       float l = 0.f;                                   // of the lane's row
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        if (r < u.rows) to_o[r * kPaDim + t128] = was[r] + (o[r] + low[r]);
-        if (lane == r) l = sum[r] + sum_low[r];
+        if (r < u.rows) to_o[r * kPaDim + t128] = was[r] + (o[r] + (low[0][r] + low[1][r]));
+        if (lane == r) l = sum[r] + (sum_low[0][r] + sum_low[1][r]);
       }
       sum_all = LONG && u.later() ? sum_all + l : l;
       if (!(LONG && u.more()) && q4 == 0 && lane < u.rows) *reinterpret_cast<float4*>(to_ml + lane * 4) = make_float4(ref, sum_all, ref, 0.f);
@@ -976,9 +984,14 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   const size_t n_ctas = pp.n_shares * n_kv_heads;
   // partial results (rows of either kind: the list's, and what a CTA adds), the sequences' plans
   // (The form without LONG has less code to fetch: one sequence of 700 positions 9.3 us, with it 9.8; 16 groups of four samples 40.5 and 41.6.)
-  pp.window = kPuWindow[!p.out_f32];
-  const size_t longest = ((size_t)p.max_len + kPfTile - 1) / kPfTile;      // (tiles of a run: no more than a sequence has)
-  auto kern = longest > (size_t)pp.window + 1 ? paged_decode_kernel<true> : paged_decode_kernel<false>;
+  // (tiles of a run: no more than a sequence has)
+  const size_t longest[2] = {((size_t)p.max_len + kPfTile - 1) / kPfTile, p.n_groups ? (size_t)p.max_shared / kPfTile : 0};
+  bool pieces = false;
+  for (int k = 0; k < 2; ++k) {
+    pp.window[k] = kPuWindow[!p.out_f32][k];
+    pieces = pieces || longest[k] > (size_t)pp.window[k] + 1;
+  }
+  auto kern = pieces ? paged_decode_kernel<true> : paged_decode_kernel<false>;
   const size_t own_rows = batch * n_heads + 8 * n_ctas, pre_rows = p.n_groups ? batch * n_heads + 128 * n_ctas : 0, floats = (own_rows + pre_rows) * (kPaDim + 4);
   if (int st = ensure_scratch(ctx, floats * sizeof(float) + (batch + 1) * sizeof(PuSeqPlan))) return st;
   pp.own_o = static_cast<float*>(ctx->scratch);

@@ -411,7 +411,7 @@ def test_bf16_results_are_off_by_their_own_rounding(dev, name):
 @pytest.mark.parametrize("shared", [False, True])
 def test_a_loose_bound_costs_no_precision(dev, shared):
     """As ``test_long_sums_keep_the_precision_of_f32``, with the bounds of a caller who has recorded a graph for any length: eight KV heads, tables for a
-    million positions.  A piece has 2176 positions at most."""
+    million positions.  A piece has no more than 2176 positions."""
     import tang_b200 as tb
 
     rng, L, P, B, nh, nkv, ld = np.random.default_rng(28), 16384, 128, 64, 32, 8, 8192
@@ -518,3 +518,30 @@ def test_rows_that_are_attended_again(dev, P, f32):
     assert np.isnan(g[s.lens > 1][:, :, 5]).all()
     off = (2.0 ** -14 + 128 * 2.0 ** -24 * 8 * 12) * size              # scores up to 8 * 12 here, sums of 128 products
     assert (np.abs(g - want)[ok] <= (off + (0 if f32 else 2.0 ** -8) * (np.abs(want) + off))[ok]).all()
+
+
+@pytest.mark.parametrize("case", ["few rows", "many rows"])
+def test_f32_results_keep_all_bits_of_the_weights(dev, case):
+    """Scores of one product each, which f32 holds, of two keys that count and others far below them: what is left of the error is the weights'.  An exponent
+    (base 2: a score of 2.9 at most, 5.7 from the largest) is off by 2^-24 of either, 2^-21.4 of the weight, its exponential by 2^-22: for numerator and
+    denominator 2^-19.7; two sums and a division, 3 * 2^-23: 2^-19 of the sum of |weight value|.  Where rows are the lanes, a weight is two terms: 2^-16 of it
+    more."""
+    s = Setup(16, 4, 16, [(0, [16])] * 60 if case == "few rows" else [(128, [128] * 12) for _ in range(8)], seed=71)
+    rng = np.random.default_rng(72)
+    s.q_bits[:], s.q[:] = 0, 0
+    bits, f = bf16_round(rng.uniform(8, 22, (s.B, 16)).astype(np.float32))
+    s.q_bits[:, :, 0], s.q[:, :, 0] = bits.reshape(f.shape), f
+    for page in np.unique(s.tables[s.tables >= 0]):
+        x = np.full((s.P, s.nkv), -300, np.float32)
+        first = case == "few rows" or page in s.tables[:, 0]
+        for g in range(s.nkv if first else 0):
+            x[rng.permutation(s.P)[:2], g] = rng.uniform(-1, 1, 2)
+        bits, f = bf16_round(x)
+        s.kv_bits[0, page], s.kv[0, page] = 0, 0
+        s.kv_bits[0, page, :, :, 0], s.kv[0, page, :, :, 0] = bits.reshape(f.shape), f
+    s.put(dev)
+    got = s.run(True).to_vec()
+    dev.sync()
+    want, size = s.reference()
+    err = np.abs(got.reshape(want.shape) - want) / size
+    assert err.max() <= 2.0 ** -19 + (2.0 ** -16 if case == "many rows" else 0), (err.max(), np.sqrt((err ** 2).mean()))
