@@ -20,7 +20,7 @@ SCALARS = {
     "int": "c_int", "size_t": "usize", "float": "f32", "double": "f64", "uint32_t": "u32", "uint64_t": "u64",
     "int8_t": "i8", "unsigned long long": "u64", "unsigned": "c_uint", "char": "c_char", "void": "c_void",
 }
-OPAQUE = ["tq_ctx", "tq_qweight", "tq_comm", "tq_llama", "tq_moe", "tq_graph"]
+OPAQUE = re.findall(r"typedef struct (tq_\w+) \1;", open(HEADER).read())     # handles: pointers to them is all that a caller has
 
 
 def strip_comments(text: str) -> str:

@@ -14,6 +14,11 @@ pub struct tq_qweight {
 }
 
 #[repr(C)]
+pub struct tq_pages {
+    _private: [u8; 0],
+}
+
+#[repr(C)]
 pub struct tq_comm {
     _private: [u8; 0],
 }
@@ -25,6 +30,36 @@ pub struct tq_llama {
 
 #[repr(C)]
 pub struct tq_moe {
+    _private: [u8; 0],
+}
+
+#[repr(C)]
+pub struct tq_mla {
+    _private: [u8; 0],
+}
+
+#[repr(C)]
+pub struct tq_dweight {
+    _private: [u8; 0],
+}
+
+#[repr(C)]
+pub struct tq_tofazen {
+    _private: [u8; 0],
+}
+
+#[repr(C)]
+pub struct tq_numuzen {
+    _private: [u8; 0],
+}
+
+#[repr(C)]
+pub struct tq_dotanex {
+    _private: [u8; 0],
+}
+
+#[repr(C)]
+pub struct tq_sakinex {
     _private: [u8; 0],
 }
 

@@ -48,3 +48,11 @@ def test_every_exported_symbol_is_declared_with_its_arity():
                                    "max_batch", "eps", "rope_base"]
     assert dict(cfg)["eps"] == "f32" and dict(cfg)["rope_base"] == "f64" and dict(cfg)["max_seq"] == "u32"
     assert dict(enums["tq_status"])["TQ_ETIMEOUT"] == 4
+
+
+def test_every_type_that_a_declaration_names_is_declared():
+    """A handle without its struct is a crate that does not compile."""
+    text = open(os.path.join(ROOT, "rust", "tangq-sys", "src", "lib.rs")).read()
+    named = set(re.findall(r"(?:\*mut|\*const) (tq_\w+)", text))
+    declared = re.findall(r"pub struct (tq_\w+)", text)
+    assert named <= set(declared) and len(set(declared)) == len(declared), named - set(declared)
