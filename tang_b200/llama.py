@@ -4,6 +4,7 @@ for one new token per sequence) and its use of ``tang_infer::KVCache``."""
 from __future__ import annotations
 
 import ctypes as C
+import weakref
 from dataclasses import dataclass
 
 import numpy as np
@@ -94,6 +95,7 @@ class LlamaModel:
         dev._check(dev._L.tq_llama_create(dev._ctx, C.byref(cfg), C.c_void_p(comm.handle if comm else 0), C.byref(h)))
         self.handle = h.value
         self._keep = []
+        self._pools = weakref.WeakSet()      # over this model's caches
 
     def set_layer(self, layer: int, w: LlamaLayerWeights) -> None:
         self._keep.append(w)
@@ -142,14 +144,16 @@ class LlamaModel:
         """A ``PagePool`` over the caches of all layers, seen as max_batch * max_seq / page_rows pages: the rows that ``prefill`` and ``decode``
         give sequence b are the pages from b * max_seq / page_rows on.  `page_rows`: the largest of 64, 32 and 16 that divides max_seq unless
         given.  `state`: refs, tables, lens of ``PagePool``.  The pool starts empty: rows that ``prefill`` wrote become a sequence's when its state
-        says so (see ``sample``).  It must not be used once the model is destroyed."""
+        says so (see ``sample``).  It is destroyed with the model."""
         c = self.cfg
         if page_rows is None:
             page_rows = next((p for p in (64, 32, 16) if c.max_seq % p == 0), 0)
         if page_rows < 1 or c.max_seq % page_rows:
             raise _lib.TangqError(_lib.TQ_EINVAL, f"page_pool: max_seq {c.max_seq} is not a multiple of the pages' rows (16 or more)")
         arrays = [b for layer in range(c.n_layers) for b in self.kv_buffers(layer)[:2]]
-        return PagePool(self.dev, c.max_batch * c.max_seq // page_rows, page_rows, n_seqs, c.max_seq // page_rows, arrays, **state)
+        pool = PagePool(self.dev, c.max_batch * c.max_seq // page_rows, page_rows, n_seqs, c.max_seq // page_rows, arrays, **state)
+        self._pools.add(pool)
+        return pool
 
     def decode_paged(self, token_ids: Buffer, pool: PagePool, batch: int, max_len: int, logits: Buffer, seqs: Buffer | None = None,
                      group_starts: Buffer | None = None, shared: Buffer | None = None, n_groups: int = 0, max_shared: int = 0) -> None:
@@ -234,5 +238,7 @@ class LlamaModel:
 
     def destroy(self) -> None:
         if self.handle:
+            for pool in list(self._pools):
+                pool.destroy()
             self.dev._L.tq_llama_destroy(C.c_void_p(self.handle))
             self.handle = 0

@@ -466,3 +466,38 @@ def test_the_calls_of_the_integration_guide(dev):
     ok(L.tq_graph_free(ctx, g))
     L.tq_pages_destroy(pool)
     model.destroy()
+
+
+def test_a_models_pools_go_with_it(dev):
+    """They would copy rows of caches that are gone; so would a recorded step."""
+    import tang_b200 as tb
+
+    host = host_model(29)
+    model, other = host.to_device(dev, 64, 2), host.to_device(dev, 64, 2)
+    pool, more = model.page_pool(2), other.page_pool(2)
+    seqs, tok, lg = dev.upload(np.arange(2, dtype=np.int32), tb.I32), dev.upload(np.zeros(2, np.int32), tb.I32), dev.alloc(2 * host.vocab)
+
+    def step(m, p):
+        p.extend(seqs)
+        m.decode_paged(tok, p, 2, 64, lg)
+
+    graphs = []
+    for m, p in ((model, pool), (other, more)):
+        step(m, p)
+        dev.sync()
+        dev.begin_capture()
+        step(m, p)
+        graphs.append(dev.end_capture())
+    model.destroy()
+    with pytest.raises(tb.TangqError, match="pool of pages"):
+        graphs[0].launch()
+    for call in (lambda: pool.extend(seqs), lambda: pool.free(seqs), pool.compact):
+        with pytest.raises(tb.TangqError):
+            call()
+    graphs[1].launch()
+    dev.sync()
+    assert more.state()[2].tolist() == [2, 2]
+    for x in graphs:
+        x.free()
+    other.destroy()
+    pool.destroy()
