@@ -5,8 +5,9 @@
 //     log sum exp x = m + log c + log1p(s / c),      H = log c + log1p(s / c) + sum (m - x) exp(x - m) / (c + s),
 // so that a model that is sure of a token (log probability and entropy near zero) loses nothing to the addition of the leading one.
 //
-// What bounds it: the logits' bytes where rows are many (1024 x 128256 f32 79.5 us, 6.6 TB/s; as many bytes of bf16 86 us, 6.1 TB/s, where
-// every logit costs an exponential, a share of a maximum and half an addition and multiplication); the latency of the launch, the
+// What bounds it: the logits' bytes where rows are many (1024 x 128256 f32 79 us, 6.6 TB/s; as many bytes of bf16 85 us, 6.2 TB/s, where
+// every logit costs an exponential, a share of a maximum and half an addition and multiplication; from a graph over six inputs: calls from Python over one
+// input take 93 to 98); the latency of the launch, the
 // cluster's meeting and, with alternatives, of sorting 128 maxima where they are few (one row of 32000 4.0 us, 6.6 with five alternatives).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

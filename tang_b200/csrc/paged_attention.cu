@@ -43,9 +43,10 @@ __device__ __forceinline__ int paged_row_of(const PagedParams& p, int b) {
 //
 // What bounds it: the bytes of the cache, once, where sequences are long (537 MB in 97 us, 5.5 TB/s; the steady state is 2800 cycles for a tile of 64 KB,
 // which is an SM's share of the memory's rate); beside them a start of 5 us (lengths, plan, first pages, first tile: six loads in a row) and 4 us until the
-// second kernel is through, which are most of a small call (one sequence of 700 positions 8.8 us, 8 samples of a prompt of 2040 16.3).  A shared tile of
-// 128 rows is 2000 cycles: two products of 670 each, of two softmax groups in turn, and 64 KB from L2 (64 samples of a prompt of 8192: 42 us, of which the
-// shared part is 11).
+// second kernel is through, which are most of a small call (one sequence of 700 positions 8.5 us, 8 samples of a prompt of 2040 16.0, of which 5.5 come with
+// the first shared tile: queries, the first instructions of that path and 128 rows to read out).  A shared tile of 128 rows is a product for the scores and
+// two for the weights' terms, of two softmax groups in turn, and 64 KB from L2 (64 samples with 512 positions of their own: 35.5 us behind a prompt of
+// 2048, 38.7 of 4096, 45.0 of 8192).
 // ---------------------------------------------------------------------------------------------
 constexpr int kPuThreads = 416;
 constexpr int kPuTile = 4 * kPfBox / 2;               // bytes of 128 rows of keys or values
@@ -336,8 +337,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
     PuPiece w{};
     w.kv = (int)blockIdx.x - cta * p.n_kv;
     // Own tiles first where there are several shared ones: the first burst of copies is the own tiles', which only one CTA reads, and shared ones find the
-    // other heads' rows in L2 by the time they are needed (64 samples by fours 69.0 us, the other way 71.8; one prefix 41.5 and 42.2; but 8 samples with a
-    // shared tile a CTA 16.9 and 16.4).
+    // other heads' rows in L2 by the time they are needed (64 samples by fours 59.2 us, the other way 60.4; one prefix 44.9 and 46.6; but 8 samples with a
+    // shared tile a CTA 16.6 and 16.0).
     const bool own_first = l.share[1] > 1;
     int run = 0;
 #pragma unroll 1
@@ -555,9 +556,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
     if (!ok) abandon(DERR_FULL_WAIT);
   } else if (warp >= 4) {
     // ---- softmax of the tiles of a parity.  More than eight rows: S = Q K^T, a thread per row, the weights over the scores' columns.  Up to eight: the keys
-    // are the tensor memory's lanes, S^T = K Q^T and O^T = V^T P with 16 columns (a product of 128 x 128 x 16 takes 84 cycles for four rows too, one of
-    // 128 x 16 x 16 a fraction): a thread per key, whose weights go to shared memory, and the weights' sums come from a product with ones.  (Both ways for 9
-    // to 32 rows: 16 groups of four samples 41.8 us with keys as lanes and 42.4 with rows, 64 samples by fours 71.6 and 70.4.)
+    // are the tensor memory's lanes, S^T = K Q^T with 16 columns and O^T = V^T P with 32 (a product of 128 x 128 x 16 takes 84 cycles for four rows too,
+    // one of 128 x 16 x 16 a fraction): a thread per key, whose weights go to shared memory, and the weights' sums come from a product with ones.  (Both ways for 9
+    // to 32 rows, with two terms of a weight: 16 groups of four samples 41.8 us with keys as lanes and 42.4 with rows, 64 samples by fours 71.6 and 70.4.)
     // A weight is bf16 terms, each the rounding of what those before leave.  Two, within 2^-16 of it as in the attention over slots, where rows are the lanes
     // (one, within 2^-8, would be as far off as the rounding of a bf16 result).  Three, an f32 number's bits, where keys are: their columns are there and cost
     // nothing (8 sequences of up to 700 positions, f32 results: error from 64 bits 1.9e-6 with two, 0.5e-6 with three, 14.2 us both), while a third product of
@@ -983,7 +984,6 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   pp.n_shares = (int)(most_ctas > n_kv_heads ? most_ctas / n_kv_heads : 1);
   const size_t n_ctas = pp.n_shares * n_kv_heads;
   // partial results (rows of either kind: the list's, and what a CTA adds), the sequences' plans
-  // (The form without LONG has less code to fetch: one sequence of 700 positions 9.3 us, with it 9.8; 16 groups of four samples 40.5 and 41.6.)
   // (tiles of a run: no more than a sequence has)
   const size_t longest[2] = {((size_t)p.max_len + kPfTile - 1) / kPfTile, p.n_groups ? (size_t)p.max_shared / kPfTile : 0};
   bool pieces = false;

@@ -7,7 +7,8 @@
 // written and the status word says why.  Pages are handed out lowest number first, in the order of the list, so that the same calls give
 // the same tables.  What is copied is listed by that CTA and moved by a second kernel over all SMs.
 // What bounds it: the copied bytes, where there are many (64 half pages in 32 arrays, 134 MB each way, 54 us with the calls before), else launches and one
-// CTA's chain of loads: tq_pages_free 2.3 us for 64 sequences, tq_pages_fork 4.0, tq_pages_extend without a copy 6.5 (two kernels).
+// CTA's chain of loads: tq_pages_free 2.9 us for 64 sequences, tq_pages_fork 5.9 (0.6 and 1.5 of these for the look at all table
+// entries before any is changed), tq_pages_extend without a copy 6.2 (two kernels).
 #include <new>
 
 #include "common.cuh"
