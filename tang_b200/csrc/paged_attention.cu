@@ -66,6 +66,10 @@ constexpr int kPuPieces = 4;                          // pieces that are told ah
 // a thread that adds to a partial result adds to what it wrote itself.
 constexpr int kPuWindow[2][2] = {{8, 4}, {128, 128}};
 __device__ __forceinline__ int pu_piece(int left, int window) { return left <= window + 1 ? left : ((left - 2) & (window - 1)) + 2; }
+// f32 results: groups of up to so many rows are attended by eight rows at a time, keys as the lanes, with three terms of a weight; more rows than that read the
+// same tiles too often.  16 rows: 16 groups of four samples 39.5 -> 40.6 us and 1.9e-6 -> 0.9e-6 of error from 64 bits, four groups behind prompts of 8192
+// 31.1 -> 34.5 and 2.7e-6 -> 0.8e-6; 32 rows: 8 groups behind prompts of 2040 41.8 -> 61.1 for 2.6e-6 -> 0.8e-6; 64 rows: 40.6 -> 97.8.
+constexpr int kPuFewRows = 16;
 constexpr int kPuBatch = 1024;                        // sequences of a call
 constexpr size_t kPuFixed = 2 * (size_t)kPfBox + kPuRing * (size_t)kPuTile + 2 * (size_t)kPuWeights + kPuOnes + kPuMeet + kPuHeader;
 
@@ -73,7 +77,8 @@ constexpr size_t kPuFixed = 2 * (size_t)kPfBox + kPuRing * (size_t)kPuTile + 2 *
 struct PuPlan {
   int *own, *last, *pre;                              // [batch + 1] own tiles of the sequences before; [batch] shared tiles << 8 | keys of the last tile - 1;
                                                       // [groups + 1] units' shared tiles of the groups before
-  int batch, groups, group, per_tile;
+  int batch, groups, group, per_tile, per_eight, few;
+  __device__ __forceinline__ int unit(int members) const { return members <= few ? per_eight : per_tile; }      // members of a unit of such a group
   int share[2];                                       // own, shared tiles of a CTA
 };
 // What the kernel that joins the pieces has to know: where a sequence's tiles stand in a KV head's list.
@@ -103,9 +108,9 @@ __device__ __forceinline__ PuUnit pu_locate(const PagedParams& p, const PuPlan& 
     u.tiles = l.last[start] >> 8;
     const int rest = f - l.pre[g], rt = rest < u.tiles ? 0 : rest / u.tiles;
     u.tile = rest - rt * u.tiles;
-    u.b0 = start + rt * l.per_tile;
+    u.b0 = start + rt * l.unit(members);
     u.head = start;                    // the group's first member
-    u.rows = min(l.per_tile, members - rt * l.per_tile) * l.group;
+    u.rows = min(l.unit(members), members - rt * l.unit(members)) * l.group;
     u.shared_tiles = 0;
     u.last = kPfTile;
   } else {
@@ -137,7 +142,7 @@ __device__ __forceinline__ int pu_values_at(int t) { return 2 * t + 2; }
 
 struct PuParams {
   PagedParams a;
-  int per_tile, per_eight, n_shares;                  // members of a row tile; of eight rows; CTAs of a KV head
+  int per_tile, per_eight, few, n_shares;             // members of a row tile; of eight rows; of a group that is attended by eight rows; CTAs of a KV head
   int window[2];                                      // own, shared tiles of a piece
   float *own_o, *own_ml, *pre_o, *pre_ml;             // partial results: [row][128], [row][2] references and sums (of the groups)
   PuSeqPlan* plan;                                    // [batch]
@@ -214,6 +219,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
   l.batch = p.batch;
   l.group = p.group;
   l.per_tile = pp.per_tile;
+  l.per_eight = pp.per_eight;
+  l.few = pp.few;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
     if (lane == 0) {
@@ -287,7 +294,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
     least = __reduce_min_sync(0xffffffffu, least);
     const int tiles = members > 1 ? least / kPfTile : 0;
     for (int b = start + lane; b < end; b += 32) l.last[b] = tiles << 8;
-    if (lane == 0) l.pre[g] = members <= pp.per_tile ? tiles : tiles * ((members + pp.per_tile - 1) / pp.per_tile);
+    if (lane == 0) l.pre[g] = members <= l.unit(members) ? tiles : tiles * ((members + l.unit(members) - 1) / l.unit(members));
   }
   if (l.groups) __syncthreads();
   if (warp == 0)
@@ -442,7 +449,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
             if (pu_group_start(p, mid) <= b) lo = mid;
             else hi = mid;
           }
-          pre_f = l.pre[lo] + (b - pu_group_start(p, lo)) / l.per_tile * shared;
+          const int start = pu_group_start(p, lo);
+          pre_f = l.pre[lo] + (b - start) / l.unit(pu_group_end(p, lo, start) - start) * shared;
         }
         pp.plan[b] = PuSeqPlan{l.own[b], l.own[b + 1] - l.own[b], pre_f, shared};
       }
@@ -562,7 +570,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap q_eight, const __grid_co
     // A weight is bf16 terms, each the rounding of what those before leave.  Two, within 2^-16 of it as in the attention over slots, where rows are the lanes
     // (one, within 2^-8, would be as far off as the rounding of a bf16 result).  Three, an f32 number's bits, where keys are: their columns are there and cost
     // nothing (8 sequences of up to 700 positions, f32 results: error from 64 bits 1.9e-6 with two, 0.5e-6 with three, 14.2 us both), while a third product of
-    // 128 rows does (16 groups of four samples 39 -> 46 us for 2.0e-6 -> 1.6e-6).
+    // 128 rows does (64 samples of a prompt of 8192 42.5 -> 50.7 us for 2.8e-6 -> 2.1e-6).
     // The reference that scores are taken from is their maximum in the run's first tile, which the group with that tile tells the other one: a bf16 weight
     // may be as large as an f32 one, so that nothing is rescaled; a weight above 2^96 becomes no number, and the joining kernel goes through the row's keys
     // one by one.
@@ -978,6 +986,7 @@ extern "C" int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k
   PuParams pp;
   pp.per_tile = 128 / p.group;
   pp.per_eight = 8 / p.group;
+  pp.few = p.out_f32 ? kPuFewRows / p.group : 0;
   const size_t tiles = batch * (((size_t)p.max_len + kPfTile - 1) / kPfTile) * n_kv_heads;
   TQ_REQUIRE(ctx, tiles < (1ull << 30) && (size_t)p.n_pages * pages->page_rows < (1ull << 31), "tq_gqa_decode_paged: too many positions");
   const size_t most_ctas = tiles < (size_t)ctx->sm_count ? tiles : (size_t)ctx->sm_count;

@@ -520,13 +520,13 @@ def test_rows_that_are_attended_again(dev, P, f32):
     assert (np.abs(g - want)[ok] <= (off + (0 if f32 else 2.0 ** -8) * (np.abs(want) + off))[ok]).all()
 
 
-@pytest.mark.parametrize("case", ["few rows", "many rows"])
+@pytest.mark.parametrize("case", ["few rows", "sixteen rows", "many rows"])
 def test_f32_results_keep_all_bits_of_the_weights(dev, case):
     """Scores of one product each, which f32 holds, of two keys that count and others far below them: what is left of the error is the weights'.  An exponent
     (base 2: a score of 2.9 at most, 5.7 from the largest) is off by 2^-24 of either, 2^-21.4 of the weight, its exponential by 2^-22: for numerator and
-    denominator 2^-19.7; two sums and a division, 3 * 2^-23: 2^-19 of the sum of |weight value|.  Where rows are the lanes, a weight is two terms: 2^-16 of it
-    more."""
-    s = Setup(16, 4, 16, [(0, [16])] * 60 if case == "few rows" else [(128, [128] * 12) for _ in range(8)], seed=71)
+    denominator 2^-19.7; two sums and a division, 3 * 2^-23: 2^-19 of the sum of |weight value|.  Where rows are the lanes (more than 16 of a
+    group), a weight is two terms: 2^-16 of it more."""
+    s = Setup(16, 4, 16, {"few rows": [(0, [16])] * 60, "sixteen rows": [(128, [128] * 4)] * 20, "many rows": [(128, [128] * 12)] * 8}[case], seed=71)
     rng = np.random.default_rng(72)
     s.q_bits[:], s.q[:] = 0, 0
     bits, f = bf16_round(rng.uniform(8, 22, (s.B, 16)).astype(np.float32))
