@@ -397,9 +397,9 @@ TQ_API int tq_llama_decode_at(tq_llama* model, const int* token_ids_dev, const i
                               size_t batch, size_t max_len, float* logits_dev);
 /* The same step over a pool whose pages are rows of the model's caches (at most max_batch*max_seq rows of every layer: page p's are rows
  * p*page_rows .. of the cache seen as one, so that sequence b's own rows are the pages from b*max_seq/page_rows on).  tq_pages_extend has made
- * room for the new tokens: each is its sequence's last position, below max_len.  A sequence for which the last tq_pages_extend was refused, or whose last
- * page another one holds, is reported by tq_sync (TQ_EINVAL, behind an earlier report), nothing is written for it and its logits are not defined.
- * Sequences (each once) and groups as in tq_gqa_decode_paged, batch at most max_batch. */
+ * room for the new tokens: each is its sequence's last position, below max_len.  A sequence for which the last tq_pages_extend was refused, whose last
+ * page another one holds, or that stands in seqs twice, is reported by tq_sync (TQ_EINVAL, behind an earlier report), nothing is written for it and its
+ * logits are not defined.  Sequences and groups as in tq_gqa_decode_paged, batch at most max_batch. */
 TQ_API int tq_llama_decode_paged(tq_llama* model, const int* token_ids_dev, const tq_pages* pages, const int* seqs_dev_or_null, size_t batch,
                                  const int* group_starts_dev_or_null, const int* shared_dev_or_null, size_t n_groups, size_t max_shared,
                                  size_t max_len, float* logits_dev);

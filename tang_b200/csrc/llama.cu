@@ -47,7 +47,8 @@ __global__ void lens_kernel(const int* positions, int* lens, int n, int max_seq)
 
 // The same for a cache of pages, whose pool has counted the new tokens already: a sequence's new token is its last position, and goes to that
 // position's row of its page.  Whatever does not exist gives row -1, which the kernel that appends K/V reports.  So does a last position that is not the
-// sequence's to write: the pool was asked for room and refused (`refused`), or the page has other holders (it was forked and not extended).
+// sequence's to write: the pool was asked for room and refused (`refused`), the page has other holders (it was forked and not extended), or the sequence
+// stands in the step twice (two tokens for one place).
 __global__ void paged_rows_kernel(const int* tables, const int* lens, const int* refs, const int* refused, const int* seqs, int n, int n_seqs, int table_ld,
                                   int n_pages, int page_rows, int max_len, int* rows, int* positions, int* err) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -60,7 +61,10 @@ __global__ void paged_rows_kernel(const int* tables, const int* lens, const int*
     pos = lens[s] - 1;
     const int page = tables[(size_t)s * table_ld + pos / page_rows];
     if (page >= 0 && page < n_pages) {
-      if (refused[s] == 0 && refs[page] == 1) row = page * page_rows + pos % page_rows;
+      bool once = true;
+      if (seqs)
+        for (int j = 0; j < n; ++j) once = once && (j == i || seqs[j] != s);
+      if (once && refused[s] == 0 && refs[page] == 1) row = page * page_rows + pos % page_rows;
       else atomicCAS(err, 0, (int)DERR_PAGE_LIST);
     }
   }

@@ -501,3 +501,35 @@ def test_a_models_pools_go_with_it(dev):
         x.free()
     other.destroy()
     pool.destroy()
+
+
+def test_a_sequence_that_stands_in_a_step_twice(dev):
+    """Two tokens for one place: reported, and nothing is written for it; the others' step is what it is without it."""
+    import tang_b200 as tb
+
+    host = host_model(31)
+    model = host.to_device(dev, 64, 4)
+    pool, ints, lg = model.page_pool(4, 16), lambda v: dev.upload(np.asarray(v, np.int32), tb.I32), dev.alloc(4 * host.vocab)
+    for t in range(7):
+        pool.extend([0, 1, 2])
+        model.decode_paged(ints([t, t + 1, t + 2]), pool, 3, 64, lg)
+    pool.extend([0, 1, 2])
+    dev.sync()
+    before = caches(model)
+    model.decode_paged(ints([5, 6, 7, 8]), pool, 4, 64, lg, seqs=ints([0, 1, 0, 2]))
+    with pytest.raises(tb.TangqError) as e:
+        dev.sync()
+    assert e.value.status == tb._lib.TQ_EINVAL
+    after, refs_tables = caches(model), pool.state()[1]
+    pages = [int(refs_tables[s, 0]) for s in range(3)]
+    width = host.n_kv * host.hd
+    for a, b in zip(before, after):
+        a, b = (x.reshape(-1, 16, width) for x in (a, b))
+        assert np.array_equal(a[pages[0]], b[pages[0]]) and not np.array_equal(a[pages[1], 7], b[pages[1], 7]) and not np.array_equal(a[pages[2], 7], b[pages[2], 7])
+        rest = np.ones(a.shape[:2], bool)
+        rest[pages[1], 7] = rest[pages[2], 7] = False
+        assert np.array_equal(a[rest], b[rest])
+    model.decode_paged(ints([5, 6, 8]), pool, 3, 64, lg)
+    dev.sync()
+    pool.destroy()
+    model.destroy()
