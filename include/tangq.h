@@ -309,6 +309,44 @@ TQ_API int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k_pag
                                size_t n_groups, size_t max_shared, size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t max_len,
                                void* out_dev, int out_dtype);
 
+/* Packed rows: the new tokens of several sequences behind one another, as a step over prompts of different lengths has them.  Rows seq_rows[i] ..
+ * seq_rows[i+1]-1 ([batch + 1] device values that ascend from 0 to at most `rows`; NULL: row i, and rows = batch) are the last positions of sequence
+ * seqs[i] of the pool (NULL: i), which tq_pages_extend has counted already.  Rows from seq_rows[batch] on are left as they are, so that a recorded
+ * step may have room for more rows than it has.  batch is at most 1024, head_dim 128; arrays are 16-byte aligned.  What does not fit (starts that do not
+ * ascend, a sequence or page that does not exist, more rows than positions) is reported by tq_sync and left out.
+ *
+ * A cache row holds all KV heads of a position: bf16, or 4 bits in tq_q4_row_bytes(n_kv_heads) bytes.  Those are, for each head, 64 bytes of codes (byte i has
+ * value 2i in its low and value 2i+1 in its high four bits, an integer of -7 .. 7 stored as 8 more), then for each head four bf16 scales, one for 32 values, then
+ * zeros up to a multiple of 16 bytes.  A scale is the block's largest magnitude / 7, rounded up to 5 significant bits, so that integer times scale is a
+ * bf16 number exactly.  Blocks below 2^-100 are zeros; a block with a NaN, an infinity or a magnitude of 2^120 is NaN. */
+typedef enum tq_page_rows { TQ_PAGES_BF16 = 0, TQ_PAGES_Q4 = 1 } tq_page_rows;
+TQ_API size_t tq_q4_row_bytes(size_t n_kv_heads);
+/* The step between the fused q/k/v projection and the attention (crates/tang-train/examples/smollm.rs:84-95) for packed rows: x [rows][n_heads query heads,
+ * n_kv_heads keys, n_kv_heads values of 128] f32 or bf16, ldx elements apart (0: dense; a multiple of 16 bytes).  Queries and keys are rotated as by
+ * tq_rope_forward by their positions' rows of the tables [n_positions][64]; queries go to q_out bf16 [rows][n_heads*128], keys and values to the
+ * cache rows of their positions.  Nothing is written for a row whose position is not its sequence's to write (the last tq_pages_extend was refused, the page has
+ * other holders, the sequence stands in seqs twice) or has no row in the tables: it is reported by tq_sync. */
+TQ_API int tq_kv_append_paged(tq_ctx* ctx, const void* x_dev, int x_dtype, size_t ldx, const float* cos_dev, const float* sin_dev, size_t n_positions,
+                              const tq_pages* pages, const int* seqs_dev_or_null, const int* seq_rows_dev_or_null, size_t batch, size_t rows,
+                              size_t n_heads, size_t n_kv_heads, size_t head_dim, void* q_out_dev, void* k_pages_dev, void* v_pages_dev,
+                              int page_rows_as);
+/* The cache rows of packed rows as what they stand for, bf16 [rows][n_kv_heads*128] each: to take a sequence out of the pool, or to look at it. */
+TQ_API int tq_kv_read_paged(tq_ctx* ctx, const void* k_pages_dev, const void* v_pages_dev, int page_rows_as, const tq_pages* pages,
+                            const int* seqs_dev_or_null, const int* seq_rows_dev_or_null, size_t batch, size_t rows, size_t n_kv_heads,
+                            size_t head_dim, void* k_out_dev, void* v_out_dev);
+/* tq_gqa_prefill over pages, for packed rows: q bf16 [rows][n_heads*128], out bf16 the same; a row attends its sequence's positions up to its own, cached ones
+ * and those of the rows before it.  n_heads/n_kv_heads is 1 to 8.  max_len bounds the sequences' lengths: what lies behind it is not attended.  Results of a
+ * sequence with a page that does not exist are not defined.  Weights enter the tensor cores as bf16, 2^-9 of themselves off, and what is divided by is the sum
+ * of what entered. */
+TQ_API int tq_gqa_prefill_paged(tq_ctx* ctx, const void* q_dev, const void* k_pages_dev, const void* v_pages_dev, int page_rows_as,
+                                const tq_pages* pages, const int* seqs_dev_or_null, const int* seq_rows_dev_or_null, size_t batch, size_t rows,
+                                size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t max_len, void* out_dev);
+/* tq_gqa_decode_paged over pages of 4 bits, without groups: one new token for each of `batch` sequences, q and out bf16 [batch, n_heads*128].  A sequence of
+ * length 0 has the result 0. */
+TQ_API int tq_gqa_decode_paged_q4(tq_ctx* ctx, const void* q_dev, const void* k_pages_dev, const void* v_pages_dev, const tq_pages* pages,
+                                  const int* seqs_dev_or_null, size_t batch, size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t max_len,
+                                  void* out_dev);
+
 /* ---- collectives -----------------------------------------------------------------------------
  * NCCL over NVLink at the shard boundaries (the reference's only collective is a star sum over
  * QUIC, crates/tang-mesh/src/allreduce.rs:43-70).  One communicator per context; calls are

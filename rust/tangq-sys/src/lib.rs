@@ -89,6 +89,9 @@ pub const TQ_Q4_F16: c_int = 1;
 pub const TQ_Q8_F32: c_int = 2;
 pub const TQ_I8_ROW: c_int = 3;
 
+pub const TQ_PAGES_BF16: c_int = 0;
+pub const TQ_PAGES_Q4: c_int = 1;
+
 pub const TQ_TZ_EMBED: c_int = 0;
 pub const TQ_TZ_POS: c_int = 1;
 pub const TQ_TZ_FINAL_NORM: c_int = 2;
@@ -519,6 +522,11 @@ extern "C" {
     pub fn tq_pages_free(pages: *mut tq_pages, seqs_dev: *const c_int, n: usize) -> c_int;
     pub fn tq_pages_compact(pages: *mut tq_pages, used_out_dev_or_null: *mut c_int) -> c_int;
     pub fn tq_gqa_decode_paged(ctx: *mut tq_ctx, q_dev: *const c_void, k_pages_dev: *const c_void, v_pages_dev: *const c_void, pages: *const tq_pages, seqs_dev_or_null: *const c_int, batch: usize, group_starts_dev_or_null: *const c_int, shared_dev_or_null: *const c_int, n_groups: usize, max_shared: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, max_len: usize, out_dev: *mut c_void, out_dtype: c_int) -> c_int;
+    pub fn tq_q4_row_bytes(n_kv_heads: usize) -> usize;
+    pub fn tq_kv_append_paged(ctx: *mut tq_ctx, x_dev: *const c_void, x_dtype: c_int, ldx: usize, cos_dev: *const f32, sin_dev: *const f32, n_positions: usize, pages: *const tq_pages, seqs_dev_or_null: *const c_int, seq_rows_dev_or_null: *const c_int, batch: usize, rows: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, q_out_dev: *mut c_void, k_pages_dev: *mut c_void, v_pages_dev: *mut c_void, page_rows_as: c_int) -> c_int;
+    pub fn tq_kv_read_paged(ctx: *mut tq_ctx, k_pages_dev: *const c_void, v_pages_dev: *const c_void, page_rows_as: c_int, pages: *const tq_pages, seqs_dev_or_null: *const c_int, seq_rows_dev_or_null: *const c_int, batch: usize, rows: usize, n_kv_heads: usize, head_dim: usize, k_out_dev: *mut c_void, v_out_dev: *mut c_void) -> c_int;
+    pub fn tq_gqa_prefill_paged(ctx: *mut tq_ctx, q_dev: *const c_void, k_pages_dev: *const c_void, v_pages_dev: *const c_void, page_rows_as: c_int, pages: *const tq_pages, seqs_dev_or_null: *const c_int, seq_rows_dev_or_null: *const c_int, batch: usize, rows: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, max_len: usize, out_dev: *mut c_void) -> c_int;
+    pub fn tq_gqa_decode_paged_q4(ctx: *mut tq_ctx, q_dev: *const c_void, k_pages_dev: *const c_void, v_pages_dev: *const c_void, pages: *const tq_pages, seqs_dev_or_null: *const c_int, batch: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, max_len: usize, out_dev: *mut c_void) -> c_int;
     pub fn tq_comm_unique_id(id_out128: *mut c_void) -> c_int;
     pub fn tq_comm_create(ctx: *mut tq_ctx, id128: *const c_void, rank: c_int, world: c_int, out: *mut *mut tq_comm) -> c_int;
     pub fn tq_comm_destroy(ctx: *mut tq_ctx, comm: *mut tq_comm) -> c_int;

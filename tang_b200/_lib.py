@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(HERE, "libtangq.so")
 TQ_OK, TQ_EINVAL, TQ_ECUDA, TQ_ENCCL, TQ_ETIMEOUT, TQ_ENOMEM, TQ_EUNSUPPORTED = range(7)
 F32, BF16, F16, I8, U8, I32, F64 = range(7)
 Q4_F32, Q4_F16, Q8_F32, I8_ROW = range(4)
+PAGES_BF16, PAGES_Q4 = range(2)
 
 _STATUS = {0: "TQ_OK", 1: "TQ_EINVAL", 2: "TQ_ECUDA", 3: "TQ_ENCCL", 4: "TQ_ETIMEOUT", 5: "TQ_ENOMEM",
            6: "TQ_EUNSUPPORTED"}
@@ -74,6 +75,11 @@ PROTOTYPES = {
     "tq_pages_free": (_i, [_p, _p, _sz]),
     "tq_pages_compact": (_i, [_p, _p]),
     "tq_gqa_decode_paged": (_i, [_p, _p, _p, _p, _p, _p, _sz, _p, _p, _sz, _sz, _sz, _sz, _sz, _sz, _p, _i]),
+    "tq_q4_row_bytes": (_sz, [_sz]),
+    "tq_kv_append_paged": (_i, [_p, _p, _i, _sz, _p, _p, _sz, _p, _p, _p, _sz, _sz, _sz, _sz, _sz, _p, _p, _p, _i]),
+    "tq_kv_read_paged": (_i, [_p, _p, _p, _i, _p, _p, _p, _sz, _sz, _sz, _sz, _p, _p]),
+    "tq_gqa_prefill_paged": (_i, [_p, _p, _p, _p, _i, _p, _p, _p, _sz, _sz, _sz, _sz, _sz, _sz, _p]),
+    "tq_gqa_decode_paged_q4": (_i, [_p, _p, _p, _p, _p, _p, _sz, _sz, _sz, _sz, _sz, _p]),
     "tq_comm_unique_id": (_i, [_p]),
     "tq_comm_create": (_i, [_p, _p, _i, _i, _pp]),
     "tq_comm_destroy": (_i, [_p, _p]),

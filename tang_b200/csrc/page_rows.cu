@@ -1,0 +1,273 @@
+// Rows of a cache of pages (include/tangq.h: tq_kv_append_paged, tq_kv_read_paged): the new tokens of several sequences go to their pages, with the
+// rotation of queries and keys on the way (crates/tang-train/examples/smollm.rs:84-95 does it for one token and a cache of one sequence), and are read back.
+// A cache row is bf16 or of 4 bits: s = the block's largest magnitude / 7, rounded up to 5 significant bits, an integer c = x / s rounded to nearest
+// even, within -7 .. 7, and the value c s, which is a bf16 number (3 + 5 bits): what reads 4 bits multiplies the same numbers as what reads bf16.
+#include "page_rows.cuh"
+
+namespace tq {
+
+constexpr int kAppendThreads = 256;
+
+struct AppendParams {
+  PackedSeqs s;
+  const void* x;
+  size_t ldx;
+  const float *cos_t, *sin_t;
+  int n_positions, n_heads, n_kv;
+  __nv_bfloat16* q_out;
+  uint8_t *k, *v;                      // cache rows of row_bytes
+  size_t row_bytes;
+  int* err;
+};
+
+// The scale of 32 values whose largest magnitude is amax.  Blocks below 2^-100 are zeros, those of 2^120 and above NaN: 24 s, which the readers
+// form, is then a normal number.
+__device__ __forceinline__ float q4_scale(float amax) {
+  if (!(amax < 1.329227995784916e36f)) return __uint_as_float(0x7FC00000u);
+  if (amax < 7.888609052210118e-31f) return 0.f;
+  return __uint_as_float((__float_as_uint(__fdiv_rn(amax, 7.f)) + 0x7FFFFu) & 0xFFF80000u);
+}
+
+// A CTA takes ROWS rows and 256 eighths of a head: 32 bytes (f32) in, 16 or 4 out for a thread and row.  Rows' places are looked up by a warp each
+// (starts, sequence, length, page, holders: five loads one after the other) while the values are on their way.
+template <typename X, int ROWS, bool Q4>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
+  __shared__ int place_s[ROWS], pos_s[ROWS];           // cache row (-1: none), position
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m0 = blockIdx.x * ROWS;
+  const int at = 8 * (blockIdx.y * kAppendThreads + threadIdx.x), width = (p.n_heads + 2 * p.n_kv) * kRowDim;   // value of the row
+  uint4 raw[ROWS][sizeof(X) / 2];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+    if (at < width && m0 + r < p.s.rows) {
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const X*>(p.x) + (size_t)(m0 + r) * p.ldx + at);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(X) / 2; ++i) raw[r][i] = src[i];
+    }
+  if (warp < ROWS) {
+    int place = -1, pos = 0;
+    if (m0 + warp < p.s.rows) {
+      const PackedRow row = packed_row(p.s, m0 + warp, lane);
+      int why = row.bad ? (int)DERR_PAGE_LIST : 0, page = 0, same = 0;
+      if (row.seq >= 0) {
+        pos = row.pos;
+        place = page_row_of(p.s, row.seq, pos, &page);
+        if (place < 0 || pos >= p.n_positions) {
+          why = DERR_POSITION;
+        } else {
+          // a position that is not the sequence's to write: the pool refused to make room, the page has other holders, or the sequence stands in the
+          // list twice
+          if (p.s.seqs)
+#pragma unroll 4
+            for (int j = lane; j < p.s.batch; j += 32) same += p.s.seqs[j] == row.seq;
+          same = p.s.seqs ? (int)__reduce_add_sync(0xffffffffu, same) : 1;
+          if (same != 1 || p.s.refused[row.seq] != 0 || p.s.refs[page] != 1) why = DERR_PAGE_LIST;
+        }
+      }
+      if (why) {
+        place = -1;
+        if (lane == 0 && blockIdx.y == 0) atomicCAS(p.err, 0, why);
+      }
+    }
+    if (lane == 0) {
+      place_s[warp] = place;
+      pos_s[warp] = pos;
+    }
+  }
+  __syncthreads();
+  const int head = at / kRowDim, d = at % kRowDim;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int place = place_s[r], pos = pos_s[r];
+    if (place < 0) continue;           // (the whole CTA)
+    float x[8];
+    if (at < width) {
+      if constexpr (sizeof(X) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(reinterpret_cast<const uint32_t*>(&raw[r][0])[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = reinterpret_cast<const uint32_t*>(&raw[r][0])[i];
+          x[2 * i] = __uint_as_float(w << 16);
+          x[2 * i + 1] = __uint_as_float(w & 0xFFFF0000u);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    }
+    if (head < p.n_heads + p.n_kv) {
+      const float4 c4 = *reinterpret_cast<const float4*>(p.cos_t + (size_t)pos * (kRowDim / 2) + d / 2);
+      const float4 s4 = *reinterpret_cast<const float4*>(p.sin_t + (size_t)pos * (kRowDim / 2) + d / 2);
+      const float cs[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {    // (each product rounded: which 4-bit integer a value becomes does not depend on how a compiler joins them)
+        const float x0 = x[2 * i], x1 = x[2 * i + 1];
+        x[2 * i] = __fsub_rn(__fmul_rn(x0, cs[i]), __fmul_rn(x1, sn[i]));
+        x[2 * i + 1] = __fadd_rn(__fmul_rn(x0, sn[i]), __fmul_rn(x1, cs[i]));
+      }
+    }
+    const bool key = head < p.n_heads + p.n_kv;
+    const int kv_head = head - p.n_heads - (key ? 0 : p.n_kv);
+    uint8_t* row = (key ? p.k : p.v) + (size_t)place * p.row_bytes;
+    if constexpr (Q4) {
+      float amax = 0.f;                // (NaN and infinities have the largest bits)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = __uint_as_float(max(__float_as_uint(amax), __float_as_uint(x[i]) & 0x7FFFFFFFu));
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) amax = __uint_as_float(max(__float_as_uint(amax), __shfl_xor_sync(0xffffffffu, __float_as_uint(amax), o)));
+      if (head >= p.n_heads && at < width) {
+        const float s = q4_scale(amax);
+        uint32_t word = 0x88888888u;
+        if (s > 0.f) {
+          word = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) word |= (uint32_t)((int)rintf(__fdiv_rn(x[i], s)) + 8) << (4 * i);
+        }
+        *reinterpret_cast<uint32_t*>(row + kv_head * kQ4HeadBytes + d / 2) = word;
+        if (d % kQ4Block == 0) {
+          uint16_t* to = reinterpret_cast<uint16_t*>(row + p.n_kv * kQ4HeadBytes) + kv_head * kQ4HeadScales;
+          to[d / kQ4Block] = (uint16_t)(__float_as_uint(s) >> 16);
+          if (kv_head == p.n_kv - 1 && (p.n_kv & 1) && d == 0) *reinterpret_cast<uint2*>(to + kQ4HeadScales) = make_uint2(0u, 0u);      // (the row's end)
+        }
+        continue;
+      }
+    }
+    if (at >= width) continue;
+    __nv_bfloat16* dst = head < p.n_heads ? p.q_out + (size_t)(m0 + r) * p.n_heads * kRowDim + at : reinterpret_cast<__nv_bfloat16*>(row) + kv_head * kRowDim + d;
+    uint4 o;
+    __nv_bfloat162* pk = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pk[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<uint4*>(dst) = o;
+  }
+}
+
+struct ReadParams {
+  PackedSeqs s;
+  const uint8_t *k, *v;
+  size_t row_bytes;
+  int n_kv;
+  __nv_bfloat16 *k_out, *v_out;
+  int* err;
+};
+
+// A CTA takes a row: eight values a thread and turn, keys and then values.
+template <bool Q4>
+__global__ void __launch_bounds__(kAppendThreads) kv_read_kernel(const ReadParams p) {
+  __shared__ int place_s;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, m = blockIdx.x;
+  if (threadIdx.x < 32) {
+    const PackedRow row = packed_row(p.s, m, lane);
+    int place = row.seq < 0 ? -1 : page_row_of(p.s, row.seq, row.pos);
+    if (lane == 0) {
+      if (row.bad) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
+      else if (row.seq >= 0 && place < 0) atomicCAS(p.err, 0, (int)DERR_POSITION);
+      place_s = place;
+    }
+  }
+  __syncthreads();
+  const int place = place_s, parts = p.n_kv * (kRowDim / 8);
+  if (place < 0) return;
+  for (int i = threadIdx.x; i < 2 * parts; i += kAppendThreads) {
+    const bool key = i < parts;
+    const int part = key ? i : i - parts;
+    const uint8_t* row = (key ? p.k : p.v) + (size_t)place * p.row_bytes;
+    uint4 o;
+    if constexpr (Q4) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(row + 4 * part);
+      const float s = bf16_bits_to_float(*reinterpret_cast<const uint16_t*>(row + p.n_kv * kQ4HeadBytes + 2 * (part / 4)));
+      __nv_bfloat162* pk = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        pk[j] = __floats2bfloat162_rn((float)((int)(w >> (8 * j) & 15u) - 8) * s, (float)((int)(w >> (8 * j + 4) & 15u) - 8) * s);
+    } else {
+      o = *reinterpret_cast<const uint4*>(row + 16 * part);
+    }
+    *reinterpret_cast<uint4*>((key ? p.k_out : p.v_out) + ((size_t)m * parts + part) * 8) = o;
+  }
+}
+
+}  // namespace tq
+
+using namespace tq;
+
+extern "C" {
+
+size_t tq_q4_row_bytes(size_t n_kv_heads) { return q4_row_bytes(n_kv_heads); }
+
+int tq_kv_append_paged(tq_ctx* ctx, const void* x_dev, int x_dtype, size_t ldx, const float* cos_dev, const float* sin_dev, size_t n_positions,
+                       const tq_pages* pages, const int* seqs_dev, const int* seq_rows_dev, size_t batch, size_t rows, size_t n_heads, size_t n_kv_heads,
+                       size_t head_dim, void* q_out_dev, void* k_pages_dev, void* v_pages_dev, int page_rows_as) {
+  if (int st = bind(ctx)) return st;
+  if (batch == 0 || rows == 0) return TQ_OK;
+  if (int st = check_packed(ctx, "tq_kv_append_paged", pages, seqs_dev, seq_rows_dev, batch, rows, n_kv_heads, head_dim, page_rows_as)) return st;
+  TQ_REQUIRE(ctx, x_dev && cos_dev && sin_dev && q_out_dev && k_pages_dev && v_pages_dev, "tq_kv_append_paged: null pointer");
+  TQ_REQUIRE(ctx, x_dtype == TQ_F32 || x_dtype == TQ_BF16, "tq_kv_append_paged: rows are f32 or bf16");
+  TQ_REQUIRE(ctx, n_heads >= 1 && n_heads <= 65535, "tq_kv_append_paged: too many heads");
+  const size_t width = (n_heads + 2 * n_kv_heads) * kRowDim;
+  if (ldx == 0) ldx = width;
+  TQ_REQUIRE(ctx, ldx >= width && ldx * dtype_size(x_dtype) % 16 == 0, "tq_kv_append_paged: rows stand a multiple of 16 bytes apart and do not overlap");
+  TQ_REQUIRE(ctx, (((uintptr_t)x_dev | (uintptr_t)cos_dev | (uintptr_t)sin_dev | (uintptr_t)q_out_dev | (uintptr_t)k_pages_dev | (uintptr_t)v_pages_dev) & 15) == 0,
+             "tq_kv_append_paged: arrays must be 16-byte aligned");
+  TQ_REQUIRE(ctx, n_positions >= 1, "tq_kv_append_paged: tables of the rotation without positions");
+  AppendParams p;
+  p.s = packed_seqs(pages, seqs_dev, seq_rows_dev, batch, rows);
+  p.x = x_dev;
+  p.ldx = ldx;
+  p.cos_t = cos_dev;
+  p.sin_t = sin_dev;
+  p.n_positions = (int)(n_positions < 0x7fffffff ? n_positions : 0x7fffffff);
+  p.n_heads = (int)n_heads;
+  p.n_kv = (int)n_kv_heads;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out_dev);
+  p.k = static_cast<uint8_t*>(k_pages_dev);
+  p.v = static_cast<uint8_t*>(v_pages_dev);
+  const bool q4 = page_rows_as == TQ_PAGES_Q4;
+  p.row_bytes = q4 ? q4_row_bytes(n_kv_heads) : n_kv_heads * kRowDim * 2;
+  p.err = ctx->dev_err;
+  if (int st = pages_use(ctx, pages)) return st;
+  const unsigned parts = (unsigned)((width / 8 + kAppendThreads - 1) / kAppendThreads);
+  // Four rows a CTA once that leaves a CTA for every SM.
+  const bool four = rows * parts >= 4 * (size_t)ctx->sm_count;
+  const dim3 grid((unsigned)(four ? (rows + 3) / 4 : rows), parts), block(kAppendThreads);
+  auto go = [&](auto kern) { return launch_k(ctx, kern, grid, block, 0, p); };
+  if (x_dtype == TQ_F32) {
+    TQ_CUDA(ctx, q4 ? (four ? go(kv_append_kernel<float, 4, true>) : go(kv_append_kernel<float, 1, true>))
+                    : (four ? go(kv_append_kernel<float, 4, false>) : go(kv_append_kernel<float, 1, false>)));
+  } else {
+    using bf = __nv_bfloat16;
+    TQ_CUDA(ctx, q4 ? (four ? go(kv_append_kernel<bf, 4, true>) : go(kv_append_kernel<bf, 1, true>))
+                    : (four ? go(kv_append_kernel<bf, 4, false>) : go(kv_append_kernel<bf, 1, false>)));
+  }
+  return TQ_OK;
+}
+
+int tq_kv_read_paged(tq_ctx* ctx, const void* k_pages_dev, const void* v_pages_dev, int page_rows_as, const tq_pages* pages, const int* seqs_dev,
+                     const int* seq_rows_dev, size_t batch, size_t rows, size_t n_kv_heads, size_t head_dim, void* k_out_dev, void* v_out_dev) {
+  if (int st = bind(ctx)) return st;
+  if (batch == 0 || rows == 0) return TQ_OK;
+  if (int st = check_packed(ctx, "tq_kv_read_paged", pages, seqs_dev, seq_rows_dev, batch, rows, n_kv_heads, head_dim, page_rows_as)) return st;
+  TQ_REQUIRE(ctx, k_pages_dev && v_pages_dev && k_out_dev && v_out_dev, "tq_kv_read_paged: null pointer");
+  TQ_REQUIRE(ctx, (((uintptr_t)k_pages_dev | (uintptr_t)v_pages_dev | (uintptr_t)k_out_dev | (uintptr_t)v_out_dev) & 15) == 0,
+             "tq_kv_read_paged: arrays must be 16-byte aligned");
+  ReadParams p;
+  p.s = packed_seqs(pages, seqs_dev, seq_rows_dev, batch, rows);
+  p.k = static_cast<const uint8_t*>(k_pages_dev);
+  p.v = static_cast<const uint8_t*>(v_pages_dev);
+  const bool q4 = page_rows_as == TQ_PAGES_Q4;
+  p.row_bytes = q4 ? q4_row_bytes(n_kv_heads) : n_kv_heads * kRowDim * 2;
+  p.n_kv = (int)n_kv_heads;
+  p.k_out = static_cast<__nv_bfloat16*>(k_out_dev);
+  p.v_out = static_cast<__nv_bfloat16*>(v_out_dev);
+  p.err = ctx->dev_err;
+  if (int st = pages_use(ctx, pages)) return st;
+  TQ_CUDA(ctx, launch_k(ctx, q4 ? kv_read_kernel<true> : kv_read_kernel<false>, dim3((unsigned)rows), dim3(kAppendThreads), 0, p));
+  return TQ_OK;
+}
+
+}  // extern "C"

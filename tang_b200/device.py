@@ -389,6 +389,11 @@ def _check_types(call: str, dtype: int, **buffers) -> None:
             raise TangqError(_lib.TQ_EINVAL, f"{call}: {name} has elements of another type than the call takes")
 
 
+def q4_row_bytes(n_kv_heads: int) -> int:
+    """Bytes of a cache row of 4 bits (``tq_q4_row_bytes``): codes and scales of all KV heads of a position."""
+    return (n_kv_heads * 72 + 15) // 16 * 16
+
+
 def _opt_ptr(buf) -> C.c_void_p:
     return C.c_void_p(buf.ptr if buf is not None else 0)
 
@@ -498,6 +503,89 @@ def _add_ops(cls):
                                                 head_dim, max_len, C.c_void_p(out.ptr), out.dtype))
         return out
 
+    def _page_form(self, call: str, pool, n_kv_heads: int, k_pages: Buffer, v_pages: Buffer) -> int:
+        """What the pages' rows are, by the buffers' type: bf16, or bytes (rows of 4 bits)."""
+        form, row = (_lib.PAGES_BF16, n_kv_heads * 128) if k_pages.dtype == BF16 else (_lib.PAGES_Q4, q4_row_bytes(n_kv_heads))
+        _check_types(call, BF16 if form == _lib.PAGES_BF16 else _lib.U8, k_pages=k_pages, v_pages=v_pages)
+        if k_pages.n != pool.n_pages * pool.page_rows * row or v_pages.n != k_pages.n:
+            raise TangqError(_lib.TQ_EINVAL, f"{call}: the pages are not the pool's {pool.n_pages * pool.page_rows} rows of {row} elements")
+        return form
+
+    def _packed(self, call: str, batch: int, rows: int, seqs: Buffer | None, seq_rows: Buffer | None) -> None:
+        if (seqs is not None and seqs.n < batch) or (seq_rows is not None and seq_rows.n < batch + 1) or (seq_rows is None and rows != batch):
+            raise TangqError(_lib.TQ_EINVAL, f"{call}: {batch} sequences need as many numbers and one more start, or one row each without starts")
+        _check_types(call, _lib.I32, seqs=seqs, seq_rows=seq_rows)
+
+    def kv_append_paged(self, x: Buffer, cos: Buffer, sin: Buffer, pool, k_pages: Buffer, v_pages: Buffer, batch: int, rows: int, n_heads: int,
+                        n_kv_heads: int, head_dim: int, seqs: Buffer | None = None, seq_rows: Buffer | None = None, ldx: int = 0,
+                        q_out: Buffer | None = None) -> Buffer:
+        """``rope_forward`` of queries and keys and ``KVCache::append`` (crates/tang-train/examples/smollm.rs:84-95) for the new tokens of several
+        sequences, packed (``tq_kv_append_paged``): x [rows][n_heads + 2 n_kv_heads][head_dim] f32 or bf16; rows seq_rows[i] .. seq_rows[i+1]-1 (row i unless
+        given) are the last positions of sequence seqs[i] (i unless given) of the pool, for which ``PagePool.extend`` has made room.  The pages are bf16, or
+        bytes: rows of 4 bits (``q4_row_bytes``).  Returns the rotated queries, bf16."""
+        width = (n_heads + 2 * n_kv_heads) * head_dim
+        if x.n < ((rows - 1) * (ldx or width) + width if rows else 0) or 2 * cos.n < head_dim or cos.n != sin.n:
+            raise TangqError(_lib.TQ_EINVAL, "kv_append_paged: buffer sizes do not match the shapes")
+        form = self._page_form("kv_append_paged", pool, n_kv_heads, k_pages, v_pages)
+        self._packed("kv_append_paged", batch, rows, seqs, seq_rows)
+        _check_types("kv_append_paged", F32, cos=cos, sin=sin)
+        if q_out is None:
+            q_out = self.alloc(rows * n_heads * head_dim, BF16)
+        elif q_out.n < rows * n_heads * head_dim:
+            raise TangqError(_lib.TQ_EINVAL, "kv_append_paged: no room for the queries")
+        _check_types("kv_append_paged", BF16, q_out=q_out)
+        self._check(self._L.tq_kv_append_paged(self._ctx, x.ptr, x.dtype, ldx, cos.ptr, sin.ptr, 2 * cos.n // head_dim, pool.handle, _opt_ptr(seqs),
+                                               _opt_ptr(seq_rows), batch, rows, n_heads, n_kv_heads, head_dim, q_out.ptr, k_pages.ptr, v_pages.ptr, form))
+        return q_out
+
+    def kv_read_paged(self, k_pages: Buffer, v_pages: Buffer, pool, batch: int, rows: int, n_kv_heads: int, head_dim: int, seqs: Buffer | None = None,
+                      seq_rows: Buffer | None = None, k_out: Buffer | None = None, v_out: Buffer | None = None):
+        """Keys and values of packed rows (as in ``kv_append_paged``) as the pages hold them, bf16 [rows][n_kv_heads][head_dim] (``tq_kv_read_paged``)."""
+        form = self._page_form("kv_read_paged", pool, n_kv_heads, k_pages, v_pages)
+        self._packed("kv_read_paged", batch, rows, seqs, seq_rows)
+        n = rows * n_kv_heads * head_dim
+        k_out, v_out = (self.alloc(n, BF16) if b is None else b for b in (k_out, v_out))
+        if k_out.n < n or v_out.n < n:
+            raise TangqError(_lib.TQ_EINVAL, "kv_read_paged: no room for the rows")
+        _check_types("kv_read_paged", BF16, k_out=k_out, v_out=v_out)
+        self._check(self._L.tq_kv_read_paged(self._ctx, k_pages.ptr, v_pages.ptr, form, pool.handle, _opt_ptr(seqs), _opt_ptr(seq_rows), batch, rows, n_kv_heads,
+                                             head_dim, k_out.ptr, v_out.ptr))
+        return k_out, v_out
+
+    def gqa_prefill_paged(self, q: Buffer, k_pages: Buffer, v_pages: Buffer, pool, batch: int, rows: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                          max_len: int, seqs: Buffer | None = None, seq_rows: Buffer | None = None, out: Buffer | None = None) -> Buffer:
+        """``gqa_prefill`` over the pages of a ``PagePool`` for packed rows (as in ``kv_append_paged``, whose queries these are; ``tq_gqa_prefill_paged``):
+        a row attends its sequence up to its own position.  max_len bounds the lengths."""
+        form = self._page_form("gqa_prefill_paged", pool, n_kv_heads, k_pages, v_pages)
+        self._packed("gqa_prefill_paged", batch, rows, seqs, seq_rows)
+        if q.n < rows * n_heads * head_dim:
+            raise TangqError(_lib.TQ_EINVAL, "gqa_prefill_paged: buffer sizes do not match the shapes")
+        if out is None:
+            out = self.alloc(rows * n_heads * head_dim, BF16)
+        elif out.n < rows * n_heads * head_dim:
+            raise TangqError(_lib.TQ_EINVAL, "gqa_prefill_paged: no room for the results")
+        _check_types("gqa_prefill_paged", BF16, q=q, out=out)
+        self._check(self._L.tq_gqa_prefill_paged(self._ctx, q.ptr, k_pages.ptr, v_pages.ptr, form, pool.handle, _opt_ptr(seqs), _opt_ptr(seq_rows), batch, rows,
+                                                 n_heads, n_kv_heads, head_dim, max_len, out.ptr))
+        return out
+
+    def gqa_decode_paged_q4(self, q: Buffer, k_pages: Buffer, v_pages: Buffer, pool, batch: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int,
+                            seqs: Buffer | None = None, out: Buffer | None = None) -> Buffer:
+        """``gqa_decode_paged`` over pages of 4 bits (``tq_gqa_decode_paged_q4``); no groups, bf16 results."""
+        self._page_form("gqa_decode_paged_q4", pool, n_kv_heads, k_pages, v_pages)
+        self._packed("gqa_decode_paged_q4", batch, batch, seqs, None)
+        _check_types("gqa_decode_paged_q4", _lib.U8, k_pages=k_pages)
+        if q.n < batch * n_heads * head_dim:
+            raise TangqError(_lib.TQ_EINVAL, "gqa_decode_paged_q4: buffer sizes do not match the shapes")
+        if out is None:
+            out = self.alloc(batch * n_heads * head_dim, BF16)
+        elif out.n < batch * n_heads * head_dim:
+            raise TangqError(_lib.TQ_EINVAL, "gqa_decode_paged_q4: no room for the results")
+        _check_types("gqa_decode_paged_q4", BF16, q=q, out=out)
+        self._check(self._L.tq_gqa_decode_paged_q4(self._ctx, q.ptr, k_pages.ptr, v_pages.ptr, pool.handle, _opt_ptr(seqs), batch, n_heads, n_kv_heads, head_dim,
+                                                   max_len, out.ptr))
+        return out
+
     def concat_rows(self, parts) -> QBuffer:
         arr = (C.c_void_p * len(parts))(*[p.handle for p in parts])
         h = C.c_void_p()
@@ -515,7 +603,8 @@ def _add_ops(cls):
         return out
 
     for f in (rms_norm, rms_norm_residual, rope_tables, rope_forward, swiglu_fused, embedding, kv_attention, gqa_decode,
-              gqa_prefill, gqa_decode_paged, concat_rows, interleave_gate_up):
+              gqa_prefill, gqa_decode_paged, _page_form, _packed, kv_append_paged, kv_read_paged, gqa_prefill_paged, gqa_decode_paged_q4, concat_rows,
+              interleave_gate_up):
         setattr(cls, f.__name__, f)
 
 
