@@ -1,19 +1,40 @@
 // Causal attention of several sequences' new positions, packed, over their pages (include/tangq.h: tq_gqa_prefill_paged).
+//
+// A CTA takes two tiles of 128 rows (128 / group positions x the group's heads of one KV head) of a sequence over the same tiles of 128 keys:
+//   warp 0        queries, then tiles of keys: tensor copies page by page, or, for pages of 4 bits, codes that it turns into the same bf16 rows
+//   warps 1, 2    issue a row tile's products: S = Q K^T (both from shared memory), then O += P V (P from tensor memory, V N-major)
+//   warp 3        tiles of values, likewise; rows behind the last key are zeros (whatever a page holds there must not meet a weight of zero)
+//   warps 4..7, 8..11   softmax of a row tile, a thread a row
+// Tensor memory: S / P and O of both tiles, 4 x 128 columns.  A row's scores are read once, into registers; its weights go over their columns in two halves, the
+// first of which is multiplied while the second is computed.  A weight is one bf16 number, and the sum that results are divided by is that of the numbers as they
+// entered: a row of a few keys, where the roundings do not average out, is then nearer (the largest weight need not be 1 for that, so that the reference
+// may lag: a row's sums are rescaled only when its maximum grew by more than 2^8).
+// Few rows: a tile pair's keys are cut into parts, a CTA each, and a second kernel joins the results.
 #include <cfloat>
 
 #include "attn_mma.cuh"
+#include "attn_umma.cuh"
 #include "page_rows.cuh"
 
 namespace tq {
+
+constexpr int kPpThreads = 384;
+constexpr int kPpSlots = 2;                           // of keys, and of values: a tile each
+constexpr int kPpTile = 2 * kPfBox;                   // bytes: two boxes of 64 columns
+constexpr size_t kPpSmem = 1024 + 1024 + 4 * (size_t)kPfBox + 2 * kPpSlots * (size_t)kPpTile;
+constexpr float kPpLag = 8.f;                         // a reference may be so far below its row's maximum (log2)
+constexpr int kPpMaxParts = 16;
 
 struct PackedPrefillParams {
   PackedSeqs s;
   const __nv_bfloat16* q;
   const uint8_t *k, *v;
   size_t row_bytes;
-  int n_heads, n_kv, max_len;
+  int n_heads, n_kv, group, max_len;
+  int per_tile, parts;                 // positions of a row tile; parts of a tile pair's keys
   float scale_log2;
   __nv_bfloat16* out;
+  float *part_o, *part_ml;             // [part][rows][n_heads][128], [..][2] (reference and sum) where there are several
   int* err;
 };
 
@@ -34,42 +55,550 @@ __device__ __forceinline__ void row_values(const uint8_t* row, int n_kv, int hea
   }
 }
 
-// A warp takes a row's head, key by key.
+// One row's softmax attention over keys first .. end - 1 by a warp, key by key, for the rows of a tile that met, with a weight of zero, a value of a key that
+// they do not see and that is no number: zero times that is NaN.  Lane i has values 4 i .. of the query and of the sums.
 template <bool Q4>
-__global__ void __launch_bounds__(128) paged_prefill_rows_kernel(const PackedPrefillParams p) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, m = blockIdx.x, h = 4 * blockIdx.y + (threadIdx.x >> 5);
-  if (h >= p.n_heads) return;
-  const PackedRow row = packed_row(p.s, m, lane);
-  if (row.bad && lane == 0 && h == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
-  if (row.seq < 0) return;
-  const size_t at = ((size_t)m * p.n_heads + h) * kRowDim + 4 * lane;
-  const int kv = h / (p.n_heads / p.n_kv), end = min(row.pos + 1, p.max_len);
-  float q[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, top = -FLT_MAX, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = __bfloat162float(p.q[at + i]);
-  for (int j = 0; j < end; ++j) {
-    int place = page_row_of(p.s, row.seq, j);
-    if (place < 0) {
-      if (lane == 0) atomicCAS(p.err, 0, (int)DERR_POSITION);
-      return;
-    }
+__device__ __forceinline__ void attend_paged_row(const PackedPrefillParams& p, int seq, int kv, int first, int end, const float (&q)[4], int lane, float& top, float& l,
+                                              float (&acc)[4]) {
+#pragma unroll 1
+  for (int j = first; j < end; ++j) {
+    const int place = max(page_row_of(p.s, seq, j), 0);
     float k[4], v[4], s = 0.f;
     row_values<Q4>(p.k + (size_t)place * p.row_bytes, p.n_kv, kv, lane, k);
     row_values<Q4>(p.v + (size_t)place * p.row_bytes, p.n_kv, kv, lane, v);
 #pragma unroll
     for (int i = 0; i < 4; ++i) s = fmaf(q[i], k[i], s);
     s = warp_sum(s) * p.scale_log2;
-    const float mn = fmaxf(top, s), f = ex2_ftz(top - mn), w = ex2_ftz(s - mn);
+    const float mn = fmaxf(top, s), f = ex2(top - mn), w = ex2(s - mn);
     top = mn;
     l = l * f + w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = fmaf(w, v[i], acc[i] * f);
   }
-  const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+}
+
+// What a CTA does.
+struct PpItem {
+  int seq, kv;                         // of the pool (-1: nothing), KV head
+  int row0, rows;                      // first packed row, rows of both tiles
+  int pos0;                            // position of the first row
+  int tile0, tiles;                    // tiles of keys: the part's first, how many
+  int k_end;                           // keys that the last row sees, or the bound
+};
+// Tile pair x of all sequences, the longest of each sequence first, by one warp.
+__device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, int kv, int part, int lane) {
+  PpItem it{-1, kv, 0, 0, 0, 0, 0, 0};
+  const int per_pair = 2 * p.per_tile;
+  int i = -1, first = 0, count = 0, pair = 0;
+  if (!p.s.seq_rows) {
+    if (x < p.s.batch) i = x, first = x, count = 1;
+  } else {
+    int before = 0;
+    bool bad = false;
+    for (int base = 0; base < p.s.batch; base += 32) {
+      const int j = base + lane;
+      int f = 0, c = 0;
+      if (j < p.s.batch) {
+        const int a = p.s.seq_rows[j], b = p.s.seq_rows[j + 1];
+        if (a < 0 || b < a || b > p.s.rows || (j == 0 && a != 0)) bad = true;
+        else f = a, c = b - a;
+      }
+      const int pairs = (c + per_pair - 1) / per_pair;
+      int incl = pairs;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p.out[at + i] = __float2bfloat16_rn(acc[i] * inv);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int w = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += w;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, x >= before + incl - pairs && x < before + incl);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        i = base + src;
+        first = __shfl_sync(0xffffffffu, f, src);
+        count = __shfl_sync(0xffffffffu, c, src);
+        pair = __shfl_sync(0xffffffffu, before + incl, src) - 1 - x;   // (the last pair first)
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+      if (i >= 0) break;
+    }
+    if (bad && lane == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
+  }
+  if (i < 0) return it;
+  const int s = packed_seq(p.s, i), len = s < 0 ? 0 : p.s.lens[s];
+  if (s < 0 || len < count || len > (long long)p.s.table_ld << p.s.page_shift) {
+    if (lane == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
+    return it;
+  }
+  it.seq = s;
+  it.row0 = first + pair * per_pair;
+  it.rows = min(per_pair, count - pair * per_pair);
+  it.pos0 = len - count + pair * per_pair;
+  it.k_end = min(it.pos0 + it.rows, p.max_len);
+  const int all = (it.k_end + kPfTile - 1) / kPfTile, per = max((all + p.parts - 1) / p.parts, 2);
+  it.tile0 = min(part * per, all);
+  it.tiles = min(per, all - it.tile0);
+  return it;
+}
+
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 32 columns of the warp's lanes; nothing may touch v before pp_landed.
+__device__ __forceinline__ void pp_ask(uint32_t taddr, float (&v)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+                 "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+                 "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+                 "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void pp_landed(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]),
+                 "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]),
+                 "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
+                 "+f"(v[31])::"memory");
+}
+
+// Pages of 4 bits: a loader's tiles.  A lane takes key lane + 32 u of a tile, u = 0 .. 3: its codes are asked for a turn ahead, its page two.
+struct PpCodes {
+  uint4 w[4];
+  uint2 s;
+};
+__device__ __forceinline__ void pp_convert(uint8_t* tile, int key, const PpCodes& x) {
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {        // a scale's 32 values
+    const uint32_t half = b < 2 ? x.s.x : x.s.y, sc = prmt(half, half, b & 1 ? 0x3232 : 0x1010), off = bf16x2_mul(sc, 0xC1C0C1C0u);      // -24 s
+    const uint32_t w[4] = {x.w[b].x, x.w[b].y, x.w[b].z, x.w[b].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t a[4];
+      dequant_q4_word_24(w[i], a);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a[j] = bf16x2_fma(a[j], sc, off);
+      const int c = 4 * (b & 1) + i;   // 16-byte chunk of the row's half
+      *reinterpret_cast<uint4*>(tile + (b >> 1) * kPfBox + key * 128 + ((c ^ (key & 7)) << 4)) =
+          make_uint4(prmt(a[0], a[1], 0x5410), prmt(a[2], a[3], 0x5410), prmt(a[0], a[1], 0x7632), prmt(a[2], a[3], 0x7632));
+    }
+  }
+}
+
+template <bool Q4>
+__global__ void __launch_bounds__(kPpThreads, 1)
+paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                     const __grid_constant__ PackedPrefillParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem_raw);
+  uint64_t* k_full = q_full + 1;                      // [slots]
+  uint64_t* k_empty = k_full + kPpSlots;              // [slots] both row tiles' products done
+  uint64_t* v_full = k_empty + kPpSlots;
+  uint64_t* v_empty = v_full + kPpSlots;
+  uint64_t* v_raw = v_empty + kPpSlots;               // the last tile's values, before the rows behind the last key are zeroed
+  uint64_t* s_full = v_raw + 1;                       // [row tile]
+  uint64_t* p_half = s_full + 2;
+  uint64_t* p_full = p_half + 2;
+  uint64_t* o_done = p_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+  volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  PpItem* item_s = reinterpret_cast<PpItem*>(smem_raw + 512);
+  uint8_t* q_s = smem_raw + 1024 + ((1024 - ((smem_u32(smem_raw) + 1024) & 1023)) & 1023);
+  uint8_t *k_s = q_s + 4 * kPfBox, *v_s = k_s + kPpSlots * kPpTile;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_init(q_full, 1);
+      for (int s = 0; s < kPpSlots; ++s) {
+        mbar_init(&k_full[s], 1);
+        mbar_init(&k_empty[s], 2);
+        mbar_init(&v_full[s], 1);
+        mbar_init(&v_empty[s], 2);
+      }
+      mbar_init(v_raw, 1);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&s_full[x], 1);
+        mbar_init(&p_half[x], 4);
+        mbar_init(&p_full[x], 4);
+        mbar_init(&o_done[x], 1);
+      }
+      *failed = 0;
+      mbar_init_fence();
+    }
+  } else if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+  } else if (warp == 2 && lane == 0) {
+    prefetch_map(&q_map);
+    if (!Q4) {
+      prefetch_map(&k_map);
+      prefetch_map(&v_map);
+    }
+  }
+  tc_fence_before();
+  pdl_wait();
+  pdl_launch_dependents();
+  if (warp == 3) {
+    const PpItem it = pp_item(p, blockIdx.y, blockIdx.x, blockIdx.z, lane);
+    if (lane == 0) *item_s = it;
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const PpItem it = *item_s;
+  auto give_up = [&](int code) {
+    atomicCAS(p.err, 0, code);
+    *failed = 1;
+  };
+  const int n = it.seq < 0 ? 0 : it.tiles;
+  // tiles of keys that a row tile needs
+  const int need[2] = {max(0, min(n, (min(it.pos0 + min(it.rows, p.per_tile), p.max_len) + kPfTile - 1) / kPfTile - it.tile0)), it.rows > p.per_tile ? n : 0};
+
+  // (registers: 384 threads of 168 at the start, then 128 of 88 or 104 and 256 of 208 or 200, the same in all)
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q4 ? 104 : 88));
+  if (warp == 0 || warp == 3) {
+    // ---- tiles of keys (and the queries), tiles of values
+    const bool values = warp == 3;
+    uint64_t *full = values ? v_full : k_full, *empty = values ? v_empty : k_empty;
+    uint8_t* to = values ? v_s : k_s;
+    bool ok = true;
+    if (!values && n > 0) {
+      if (lane == 0) mbar_arrive_expect_tx(q_full, 4u * p.per_tile * p.group * 128u);
+      __syncwarp();
+      if (lane < 4)
+        tma_load_3d(q_s + lane * kPfBox, &q_map, 64 * (lane & 1), it.kv * p.group, it.row0 + (lane >> 1) * p.per_tile, q_full);
+      __syncwarp();
+    }
+    const int* table = p.s.tables + (size_t)max(it.seq, 0) * p.s.table_ld;
+    if constexpr (Q4) {
+      const uint8_t* from = (values ? p.v : p.k) + it.kv * kQ4HeadBytes;
+      const int steps = 4 * n, key0 = it.tile0 * kPfTile + lane, scales = p.n_kv * kQ4HeadBytes - it.kv * kQ4HeadBytes + it.kv * 2 * kQ4HeadScales;
+      auto page_at = [&](int m) {      // of key `lane` of step m
+        const int key = key0 + 32 * m;
+        return m < steps && key < it.k_end ? table[key >> p.s.page_shift] : 0;
+      };
+      auto codes_at = [&](int m, int page) {
+        PpCodes x;
+        const int key = key0 + 32 * m;
+        if (m < steps && key < it.k_end) {
+          if (page < 0 || page >= p.s.n_pages) {
+            atomicCAS(p.err, 0, (int)DERR_POSITION);
+            page = 0;
+          }
+          const uint8_t* row = from + ((size_t)(page << p.s.page_shift) + (key & ((1 << p.s.page_shift) - 1))) * p.row_bytes;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x.w[i] = *reinterpret_cast<const uint4*>(row + 16 * i);
+          x.s = *reinterpret_cast<const uint2*>(row + scales);
+        } else {                       // rows of zeros
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x.w[i] = make_uint4(0u, 0u, 0u, 0u);
+          x.s = make_uint2(0u, 0u);
+        }
+        return x;
+      };
+      PpCodes next = codes_at(0, page_at(0));
+      int page = page_at(1);
+      for (int i = 0; i < n && ok; ++i) {
+        const int slot = i % kPpSlots;
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)((i / kPpSlots) & 1) ^ 1u));
+        if (!ok) break;
+#pragma unroll 1
+        for (int u = 0; u < 4; ++u) {
+          const PpCodes x = next;
+          next = codes_at(4 * i + u + 1, page);
+          page = page_at(4 * i + u + 2);
+          pp_convert(to + slot * kPpTile, 32 * u + lane, x);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[slot]);
+        __syncwarp();
+      }
+    } else {
+      // a lane per box: a page's rows, half their columns
+      const int box_rows = min(1 << p.s.page_shift, kPfTile), boxes = kPfTile / box_rows, j = lane >> 1, c = lane & 1;
+      auto page_at = [&](int i) {
+        const int key = (it.tile0 + i) * kPfTile + j * box_rows;
+        return i < n && j < boxes && key < it.k_end ? table[key >> p.s.page_shift] : 0;
+      };
+      int next = page_at(0);
+      for (int i = 0; i < n && ok; ++i) {
+        int page = next;
+        next = page_at(i + 1);
+        const int slot = i % kPpSlots, key = (it.tile0 + i) * kPfTile, keys = min(kPfTile, it.k_end - key), used = (keys + box_rows - 1) / box_rows;
+        if (page < 0 || page >= p.s.n_pages) {
+          atomicCAS(p.err, 0, (int)DERR_POSITION);
+          page = 0;
+        }
+        const int row = (page << p.s.page_shift) + (key & ((1 << p.s.page_shift) - 1) & ~(box_rows - 1));
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)((i / kPpSlots) & 1) ^ 1u));
+        if (!ok) break;
+        const bool cut = values && keys < kPfTile;
+        uint64_t* bar = cut ? v_raw : &full[slot];
+        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(used * box_rows) * 256u);
+        __syncwarp();
+        if (j < used) tma_load_2d(to + slot * kPpTile + c * kPfBox + j * box_rows * 128, values ? &v_map : &k_map, it.kv * kRowDim + 64 * c, row, bar);
+        __syncwarp();
+        if (cut) {                     // (the last tile)
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(v_raw, 0));
+          if (!ok) break;
+          uint8_t* at = to + slot * kPpTile;
+          for (int k = lane; k < 2 * (kPfTile - keys) * 8; k += 32)    // (a row's 128 bytes of either box, whatever their order)
+            *reinterpret_cast<uint4*>(at + ((k >> 3) & 1) * kPfBox + (keys + (k >> 4)) * 128 + 16 * (k & 7)) = make_uint4(0u, 0u, 0u, 0u);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[slot]);
+          __syncwarp();
+        }
+      }
+    }
+    if (!ok && lane == 0) give_up(DERR_EMPTY_WAIT);
+  } else {
+    // ---- products
+    const bool leader = elect_one();
+    const int x = warp - 1, mine = need[x];
+    const uint32_t idesc_s = umma_idesc_bf16(kPfTile), idesc_o = idesc_s | (1u << 16);   // (bit 16: B is N-major)
+    const uint64_t qd = umma_desc_sw128(q_s + 2 * x * kPfBox), kd = umma_desc_sw128(k_s), vd = pf_desc_mn(v_s);
+    const uint32_t s_t = tmem + (uint32_t)(x * 256), o_t = s_t + 128u;
+    bool ok = n == 0 || __all_sync(0xffffffffu, mbar_wait_spin(q_full, 0));
+    for (int i = 0; i < n && ok; ++i) {
+      const int slot = i % kPpSlots;
+      const uint32_t ph = (uint32_t)((i / kPpSlots) & 1);
+      const uint64_t slot_off = (uint64_t)(slot * (kPpTile >> 4));
+      // (the scores' columns hold the weights of the tile before until its products are done)
+      ok = __all_sync(0xffffffffu, mbar_wait_spin(&k_full[slot], ph) && (i == 0 || i >= mine || mbar_wait_spin(&o_done[x], (uint32_t)((i - 1) & 1))));
+      if (!ok) break;
+      tc_fence_after();
+      if (leader) {
+        if (i < mine) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint64_t off = (uint64_t)((k >> 2) * (kPfBox >> 4) + 2 * (k & 3));
+            umma_f16(s_t, qd + off, kd + slot_off + off, idesc_s, k != 0);
+          }
+          umma_commit(&s_full[x]);
+          umma_commit(&k_empty[slot]);
+        } else {
+          mbar_arrive(&k_empty[slot]);
+        }
+      }
+      __syncwarp();
+      ok = __all_sync(0xffffffffu, mbar_wait_spin(&v_full[slot], ph) && (i >= mine || mbar_wait_spin(&p_half[x], (uint32_t)(i & 1))));
+      if (!ok) break;
+      if (i >= mine) {
+        if (leader) mbar_arrive(&v_empty[slot]);
+        __syncwarp();
+        continue;
+      }
+      tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_f16_ts(o_t, s_t + 8u * k, vd + slot_off + (uint64_t)(k * (2048 >> 4)), idesc_o, (i | k) != 0);
+      }
+      __syncwarp();
+      ok = __all_sync(0xffffffffu, mbar_wait_spin(&p_full[x], (uint32_t)(i & 1)));
+      if (!ok) break;
+      tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int k = 4; k < 8; ++k) umma_f16_ts(o_t, s_t + 8u * k, vd + slot_off + (uint64_t)(k * (2048 >> 4)), idesc_o, 1u);
+        umma_commit(&o_done[x]);
+        umma_commit(&v_empty[slot]);
+      }
+      __syncwarp();
+    }
+    if (!ok && lane == 0) give_up(DERR_FULL_WAIT);
+  }
+  } else {
+    // ---- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q4 ? 200 : 208));
+    const int x = (warp - 4) >> 2, q4 = warp & 3, r = 32 * q4 + lane, mine = need[x];
+    const int at_row = x * p.per_tile + r / p.group, head = it.kv * p.group + r % p.group;       // of the item's rows
+    const bool live = r < p.per_tile * p.group && at_row < it.rows && it.seq >= 0;
+    const int limit = live ? min(it.pos0 + at_row, p.max_len - 1) : -1;                          // the last key of this row
+    const uint32_t s_t = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)(x * 256), o_t = s_t + 128u;
+    const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
+    float m = -FLT_MAX, l = 0.f;
+    bool ok = true;
+#pragma unroll 1
+    for (int i = 0; i < mine && ok; ++i) {
+      ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[x], (uint32_t)(i & 1)));
+      if (!ok) break;
+      tc_fence_after();
+      __syncwarp();
+      float v[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) pp_ask(s_t + 32u * c, v[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) pp_landed(v[c]);
+      const int last = limit - (it.tile0 + i) * kPfTile;               // keys 0 .. last of the tile count
+      if (!__all_sync(0xffffffffu, last >= kPfTile - 1)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[c][j] = 32 * c + j <= last ? v[c][j] : -INFINITY;
+      }
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = fmaxf(v[c][0], v[c][1]);
+#pragma unroll
+        for (int j = 2; j < 32; j += 2) mx[c] = fmaxf(mx[c], fmaxf(v[c][j], v[c][j + 1]));
+      }
+      const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2, -FLT_MAX);
+      if (i == 0) {
+        m = top;
+      } else if (__any_sync(0xffffffffu, top > m + kPpLag)) {          // (the products so far are done, or these scores would not be here)
+        const float m_new = top > m + kPpLag ? top : m, f = ex2(m - m_new);
+#pragma unroll 1
+        for (int c = 0; c < kRowDim; c += 16) {
+          float o[16];
+          uint32_t w[16];
+          tmem_ld16(o_t + (uint32_t)c, o);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[j] * f);
+          tmem_st16(o_t + (uint32_t)c, w);
+        }
+        l *= f;
+        m = m_new;
+      }
+      const uint64_t less = pack2(-m, -m);
+      uint64_t sum[2] = {0, 0};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float a, b;
+          unpack2(fma2(pack2(v[c][2 * j], v[c][2 * j + 1]), scale2, less), a, b);
+          w[j] = pack_bf16(ex2(a), ex2(b));
+          sum[j & 1] = add2(sum[j & 1], pack2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u)));
+        }
+        tmem_st16(s_t + 16u * c, w);                  // over scores that this thread has read
+        if (c & 1) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(c == 1 ? &p_half[x] : &p_full[x]);
+          __syncwarp();
+        }
+      }
+      float a, b;
+      unpack2(add2(sum[0], sum[1]), a, b);
+      l += a + b;
+    }
+    if (ok && mine) ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[x], (uint32_t)((mine - 1) & 1)));
+    if (!ok && lane == 0) give_up(DERR_TMEM);
+    tc_fence_after();
+    __syncwarp();
+    const bool parts = p.parts > 1;
+    const size_t at = ((size_t)(live ? it.row0 + at_row : 0) * p.n_heads + head) * kRowDim;
+    const size_t part_at = (size_t)blockIdx.z * p.s.rows * p.n_heads * kRowDim;
+    if (parts && live && ok) *reinterpret_cast<float2*>(p.part_ml + (part_at + at) / (kRowDim / 2)) = make_float2(m, l);
+    if (ok && mine) {
+      const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+      float zero = 0.f;                               // NaN if some sum is not finite
+#pragma unroll 1
+      for (int c = 0; c < kRowDim; c += 32) {
+        float o[32];
+        __syncwarp();
+        pp_ask(o_t + (uint32_t)c, o);
+        pp_landed(o);
+        if (!live) continue;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) zero = fmaf(o[j], 0.f, zero);
+        if (parts) {
+          float4* y = reinterpret_cast<float4*>(p.part_o + part_at + at + c);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        } else {
+          uint4* y = reinterpret_cast<uint4*>(p.out + at + c);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            y[j] = make_uint4(pack_bf16(o[8 * j] * inv, o[8 * j + 1] * inv), pack_bf16(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
+                              pack_bf16(o[8 * j + 4] * inv, o[8 * j + 5] * inv), pack_bf16(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
+        }
+      }
+      unsigned rows = __ballot_sync(0xffffffffu, live && zero != zero);
+      if (rows) {
+        // Keys that rows of this CTA do not see and their tiles hold: from its first position on.
+        const int first = it.tile0 * kPfTile, end = min((it.tile0 + n) * kPfTile, it.k_end);
+        float z = 0.f;
+        for (int key = max(it.pos0 + 1, first); key < end; ++key) {
+          float v[4];
+          row_values<Q4>(p.v + (size_t)max(page_row_of(p.s, it.seq, key), 0) * p.row_bytes, p.n_kv, it.kv, lane, v);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) z = fmaf(v[i], 0.f, z);
+        }
+        if (!__any_sync(0xffffffffu, z != z)) rows = 0u;
+        while (rows) {
+          const int src = __ffs(rows) - 1;
+          rows &= rows - 1;
+          const int row_limit = __shfl_sync(0xffffffffu, limit, src);
+          const size_t row_at = __shfl_sync(0xffffffffu, (unsigned long long)at, src);
+          float qr[4], rm = -FLT_MAX, rl = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) qr[i] = __bfloat162float(p.q[row_at + 4 * lane + i]);
+          attend_paged_row<Q4>(p, it.seq, it.kv, first, min(end, row_limit + 1), qr, lane, rm, rl, acc);
+          if (parts) {
+            *reinterpret_cast<float4*>(p.part_o + part_at + row_at + 4 * lane) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + (part_at + row_at) / (kRowDim / 2)) = make_float2(rm, rl);
+          } else {
+            const float rinv = rl > 0.f || rl != rl ? 1.0f / rl : 0.f;
+            *reinterpret_cast<uint2*>(p.out + row_at + 4 * lane) = make_uint2(pack_bf16(acc[0] * rinv, acc[1] * rinv), pack_bf16(acc[2] * rinv, acc[3] * rinv));
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*failed && threadIdx.x == 0) {
+    // copies and products that are still in flight target this CTA's memories: give them time to land before leaving
+    for (int i = 0; i < 10000; ++i) __nanosleep(1000);
+  }
+  __syncthreads();
+  __syncwarp();                        // (the release is one instruction of the whole warp)
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of a row's head, in their order: a warp, four columns a lane.
+__global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PackedPrefillParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const size_t i = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5), heads = (size_t)p.s.rows * p.n_heads;      // the row's head
+  if (i >= heads) return;
+  // rows that nobody attended for are left as they are
+  const int m = (int)(i / p.n_heads);
+  if (packed_row(p.s, m, lane).seq < 0) return;
+  const float2 ml = lane < p.parts ? *reinterpret_cast<const float2*>(p.part_ml + (lane * heads + i) * 2) : make_float2(-FLT_MAX, 0.f);
+  const float top = warp_max(ml.x), w = ex2(ml.x - top), l = warp_sum(ml.y * w);
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < p.parts; ++k) {
+    const float f = __shfl_sync(0xffffffffu, w, k), has = __shfl_sync(0xffffffffu, ml.y, k);
+    if (has == 0.f) continue;          // (a part without keys of this row has left nothing)
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + ((size_t)k * heads + i) * kRowDim + 4 * lane);
+    o[0] = fmaf(v.x, f, o[0]);
+    o[1] = fmaf(v.y, f, o[1]);
+    o[2] = fmaf(v.z, f, o[2]);
+    o[3] = fmaf(v.w, f, o[3]);
+  }
+  const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+  *reinterpret_cast<uint2*>(p.out + i * kRowDim + 4 * lane) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
 }
 
 }  // namespace tq
@@ -100,8 +629,37 @@ extern "C" int tq_gqa_prefill_paged(tq_ctx* ctx, const void* q_dev, const void* 
   p.scale_log2 = 1.44269504088896340736f / sqrtf((float)head_dim);
   p.out = static_cast<__nv_bfloat16*>(out_dev);
   p.err = ctx->dev_err;
+  p.group = (int)(n_heads / n_kv_heads);
+  p.per_tile = kPfTile / p.group;
+  // Tile pairs there may be; parts of their keys where these leave SMs idle, of four tiles or more.
+  const size_t per_pair = 2 * (size_t)p.per_tile, pairs = seq_rows_dev ? rows / per_pair + (batch < rows ? batch : rows) : rows;
+  const size_t most = (size_t)pages->table_ld * pages->page_rows, longest = max_len < most ? max_len : most, ctas = pairs * n_kv_heads;
+  TQ_REQUIRE(ctx, pairs <= 65535, "tq_gqa_prefill_paged: too many rows");
+  size_t parts = 1;
+  if (ctas < (size_t)ctx->sm_count) {
+    parts = (2 * (size_t)ctx->sm_count + ctas - 1) / ctas;
+    const size_t tiles = (longest + kPfTile - 1) / kPfTile, few = tiles / 4;
+    parts = parts > few ? few : parts;
+    parts = parts < 1 ? 1 : parts > (size_t)kPpMaxParts ? (size_t)kPpMaxParts : parts;
+  }
+  p.parts = (int)parts;
+  p.part_o = p.part_ml = nullptr;
+  if (parts > 1) {
+    const size_t heads = parts * rows * n_heads;
+    if (int st = ensure_scratch(ctx, heads * (kRowDim + 2) * sizeof(float))) return st;
+    p.part_o = static_cast<float*>(ctx->scratch);
+    p.part_ml = p.part_o + heads * kRowDim;
+  }
+  CUtensorMap qm, km = {}, vm = {};
+  const size_t row = n_kv_heads * kRowDim, cache_rows = (size_t)pages->n_pages * pages->page_rows;
+  const unsigned box = pages->page_rows < kPfTile ? (unsigned)pages->page_rows : (unsigned)kPfTile;
+  if (!encode_bf16_boxes(&qm, q_dev, kRowDim, n_heads, rows, kRowDim * 2, n_heads * kRowDim * 2, (unsigned)p.group, (unsigned)p.per_tile) ||
+      (!q4 && (!encode_bf16_k64(&km, k_pages_dev, cache_rows, row, row, box) || !encode_bf16_k64(&vm, v_pages_dev, cache_rows, row, row, box))))
+    return fail(ctx, TQ_ECUDA, "cuTensorMapEncodeTiled failed");
   if (int st = pages_use(ctx, pages)) return st;
-  TQ_CUDA(ctx, launch_k(ctx, q4 ? paged_prefill_rows_kernel<true> : paged_prefill_rows_kernel<false>, dim3((unsigned)rows, (unsigned)((n_heads + 3) / 4)),
-                        dim3(128), 0, p));
+  auto kern = q4 ? paged_prefill_kernel<true> : paged_prefill_kernel<false>;
+  TQ_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPpSmem));
+  TQ_CUDA(ctx, launch_k(ctx, kern, dim3((unsigned)n_kv_heads, (unsigned)pairs, (unsigned)parts), dim3(kPpThreads), kPpSmem, qm, km, vm, p));
+  if (parts > 1) TQ_CUDA(ctx, launch_k(ctx, paged_prefill_join_kernel, dim3((unsigned)((rows * n_heads + 3) / 4)), dim3(128), 0, p));
   return TQ_OK;
 }
