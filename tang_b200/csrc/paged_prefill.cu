@@ -5,7 +5,7 @@
 //   warps 1, 2    issue a row tile's products: S = Q K^T (both from shared memory), then O += P V (P from tensor memory, V N-major)
 //   warp 3        tiles of values, likewise; rows behind the last key are zeros (whatever a page holds there must not meet a weight of zero)
 //   warps 4..7, 8..11   softmax of a row tile, a thread a row
-// Tensor memory: S / P and O of both tiles, 4 x 128 columns.  A row's scores are read once, into registers; its weights go over their columns in two halves, the
+// Tensor memory: S / P and O of both tiles, 4 x 128 columns.  A row's scores are read once, into registers; its weights go over their columns, block by
 // first of which is multiplied while the second is computed.  A weight is one bf16 number, and the sum that results are divided by is that of the numbers as they
 // entered: a row of a few keys, where the roundings do not average out, is then nearer (the largest weight need not be 1 for that, so that the reference
 // may lag: a row's sums are rescaled only when its maximum grew by more than 2^8).
@@ -21,9 +21,11 @@ namespace tq {
 constexpr int kPpThreads = 384;
 constexpr int kPpSlots = 2;                           // of keys, and of values: a tile each
 constexpr int kPpTile = 2 * kPfBox;                   // bytes: two boxes of 64 columns
+constexpr int kPpBlock = 64;                          // keys whose scores are computed, and become weights, at a time
 constexpr size_t kPpSmem = 1024 + 1024 + 4 * (size_t)kPfBox + 2 * kPpSlots * (size_t)kPpTile;
 constexpr float kPpLag = 8.f;                         // a reference may be so far below its row's maximum (log2)
 constexpr int kPpMaxParts = 16;
+constexpr int kPpPoly = 4;                            // one of so many pairs of weights is a polynomial
 
 struct PackedPrefillParams {
   PackedSeqs s;
@@ -89,17 +91,23 @@ struct PpItem {
 __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, int kv, int part, int lane) {
   PpItem it{-1, kv, 0, 0, 0, 0, 0, 0};
   const int per_pair = 2 * p.per_tile;
-  int i = -1, first = 0, count = 0, pair = 0;
+  int i = -1, first = 0, count = 0, pair = 0, s = -1, len = 0;
   if (!p.s.seq_rows) {
-    if (x < p.s.batch) i = x, first = x, count = 1;
+    if (x < p.s.batch) {
+      i = x, first = x, count = 1;
+      s = packed_seq(p.s, i);
+      len = s < 0 ? 0 : p.s.lens[s];
+    }
   } else {
     int before = 0;
     bool bad = false;
     for (int base = 0; base < p.s.batch; base += 32) {
       const int j = base + lane;
-      int f = 0, c = 0;
+      int f = 0, c = 0, js = -1, jl = 0;
       if (j < p.s.batch) {
         const int a = p.s.seq_rows[j], b = p.s.seq_rows[j + 1];
+        js = packed_seq(p.s, j);       // (on their way beside the starts)
+        jl = js < 0 ? 0 : p.s.lens[js];
         if (a < 0 || b < a || b > p.s.rows || (j == 0 && a != 0)) bad = true;
         else f = a, c = b - a;
       }
@@ -116,6 +124,8 @@ __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, i
         i = base + src;
         first = __shfl_sync(0xffffffffu, f, src);
         count = __shfl_sync(0xffffffffu, c, src);
+        s = __shfl_sync(0xffffffffu, js, src);
+        len = __shfl_sync(0xffffffffu, jl, src);
         pair = __shfl_sync(0xffffffffu, before + incl, src) - 1 - x;   // (the last pair first)
       }
       before += __shfl_sync(0xffffffffu, incl, 31);
@@ -124,7 +134,6 @@ __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, i
     if (bad && lane == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
   }
   if (i < 0) return it;
-  const int s = packed_seq(p.s, i), len = s < 0 ? 0 : p.s.lens[s];
   if (s < 0 || len < count || len > (long long)p.s.table_ld << p.s.page_shift) {
     if (lane == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
     return it;
@@ -155,6 +164,30 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+// Adds a pair of bf16 to f32 sums.
+__device__ __forceinline__ void add_bf16x2(float& a, float& b, uint32_t w) {
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tadd.f32.bf16 %0, lo, %0;\n\tadd.f32.bf16 %1, hi, %1;\n\t}" : "+f"(a), "+f"(b) : "r"(w));
+}
+// 2^x of two x of up to 2^7, without the special function unit: x = r + f with a whole r and f within 1/2, a polynomial of degree 3 for 2^f (its coefficients
+// minimise the largest relative error, 7.5e-5, a fifteenth of what rounding to bf16 takes away) and r added to its exponent; zero below 2^-126, and a
+// NaN becomes too large for bf16.
+__device__ __forceinline__ void ex2_poly(uint64_t x, float& a, float& b) {
+  unpack2(x, a, b);
+  asm("max.NaN.f32 %0, %0, 0fC3000000;" : "+f"(a));     // -128
+  asm("max.NaN.f32 %0, %0, 0fC3000000;" : "+f"(b));
+  const uint64_t magic = pack2(12582912.f, 12582912.f), minus = pack2(-12582912.f, -12582912.f), neg = pack2(-1.f, -1.f);       // 1.5 * 2^23
+  x = pack2(a, b);
+  const uint64_t r = add2(x, magic), f = fma2(add2(r, minus), neg, x);
+  uint64_t y = pack2(0.055171669f, 0.055171669f);
+  y = fma2(y, f, pack2(0.24261112f, 0.24261112f));
+  y = fma2(y, f, pack2(0.69326099f, 0.69326099f));
+  y = fma2(y, f, pack2(0.99992807f, 0.99992807f));
+  float ra, rb, ya, yb;
+  unpack2(r, ra, rb);
+  unpack2(y, ya, yb);
+  a = __int_as_float(max(__float_as_int(ya) + (int)((uint32_t)__float_as_int(ra) << 23), 0));
+  b = __int_as_float(max(__float_as_int(yb) + (int)((uint32_t)__float_as_int(rb) << 23), 0));
 }
 // 32 columns of the warp's lanes; nothing may touch v before pp_landed.
 __device__ __forceinline__ void pp_ask(uint32_t taddr, float (&v)[32]) {
@@ -209,11 +242,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
   uint64_t* v_full = k_empty + kPpSlots;
   uint64_t* v_empty = v_full + kPpSlots;
   uint64_t* v_raw = v_empty + kPpSlots;               // the last tile's values, before the rows behind the last key are zeroed
-  uint64_t* s_full = v_raw + 1;                       // [row tile]
-  uint64_t* p_half = s_full + 2;
-  uint64_t* p_full = p_half + 2;
-  uint64_t* o_done = p_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+  uint64_t* s_full = v_raw + 1;                       // [row tile][parity of the block]
+  uint64_t* p_full = s_full + 4;                      // likewise
+  uint64_t* o_done = p_full + 4;                      // [row tile]
+  uint64_t* begun = o_done + 2;                       // the first row tile's first weights are there
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(begun + 1);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
   PpItem* item_s = reinterpret_cast<PpItem*>(smem_raw + 512);
   uint8_t* q_s = smem_raw + 1024 + ((1024 - ((smem_u32(smem_raw) + 1024) & 1023)) & 1023);
@@ -229,12 +262,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
         mbar_init(&v_empty[s], 2);
       }
       mbar_init(v_raw, 1);
-      for (int x = 0; x < 2; ++x) {
+      for (int x = 0; x < 4; ++x) {
         mbar_init(&s_full[x], 1);
-        mbar_init(&p_half[x], 4);
         mbar_init(&p_full[x], 4);
-        mbar_init(&o_done[x], 1);
       }
+      for (int x = 0; x < 2; ++x) mbar_init(&o_done[x], 1);
+      mbar_init(begun, 1);
       *failed = 0;
       mbar_init_fence();
     }
@@ -250,9 +283,22 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
   tc_fence_before();
   pdl_wait();
   pdl_launch_dependents();
-  if (warp == 3) {
-    const PpItem it = pp_item(p, blockIdx.y, blockIdx.x, blockIdx.z, lane);
-    if (lane == 0) *item_s = it;
+  // The loaders look up for themselves what the CTA does, and ask for their first pages; the queries are on their way before the others know.
+  int first_page = 0;
+  if (warp == 0 || warp == 3) {
+    const PpItem mine = pp_item(p, blockIdx.y, blockIdx.x, blockIdx.z, lane);
+    if (warp == 3 && lane == 0) *item_s = mine;
+    if (mine.seq >= 0 && mine.tiles > 0) {
+      if (warp == 0) {
+        if (lane == 0) mbar_arrive_expect_tx(q_full, 4u * p.per_tile * p.group * 128u);
+        __syncwarp();
+        if (lane < 4) tma_load_3d(q_s + lane * kPfBox, &q_map, 64 * (lane & 1), mine.kv * p.group, mine.row0 + (lane >> 1) * p.per_tile, q_full);
+      }
+      const int key = mine.tile0 * kPfTile + (Q4 ? lane : (lane >> 1) * min(1 << p.s.page_shift, kPfTile));
+      if ((Q4 || (lane >> 1) * min(1 << p.s.page_shift, kPfTile) < kPfTile) && key < mine.k_end)
+        first_page = p.s.tables[(size_t)mine.seq * p.s.table_ld + (key >> p.s.page_shift)];
+    }
+    __syncwarp();
   }
   __syncthreads();
   tc_fence_after();
@@ -263,8 +309,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     *failed = 1;
   };
   const int n = it.seq < 0 ? 0 : it.tiles;
-  // tiles of keys that a row tile needs
-  const int need[2] = {max(0, min(n, (min(it.pos0 + min(it.rows, p.per_tile), p.max_len) + kPfTile - 1) / kPfTile - it.tile0)), it.rows > p.per_tile ? n : 0};
+  // blocks of keys that a row tile needs
+  auto blocks = [&](int rows) { return max(0, min((min(it.pos0 + rows, p.max_len) + kPpBlock - 1) / kPpBlock - 2 * it.tile0, 2 * n)); };
+  const int need[2] = {n ? blocks(min(it.rows, p.per_tile)) : 0, n && it.rows > p.per_tile ? blocks(it.rows) : 0};
 
   // (registers: 384 threads of 168 at the start, then 128 of 88 or 104 and 256 of 208 or 200, the same in all)
   if (warp < 4) {
@@ -275,13 +322,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     uint64_t *full = values ? v_full : k_full, *empty = values ? v_empty : k_empty;
     uint8_t* to = values ? v_s : k_s;
     bool ok = true;
-    if (!values && n > 0) {
-      if (lane == 0) mbar_arrive_expect_tx(q_full, 4u * p.per_tile * p.group * 128u);
-      __syncwarp();
-      if (lane < 4)
-        tma_load_3d(q_s + lane * kPfBox, &q_map, 64 * (lane & 1), it.kv * p.group, it.row0 + (lane >> 1) * p.per_tile, q_full);
-      __syncwarp();
-    }
     const int* table = p.s.tables + (size_t)max(it.seq, 0) * p.s.table_ld;
     if constexpr (Q4) {
       const uint8_t* from = (values ? p.v : p.k) + it.kv * kQ4HeadBytes;
@@ -309,7 +349,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
         }
         return x;
       };
-      PpCodes next = codes_at(0, page_at(0));
+      PpCodes next = codes_at(0, first_page);
       int page = page_at(1);
       for (int i = 0; i < n && ok; ++i) {
         const int slot = i % kPpSlots;
@@ -334,7 +374,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
         const int key = (it.tile0 + i) * kPfTile + j * box_rows;
         return i < n && j < boxes && key < it.k_end ? table[key >> p.s.page_shift] : 0;
       };
-      int next = page_at(0);
+      int next = first_page;
       for (int i = 0; i < n && ok; ++i) {
         int page = next;
         next = page_at(i + 1);
@@ -367,57 +407,60 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     }
     if (!ok && lane == 0) give_up(DERR_EMPTY_WAIT);
   } else {
-    // ---- products
+    // ---- products: a block's scores, then the weighted values of the block before
     const bool leader = elect_one();
     const int x = warp - 1, mine = need[x];
-    const uint32_t idesc_s = umma_idesc_bf16(kPfTile), idesc_o = idesc_s | (1u << 16);   // (bit 16: B is N-major)
+    const uint32_t idesc_s = umma_idesc_bf16(kPpBlock), idesc_o = umma_idesc_bf16(kRowDim) | (1u << 16);       // (bit 16: B is N-major)
     const uint64_t qd = umma_desc_sw128(q_s + 2 * x * kPfBox), kd = umma_desc_sw128(k_s), vd = pf_desc_mn(v_s);
     const uint32_t s_t = tmem + (uint32_t)(x * 256), o_t = s_t + 128u;
     bool ok = n == 0 || __all_sync(0xffffffffu, mbar_wait_spin(q_full, 0));
-    for (int i = 0; i < n && ok; ++i) {
-      const int slot = i % kPpSlots;
-      const uint32_t ph = (uint32_t)((i / kPpSlots) & 1);
-      const uint64_t slot_off = (uint64_t)(slot * (kPpTile >> 4));
-      // (the scores' columns hold the weights of the tile before until its products are done)
-      ok = __all_sync(0xffffffffu, mbar_wait_spin(&k_full[slot], ph) && (i == 0 || i >= mine || mbar_wait_spin(&o_done[x], (uint32_t)((i - 1) & 1))));
-      if (!ok) break;
-      tc_fence_after();
-      if (leader) {
-        if (i < mine) {
+    // The second row tile begins half a turn behind the first: its products run while the other's weights are computed, and the other way round.
+    if (ok && x == 1 && mine > 0 && need[0] > 0) ok = __all_sync(0xffffffffu, mbar_wait_spin(begun, 0));
+    for (int j = 0; j <= mine && ok && mine; ++j) {
+      if (j < mine) {
+        const int slot = (j >> 1) % kPpSlots;
+        // (the scores' columns hold the weights of the block two before until its products are done)
+        ok = __all_sync(0xffffffffu, ((j & 1) || mbar_wait_spin(&k_full[slot], (uint32_t)((j >> 1) / kPpSlots & 1))) &&
+                                         (j < 2 || mbar_wait_spin(&o_done[x], (uint32_t)(j & 1))));
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+          const uint64_t kt = kd + (uint64_t)(slot * (kPpTile >> 4) + (j & 1) * (kPpBlock * 128 >> 4));
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint64_t off = (uint64_t)((k >> 2) * (kPfBox >> 4) + 2 * (k & 3));
-            umma_f16(s_t, qd + off, kd + slot_off + off, idesc_s, k != 0);
+            umma_f16(s_t + (uint32_t)((j & 1) * kPpBlock), qd + off, kt + off, idesc_s, k != 0);
           }
-          umma_commit(&s_full[x]);
-          umma_commit(&k_empty[slot]);
-        } else {
-          mbar_arrive(&k_empty[slot]);
+          umma_commit(&s_full[2 * x + (j & 1)]);
+          if ((j & 1) || j + 1 == mine) umma_commit(&k_empty[slot]);
         }
-      }
-      __syncwarp();
-      ok = __all_sync(0xffffffffu, mbar_wait_spin(&v_full[slot], ph) && (i >= mine || mbar_wait_spin(&p_half[x], (uint32_t)(i & 1))));
-      if (!ok) break;
-      if (i >= mine) {
-        if (leader) mbar_arrive(&v_empty[slot]);
         __syncwarp();
-        continue;
       }
-      tc_fence_after();
-      if (leader) {
+      if (j > 0) {
+        const int h = j - 1, slot = (h >> 1) % kPpSlots;
+        ok = __all_sync(0xffffffffu, ((h & 1) || mbar_wait_spin(&v_full[slot], (uint32_t)((h >> 1) / kPpSlots & 1))) &&
+                                         mbar_wait_spin(&p_full[2 * x + (h & 1)], (uint32_t)(h >> 1 & 1)));
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+          const uint64_t vt = vd + (uint64_t)(slot * (kPpTile >> 4) + (h & 1) * (kPpBlock * 128 >> 4));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_f16_ts(o_t, s_t + 8u * k, vd + slot_off + (uint64_t)(k * (2048 >> 4)), idesc_o, (i | k) != 0);
+          for (int k = 0; k < kPpBlock / 16; ++k)
+            umma_f16_ts(o_t, s_t + (uint32_t)((h & 1) * kPpBlock) + 8u * k, vt + (uint64_t)(k * (2048 >> 4)), idesc_o, (h | k) != 0);
+          umma_commit(&o_done[x]);
+          if ((h & 1) || j == mine) umma_commit(&v_empty[slot]);
+        }
+        __syncwarp();
       }
+    }
+    for (int i = (mine + 1) / 2; i < n && ok; ++i) {   // tiles that only the other row tile needs
+      const int slot = i % kPpSlots;
+      const uint32_t ph = (uint32_t)(i / kPpSlots & 1);
+      ok = __all_sync(0xffffffffu, mbar_wait_spin(&k_full[slot], ph));
+      if (ok && leader) mbar_arrive(&k_empty[slot]);
       __syncwarp();
-      ok = __all_sync(0xffffffffu, mbar_wait_spin(&p_full[x], (uint32_t)(i & 1)));
-      if (!ok) break;
-      tc_fence_after();
-      if (leader) {
-#pragma unroll
-        for (int k = 4; k < 8; ++k) umma_f16_ts(o_t, s_t + 8u * k, vd + slot_off + (uint64_t)(k * (2048 >> 4)), idesc_o, 1u);
-        umma_commit(&o_done[x]);
-        umma_commit(&v_empty[slot]);
-      }
+      ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(&v_full[slot], ph));
+      if (ok && leader) mbar_arrive(&v_empty[slot]);
       __syncwarp();
     }
     if (!ok && lane == 0) give_up(DERR_FULL_WAIT);
@@ -434,34 +477,39 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     float m = -FLT_MAX, l = 0.f;
     bool ok = true;
 #pragma unroll 1
-    for (int i = 0; i < mine && ok; ++i) {
-      ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[x], (uint32_t)(i & 1)));
+    for (int j = 0; j < mine && ok; ++j) {
+      const uint32_t b_t = s_t + (uint32_t)((j & 1) * kPpBlock);
+      ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[2 * x + (j & 1)], (uint32_t)(j >> 1 & 1)));
       if (!ok) break;
       tc_fence_after();
       __syncwarp();
-      float v[4][32];
+      float v[2][32];
+      pp_ask(b_t, v[0]);
+      pp_ask(b_t + 32u, v[1]);
+      pp_landed(v[0]);
+      pp_landed(v[1]);
+      const int last = limit - it.tile0 * kPfTile - j * kPpBlock;      // keys 0 .. last of the block count
+      if (!__all_sync(0xffffffffu, last >= kPpBlock - 1)) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) pp_ask(s_t + 32u * c, v[c]);
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) pp_landed(v[c]);
-      const int last = limit - (it.tile0 + i) * kPfTile;               // keys 0 .. last of the tile count
-      if (!__all_sync(0xffffffffu, last >= kPfTile - 1)) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[c][j] = 32 * c + j <= last ? v[c][j] : -INFINITY;
+          for (int k = 0; k < 32; ++k) v[c][k] = 32 * c + k <= last ? v[c][k] : -INFINITY;
       }
       float mx[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        mx[c] = fmaxf(v[c][0], v[c][1]);
+        mx[c] = fmaxf(v[c >> 1][16 * (c & 1)], v[c >> 1][16 * (c & 1) + 1]);
 #pragma unroll
-        for (int j = 2; j < 32; j += 2) mx[c] = fmaxf(mx[c], fmaxf(v[c][j], v[c][j + 1]));
+        for (int k = 2; k < 16; k += 2) mx[c] = fmaxf(mx[c], fmaxf(v[c >> 1][16 * (c & 1) + k], v[c >> 1][16 * (c & 1) + k + 1]));
       }
       const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2, -FLT_MAX);
-      if (i == 0) {
+      if (j == 0) {
         m = top;
-      } else if (__any_sync(0xffffffffu, top > m + kPpLag)) {          // (the products so far are done, or these scores would not be here)
+      } else if (__any_sync(0xffffffffu, top > m + kPpLag)) {
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[x], (uint32_t)((j - 1) & 1)));
+        if (!ok) break;
+        tc_fence_after();
+        __syncwarp();
         const float m_new = top > m + kPpLag ? top : m, f = ex2(m - m_new);
 #pragma unroll 1
         for (int c = 0; c < kRowDim; c += 16) {
@@ -469,37 +517,43 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
           uint32_t w[16];
           tmem_ld16(o_t + (uint32_t)c, o);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[j] * f);
+          for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(o[k] * f);
           tmem_st16(o_t + (uint32_t)c, w);
         }
         l *= f;
         m = m_new;
       }
       const uint64_t less = pack2(-m, -m);
-      uint64_t sum[2] = {0, 0};
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t w[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int k = 0; k < 16; ++k) {
           float a, b;
-          unpack2(fma2(pack2(v[c][2 * j], v[c][2 * j + 1]), scale2, less), a, b);
-          w[j] = pack_bf16(ex2(a), ex2(b));
-          sum[j & 1] = add2(sum[j & 1], pack2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u)));
+          const uint64_t t = fma2(pack2(v[c][2 * k], v[c][2 * k + 1]), scale2, less);
+          if (k % kPpPoly == kPpPoly - 1) {
+            ex2_poly(t, a, b);
+          } else {
+            unpack2(t, a, b);
+            a = ex2(a);
+            b = ex2(b);
+          }
+          w[k] = pack_bf16(a, b);
+          add_bf16x2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], w[k]);
         }
-        tmem_st16(s_t + 16u * c, w);                  // over scores that this thread has read
-        if (c & 1) {
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(c == 1 ? &p_half[x] : &p_full[x]);
-          __syncwarp();
-        }
+        tmem_st16(b_t + 16u * c, w);                  // over scores that this thread has read
       }
-      float a, b;
-      unpack2(add2(sum[0], sum[1]), a, b);
-      l += a + b;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[2 * x + (j & 1)]);
+      if (j == 0 && warp == 4 && lane == 0) mbar_arrive(begun);
+      __syncwarp();
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
+    // (the last scores tell of the products up to the last but two: a look at the last ones' parity would not tell them from those)
+    if (ok && mine > 1) ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[x], (uint32_t)(mine & 1)));
     if (ok && mine) ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[x], (uint32_t)((mine - 1) & 1)));
     if (!ok && lane == 0) give_up(DERR_TMEM);
     tc_fence_after();
@@ -510,29 +564,55 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     if (parts && live && ok) *reinterpret_cast<float2*>(p.part_ml + (part_at + at) / (kRowDim / 2)) = make_float2(m, l);
     if (ok && mine) {
       const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-      float zero = 0.f;                               // NaN if some sum is not finite
+      float zero[4] = {0.f, 0.f, 0.f, 0.f};           // NaN if some sum is not finite
+      // A row's results go over its warp's part of the queries, so that 16 lanes store 256 bytes of a row (a lane with a row of its own 5000 cycles for the
+      // tile, its stores each to 32 places).
+      uint8_t* mine_s = q_s + 2 * x * kPfBox + q4 * 32 * 256;
+      const unsigned to_store = __ballot_sync(0xffffffffu, live);
+      const int turns = parts ? 2 : 1;
 #pragma unroll 1
-      for (int c = 0; c < kRowDim; c += 32) {
-        float o[32];
-        __syncwarp();
-        pp_ask(o_t + (uint32_t)c, o);
-        pp_landed(o);
-        if (!live) continue;
+      for (int turn = 0; turn < turns; ++turn) {
+#pragma unroll 1
+        for (int c = 0; c < kRowDim / turns; c += 32) {
+          float o[32];
+          __syncwarp();
+          pp_ask(o_t + (uint32_t)(turn * (kRowDim / 2) + c), o);
+          pp_landed(o);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) zero = fmaf(o[j], 0.f, zero);
-        if (parts) {
-          float4* y = reinterpret_cast<float4*>(p.part_o + part_at + at + c);
+          for (int k = 0; k < 32; ++k) zero[k & 3] = fmaf(o[k], 0.f, zero[k & 3]);
+          if (parts) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-        } else {
-          uint4* y = reinterpret_cast<uint4*>(p.out + at + c);
+            for (int k = 0; k < 8; ++k)
+              *reinterpret_cast<float4*>(mine_s + lane * 256 + (((c / 4 + k) ^ (lane & 15)) << 4)) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            y[j] = make_uint4(pack_bf16(o[8 * j] * inv, o[8 * j + 1] * inv), pack_bf16(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
-                              pack_bf16(o[8 * j + 4] * inv, o[8 * j + 5] * inv), pack_bf16(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint4*>(mine_s + lane * 256 + (((c / 8 + k) ^ (lane & 15)) << 4)) =
+                  make_uint4(pack_bf16(o[8 * k] * inv, o[8 * k + 1] * inv), pack_bf16(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+                             pack_bf16(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack_bf16(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+          }
         }
+        __syncwarp();
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {         // (all loads of a half before its stores)
+          uint4 y[8];
+          unsigned long long to[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int row = 16 * half + 2 * k + (lane >> 4);
+            to[k] = __shfl_sync(0xffffffffu, (unsigned long long)at, row);
+            y[k] = *reinterpret_cast<const uint4*>(mine_s + row * 256 + (((lane & 15) ^ (row & 15)) << 4));
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            uint4* dst = parts ? reinterpret_cast<uint4*>(p.part_o + part_at + to[k] + turn * (kRowDim / 2)) : reinterpret_cast<uint4*>(p.out + to[k]);
+            if (to_store >> (16 * half + 2 * k + (lane >> 4)) & 1u) dst[lane & 15] = y[k];
+          }
+        }
+        __syncwarp();
       }
-      unsigned rows = __ballot_sync(0xffffffffu, live && zero != zero);
+      zero[0] += zero[1] + (zero[2] + zero[3]);
+      unsigned rows = __ballot_sync(0xffffffffu, live && zero[0] != zero[0]);
       if (rows) {
         // Keys that rows of this CTA do not see and their tiles hold: from its first position on.
         const int first = it.tile0 * kPfTile, end = min((it.tile0 + n) * kPfTile, it.k_end);

@@ -267,6 +267,27 @@ def test_prefill_values_that_earlier_rows_do_not_see(dev, bad):
         assert (np.abs(got - want)[before] <= tol[before]).all() and (np.abs(got - want)[~before][:, ok] <= tol[~before][:, ok]).all()
 
 
+@pytest.mark.parametrize("form", ["bf16", "q4"])
+def test_prefill_keys_that_are_no_number(dev, form):
+    """Rows that see such a key are NaN, in its KV head; those before it are what they were."""
+    for at_pos in (0, 3, 130, 131, 170, 199):
+        s = Sequences(8, 2, 32, [200], [200], 34, form)
+        place = s.places(0, [at_pos])[0]
+        if form == "q4":
+            s.raw[0][place, 2 * 64:].view(np.uint16)[5] = 0x7FC0
+        else:
+            s.raw[0][place, HD + 40] = 0x7FC0
+        s.put(dev)
+        got = widen(s.prefill().to_vec()).reshape(s.rows, 8, HD)
+        dev.sync()
+        want, size = s.reference()
+        bad = np.zeros((200, 8), bool)
+        bad[at_pos:, 4:] = True
+        assert np.isnan(got[bad]).all()
+        tol = 2.0 ** -14 * size + 2.0 ** -7 * (size + np.abs(want))
+        assert (np.abs(got - want)[~bad] <= tol[~bad]).all()
+
+
 def test_prefill_scores_that_grow(dev):
     """Keys in ascending order of their scores, far apart: the reference has to follow."""
     s = Sequences(8, 2, 32, [640], [640], 33, "bf16")
