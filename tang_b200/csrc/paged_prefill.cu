@@ -1,15 +1,15 @@
 // Causal attention of several sequences' new positions, packed, over their pages (include/tangq.h: tq_gqa_prefill_paged).
 //
-// A CTA takes two tiles of 128 rows (128 / group positions x the group's heads of one KV head) of a sequence over the same tiles of 128 keys:
-//   warp 0        queries, then tiles of keys: tensor copies page by page, or, for pages of 4 bits, codes that it turns into the same bf16 rows
-//   warps 1, 2    issue a row tile's products: S = Q K^T (both from shared memory), then O += P V (P from tensor memory, V N-major)
-//   warp 3        tiles of values, likewise; rows behind the last key are zeros (whatever a page holds there must not meet a weight of zero)
-//   warps 4..7, 8..11   softmax of a row tile, a thread a row
-// Tensor memory: S / P and O of both tiles, 4 x 128 columns.  A row's scores are read once, into registers; its weights go over their columns, block by
-// first of which is multiplied while the second is computed.  A weight is one bf16 number, and the sum that results are divided by is that of the numbers as they
-// entered: a row of a few keys, where the roundings do not average out, is then nearer (the largest weight need not be 1 for that, so that the reference
-// may lag: a row's sums are rescaled only when its maximum grew by more than 2^8).
-// Few rows: a tile pair's keys are cut into parts, a CTA each, and a second kernel joins the results.
+// A CTA takes a tile of 128 rows (128 / group positions x the group's heads of one KV head) of a sequence and walks its keys in blocks of 64:
+//   warp 0        queries, then blocks of keys: tensor copies page by page, or, for pages of 4 bits, codes that it turns into the same bf16 rows
+//   warp 1        issues the products: a block's S = Q K^T (both from shared memory), then O += P V of the block before (P from tensor memory, V N-major)
+//   warp 2        blocks of values, likewise; rows behind the last key are zeros (whatever a page holds there must not meet a weight of zero)
+//   warps 4..7    softmax, a thread a row
+// Tensor memory: two blocks' S / P and O, 256 columns, so that two CTAs share an SM: one's products run while the other's weights are computed, and starts and
+// ends (look-up, first copies, results: 10000 of 50000 cycles for 12 times 128 keys) are hidden.  A weight is one bf16 number, and the sum that results are
+// divided by is that of the numbers as they entered: a row of a few keys, where the roundings do not average out, is then nearer (the largest weight need not
+// be 1 for that, so that the reference may lag: a row's sums are rescaled only when its maximum grew by more than 2^8).
+// Few rows: a tile's keys are cut into parts, a CTA each, and a second kernel joins the results.
 #include <cfloat>
 
 #include "attn_mma.cuh"
@@ -18,11 +18,12 @@
 
 namespace tq {
 
-constexpr int kPpThreads = 384;
-constexpr int kPpSlots = 2;                           // of keys, and of values: a tile each
-constexpr int kPpTile = 2 * kPfBox;                   // bytes: two boxes of 64 columns
+constexpr int kPpThreads = 256;
 constexpr int kPpBlock = 64;                          // keys whose scores are computed, and become weights, at a time
-constexpr size_t kPpSmem = 1024 + 1024 + 4 * (size_t)kPfBox + 2 * kPpSlots * (size_t)kPpTile;
+constexpr int kPpSlots = 2;                           // of keys, and of values: a block each
+constexpr int kPpBox = kPpBlock * 128;                // bytes of a block's 64 columns
+constexpr int kPpTile = 2 * kPpBox;
+constexpr size_t kPpSmem = 1024 + 1024 + 2 * (size_t)kPfBox + 2 * kPpSlots * (size_t)kPpTile;
 constexpr float kPpLag = 8.f;                         // a reference may be so far below its row's maximum (log2)
 constexpr int kPpMaxParts = 16;
 constexpr int kPpPoly = 4;                            // one of so many pairs of weights is a polynomial
@@ -33,7 +34,7 @@ struct PackedPrefillParams {
   const uint8_t *k, *v;
   size_t row_bytes;
   int n_heads, n_kv, group, max_len;
-  int per_tile, parts;                 // positions of a row tile; parts of a tile pair's keys
+  int per_tile, parts;                 // positions of a row tile; parts of a tile's keys
   float scale_log2;
   __nv_bfloat16* out;
   float *part_o, *part_ml;             // [part][rows][n_heads][128], [..][2] (reference and sum) where there are several
@@ -82,16 +83,15 @@ __device__ __forceinline__ void attend_paged_row(const PackedPrefillParams& p, i
 // What a CTA does.
 struct PpItem {
   int seq, kv;                         // of the pool (-1: nothing), KV head
-  int row0, rows;                      // first packed row, rows of both tiles
+  int row0, rows;                      // first packed row, rows
   int pos0;                            // position of the first row
-  int tile0, tiles;                    // tiles of keys: the part's first, how many
+  int block0, blocks;                  // blocks of keys: the part's first, how many
   int k_end;                           // keys that the last row sees, or the bound
 };
-// Tile pair x of all sequences, the longest of each sequence first, by one warp.
+// Tile x of all sequences, the longest of each sequence first, by one warp.
 __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, int kv, int part, int lane) {
   PpItem it{-1, kv, 0, 0, 0, 0, 0, 0};
-  const int per_pair = 2 * p.per_tile;
-  int i = -1, first = 0, count = 0, pair = 0, s = -1, len = 0;
+  int i = -1, first = 0, count = 0, tile = 0, s = -1, len = 0;
   if (!p.s.seq_rows) {
     if (x < p.s.batch) {
       i = x, first = x, count = 1;
@@ -111,14 +111,14 @@ __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, i
         if (a < 0 || b < a || b > p.s.rows || (j == 0 && a != 0)) bad = true;
         else f = a, c = b - a;
       }
-      const int pairs = (c + per_pair - 1) / per_pair;
-      int incl = pairs;
+      const int tiles = (c + p.per_tile - 1) / p.per_tile;
+      int incl = tiles;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int w = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += w;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, x >= before + incl - pairs && x < before + incl);
+      const unsigned hit = __ballot_sync(0xffffffffu, x >= before + incl - tiles && x < before + incl);
       if (hit) {
         const int src = __ffs(hit) - 1;
         i = base + src;
@@ -126,7 +126,7 @@ __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, i
         count = __shfl_sync(0xffffffffu, c, src);
         s = __shfl_sync(0xffffffffu, js, src);
         len = __shfl_sync(0xffffffffu, jl, src);
-        pair = __shfl_sync(0xffffffffu, before + incl, src) - 1 - x;   // (the last pair first)
+        tile = __shfl_sync(0xffffffffu, before + incl, src) - 1 - x;   // (the last tile first)
       }
       before += __shfl_sync(0xffffffffu, incl, 31);
       if (i >= 0) break;
@@ -139,13 +139,13 @@ __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, i
     return it;
   }
   it.seq = s;
-  it.row0 = first + pair * per_pair;
-  it.rows = min(per_pair, count - pair * per_pair);
-  it.pos0 = len - count + pair * per_pair;
+  it.row0 = first + tile * p.per_tile;
+  it.rows = min(p.per_tile, count - tile * p.per_tile);
+  it.pos0 = len - count + tile * p.per_tile;
   it.k_end = min(it.pos0 + it.rows, p.max_len);
-  const int all = (it.k_end + kPfTile - 1) / kPfTile, per = max((all + p.parts - 1) / p.parts, 2);
-  it.tile0 = min(part * per, all);
-  it.tiles = min(per, all - it.tile0);
+  const int all = (it.k_end + kPpBlock - 1) / kPpBlock, per = max((all + p.parts - 1) / p.parts, 4);
+  it.block0 = min(part * per, all);
+  it.blocks = min(per, all - it.block0);
   return it;
 }
 
@@ -208,7 +208,7 @@ __device__ __forceinline__ void pp_landed(float (&v)[32]) {
                  "+f"(v[31])::"memory");
 }
 
-// Pages of 4 bits: a loader's tiles.  A lane takes key lane + 32 u of a tile, u = 0 .. 3: its codes are asked for a turn ahead, its page two.
+// Pages of 4 bits: a loader's blocks.  A lane takes key lane + 32 u of a block, u = 0, 1: its codes are asked for a turn ahead, its page two.
 struct PpCodes {
   uint4 w[4];
   uint2 s;
@@ -225,55 +225,58 @@ __device__ __forceinline__ void pp_convert(uint8_t* tile, int key, const PpCodes
 #pragma unroll
       for (int j = 0; j < 4; ++j) a[j] = bf16x2_fma(a[j], sc, off);
       const int c = 4 * (b & 1) + i;   // 16-byte chunk of the row's half
-      *reinterpret_cast<uint4*>(tile + (b >> 1) * kPfBox + key * 128 + ((c ^ (key & 7)) << 4)) =
+      *reinterpret_cast<uint4*>(tile + (b >> 1) * kPpBox + key * 128 + ((c ^ (key & 7)) << 4)) =
           make_uint4(prmt(a[0], a[1], 0x5410), prmt(a[2], a[3], 0x5410), prmt(a[0], a[1], 0x7632), prmt(a[2], a[3], 0x7632));
     }
   }
 }
 
+// Shared-memory descriptor of a block of values: keys are k, their 64-column halves a box apart (MN-major, 128-byte swizzle).
+__device__ __forceinline__ uint64_t pp_desc_values(const void* smem_ptr) {
+  return (uint64_t)((smem_u32(smem_ptr) >> 4) & 0x3FFF) | (uint64_t)(kPpBox >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
 template <bool Q4>
-__global__ void __launch_bounds__(kPpThreads, 1)
+__global__ void __launch_bounds__(kPpThreads, 2)
 paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                      const __grid_constant__ PackedPrefillParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem_raw);
   uint64_t* k_full = q_full + 1;                      // [slots]
-  uint64_t* k_empty = k_full + kPpSlots;              // [slots] both row tiles' products done
+  uint64_t* k_empty = k_full + kPpSlots;
   uint64_t* v_full = k_empty + kPpSlots;
   uint64_t* v_empty = v_full + kPpSlots;
-  uint64_t* v_raw = v_empty + kPpSlots;               // the last tile's values, before the rows behind the last key are zeroed
-  uint64_t* s_full = v_raw + 1;                       // [row tile][parity of the block]
-  uint64_t* p_full = s_full + 4;                      // likewise
-  uint64_t* o_done = p_full + 4;                      // [row tile]
-  uint64_t* begun = o_done + 2;                       // the first row tile's first weights are there
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(begun + 1);
+  uint64_t* v_raw = v_empty + kPpSlots;               // the last block's values, before the rows behind the last key are zeroed
+  uint64_t* s_full = v_raw + 1;                       // [parity of the block]
+  uint64_t* p_full = s_full + 2;                      // likewise
+  uint64_t* o_done = p_full + 2;                      // likewise: whoever waits for a block's products has seen those of the block two before
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
   PpItem* item_s = reinterpret_cast<PpItem*>(smem_raw + 512);
   uint8_t* q_s = smem_raw + 1024 + ((1024 - ((smem_u32(smem_raw) + 1024) & 1023)) & 1023);
-  uint8_t *k_s = q_s + 4 * kPfBox, *v_s = k_s + kPpSlots * kPpTile;
+  uint8_t *k_s = q_s + 2 * kPfBox, *v_s = k_s + kPpSlots * kPpTile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
     if (lane == 0) {
       mbar_init(q_full, 1);
       for (int s = 0; s < kPpSlots; ++s) {
         mbar_init(&k_full[s], 1);
-        mbar_init(&k_empty[s], 2);
+        mbar_init(&k_empty[s], 1);
         mbar_init(&v_full[s], 1);
-        mbar_init(&v_empty[s], 2);
+        mbar_init(&v_empty[s], 1);
       }
       mbar_init(v_raw, 1);
-      for (int x = 0; x < 4; ++x) {
+      for (int x = 0; x < 2; ++x) {
         mbar_init(&s_full[x], 1);
         mbar_init(&p_full[x], 4);
+        mbar_init(&o_done[x], 1);
       }
-      for (int x = 0; x < 2; ++x) mbar_init(&o_done[x], 1);
-      mbar_init(begun, 1);
       *failed = 0;
       mbar_init_fence();
     }
   } else if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-  } else if (warp == 2 && lane == 0) {
+    tmem_alloc(tmem_slot, 256);
+  } else if (warp == 3 && lane == 0) {
     prefetch_map(&q_map);
     if (!Q4) {
       prefetch_map(&k_map);
@@ -284,19 +287,19 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
   pdl_wait();
   pdl_launch_dependents();
   // The loaders look up for themselves what the CTA does, and ask for their first pages; the queries are on their way before the others know.
+  const int box_rows = min(1 << p.s.page_shift, kPpBlock), boxes = kPpBlock / box_rows;
   int first_page = 0;
-  if (warp == 0 || warp == 3) {
+  if (warp == 0 || warp == 2) {
     const PpItem mine = pp_item(p, blockIdx.y, blockIdx.x, blockIdx.z, lane);
-    if (warp == 3 && lane == 0) *item_s = mine;
-    if (mine.seq >= 0 && mine.tiles > 0) {
+    if (warp == 2 && lane == 0) *item_s = mine;
+    if (mine.seq >= 0 && mine.blocks > 0) {
       if (warp == 0) {
-        if (lane == 0) mbar_arrive_expect_tx(q_full, 4u * p.per_tile * p.group * 128u);
+        if (lane == 0) mbar_arrive_expect_tx(q_full, 2u * p.per_tile * p.group * 128u);
         __syncwarp();
-        if (lane < 4) tma_load_3d(q_s + lane * kPfBox, &q_map, 64 * (lane & 1), mine.kv * p.group, mine.row0 + (lane >> 1) * p.per_tile, q_full);
+        if (lane < 2) tma_load_3d(q_s + lane * kPfBox, &q_map, 64 * lane, mine.kv * p.group, mine.row0, q_full);
       }
-      const int key = mine.tile0 * kPfTile + (Q4 ? lane : (lane >> 1) * min(1 << p.s.page_shift, kPfTile));
-      if ((Q4 || (lane >> 1) * min(1 << p.s.page_shift, kPfTile) < kPfTile) && key < mine.k_end)
-        first_page = p.s.tables[(size_t)mine.seq * p.s.table_ld + (key >> p.s.page_shift)];
+      const int key = mine.block0 * kPpBlock + (Q4 ? lane : (lane >> 1) * box_rows);
+      if ((Q4 || (lane >> 1) < boxes) && key < mine.k_end) first_page = p.s.tables[(size_t)mine.seq * p.s.table_ld + (key >> p.s.page_shift)];
     }
     __syncwarp();
   }
@@ -308,178 +311,159 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     atomicCAS(p.err, 0, code);
     *failed = 1;
   };
-  const int n = it.seq < 0 ? 0 : it.tiles;
-  // blocks of keys that a row tile needs
-  auto blocks = [&](int rows) { return max(0, min((min(it.pos0 + rows, p.max_len) + kPpBlock - 1) / kPpBlock - 2 * it.tile0, 2 * n)); };
-  const int need[2] = {n ? blocks(min(it.rows, p.per_tile)) : 0, n && it.rows > p.per_tile ? blocks(it.rows) : 0};
+  const int n = it.seq < 0 ? 0 : it.blocks;
 
-  // (registers: 384 threads of 168 at the start, then 128 of 88 or 104 and 256 of 208 or 200, the same in all)
+  // (registers: 256 threads of 128 at the start, then 128 of 88 or 104 and 128 of 168 or 152, the same in all)
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q4 ? 104 : 88));
-  if (warp == 0 || warp == 3) {
-    // ---- tiles of keys (and the queries), tiles of values
-    const bool values = warp == 3;
-    uint64_t *full = values ? v_full : k_full, *empty = values ? v_empty : k_empty;
-    uint8_t* to = values ? v_s : k_s;
-    bool ok = true;
-    const int* table = p.s.tables + (size_t)max(it.seq, 0) * p.s.table_ld;
-    if constexpr (Q4) {
-      const uint8_t* from = (values ? p.v : p.k) + it.kv * kQ4HeadBytes;
-      const int steps = 4 * n, key0 = it.tile0 * kPfTile + lane, scales = p.n_kv * kQ4HeadBytes - it.kv * kQ4HeadBytes + it.kv * 2 * kQ4HeadScales;
-      auto page_at = [&](int m) {      // of key `lane` of step m
-        const int key = key0 + 32 * m;
-        return m < steps && key < it.k_end ? table[key >> p.s.page_shift] : 0;
-      };
-      auto codes_at = [&](int m, int page) {
-        PpCodes x;
-        const int key = key0 + 32 * m;
-        if (m < steps && key < it.k_end) {
-          if (page < 0 || page >= p.s.n_pages) {
-            atomicCAS(p.err, 0, (int)DERR_POSITION);
-            page = 0;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q4 ? 104 : 88));
+    if (warp == 0 || warp == 2) {
+      // ---- blocks of keys, blocks of values
+      const bool values = warp == 2;
+      uint64_t *full = values ? v_full : k_full, *empty = values ? v_empty : k_empty;
+      uint8_t* to = values ? v_s : k_s;
+      bool ok = true;
+      const int* table = p.s.tables + (size_t)max(it.seq, 0) * p.s.table_ld;
+      if constexpr (Q4) {
+        const uint8_t* from = (values ? p.v : p.k) + it.kv * kQ4HeadBytes;
+        const int steps = 2 * n, key0 = it.block0 * kPpBlock + lane, scales = p.n_kv * kQ4HeadBytes - it.kv * kQ4HeadBytes + it.kv * 2 * kQ4HeadScales;
+        auto page_at = [&](int m) {    // of key `lane` of step m
+          const int key = key0 + 32 * m;
+          return m < steps && key < it.k_end ? table[key >> p.s.page_shift] : 0;
+        };
+        auto codes_at = [&](int m, int page) {
+          PpCodes x;
+          const int key = key0 + 32 * m;
+          if (m < steps && key < it.k_end) {
+            if (page < 0 || page >= p.s.n_pages) {
+              atomicCAS(p.err, 0, (int)DERR_POSITION);
+              page = 0;
+            }
+            const uint8_t* row = from + ((size_t)(page << p.s.page_shift) + (key & ((1 << p.s.page_shift) - 1))) * p.row_bytes;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.w[i] = *reinterpret_cast<const uint4*>(row + 16 * i);
+            x.s = *reinterpret_cast<const uint2*>(row + scales);
+          } else {                     // rows of zeros
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.w[i] = make_uint4(0u, 0u, 0u, 0u);
+            x.s = make_uint2(0u, 0u);
           }
-          const uint8_t* row = from + ((size_t)(page << p.s.page_shift) + (key & ((1 << p.s.page_shift) - 1))) * p.row_bytes;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x.w[i] = *reinterpret_cast<const uint4*>(row + 16 * i);
-          x.s = *reinterpret_cast<const uint2*>(row + scales);
-        } else {                       // rows of zeros
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x.w[i] = make_uint4(0u, 0u, 0u, 0u);
-          x.s = make_uint2(0u, 0u);
-        }
-        return x;
-      };
-      PpCodes next = codes_at(0, first_page);
-      int page = page_at(1);
-      for (int i = 0; i < n && ok; ++i) {
-        const int slot = i % kPpSlots;
-        ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)((i / kPpSlots) & 1) ^ 1u));
-        if (!ok) break;
-#pragma unroll 1
-        for (int u = 0; u < 4; ++u) {
-          const PpCodes x = next;
-          next = codes_at(4 * i + u + 1, page);
-          page = page_at(4 * i + u + 2);
-          pp_convert(to + slot * kPpTile, 32 * u + lane, x);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[slot]);
-        __syncwarp();
-      }
-    } else {
-      // a lane per box: a page's rows, half their columns
-      const int box_rows = min(1 << p.s.page_shift, kPfTile), boxes = kPfTile / box_rows, j = lane >> 1, c = lane & 1;
-      auto page_at = [&](int i) {
-        const int key = (it.tile0 + i) * kPfTile + j * box_rows;
-        return i < n && j < boxes && key < it.k_end ? table[key >> p.s.page_shift] : 0;
-      };
-      int next = first_page;
-      for (int i = 0; i < n && ok; ++i) {
-        int page = next;
-        next = page_at(i + 1);
-        const int slot = i % kPpSlots, key = (it.tile0 + i) * kPfTile, keys = min(kPfTile, it.k_end - key), used = (keys + box_rows - 1) / box_rows;
-        if (page < 0 || page >= p.s.n_pages) {
-          atomicCAS(p.err, 0, (int)DERR_POSITION);
-          page = 0;
-        }
-        const int row = (page << p.s.page_shift) + (key & ((1 << p.s.page_shift) - 1) & ~(box_rows - 1));
-        ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)((i / kPpSlots) & 1) ^ 1u));
-        if (!ok) break;
-        const bool cut = values && keys < kPfTile;
-        uint64_t* bar = cut ? v_raw : &full[slot];
-        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(used * box_rows) * 256u);
-        __syncwarp();
-        if (j < used) tma_load_2d(to + slot * kPpTile + c * kPfBox + j * box_rows * 128, values ? &v_map : &k_map, it.kv * kRowDim + 64 * c, row, bar);
-        __syncwarp();
-        if (cut) {                     // (the last tile)
-          ok = __all_sync(0xffffffffu, mbar_wait_spin(v_raw, 0));
+          return x;
+        };
+        PpCodes next = codes_at(0, first_page);
+        int page = page_at(1);
+        for (int i = 0; i < n && ok; ++i) {
+          const int slot = i % kPpSlots;
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)((i / kPpSlots) & 1) ^ 1u));
           if (!ok) break;
-          uint8_t* at = to + slot * kPpTile;
-          for (int k = lane; k < 2 * (kPfTile - keys) * 8; k += 32)    // (a row's 128 bytes of either box, whatever their order)
-            *reinterpret_cast<uint4*>(at + ((k >> 3) & 1) * kPfBox + (keys + (k >> 4)) * 128 + 16 * (k & 7)) = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+          for (int u = 0; u < 2; ++u) {
+            const PpCodes x = next;
+            next = codes_at(2 * i + u + 1, page);
+            page = page_at(2 * i + u + 2);
+            pp_convert(to + slot * kPpTile, 32 * u + lane, x);
+          }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) mbar_arrive(&full[slot]);
           __syncwarp();
         }
-      }
-    }
-    if (!ok && lane == 0) give_up(DERR_EMPTY_WAIT);
-  } else {
-    // ---- products: a block's scores, then the weighted values of the block before
-    const bool leader = elect_one();
-    const int x = warp - 1, mine = need[x];
-    const uint32_t idesc_s = umma_idesc_bf16(kPpBlock), idesc_o = umma_idesc_bf16(kRowDim) | (1u << 16);       // (bit 16: B is N-major)
-    const uint64_t qd = umma_desc_sw128(q_s + 2 * x * kPfBox), kd = umma_desc_sw128(k_s), vd = pf_desc_mn(v_s);
-    const uint32_t s_t = tmem + (uint32_t)(x * 256), o_t = s_t + 128u;
-    bool ok = n == 0 || __all_sync(0xffffffffu, mbar_wait_spin(q_full, 0));
-    // The second row tile begins half a turn behind the first: its products run while the other's weights are computed, and the other way round.
-    if (ok && x == 1 && mine > 0 && need[0] > 0) ok = __all_sync(0xffffffffu, mbar_wait_spin(begun, 0));
-    for (int j = 0; j <= mine && ok && mine; ++j) {
-      if (j < mine) {
-        const int slot = (j >> 1) % kPpSlots;
-        // (the scores' columns hold the weights of the block two before until its products are done)
-        ok = __all_sync(0xffffffffu, ((j & 1) || mbar_wait_spin(&k_full[slot], (uint32_t)((j >> 1) / kPpSlots & 1))) &&
-                                         (j < 2 || mbar_wait_spin(&o_done[x], (uint32_t)(j & 1))));
-        if (!ok) break;
-        tc_fence_after();
-        if (leader) {
-          const uint64_t kt = kd + (uint64_t)(slot * (kPpTile >> 4) + (j & 1) * (kPpBlock * 128 >> 4));
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint64_t off = (uint64_t)((k >> 2) * (kPfBox >> 4) + 2 * (k & 3));
-            umma_f16(s_t + (uint32_t)((j & 1) * kPpBlock), qd + off, kt + off, idesc_s, k != 0);
+      } else {
+        // a lane per box: a page's rows, half their columns
+        const int j = lane >> 1, c = lane & 1;
+        auto page_at = [&](int i) {
+          const int key = (it.block0 + i) * kPpBlock + j * box_rows;
+          return i < n && j < boxes && key < it.k_end ? table[key >> p.s.page_shift] : 0;
+        };
+        int next = first_page;
+        for (int i = 0; i < n && ok; ++i) {
+          int page = next;
+          next = page_at(i + 1);
+          const int slot = i % kPpSlots, key = (it.block0 + i) * kPpBlock, keys = min(kPpBlock, it.k_end - key), used = (keys + box_rows - 1) / box_rows;
+          if (page < 0 || page >= p.s.n_pages) {
+            atomicCAS(p.err, 0, (int)DERR_POSITION);
+            page = 0;
           }
-          umma_commit(&s_full[2 * x + (j & 1)]);
-          if ((j & 1) || j + 1 == mine) umma_commit(&k_empty[slot]);
+          const int row = (page << p.s.page_shift) + (key & ((1 << p.s.page_shift) - 1) & ~(box_rows - 1));
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)((i / kPpSlots) & 1) ^ 1u));
+          if (!ok) break;
+          const bool cut = values && keys < kPpBlock;
+          uint64_t* bar = cut ? v_raw : &full[slot];
+          if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(used * box_rows) * 256u);
+          __syncwarp();
+          if (j < used) tma_load_2d(to + slot * kPpTile + c * kPpBox + j * box_rows * 128, values ? &v_map : &k_map, it.kv * kRowDim + 64 * c, row, bar);
+          __syncwarp();
+          if (cut) {                   // (the last block)
+            ok = __all_sync(0xffffffffu, mbar_wait_spin(v_raw, 0));
+            if (!ok) break;
+            uint8_t* at = to + slot * kPpTile;
+            for (int k = lane; k < 2 * (kPpBlock - keys) * 8; k += 32)       // (a row's 128 bytes of either box, whatever their order)
+              *reinterpret_cast<uint4*>(at + ((k >> 3) & 1) * kPpBox + (keys + (k >> 4)) * 128 + 16 * (k & 7)) = make_uint4(0u, 0u, 0u, 0u);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[slot]);
+            __syncwarp();
+          }
         }
-        __syncwarp();
       }
-      if (j > 0) {
-        const int h = j - 1, slot = (h >> 1) % kPpSlots;
-        ok = __all_sync(0xffffffffu, ((h & 1) || mbar_wait_spin(&v_full[slot], (uint32_t)((h >> 1) / kPpSlots & 1))) &&
-                                         mbar_wait_spin(&p_full[2 * x + (h & 1)], (uint32_t)(h >> 1 & 1)));
-        if (!ok) break;
-        tc_fence_after();
-        if (leader) {
-          const uint64_t vt = vd + (uint64_t)(slot * (kPpTile >> 4) + (h & 1) * (kPpBlock * 128 >> 4));
+      if (!ok && lane == 0) give_up(DERR_EMPTY_WAIT);
+    } else if (warp == 1 && n > 0) {
+      // ---- products: a block's scores, then the weighted values of the block before
+      const bool leader = elect_one();
+      const uint32_t idesc_s = umma_idesc_bf16(kPpBlock), idesc_o = umma_idesc_bf16(kRowDim) | (1u << 16);     // (bit 16: B is N-major)
+      const uint64_t qd = umma_desc_sw128(q_s), kd = umma_desc_sw128(k_s), vd = pp_desc_values(v_s);
+      const uint32_t o_t = tmem + 128u;
+      bool ok = __all_sync(0xffffffffu, mbar_wait_spin(q_full, 0));
+      for (int j = 0; j <= n && ok; ++j) {
+        if (j < n) {
+          const int slot = j % kPpSlots;
+          // (the scores' columns hold the weights of the block two before until its products are done)
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(&k_full[slot], (uint32_t)(j / kPpSlots & 1)) && (j < 2 || mbar_wait_spin(&o_done[j & 1], (uint32_t)((j - 2) >> 1 & 1))));
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            const uint64_t kt = kd + (uint64_t)(slot * (kPpTile >> 4));
 #pragma unroll
-          for (int k = 0; k < kPpBlock / 16; ++k)
-            umma_f16_ts(o_t, s_t + (uint32_t)((h & 1) * kPpBlock) + 8u * k, vt + (uint64_t)(k * (2048 >> 4)), idesc_o, (h | k) != 0);
-          umma_commit(&o_done[x]);
-          if ((h & 1) || j == mine) umma_commit(&v_empty[slot]);
+            for (int k = 0; k < 8; ++k)
+              umma_f16(tmem + (uint32_t)((j & 1) * kPpBlock), qd + (uint64_t)((k >> 2) * (kPfBox >> 4) + 2 * (k & 3)),
+                       kt + (uint64_t)((k >> 2) * (kPpBox >> 4) + 2 * (k & 3)), idesc_s, k != 0);
+            umma_commit(&s_full[j & 1]);
+            umma_commit(&k_empty[slot]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (j > 0) {
+          const int h = j - 1, slot = h % kPpSlots;
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(&v_full[slot], (uint32_t)(h / kPpSlots & 1)) && mbar_wait_spin(&p_full[h & 1], (uint32_t)(h >> 1 & 1)));
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            const uint64_t vt = vd + (uint64_t)(slot * (kPpTile >> 4));
+#pragma unroll
+            for (int k = 0; k < kPpBlock / 16; ++k)
+              umma_f16_ts(o_t, tmem + (uint32_t)((h & 1) * kPpBlock) + 8u * k, vt + (uint64_t)(k * (2048 >> 4)), idesc_o, (h | k) != 0);
+            umma_commit(&o_done[h & 1]);
+            umma_commit(&v_empty[slot]);
+          }
+          __syncwarp();
+        }
       }
+      if (!ok && lane == 0) give_up(DERR_FULL_WAIT);
     }
-    for (int i = (mine + 1) / 2; i < n && ok; ++i) {   // tiles that only the other row tile needs
-      const int slot = i % kPpSlots;
-      const uint32_t ph = (uint32_t)(i / kPpSlots & 1);
-      ok = __all_sync(0xffffffffu, mbar_wait_spin(&k_full[slot], ph));
-      if (ok && leader) mbar_arrive(&k_empty[slot]);
-      __syncwarp();
-      ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(&v_full[slot], ph));
-      if (ok && leader) mbar_arrive(&v_empty[slot]);
-      __syncwarp();
-    }
-    if (!ok && lane == 0) give_up(DERR_FULL_WAIT);
-  }
   } else {
     // ---- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q4 ? 200 : 208));
-    const int x = (warp - 4) >> 2, q4 = warp & 3, r = 32 * q4 + lane, mine = need[x];
-    const int at_row = x * p.per_tile + r / p.group, head = it.kv * p.group + r % p.group;       // of the item's rows
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q4 ? 152 : 168));
+    const int q4 = warp & 3, r = 32 * q4 + lane;
+    const int at_row = r / p.group, head = it.kv * p.group + r % p.group;                        // of the item's rows
     const bool live = r < p.per_tile * p.group && at_row < it.rows && it.seq >= 0;
     const int limit = live ? min(it.pos0 + at_row, p.max_len - 1) : -1;                          // the last key of this row
-    const uint32_t s_t = tmem + ((uint32_t)(32 * q4) << 16) + (uint32_t)(x * 256), o_t = s_t + 128u;
+    const uint32_t s_t = tmem + ((uint32_t)(32 * q4) << 16), o_t = s_t + 128u;
     const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
     float m = -FLT_MAX, l = 0.f;
     bool ok = true;
 #pragma unroll 1
-    for (int j = 0; j < mine && ok; ++j) {
+    for (int j = 0; j < n && ok; ++j) {
       const uint32_t b_t = s_t + (uint32_t)((j & 1) * kPpBlock);
-      ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[2 * x + (j & 1)], (uint32_t)(j >> 1 & 1)));
+      ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[j & 1], (uint32_t)(j >> 1 & 1)));
       if (!ok) break;
       tc_fence_after();
       __syncwarp();
@@ -488,7 +472,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
       pp_ask(b_t + 32u, v[1]);
       pp_landed(v[0]);
       pp_landed(v[1]);
-      const int last = limit - it.tile0 * kPfTile - j * kPpBlock;      // keys 0 .. last of the block count
+      const int last = limit - (it.block0 + j) * kPpBlock;      // keys 0 .. last of the block count
       if (!__all_sync(0xffffffffu, last >= kPpBlock - 1)) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -506,7 +490,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
       if (j == 0) {
         m = top;
       } else if (__any_sync(0xffffffffu, top > m + kPpLag)) {
-        ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[x], (uint32_t)((j - 1) & 1)));
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[(j - 1) & 1], (uint32_t)((j - 1) >> 1 & 1)));
         if (!ok) break;
         tc_fence_after();
         __syncwarp();
@@ -547,14 +531,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[2 * x + (j & 1)]);
-      if (j == 0 && warp == 4 && lane == 0) mbar_arrive(begun);
+      if (lane == 0) mbar_arrive(&p_full[j & 1]);
       __syncwarp();
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
-    // (the last scores tell of the products up to the last but two: a look at the last ones' parity would not tell them from those)
-    if (ok && mine > 1) ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[x], (uint32_t)(mine & 1)));
-    if (ok && mine) ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[x], (uint32_t)((mine - 1) & 1)));
+    if (ok && n) ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[(n - 1) & 1], (uint32_t)((n - 1) >> 1 & 1)));
     if (!ok && lane == 0) give_up(DERR_TMEM);
     tc_fence_after();
     __syncwarp();
@@ -562,12 +543,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     const size_t at = ((size_t)(live ? it.row0 + at_row : 0) * p.n_heads + head) * kRowDim;
     const size_t part_at = (size_t)blockIdx.z * p.s.rows * p.n_heads * kRowDim;
     if (parts && live && ok) *reinterpret_cast<float2*>(p.part_ml + (part_at + at) / (kRowDim / 2)) = make_float2(m, l);
-    if (ok && mine) {
+    if (ok && n) {
       const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
       float zero[4] = {0.f, 0.f, 0.f, 0.f};           // NaN if some sum is not finite
       // A row's results go over its warp's part of the queries, so that 16 lanes store 256 bytes of a row (a lane with a row of its own 5000 cycles for the
       // tile, its stores each to 32 places).
-      uint8_t* mine_s = q_s + 2 * x * kPfBox + q4 * 32 * 256;
+      uint8_t* mine_s = q_s + q4 * 32 * 256;
       const unsigned to_store = __ballot_sync(0xffffffffu, live);
       const int turns = parts ? 2 : 1;
 #pragma unroll 1
@@ -614,8 +595,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
       zero[0] += zero[1] + (zero[2] + zero[3]);
       unsigned rows = __ballot_sync(0xffffffffu, live && zero[0] != zero[0]);
       if (rows) {
-        // Keys that rows of this CTA do not see and their tiles hold: from its first position on.
-        const int first = it.tile0 * kPfTile, end = min((it.tile0 + n) * kPfTile, it.k_end);
+        // Keys that rows of this CTA do not see and their blocks hold: from its first position on.
+        const int first = it.block0 * kPpBlock, end = min((it.block0 + n) * kPpBlock, it.k_end);
         float z = 0.f;
         for (int key = max(it.pos0 + 1, first); key < end; ++key) {
           float v[4];
@@ -652,7 +633,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
   }
   __syncthreads();
   __syncwarp();                        // (the release is one instruction of the whole warp)
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  if (warp == 1) tmem_dealloc(tmem, 256);
 }
 
 // Joins the parts of a row's head, in their order: a warp, four columns a lane.
@@ -711,14 +692,14 @@ extern "C" int tq_gqa_prefill_paged(tq_ctx* ctx, const void* q_dev, const void* 
   p.err = ctx->dev_err;
   p.group = (int)(n_heads / n_kv_heads);
   p.per_tile = kPfTile / p.group;
-  // Tile pairs there may be; parts of their keys where these leave SMs idle, of four tiles or more.
-  const size_t per_pair = 2 * (size_t)p.per_tile, pairs = seq_rows_dev ? rows / per_pair + (batch < rows ? batch : rows) : rows;
-  const size_t most = (size_t)pages->table_ld * pages->page_rows, longest = max_len < most ? max_len : most, ctas = pairs * n_kv_heads;
-  TQ_REQUIRE(ctx, pairs <= 65535, "tq_gqa_prefill_paged: too many rows");
+  // Tiles there may be; parts of their keys, of eight blocks or more, where these leave SMs idle (each takes two CTAs).
+  const size_t tiles = seq_rows_dev ? rows / p.per_tile + (batch < rows ? batch : rows) : rows;
+  const size_t most = (size_t)pages->table_ld * pages->page_rows, longest = max_len < most ? max_len : most, ctas = tiles * n_kv_heads;
+  TQ_REQUIRE(ctx, tiles <= 65535, "tq_gqa_prefill_paged: too many rows");
   size_t parts = 1;
-  if (ctas < (size_t)ctx->sm_count) {
+  if (ctas < 2 * (size_t)ctx->sm_count) {
     parts = (2 * (size_t)ctx->sm_count + ctas - 1) / ctas;
-    const size_t tiles = (longest + kPfTile - 1) / kPfTile, few = tiles / 4;
+    const size_t few = longest / (8 * kPpBlock);
     parts = parts > few ? few : parts;
     parts = parts < 1 ? 1 : parts > (size_t)kPpMaxParts ? (size_t)kPpMaxParts : parts;
   }
@@ -732,14 +713,14 @@ extern "C" int tq_gqa_prefill_paged(tq_ctx* ctx, const void* q_dev, const void* 
   }
   CUtensorMap qm, km = {}, vm = {};
   const size_t row = n_kv_heads * kRowDim, cache_rows = (size_t)pages->n_pages * pages->page_rows;
-  const unsigned box = pages->page_rows < kPfTile ? (unsigned)pages->page_rows : (unsigned)kPfTile;
+  const unsigned box = pages->page_rows < kPpBlock ? (unsigned)pages->page_rows : (unsigned)kPpBlock;
   if (!encode_bf16_boxes(&qm, q_dev, kRowDim, n_heads, rows, kRowDim * 2, n_heads * kRowDim * 2, (unsigned)p.group, (unsigned)p.per_tile) ||
       (!q4 && (!encode_bf16_k64(&km, k_pages_dev, cache_rows, row, row, box) || !encode_bf16_k64(&vm, v_pages_dev, cache_rows, row, row, box))))
     return fail(ctx, TQ_ECUDA, "cuTensorMapEncodeTiled failed");
   if (int st = pages_use(ctx, pages)) return st;
   auto kern = q4 ? paged_prefill_kernel<true> : paged_prefill_kernel<false>;
   TQ_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPpSmem));
-  TQ_CUDA(ctx, launch_k(ctx, kern, dim3((unsigned)n_kv_heads, (unsigned)pairs, (unsigned)parts), dim3(kPpThreads), kPpSmem, qm, km, vm, p));
+  TQ_CUDA(ctx, launch_k(ctx, kern, dim3((unsigned)n_kv_heads, (unsigned)tiles, (unsigned)parts), dim3(kPpThreads), kPpSmem, qm, km, vm, p));
   if (parts > 1) TQ_CUDA(ctx, launch_k(ctx, paged_prefill_join_kernel, dim3((unsigned)((rows * n_heads + 3) / 4)), dim3(128), 0, p));
   return TQ_OK;
 }
