@@ -14,7 +14,7 @@
 
 namespace tq {
 
-constexpr int kQdWarps = 12, kQdChunk = 32, kQdStages = 3;
+constexpr int kQdWarps = 4, kQdCtas = 4, kQdChunk = 32, kQdStages = 2;        // warps of a CTA, CTAs of an SM
 constexpr int kQdKeyBytes = 64, kQdValueBytes = 80;    // of a row in shared memory (80: four rows' 8-byte reads meet all banks)
 constexpr int kQdStageBytes = kQdChunk * (kQdKeyBytes + kQdValueBytes + 16);
 constexpr float kQdLag = 8.f;          // a reference may be so far below its maximum (log2)
@@ -27,6 +27,7 @@ struct Q4DecodeParams {
   int n_heads, n_kv, group, max_len, n_shares;         // n_shares: warps of a KV head
   float scale_log2;
   float *o, *ml;                       // partial results [kv][batch + n_shares][group][128], [..][2]
+  int2* plan;                          // [batch] a sequence's first share, how many have a part of it
   __nv_bfloat16* out;
   int* err;
 };
@@ -46,7 +47,7 @@ __device__ __forceinline__ int q4d_len(const Q4DecodeParams& p, int b) {
 
 // SPLIT: up to four query heads of a KV head.
 template <bool SPLIT>
-__global__ void __launch_bounds__(32 * kQdWarps) q4_decode_kernel(const Q4DecodeParams p) {
+__global__ void __launch_bounds__(32 * kQdWarps, kQdCtas) q4_decode_kernel(const Q4DecodeParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   int* before = reinterpret_cast<int*>(smem + kQdWarps * kQdStages * kQdStageBytes);       // [batch + 1] chunks of the sequences before
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -75,6 +76,11 @@ __global__ void __launch_bounds__(32 * kQdWarps) q4_decode_kernel(const Q4Decode
   __syncthreads();
   const int total = before[p.s.batch], share = max(1, (total + p.n_shares - 1) / p.n_shares);
   const int w = blockIdx.x * kQdWarps + warp, c = w / p.n_kv, kv = w - c * p.n_kv;         // neighbours: the KV heads of the same rows
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b < p.s.batch; b += 32 * kQdWarps) {
+      const int f = before[b], n = before[b + 1] - f;
+      p.plan[b] = make_int2(f / share, n ? (f + n - 1) / share - f / share + 1 : 0);
+    }
   if (c >= p.n_shares) return;
   const int from = c * share, to = min(from + share, total);
   if (from >= to) return;
@@ -170,6 +176,7 @@ __global__ void __launch_bounds__(32 * kQdWarps) q4_decode_kernel(const Q4Decode
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.f;
+      float more[4] = {0.f, 0.f, 0.f, 0.f};            // (two sums: half as many products wait for one another)
       uint32_t words[2][4], sc[2], off[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -192,17 +199,21 @@ __global__ void __launch_bounds__(32 * kQdWarps) q4_decode_kernel(const Q4Decode
           for (int j = 0; j < 4; ++j) a[r][j] = bf16x2_fma(a[r][j], sc[r], off[r]);
         }
         mma_bf16_16816(s[h], a[0][0], a[1][0], a[0][1], a[1][1], q[2 * i][0], q[2 * i][1]);
-        mma_bf16_16816(s[h], a[0][2], a[1][2], a[0][3], a[1][3], q[2 * i + 1][0], q[2 * i + 1][1]);
+        mma_bf16_16816(more, a[0][2], a[1][2], a[0][3], a[1][3], q[2 * i + 1][0], q[2 * i + 1][1]);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[h][j] += more[j];
     }
     const int left = len - (f - before[b]) * kQdChunk;                 // keys of the chunk
+    if (left < kQdChunk) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[h][j] = 16 * h + 8 * (j >> 1) + g < left ? s[h][j] * p.scale_log2 : -INFINITY;
+        for (int j = 0; j < 4; ++j) s[h][j] = 16 * h + 8 * (j >> 1) + g < left ? s[h][j] : -INFINITY;
+    }
     float top[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) top[j] = fmaxf(fmaxf(s[0][j], s[0][2 + j]), fmaxf(s[1][j], s[1][2 + j]));
+    for (int j = 0; j < 2; ++j) top[j] = fmaxf(fmaxf(s[0][j], s[0][2 + j]), fmaxf(s[1][j], s[1][2 + j])) * p.scale_log2;
     if (__any_sync(0xffffffffu, first || top[0] > ref[0] + kQdLag || top[1] > ref[1] + kQdLag)) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -228,7 +239,7 @@ __global__ void __launch_bounds__(32 * kQdWarps) q4_decode_kernel(const Q4Decode
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float w0 = ex2_ftz(s[h][2 * i] - ref[0]), w1 = ex2_ftz(s[h][2 * i + 1] - ref[1]);
+        const float w0 = ex2_ftz(fmaf(s[h][2 * i], p.scale_log2, -ref[0])), w1 = ex2_ftz(fmaf(s[h][2 * i + 1], p.scale_log2, -ref[1]));
         sum[0] += w0;
         sum[1] += w1;
         uint32_t a, b2;
@@ -300,67 +311,75 @@ __global__ void __launch_bounds__(32 * kQdWarps) q4_decode_kernel(const Q4Decode
   }
 }
 
-// Joins the partial results of a query head, in the order of the chunks: a CTA, every fourth one a warp, four columns a lane.
-__global__ void __launch_bounds__(128) q4_join_kernel(const Q4DecodeParams p) {
-  __shared__ float4 part[4][32];
-  __shared__ float2 part_ml[4];
-  __shared__ int sums_s[4][2];
+// Joins the partial results of a query head, in the order of the chunks: WARPS warps, every WARPS-th result each, four columns a lane; eight of a warp's are on
+// their way at a time (one after the other: 230 of a sequence of 65537 positions took 25 us).
+template <int WARPS>
+__global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : 128) q4_join_kernel(const Q4DecodeParams p) {
+  __shared__ float4 part[WARPS][32];
+  __shared__ float2 part_ml[WARPS];
   pdl_wait();
   pdl_launch_dependents();
-  const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // chunks before the sequence, and in all
-  int lower = 0, all = 0;
-  for (int i = threadIdx.x; i < p.s.batch; i += 128) {
-    const int n = (q4d_len(p, i) + kQdChunk - 1) / kQdChunk;
-    all += n;
-    lower += i < b ? n : 0;
-  }
-  lower = __reduce_add_sync(0xffffffffu, lower);
-  all = __reduce_add_sync(0xffffffffu, all);
-  if (lane == 0) {
-    sums_s[warp][0] = lower;
-    sums_s[warp][1] = all;
-  }
-  __syncthreads();
-  lower = sums_s[0][0] + sums_s[1][0] + sums_s[2][0] + sums_s[3][0];
-  all = sums_s[0][1] + sums_s[1][1] + sums_s[2][1] + sums_s[3][1];
-  const int share = max(1, (all + p.n_shares - 1) / p.n_shares), n = (q4d_len(p, b) + kQdChunk - 1) / kQdChunk;
-  const int c0 = lower / share, pieces = n ? (lower + n - 1) / share - c0 + 1 : 0, kv = head / p.group;
-  const size_t row0 = ((size_t)kv * (p.s.batch + p.n_shares) + b + c0) * p.group + head - kv * p.group;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int i = WARPS > 1 ? blockIdx.x : 4 * blockIdx.x + warp, first = WARPS > 1 ? warp : 0;
+  if (i >= p.s.batch * p.n_heads) return;
+  const int b = i / p.n_heads, head = i - b * p.n_heads, kv = head / p.group;
+  const int2 plan = p.plan[b];
+  const size_t row0 = ((size_t)kv * (p.s.batch + p.n_shares) + b + plan.x) * p.group + head - kv * p.group;
   float top = -FLT_MAX, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = warp; i < pieces; i += 4) {
-    const size_t row = row0 + (size_t)i * p.group;
-    const float2 ml = *reinterpret_cast<const float2*>(p.ml + row * 2);
-    const float4 v = *reinterpret_cast<const float4*>(p.o + row * kRowDim + 4 * lane);
-    const float to = fmaxf(top, ml.x), f0 = ex2_ftz(top - to), f1 = ex2_ftz(ml.x - to);
-    top = to;
-    l = l * f0 + ml.y * f1;
-    o[0] = o[0] * f0 + v.x * f1;
-    o[1] = o[1] * f0 + v.y * f1;
-    o[2] = o[2] * f0 + v.z * f1;
-    o[3] = o[3] * f0 + v.w * f1;
-  }
-  part[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
-  if (lane == 0) part_ml[warp] = make_float2(top, l);
-  __syncthreads();
-  if (warp) return;
-  top = fmaxf(fmaxf(part_ml[0].x, part_ml[1].x), fmaxf(part_ml[2].x, part_ml[3].x));
-  l = o[0] = o[1] = o[2] = o[3] = 0.f;
+  for (int base = first; base < plan.y; base += 8 * WARPS) {
+    float2 ml[8];
+    float4 v[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float4 v = part[i][lane];
-    const float f = ex2_ftz(part_ml[i].x - top);
-    l += part_ml[i].y * f;
-    o[0] += v.x * f;
-    o[1] += v.y * f;
-    o[2] += v.z * f;
-    o[3] += v.w * f;
+    for (int k = 0; k < 8; ++k) {
+      const int piece = base + k * WARPS;
+      const size_t row = row0 + (size_t)piece * p.group;
+      ml[k] = make_float2(-FLT_MAX, 0.f);
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (piece < plan.y) {
+        ml[k] = *reinterpret_cast<const float2*>(p.ml + row * 2);
+        v[k] = *reinterpret_cast<const float4*>(p.o + row * kRowDim + 4 * lane);
+      }
+    }
+    float to = top;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) to = fmaxf(to, ml[k].x);
+    const float f0 = ex2_ftz(top - to);
+    top = to;
+    l *= f0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] *= f0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = ex2_ftz(ml[k].x - to);
+      l = fmaf(ml[k].y, f, l);
+      o[0] = fmaf(v[k].x, f, o[0]);
+      o[1] = fmaf(v[k].y, f, o[1]);
+      o[2] = fmaf(v[k].z, f, o[2]);
+      o[3] = fmaf(v[k].w, f, o[3]);
+    }
+  }
+  if (WARPS > 1) {
+    part[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
+    if (lane == 0) part_ml[warp] = make_float2(top, l);
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) top = fmaxf(top, part_ml[k].x);
+    l = o[0] = o[1] = o[2] = o[3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) {
+      const float4 v = part[k][lane];
+      const float f = ex2_ftz(part_ml[k].x - top);
+      l = fmaf(part_ml[k].y, f, l);
+      o[0] = fmaf(v.x, f, o[0]);
+      o[1] = fmaf(v.y, f, o[1]);
+      o[2] = fmaf(v.z, f, o[2]);
+      o[3] = fmaf(v.w, f, o[3]);
+    }
   }
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;                // (a NaN stays one)
-  uint2 w;
-  w.x = pack_bf16(o[0] * inv, o[1] * inv);
-  w.y = pack_bf16(o[2] * inv, o[3] * inv);
-  *reinterpret_cast<uint2*>(p.out + ((size_t)b * p.n_heads + head) * kRowDim + 4 * lane) = w;
+  *reinterpret_cast<uint2*>(p.out + ((size_t)b * p.n_heads + head) * kRowDim + 4 * lane) =
+      make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
 }
 
 }  // namespace tq
@@ -393,18 +412,22 @@ extern "C" int tq_gqa_decode_paged_q4(tq_ctx* ctx, const void* q_dev, const void
   p.err = ctx->dev_err;
   const size_t chunks = batch * (((size_t)p.max_len + kQdChunk - 1) / kQdChunk);
   TQ_REQUIRE(ctx, chunks < (1ull << 30), "tq_gqa_decode_paged_q4: too many positions");
-  // One CTA an SM, or as many as there may be chunks.
-  const size_t most_warps = (size_t)ctx->sm_count * kQdWarps, shares = most_warps > n_kv_heads ? most_warps / n_kv_heads : 1;
+  // All SMs' warps, or as many as there may be chunks.
+  const size_t most_warps = (size_t)ctx->sm_count * kQdCtas * kQdWarps, shares = most_warps > n_kv_heads ? most_warps / n_kv_heads : 1;
   p.n_shares = (int)(shares < chunks ? shares : chunks);
   const size_t n_ctas = (p.n_shares * n_kv_heads + kQdWarps - 1) / kQdWarps, rows = (batch + p.n_shares) * n_heads;
-  if (int st = ensure_scratch(ctx, rows * (kRowDim + 2) * sizeof(float))) return st;
+  if (int st = ensure_scratch(ctx, rows * (kRowDim + 2) * sizeof(float) + batch * sizeof(int2))) return st;
   p.o = static_cast<float*>(ctx->scratch);
   p.ml = p.o + rows * kRowDim;
+  p.plan = reinterpret_cast<int2*>(p.ml + rows * 2);
   if (int st = pages_use(ctx, pages)) return st;
   const size_t smem = kQdWarps * kQdStages * kQdStageBytes + (batch + 1) * sizeof(int), most_smem = kQdWarps * kQdStages * kQdStageBytes + (kPageCalls + 1) * sizeof(int);
   auto kern = p.group <= 4 ? q4_decode_kernel<true> : q4_decode_kernel<false>;
   TQ_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most_smem));
   TQ_CUDA(ctx, launch_k(ctx, kern, dim3((unsigned)n_ctas), dim3(32 * kQdWarps), smem, p));
-  TQ_CUDA(ctx, launch_k(ctx, q4_join_kernel, dim3((unsigned)n_heads, (unsigned)batch), dim3(128), 0, p));
+  // A warp a query head where a sequence has few parts on the average (in CTAs of four heads), sixteen where it has many.
+  const unsigned heads = (unsigned)(batch * n_heads);
+  if ((size_t)p.n_shares > 16 * batch) TQ_CUDA(ctx, launch_k(ctx, q4_join_kernel<16>, dim3(heads), dim3(512), 0, p));
+  else TQ_CUDA(ctx, launch_k(ctx, q4_join_kernel<1>, dim3((heads + 3) / 4), dim3(128), 0, p));
   return TQ_OK;
 }
