@@ -551,6 +551,7 @@ extern "C" {
     pub fn tq_llama_decode_at(model: *mut tq_llama, token_ids_dev: *const c_int, positions_dev: *const c_int, rope_positions_dev: *const c_int, batch: usize, max_len: usize, logits_dev: *mut f32) -> c_int;
     pub fn tq_llama_decode_paged(model: *mut tq_llama, token_ids_dev: *const c_int, pages: *const tq_pages, seqs_dev_or_null: *const c_int, batch: usize, group_starts_dev_or_null: *const c_int, shared_dev_or_null: *const c_int, n_groups: usize, max_shared: usize, max_len: usize, logits_dev: *mut f32) -> c_int;
     pub fn tq_llama_prefill(model: *mut tq_llama, token_ids_dev: *const c_int, cache_start_dev: *const c_int, batch: usize, q_len: usize, logits_dev: *mut f32) -> c_int;
+    pub fn tq_llama_prefill_paged(model: *mut tq_llama, token_ids_dev: *const c_int, pages: *const tq_pages, seqs_dev_or_null: *const c_int, seq_rows_dev_or_null: *const c_int, batch: usize, rows: usize, max_len: usize, logits_dev: *mut f32) -> c_int;
     pub fn tq_moe_router(ctx: *mut tq_ctx, h_bf16_dev: *const c_void, wg_bf16_dev: *const c_void, n_tokens: usize, d_model: usize, n_experts: usize, top_k: usize, renormalize: c_int, idx_out_dev: *mut c_int, weight_out_dev: *mut f32, logits_out_dev: *mut f64) -> c_int;
     pub fn tq_moe_create(ctx: *mut tq_ctx, cfg: *const tq_moe_config, wg_bf16_dev: *const c_void, w_gate_up_stacked: *const tq_qweight, w_down_stacked: *const tq_qweight, shared_gate_up: *const *const tq_qweight, shared_down: *const *const tq_qweight, out: *mut *mut tq_moe) -> c_int;
     pub fn tq_moe_destroy(moe: *mut tq_moe) -> c_int;

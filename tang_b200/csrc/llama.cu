@@ -72,6 +72,15 @@ __global__ void paged_rows_kernel(const int* tables, const int* lens, const int*
   positions[i] = pos;
 }
 
+// out[i] = x[last row of sequence i of the packed rows], zeros where it has none.
+__global__ void last_rows_kernel(const __nv_bfloat16* x, const int* seq_rows, int rows, int d, __nv_bfloat16* out) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int i = blockIdx.x, first = seq_rows ? seq_rows[i] : i, end = seq_rows ? seq_rows[i + 1] : i + 1;
+  const bool has = first >= 0 && first < end && end <= rows;
+  for (int c = threadIdx.x; c < d; c += blockDim.x) out[(size_t)i * d + c] = has ? x[(size_t)(end - 1) * d + c] : __float2bfloat16(0.f);
+}
+
 // KVCache::trim_to (crates/tang-infer/src/kv_cache.rs:138-149) for one layer's K and V caches: a sequence that
 // holds more than `keep` positions drops its OLDEST ones, i.e. rows [len - keep, len) move to [0, keep).  The move
 // is in place: each thread owns one 16-byte column of a sequence's rows and walks it front to back, eight rows at
@@ -139,6 +148,33 @@ using namespace tq;
 static int dev_alloc(tq_llama* m, void** p, size_t bytes) {
   TQ_CUDA(m->ctx, cudaMalloc(p, bytes ? bytes : 16));
   m->owned.push_back(*p);
+  return TQ_OK;
+}
+
+// The workspaces of a chunk of R rows.
+static int size_chunk(tq_llama* m, size_t R, const char* call) {
+  if (R <= m->pre_rows) return TQ_OK;
+  tq_ctx* ctx = m->ctx;
+  const tq_llama_config& c = m->cfg;
+  const size_t d = c.d_model, q_dim = (size_t)m->heads_l * c.head_dim, kv_dim = (size_t)m->kv_l * c.head_dim;
+  TQ_REQUIRE(ctx, !ctx->capturing, "%s: workspaces must be sized before graph capture (run once eagerly)", call);
+  TQ_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+  ctx->ws_generation++;   // graphs recorded over the old chunk buffers must not be replayed
+  m->pre_rows = 0;        // (until all of them are there again)
+  void** slots[] = {(void**)&m->p_h, (void**)&m->p_delta, (void**)&m->p_qkv, (void**)&m->p_gu, (void**)&m->p_xn,
+                    (void**)&m->p_qb, (void**)&m->p_attn, (void**)&m->p_act, (void**)&m->p_last};
+  const size_t bytes[] = {R * d * 4, R * d * 4, R * (q_dim + 2 * kv_dim) * 4, R * 2 * m->ffn_l * 4, R * d * 2,
+                          R * q_dim * 2, R * q_dim * 2, R * (size_t)m->ffn_l * 2, (size_t)c.max_batch * d * 2};
+  for (int i = 0; i < 9; ++i) {
+    if (*slots[i]) {
+      for (auto& o : m->owned)
+        if (o == *slots[i]) o = nullptr;
+      cudaFree(*slots[i]);
+      *slots[i] = nullptr;
+    }
+    if (int st = dev_alloc(m, slots[i], bytes[i])) return st;
+  }
+  m->pre_rows = R;
   return TQ_OK;
 }
 
@@ -386,25 +422,7 @@ int tq_llama_prefill(tq_llama* m, const int* token_ids_dev, const int* cache_sta
   const size_t R = batch * q_len, d = c.d_model, hd = c.head_dim;
   const size_t q_dim = (size_t)m->heads_l * hd, kv_dim = (size_t)m->kv_l * hd;
   const size_t seq_stride = (size_t)c.max_seq * kv_dim;
-  if (R > m->pre_rows) {   // (re)size the chunk's workspaces
-    TQ_REQUIRE(ctx, !ctx->capturing, "tq_llama_prefill: workspaces must be sized before graph capture (run once eagerly)");
-    TQ_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-    ctx->ws_generation++;   // graphs recorded over the old chunk buffers must not be replayed
-    void** slots[] = {(void**)&m->p_h, (void**)&m->p_delta, (void**)&m->p_qkv, (void**)&m->p_gu, (void**)&m->p_xn,
-                      (void**)&m->p_qb, (void**)&m->p_attn, (void**)&m->p_act, (void**)&m->p_last};
-    const size_t bytes[] = {R * d * 4, R * d * 4, R * (q_dim + 2 * kv_dim) * 4, R * 2 * m->ffn_l * 4, R * d * 2,
-                            R * q_dim * 2, R * q_dim * 2, R * (size_t)m->ffn_l * 2, (size_t)c.max_batch * d * 2};
-    for (int i = 0; i < 9; ++i) {
-      if (*slots[i]) {
-        for (auto& o : m->owned)
-          if (o == *slots[i]) o = nullptr;
-        cudaFree(*slots[i]);
-        *slots[i] = nullptr;
-      }
-      if (int st = dev_alloc(m, slots[i], bytes[i])) return st;
-    }
-    m->pre_rows = R;
-  }
+  if (int grown = size_chunk(m, R, "tq_llama_prefill")) return grown;
   int st;
 #define TQ_STEP(expr) \
   if ((st = (expr)) != TQ_OK) return st;
@@ -437,6 +455,66 @@ int tq_llama_prefill(tq_llama* m, const int* token_ids_dev, const int* cache_sta
   // the LM head only sees each sequence's last row
   TQ_CUDA(ctx, cudaMemcpy2DAsync(m->p_last, d * 2, m->p_xn + (q_len - 1) * d, q_len * d * 2, d * 2, batch, cudaMemcpyDeviceToDevice,
                                  ctx->stream));
+  if (m->tp == 1) {
+    TQ_STEP(tq_qlinear(ctx, m->lm_head, m->p_last, TQ_BF16, d, B, logits_dev, TQ_F32, c.vocab, nullptr));
+  } else {
+    TQ_STEP(tq_qlinear(ctx, m->lm_head, m->p_last, TQ_BF16, d, B, m->logits_l, TQ_F32, m->vocab_l, nullptr));
+    TQ_STEP(tq_all_gather(ctx, m->comm, m->logits_l, logits_dev, (size_t)B * m->vocab_l * sizeof(float)));
+  }
+#undef TQ_STEP
+  return TQ_OK;
+}
+
+int tq_llama_prefill_paged(tq_llama* m, const int* token_ids_dev, const tq_pages* pages, const int* seqs_dev, const int* seq_rows_dev, size_t batch,
+                           size_t rows, size_t max_len, float* logits_dev) {
+  if (!m) return TQ_EINVAL;
+  tq_ctx* ctx = m->ctx;
+  if (int st = bind(ctx)) return st;
+  const tq_llama_config& c = m->cfg;
+  TQ_REQUIRE(ctx, batch > 0 && batch <= c.max_batch, "tq_llama_prefill_paged: batch must be 1..%u", c.max_batch);
+  TQ_REQUIRE(ctx, rows > 0 && max_len > 0 && max_len <= c.max_seq, "tq_llama_prefill_paged: there must be rows, and max_len 1..max_seq");
+  TQ_REQUIRE(ctx, token_ids_dev && pages && logits_dev, "tq_llama_prefill_paged: null pointer");
+  TQ_REQUIRE(ctx, pages->ctx == ctx, "tq_llama_prefill_paged: the pool belongs to another context");
+  const size_t cache_rows = (size_t)pages->n_pages * pages->page_rows;
+  TQ_REQUIRE(ctx, cache_rows <= (size_t)c.max_batch * c.max_seq && cache_rows < (1ull << 31), "tq_llama_prefill_paged: the cache has %zu rows, the pool's pages %zu",
+             (size_t)c.max_batch * c.max_seq, cache_rows);
+  TQ_REQUIRE(ctx, m->lm_head != nullptr, "tq_llama_prefill_paged: head weights not set");
+  for (auto& L : m->layers) TQ_REQUIRE(ctx, L.wqkv != nullptr, "tq_llama_prefill_paged: a layer has no weights");
+  const size_t R = rows, d = c.d_model, hd = c.head_dim;
+  const size_t q_dim = (size_t)m->heads_l * hd, kv_dim = (size_t)m->kv_l * hd;
+  if (int grown = size_chunk(m, R, "tq_llama_prefill_paged")) return grown;
+  int st;
+#define TQ_STEP(expr) \
+  if ((st = (expr)) != TQ_OK) return st;
+  const int B = (int)batch;
+  TQ_STEP(tq_embedding(ctx, m->embed, TQ_BF16, token_ids_dev, R, d, c.vocab, m->p_h, TQ_F32));
+  bool have_delta = false;
+  for (size_t l = 0; l < m->layers.size(); ++l) {
+    const LlamaLayerW& L = m->layers[l];
+    TQ_STEP(tq_rms_norm(ctx, have_delta ? (const void*)m->p_delta : (const void*)m->p_h, TQ_F32, have_delta ? m->p_h : nullptr,
+                        L.attn_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, have_delta ? m->p_h : nullptr));
+    TQ_STEP(tq_qlinear(ctx, L.wqkv, m->p_xn, TQ_BF16, d, R, m->p_qkv, TQ_F32, q_dim + 2 * kv_dim, nullptr));
+    TQ_STEP(tq_kv_append_paged(ctx, m->p_qkv, TQ_F32, 0, m->cos_t, m->sin_t, c.max_seq, pages, seqs_dev, seq_rows_dev, batch, R, m->heads_l, m->kv_l, hd, m->p_qb,
+                               L.k_cache, L.v_cache, TQ_PAGES_BF16));
+    TQ_STEP(tq_gqa_prefill_paged(ctx, m->p_qb, L.k_cache, L.v_cache, TQ_PAGES_BF16, pages, seqs_dev, seq_rows_dev, batch, R, m->heads_l, m->kv_l, hd, max_len,
+                                 m->p_attn));
+    TQ_STEP(tq_qlinear(ctx, L.wo, m->p_attn, TQ_BF16, q_dim, R, m->p_delta, TQ_F32, d, nullptr));
+    TQ_STEP(tq_all_reduce_f32(ctx, m->comm, m->p_delta, R * d));
+    TQ_STEP(tq_rms_norm(ctx, m->p_delta, TQ_F32, m->p_h, L.ffn_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, m->p_h));
+    if (L.wgu->gate_up_interleaved) {
+      TQ_STEP(qlinear_fused(ctx, L.wgu, m->p_xn, nullptr, R, m->p_act, TQ_BF16, m->ffn_l, true, m->p_gu));
+    } else {
+      TQ_STEP(tq_qlinear(ctx, L.wgu, m->p_xn, TQ_BF16, d, R, m->p_gu, TQ_F32, 2 * (size_t)m->ffn_l, nullptr));
+      TQ_STEP(tq_swiglu(ctx, m->p_gu, m->p_gu + m->ffn_l, TQ_F32, 2 * (size_t)m->ffn_l, R, m->ffn_l, m->p_act, TQ_BF16));
+    }
+    TQ_STEP(tq_qlinear(ctx, L.wdown, m->p_act, TQ_BF16, m->ffn_l, R, m->p_delta, TQ_F32, d, nullptr));
+    TQ_STEP(tq_all_reduce_f32(ctx, m->comm, m->p_delta, R * d));
+    have_delta = true;
+  }
+  TQ_STEP(tq_rms_norm(ctx, m->p_delta, TQ_F32, m->p_h, m->final_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, m->p_h));
+  // the LM head only sees each sequence's last row
+  TQ_CUDA(ctx, launch_k(ctx, last_rows_kernel, dim3((unsigned)B), dim3(256), 0, (const __nv_bfloat16*)m->p_xn, seq_rows_dev, (int)R, (int)d,
+                        (__nv_bfloat16*)m->p_last));
   if (m->tp == 1) {
     TQ_STEP(tq_qlinear(ctx, m->lm_head, m->p_last, TQ_BF16, d, B, logits_dev, TQ_F32, c.vocab, nullptr));
   } else {

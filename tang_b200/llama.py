@@ -169,14 +169,32 @@ class LlamaModel:
         self.dev._check(self.dev._L.tq_llama_decode_paged(C.c_void_p(self.handle), ptr(token_ids), C.c_void_p(pool.handle), ptr(seqs), batch,
                                                           ptr(group_starts), ptr(shared), n_groups, max_shared, max_len, ptr(logits)))
 
+    def prefill_paged(self, token_ids: Buffer, pool: PagePool, batch: int, rows: int, max_len: int, logits: Buffer, seqs: Buffer | None = None,
+                      seq_rows: Buffer | None = None) -> None:
+        """``prefill`` over a ``page_pool`` for prompts (or portions) of different lengths, packed (``tq_llama_prefill_paged``): rows seq_rows[i] ..
+        seq_rows[i+1]-1 are the last positions of sequence seqs[i], for which ``PagePool.extend`` has made room with counts; what the sequence held before, its own or
+        forked, is attended.  Leaves the logits of each sequence's last row; asynchronous."""
+        if token_ids.n < rows or logits.n < batch * self.cfg.vocab or (seqs is not None and seqs.n < batch) or \
+                (seq_rows.n < batch + 1 if seq_rows is not None else rows != batch):
+            raise _lib.TangqError(_lib.TQ_EINVAL, "prefill_paged: buffer sizes do not match the batch")
+        _check_types("prefill_paged", _lib.I32, token_ids=token_ids, seqs=seqs, seq_rows=seq_rows)
+        _check_types("prefill_paged", _lib.F32, logits=logits)
+        ptr = lambda b: C.c_void_p(b.ptr if b is not None else 0)
+        self.dev._check(self.dev._L.tq_llama_prefill_paged(C.c_void_p(self.handle), ptr(token_ids), C.c_void_p(pool.handle), ptr(seqs), ptr(seq_rows), batch,
+                                                           rows, max_len, ptr(logits)))
+
     def sample(self, prompts, n_new: int, samples: int, sampling=None, seed: int = 42, comm_world: int = 1) -> Samples:
-        """`samples` continuations of each prompt (equal lengths), each with its log probability.  A prompt is run through the model and kept in
+        """`samples` continuations of each prompt, each with its log probability.  A prompt is run through the model and kept in
         the cache once: its samples are forked from it, share its pages and attend them as one group.  Sample j draws as ``generate`` with
-        seed + j does.  Uses the whole cache; prompts * samples are at most max_batch."""
-        prompts = np.asarray(prompts, np.int32)
+        seed + j does.  Uses the whole cache; prompts * samples are at most max_batch.  Prompts of different lengths go through ``prefill_paged``, those
+        of one length through ``prefill``."""
+        prompts = [np.asarray(p, np.int32) for p in prompts]
+        if any(p.ndim != 1 for p in prompts):
+            raise _lib.TangqError(_lib.TQ_EINVAL, "sample: every prompt is a list of tokens")
         check_lengths(prompts, n_new, self.cfg.max_seq)
         dev, c = self.dev, self.cfg
-        B, P = prompts.shape
+        before = np.array([len(p) - 1 for p in prompts], np.int32)       # tokens that are run before the first new one
+        B, P, even = len(prompts), int(before.max()) + 1, (before == before[0]).all()
         if samples < 1 or B * samples > c.max_batch:
             raise _lib.TangqError(_lib.TQ_EINVAL, f"sample: {B} prompts with {samples} samples each need a model of that many sequences")
         N, first = B * samples, np.arange(B, dtype=np.int32) * samples
@@ -184,7 +202,8 @@ class LlamaModel:
         try:
             if P > 1:
                 scratch = dev.alloc(B * c.vocab, _lib.F32)
-                self.prefill(dev.upload(np.ascontiguousarray(prompts[:, :P - 1]), _lib.I32), dev.upload(np.zeros(B, np.int32), _lib.I32), B, P - 1,
+            if P > 1 and even:
+                self.prefill(dev.upload(np.stack(prompts)[:, :P - 1], _lib.I32), dev.upload(np.zeros(B, np.int32), _lib.I32), B, P - 1,
                              scratch)
                 # the first sample of prompt i takes over the pages of the rows that prefill gave prompt i
                 refs, tables, lens = np.zeros(pool.n_pages, np.int32), np.full((N, pool.max_pages), -1, np.int32), np.zeros(N, np.int32)
@@ -195,16 +214,20 @@ class LlamaModel:
                     lens[s] = P - 1
                 for buf, v in ((pool.refs, refs), (pool.tables, tables), (pool.lens, lens)):
                     dev.upload_into(buf, v)
-                if samples > 1:
-                    pool.fork(np.repeat(first, samples - 1), [s + j for s in first for j in range(1, samples)])
+            elif P > 1:
+                pool.extend(first, counts=before)
+                self.prefill_paged(dev.upload(np.concatenate([p[:-1] for p in prompts]), _lib.I32), pool, B, int(before.sum()), P, scratch,
+                                   seqs=dev.upload(first, _lib.I32), seq_rows=dev.upload(np.concatenate([[0], np.cumsum(before)]).astype(np.int32), _lib.I32))
+            if P > 1 and samples > 1:
+                pool.fork(np.repeat(first, samples - 1), [s + j for s in first for j in range(1, samples)])
             every, starts = dev.upload(np.arange(N, dtype=np.int32), _lib.I32), dev.upload(first, _lib.I32)
-            shared = dev.upload(np.full(B, P - 1, np.int32), _lib.I32)
+            shared = dev.upload(before, _lib.I32)
 
             def step(tok, pos, logits):
                 pool.extend(every, N)
                 self.decode_paged(tok, pool, N, P + n_new, logits, group_starts=starts, shared=shared, n_groups=B, max_shared=P - 1)
 
-            tokens, logprobs = decode_loop(dev, step, np.repeat(prompts, samples, 0), n_new, c.vocab, sampling,
+            tokens, logprobs = decode_loop(dev, step, [p for p in prompts for _ in range(samples)], n_new, c.vocab, sampling,
                                            np.tile(seed + np.arange(samples, dtype=np.uint64), B), comm_world, logprobs=True)
         finally:
             dev.sync()

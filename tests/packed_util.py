@@ -35,7 +35,7 @@ def pack(x):
     out[:, :nkv * HD // 2] = u[:, :, 0] | u[:, :, 1] << 4
     bits = (s.astype(np.float32).view(np.uint32) >> 16).astype(np.uint16)
     bits[np.isnan(s)] = 0x7FC0
-    out[:, nkv * HD // 2:nkv * (HD // 2 + 8)] = bits.reshape(n, -1).view(np.uint8).reshape(n, -1)
+    out[:, nkv * HD // 2:nkv * (HD // 2 + 8)] = bits.reshape(n, nkv * 4).view(np.uint8)
     return out, (code * s[..., None]).reshape(n, nkv, HD)
 
 
