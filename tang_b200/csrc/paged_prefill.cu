@@ -4,9 +4,12 @@
 //   warp 0        queries, then blocks of keys: tensor copies page by page, or, for pages of 4 bits, codes that it turns into the same bf16 rows
 //   warp 1        issues the products: a block's S = Q K^T (both from shared memory), then O += P V of the block before (P from tensor memory, V N-major)
 //   warp 2        blocks of values, likewise; rows behind the last key are zeros (whatever a page holds there must not meet a weight of zero)
-//   warps 4..7    softmax, a thread a row
-// Tensor memory: two blocks' S / P and O, 256 columns, so that two CTAs share an SM: one's products run while the other's weights are computed, and starts and
-// ends (look-up, first copies, results: 10000 of 50000 cycles for 12 times 128 keys) are hidden.  A weight is one bf16 number, and the sum that results are
+//   warp 3        finds out what the CTA does: its own tile, then those that it takes over from CTAs of the grid that have not begun (the hardware
+//                 hands them out one by one), looked up while the tile before is worked on
+//   warps 4..7    softmax, a thread a row, and the results
+// Tensor memory: two blocks' S / P and O, 256 columns, so that two CTAs share an SM: one's products run while the other's weights are computed.  The roles go
+// from tile to tile on their own: copies and scores of the next one run while the results of this one are stored (a tile a CTA: look-up, first copies and results
+// took 10000 of 21000 cycles for 8 blocks).  A weight is one bf16 number, and the sum that results are
 // divided by is that of the numbers as they entered: a row of a few keys, where the roundings do not average out, is then nearer (the largest weight need not
 // be 1 for that, so that the reference may lag: a row's sums are rescaled only when its maximum grew by more than 2^8).
 // Few rows: a tile's keys are cut into parts, a CTA each, and a second kernel joins the results.
@@ -23,7 +26,11 @@ constexpr int kPpBlock = 64;                          // keys whose scores are c
 constexpr int kPpSlots = 2;                           // of keys, and of values: a block each
 constexpr int kPpBox = kPpBlock * 128;                // bytes of a block's 64 columns
 constexpr int kPpTile = 2 * kPpBox;
-constexpr size_t kPpSmem = 1024 + 1024 + 2 * (size_t)kPfBox + 2 * kPpSlots * (size_t)kPpTile;
+constexpr int kPpItems = 2;                            // tiles that the roles are told ahead
+constexpr int kPpAhead = 2;                            // the next tile is asked for when so many blocks of keys are still to be copied
+constexpr int kPpReaders = 7;                         // warps that are told
+constexpr int kPpStage = 32 * 64;                     // bytes of results that a warp stores at a time
+constexpr size_t kPpSmem = 1024 + 1024 + 2 * (size_t)kPfBox + 2 * kPpSlots * (size_t)kPpTile + 4 * (size_t)kPpStage;
 constexpr float kPpLag = 8.f;                         // a reference may be so far below its row's maximum (log2)
 constexpr int kPpMaxParts = 16;
 constexpr int kPpPoly = 4;                            // one of so many pairs of weights is a polynomial
@@ -82,7 +89,7 @@ __device__ __forceinline__ void attend_paged_row(const PackedPrefillParams& p, i
 
 // What a CTA does.
 struct PpItem {
-  int seq, kv;                         // of the pool (-1: nothing), KV head
+  int seq, kv, part;                   // of the pool (-1: there is no more), KV head, part of the keys
   int row0, rows;                      // first packed row, rows
   int pos0;                            // position of the first row
   int block0, blocks;                  // blocks of keys: the part's first, how many
@@ -90,7 +97,7 @@ struct PpItem {
 };
 // Tile x of all sequences, the longest of each sequence first, by one warp.
 __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, int kv, int part, int lane) {
-  PpItem it{-1, kv, 0, 0, 0, 0, 0, 0};
+  PpItem it{-1, kv, part, 0, 0, 0, 0, 0, 0};
   int i = -1, first = 0, count = 0, tile = 0, s = -1, len = 0;
   if (!p.s.seq_rows) {
     if (x < p.s.batch) {
@@ -236,29 +243,64 @@ __device__ __forceinline__ uint64_t pp_desc_values(const void* smem_ptr) {
   return (uint64_t)((smem_u32(smem_ptr) >> 4) & 0x3FFF) | (uint64_t)(kPpBox >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
+// Asks for a CTA of this grid that has not begun: its place is then the asking CTA's to do, and it never begins.  The answer lands in 16 bytes of shared memory.
+__device__ __forceinline__ void ask_for_cta(uint32_t answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool answered_cta(uint32_t answer, int& x, int& y, int& z) {
+  uint32_t ok, a = 0, b = 0, c = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%4];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, r;\n\t}"
+      : "=r"(ok), "+r"(a), "+r"(b), "+r"(c)
+      : "r"(answer)
+      : "memory");
+  x = (int)a, y = (int)b, z = (int)c;
+  return ok != 0;
+}
+
 template <bool Q4>
 __global__ void __launch_bounds__(kPpThreads, 2)
 paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                      const __grid_constant__ PackedPrefillParams p) {
   extern __shared__ uint8_t smem_raw[];
+  // (phases run on from tile to tile: block R of all that the CTA does uses slots and columns R & 1)
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem_raw);
-  uint64_t* k_full = q_full + 1;                      // [slots]
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* k_full = q_empty + 1;                     // [slots]
   uint64_t* k_empty = k_full + kPpSlots;
   uint64_t* v_full = k_empty + kPpSlots;
   uint64_t* v_empty = v_full + kPpSlots;
-  uint64_t* v_raw = v_empty + kPpSlots;               // the last block's values, before the rows behind the last key are zeroed
+  uint64_t* v_raw = v_empty + kPpSlots;               // a last block's values, before the rows behind the last key are zeroed
   uint64_t* s_full = v_raw + 1;                       // [parity of the block]
   uint64_t* p_full = s_full + 2;                      // likewise
   uint64_t* o_done = p_full + 2;                      // likewise: whoever waits for a block's products has seen those of the block two before
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+  uint64_t* o_free = o_done + 2;                      // a tile's sums have been read
+  uint64_t* item_full = o_free + 1;                   // [items]
+  uint64_t* item_empty = item_full + kPpItems;
+  uint64_t* answer_bar = item_empty + kPpItems;
+  uint64_t* nearly = answer_bar + 1;                  // a tile's last keys but a few have been asked for
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(nearly + 1);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
   PpItem* item_s = reinterpret_cast<PpItem*>(smem_raw + 512);
+  const uint32_t answer = smem_u32(smem_raw) + 768;
   uint8_t* q_s = smem_raw + 1024 + ((1024 - ((smem_u32(smem_raw) + 1024) & 1023)) & 1023);
-  uint8_t *k_s = q_s + 2 * kPfBox, *v_s = k_s + kPpSlots * kPpTile;
+  uint8_t *k_s = q_s + 2 * kPfBox, *v_s = k_s + kPpSlots * kPpTile, *stage_s = v_s + kPpSlots * kPpTile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
     if (lane == 0) {
       mbar_init(q_full, 1);
+      mbar_init(q_empty, 1);
+      mbar_init(o_free, 4);
+      mbar_init(answer_bar, 1);
+      mbar_init(nearly, 1);
+      for (int i = 0; i < kPpItems; ++i) {
+        mbar_init(&item_full[i], 1);
+        mbar_init(&item_empty[i], kPpReaders);
+      }
       for (int s = 0; s < kPpSlots; ++s) {
         mbar_init(&k_full[s], 1);
         mbar_init(&k_empty[s], 1);
@@ -286,184 +328,246 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
   tc_fence_before();
   pdl_wait();
   pdl_launch_dependents();
-  // The loaders look up for themselves what the CTA does, and ask for their first pages; the queries are on their way before the others know.
-  const int box_rows = min(1 << p.s.page_shift, kPpBlock), boxes = kPpBlock / box_rows;
-  int first_page = 0;
-  if (warp == 0 || warp == 2) {
-    const PpItem mine = pp_item(p, blockIdx.y, blockIdx.x, blockIdx.z, lane);
-    if (warp == 2 && lane == 0) *item_s = mine;
-    if (mine.seq >= 0 && mine.blocks > 0) {
-      if (warp == 0) {
-        if (lane == 0) mbar_arrive_expect_tx(q_full, 2u * p.per_tile * p.group * 128u);
-        __syncwarp();
-        if (lane < 2) tma_load_3d(q_s + lane * kPfBox, &q_map, 64 * lane, mine.kv * p.group, mine.row0, q_full);
-      }
-      const int key = mine.block0 * kPpBlock + (Q4 ? lane : (lane >> 1) * box_rows);
-      if ((Q4 || (lane >> 1) < boxes) && key < mine.k_end) first_page = p.s.tables[(size_t)mine.seq * p.s.table_ld + (key >> p.s.page_shift)];
-    }
-    __syncwarp();
-  }
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const PpItem it = *item_s;
   auto give_up = [&](int code) {
     atomicCAS(p.err, 0, code);
     *failed = 1;
   };
-  const int n = it.seq < 0 ? 0 : it.blocks;
+  // One arrival for the warp, whose lanes meet before it and behind it.
+  auto arrive = [&](uint64_t* bar) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+    __syncwarp();
+  };
+  int told = 0;                        // tiles that the warp has been told
+  auto take = [&](bool& ok, PpItem& it) {
+    const int slot = told % kPpItems;
+    ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(&item_full[slot], (uint32_t)(told / kPpItems & 1)));
+    if (ok) it = item_s[slot];
+    else it.seq = -1;
+    arrive(&item_empty[slot]);
+    ++told;
+    return it.seq >= 0;
+  };
 
   // (registers: 256 threads of 128 at the start, then 128 of 88 or 104 and 128 of 168 or 152, the same in all)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q4 ? 104 : 88));
+    if (warp == 3) {
+      // ---- what to do
+      bool ok = true;
+      int x = blockIdx.x, y = blockIdx.y, z = blockIdx.z;
+      for (int asked = 0;; ++asked) {
+        const PpItem it = pp_item(p, y, x, z, lane);
+        if (it.seq >= 0 && (it.blocks > 0 || p.parts > 1)) {
+          const int slot = told % kPpItems;
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(&item_empty[slot], (uint32_t)(told / kPpItems & 1) ^ 1u));
+          if (lane == 0) item_s[slot] = it;
+          arrive(&item_full[slot]);
+          // (not earlier: CTAs that are just being started elsewhere would be taken, and a long tile's CTA would hold the next one)
+          ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(nearly, (uint32_t)(told & 1)));
+          ++told;
+        }
+        if (ok && lane == 0) {
+          mbar_arrive_expect_tx(answer_bar, 16);
+          ask_for_cta(answer, answer_bar);
+        }
+        __syncwarp();
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(answer_bar, (uint32_t)(asked & 1)));
+        if (!ok || !answered_cta(answer, x, y, z)) break;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // (the answer has been read before the next one is written)
+        __syncwarp();
+      }
+      const int slot = told % kPpItems;                // the end
+      ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(&item_empty[slot], (uint32_t)(told / kPpItems & 1) ^ 1u));
+      if (lane == 0) item_s[slot].seq = -1;
+      arrive(&item_full[slot]);
+      if (!ok && lane == 0) give_up(DERR_EMPTY_WAIT);
+    }
     if (warp == 0 || warp == 2) {
-      // ---- blocks of keys, blocks of values
+      // ---- blocks of keys (and queries), blocks of values
       const bool values = warp == 2;
       uint64_t *full = values ? v_full : k_full, *empty = values ? v_empty : k_empty;
       uint8_t* to = values ? v_s : k_s;
+      const int box_rows = min(1 << p.s.page_shift, kPpBlock), boxes = kPpBlock / box_rows;
       bool ok = true;
-      const int* table = p.s.tables + (size_t)max(it.seq, 0) * p.s.table_ld;
-      if constexpr (Q4) {
-        const uint8_t* from = (values ? p.v : p.k) + it.kv * kQ4HeadBytes;
-        const int steps = 2 * n, key0 = it.block0 * kPpBlock + lane, scales = p.n_kv * kQ4HeadBytes - it.kv * kQ4HeadBytes + it.kv * 2 * kQ4HeadScales;
-        auto page_at = [&](int m) {    // of key `lane` of step m
-          const int key = key0 + 32 * m;
-          return m < steps && key < it.k_end ? table[key >> p.s.page_shift] : 0;
-        };
-        auto codes_at = [&](int m, int page) {
-          PpCodes x;
-          const int key = key0 + 32 * m;
-          if (m < steps && key < it.k_end) {
+      int run = 0, tiles = 0, cuts = 0;                // blocks, tiles with keys, and last blocks with rows to zero so far
+      PpItem it;
+      while (take(ok, it)) {
+        const int n = it.blocks, call = max(n - kPpAhead, 0);
+        if (n == 0) {
+          if (!values) arrive(nearly);
+          continue;
+        }
+        const int* table = p.s.tables + (size_t)it.seq * p.s.table_ld;
+        if (!values) {
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(q_empty, (uint32_t)(tiles & 1) ^ 1u));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(q_full, 2u * p.per_tile * p.group * 128u);
+          __syncwarp();
+          if (lane < 2) tma_load_3d(q_s + lane * kPfBox, &q_map, 64 * lane, it.kv * p.group, it.row0, q_full);
+          __syncwarp();
+          ++tiles;
+        }
+        if constexpr (Q4) {
+          const uint8_t* from = (values ? p.v : p.k) + it.kv * kQ4HeadBytes;
+          const int steps = 2 * n, key0 = it.block0 * kPpBlock + lane, scales = p.n_kv * kQ4HeadBytes - it.kv * kQ4HeadBytes + it.kv * 2 * kQ4HeadScales;
+          auto page_at = [&](int m) {  // of key `lane` of step m
+            const int key = key0 + 32 * m;
+            return m < steps && key < it.k_end ? table[key >> p.s.page_shift] : 0;
+          };
+          auto codes_at = [&](int m, int page) {
+            PpCodes x;
+            const int key = key0 + 32 * m;
+            if (m < steps && key < it.k_end) {
+              if (page < 0 || page >= p.s.n_pages) {
+                atomicCAS(p.err, 0, (int)DERR_POSITION);
+                page = 0;
+              }
+              const uint8_t* row = from + ((size_t)(page << p.s.page_shift) + (key & ((1 << p.s.page_shift) - 1))) * p.row_bytes;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x.w[i] = *reinterpret_cast<const uint4*>(row + 16 * i);
+              x.s = *reinterpret_cast<const uint2*>(row + scales);
+            } else {                   // rows of zeros
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x.w[i] = make_uint4(0u, 0u, 0u, 0u);
+              x.s = make_uint2(0u, 0u);
+            }
+            return x;
+          };
+          PpCodes next = codes_at(0, page_at(0));
+          int page = page_at(1);
+          for (int i = 0; i < n && ok; ++i, ++run) {
+            const int slot = run % kPpSlots;
+            ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)(run / kPpSlots & 1) ^ 1u));
+            if (!ok) break;
+#pragma unroll 1
+            for (int u = 0; u < 2; ++u) {
+              const PpCodes x = next;
+              next = codes_at(2 * i + u + 1, page);
+              page = page_at(2 * i + u + 2);
+              pp_convert(to + slot * kPpTile, 32 * u + lane, x);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive(&full[slot]);
+            if (!values && i == call) arrive(nearly);
+          }
+        } else {
+          // a lane per box: a page's rows, half their columns
+          const int j = lane >> 1, c = lane & 1;
+          auto page_at = [&](int i) {
+            const int key = (it.block0 + i) * kPpBlock + j * box_rows;
+            return i < n && j < boxes && key < it.k_end ? table[key >> p.s.page_shift] : 0;
+          };
+          int next = page_at(0);
+          for (int i = 0; i < n && ok; ++i, ++run) {
+            int page = next;
+            next = page_at(i + 1);
+            const int slot = run % kPpSlots, key = (it.block0 + i) * kPpBlock, keys = min(kPpBlock, it.k_end - key), used = (keys + box_rows - 1) / box_rows;
             if (page < 0 || page >= p.s.n_pages) {
               atomicCAS(p.err, 0, (int)DERR_POSITION);
               page = 0;
             }
-            const uint8_t* row = from + ((size_t)(page << p.s.page_shift) + (key & ((1 << p.s.page_shift) - 1))) * p.row_bytes;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x.w[i] = *reinterpret_cast<const uint4*>(row + 16 * i);
-            x.s = *reinterpret_cast<const uint2*>(row + scales);
-          } else {                     // rows of zeros
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x.w[i] = make_uint4(0u, 0u, 0u, 0u);
-            x.s = make_uint2(0u, 0u);
-          }
-          return x;
-        };
-        PpCodes next = codes_at(0, first_page);
-        int page = page_at(1);
-        for (int i = 0; i < n && ok; ++i) {
-          const int slot = i % kPpSlots;
-          ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)((i / kPpSlots) & 1) ^ 1u));
-          if (!ok) break;
-#pragma unroll 1
-          for (int u = 0; u < 2; ++u) {
-            const PpCodes x = next;
-            next = codes_at(2 * i + u + 1, page);
-            page = page_at(2 * i + u + 2);
-            pp_convert(to + slot * kPpTile, 32 * u + lane, x);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[slot]);
-          __syncwarp();
-        }
-      } else {
-        // a lane per box: a page's rows, half their columns
-        const int j = lane >> 1, c = lane & 1;
-        auto page_at = [&](int i) {
-          const int key = (it.block0 + i) * kPpBlock + j * box_rows;
-          return i < n && j < boxes && key < it.k_end ? table[key >> p.s.page_shift] : 0;
-        };
-        int next = first_page;
-        for (int i = 0; i < n && ok; ++i) {
-          int page = next;
-          next = page_at(i + 1);
-          const int slot = i % kPpSlots, key = (it.block0 + i) * kPpBlock, keys = min(kPpBlock, it.k_end - key), used = (keys + box_rows - 1) / box_rows;
-          if (page < 0 || page >= p.s.n_pages) {
-            atomicCAS(p.err, 0, (int)DERR_POSITION);
-            page = 0;
-          }
-          const int row = (page << p.s.page_shift) + (key & ((1 << p.s.page_shift) - 1) & ~(box_rows - 1));
-          ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)((i / kPpSlots) & 1) ^ 1u));
-          if (!ok) break;
-          const bool cut = values && keys < kPpBlock;
-          uint64_t* bar = cut ? v_raw : &full[slot];
-          if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(used * box_rows) * 256u);
-          __syncwarp();
-          if (j < used) tma_load_2d(to + slot * kPpTile + c * kPpBox + j * box_rows * 128, values ? &v_map : &k_map, it.kv * kRowDim + 64 * c, row, bar);
-          __syncwarp();
-          if (cut) {                   // (the last block)
-            ok = __all_sync(0xffffffffu, mbar_wait_spin(v_raw, 0));
+            const int row = (page << p.s.page_shift) + (key & ((1 << p.s.page_shift) - 1) & ~(box_rows - 1));
+            ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)(run / kPpSlots & 1) ^ 1u));
             if (!ok) break;
-            uint8_t* at = to + slot * kPpTile;
-            for (int k = lane; k < 2 * (kPpBlock - keys) * 8; k += 32)       // (a row's 128 bytes of either box, whatever their order)
-              *reinterpret_cast<uint4*>(at + ((k >> 3) & 1) * kPpBox + (keys + (k >> 4)) * 128 + 16 * (k & 7)) = make_uint4(0u, 0u, 0u, 0u);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            const bool cut = values && keys < kPpBlock;
+            uint64_t* bar = cut ? v_raw : &full[slot];
+            if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(used * box_rows) * 256u);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&full[slot]);
+            if (j < used) tma_load_2d(to + slot * kPpTile + c * kPpBox + j * box_rows * 128, values ? &v_map : &k_map, it.kv * kRowDim + 64 * c, row, bar);
             __syncwarp();
+            if (!values && i == call) arrive(nearly);
+            if (cut) {                 // (the tile's last block)
+              ok = __all_sync(0xffffffffu, mbar_wait_spin(v_raw, (uint32_t)(cuts++ & 1)));
+              if (!ok) break;
+              uint8_t* at = to + slot * kPpTile;
+              for (int k = lane; k < 2 * (kPpBlock - keys) * 8; k += 32)     // (a row's 128 bytes of either box, whatever their order)
+                *reinterpret_cast<uint4*>(at + ((k >> 3) & 1) * kPpBox + (keys + (k >> 4)) * 128 + 16 * (k & 7)) = make_uint4(0u, 0u, 0u, 0u);
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              arrive(&full[slot]);
+            }
           }
         }
       }
       if (!ok && lane == 0) give_up(DERR_EMPTY_WAIT);
-    } else if (warp == 1 && n > 0) {
+    } else if (warp == 1) {
       // ---- products: a block's scores, then the weighted values of the block before
       const bool leader = elect_one();
       const uint32_t idesc_s = umma_idesc_bf16(kPpBlock), idesc_o = umma_idesc_bf16(kRowDim) | (1u << 16);     // (bit 16: B is N-major)
       const uint64_t qd = umma_desc_sw128(q_s), kd = umma_desc_sw128(k_s), vd = pp_desc_values(v_s);
       const uint32_t o_t = tmem + 128u;
-      bool ok = __all_sync(0xffffffffu, mbar_wait_spin(q_full, 0));
-      for (int j = 0; j <= n && ok; ++j) {
-        if (j < n) {
-          const int slot = j % kPpSlots;
-          // (the scores' columns hold the weights of the block two before until its products are done)
-          ok = __all_sync(0xffffffffu, mbar_wait_spin(&k_full[slot], (uint32_t)(j / kPpSlots & 1)) && (j < 2 || mbar_wait_spin(&o_done[j & 1], (uint32_t)((j - 2) >> 1 & 1))));
-          if (!ok) break;
-          tc_fence_after();
-          if (leader) {
-            const uint64_t kt = kd + (uint64_t)(slot * (kPpTile >> 4));
+      bool ok = true;
+      int run = 0, tiles = 0;          // blocks and tiles with keys before this one
+      PpItem it;
+      while (take(ok, it)) {
+        const int n = it.blocks;
+        if (n == 0) continue;
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(q_full, (uint32_t)(tiles & 1)));
+        for (int j = 0; j <= n && ok; ++j) {
+          if (j < n) {
+            const int r = run + j, slot = r % kPpSlots;
+            // (the scores' columns hold the weights of the block two before until its products are done)
+            ok = __all_sync(0xffffffffu, mbar_wait_spin(&k_full[slot], (uint32_t)(r / kPpSlots & 1)) &&
+                                             (r < 2 || mbar_wait_spin(&o_done[r & 1], (uint32_t)((r - 2) >> 1 & 1))));
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
+              const uint64_t kt = kd + (uint64_t)(slot * (kPpTile >> 4));
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              umma_f16(tmem + (uint32_t)((j & 1) * kPpBlock), qd + (uint64_t)((k >> 2) * (kPfBox >> 4) + 2 * (k & 3)),
-                       kt + (uint64_t)((k >> 2) * (kPpBox >> 4) + 2 * (k & 3)), idesc_s, k != 0);
-            umma_commit(&s_full[j & 1]);
-            umma_commit(&k_empty[slot]);
+              for (int k = 0; k < 8; ++k)
+                umma_f16(tmem + (uint32_t)((r & 1) * kPpBlock), qd + (uint64_t)((k >> 2) * (kPfBox >> 4) + 2 * (k & 3)),
+                         kt + (uint64_t)((k >> 2) * (kPpBox >> 4) + 2 * (k & 3)), idesc_s, k != 0);
+              umma_commit(&s_full[r & 1]);
+              umma_commit(&k_empty[slot]);
+              if (j + 1 == n) umma_commit(q_empty);
+            }
+            __syncwarp();
           }
-          __syncwarp();
-        }
-        if (j > 0) {
-          const int h = j - 1, slot = h % kPpSlots;
-          ok = __all_sync(0xffffffffu, mbar_wait_spin(&v_full[slot], (uint32_t)(h / kPpSlots & 1)) && mbar_wait_spin(&p_full[h & 1], (uint32_t)(h >> 1 & 1)));
-          if (!ok) break;
-          tc_fence_after();
-          if (leader) {
-            const uint64_t vt = vd + (uint64_t)(slot * (kPpTile >> 4));
+          if (j > 0) {
+            const int r = run + j - 1, slot = r % kPpSlots;
+            ok = __all_sync(0xffffffffu, mbar_wait_spin(&v_full[slot], (uint32_t)(r / kPpSlots & 1)) && mbar_wait_spin(&p_full[r & 1], (uint32_t)(r >> 1 & 1)) &&
+                                             (j > 1 || tiles == 0 || mbar_wait_spin(o_free, (uint32_t)((tiles - 1) & 1))));
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
+              const uint64_t vt = vd + (uint64_t)(slot * (kPpTile >> 4));
 #pragma unroll
-            for (int k = 0; k < kPpBlock / 16; ++k)
-              umma_f16_ts(o_t, tmem + (uint32_t)((h & 1) * kPpBlock) + 8u * k, vt + (uint64_t)(k * (2048 >> 4)), idesc_o, (h | k) != 0);
-            umma_commit(&o_done[h & 1]);
-            umma_commit(&v_empty[slot]);
+              for (int k = 0; k < kPpBlock / 16; ++k)
+                umma_f16_ts(o_t, tmem + (uint32_t)((r & 1) * kPpBlock) + 8u * k, vt + (uint64_t)(k * (2048 >> 4)), idesc_o, ((j - 1) | k) != 0);
+              umma_commit(&o_done[r & 1]);
+              umma_commit(&v_empty[slot]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
+        run += n;
+        ++tiles;
       }
       if (!ok && lane == 0) give_up(DERR_FULL_WAIT);
     }
   } else {
     // ---- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q4 ? 152 : 168));
-    const int q4 = warp & 3, r = 32 * q4 + lane;
-    const int at_row = r / p.group, head = it.kv * p.group + r % p.group;                        // of the item's rows
-    const bool live = r < p.per_tile * p.group && at_row < it.rows && it.seq >= 0;
-    const int limit = live ? min(it.pos0 + at_row, p.max_len - 1) : -1;                          // the last key of this row
+    const int q4 = warp & 3, r = 32 * q4 + lane, r_pos = r / p.group, r_head = r - r_pos * p.group;
     const uint32_t s_t = tmem + ((uint32_t)(32 * q4) << 16), o_t = s_t + 128u;
     const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
-    float m = -FLT_MAX, l = 0.f;
+    const bool parts = p.parts > 1;
+    uint8_t* mine_s = stage_s + q4 * kPpStage;
     bool ok = true;
+    int run = 0;                       // blocks before this tile
+    PpItem it;
+    while (take(ok, it)) {
+    const int n = it.blocks, head = it.kv * p.group + r_head;
+    const bool live = r_pos < min(p.per_tile, it.rows);
+    const int limit = live ? min(it.pos0 + r_pos, p.max_len - 1) : -1;                           // the last key of this row
+    float m = -FLT_MAX, l = 0.f;
 #pragma unroll 1
     for (int j = 0; j < n && ok; ++j) {
-      const uint32_t b_t = s_t + (uint32_t)((j & 1) * kPpBlock);
-      ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[j & 1], (uint32_t)(j >> 1 & 1)));
+      const uint32_t b_t = s_t + (uint32_t)(((run + j) & 1) * kPpBlock);
+      ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[(run + j) & 1], (uint32_t)((run + j) >> 1 & 1)));
       if (!ok) break;
       tc_fence_after();
       __syncwarp();
@@ -490,7 +594,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
       if (j == 0) {
         m = top;
       } else if (__any_sync(0xffffffffu, top > m + kPpLag)) {
-        ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[(j - 1) & 1], (uint32_t)((j - 1) >> 1 & 1)));
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[(run + j - 1) & 1], (uint32_t)((run + j - 1) >> 1 & 1)));
         if (!ok) break;
         tc_fence_after();
         __syncwarp();
@@ -530,67 +634,69 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
       }
       tmem_st_wait();
       tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[j & 1]);
-      __syncwarp();
+      arrive(&p_full[(run + j) & 1]);
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
-    if (ok && n) ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[(n - 1) & 1], (uint32_t)((n - 1) >> 1 & 1)));
-    if (!ok && lane == 0) give_up(DERR_TMEM);
+    if (ok && n) ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[(run + n - 1) & 1], (uint32_t)((run + n - 1) >> 1 & 1)));
+    if (!ok) break;
+    run += n;
     tc_fence_after();
     __syncwarp();
-    const bool parts = p.parts > 1;
-    const size_t at = ((size_t)(live ? it.row0 + at_row : 0) * p.n_heads + head) * kRowDim;
-    const size_t part_at = (size_t)blockIdx.z * p.s.rows * p.n_heads * kRowDim;
-    if (parts && live && ok) *reinterpret_cast<float2*>(p.part_ml + (part_at + at) / (kRowDim / 2)) = make_float2(m, l);
-    if (ok && n) {
+    const size_t at = ((size_t)(live ? it.row0 + r_pos : 0) * p.n_heads + head) * kRowDim;
+    const size_t part_at = (size_t)it.part * p.s.rows * p.n_heads * kRowDim;
+    if (parts && live) *reinterpret_cast<float2*>(p.part_ml + (part_at + at) / (kRowDim / 2)) = make_float2(m, l);
+    if (n) {
       const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
       float zero[4] = {0.f, 0.f, 0.f, 0.f};           // NaN if some sum is not finite
-      // A row's results go over its warp's part of the queries, so that 16 lanes store 256 bytes of a row (a lane with a row of its own 5000 cycles for the
-      // tile, its stores each to 32 places).
-      uint8_t* mine_s = q_s + q4 * 32 * 256;
+      // Rows go over shared memory 64 bytes at a time, so that four lanes store what stands together (a lane with a row of its own would store to 32 places at once).
       const unsigned to_store = __ballot_sync(0xffffffffu, live);
-      const int turns = parts ? 2 : 1;
+      const int columns = parts ? 16 : 32;
+      uint8_t* base = parts ? reinterpret_cast<uint8_t*>(p.part_o + part_at) : reinterpret_cast<uint8_t*>(p.out);
+      const unsigned long long row_bytes_at = (unsigned long long)at * (parts ? 4 : 2);
+      unsigned long long to[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, row_bytes_at, 8 * k + (lane >> 2)) + 16 * (lane & 3);
 #pragma unroll 1
-      for (int turn = 0; turn < turns; ++turn) {
-#pragma unroll 1
-        for (int c = 0; c < kRowDim / turns; c += 32) {
-          float o[32];
-          __syncwarp();
-          pp_ask(o_t + (uint32_t)(turn * (kRowDim / 2) + c), o);
-          pp_landed(o);
+      for (int c = 0; c < kRowDim; c += 32) {
+        float o[32];
+        __syncwarp();
+        pp_ask(o_t + (uint32_t)c, o);
+        pp_landed(o);
+        if (c == kRowDim - 32) {       // (the next tile's products may begin)
+          tc_fence_before();
+          arrive(o_free);
+        }
 #pragma unroll
-          for (int k = 0; k < 32; ++k) zero[k & 3] = fmaf(o[k], 0.f, zero[k & 3]);
-          if (parts) {
+        for (int k = 0; k < 32; ++k) zero[k & 3] = fmaf(o[k], 0.f, zero[k & 3]);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              *reinterpret_cast<float4*>(mine_s + lane * 256 + (((c / 4 + k) ^ (lane & 15)) << 4)) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-          } else {
+        for (int half = 0; half < 2; ++half) {
+          if (half && !parts) break;
+          uint8_t* row = mine_s + lane * 64;
+          const int turn = (lane >> 1) & 3;            // (eight lanes' 16 bytes meet all banks)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<uint4*>(mine_s + lane * 256 + (((c / 8 + k) ^ (lane & 15)) << 4)) =
-                  make_uint4(pack_bf16(o[8 * k] * inv, o[8 * k + 1] * inv), pack_bf16(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+          for (int k = 0; k < 4; ++k) {
+            uint4 y;
+            if (parts) {
+              y = make_uint4(__float_as_uint(half ? o[16 + 4 * k] : o[4 * k]), __float_as_uint(half ? o[17 + 4 * k] : o[4 * k + 1]),
+                             __float_as_uint(half ? o[18 + 4 * k] : o[4 * k + 2]), __float_as_uint(half ? o[19 + 4 * k] : o[4 * k + 3]));
+            } else {
+              y = make_uint4(pack_bf16(o[8 * k] * inv, o[8 * k + 1] * inv), pack_bf16(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
                              pack_bf16(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack_bf16(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+            }
+            *reinterpret_cast<uint4*>(row + ((k ^ turn) << 4)) = y;
           }
+          __syncwarp();
+          uint4 y[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int from = 8 * k + (lane >> 2);
+            y[k] = *reinterpret_cast<const uint4*>(mine_s + from * 64 + (((lane & 3) ^ ((from >> 1) & 3)) << 4));
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (to_store >> (8 * k + (lane >> 2)) & 1u) *reinterpret_cast<uint4*>(base + to[k] + (c + 16 * half) / columns * 64) = y[k];
+          __syncwarp();
         }
-        __syncwarp();
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {         // (all loads of a half before its stores)
-          uint4 y[8];
-          unsigned long long to[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int row = 16 * half + 2 * k + (lane >> 4);
-            to[k] = __shfl_sync(0xffffffffu, (unsigned long long)at, row);
-            y[k] = *reinterpret_cast<const uint4*>(mine_s + row * 256 + (((lane & 15) ^ (row & 15)) << 4));
-          }
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            uint4* dst = parts ? reinterpret_cast<uint4*>(p.part_o + part_at + to[k] + turn * (kRowDim / 2)) : reinterpret_cast<uint4*>(p.out + to[k]);
-            if (to_store >> (16 * half + 2 * k + (lane >> 4)) & 1u) dst[lane & 15] = y[k];
-          }
-        }
-        __syncwarp();
       }
       zero[0] += zero[1] + (zero[2] + zero[3]);
       unsigned rows = __ballot_sync(0xffffffffu, live && zero[0] != zero[0]);
@@ -624,6 +730,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
         }
       }
     }
+    }
+    if (!ok && lane == 0) give_up(DERR_TMEM);
   }
   tc_fence_before();
   __syncthreads();
