@@ -65,25 +65,42 @@ __device__ __forceinline__ void row_values(const uint8_t* row, int n_kv, int hea
   }
 }
 
-// One row's softmax attention over keys first .. end - 1 by a warp, key by key, for the rows of a tile that met, with a weight of zero, a value of a key that
-// they do not see and that is no number: zero times that is NaN.  Lane i has values 4 i .. of the query and of the sums.
+// One row's softmax attention over keys first .. end - 1 (first a multiple of 4) by a warp, four keys at a time, for the rows of a tile that met, with a weight of
+// zero, a value of a key that they do not see and that is no number: zero times that is NaN.  Lane i has values 4 i .. of the query and of the sums.
 template <bool Q4>
 __device__ __forceinline__ void attend_paged_row(const PackedPrefillParams& p, int seq, int kv, int first, int end, const float (&q)[4], int lane, float& top, float& l,
-                                              float (&acc)[4]) {
+                                                 float (&acc)[4]) {
 #pragma unroll 1
-  for (int j = first; j < end; ++j) {
-    const int place = max(page_row_of(p.s, seq, j), 0);
-    float k[4], v[4], s = 0.f;
-    row_values<Q4>(p.k + (size_t)place * p.row_bytes, p.n_kv, kv, lane, k);
-    row_values<Q4>(p.v + (size_t)place * p.row_bytes, p.n_kv, kv, lane, v);
+  for (int j0 = first; j0 < end; j0 += 4) {            // (of one page: pages have 16 rows or more)
+    const int place = max(page_row_of(p.s, seq, j0), 0);
+    float s[4], v[4][4], mn = top;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s = fmaf(q[i], k[i], s);
-    s = warp_sum(s) * p.scale_log2;
-    const float mn = fmaxf(top, s), f = ex2(top - mn), w = ex2(s - mn);
+    for (int i = 0; i < 4; ++i) {
+      float k[4];
+      row_values<Q4>(p.k + (size_t)(place + i) * p.row_bytes, p.n_kv, kv, lane, k);
+      row_values<Q4>(p.v + (size_t)(place + i) * p.row_bytes, p.n_kv, kv, lane, v[i]);
+      s[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[i] = fmaf(q[c], k[c], s[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = warp_sum(s[i]) * p.scale_log2;
+      if (j0 + i < end) mn = fmaxf(mn, s[i]);
+    }
+    const float f = ex2(top - mn);
     top = mn;
-    l = l * f + w;
+    l *= f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = fmaf(w, v[i], acc[i] * f);
+    for (int c = 0; c < 4; ++c) acc[c] *= f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (j0 + i < end) {
+        const float w = ex2(s[i] - mn);
+        l += w;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] = fmaf(w, v[i][c], acc[c]);
+      }
   }
 }
 
@@ -560,176 +577,178 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     int run = 0;                       // blocks before this tile
     PpItem it;
     while (take(ok, it)) {
-    const int n = it.blocks, head = it.kv * p.group + r_head;
-    const bool live = r_pos < min(p.per_tile, it.rows);
-    const int limit = live ? min(it.pos0 + r_pos, p.max_len - 1) : -1;                           // the last key of this row
-    float m = -FLT_MAX, l = 0.f;
+      const int n = it.blocks, head = it.kv * p.group + r_head;
+      const bool live = r_pos < min(p.per_tile, it.rows);
+      const int limit = live ? min(it.pos0 + r_pos, p.max_len - 1) : -1;                           // the last key of this row
+      float m = -FLT_MAX, l = 0.f;
 #pragma unroll 1
-    for (int j = 0; j < n && ok; ++j) {
-      const uint32_t b_t = s_t + (uint32_t)(((run + j) & 1) * kPpBlock);
-      ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[(run + j) & 1], (uint32_t)((run + j) >> 1 & 1)));
-      if (!ok) break;
-      tc_fence_after();
-      __syncwarp();
-      float v[2][32];
-      pp_ask(b_t, v[0]);
-      pp_ask(b_t + 32u, v[1]);
-      pp_landed(v[0]);
-      pp_landed(v[1]);
-      const int last = limit - (it.block0 + j) * kPpBlock;      // keys 0 .. last of the block count
-      if (!__all_sync(0xffffffffu, last >= kPpBlock - 1)) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int k = 0; k < 32; ++k) v[c][k] = 32 * c + k <= last ? v[c][k] : -INFINITY;
-      }
-      float mx[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = fmaxf(v[c >> 1][16 * (c & 1)], v[c >> 1][16 * (c & 1) + 1]);
-#pragma unroll
-        for (int k = 2; k < 16; k += 2) mx[c] = fmaxf(mx[c], fmaxf(v[c >> 1][16 * (c & 1) + k], v[c >> 1][16 * (c & 1) + k + 1]));
-      }
-      const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2, -FLT_MAX);
-      if (j == 0) {
-        m = top;
-      } else if (__any_sync(0xffffffffu, top > m + kPpLag)) {
-        ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[(run + j - 1) & 1], (uint32_t)((run + j - 1) >> 1 & 1)));
+      for (int j = 0; j < n && ok; ++j) {
+        const uint32_t b_t = s_t + (uint32_t)(((run + j) & 1) * kPpBlock);
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[(run + j) & 1], (uint32_t)((run + j) >> 1 & 1)));
         if (!ok) break;
         tc_fence_after();
         __syncwarp();
-        const float m_new = top > m + kPpLag ? top : m, f = ex2(m - m_new);
+        float v[2][32];
+        pp_ask(b_t, v[0]);
+        pp_ask(b_t + 32u, v[1]);
+        pp_landed(v[0]);
+        pp_landed(v[1]);
+        const int last = limit - (it.block0 + j) * kPpBlock;      // keys 0 .. last of the block count
+        if (!__all_sync(0xffffffffu, last >= kPpBlock - 1)) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[c][k] = 32 * c + k <= last ? v[c][k] : -INFINITY;
+        }
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          mx[c] = fmaxf(v[c >> 1][16 * (c & 1)], v[c >> 1][16 * (c & 1) + 1]);
+#pragma unroll
+          for (int k = 2; k < 16; k += 2) mx[c] = fmaxf(mx[c], fmaxf(v[c >> 1][16 * (c & 1) + k], v[c >> 1][16 * (c & 1) + k + 1]));
+        }
+        const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2, -FLT_MAX);
+        if (j == 0) {
+          m = top;
+        } else if (__any_sync(0xffffffffu, top > m + kPpLag)) {
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[(run + j - 1) & 1], (uint32_t)((run + j - 1) >> 1 & 1)));
+          if (!ok) break;
+          tc_fence_after();
+          __syncwarp();
+          const float m_new = top > m + kPpLag ? top : m, f = ex2(m - m_new);
 #pragma unroll 1
-        for (int c = 0; c < kRowDim; c += 16) {
-          float o[16];
+          for (int c = 0; c < kRowDim; c += 16) {
+            float o[16];
+            uint32_t w[16];
+            tmem_ld16(o_t + (uint32_t)c, o);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(o[k] * f);
+            tmem_st16(o_t + (uint32_t)c, w);
+          }
+          l *= f;
+          m = m_new;
+        }
+        const uint64_t less = pack2(-m, -m);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
           uint32_t w[16];
-          tmem_ld16(o_t + (uint32_t)c, o);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(o[k] * f);
-          tmem_st16(o_t + (uint32_t)c, w);
-        }
-        l *= f;
-        m = m_new;
-      }
-      const uint64_t less = pack2(-m, -m);
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          float a, b;
-          const uint64_t t = fma2(pack2(v[c][2 * k], v[c][2 * k + 1]), scale2, less);
-          if (k % kPpPoly == kPpPoly - 1) {
-            ex2_poly(t, a, b);
-          } else {
-            unpack2(t, a, b);
-            a = ex2(a);
-            b = ex2(b);
-          }
-          w[k] = pack_bf16(a, b);
-          add_bf16x2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], w[k]);
-        }
-        tmem_st16(b_t + 16u * c, w);                  // over scores that this thread has read
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      arrive(&p_full[(run + j) & 1]);
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    }
-    if (ok && n) ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[(run + n - 1) & 1], (uint32_t)((run + n - 1) >> 1 & 1)));
-    if (!ok) break;
-    run += n;
-    tc_fence_after();
-    __syncwarp();
-    const size_t at = ((size_t)(live ? it.row0 + r_pos : 0) * p.n_heads + head) * kRowDim;
-    const size_t part_at = (size_t)it.part * p.s.rows * p.n_heads * kRowDim;
-    if (parts && live) *reinterpret_cast<float2*>(p.part_ml + (part_at + at) / (kRowDim / 2)) = make_float2(m, l);
-    if (n) {
-      const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-      float zero[4] = {0.f, 0.f, 0.f, 0.f};           // NaN if some sum is not finite
-      // Rows go over shared memory 64 bytes at a time, so that four lanes store what stands together (a lane with a row of its own would store to 32 places at once).
-      const unsigned to_store = __ballot_sync(0xffffffffu, live);
-      const int columns = parts ? 16 : 32;
-      uint8_t* base = parts ? reinterpret_cast<uint8_t*>(p.part_o + part_at) : reinterpret_cast<uint8_t*>(p.out);
-      const unsigned long long row_bytes_at = (unsigned long long)at * (parts ? 4 : 2);
-      unsigned long long to[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, row_bytes_at, 8 * k + (lane >> 2)) + 16 * (lane & 3);
-#pragma unroll 1
-      for (int c = 0; c < kRowDim; c += 32) {
-        float o[32];
-        __syncwarp();
-        pp_ask(o_t + (uint32_t)c, o);
-        pp_landed(o);
-        if (c == kRowDim - 32) {       // (the next tile's products may begin)
-          tc_fence_before();
-          arrive(o_free);
-        }
-#pragma unroll
-        for (int k = 0; k < 32; ++k) zero[k & 3] = fmaf(o[k], 0.f, zero[k & 3]);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (half && !parts) break;
-          uint8_t* row = mine_s + lane * 64;
-          const int turn = (lane >> 1) & 3;            // (eight lanes' 16 bytes meet all banks)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint4 y;
-            if (parts) {
-              y = make_uint4(__float_as_uint(half ? o[16 + 4 * k] : o[4 * k]), __float_as_uint(half ? o[17 + 4 * k] : o[4 * k + 1]),
-                             __float_as_uint(half ? o[18 + 4 * k] : o[4 * k + 2]), __float_as_uint(half ? o[19 + 4 * k] : o[4 * k + 3]));
+          for (int k = 0; k < 16; ++k) {
+            float a, b;
+            const uint64_t t = fma2(pack2(v[c][2 * k], v[c][2 * k + 1]), scale2, less);
+            if (k % kPpPoly == kPpPoly - 1) {
+              ex2_poly(t, a, b);
             } else {
-              y = make_uint4(pack_bf16(o[8 * k] * inv, o[8 * k + 1] * inv), pack_bf16(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
-                             pack_bf16(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack_bf16(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+              unpack2(t, a, b);
+              a = ex2(a);
+              b = ex2(b);
             }
-            *reinterpret_cast<uint4*>(row + ((k ^ turn) << 4)) = y;
+            w[k] = pack_bf16(a, b);
+            add_bf16x2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], w[k]);
           }
-          __syncwarp();
-          uint4 y[4];
+          tmem_st16(b_t + 16u * c, w);                  // over scores that this thread has read
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        arrive(&p_full[(run + j) & 1]);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      }
+      if (ok && n) ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[(run + n - 1) & 1], (uint32_t)((run + n - 1) >> 1 & 1)));
+      if (!ok) break;
+      run += n;
+      tc_fence_after();
+      __syncwarp();
+      const size_t at = ((size_t)(live ? it.row0 + r_pos : 0) * p.n_heads + head) * kRowDim;
+      const size_t part_at = (size_t)it.part * p.s.rows * p.n_heads * kRowDim;
+      if (parts && live) *reinterpret_cast<float2*>(p.part_ml + (part_at + at) / (kRowDim / 2)) = make_float2(m, l);
+      if (n) {
+        const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+        float zero[4] = {0.f, 0.f, 0.f, 0.f};           // NaN if some sum is not finite
+        // Rows go over shared memory 64 bytes at a time, so that four lanes store what stands together (a lane with a row of its own would store to 32 places at once).
+        const unsigned to_store = __ballot_sync(0xffffffffu, live);
+        const int columns = parts ? 16 : 32;
+        uint8_t* base = parts ? reinterpret_cast<uint8_t*>(p.part_o + part_at) : reinterpret_cast<uint8_t*>(p.out);
+        const unsigned long long row_bytes_at = (unsigned long long)at * (parts ? 4 : 2);
+        unsigned long long to[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int from = 8 * k + (lane >> 2);
-            y[k] = *reinterpret_cast<const uint4*>(mine_s + from * 64 + (((lane & 3) ^ ((from >> 1) & 3)) << 4));
+        for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, row_bytes_at, 8 * k + (lane >> 2)) + 16 * (lane & 3);
+#pragma unroll 1
+        for (int c = 0; c < kRowDim; c += 32) {
+          float o[32];
+          __syncwarp();
+          pp_ask(o_t + (uint32_t)c, o);
+          pp_landed(o);
+          if (c == kRowDim - 32) {       // (the next tile's products may begin)
+            tc_fence_before();
+            arrive(o_free);
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (to_store >> (8 * k + (lane >> 2)) & 1u) *reinterpret_cast<uint4*>(base + to[k] + (c + 16 * half) / columns * 64) = y[k];
-          __syncwarp();
+          for (int k = 0; k < 32; ++k) zero[k & 3] = fmaf(o[k], 0.f, zero[k & 3]);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (half && !parts) break;
+            uint8_t* row = mine_s + lane * 64;
+            const int turn = (lane >> 1) & 3;            // (eight lanes' 16 bytes meet all banks)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint4 y;
+              if (parts) {
+                y = make_uint4(__float_as_uint(half ? o[16 + 4 * k] : o[4 * k]), __float_as_uint(half ? o[17 + 4 * k] : o[4 * k + 1]),
+                               __float_as_uint(half ? o[18 + 4 * k] : o[4 * k + 2]), __float_as_uint(half ? o[19 + 4 * k] : o[4 * k + 3]));
+              } else {
+                y = make_uint4(pack_bf16(o[8 * k] * inv, o[8 * k + 1] * inv), pack_bf16(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+                               pack_bf16(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack_bf16(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+              }
+              *reinterpret_cast<uint4*>(row + ((k ^ turn) << 4)) = y;
+            }
+            __syncwarp();
+            uint4 y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int from = 8 * k + (lane >> 2);
+              y[k] = *reinterpret_cast<const uint4*>(mine_s + from * 64 + (((lane & 3) ^ ((from >> 1) & 3)) << 4));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (to_store >> (8 * k + (lane >> 2)) & 1u) *reinterpret_cast<uint4*>(base + to[k] + (c + 16 * half) / columns * 64) = y[k];
+            __syncwarp();
+          }
+        }
+        zero[0] += zero[1] + (zero[2] + zero[3]);
+        unsigned rows = __ballot_sync(0xffffffffu, live && zero[0] != zero[0]);
+        if (rows) {
+          // The last key with a value that is no number among those that some rows of this tile do not see: rows from its position on see them all.
+          const int first = it.block0 * kPpBlock, end = min((it.block0 + n) * kPpBlock, it.k_end);
+          int last_bad = -1;
+          for (int key = max(it.pos0 + 1, first); key < end; ++key) {
+            float v[4], z = 0.f;
+            row_values<Q4>(p.v + (size_t)max(page_row_of(p.s, it.seq, key), 0) * p.row_bytes, p.n_kv, it.kv, lane, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z = fmaf(v[i], 0.f, z);
+            if (__any_sync(0xffffffffu, z != z)) last_bad = key;
+          }
+          rows &= __ballot_sync(0xffffffffu, limit < last_bad);
+#pragma unroll 1
+          while (rows) {
+            const int src = __ffs(rows) - 1;
+            rows &= rows - 1;
+            const int row_limit = __shfl_sync(0xffffffffu, limit, src);
+            const size_t row_at = __shfl_sync(0xffffffffu, (unsigned long long)at, src);
+            float qr[4], rm = -FLT_MAX, rl = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qr[i] = __bfloat162float(p.q[row_at + 4 * lane + i]);
+            attend_paged_row<Q4>(p, it.seq, it.kv, first, min(end, row_limit + 1), qr, lane, rm, rl, acc);
+            if (parts) {
+              *reinterpret_cast<float4*>(p.part_o + part_at + row_at + 4 * lane) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+              if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + (part_at + row_at) / (kRowDim / 2)) = make_float2(rm, rl);
+            } else {
+              const float rinv = rl > 0.f || rl != rl ? 1.0f / rl : 0.f;
+              *reinterpret_cast<uint2*>(p.out + row_at + 4 * lane) = make_uint2(pack_bf16(acc[0] * rinv, acc[1] * rinv), pack_bf16(acc[2] * rinv, acc[3] * rinv));
+            }
+          }
         }
       }
-      zero[0] += zero[1] + (zero[2] + zero[3]);
-      unsigned rows = __ballot_sync(0xffffffffu, live && zero[0] != zero[0]);
-      if (rows) {
-        // Keys that rows of this CTA do not see and their blocks hold: from its first position on.
-        const int first = it.block0 * kPpBlock, end = min((it.block0 + n) * kPpBlock, it.k_end);
-        float z = 0.f;
-        for (int key = max(it.pos0 + 1, first); key < end; ++key) {
-          float v[4];
-          row_values<Q4>(p.v + (size_t)max(page_row_of(p.s, it.seq, key), 0) * p.row_bytes, p.n_kv, it.kv, lane, v);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) z = fmaf(v[i], 0.f, z);
-        }
-        if (!__any_sync(0xffffffffu, z != z)) rows = 0u;
-        while (rows) {
-          const int src = __ffs(rows) - 1;
-          rows &= rows - 1;
-          const int row_limit = __shfl_sync(0xffffffffu, limit, src);
-          const size_t row_at = __shfl_sync(0xffffffffu, (unsigned long long)at, src);
-          float qr[4], rm = -FLT_MAX, rl = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) qr[i] = __bfloat162float(p.q[row_at + 4 * lane + i]);
-          attend_paged_row<Q4>(p, it.seq, it.kv, first, min(end, row_limit + 1), qr, lane, rm, rl, acc);
-          if (parts) {
-            *reinterpret_cast<float4*>(p.part_o + part_at + row_at + 4 * lane) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-            if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + (part_at + row_at) / (kRowDim / 2)) = make_float2(rm, rl);
-          } else {
-            const float rinv = rl > 0.f || rl != rl ? 1.0f / rl : 0.f;
-            *reinterpret_cast<uint2*>(p.out + row_at + 4 * lane) = make_uint2(pack_bf16(acc[0] * rinv, acc[1] * rinv), pack_bf16(acc[2] * rinv, acc[3] * rinv));
-          }
-        }
-      }
-    }
     }
     if (!ok && lane == 0) give_up(DERR_TMEM);
   }
@@ -757,14 +776,23 @@ __global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PackedPre
   const float2 ml = lane < p.parts ? *reinterpret_cast<const float2*>(p.part_ml + (lane * heads + i) * 2) : make_float2(-FLT_MAX, 0.f);
   const float top = warp_max(ml.x), w = ex2(ml.x - top), l = warp_sum(ml.y * w);
   float o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < p.parts; ++k) {
-    const float f = __shfl_sync(0xffffffffu, w, k), has = __shfl_sync(0xffffffffu, ml.y, k);
-    if (has == 0.f) continue;          // (a part without keys of this row has left nothing)
-    const float4 v = *reinterpret_cast<const float4*>(p.part_o + ((size_t)k * heads + i) * kRowDim + 4 * lane);
-    o[0] = fmaf(v.x, f, o[0]);
-    o[1] = fmaf(v.y, f, o[1]);
-    o[2] = fmaf(v.z, f, o[2]);
-    o[3] = fmaf(v.w, f, o[3]);
+  for (int base = 0; base < p.parts; base += 8) {      // (eight on their way at a time)
+    float4 v[8];
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      f[k] = __shfl_sync(0xffffffffu, w, base + k);
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      // (a part without keys of this row has left nothing)
+      if (__shfl_sync(0xffffffffu, ml.y, base + k) != 0.f) v[k] = *reinterpret_cast<const float4*>(p.part_o + ((size_t)(base + k) * heads + i) * kRowDim + 4 * lane);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      o[0] = fmaf(v[k].x, f[k], o[0]);
+      o[1] = fmaf(v[k].y, f[k], o[1]);
+      o[2] = fmaf(v[k].z, f[k], o[2]);
+      o[3] = fmaf(v[k].w, f[k], o[3]);
+    }
   }
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
   *reinterpret_cast<uint2*>(p.out + i * kRowDim + 4 * lane) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
@@ -806,7 +834,7 @@ extern "C" int tq_gqa_prefill_paged(tq_ctx* ctx, const void* q_dev, const void* 
   TQ_REQUIRE(ctx, tiles <= 65535, "tq_gqa_prefill_paged: too many rows");
   size_t parts = 1;
   if (ctas < 2 * (size_t)ctx->sm_count) {
-    parts = (2 * (size_t)ctx->sm_count + ctas - 1) / ctas;
+    parts = 2 * (size_t)ctx->sm_count / ctas;          // (one more would begin when the others are through)
     const size_t few = longest / (8 * kPpBlock);
     parts = parts > few ? few : parts;
     parts = parts < 1 ? 1 : parts > (size_t)kPpMaxParts ? (size_t)kPpMaxParts : parts;
