@@ -232,7 +232,7 @@ __device__ __forceinline__ void pp_landed(float (&v)[32]) {
                  "+f"(v[31])::"memory");
 }
 
-// Pages of 4 bits: a loader's blocks.  A lane takes key lane + 32 u of a block, u = 0, 1: its codes are asked for a turn ahead, its page two.
+// Pages of 4 bits: a loader's blocks.  A lane takes keys lane and lane + 32 of a block: their codes are asked for a block ahead, their pages two.
 struct PpCodes {
   uint4 w[4];
   uint2 s;
@@ -454,19 +454,18 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
             }
             return x;
           };
-          PpCodes next = codes_at(0, page_at(0));
-          int page = page_at(1);
+          PpCodes even = codes_at(0, page_at(0)), odd = codes_at(1, page_at(1));
+          int even_page = page_at(2), odd_page = page_at(3);
           for (int i = 0; i < n && ok; ++i, ++run) {
             const int slot = run % kPpSlots;
             ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)(run / kPpSlots & 1) ^ 1u));
             if (!ok) break;
-#pragma unroll 1
-            for (int u = 0; u < 2; ++u) {
-              const PpCodes x = next;
-              next = codes_at(2 * i + u + 1, page);
-              page = page_at(2 * i + u + 2);
-              pp_convert(to + slot * kPpTile, 32 * u + lane, x);
-            }
+            pp_convert(to + slot * kPpTile, lane, even);
+            even = codes_at(2 * i + 2, even_page);
+            even_page = page_at(2 * i + 4);
+            pp_convert(to + slot * kPpTile, 32 + lane, odd);
+            odd = codes_at(2 * i + 3, odd_page);
+            odd_page = page_at(2 * i + 5);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             arrive(&full[slot]);
             if (!values && i == call) arrive(nearly);
@@ -828,14 +827,14 @@ extern "C" int tq_gqa_prefill_paged(tq_ctx* ctx, const void* q_dev, const void* 
   p.err = ctx->dev_err;
   p.group = (int)(n_heads / n_kv_heads);
   p.per_tile = kPfTile / p.group;
-  // Tiles there may be; parts of their keys, of eight blocks or more, where these leave SMs idle (each takes two CTAs).
+  // Tiles there may be; parts of their keys, of four blocks or more, where these leave SMs idle (each takes two CTAs).
   const size_t tiles = seq_rows_dev ? rows / p.per_tile + (batch < rows ? batch : rows) : rows;
   const size_t most = (size_t)pages->table_ld * pages->page_rows, longest = max_len < most ? max_len : most, ctas = tiles * n_kv_heads;
   TQ_REQUIRE(ctx, tiles <= 65535, "tq_gqa_prefill_paged: too many rows");
   size_t parts = 1;
   if (ctas < 2 * (size_t)ctx->sm_count) {
     parts = 2 * (size_t)ctx->sm_count / ctas;          // (one more would begin when the others are through)
-    const size_t few = longest / (8 * kPpBlock);
+    const size_t few = longest / (4 * kPpBlock);
     parts = parts > few ? few : parts;
     parts = parts < 1 ? 1 : parts > (size_t)kPpMaxParts ? (size_t)kPpMaxParts : parts;
   }
