@@ -21,11 +21,13 @@ struct AppendParams {
 };
 
 // The scale of 32 values whose largest magnitude is amax.  Blocks below 2^-100 are zeros, those of 2^120 and above NaN: 24 s, which the readers
-// form, is then a normal number.
+// form, is then a normal number.  A product with a number just below 1 / 7, rounded up to 5 bits, is the scale or, where amax / 7 is on the border, the number
+// below it; seven times 5 bits are exact, and tell.
 __device__ __forceinline__ float q4_scale(float amax) {
   if (!(amax < 1.329227995784916e36f)) return __uint_as_float(0x7FC00000u);
   if (amax < 7.888609052210118e-31f) return 0.f;
-  return __uint_as_float((__float_as_uint(__fdiv_rn(amax, 7.f)) + 0x7FFFFu) & 0xFFF80000u);
+  const float s = __uint_as_float((__float_as_uint(amax * 0.14285707f) + 0x7FFFFu) & 0xFFF80000u);
+  return 7.f * s < amax ? __uint_as_float(__float_as_uint(s) + 0x80000u) : s;
 }
 
 __device__ __forceinline__ float max_or_nan(float a, float b) {
@@ -34,11 +36,14 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
   return r;
 }
 // The codes of eight values of a scale s, the first in the lowest four bits: 8 + x / s rounded to nearest even.  The quotient comes from the reciprocal with one
-// correction by its remainder, which fused operations have exactly, and is the rounded one that way; that no such quotient is a tie unless x / s is one follows
-// from s having 5 bits.  (The compiler's division instead: 5800 rows of 1024 keys and values from bf16 41.8 us.)  Adding 1.5 * 2^23 + 8 leaves the code in the
+// correction by its remainder, which fused operations have exactly: 2^-46 of it off before its last rounding.  s has 5 bits, a tie (k + 1/2) s nine at most, so
+// that the f32 numbers beside a tie are 2^-24 (1 + 2^-9) of it away and their quotients do not round to one.  (The compiler's division instead: 5800 rows of 1024
+// keys and values from bf16 41.8 us.)  Adding 1.5 * 2^23 + 8 leaves the code in the
 // number's low bits, and what else is in them is the same for all.
 __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float s) {
-  const float inv = __frcp_rn(s);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  inv = __fmaf_rn(__fmaf_rn(-s, inv, 1.f), inv, inv);
   uint32_t word = 0, rest = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -52,7 +57,7 @@ __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float s) {
 // A CTA takes ROWS rows and 128 eighths of a head: 32 bytes (f32) in, 16 or 4 out for a thread and row.  Rows' places are looked up by a warp each
 // (starts, sequence, length, page, holders: five loads one after the other) while the values are on their way.  What bounds it: the bytes (5000 rows of 32 + 16
 // heads f32 to bf16 pages, 200 MB, 35.0 us, 5.7 TB/s), beside the look-ups (CTAs of 256 threads 37.1, of 512 44.1; eight rows each 47.2); to 4 bits instructions
-// (5800 rows from bf16 32 us).  A single row 4.2 us.
+// (5800 rows from bf16 30 us; two groups of columns a thread, for half as many look-ups, 32).  A single row 4.2 us.
 template <typename X, int ROWS, bool Q4>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
   __shared__ int place_s[ROWS], pos_s[ROWS];           // cache row (-1: none), position

@@ -77,3 +77,17 @@ def test_four_bits_of_ordinary_numbers():
     assert raw.shape == (50, row_bytes(3)) and (raw[:, 216:] == 0).all()
     assert np.array_equal(v, ((v.astype(np.float32).view(np.uint32) & 0xFFFF0000).view(np.float32)))
     assert (np.abs(v - x).reshape(50, 3, 4, 32).max(-1) <= amax / 7 * (1 + 1 / 16) / 2 * (1 + 2.0 ** -20)).all()
+
+
+def test_the_scale_from_a_product():
+    """What the kernel computes instead of a division (a product with a number just below 1 / 7, rounded up to 5 bits, and one step more where seven times
+    that is still below the largest magnitude) is the rule: at the borders, beside them and elsewhere."""
+    f = np.float32
+    rng = np.random.default_rng(0)
+    k = (np.arange(16, 33)[:, None] * 7.0 * 2.0 ** np.arange(-90, 110)[None]).ravel().astype(f)
+    a = np.concatenate([np.exp(rng.uniform(-60, 80, 200000)).astype(f), *((k.view(np.int32) + np.int32(d)).view(f) for d in range(-20, 21))])
+    a = a[(a >= 2.0 ** -100) & (a < 2.0 ** 120)]
+    s = (((a * f(0.14285707)).view(np.uint32) + np.uint32(0x7FFFF)) & np.uint32(0xFFF80000)).view(f)
+    s = np.where(f(7) * s < a, (s.view(np.uint32) + np.uint32(0x80000)).view(f), s)
+    frac, e = np.frexp(a.astype(np.float64) / 7)
+    assert np.array_equal(s.astype(np.float64), np.ldexp(np.ceil(frac * 32) / 32, e))
