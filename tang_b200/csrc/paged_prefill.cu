@@ -149,7 +149,7 @@ __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, i
         if (lane >= o) incl += w;
       }
       const unsigned hit = __ballot_sync(0xffffffffu, x >= before + incl - tiles && x < before + incl);
-      if (hit) {
+      if (hit && i < 0) {
         const int src = __ffs(hit) - 1;
         i = base + src;
         first = __shfl_sync(0xffffffffu, f, src);
@@ -159,9 +159,9 @@ __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, i
         tile = __shfl_sync(0xffffffffu, before + incl, src) - 1 - x;   // (the last tile first)
       }
       before += __shfl_sync(0xffffffffu, incl, 31);
-      if (i >= 0) break;
+      if (i >= 0 && x > 0) break;      // (the first tile's CTAs look at all starts)
     }
-    if (bad && lane == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
+    if (__any_sync(0xffffffffu, bad) && lane == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
   }
   if (i < 0) return it;
   if (s < 0 || len < count || len > (long long)p.s.table_ld << p.s.page_shift) {
@@ -818,6 +818,7 @@ extern "C" int tq_gqa_prefill_paged(tq_ctx* ctx, const void* q_dev, const void* 
   TQ_REQUIRE(ctx, max_len > 0 && max_len <= (1u << 30), "tq_gqa_prefill_paged: max_len must bound the sequence lengths");
   TQ_REQUIRE(ctx, (((uintptr_t)q_dev | (uintptr_t)k_pages_dev | (uintptr_t)v_pages_dev | (uintptr_t)out_dev) & 15) == 0,
              "tq_gqa_prefill_paged: arrays must be 16-byte aligned");
+  TQ_REQUIRE(ctx, q_dev != out_dev, "tq_gqa_prefill_paged: results need a buffer of their own (rows may be attended again)");
   const bool q4 = page_rows_as == TQ_PAGES_Q4;
   PackedPrefillParams p;
   p.s = packed_seqs(pages, seqs_dev, seq_rows_dev, batch, rows);

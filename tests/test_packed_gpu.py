@@ -377,3 +377,59 @@ def test_decode_over_four_bits_with_values_that_are_no_number(dev):
         ok = widen(s.decode().to_vec()).reshape(2, 8, HD)
         dev.sync()
         assert np.array_equal(got[~bad], ok[~bad])
+
+
+@pytest.mark.parametrize("form", ["bf16", "q4"])
+def test_the_largest_batch(dev, form):
+    """1024 sequences in an order of their own: one row each, and several, some none."""
+    import tang_b200 as tb
+
+    rng = np.random.default_rng(7)
+    order = rng.permutation(1100)[:1024]
+    for most in (1, 9):
+        lens = rng.integers(1, 60, 1024)
+        counts = np.minimum(lens, rng.integers(0 if most > 1 else 1, most + 1, 1024))
+        s = Sequences(4, 2, 16, lens, counts, 8, form, seqs=order).put(dev)
+        x = s.rng.standard_normal((s.rows, 8, HD)).astype(np.float32)
+        at = s.new_places()
+        k, v = dev.kv_read_paged(s.kb, s.vb, s.pool, 1024, s.rows, 2, HD, seqs=s.seqs, seq_rows=s.seq_rows)
+        assert np.array_equal(widen(k.to_vec()).reshape(s.rows, 2, HD), s.values[0][at]) and np.array_equal(widen(v.to_vec()).reshape(s.rows, 2, HD), s.values[1][at])
+        got = s.prefill().to_vec()
+        want = s.reference()
+        check_attention(got, *want, terms=1)
+        if form == "q4" and most == 1:
+            check_attention(s.decode().to_vec(), *want, terms=2)
+        appended(s, dev, x, tb.F32, 64)
+        new = s.kb.to_vec().reshape(s.raw[0].shape)
+        cos, sin = tables(64)
+        turned = rotate(x[:, 4:6], cos[s.new_positions()], sin[s.new_positions()])
+        assert np.array_equal(new[at], pack(turned)[0] if form == "q4" else bf16_round(np.ascontiguousarray(turned))[0].reshape(s.rows, -1))
+        dev.sync()
+
+
+@pytest.mark.parametrize("form", ["bf16", "q4"])
+def test_starts_that_do_not_ascend(dev, form):
+    """Reported; rows of the sequences whose starts are sound are what they are without the others."""
+    import tang_b200 as tb
+
+    for starts, sound in (([0, 20, 10, 30], [(0, 0, 10)]), ([0, 10, 40, 30], [(0, 0, 10)]), ([-3, 10, 20, 30], [(1, 10, 10), (2, 20, 10)])):
+        s = Sequences(4, 2, 16, [50, 60, 70], [10, 10, 10], 9, form).put(dev)
+        want, size = s.reference()
+        s.seq_rows = dev.upload(np.array(starts, np.int32), tb.I32)
+        out = dev.upload(np.zeros(30 * 4 * HD, np.uint16), tb.BF16)
+        got = s.prefill(out=out).to_vec().reshape(30, 4, HD)
+        with pytest.raises(tb.TangqError):
+            dev.sync()
+        if starts[1] == 10 and starts[0] == 0 or starts[0] < 0:
+            for i, first, n in sound:
+                check_attention(got[first:first + n], want[first:first + n], size[first:first + n], terms=1)
+        before = s.kb.to_vec()
+        x = s.rng.standard_normal((30, 8, HD)).astype(np.float32)
+        appended(s, dev, x, tb.F32, 80)
+        with pytest.raises(tb.TangqError):
+            dev.sync()
+        changed = set(np.nonzero((s.kb.to_vec() != before).reshape(s.raw[0].shape).any(1))[0])
+        allowed = set()
+        for b in range(3):
+            allowed |= set(s.places(b, range(s.lens[b])).tolist())
+        assert changed <= allowed

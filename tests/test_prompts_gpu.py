@@ -268,6 +268,48 @@ def test_two_recorded_generations_share_the_workspace_and_two_handles_do_not():
         g.pool.destroy()
 
 
+@pytest.mark.parametrize("form", ["bf16", "q4"])
+def test_pages_whose_bytes_are_behind_32_bits(dev, form):
+    """A cache of more than 5 GB for keys and as much for values, the sequences in its last pages."""
+    import tang_b200 as tb
+
+    nh, nkv, P, B = 32, 8, 1024, 2
+    row = nkv * HD * 2 if form == "bf16" else row_bytes(nkv)
+    pages = -(-(5 << 30) // (row * P))
+    per = 1 if form == "q4" else 2
+    k, v = (dev.alloc(pages * P * row // per, tb.U8 if form == "q4" else tb.BF16) for _ in range(2))
+    tables_h, lens = np.full((B, 3), -1, np.int32), np.array([1500, 90], np.int32)
+    tables_h[0, :2], tables_h[1, 0] = [pages - 1, pages - 3], pages - 2
+    refs = np.zeros(pages, np.int32)
+    refs[[pages - 1, pages - 2, pages - 3]] = 1
+    state = [dev.upload(a, tb.I32) for a in (refs, tables_h, lens)]
+    pool = tb.PagePool(dev, pages, P, B, 3, None, *state)
+    rng, cs = np.random.default_rng(3), tables(1500)
+    x = rng.standard_normal((1590, nh + 2 * nkv, HD)).astype(np.float32)
+    starts = dev.upload(np.array([0, 1500, 1590], np.int32), tb.I32)
+    q = dev.kv_append_paged(dev.upload(x), dev.upload(cs[0]), dev.upload(cs[1]), pool, k, v, B, 1590, nh, nkv, HD, seq_rows=starts)
+    ko, vo = dev.kv_read_paged(k, v, pool, B, 1590, nkv, HD, seq_rows=starts)
+    out = dev.gqa_prefill_paged(q, k, v, pool, B, 1590, nh, nkv, HD, 1500, seq_rows=starts)
+    pos = np.concatenate([np.arange(1500), np.arange(90)])
+    turned = rotate(x[:, :nh + nkv], cs[0][pos], cs[1][pos])
+    stored = lambda a: pack(a)[1] if form == "q4" else bf16_round(np.ascontiguousarray(a))[1].reshape(a.shape)  # noqa: E731
+    kv = [stored(turned[:, nh:]), stored(x[:, nh + nkv:])]
+    for got, want in ((ko, kv[0]), (vo, kv[1])):
+        assert np.array_equal((got.to_vec().astype(np.uint32) << 16).view(np.float32).reshape(want.shape), want)
+    qf = bf16_round(np.ascontiguousarray(turned[:, :nh]))[1].reshape(1590, nh, HD)
+    got = out.to_vec().reshape(1590, nh, HD)
+    for r, n in ((1499, 1500), (1023, 1024), (0, 1)):
+        check_attention(got[r:r + 1], *attend(qf[r:r + 1], kv[0][:n], kv[1][:n]), terms=1)
+    check_attention(got[1500:], *attend(qf[1500:], kv[0][1500:], kv[1][1500:]), terms=1)
+    if form == "q4":
+        last = dev.upload(np.ascontiguousarray(q.to_vec().reshape(1590, -1)[[1499, 1589]]), tb.BF16)
+        one = dev.gqa_decode_paged_q4(last, k, v, pool, B, nh, nkv, HD, 1500).to_vec().reshape(B, nh, HD)
+        check_attention(one[:1], *attend(qf[1499:1500], kv[0][:1500], kv[1][:1500]), terms=2)
+        check_attention(one[1:], *attend(qf[1589:], kv[0][1500:], kv[1][1500:]), terms=2)
+    dev.sync()
+    pool.destroy()
+
+
 def test_prefill_is_recorded_with_room_for_more_rows(dev):
     """One graph for steps of up to 60 rows: what the starts say is read when it is replayed; parts of the keys share a workspace that has its size."""
     import tang_b200 as tb
@@ -317,14 +359,14 @@ def test_refusals(dev):
     h, L, ctx = pool.handle, dev._L, dev._ctx
     append = [ctx, f, 0, 0, f, f, 64, h, None, None, 2, 2, 4, 2, 128, b, b, b, 0]
     read = [ctx, b, b, 0, h, None, None, 2, 2, 2, 128, b, b]
-    prefill = [ctx, b, b, b, 0, h, None, None, 2, 2, 4, 2, 128, 64, b]
+    prefill = [ctx, b, b, b, 0, h, None, None, 2, 2, 4, 2, 128, 64, b + 4096]
     decode = [ctx, b, b, b, h, None, 2, 4, 2, 128, 64, b]
     for fn, ok, batch, bad in (
             (L.tq_kv_append_paged, append, 10, {1: [None, f + 4], 2: [2, 9], 3: [100, 8 * 128 + 2], 4: [None, f + 8], 5: [None], 6: [0], 7: [None, theirs.handle], 10: [3, 1025],
                                             11: [1, 3], 12: [0, 70000], 13: [0], 14: [64], 15: [None, b + 2], 16: [None], 17: [None, b + 8], 18: [2, -1]}),
             (L.tq_kv_read_paged, read, 7, {1: [None], 2: [None, b + 8], 3: [2], 4: [None, theirs.handle], 7: [3], 8: [1], 9: [0], 10: [64], 11: [None], 12: [None, b + 4]}),
             (L.tq_gqa_prefill_paged, prefill, 8, {1: [None, b + 8], 2: [None], 3: [None], 4: [2], 5: [None, theirs.handle], 8: [3, 5000], 9: [1], 10: [0, 3, 18], 11: [0], 12: [64],
-                                               13: [0, 1 << 31], 14: [None, b + 2]}),
+                                               13: [0, 1 << 31], 14: [None, b + 2, b]}),
             (L.tq_gqa_decode_paged_q4, decode, 6, {1: [None, b + 8], 2: [None], 3: [None, b + 4], 4: [None, theirs.handle], 6: [3], 7: [3, 18, 0], 8: [0], 9: [64],
                                                 10: [0, 1 << 31], 11: [None, b + 2]})):
         for at, values in bad.items():
