@@ -433,3 +433,36 @@ def test_starts_that_do_not_ascend(dev, form):
         for b in range(3):
             allowed |= set(s.places(b, range(s.lens[b])).tolist())
         assert changed <= allowed
+
+
+@pytest.mark.parametrize("form", ["bf16", "q4"])
+@pytest.mark.parametrize("what", ["page", "sequence", "length"])
+def test_what_does_not_exist_is_reported(dev, form, what):
+    """A page, a sequence, more rows than positions: the other sequences' results are what they are."""
+    import tang_b200 as tb
+
+    for counts in ([10, 1, 30], [1, 1, 1]):
+        s = Sequences(8, 2, 16, [100, 40, 90], counts, 11, form, seqs=[2, 0, 1])
+        want, size = s.reference()
+        if what == "page":
+            s.tables[0, 1] = -5
+        elif what == "sequence":
+            s.order = np.array([2, 99, 1])
+        else:
+            s.lens_all[0] = -1 if counts[1] == 1 else 0
+        s.put(dev)
+        calls = [lambda: s.prefill(), lambda: dev.kv_read_paged(s.kb, s.vb, s.pool, 3, s.rows, 2, HD, seqs=s.seqs, seq_rows=s.seq_rows)[0]]
+        if form == "q4" and counts[0] == 1 and what != "length":
+            calls.append(lambda: s.decode())
+        for i, call in enumerate(calls):
+            got = call().to_vec()
+            reads_it = what != "page" or i != 1 or counts[1] > 24       # (the page holds positions 16 to 31, the new rows are behind it)
+            if reads_it:
+                with pytest.raises(tb.TangqError):
+                    dev.sync()
+            else:
+                dev.sync()
+            if i != 1:
+                ok = np.ones(s.rows, bool)
+                ok[s.starts[1]:s.starts[2]] = False
+                check_attention(got.reshape(want.shape)[ok], want[ok], size[ok], terms=1 if i == 0 else 2)
