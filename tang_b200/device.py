@@ -383,7 +383,9 @@ class Graph:
 
 # ---------------------------------------------------------------------- operators of the decode step
 def _check_types(call: str, dtype: int, **buffers) -> None:
-    """A kernel takes a buffer's elements as what it needs: of another type they would be other values, or fewer bytes."""
+    """A kernel takes a buffer's elements as what it needs: of another type they would be other values, or fewer bytes.
+    The calls over pages compare first and come here only to raise: a token's time is the host's for them, and this loop was a
+    third of their wrappers."""
     for name, b in buffers.items():
         if b is not None and b.dtype != dtype:
             raise TangqError(_lib.TQ_EINVAL, f"{call}: {name} has elements of another type than the call takes")
@@ -396,6 +398,11 @@ def q4_row_bytes(n_kv_heads: int) -> int:
 
 def _opt_ptr(buf) -> C.c_void_p:
     return C.c_void_p(buf.ptr if buf is not None else 0)
+
+
+def _raw(buf: Buffer | None) -> int | None:
+    """The same address as a plain number: the declared argument types take it. An empty buffer is false and yet a buffer."""
+    return None if buf is None else buf.ptr
 
 
 def _add_ops(cls):
@@ -505,16 +512,19 @@ def _add_ops(cls):
 
     def _page_form(self, call: str, pool, n_kv_heads: int, k_pages: Buffer, v_pages: Buffer) -> int:
         """What the pages' rows are, by the buffers' type: bf16, or bytes (rows of 4 bits)."""
-        form, row = (_lib.PAGES_BF16, n_kv_heads * 128) if k_pages.dtype == BF16 else (_lib.PAGES_Q4, q4_row_bytes(n_kv_heads))
-        _check_types(call, BF16 if form == _lib.PAGES_BF16 else _lib.U8, k_pages=k_pages, v_pages=v_pages)
+        bf16 = k_pages.dtype == BF16
+        if v_pages.dtype != k_pages.dtype or not (bf16 or k_pages.dtype == _lib.U8):
+            _check_types(call, BF16 if bf16 else _lib.U8, k_pages=k_pages, v_pages=v_pages)
+        row = n_kv_heads * 128 if bf16 else q4_row_bytes(n_kv_heads)
         if k_pages.n != pool.n_pages * pool.page_rows * row or v_pages.n != k_pages.n:
             raise TangqError(_lib.TQ_EINVAL, f"{call}: the pages are not the pool's {pool.n_pages * pool.page_rows} rows of {row} elements")
-        return form
+        return _lib.PAGES_BF16 if bf16 else _lib.PAGES_Q4
 
     def _packed(self, call: str, batch: int, rows: int, seqs: Buffer | None, seq_rows: Buffer | None) -> None:
-        if (seqs is not None and seqs.n < batch) or (seq_rows is not None and seq_rows.n < batch + 1) or (seq_rows is None and rows != batch):
+        if (seqs is not None and seqs.n < batch) or (rows != batch if seq_rows is None else seq_rows.n < batch + 1):
             raise TangqError(_lib.TQ_EINVAL, f"{call}: {batch} sequences need as many numbers and one more start, or one row each without starts")
-        _check_types(call, _lib.I32, seqs=seqs, seq_rows=seq_rows)
+        if (seqs is not None and seqs.dtype != _lib.I32) or (seq_rows is not None and seq_rows.dtype != _lib.I32):
+            _check_types(call, _lib.I32, seqs=seqs, seq_rows=seq_rows)
 
     def kv_append_paged(self, x: Buffer, cos: Buffer, sin: Buffer, pool, k_pages: Buffer, v_pages: Buffer, batch: int, rows: int, n_heads: int,
                         n_kv_heads: int, head_dim: int, seqs: Buffer | None = None, seq_rows: Buffer | None = None, ldx: int = 0,
@@ -528,14 +538,16 @@ def _add_ops(cls):
             raise TangqError(_lib.TQ_EINVAL, "kv_append_paged: buffer sizes do not match the shapes")
         form = self._page_form("kv_append_paged", pool, n_kv_heads, k_pages, v_pages)
         self._packed("kv_append_paged", batch, rows, seqs, seq_rows)
-        _check_types("kv_append_paged", F32, cos=cos, sin=sin)
+        if cos.dtype != F32 or sin.dtype != F32:
+            _check_types("kv_append_paged", F32, cos=cos, sin=sin)
         if q_out is None:
             q_out = self.alloc(rows * n_heads * head_dim, BF16)
         elif q_out.n < rows * n_heads * head_dim:
             raise TangqError(_lib.TQ_EINVAL, "kv_append_paged: no room for the queries")
-        _check_types("kv_append_paged", BF16, q_out=q_out)
-        self._check(self._L.tq_kv_append_paged(self._ctx, x.ptr, x.dtype, ldx, cos.ptr, sin.ptr, 2 * cos.n // head_dim, pool.handle, _opt_ptr(seqs),
-                                               _opt_ptr(seq_rows), batch, rows, n_heads, n_kv_heads, head_dim, q_out.ptr, k_pages.ptr, v_pages.ptr, form))
+        if q_out.dtype != BF16:
+            _check_types("kv_append_paged", BF16, q_out=q_out)
+        self._check(self._L.tq_kv_append_paged(self._ctx, x.ptr, x.dtype, ldx, cos.ptr, sin.ptr, 2 * cos.n // head_dim, pool.handle, _raw(seqs),
+                                               _raw(seq_rows), batch, rows, n_heads, n_kv_heads, head_dim, q_out.ptr, k_pages.ptr, v_pages.ptr, form))
         return q_out
 
     def kv_read_paged(self, k_pages: Buffer, v_pages: Buffer, pool, batch: int, rows: int, n_kv_heads: int, head_dim: int, seqs: Buffer | None = None,
@@ -547,8 +559,9 @@ def _add_ops(cls):
         k_out, v_out = (self.alloc(n, BF16) if b is None else b for b in (k_out, v_out))
         if k_out.n < n or v_out.n < n:
             raise TangqError(_lib.TQ_EINVAL, "kv_read_paged: no room for the rows")
-        _check_types("kv_read_paged", BF16, k_out=k_out, v_out=v_out)
-        self._check(self._L.tq_kv_read_paged(self._ctx, k_pages.ptr, v_pages.ptr, form, pool.handle, _opt_ptr(seqs), _opt_ptr(seq_rows), batch, rows, n_kv_heads,
+        if k_out.dtype != BF16 or v_out.dtype != BF16:
+            _check_types("kv_read_paged", BF16, k_out=k_out, v_out=v_out)
+        self._check(self._L.tq_kv_read_paged(self._ctx, k_pages.ptr, v_pages.ptr, form, pool.handle, _raw(seqs), _raw(seq_rows), batch, rows, n_kv_heads,
                                              head_dim, k_out.ptr, v_out.ptr))
         return k_out, v_out
 
@@ -564,8 +577,9 @@ def _add_ops(cls):
             out = self.alloc(rows * n_heads * head_dim, BF16)
         elif out.n < rows * n_heads * head_dim:
             raise TangqError(_lib.TQ_EINVAL, "gqa_prefill_paged: no room for the results")
-        _check_types("gqa_prefill_paged", BF16, q=q, out=out)
-        self._check(self._L.tq_gqa_prefill_paged(self._ctx, q.ptr, k_pages.ptr, v_pages.ptr, form, pool.handle, _opt_ptr(seqs), _opt_ptr(seq_rows), batch, rows,
+        if q.dtype != BF16 or out.dtype != BF16:
+            _check_types("gqa_prefill_paged", BF16, q=q, out=out)
+        self._check(self._L.tq_gqa_prefill_paged(self._ctx, q.ptr, k_pages.ptr, v_pages.ptr, form, pool.handle, _raw(seqs), _raw(seq_rows), batch, rows,
                                                  n_heads, n_kv_heads, head_dim, max_len, out.ptr))
         return out
 
@@ -574,15 +588,17 @@ def _add_ops(cls):
         """``gqa_decode_paged`` over pages of 4 bits (``tq_gqa_decode_paged_q4``); no groups, bf16 results."""
         self._page_form("gqa_decode_paged_q4", pool, n_kv_heads, k_pages, v_pages)
         self._packed("gqa_decode_paged_q4", batch, batch, seqs, None)
-        _check_types("gqa_decode_paged_q4", _lib.U8, k_pages=k_pages)
+        if k_pages.dtype != _lib.U8:
+            _check_types("gqa_decode_paged_q4", _lib.U8, k_pages=k_pages)
         if q.n < batch * n_heads * head_dim:
             raise TangqError(_lib.TQ_EINVAL, "gqa_decode_paged_q4: buffer sizes do not match the shapes")
         if out is None:
             out = self.alloc(batch * n_heads * head_dim, BF16)
         elif out.n < batch * n_heads * head_dim:
             raise TangqError(_lib.TQ_EINVAL, "gqa_decode_paged_q4: no room for the results")
-        _check_types("gqa_decode_paged_q4", BF16, q=q, out=out)
-        self._check(self._L.tq_gqa_decode_paged_q4(self._ctx, q.ptr, k_pages.ptr, v_pages.ptr, pool.handle, _opt_ptr(seqs), batch, n_heads, n_kv_heads, head_dim,
+        if q.dtype != BF16 or out.dtype != BF16:
+            _check_types("gqa_decode_paged_q4", BF16, q=q, out=out)
+        self._check(self._L.tq_gqa_decode_paged_q4(self._ctx, q.ptr, k_pages.ptr, v_pages.ptr, pool.handle, _raw(seqs), batch, n_heads, n_kv_heads, head_dim,
                                                    max_len, out.ptr))
         return out
 

@@ -68,6 +68,41 @@ def test_sizes_and_types_are_checked_before_the_call(tb):
             dev.gqa_decode_paged_q4(**{**ok, **kw})
 
 
+def test_what_reaches_the_library_of_buffers_that_may_be_missing(tb):
+    """No sequences, empty ones and present ones: null or the buffer's address, which the declared types have to take."""
+    seen = []
+
+    class Library:
+        def __getattr__(self, name):
+            types = getattr(tb.load(), name).argtypes
+
+            def call(*args):
+                assert len(args) == len(types)
+                for t, a in zip(types[1:], args[1:]):
+                    t.from_param(a)
+                seen.append((name, args))
+                return 0
+            return call
+
+    dev = tb.QuantComputeDevice.__new__(tb.QuantComputeDevice)
+    dev._ctx, dev._L = None, Library()
+    at = iter(range(64, 1 << 20, 64))
+    buf = lambda n, dt=tb.I32: tb.Buffer(dev, next(at), n, dt, owns=False)  # noqa: E731
+    pool = tb.PagePool.__new__(tb.PagePool)
+    pool.dev, pool.n_pages, pool.page_rows, pool.handle = dev, 2, 16, 0
+    k, v, q, out, table = buf(32 * 144, tb.U8), buf(32 * 144, tb.U8), buf(2048, tb.BF16), buf(2048, tb.BF16), buf(640, tb.F32)
+    for batch, seqs, starts in ((2, None, None), (2, buf(2), buf(3)), (2, None, buf(3)), (0, buf(0), buf(1)), (0, buf(0), None)):
+        seen.clear()
+        packed = dict(seqs=seqs, seq_rows=starts)
+        dev.kv_append_paged(buf(batch * 12 * 128, tb.F32), table, table, pool, k, v, batch, batch, 8, 2, 128, q_out=q, **packed)
+        dev.kv_read_paged(k, v, pool, batch, batch, 2, 128, k_out=q, v_out=out, **packed)
+        dev.gqa_prefill_paged(q, k, v, pool, batch, batch, 8, 2, 128, 9, out=out, **packed)
+        dev.gqa_decode_paged_q4(q, k, v, pool, batch, 8, 2, 128, 9, seqs=seqs, out=out)
+        assert [n for n, _ in seen] == ["tq_kv_append_paged", "tq_kv_read_paged", "tq_gqa_prefill_paged", "tq_gqa_decode_paged_q4"]
+        s, r = (None if b is None else b.ptr for b in (seqs, starts))
+        assert [a[i:i + 2] for (_, a), i in zip(seen, (8, 5, 6))] == [(s, r)] * 3 and seen[3][1][5] == s
+
+
 def test_four_bits_of_ordinary_numbers():
     """Values are bf16 numbers, within half a step (the scale, up to a sixteenth more than the largest / 7) of what they stand for."""
     rng = np.random.default_rng(0)
