@@ -44,12 +44,16 @@ __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float s) {
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
   inv = __fmaf_rn(__fmaf_rn(-s, inv, 1.f), inv, inv);
+  const uint64_t inv2 = pack2(inv, inv), less = pack2(-s, -s), up = pack2(12582920.f, 12582920.f);
   uint32_t word = 0, rest = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = __fmul_rn(x[i], inv), quotient = __fmaf_rn(__fmaf_rn(-q, s, x[i]), inv, q);
-    word += __float_as_uint(__fadd_rn(quotient, 12582920.f)) << (4 * i);
-    rest += 0x4B400000u << (4 * i);
+  for (int j = 0; j < 4; ++j) {
+    const int i = j / 2 * 4 + j % 2;   // (and i + 2: the rotation's pairs)
+    const uint64_t v = pack2(x[i], x[i + 2]), q = mul2(v, inv2);
+    float a, b;
+    unpack2(add2(fma2(fma2(q, less, v), inv2, q), up), a, b);
+    word += (__float_as_uint(a) << (4 * i)) + (__float_as_uint(b) << (4 * i + 8));
+    rest += (0x4B400000u << (4 * i)) + (0x4B400000u << (4 * i + 8));
   }
   return word - rest;
 }
@@ -57,7 +61,8 @@ __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float s) {
 // A CTA takes ROWS rows and 128 eighths of a head: 32 bytes (f32) in, 16 or 4 out for a thread and row.  Rows' places are looked up by a warp each
 // (starts, sequence, length, page, holders: five loads one after the other) while the values are on their way.  What bounds it: the bytes (5000 rows of 32 + 16
 // heads f32 to bf16 pages, 200 MB, 35.0 us, 5.7 TB/s), beside the look-ups (CTAs of 256 threads 37.1, of 512 44.1; eight rows each 47.2); to 4 bits instructions
-// (5800 rows from bf16 30 us; two groups of columns a thread, for half as many look-ups, 32).  A single row 4.2 us.
+// (5800 rows from bf16 28 us, 30 with single products and
+// quotients; two groups of columns a thread, for half as many look-ups, 32; one warp's lanes for all rows' look-ups no difference).  A single row 4.2 us.
 template <typename X, int ROWS, bool Q4>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
   __shared__ int place_s[ROWS], pos_s[ROWS];           // cache row (-1: none), position
@@ -130,12 +135,19 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
     if (head < p.n_heads + p.n_kv) {
       const float4 c4 = *reinterpret_cast<const float4*>(p.cos_t + (size_t)pos * (kRowDim / 2) + d / 2);
       const float4 s4 = *reinterpret_cast<const float4*>(p.sin_t + (size_t)pos * (kRowDim / 2) + d / 2);
-      const float cs[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
+      const uint64_t cs[2] = {pack2(c4.x, c4.y), pack2(c4.z, c4.w)}, sn[2] = {pack2(s4.x, s4.y), pack2(s4.z, s4.w)};
+      // Each product is rounded: which 4-bit integer a value becomes does not depend on how a compiler joins them.  It does join packed products with
+      // packed sums, .rn or not (results a bit off), and leaves the single sums alone, which the bit-for-bit tests hold it to.
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {    // (each product rounded: which 4-bit integer a value becomes does not depend on how a compiler joins them)
-        const float x0 = x[2 * i], x1 = x[2 * i + 1];
-        x[2 * i] = __fsub_rn(__fmul_rn(x0, cs[i]), __fmul_rn(x1, sn[i]));
-        x[2 * i + 1] = __fadd_rn(__fmul_rn(x0, sn[i]), __fmul_rn(x1, cs[i]));
+      for (int i = 0; i < 8; i += 4) {
+        const uint64_t x0 = pack2(x[i], x[i + 2]), x1 = pack2(x[i + 1], x[i + 3]), c = cs[i / 4], s = sn[i / 4];
+        float a0, a1, b0, b1;
+        unpack2(mul2(x0, c), a0, a1);
+        unpack2(mul2(x1, s), b0, b1);
+        x[i] = __fsub_rn(a0, b0), x[i + 2] = __fsub_rn(a1, b1);
+        unpack2(mul2(x0, s), a0, a1);
+        unpack2(mul2(x1, c), b0, b1);
+        x[i + 1] = __fadd_rn(a0, b0), x[i + 3] = __fadd_rn(a1, b1);
       }
     }
     const bool key = head < p.n_heads + p.n_kv;

@@ -14,6 +14,29 @@ constexpr int kQ4Block = 32;           // values that share a scale
 constexpr int kQ4HeadBytes = kRowDim / 2, kQ4HeadScales = kRowDim / kQ4Block;
 __host__ __device__ inline size_t q4_row_bytes(size_t n_kv) { return (n_kv * (kQ4HeadBytes + 2 * kQ4HeadScales) + 15) / 16 * 16; }
 
+// Two f32 numbers in one operation.  (A product that goes into a sum may come out as one fused operation.)
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // A pool's state and a list of sequences whose last positions are packed rows (include/tangq.h: tq_kv_append_paged).
 struct PackedSeqs {
   const int *tables, *lens, *refs, *refused;           // of the pool
