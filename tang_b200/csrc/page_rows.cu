@@ -60,10 +60,10 @@ __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float s) {
 
 // A CTA takes ROWS rows and 128 eighths of a head: 32 bytes (f32) in, 16 or 4 out for a thread and row.  Rows' places are looked up by a warp each
 // (starts, sequence, length, page, holders: five loads one after the other) while the values are on their way.  What bounds it: the bytes (5000 rows of 32 + 16
-// heads f32 to bf16 pages, 200 MB, 35.0 us, 5.7 TB/s), beside the look-ups (CTAs of 256 threads 37.1, of 512 44.1; eight rows each 47.2); to 4 bits instructions
-// (5800 rows from bf16 28 us, 30 with single products and
-// quotients; two groups of columns a thread, for half as many look-ups, 32; one warp's lanes for all rows' look-ups no difference).
-// With its reading back: four rows 37.0, two 39.2, three 37.7, four in shared memory by cp.async 39.0.  A single row 4.2 us.
+// heads f32 to bf16 pages, 200 MB, 35.0 us, 5.7 TB/s), beside the look-ups (CTAs of 256 threads 37.1, of 512 44.1; eight rows each 47.2); to 4 bits
+// instructions and loads on their way (5800 rows from bf16 28 us, 30 with single products and quotients; two groups of columns a thread, for half as many
+// look-ups, 32; one warp's lanes for all rows' look-ups no difference).  With its reading back: four rows 37.0, two 39.2, three 37.7, four in shared memory by
+// cp.async 39.0.  A single row 4.2 us.
 template <typename X, int ROWS, bool Q4>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
   __shared__ int place_s[ROWS], pos_s[ROWS];           // cache row (-1: none), position
