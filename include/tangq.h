@@ -313,7 +313,8 @@ TQ_API int tq_gqa_decode_paged(tq_ctx* ctx, const void* q_dev, const void* k_pag
  * seq_rows[i+1]-1 ([batch + 1] device values that ascend from 0 to at most `rows`; NULL: row i, and rows = batch) are the last positions of sequence
  * seqs[i] of the pool (NULL: i), which tq_pages_extend has counted already.  Rows from seq_rows[batch] on are left as they are, so that a recorded
  * step may have room for more rows than it has.  batch is at most 1024, head_dim 128; arrays are 16-byte aligned.  What does not fit (starts that do not
- * ascend, a sequence or page that does not exist, more rows than positions) is reported by tq_sync and left out.
+ * ascend from 0, a sequence or page that does not exist, more rows than positions) is reported by tq_sync and left out, by all calls alike: where starts do not
+ * ascend, rows remain a sequence's if no start before theirs is larger (the first sequence's: if it is 0) and they end neither before they begin nor behind `rows`.
  *
  * A cache row holds all KV heads of a position: bf16, or 4 bits in tq_q4_row_bytes(n_kv_heads) bytes.  Those are, for each head, 64 bytes of codes (byte i has
  * value 2i in its low and value 2i+1 in its high four bits, an integer of -7 .. 7 stored as 8 more), then for each head four bf16 scales, one for 32 values, then

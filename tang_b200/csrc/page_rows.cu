@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
 #pragma unroll
       for (int i = 0; i < (int)sizeof(X) / 2; ++i) raw[r][i] = src[i];
     }
+  if (blockIdx.x == 0 && blockIdx.y == 0 && warp == kAppendThreads / 32 - 1 && !packed_starts_sound(p.s, lane) && lane == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
   if (warp < ROWS) {
     int place = -1, pos = 0;
     if (m0 + warp < p.s.rows) {
@@ -199,6 +200,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_read_kernel(const ReadParam
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m0 = blockIdx.x * ROWS;
+  if (blockIdx.x == 0 && warp == kAppendThreads / 32 - 1 && !packed_starts_sound(p.s, lane) && lane == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
   if (warp < ROWS) {
     int place = -1;
     if (m0 + warp < p.s.rows) {

@@ -129,17 +129,34 @@ __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, i
       len = s < 0 ? 0 : p.s.lens[s];
     }
   } else {
-    int before = 0;
-    bool bad = false;
+    int before = 0, largest = 0;       // tiles of the sequences before; the largest start so far, where some do not ascend
+    bool bad = false, ascend = true;   // (packed_row has the rule)
     for (int base = 0; base < p.s.batch; base += 32) {
       const int j = base + lane;
       int f = 0, c = 0, js = -1, jl = 0;
+      bool down = false;
       if (j < p.s.batch) {
         const int a = p.s.seq_rows[j], b = p.s.seq_rows[j + 1];
         js = packed_seq(p.s, j);       // (on their way beside the starts)
         jl = js < 0 ? 0 : p.s.lens[js];
-        if (a < 0 || b < a || b > p.s.rows || (j == 0 && a != 0)) bad = true;
-        else f = a, c = b - a;
+        down = b < a;
+        f = a;
+        c = down || a < 0 || b > p.s.rows || (j == 0 && a != 0) ? 0 : b - a;
+        bad = bad || down || b > p.s.rows || (j == 0 && a != 0);
+      }
+      if (ascend) ascend = !__any_sync(0xffffffffu, down);
+      if (!ascend) {                   // the largest start before a sequence's own
+        int most = j < p.s.batch ? f : -0x7fffffff - 1;
+        if (lane == 0 && base > 0) most = max(most, largest);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int w = __shfl_up_sync(0xffffffffu, most, o);
+          if (lane >= o) most = max(most, w);
+        }
+        if (most != f) c = 0;
+        largest = __shfl_sync(0xffffffffu, most, 31);
+      } else {
+        largest = __shfl_sync(0xffffffffu, f, 31);     // (of a last, shorter round: not looked at again)
       }
       const int tiles = (c + p.per_tile - 1) / p.per_tile;
       int incl = tiles;
