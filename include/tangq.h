@@ -452,7 +452,8 @@ TQ_API int tq_llama_prefill(tq_llama* model, const int* token_ids_dev, const int
 
 /* The same for prompts, or portions of prompts, of different lengths over a pool whose pages are rows of the model's caches (as in tq_llama_decode_paged):
  * token_ids [rows] packed, sequences and starts as in tq_kv_append_paged, for which tq_pages_extend has made room.  max_len (at most max_seq) bounds the
- * sequences' lengths; positions below it may be cached already, shared with others or not.  logits [batch, vocab] are those of each sequence's last row (those of
+ * sequences' lengths: rows of positions from there on are reported by tq_sync and not written to the caches.  Positions below it may be cached already, shared with
+ * others or not.  logits [batch, vocab] are those of each sequence's last row (those of
  * a sequence without rows mean nothing).  batch is at most max_batch.  Workspaces grow on first use: not inside a graph capture. */
 TQ_API int tq_llama_prefill_paged(tq_llama* model, const int* token_ids_dev, const tq_pages* pages, const int* seqs_dev_or_null,
                                   const int* seq_rows_dev_or_null, size_t batch, size_t rows, size_t max_len, float* logits_dev);

@@ -494,7 +494,8 @@ int tq_llama_prefill_paged(tq_llama* m, const int* token_ids_dev, const tq_pages
     TQ_STEP(tq_rms_norm(ctx, have_delta ? (const void*)m->p_delta : (const void*)m->p_h, TQ_F32, have_delta ? m->p_h : nullptr,
                         L.attn_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, have_delta ? m->p_h : nullptr));
     TQ_STEP(tq_qlinear(ctx, L.wqkv, m->p_xn, TQ_BF16, d, R, m->p_qkv, TQ_F32, q_dim + 2 * kv_dim, nullptr));
-    TQ_STEP(tq_kv_append_paged(ctx, m->p_qkv, TQ_F32, 0, m->cos_t, m->sin_t, c.max_seq, pages, seqs_dev, seq_rows_dev, batch, R, m->heads_l, m->kv_l, hd, m->p_qb,
+    // (max_len for the tables' length: a position that the attention would not see is reported and not written)
+    TQ_STEP(tq_kv_append_paged(ctx, m->p_qkv, TQ_F32, 0, m->cos_t, m->sin_t, max_len, pages, seqs_dev, seq_rows_dev, batch, R, m->heads_l, m->kv_l, hd, m->p_qb,
                                L.k_cache, L.v_cache, TQ_PAGES_BF16));
     TQ_STEP(tq_gqa_prefill_paged(ctx, m->p_qb, L.k_cache, L.v_cache, TQ_PAGES_BF16, pages, seqs_dev, seq_rows_dev, batch, R, m->heads_l, m->kv_l, hd, max_len,
                                  m->p_attn));
