@@ -64,8 +64,9 @@ __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float s) {
 // instructions and loads on their way (5800 rows from bf16 28 us, 30 with single products and quotients; two groups of columns a thread, for half as many
 // look-ups, 32; one warp's lanes for all rows' look-ups no difference).  With its reading back: four rows 37.0, two 39.2, three 37.7, four in shared memory by
 // cp.async 39.0.  A single row 4.2 us.
+// (CTAs of an SM: what the values alone take; without the bound the look-up takes four registers and two CTAs more, appending and reading back 39.7 instead of 38.7.)
 template <typename X, int ROWS, bool Q4>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, ROWS == 1 ? 16 : sizeof(X) == 2 ? 12 : 9) kv_append_kernel(const AppendParams p) {
   __shared__ int place_s[ROWS], pos_s[ROWS];           // cache row (-1: none), position
   pdl_wait();
   pdl_launch_dependents();
@@ -79,12 +80,11 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
 #pragma unroll
       for (int i = 0; i < (int)sizeof(X) / 2; ++i) raw[r][i] = src[i];
     }
-  if (blockIdx.x == 0 && blockIdx.y == 0 && warp == kAppendThreads / 32 - 1 && !packed_starts_sound(p.s, lane) && lane == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
   if (warp < ROWS) {
     int place = -1, pos = 0;
     if (m0 + warp < p.s.rows) {
       const PackedRow row = packed_row(p.s, m0 + warp, lane);
-      int why = row.bad ? (int)DERR_PAGE_LIST : 0, page = 0, same = 0;
+      int why = 0, page = 0, same = 0;
       if (row.seq >= 0) {
         const int refused = p.s.refused[row.seq];      // (on its way beside the page)
         pos = row.pos;
@@ -101,10 +101,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
           if (same != 1 || refused != 0 || p.s.refs[page] != 1) why = DERR_PAGE_LIST;
         }
       }
-      if (why) {
-        place = -1;
-        if (lane == 0 && blockIdx.y == 0) atomicCAS(p.err, 0, why);
-      }
+      if (why) place = -1;
+      if ((why || row.bad) && lane == 0 && blockIdx.y == 0) atomicCAS(p.err, 0, why ? why : (int)DERR_PAGE_LIST);
     }
     if (lane == 0) {
       place_s[warp] = place;
@@ -200,7 +198,6 @@ __global__ void __launch_bounds__(kAppendThreads) kv_read_kernel(const ReadParam
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m0 = blockIdx.x * ROWS;
-  if (blockIdx.x == 0 && warp == kAppendThreads / 32 - 1 && !packed_starts_sound(p.s, lane) && lane == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
   if (warp < ROWS) {
     int place = -1;
     if (m0 + warp < p.s.rows) {

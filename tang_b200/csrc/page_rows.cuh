@@ -59,61 +59,45 @@ __device__ __forceinline__ int packed_seq(const PackedSeqs& p, int i) {
 struct PackedRow {
   int seq, pos;                        // of the pool (-1: nowhere), position
   int i;                               // of the list
-  bool bad;                            // there is something to report
+  bool bad;                            // there is something to report: about this row, or the starts as a whole
 };
 // Starts need not be what they should be: they are the device's.  Rows seq_rows[i] .. seq_rows[i+1]-1 are sequence i's if no start before seq_rows[i] is larger (the first
 // one is 0) and they end neither before they begin nor behind the last row; such rows are never two sequences'.  Every kernel goes by that, whatever else the list
 // holds, so that a row which is appended is attended, and one which is not is left alone by all of them.
 //
-// Row m's, by a whole warp.  Rows behind the last sequence are nowhere, and that is nothing to report.
+// Row m's, by a whole warp.  Rows behind the last sequence are nowhere, and that is nothing to report; a list with something to report need not be the row's fault.
 __device__ __forceinline__ PackedRow packed_row(const PackedSeqs& p, int m, int lane) {
   PackedRow r{-1, 0, m, false};
   int first = m, count = 1;
   if (p.seq_rows) {
-    int behind = -1, largest = -0x7fffffff - 1;        // the first start behind the row; the largest of those before that one
-    for (int base = 0; base <= p.batch && behind < 0; base += 128) {
-      int start[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int j = base + 32 * k + lane;
-        start[k] = j <= p.batch ? p.seq_rows[j] : -0x7fffffff - 1;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const unsigned hit = __ballot_sync(0xffffffffu, start[k] > m);
-        if (behind < 0) {
-          if (hit) behind = base + 32 * k + __ffs(hit) - 1;
-          if (!hit || lane < __ffs(hit) - 1) largest = max(largest, start[k]);
-        }
-      }
+    unsigned seen = 0;                 // starts at or before the row; from bit 16 on, those that are not what they should be
+#pragma unroll 4
+    for (int j = lane; j <= p.batch; j += 32) {
+      const int start = p.seq_rows[j], next = j < p.batch ? p.seq_rows[j + 1] : p.rows;
+      seen += (start <= m) + (start > next || (j == 0 && start != 0) ? 1u << 16 : 0u);
     }
-    if (behind < 0) return r;
-    r.bad = behind == 0;
-    if (r.bad) return r;
+    seen = __reduce_add_sync(0xffffffffu, seen);
+    int behind = seen & 0xFFFFu;       // the first start behind the row
+    r.bad = seen >> 16;
+    int largest = 0;                   // (of the starts before it: its neighbour, where they ascend)
+    if (r.bad) {
+      for (behind = 0; behind <= p.batch && p.seq_rows[behind] <= m; ++behind) largest = max(largest, p.seq_rows[behind]);
+    }
+    if (behind > p.batch || behind == 0) return r;
     r.i = behind - 1;
     first = p.seq_rows[r.i];
     const int end = p.seq_rows[behind];
     count = end - first;
-    r.bad = first < 0 || end > p.rows || (r.i == 0 && first != 0) || __reduce_max_sync(0xffffffffu, largest) != first;
-    if (r.bad) return r;
+    if (r.bad && (first != largest || (r.i == 0 && first != 0) || end > p.rows)) return r;
   }
   const int s = packed_seq(p, r.i), len = s < 0 ? 0 : p.lens[s];
-  r.bad = s < 0 || len < count || len > (long long)p.table_ld << p.page_shift;
-  if (r.bad) return r;
+  if (s < 0 || len < count || len > (long long)p.table_ld << p.page_shift) {
+    r.bad = true;
+    return r;
+  }
   r.seq = s;
   r.pos = len - count + (m - first);
   return r;
-}
-
-// Whether all starts are what they should be, by a whole warp: what is wrong with them need not stand at a row that there is.
-__device__ __forceinline__ bool packed_starts_sound(const PackedSeqs& p, int lane) {
-  bool sound = true;
-  if (p.seq_rows)
-    for (int j = lane; j <= p.batch; j += 32) {
-      const int before = j ? p.seq_rows[j - 1] : 0, start = p.seq_rows[j];
-      sound = sound && start >= before && start <= p.rows && (j || start == 0);
-    }
-  return __all_sync(0xffffffffu, sound);
 }
 
 // Cache row of a position, the cache seen as one; -1 where the table names a page that does not exist.

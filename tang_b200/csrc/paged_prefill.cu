@@ -129,25 +129,25 @@ __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, i
       len = s < 0 ? 0 : p.s.lens[s];
     }
   } else {
-    int before = 0, largest = 0;       // tiles of the sequences before; the largest start so far, where some do not ascend
-    bool bad = false, ascend = true;   // (packed_row has the rule)
+    int before = 0, largest = 0;       // tiles of the sequences before; the largest start so far, once some are not as they should be
+    bool bad = false;
     for (int base = 0; base < p.s.batch; base += 32) {
       const int j = base + lane;
-      int f = 0, c = 0, js = -1, jl = 0;
-      bool down = false;
+      int f = -0x7fffffff - 1, c = 0, js = -1, jl = 0;
+      bool odd = false;
       if (j < p.s.batch) {
-        const int a = p.s.seq_rows[j], b = p.s.seq_rows[j + 1];
+        const int b = p.s.seq_rows[j + 1];
+        f = p.s.seq_rows[j];
         js = packed_seq(p.s, j);       // (on their way beside the starts)
         jl = js < 0 ? 0 : p.s.lens[js];
-        down = b < a;
-        f = a;
-        c = down || a < 0 || b > p.s.rows || (j == 0 && a != 0) ? 0 : b - a;
-        bad = bad || down || b > p.s.rows || (j == 0 && a != 0);
+        odd = f < 0 || b < f || b > p.s.rows || (j == 0 && f != 0);
+        c = odd ? 0 : b - f;
       }
-      if (ascend) ascend = !__any_sync(0xffffffffu, down);
-      if (!ascend) {                   // the largest start before a sequence's own
-        int most = j < p.s.batch ? f : -0x7fffffff - 1;
-        if (lane == 0 && base > 0) most = max(most, largest);
+      const bool was = bad;
+      bad = bad || __any_sync(0xffffffffu, odd);
+      if (bad) {                       // (packed_row has the rule)
+        int most = f;
+        if (lane == 0 && base > 0) most = max(most, was ? largest : p.s.seq_rows[base - 1]);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int w = __shfl_up_sync(0xffffffffu, most, o);
@@ -155,8 +155,6 @@ __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, i
         }
         if (most != f) c = 0;
         largest = __shfl_sync(0xffffffffu, most, 31);
-      } else {
-        largest = __shfl_sync(0xffffffffu, f, 31);     // (of a last, shorter round: not looked at again)
       }
       const int tiles = (c + p.per_tile - 1) / p.per_tile;
       int incl = tiles;
@@ -178,7 +176,7 @@ __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, i
       before += __shfl_sync(0xffffffffu, incl, 31);
       if (i >= 0 && x > 0) break;      // (the first tile's CTAs look at all starts)
     }
-    if (__any_sync(0xffffffffu, bad) && lane == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
+    if (bad && lane == 0) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
   }
   if (i < 0) return it;
   if (s < 0 || len < count || len > (long long)p.s.table_ld << p.s.page_shift) {
