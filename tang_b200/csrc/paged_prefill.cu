@@ -4,6 +4,9 @@
 //   warp 0        queries, then blocks of keys: tensor copies page by page, or, for pages of 4 bits, codes that it turns into the same bf16 rows
 //   warp 1        issues the products: a block's S = Q K^T (both from shared memory), then O += P V of the block before (P from tensor memory, V N-major)
 //   warp 2        blocks of values, likewise; rows behind the last key are zeros (whatever a page holds there must not meet a weight of zero)
+//                 (values of keys that not all rows of the tile see, 127 keys at most, are looked at: those that are no number are zeros too, and are added to
+//                 the results of the rows that see them.  Rows that met such a value attended again over all of their keys, by a warp while the others
+//                 waited, took a time that grew with the sequence and could outlast the waits' limit)
 //   warp 3        finds out what the CTA does: its own tile, then those that it takes over from CTAs of the grid that have not begun (the hardware
 //                 hands them out one by one), looked up while the tile before is worked on
 //   warps 4..7    softmax, a thread a row, and the results
@@ -20,6 +23,7 @@
 // up to 1237 81 us; a few rows are a chain of blocks of 0.8 to 1 us (64 behind 2000 keys 16.4 us, one block 8.2).  Scores of 128 keys at a time, which cost the
 // tensor core less, wait for the products of the tile before: 167 us.
 #include <cfloat>
+#include <type_traits>
 
 #include "attn_mma.cuh"
 #include "attn_umma.cuh"
@@ -34,6 +38,7 @@ constexpr int kPpBox = kPpBlock * 128;                // bytes of a block's 64 c
 constexpr int kPpTile = 2 * kPpBox;
 constexpr int kPpItems = 2;                            // tiles that the roles are told ahead
 constexpr int kPpAhead = 2;                            // the next tile is asked for when so many blocks of keys are still to be copied
+constexpr int kPpStored = 4;                          // a tile's values are all there at most two tiles before its results are stored
 constexpr int kPpReaders = 7;                         // warps that are told
 constexpr int kPpStage = 32 * 64;                     // bytes of results that a warp stores at a time
 constexpr size_t kPpSmem = 1024 + 1024 + 2 * (size_t)kPfBox + 2 * kPpSlots * (size_t)kPpTile + 4 * (size_t)kPpStage;
@@ -71,43 +76,31 @@ __device__ __forceinline__ void row_values(const uint8_t* row, int n_kv, int hea
   }
 }
 
-// One row's softmax attention over keys first .. end - 1 (first a multiple of 4) by a warp, four keys at a time, for the rows of a tile that met, with a weight of
-// zero, a value of a key that they do not see and that is no number: zero times that is NaN.  Lane i has values 4 i .. of the query and of the sums.
-template <bool Q4>
-__device__ __forceinline__ void attend_paged_row(const PackedPrefillParams& p, int seq, int kv, int first, int end, const float (&q)[4], int lane, float& top, float& l,
-                                                 float (&acc)[4]) {
-#pragma unroll 1
-  for (int j0 = first; j0 < end; j0 += 4) {            // (of one page: pages have 16 rows or more)
-    const int place = max(page_row_of(p.s, seq, j0), 0);
-    float s[4], v[4][4], mn = top;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float k[4];
-      row_values<Q4>(p.k + (size_t)(place + i) * p.row_bytes, p.n_kv, kv, lane, k);
-      row_values<Q4>(p.v + (size_t)(place + i) * p.row_bytes, p.n_kv, kv, lane, v[i]);
-      s[i] = 0.f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) s[i] = fmaf(q[c], k[c], s[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[i] = warp_sum(s[i]) * p.scale_log2;
-      if (j0 + i < end) mn = fmaxf(mn, s[i]);
-    }
-    const float f = ex2(top - mn);
-    top = mn;
-    l *= f;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) acc[c] *= f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (j0 + i < end) {
-        const float w = ex2(s[i] - mn);
-        l += w;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[c] = fmaf(w, v[i][c], acc[c]);
-      }
+// Values that are no number, of keys lo .. hi - 1 of a block in shared memory, become zeros, by a warp; says whether there were any.
+__device__ __forceinline__ bool pp_zero_values(uint8_t* tile, int lo, int hi, int lane) {
+  // (a lane: 16 bytes of every other key, whatever their order in its half of the columns)
+  uint8_t* mine = tile + ((lane >> 3) & 1) * kPpBox + (lo + (lane >> 4)) * 128 + 16 * (lane & 7);
+  const int n = (hi - lo + 1 - (lane >> 4)) >> 1;
+  uint32_t z[2] = {0u, 0u};            // products with zero: NaN if there is one, or an infinity
+#pragma unroll 4
+  for (int k = 0; k < n; ++k) {
+    const uint4 x = *reinterpret_cast<const uint4*>(mine + 256 * k);
+    z[0] = bf16x2_fma(x.x, 0u, z[0]);
+    z[1] = bf16x2_fma(x.y, 0u, z[1]);
+    z[0] = bf16x2_fma(x.z, 0u, z[0]);
+    z[1] = bf16x2_fma(x.w, 0u, z[1]);
   }
+  const uint32_t nan = ((z[0] & 0x7FFF7FFFu) + 0x007F007Fu) | ((z[1] & 0x7FFF7FFFu) + 0x007F007Fu);
+  if (!__any_sync(0xffffffffu, (nan & 0x80008000u) != 0)) return false;
+#pragma unroll 1
+  for (int k = 0; k < n; ++k) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(mine + 256 * k);
+    for (int i = 0; i < 4; ++i) {
+      if ((w[i] & 0x7F80u) == 0x7F80u) w[i] &= 0xFFFF0000u;
+      if ((w[i] & 0x7F800000u) == 0x7F800000u) w[i] &= 0xFFFFu;
+    }
+  }
+  return true;
 }
 
 // What a CTA does.
@@ -284,6 +277,40 @@ __device__ __forceinline__ bool answered_cta(uint32_t answer, int& x, int& y, in
   return ok != 0;
 }
 
+// Values that were made zeros, to the results of the tile's rows that see them, by a warp: a weight is positive, so that an infinity stays one.
+template <bool Q4>
+__device__ __forceinline__ void pp_give_back(const PackedPrefillParams& p, int seq, int kv, int part, int row0, int rows, int pos0, int first, int end) {
+  const int lane = threadIdx.x & 31;
+  int key = max(pos0 + 1, first);
+  float seen[4] = {0.f, 0.f, 0.f, 0.f};                // of the lane's four columns, the keys up to a position
+#pragma unroll 1
+  for (int r = 0; r < rows; ++r) {
+#pragma unroll 1
+    for (const int behind = min(min(pos0 + r, p.max_len - 1) + 1, end); key < behind; ++key) {
+      float v[4];
+      row_values<Q4>(p.v + (size_t)max(page_row_of(p.s, seq, key), 0) * p.row_bytes, p.n_kv, kv, lane, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!(fabsf(v[i]) <= FLT_MAX)) seen[i] += v[i];
+    }
+    if (!__any_sync(0xffffffffu, seen[0] != 0.f || seen[1] != 0.f || seen[2] != 0.f || seen[3] != 0.f)) continue;
+#pragma unroll 1
+    for (int h = 0; h < p.group; ++h) {
+      const size_t at = ((size_t)(row0 + r) * p.n_heads + kv * p.group + h) * kRowDim + 4 * lane;
+      if (p.parts > 1) {
+        float4* to = reinterpret_cast<float4*>(p.part_o + (size_t)part * p.s.rows * p.n_heads * kRowDim + at);
+        const float4 x = *to;
+        *to = make_float4(x.x + seen[0], x.y + seen[1], x.z + seen[2], x.w + seen[3]);
+      } else {
+        uint2* to = reinterpret_cast<uint2*>(p.out + at);
+        const uint2 x = *to;
+        *to = make_uint2(pack_bf16(__uint_as_float(x.x << 16) + seen[0], __uint_as_float(x.x & 0xFFFF0000u) + seen[1]),
+                         pack_bf16(__uint_as_float(x.y << 16) + seen[2], __uint_as_float(x.y & 0xFFFF0000u) + seen[3]));
+      }
+    }
+  }
+}
+
 template <bool Q4>
 __global__ void __launch_bounds__(kPpThreads, 2)
 paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -305,7 +332,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
   uint64_t* item_empty = item_full + kPpItems;
   uint64_t* answer_bar = item_empty + kPpItems;
   uint64_t* nearly = answer_bar + 1;                  // a tile's last keys but a few have been asked for
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(nearly + 1);
+  uint64_t* stored = nearly + 1;                      // [kPpStored] a tile's results have been stored
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stored + kPpStored);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
   PpItem* item_s = reinterpret_cast<PpItem*>(smem_raw + 512);
   const uint32_t answer = smem_u32(smem_raw) + 768;
@@ -319,6 +347,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
       mbar_init(o_free, 4);
       mbar_init(answer_bar, 1);
       mbar_init(nearly, 1);
+      for (int i = 0; i < kPpStored; ++i) mbar_init(&stored[i], 4);
       for (int i = 0; i < kPpItems; ++i) {
         mbar_init(&item_full[i], 1);
         mbar_init(&item_empty[i], kPpReaders);
@@ -415,7 +444,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
       uint8_t* to = values ? v_s : k_s;
       const int box_rows = min(1 << p.s.page_shift, kPpBlock), boxes = kPpBlock / box_rows;
       bool ok = true;
-      int run = 0, tiles = 0, cuts = 0;                // blocks, tiles with keys, and last blocks with rows to zero so far
+      int run = 0, tiles = 0, cuts = 0;                // blocks, tiles with keys, and blocks of values that the warp has waited for so far
       PpItem it;
       while (take(ok, it)) {
         const int n = it.blocks, call = max(n - kPpAhead, 0);
@@ -423,6 +452,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
           if (!values) arrive(nearly);
           continue;
         }
+        // Values of keys that some rows of the tile do not see meet weights of zero, and zero times a value that is no number is NaN.  They are zeros for all rows,
+        // then; those that do see them get them back when the results are there.
+        bool bad = false;
         const int* table = p.s.tables + (size_t)it.seq * p.s.table_ld;
         if (!values) {
           ok = __all_sync(0xffffffffu, mbar_wait_spin(q_empty, (uint32_t)(tiles & 1) ^ 1u));
@@ -459,16 +491,28 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
             }
             return x;
           };
+          auto turn = [&](uint8_t* tile, int row, int m, PpCodes& x) {
+            if (values && key0 + 32 * m > it.pos0) {   // (behind the last key: scales of zero)
+              auto no_number_at = [](uint32_t w, uint32_t e) { return (w & e) == e; };
+              const bool no_number[4] = {no_number_at(x.s.x, 0x7F80u), no_number_at(x.s.x, 0x7F800000u), no_number_at(x.s.y, 0x7F80u), no_number_at(x.s.y, 0x7F800000u)};
+              if (no_number[0] || no_number[1] || no_number[2] || no_number[3]) {
+                bad = true;
+                x.s = make_uint2((no_number[0] ? 0u : x.s.x & 0xFFFFu) | (no_number[1] ? 0u : x.s.x & 0xFFFF0000u),
+                                 (no_number[2] ? 0u : x.s.y & 0xFFFFu) | (no_number[3] ? 0u : x.s.y & 0xFFFF0000u));
+              }
+            }
+            pp_convert(tile, row, x);
+          };
           PpCodes even = codes_at(0, page_at(0)), odd = codes_at(1, page_at(1));
           int even_page = page_at(2), odd_page = page_at(3);
           for (int i = 0; i < n && ok; ++i, ++run) {
             const int slot = run % kPpSlots;
             ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)(run / kPpSlots & 1) ^ 1u));
             if (!ok) break;
-            pp_convert(to + slot * kPpTile, lane, even);
+            turn(to + slot * kPpTile, lane, 2 * i, even);
             even = codes_at(2 * i + 2, even_page);
             even_page = page_at(2 * i + 4);
-            pp_convert(to + slot * kPpTile, 32 + lane, odd);
+            turn(to + slot * kPpTile, 32 + lane, 2 * i + 1, odd);
             odd = codes_at(2 * i + 3, odd_page);
             odd_page = page_at(2 * i + 5);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -494,23 +538,33 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
             const int row = (page << p.s.page_shift) + (key & ((1 << p.s.page_shift) - 1) & ~(box_rows - 1));
             ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[slot], (uint32_t)(run / kPpSlots & 1) ^ 1u));
             if (!ok) break;
-            const bool cut = values && keys < kPpBlock;
+            const int unseen = max(it.pos0 + 1 - key, 0);              // keys from there on are not seen by the first row
+            const bool cut = values && (keys < kPpBlock || unseen < keys);
             uint64_t* bar = cut ? v_raw : &full[slot];
             if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(used * box_rows) * 256u);
             __syncwarp();
             if (j < used) tma_load_2d(to + slot * kPpTile + c * kPpBox + j * box_rows * 128, values ? &v_map : &k_map, it.kv * kRowDim + 64 * c, row, bar);
             __syncwarp();
             if (!values && i == call) arrive(nearly);
-            if (cut) {                 // (the tile's last block)
+            if (cut) {                 // (the tile's last block, or those that its rows end in)
               ok = __all_sync(0xffffffffu, mbar_wait_spin(v_raw, (uint32_t)(cuts++ & 1)));
               if (!ok) break;
               uint8_t* at = to + slot * kPpTile;
+              if (unseen < keys) bad = pp_zero_values(at, unseen, keys, lane) || bad;
               for (int k = lane; k < 2 * (kPpBlock - keys) * 8; k += 32)     // (a row's 128 bytes of either box, whatever their order)
                 *reinterpret_cast<uint4*>(at + ((k >> 3) & 1) * kPpBox + (keys + (k >> 4)) * 128 + 16 * (k & 7)) = make_uint4(0u, 0u, 0u, 0u);
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
               arrive(&full[slot]);
             }
           }
+        }
+        if (values) {
+          if (__any_sync(0xffffffffu, ok && bad)) {
+            ok = __all_sync(0xffffffffu, mbar_wait_spin(&stored[tiles % kPpStored], (uint32_t)(tiles / kPpStored & 1)));
+            if (!ok) break;
+            pp_give_back<Q4>(p, it.seq, it.kv, it.part, it.row0, it.rows, it.pos0, it.block0 * kPpBlock, min((it.block0 + n) * kPpBlock, it.k_end));
+          }
+          ++tiles;
         }
       }
       if (!ok && lane == 0) give_up(DERR_EMPTY_WAIT);
@@ -578,7 +632,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
     const bool parts = p.parts > 1;
     uint8_t* mine_s = stage_s + q4 * kPpStage;
     bool ok = true;
-    int run = 0;                       // blocks before this tile
+    int run = 0, tiles = 0;            // blocks and tiles with keys before this one
     PpItem it;
     while (take(ok, it)) {
       const int n = it.blocks, head = it.kv * p.group + r_head;
@@ -668,90 +722,59 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
       if (parts && live) *reinterpret_cast<float2*>(p.part_ml + (part_at + at) / (kRowDim / 2)) = make_float2(m, l);
       if (n) {
         const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-        float zero[4] = {0.f, 0.f, 0.f, 0.f};           // NaN if some sum is not finite
         // Rows go over shared memory 64 bytes at a time, so that four lanes store what stands together (a lane with a row of its own would store to 32 places at once).
+        // Code of its own for parts (f32) and results (bf16): left to the compiler, which of them it writes changes with what stands around it, 4 % of many short prompts.
         const unsigned to_store = __ballot_sync(0xffffffffu, live);
-        const int columns = parts ? 16 : 32;
-        uint8_t* base = parts ? reinterpret_cast<uint8_t*>(p.part_o + part_at) : reinterpret_cast<uint8_t*>(p.out);
-        const unsigned long long row_bytes_at = (unsigned long long)at * (parts ? 4 : 2);
-        unsigned long long to[4];
+        auto store = [&](auto of_parts) {
+          constexpr bool PARTS = decltype(of_parts)::value;
+          uint8_t* base = PARTS ? reinterpret_cast<uint8_t*>(p.part_o + part_at) : reinterpret_cast<uint8_t*>(p.out);
+          const unsigned long long row_bytes_at = (unsigned long long)at * (PARTS ? 4 : 2);
+          unsigned long long to[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, row_bytes_at, 8 * k + (lane >> 2)) + 16 * (lane & 3);
+          for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, row_bytes_at, 8 * k + (lane >> 2)) + 16 * (lane & 3);
 #pragma unroll 1
-        for (int c = 0; c < kRowDim; c += 32) {
-          float o[32];
-          __syncwarp();
-          pp_ask(o_t + (uint32_t)c, o);
-          pp_landed(o);
-          if (c == kRowDim - 32) {       // (the next tile's products may begin)
-            tc_fence_before();
-            arrive(o_free);
-          }
+          for (int c = 0; c < kRowDim; c += 32) {
+            float o[32];
+            __syncwarp();
+            pp_ask(o_t + (uint32_t)c, o);
+            pp_landed(o);
+            if (c == kRowDim - 32) {     // (the next tile's products may begin)
+              tc_fence_before();
+              arrive(o_free);
+            }
 #pragma unroll
-          for (int k = 0; k < 32; ++k) zero[k & 3] = fmaf(o[k], 0.f, zero[k & 3]);
+            for (int half = 0; half < (PARTS ? 2 : 1); ++half) {
+              uint8_t* row = mine_s + lane * 64;
+              const int turn = (lane >> 1) & 3;          // (eight lanes' 16 bytes meet all banks)
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (half && !parts) break;
-            uint8_t* row = mine_s + lane * 64;
-            const int turn = (lane >> 1) & 3;            // (eight lanes' 16 bytes meet all banks)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint4 y;
-              if (parts) {
-                y = make_uint4(__float_as_uint(half ? o[16 + 4 * k] : o[4 * k]), __float_as_uint(half ? o[17 + 4 * k] : o[4 * k + 1]),
-                               __float_as_uint(half ? o[18 + 4 * k] : o[4 * k + 2]), __float_as_uint(half ? o[19 + 4 * k] : o[4 * k + 3]));
-              } else {
-                y = make_uint4(pack_bf16(o[8 * k] * inv, o[8 * k + 1] * inv), pack_bf16(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
-                               pack_bf16(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack_bf16(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+              for (int k = 0; k < 4; ++k) {
+                uint4 y;
+                if constexpr (PARTS) {
+                  const float* x = &o[16 * half + 4 * k];
+                  y = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+                } else {
+                  const float* x = &o[8 * k];
+                  y = make_uint4(pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv), pack_bf16(x[4] * inv, x[5] * inv), pack_bf16(x[6] * inv, x[7] * inv));
+                }
+                *reinterpret_cast<uint4*>(row + ((k ^ turn) << 4)) = y;
               }
-              *reinterpret_cast<uint4*>(row + ((k ^ turn) << 4)) = y;
-            }
-            __syncwarp();
-            uint4 y[4];
+              __syncwarp();
+              uint4 y[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int from = 8 * k + (lane >> 2);
-              y[k] = *reinterpret_cast<const uint4*>(mine_s + from * 64 + (((lane & 3) ^ ((from >> 1) & 3)) << 4));
-            }
+              for (int k = 0; k < 4; ++k) {
+                const int from = 8 * k + (lane >> 2);
+                y[k] = *reinterpret_cast<const uint4*>(mine_s + from * 64 + (((lane & 3) ^ ((from >> 1) & 3)) << 4));
+              }
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (to_store >> (8 * k + (lane >> 2)) & 1u) *reinterpret_cast<uint4*>(base + to[k] + (c + 16 * half) / columns * 64) = y[k];
-            __syncwarp();
-          }
-        }
-        zero[0] += zero[1] + (zero[2] + zero[3]);
-        unsigned rows = __ballot_sync(0xffffffffu, live && zero[0] != zero[0]);
-        if (rows) {
-          // The last key with a value that is no number among those that some rows of this tile do not see: rows from its position on see them all.
-          const int first = it.block0 * kPpBlock, end = min((it.block0 + n) * kPpBlock, it.k_end);
-          int last_bad = -1;
-          for (int key = max(it.pos0 + 1, first); key < end; ++key) {
-            float v[4], z = 0.f;
-            row_values<Q4>(p.v + (size_t)max(page_row_of(p.s, it.seq, key), 0) * p.row_bytes, p.n_kv, it.kv, lane, v);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z = fmaf(v[i], 0.f, z);
-            if (__any_sync(0xffffffffu, z != z)) last_bad = key;
-          }
-          rows &= __ballot_sync(0xffffffffu, limit < last_bad);
-#pragma unroll 1
-          while (rows) {
-            const int src = __ffs(rows) - 1;
-            rows &= rows - 1;
-            const int row_limit = __shfl_sync(0xffffffffu, limit, src);
-            const size_t row_at = __shfl_sync(0xffffffffu, (unsigned long long)at, src);
-            float qr[4], rm = -FLT_MAX, rl = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) qr[i] = __bfloat162float(p.q[row_at + 4 * lane + i]);
-            attend_paged_row<Q4>(p, it.seq, it.kv, first, min(end, row_limit + 1), qr, lane, rm, rl, acc);
-            if (parts) {
-              *reinterpret_cast<float4*>(p.part_o + part_at + row_at + 4 * lane) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-              if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + (part_at + row_at) / (kRowDim / 2)) = make_float2(rm, rl);
-            } else {
-              const float rinv = rl > 0.f || rl != rl ? 1.0f / rl : 0.f;
-              *reinterpret_cast<uint2*>(p.out + row_at + 4 * lane) = make_uint2(pack_bf16(acc[0] * rinv, acc[1] * rinv), pack_bf16(acc[2] * rinv, acc[3] * rinv));
+              for (int k = 0; k < 4; ++k)
+                if (to_store >> (8 * k + (lane >> 2)) & 1u) *reinterpret_cast<uint4*>(base + to[k] + (PARTS ? 4 * (c + 16 * half) : 2 * c)) = y[k];
+              __syncwarp();
             }
           }
-        }
+        };
+        if (parts) store(std::true_type{});
+        else store(std::false_type{});
+        arrive(&stored[tiles++ % kPpStored]);
       }
     }
     if (!ok && lane == 0) give_up(DERR_TMEM);

@@ -100,3 +100,124 @@ def test_starts_that_are_not_what_they_should_be(dev, form, long, name):
             assert np.array_equal(q.to_vec().reshape(rows, 4, HD)[a:a + n], bf16_round(np.ascontiguousarray(turned[:, :4]))[0].reshape(n, 4, HD))
     for buf, want in ((s.kb, wants[0]), (s.vb, wants[1])):
         assert np.array_equal(buf.to_vec().reshape(want.shape), want)
+
+
+def spoil(s, which, place, form):
+    """Makes a value of a cache row no number (an infinity or NaN, a block's scale in 4 bits); the columns of the results that it reaches, [heads, 128]."""
+    hit = np.zeros((s.nh, HD), bool)
+    group = s.nh // s.nkv
+    if form == "q4":
+        s.raw[which][place, s.nkv * 64:].view(np.uint16)[4 + 2] = 0x7FC0      # KV head 1, values 64 .. 95
+        hit[group:2 * group, slice(64, 96) if which else slice(None)] = True
+    else:
+        s.raw[which][place, HD + 40] = 0x7F80 if place % 2 else 0x7FC0
+        hit[group:2 * group, 40 if which else slice(None)] = True
+    return hit
+
+
+def near(got, want, size):
+    return (np.abs(got - want) <= 2.0 ** -14 * size + 2.0 ** -8 * (size + np.abs(want)) + 2.0 ** -8 * (np.abs(want) + 2.0 ** -7 * size)).all()
+
+
+@pytest.mark.parametrize("form", ["bf16", "q4"])
+@pytest.mark.parametrize("which", ["keys", "values"])
+@pytest.mark.parametrize("at", [[1999], [1990], [1965], [1960], [1959], [700], [1992, 3], [1963, 1980, 1995]])
+def test_what_is_no_number_where_keys_are_cut_into_parts(dev, form, which, at):
+    """One sequence of 2000 positions, 40 rows, 2 KV heads: two tiles, seven parts each.  Rows that see such a key or value are no numbers where it reaches them
+    (an infinite key that a query makes a score of minus infinity has no weight, and is not missed); the others are what they are."""
+    s = Sequences(8, 2, 32, [2000], [40], 40, form)
+    want, size = s.reference()
+    bad = np.zeros((40, 8, HD), bool)
+    for pos in at:
+        place = s.places(0, [pos])[0]
+        hit = spoil(s, which == "values", place, form)
+        bad[max(pos - 1960, 0):] |= hit
+        if which == "keys":
+            s.values[0][place, 1] = np.nan if form == "q4" else np.where(np.arange(HD) == 40, np.inf if place % 2 else np.nan, s.values[0][place, 1])
+    if which == "keys":
+        with np.errstate(invalid="ignore"):
+            want, size = s.reference()
+        assert np.isnan(want[bad]).any() and np.isfinite(want[~bad]).all()
+        bad = np.isnan(want)
+    s.put(dev)
+    got = widen(s.prefill().to_vec()).reshape(want.shape)
+    dev.sync()
+    assert not np.isfinite(got[bad]).any() and near(got[~bad], want[~bad], size[~bad])
+
+
+@pytest.mark.parametrize("form", ["bf16", "q4"])
+@pytest.mark.parametrize("nh,nkv", [(4, 4), (15, 3), (8, 2), (8, 1)])
+def test_values_that_are_no_number_in_every_position(dev, form, nh, nkv):
+    """Nothing but NaN: every row sees one, in as many tiles as there are, and the heads beside them are what they are."""
+    s = Sequences(nh, nkv, 16, [700, 130, 1], [700, 40, 1], 41, form)
+    want, size = s.reference()
+    bad = np.zeros((nh, HD), bool)
+    for b, n in enumerate(s.lens):
+        at = s.places(b, range(n))
+        if form == "q4":
+            s.raw[1][at, nkv * 64:nkv * 64 + 2] = np.array([0xC0, 0x7F], np.uint8)
+            bad[:nh // nkv, :32] = True
+        else:
+            s.raw[1][at, :HD] = 0x7FC0
+            bad[:nh // nkv] = True
+    s.put(dev)
+    got = widen(s.prefill().to_vec()).reshape(want.shape)
+    dev.sync()
+    assert np.isnan(got[:, bad]).all() and near(got[:, ~bad], want[:, ~bad], size[:, ~bad])
+
+
+def test_infinite_values_stay_infinite(dev):
+    """One is an infinity from its position on; two of different signs are NaN from the second one's on.  Rows before them are finite."""
+    for nh, nkv, c in ((8, 2, 200), (4, 4, 200), (7, 1, 60), (9, 3, 33)):
+        s = Sequences(nh, nkv, 16, [200], [c], 42, "bf16")
+        want, size = s.reference()
+        first = 200 - c
+        up, down = first + c // 3, first + c // 3 + 9
+        for pos, bits in ((up, 0x7F80), (down, 0xFF80)):
+            s.raw[1][s.places(0, [pos])[0], 17] = bits
+        s.put(dev)
+        got = widen(s.prefill().to_vec()).reshape(want.shape)
+        dev.sync()
+        group, column = nh // nkv, got[:, :nh // nkv, 17]
+        assert np.isfinite(column[:up - first]).all() and (column[up - first:down - first] == np.inf).all() and np.isnan(column[down - first:]).all()
+        rest = np.ones(got.shape, bool)
+        rest[up - first:, :group, 17] = False
+        assert near(got[rest], want[rest], size[rest])
+
+
+@pytest.mark.parametrize("form", ["bf16", "q4"])
+def test_values_that_are_no_number_behind_a_long_context(dev, form):
+    """100003 positions and as many new rows as leave a tile's keys in one part: what rows cost that do not see such a value does not grow with the context."""
+    n, c = 100003, 4800
+    s = Sequences(8, 2, 64, [n], [c], 43, form)
+    places = {pos: s.places(0, [pos])[0] for pos in (n - 1, n - 40, n - 3000, n - c + 1)}
+    for place in places.values():
+        hit = spoil(s, 1, place, form)
+    s.put(dev)
+    got = widen(s.prefill().to_vec()).reshape(c, 8, HD)
+    dev.sync()
+    seen = n - c + np.arange(c) >= n - c + 1
+    assert np.isfinite(got[~seen]).all() and np.isfinite(got[:, ~hit]).all() and not np.isfinite(got[seen][:, hit]).any()
+    at = s.places(0, range(n))
+    k, v = s.values[0][at], s.values[1][at]
+    for r in (0, 1, 30, c - 3000, c - 40, c - 1):
+        want, size = attend(s.q[r:r + 1], k[:n - c + r + 1], v[:n - c + r + 1])
+        ok = slice(None) if r == 0 else ~hit
+        assert near(got[r][ok], want[0][ok], size[0][ok])
+
+
+@pytest.mark.parametrize("form", ["bf16", "q4"])
+def test_a_value_that_is_no_number_at_the_end_of_a_long_context(dev, form):
+    """The same where only the last row sees it: all rows before it are finite."""
+    n, c = 60001, 4800
+    s = Sequences(8, 2, 64, [n], [c], 44, form)
+    hit = spoil(s, 1, s.places(0, [n - 1])[0], form)
+    s.put(dev)
+    got = widen(s.prefill().to_vec()).reshape(c, 8, HD)
+    dev.sync()
+    assert np.isfinite(got[:-1]).all() and np.isfinite(got[-1, ~hit]).all() and not np.isfinite(got[-1, hit]).any()
+    at = s.places(0, range(n))
+    k, v = s.values[0][at], s.values[1][at]
+    for r in (c - 2, c - 31):
+        want, size = attend(s.q[r:r + 1], k[:n - c + r + 1], v[:n - c + r + 1])
+        assert near(got[r], want[0], size[0])
