@@ -14,7 +14,8 @@
 // from tile to tile on their own: copies and scores of the next one run while the results of this one are stored (a tile a CTA: look-up, first copies and results
 // took 10000 of 21000 cycles for 8 blocks).  A weight is one bf16 number, and the sum that results are
 // divided by is that of the numbers as they entered: a row of a few keys, where the roundings do not average out, is then nearer (the largest weight need not
-// be 1 for that, so that the reference may lag: a row's sums are rescaled only when its maximum grew by more than 2^8).
+// be 1 for that, so that the reference may lag: a row's sums are rescaled only when its maximum grew by more than 2^8.  It begins 2^8 above the maximum, so that weights
+// are 2^-8 to 1: sums hold what those of weights of at most 1 hold, and values of 2^-110 count).
 // Few rows: a tile's keys are cut into parts, a CTA each, and a second kernel joins the results.
 //
 // What bounds it: products of 128 x 64 x 16 take 48 cycles, the bytes of their operands (32 would do for the multiplications), of 128 x 128 x 16 from tensor memory
@@ -42,7 +43,7 @@ constexpr int kPpStored = 4;                          // a tile's values are all
 constexpr int kPpReaders = 7;                         // warps that are told
 constexpr int kPpStage = 32 * 64;                     // bytes of results that a warp stores at a time
 constexpr size_t kPpSmem = 1024 + 1024 + 2 * (size_t)kPfBox + 2 * kPpSlots * (size_t)kPpTile + 4 * (size_t)kPpStage;
-constexpr float kPpLag = 8.f;                         // a reference may be so far below its row's maximum (log2)
+constexpr float kPpLag = 8.f;                         // how far a row's maximum may grow before its reference does (log2)
 constexpr int kPpMaxParts = 16;
 constexpr int kPpPoly = 4;                            // one of so many pairs of weights is a polynomial
 
@@ -666,14 +667,15 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
           for (int k = 2; k < 16; k += 2) mx[c] = fmaxf(mx[c], fmaxf(v[c >> 1][16 * (c & 1) + k], v[c >> 1][16 * (c & 1) + k + 1]));
         }
         const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2, -FLT_MAX);
+        // (m: 2^8 above the maximum that it follows, so that no weight is above 1 before the maximum has grown so far)
         if (j == 0) {
-          m = top;
-        } else if (__any_sync(0xffffffffu, top > m + kPpLag)) {
+          m = top + kPpLag;
+        } else if (__any_sync(0xffffffffu, top > m)) {
           ok = __all_sync(0xffffffffu, mbar_wait_spin(&o_done[(run + j - 1) & 1], (uint32_t)((run + j - 1) >> 1 & 1)));
           if (!ok) break;
           tc_fence_after();
           __syncwarp();
-          const float m_new = top > m + kPpLag ? top : m, f = ex2(m - m_new);
+          const float m_new = top > m ? top + kPpLag : m, f = ex2(m - m_new);
 #pragma unroll 1
           for (int c = 0; c < kRowDim; c += 16) {
             float o[16];

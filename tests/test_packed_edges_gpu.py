@@ -221,3 +221,48 @@ def test_a_value_that_is_no_number_at_the_end_of_a_long_context(dev, form):
     for r in (c - 2, c - 31):
         want, size = attend(s.q[r:r + 1], k[:n - c + r + 1], v[:n - c + r + 1])
         assert near(got[r], want[0], size[0])
+
+
+def scored(s, high, values, seed=5):
+    """All queries are one vector, keys are noise beside it, those that `high` names score 2^7.2 times the weight of the others; values are positive, `values` large."""
+    rng = np.random.default_rng(seed)
+    u = (rng.standard_normal(HD) * 1.5).astype(np.float32)
+    s.q_bits, s.q = bf16_round(np.broadcast_to(u, s.q.shape).copy())
+    u = s.q[0, 0].astype(np.float64)
+    for b, n in enumerate(s.lens):
+        at, up = s.places(b, range(n)), high(np.arange(n))
+        k = rng.standard_normal((n, s.nkv, HD)) * 0.1
+        k += (up * 7.2 * np.log(2) * np.sqrt(HD))[:, None, None] * u / (u @ u)
+        for i, x in enumerate((k, np.minimum(np.abs(rng.standard_normal((n, s.nkv, HD))), 4) * values)):
+            x = np.ascontiguousarray(x, np.float32)
+            if s.form == "q4":
+                s.raw[i][at], s.values[i][at] = pack(x)
+            else:
+                bits, s.values[i][at] = bf16_round(x)
+                s.raw[i][at] = bits.reshape(n, -1)
+    return s
+
+
+@pytest.mark.parametrize("form,values", [("bf16", 2.0 ** 120), ("q4", 2.0 ** 117)])
+@pytest.mark.parametrize("lens,counts", [([640], [640]), ([2000], [40]), ([900, 130], [30, 130])])
+def test_prefill_sums_near_the_end_of_f32(dev, form, values, lens, counts):
+    """Values so large that 2^8 times their sum is no f32 number, whose sum with weights of at most 1 is one: a row's reference may lag, and is not felt.  (bf16: 8 of
+    320 keys at a time are high, 4 bits: 64; the sums are below 2^126.)"""
+    some = 8 if form == "bf16" else 64
+    s = scored(Sequences(8, 2, 32, lens, counts, 45, form), lambda pos: (pos // 64 % 5 == 1) & (pos % 64 < some), values).put(dev)
+    got = widen(s.prefill().to_vec())
+    dev.sync()
+    want, size = s.reference()
+    assert np.isfinite(got).all() and near(got.reshape(want.shape), want, size)
+
+
+@pytest.mark.parametrize("form", ["bf16", "q4"])
+def test_values_near_the_other_end_of_f32(dev, form):
+    """Values of 2^-100: neither attention takes them for zeros."""
+    s = scored(Sequences(8, 2, 32, [640], [640 if form == "bf16" else 1], 47, form), lambda pos: pos // 64 % 5 == 1, 2.0 ** -98).put(dev)
+    got = s.prefill().to_vec()
+    want = s.reference()
+    # (the allowance of check_attention for results of zero is larger than these)
+    for out, terms in ((got, 1), *([(s.decode().to_vec(), 2)] if form == "q4" else [])):
+        check_attention(((widen(out) * 2.0 ** 98).astype(np.float32).view(np.uint32) >> 16).astype(np.uint16), want[0] * 2.0 ** 98, want[1] * 2.0 ** 98, terms)
+    dev.sync()
