@@ -3,8 +3,9 @@
 //
 // A warp works alone: no barrier, no wait but for its own copies.  It holds the query heads of one KV head as the columns of mma.sync's B operand and walks
 // chunks of 32 keys, which it copies to its own ring in shared memory a chunk ahead: S^T = K Q^T (keys are rows), softmax weights from a reference that
-// moves only when a score is 2^8 above it, O^T = V^T P^T.  Codes become bf16 in registers, exactly: 24 + c is four bits in the mantissa of 16, and
-// fma(24 + c, s, -24 s) = c s, where s has 5 significant bits and c 3.  Which row, column or step a value takes is free, as long as both operands agree:
+// begins 2^8 above the largest score and moves when one is above it (so that no weight is above 1), O^T = V^T P^T.  Codes become bf16 in registers, exactly:
+// 24 + c is four bits in the mantissa of 16, and fma(24 + c, s, -24 s) = c s, where s has 5 significant bits and c 3.  Which row, column or step a value
+// takes is free, as long as both operands agree:
 // a lane's 16 bytes of a key are its part of all eight steps of the scores, a lane's 8 bytes of four keys its part of all 128 rows of O.
 // Weights are two bf16 terms, within 2^-16.  Up to four query heads, columns 4 to 7 repeat columns 0 to 3 and take the second terms, so that these cost nothing.
 //
@@ -22,7 +23,7 @@ namespace tq {
 constexpr int kQdWarps = 4, kQdCtas = 4, kQdChunk = 32, kQdStages = 2;        // warps of a CTA, CTAs of an SM
 constexpr int kQdKeyBytes = 64, kQdValueBytes = 80;    // of a row in shared memory (80: four rows' 8-byte reads meet all banks)
 constexpr int kQdStageBytes = kQdChunk * (kQdKeyBytes + kQdValueBytes + 16);
-constexpr float kQdLag = 8.f;          // a reference may be so far below its maximum (log2)
+constexpr float kQdLag = 8.f;          // how far a maximum may grow before its reference does (log2)
 
 struct Q4DecodeParams {
   PackedSeqs s;
@@ -219,12 +220,13 @@ __global__ void __launch_bounds__(32 * kQdWarps, kQdCtas) q4_decode_kernel(const
     float top[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) top[j] = fmaxf(fmaxf(s[0][j], s[0][2 + j]), fmaxf(s[1][j], s[1][2 + j])) * p.scale_log2;
-    if (__any_sync(0xffffffffu, first || top[0] > ref[0] + kQdLag || top[1] > ref[1] + kQdLag)) {
+    if (__any_sync(0xffffffffu, first || top[0] > ref[0] || top[1] > ref[1])) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], x));
-        const float to_ref = fmaxf(first ? -FLT_MAX : ref[j], top[j]), by = first ? 0.f : ex2_ftz(ref[j] - to_ref);
+        // (2^8 above the maximum that it follows: no weight is above 1 before the maximum has grown so far)
+        const float to_ref = fmaxf(first ? -FLT_MAX : ref[j], top[j] + kQdLag), by = first ? 0.f : ex2_ftz(ref[j] - to_ref);
         ref[j] = to_ref;
         if (!first) {
           sum[j] *= by;

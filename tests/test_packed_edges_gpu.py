@@ -256,6 +256,14 @@ def test_prefill_sums_near_the_end_of_f32(dev, form, values, lens, counts):
     assert np.isfinite(got).all() and near(got.reshape(want.shape), want, size)
 
 
+def test_decode_over_four_bits_sums_near_the_end_of_f32(dev):
+    """As above; as many heads and positions as give a warp several chunks of 32 keys, every second of which is high."""
+    s = scored(Sequences(32, 32, 16, [900, 700, 33, 64, 800, 1000], [1] * 6, 46, "q4"), lambda pos: pos // 32 % 2 == 1, 2.0 ** 117).put(dev)
+    got = s.decode().to_vec()
+    dev.sync()
+    check_attention(got, *s.reference(), terms=2)
+
+
 @pytest.mark.parametrize("form", ["bf16", "q4"])
 def test_values_near_the_other_end_of_f32(dev, form):
     """Values of 2^-100: neither attention takes them for zeros."""
