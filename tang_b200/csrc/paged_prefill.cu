@@ -19,10 +19,11 @@
 // Few rows: a tile's keys are cut into parts, a CTA each, and a second kernel joins the results.
 //
 // What bounds it: products of 128 x 64 x 16 take 48 cycles, the bytes of their operands (32 would do for the multiplications), of 128 x 128 x 16 from tensor memory
-// 64: 640 a block, 1280 for two CTAs' blocks, beside 1000 of a scheduler's special function unit (a quarter of the weights are polynomials instead) and 900 of
-// its issue slots.  One prompt of 4096 positions, 32 heads, 8 KV heads, 125 us (1100 TFLOP/s, the tensor core 70 % busy; 151 us at the power limit), 13 prompts of
-// up to 1237 81 us; a few rows are a chain of blocks of 0.8 to 1 us (64 behind 2000 keys 16.4 us, one block 8.2).  Scores of 128 keys at a time, which cost the
-// tensor core less, wait for the products of the tile before: 167 us.
+// 64: 640 a block, 1280 for two CTAs' blocks, beside 1000 of a scheduler's special function unit and 900 of its issue slots.  One prompt of 4096 positions, 32 heads,
+// 8 KV heads, 118 us (1165 TFLOP/s; 141 us at the power limit, where a quarter of the weights as polynomials, to spare the special function unit, made it 149),
+// 13 prompts of up to 1237 80 us (94 at the power limit: a block of six is on the diagonal, and tiles begin and end), over 4 bits a block takes 1.6 times as long: its
+// rows are unpacked by one warp each for keys and values.  A few rows are a chain of blocks of 0.8 to 1 us (64 behind 2000 keys 16.4 us, one block 8.2).  Scores
+// of 128 keys at a time, which cost the tensor core less, wait for the products of the tile before: 167 us.
 #include <cfloat>
 #include <type_traits>
 
@@ -45,7 +46,6 @@ constexpr int kPpStage = 32 * 64;                     // bytes of results that a
 constexpr size_t kPpSmem = 1024 + 1024 + 2 * (size_t)kPfBox + 2 * kPpSlots * (size_t)kPpTile + 4 * (size_t)kPpStage;
 constexpr float kPpLag = 8.f;                         // how far a row's maximum may grow before its reference does (log2)
 constexpr int kPpMaxParts = 16;
-constexpr int kPpPoly = 4;                            // one of so many pairs of weights is a polynomial
 
 struct PackedPrefillParams {
   PackedSeqs s;
@@ -191,26 +191,6 @@ __device__ __forceinline__ PpItem pp_item(const PackedPrefillParams& p, int x, i
 // Adds a pair of bf16 to f32 sums.
 __device__ __forceinline__ void add_bf16x2(float& a, float& b, uint32_t w) {
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tadd.f32.bf16 %0, lo, %0;\n\tadd.f32.bf16 %1, hi, %1;\n\t}" : "+f"(a), "+f"(b) : "r"(w));
-}
-// 2^x of two x of up to 2^7, without the special function unit: x = r + f with a whole r and f within 1/2, a polynomial of degree 3 for 2^f (its coefficients
-// minimise the largest relative error, 7.5e-5, a fifteenth of what rounding to bf16 takes away) and r added to its exponent; zero below 2^-126, and a
-// NaN becomes too large for bf16.
-__device__ __forceinline__ void ex2_poly(uint64_t x, float& a, float& b) {
-  unpack2(x, a, b);
-  asm("max.NaN.f32 %0, %0, 0fC3000000;" : "+f"(a));     // -128
-  asm("max.NaN.f32 %0, %0, 0fC3000000;" : "+f"(b));
-  const uint64_t magic = pack2(12582912.f, 12582912.f), minus = pack2(-12582912.f, -12582912.f), neg = pack2(-1.f, -1.f);       // 1.5 * 2^23
-  x = pack2(a, b);
-  const uint64_t r = add2(x, magic), f = fma2(add2(r, minus), neg, x);
-  uint64_t y = pack2(0.055171669f, 0.055171669f);
-  y = fma2(y, f, pack2(0.24261112f, 0.24261112f));
-  y = fma2(y, f, pack2(0.69326099f, 0.69326099f));
-  y = fma2(y, f, pack2(0.99992807f, 0.99992807f));
-  float ra, rb, ya, yb;
-  unpack2(r, ra, rb);
-  unpack2(y, ya, yb);
-  a = __int_as_float(max(__float_as_int(ya) + (int)((uint32_t)__float_as_int(ra) << 23), 0));
-  b = __int_as_float(max(__float_as_int(yb) + (int)((uint32_t)__float_as_int(rb) << 23), 0));
 }
 // 32 columns of the warp's lanes; nothing may touch v before pp_landed.
 __device__ __forceinline__ void pp_ask(uint32_t taddr, float (&v)[32]) {
@@ -697,13 +677,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_con
           for (int k = 0; k < 16; ++k) {
             float a, b;
             const uint64_t t = fma2(pack2(v[c][2 * k], v[c][2 * k + 1]), scale2, less);
-            if (k % kPpPoly == kPpPoly - 1) {
-              ex2_poly(t, a, b);
-            } else {
-              unpack2(t, a, b);
-              a = ex2(a);
-              b = ex2(b);
-            }
+            unpack2(t, a, b);
+            a = ex2(a);
+            b = ex2(b);
             w[k] = pack_bf16(a, b);
             add_bf16x2(sum[2 * (k & 1)], sum[2 * (k & 1) + 1], w[k]);
           }
