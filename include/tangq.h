@@ -324,7 +324,7 @@ typedef enum tq_page_rows { TQ_PAGES_BF16 = 0, TQ_PAGES_Q4 = 1 } tq_page_rows;
 TQ_API size_t tq_q4_row_bytes(size_t n_kv_heads);
 /* The step between the fused q/k/v projection and the attention (crates/tang-train/examples/smollm.rs:84-95) for packed rows: x [rows][n_heads query heads,
  * n_kv_heads keys, n_kv_heads values of 128] f32 or bf16, ldx elements apart (0: dense; a multiple of 16 bytes).  Queries and keys are rotated as by
- * tq_rope_forward by their positions' rows of the tables [n_positions][64]; queries go to q_out bf16 [rows][n_heads*128], keys and values to the
+ * tq_rope_forward by their positions' rows of the tables [n_positions][64]; queries go to q_out (another buffer) bf16 [rows][n_heads*128], keys and values to the
  * cache rows of their positions.  Nothing is written for a row whose position is not its sequence's to write (the last tq_pages_extend was refused, the page has
  * other holders, the sequence stands in seqs twice) or has no row in the tables: it is reported by tq_sync. */
 TQ_API int tq_kv_append_paged(tq_ctx* ctx, const void* x_dev, int x_dtype, size_t ldx, const float* cos_dev, const float* sin_dev, size_t n_positions,

@@ -270,6 +270,8 @@ int tq_kv_append_paged(tq_ctx* ctx, const void* x_dev, int x_dtype, size_t ldx, 
   TQ_REQUIRE(ctx, ldx >= width && ldx * dtype_size(x_dtype) % 16 == 0, "tq_kv_append_paged: rows stand a multiple of 16 bytes apart and do not overlap");
   TQ_REQUIRE(ctx, (((uintptr_t)x_dev | (uintptr_t)cos_dev | (uintptr_t)sin_dev | (uintptr_t)q_out_dev | (uintptr_t)k_pages_dev | (uintptr_t)v_pages_dev) & 15) == 0,
              "tq_kv_append_paged: arrays must be 16-byte aligned");
+  TQ_REQUIRE(ctx, apart(x_dev, ((rows - 1) * ldx + width) * dtype_size(x_dtype), q_out_dev, rows * n_heads * kRowDim * 2),
+             "tq_kv_append_paged: queries need a buffer of their own (they are stored while other rows are read)");
   TQ_REQUIRE(ctx, n_positions >= 1, "tq_kv_append_paged: tables of the rotation without positions");
   AppendParams p;
   p.s = packed_seqs(pages, seqs_dev, seq_rows_dev, batch, rows);

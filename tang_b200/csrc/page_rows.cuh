@@ -108,6 +108,11 @@ __device__ __forceinline__ int page_row_of(const PackedSeqs& p, int seq, int pos
   return (page << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
 }
 
+// Two arrays that share no byte.
+inline bool apart(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  return (uintptr_t)a + a_bytes <= (uintptr_t)b || (uintptr_t)b + b_bytes <= (uintptr_t)a;
+}
+
 // What calls over packed rows ask of their arguments.
 inline int check_packed(tq_ctx* ctx, const char* call, const tq_pages* pages, const int* seqs, const int* seq_rows, size_t batch, size_t rows, size_t n_kv,
                         size_t head_dim, int page_rows_as) {

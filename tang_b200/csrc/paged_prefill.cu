@@ -818,7 +818,8 @@ extern "C" int tq_gqa_prefill_paged(tq_ctx* ctx, const void* q_dev, const void* 
   TQ_REQUIRE(ctx, max_len > 0 && max_len <= (1u << 30), "tq_gqa_prefill_paged: max_len must bound the sequence lengths");
   TQ_REQUIRE(ctx, (((uintptr_t)q_dev | (uintptr_t)k_pages_dev | (uintptr_t)v_pages_dev | (uintptr_t)out_dev) & 15) == 0,
              "tq_gqa_prefill_paged: arrays must be 16-byte aligned");
-  TQ_REQUIRE(ctx, q_dev != out_dev, "tq_gqa_prefill_paged: results need a buffer of their own (rows may be attended again)");
+  TQ_REQUIRE(ctx, apart(q_dev, rows * n_heads * kRowDim * 2, out_dev, rows * n_heads * kRowDim * 2),
+             "tq_gqa_prefill_paged: results need a buffer of their own (they are stored while other rows' queries are read)");
   const bool q4 = page_rows_as == TQ_PAGES_Q4;
   PackedPrefillParams p;
   p.s = packed_seqs(pages, seqs_dev, seq_rows_dev, batch, rows);

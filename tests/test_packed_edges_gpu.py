@@ -274,3 +274,30 @@ def test_values_near_the_other_end_of_f32(dev, form):
     for out, terms in ((got, 1), *([(s.decode().to_vec(), 2)] if form == "q4" else [])):
         check_attention(((widen(out) * 2.0 ** 98).astype(np.float32).view(np.uint32) >> 16).astype(np.uint16), want[0] * 2.0 ** 98, want[1] * 2.0 ** 98, terms)
     dev.sync()
+
+
+def test_results_that_share_memory_with_what_is_read_are_refused(dev):
+    """Queries of an append beside, within and into the rows it reads; results of the attention the same; next to them is another buffer."""
+    import tang_b200 as tb
+
+    s = Sequences(4, 2, 16, [20, 9], [4, 9], 48, "bf16").put(dev)
+    rows, width, nq = s.rows, 8 * HD, 4 * HD
+    cos, sin = (dev.upload(a) for a in tables(32))
+    whole = dev.upload(np.zeros(rows * width + 2 * rows * nq, np.uint16), tb.BF16)
+    part = lambda first, n: tb.Buffer(dev, whole.ptr + 2 * first, n, tb.BF16, owns=False)  # noqa: E731
+    x = part(rows * nq, rows * width)
+    append = lambda out: dev.kv_append_paged(x, cos, sin, s.pool, s.kb, s.vb, 2, rows, 4, 2, HD, seq_rows=s.seq_rows, q_out=out)  # noqa: E731
+    for first in (8, rows * nq, rows * nq + nq, rows * nq + rows * width - 8):
+        with pytest.raises(tb.TangqError):
+            append(part(first, rows * nq))
+    for first in (0, rows * nq + rows * width):
+        append(part(first, rows * nq))
+    dev.sync()
+    q = part(rows * nq, rows * nq)
+    attend_to = lambda out: dev.gqa_prefill_paged(q, s.kb, s.vb, s.pool, 2, rows, 4, 2, HD, 20, seq_rows=s.seq_rows, out=out)  # noqa: E731
+    for first in (8, rows * nq - 8, rows * nq, rows * nq + nq, 2 * rows * nq - 8):
+        with pytest.raises(tb.TangqError):
+            attend_to(part(first, rows * nq))
+    for first in (0, 2 * rows * nq):
+        attend_to(part(first, rows * nq))
+    dev.sync()
