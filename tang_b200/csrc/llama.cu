@@ -178,6 +178,50 @@ static int size_chunk(tq_llama* m, size_t R, const char* call) {
   return TQ_OK;
 }
 
+// A chunk of R rows through all layers, and the head for each sequence's last row.  attend(layer): what stands between the layer's q/k/v projection (p_qkv) and its
+// output projection (p_attn), the cache included; last_rows(): the last rows of p_xn to p_last.
+template <typename Attend, typename LastRows>
+static int prefill_rows(tq_llama* m, const int* token_ids_dev, size_t R, size_t batch, float* logits_dev, Attend attend, LastRows last_rows) {
+  tq_ctx* ctx = m->ctx;
+  const tq_llama_config& c = m->cfg;
+  const size_t d = c.d_model, q_dim = (size_t)m->heads_l * c.head_dim, kv_dim = (size_t)m->kv_l * c.head_dim;
+  int st;
+#define TQ_STEP(expr) \
+  if ((st = (expr)) != TQ_OK) return st;
+  TQ_STEP(tq_embedding(ctx, m->embed, TQ_BF16, token_ids_dev, R, d, c.vocab, m->p_h, TQ_F32));
+  bool have_delta = false;
+  for (size_t l = 0; l < m->layers.size(); ++l) {
+    const LlamaLayerW& L = m->layers[l];
+    TQ_STEP(tq_rms_norm(ctx, have_delta ? (const void*)m->p_delta : (const void*)m->p_h, TQ_F32, have_delta ? m->p_h : nullptr,
+                        L.attn_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, have_delta ? m->p_h : nullptr));
+    TQ_STEP(tq_qlinear(ctx, L.wqkv, m->p_xn, TQ_BF16, d, R, m->p_qkv, TQ_F32, q_dim + 2 * kv_dim, nullptr));
+    TQ_STEP(attend(L));
+    TQ_STEP(tq_qlinear(ctx, L.wo, m->p_attn, TQ_BF16, q_dim, R, m->p_delta, TQ_F32, d, nullptr));
+    TQ_STEP(tq_all_reduce_f32(ctx, m->comm, m->p_delta, R * d));
+    TQ_STEP(tq_rms_norm(ctx, m->p_delta, TQ_F32, m->p_h, L.ffn_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, m->p_h));
+    if (L.wgu->gate_up_interleaved) {
+      TQ_STEP(qlinear_fused(ctx, L.wgu, m->p_xn, nullptr, R, m->p_act, TQ_BF16, m->ffn_l, true, m->p_gu));
+    } else {
+      TQ_STEP(tq_qlinear(ctx, L.wgu, m->p_xn, TQ_BF16, d, R, m->p_gu, TQ_F32, 2 * (size_t)m->ffn_l, nullptr));
+      TQ_STEP(tq_swiglu(ctx, m->p_gu, m->p_gu + m->ffn_l, TQ_F32, 2 * (size_t)m->ffn_l, R, m->ffn_l, m->p_act, TQ_BF16));
+    }
+    TQ_STEP(tq_qlinear(ctx, L.wdown, m->p_act, TQ_BF16, m->ffn_l, R, m->p_delta, TQ_F32, d, nullptr));
+    TQ_STEP(tq_all_reduce_f32(ctx, m->comm, m->p_delta, R * d));
+    have_delta = true;
+  }
+  TQ_STEP(tq_rms_norm(ctx, m->p_delta, TQ_F32, m->p_h, m->final_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, m->p_h));
+  // the LM head only sees each sequence's last row
+  TQ_STEP(last_rows());
+  if (m->tp == 1) {
+    TQ_STEP(tq_qlinear(ctx, m->lm_head, m->p_last, TQ_BF16, d, batch, logits_dev, TQ_F32, c.vocab, nullptr));
+  } else {
+    TQ_STEP(tq_qlinear(ctx, m->lm_head, m->p_last, TQ_BF16, d, batch, m->logits_l, TQ_F32, m->vocab_l, nullptr));
+    TQ_STEP(tq_all_gather(ctx, m->comm, m->logits_l, logits_dev, batch * m->vocab_l * sizeof(float)));
+  }
+#undef TQ_STEP
+  return TQ_OK;
+}
+
 // How the sequences of a step over pages are told (tq_gqa_decode_paged).
 struct PagedStep {
   const tq_pages* pages;
@@ -420,49 +464,20 @@ int tq_llama_prefill(tq_llama* m, const int* token_ids_dev, const int* cache_sta
   TQ_REQUIRE(ctx, m->lm_head != nullptr, "tq_llama_prefill: head weights not set");
   for (auto& L : m->layers) TQ_REQUIRE(ctx, L.wqkv != nullptr, "tq_llama_prefill: a layer has no weights");
   const size_t R = batch * q_len, d = c.d_model, hd = c.head_dim;
-  const size_t q_dim = (size_t)m->heads_l * hd, kv_dim = (size_t)m->kv_l * hd;
-  const size_t seq_stride = (size_t)c.max_seq * kv_dim;
+  const size_t seq_stride = (size_t)c.max_seq * m->kv_l * hd;
   if (int grown = size_chunk(m, R, "tq_llama_prefill")) return grown;
-  int st;
-#define TQ_STEP(expr) \
-  if ((st = (expr)) != TQ_OK) return st;
-  const int Ri = (int)R, B = (int)batch;
-  TQ_STEP(tq_embedding(ctx, m->embed, TQ_BF16, token_ids_dev, R, d, c.vocab, m->p_h, TQ_F32));
-  bool have_delta = false;
-  for (size_t l = 0; l < m->layers.size(); ++l) {
-    const LlamaLayerW& L = m->layers[l];
-    TQ_STEP(tq_rms_norm(ctx, have_delta ? (const void*)m->p_delta : (const void*)m->p_h, TQ_F32, have_delta ? m->p_h : nullptr,
-                        L.attn_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, have_delta ? m->p_h : nullptr));
-    TQ_STEP(tq_qlinear(ctx, L.wqkv, m->p_xn, TQ_BF16, d, R, m->p_qkv, TQ_F32, q_dim + 2 * kv_dim, nullptr));
-    TQ_STEP(launch_qkv_post(ctx, m->p_qkv, m->cos_t, m->sin_t, cache_start_dev, nullptr, Ri, m->heads_l, m->kv_l, (int)hd, (int)c.max_seq,
-                            m->p_qb, L.k_cache, L.v_cache, seq_stride, (int)q_len));
-    TQ_STEP(tq_gqa_prefill(ctx, m->p_qb, L.k_cache, L.v_cache, cache_start_dev, batch, q_len, m->heads_l, m->kv_l, hd, seq_stride,
-                           m->p_attn, TQ_BF16));
-    TQ_STEP(tq_qlinear(ctx, L.wo, m->p_attn, TQ_BF16, q_dim, R, m->p_delta, TQ_F32, d, nullptr));
-    TQ_STEP(tq_all_reduce_f32(ctx, m->comm, m->p_delta, R * d));
-    TQ_STEP(tq_rms_norm(ctx, m->p_delta, TQ_F32, m->p_h, L.ffn_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, m->p_h));
-    if (L.wgu->gate_up_interleaved) {
-      TQ_STEP(qlinear_fused(ctx, L.wgu, m->p_xn, nullptr, R, m->p_act, TQ_BF16, m->ffn_l, true, m->p_gu));
-    } else {
-      TQ_STEP(tq_qlinear(ctx, L.wgu, m->p_xn, TQ_BF16, d, R, m->p_gu, TQ_F32, 2 * (size_t)m->ffn_l, nullptr));
-      TQ_STEP(tq_swiglu(ctx, m->p_gu, m->p_gu + m->ffn_l, TQ_F32, 2 * (size_t)m->ffn_l, R, m->ffn_l, m->p_act, TQ_BF16));
-    }
-    TQ_STEP(tq_qlinear(ctx, L.wdown, m->p_act, TQ_BF16, m->ffn_l, R, m->p_delta, TQ_F32, d, nullptr));
-    TQ_STEP(tq_all_reduce_f32(ctx, m->comm, m->p_delta, R * d));
-    have_delta = true;
-  }
-  TQ_STEP(tq_rms_norm(ctx, m->p_delta, TQ_F32, m->p_h, m->final_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, m->p_h));
-  // the LM head only sees each sequence's last row
-  TQ_CUDA(ctx, cudaMemcpy2DAsync(m->p_last, d * 2, m->p_xn + (q_len - 1) * d, q_len * d * 2, d * 2, batch, cudaMemcpyDeviceToDevice,
-                                 ctx->stream));
-  if (m->tp == 1) {
-    TQ_STEP(tq_qlinear(ctx, m->lm_head, m->p_last, TQ_BF16, d, B, logits_dev, TQ_F32, c.vocab, nullptr));
-  } else {
-    TQ_STEP(tq_qlinear(ctx, m->lm_head, m->p_last, TQ_BF16, d, B, m->logits_l, TQ_F32, m->vocab_l, nullptr));
-    TQ_STEP(tq_all_gather(ctx, m->comm, m->logits_l, logits_dev, (size_t)B * m->vocab_l * sizeof(float)));
-  }
-#undef TQ_STEP
-  return TQ_OK;
+  return prefill_rows(
+      m, token_ids_dev, R, batch, logits_dev,
+      [&](const LlamaLayerW& L) {
+        if (int st = launch_qkv_post(ctx, m->p_qkv, m->cos_t, m->sin_t, cache_start_dev, nullptr, (int)R, m->heads_l, m->kv_l, (int)hd, (int)c.max_seq, m->p_qb,
+                                     L.k_cache, L.v_cache, seq_stride, (int)q_len))
+          return st;
+        return tq_gqa_prefill(ctx, m->p_qb, L.k_cache, L.v_cache, cache_start_dev, batch, q_len, m->heads_l, m->kv_l, hd, seq_stride, m->p_attn, TQ_BF16);
+      },
+      [&]() -> int {
+        TQ_CUDA(ctx, cudaMemcpy2DAsync(m->p_last, d * 2, m->p_xn + (q_len - 1) * d, q_len * d * 2, d * 2, batch, cudaMemcpyDeviceToDevice, ctx->stream));
+        return TQ_OK;
+      });
 }
 
 int tq_llama_prefill_paged(tq_llama* m, const int* token_ids_dev, const tq_pages* pages, const int* seqs_dev, const int* seq_rows_dev, size_t batch,
@@ -481,49 +496,22 @@ int tq_llama_prefill_paged(tq_llama* m, const int* token_ids_dev, const tq_pages
   TQ_REQUIRE(ctx, m->lm_head != nullptr, "tq_llama_prefill_paged: head weights not set");
   for (auto& L : m->layers) TQ_REQUIRE(ctx, L.wqkv != nullptr, "tq_llama_prefill_paged: a layer has no weights");
   const size_t R = rows, d = c.d_model, hd = c.head_dim;
-  const size_t q_dim = (size_t)m->heads_l * hd, kv_dim = (size_t)m->kv_l * hd;
   if (int grown = size_chunk(m, R, "tq_llama_prefill_paged")) return grown;
-  int st;
-#define TQ_STEP(expr) \
-  if ((st = (expr)) != TQ_OK) return st;
-  const int B = (int)batch;
-  TQ_STEP(tq_embedding(ctx, m->embed, TQ_BF16, token_ids_dev, R, d, c.vocab, m->p_h, TQ_F32));
-  bool have_delta = false;
-  for (size_t l = 0; l < m->layers.size(); ++l) {
-    const LlamaLayerW& L = m->layers[l];
-    TQ_STEP(tq_rms_norm(ctx, have_delta ? (const void*)m->p_delta : (const void*)m->p_h, TQ_F32, have_delta ? m->p_h : nullptr,
-                        L.attn_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, have_delta ? m->p_h : nullptr));
-    TQ_STEP(tq_qlinear(ctx, L.wqkv, m->p_xn, TQ_BF16, d, R, m->p_qkv, TQ_F32, q_dim + 2 * kv_dim, nullptr));
-    // (max_len for the tables' length: a position that the attention would not see is reported and not written)
-    TQ_STEP(tq_kv_append_paged(ctx, m->p_qkv, TQ_F32, 0, m->cos_t, m->sin_t, max_len, pages, seqs_dev, seq_rows_dev, batch, R, m->heads_l, m->kv_l, hd, m->p_qb,
-                               L.k_cache, L.v_cache, TQ_PAGES_BF16));
-    TQ_STEP(tq_gqa_prefill_paged(ctx, m->p_qb, L.k_cache, L.v_cache, TQ_PAGES_BF16, pages, seqs_dev, seq_rows_dev, batch, R, m->heads_l, m->kv_l, hd, max_len,
-                                 m->p_attn));
-    TQ_STEP(tq_qlinear(ctx, L.wo, m->p_attn, TQ_BF16, q_dim, R, m->p_delta, TQ_F32, d, nullptr));
-    TQ_STEP(tq_all_reduce_f32(ctx, m->comm, m->p_delta, R * d));
-    TQ_STEP(tq_rms_norm(ctx, m->p_delta, TQ_F32, m->p_h, L.ffn_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, m->p_h));
-    if (L.wgu->gate_up_interleaved) {
-      TQ_STEP(qlinear_fused(ctx, L.wgu, m->p_xn, nullptr, R, m->p_act, TQ_BF16, m->ffn_l, true, m->p_gu));
-    } else {
-      TQ_STEP(tq_qlinear(ctx, L.wgu, m->p_xn, TQ_BF16, d, R, m->p_gu, TQ_F32, 2 * (size_t)m->ffn_l, nullptr));
-      TQ_STEP(tq_swiglu(ctx, m->p_gu, m->p_gu + m->ffn_l, TQ_F32, 2 * (size_t)m->ffn_l, R, m->ffn_l, m->p_act, TQ_BF16));
-    }
-    TQ_STEP(tq_qlinear(ctx, L.wdown, m->p_act, TQ_BF16, m->ffn_l, R, m->p_delta, TQ_F32, d, nullptr));
-    TQ_STEP(tq_all_reduce_f32(ctx, m->comm, m->p_delta, R * d));
-    have_delta = true;
-  }
-  TQ_STEP(tq_rms_norm(ctx, m->p_delta, TQ_F32, m->p_h, m->final_norm, TQ_BF16, R, d, c.eps, m->p_xn, TQ_BF16, m->p_h));
-  // the LM head only sees each sequence's last row
-  TQ_CUDA(ctx, launch_k(ctx, last_rows_kernel, dim3((unsigned)B), dim3(256), 0, (const __nv_bfloat16*)m->p_xn, seq_rows_dev, (int)R, (int)d,
-                        (__nv_bfloat16*)m->p_last));
-  if (m->tp == 1) {
-    TQ_STEP(tq_qlinear(ctx, m->lm_head, m->p_last, TQ_BF16, d, B, logits_dev, TQ_F32, c.vocab, nullptr));
-  } else {
-    TQ_STEP(tq_qlinear(ctx, m->lm_head, m->p_last, TQ_BF16, d, B, m->logits_l, TQ_F32, m->vocab_l, nullptr));
-    TQ_STEP(tq_all_gather(ctx, m->comm, m->logits_l, logits_dev, (size_t)B * m->vocab_l * sizeof(float)));
-  }
-#undef TQ_STEP
-  return TQ_OK;
+  return prefill_rows(
+      m, token_ids_dev, R, batch, logits_dev,
+      [&](const LlamaLayerW& L) {
+        // (max_len for the tables' length: a position that the attention would not see is reported and not written)
+        if (int st = tq_kv_append_paged(ctx, m->p_qkv, TQ_F32, 0, m->cos_t, m->sin_t, max_len, pages, seqs_dev, seq_rows_dev, batch, R, m->heads_l, m->kv_l, hd,
+                                        m->p_qb, L.k_cache, L.v_cache, TQ_PAGES_BF16))
+          return st;
+        return tq_gqa_prefill_paged(ctx, m->p_qb, L.k_cache, L.v_cache, TQ_PAGES_BF16, pages, seqs_dev, seq_rows_dev, batch, R, m->heads_l, m->kv_l, hd, max_len,
+                                    m->p_attn);
+      },
+      [&]() -> int {
+        TQ_CUDA(ctx, launch_k(ctx, last_rows_kernel, dim3((unsigned)batch), dim3(256), 0, (const __nv_bfloat16*)m->p_xn, seq_rows_dev, (int)R, (int)d,
+                              (__nv_bfloat16*)m->p_last));
+        return TQ_OK;
+      });
 }
 
 }  // extern "C"
