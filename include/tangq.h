@@ -337,8 +337,8 @@ TQ_API int tq_kv_read_paged(tq_ctx* ctx, const void* k_pages_dev, const void* v_
                             size_t head_dim, void* k_out_dev, void* v_out_dev);
 /* tq_gqa_prefill over pages, for packed rows: q bf16 [rows][n_heads*128], out (another buffer) bf16 the same; a row attends its sequence's positions up to its own, cached ones
  * and those of the rows before it.  n_heads/n_kv_heads is 1 to 8.  max_len bounds the sequences' lengths: what lies behind it is not attended.  Results of a
- * sequence with a page that does not exist are not defined.  Weights enter the tensor cores as bf16, 2^-9 of themselves off, and what is divided by is the sum
- * of what entered. */
+ * sequence with a page that does not exist are not defined.  Weights enter the tensor cores as bf16, up to 2^-8 of themselves off, and what is divided by is the sum
+ * of what entered.  Weights are at most 1 and sums are f32: n values above 2^128 / n may leave it. */
 TQ_API int tq_gqa_prefill_paged(tq_ctx* ctx, const void* q_dev, const void* k_pages_dev, const void* v_pages_dev, int page_rows_as,
                                 const tq_pages* pages, const int* seqs_dev_or_null, const int* seq_rows_dev_or_null, size_t batch, size_t rows,
                                 size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t max_len, void* out_dev);

@@ -9,8 +9,9 @@
 // a lane's 16 bytes of a key are its part of all eight steps of the scores, a lane's 8 bytes of four keys its part of all 128 rows of O.
 // Weights are two bf16 terms, within 2^-16.  Up to four query heads, columns 4 to 7 repeat columns 0 to 3 and take the second terms, so that these cost nothing.
 //
-// What bounds it: instructions.  A chunk's 32 keys and values of a head are 790 of them, 400 to unpack (a word of eight codes four shifts, four masks, four fused
-// operations), 100 to ask for the next one, 32 products; with four warps a scheduler issues 0.58 a cycle.  64 sequences of up to 4096 positions, 8 KV heads, 156 MB,
+// What bounds it: a warp's way through a chunk, scores, vote, exponentials, transposes and values one after the other: 3.4 us for 32 keys and values of a head, 790
+// instructions, of which 400 unpack (a word of eight codes four shifts, four masks, four fused operations), 100 ask for the next chunk and 32 are products.  Four warps a
+// scheduler issue 0.58 a cycle of them, and ask for 47 % of the memory's rate.  64 sequences of up to 4096 positions, 8 KV heads, 156 MB,
 // 51.3 us (3.0 TB/s, 47 % of the memory's rate; the same without any copies 47); one sequence of 700 8.4 us; three of up to 65537 30.9.  Tensor copies instead of
 // cp.async 53.3 us (boxes of 64 and of 16 bytes); one sum of the scores of a half chunk instead of two 53.2; 12 warps an SM with three chunks each 53.9.
 #include <cfloat>
@@ -432,7 +433,8 @@ extern "C" int tq_gqa_decode_paged_q4(tq_ctx* ctx, const void* q_dev, const void
   auto kern = p.group <= 4 ? q4_decode_kernel<true> : q4_decode_kernel<false>;
   TQ_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most_smem));
   TQ_CUDA(ctx, launch_k(ctx, kern, dim3((unsigned)n_ctas), dim3(32 * kQdWarps), smem, p));
-  // A warp a query head where a sequence has few parts on the average (in CTAs of four heads), sixteen where it has many.
+  // A warp a query head where a sequence has few parts on the average (in CTAs of four heads), sixteen where it has many.  (From 16 on: 64 sequences of up to 4096
+  // positions take 51.3 us, from 4 on 73.8; one of 700 8.6 and 8 of 8000 23.6, from 64 on 12.4 and 32.9.)
   const unsigned heads = (unsigned)(batch * n_heads);
   if ((size_t)p.n_shares > 16 * batch) TQ_CUDA(ctx, launch_k(ctx, q4_join_kernel<16>, dim3(heads), dim3(512), 0, p));
   else TQ_CUDA(ctx, launch_k(ctx, q4_join_kernel<1>, dim3((heads + 3) / 4), dim3(128), 0, p));

@@ -301,3 +301,13 @@ def test_results_that_share_memory_with_what_is_read_are_refused(dev):
     for first in (0, 2 * rows * nq):
         attend_to(part(first, rows * nq))
     dev.sync()
+
+
+@pytest.mark.parametrize("form", ["bf16", "q4"])
+def test_as_many_parts_as_there_may_be(dev, form):
+    """A tile's keys in 32 parts, 31 of 10 or 11 blocks, and two sequences of which one has fewer blocks than parts."""
+    for lens, counts in (([20011], [3]), ([9000, 40], [2, 5])):
+        s = Sequences(4, 1, 64, lens, counts, 49, form).put(dev)
+        got = s.prefill().to_vec()
+        dev.sync()
+        check_attention(got, *s.reference(), terms=1)
