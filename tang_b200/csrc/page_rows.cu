@@ -61,12 +61,11 @@ __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float s) {
 // A CTA takes ROWS rows and 128 eighths of a head: 32 bytes (f32) in, 16 or 4 out for a thread and row.  Rows' places are looked up by a warp each
 // (starts, sequence, length, page, holders: five loads one after the other) while the values are on their way.  What bounds it: the bytes (5000 rows of 32 + 16
 // heads f32 to bf16 pages, 200 MB, 35.0 us, 5.7 TB/s), beside the look-ups (CTAs of 256 threads 37.1, of 512 44.1; eight rows each 47.2); to 4 bits
-// instructions and loads on their way (5800 rows from bf16 28 us, 30 with single products and quotients; two groups of columns a thread, for half as many
-// look-ups, 32; one warp's lanes for all rows' look-ups no difference).  With its reading back: four rows 37.0, two 39.2, three 37.7, four in shared memory by
-// cp.async 39.0.  A single row 4.2 us.
-// (CTAs of an SM: what the values alone take; without the bound the look-up takes four registers and two CTAs more, appending and reading back 39.7 instead of 38.7.)
+// instructions and loads on their way, 73 % of the issue slots (5973 rows from bf16 31.7 us; 30 instead of 28 in an earlier form with single products and quotients, 32
+// with two groups of columns a thread, for half as many look-ups; one warp's lanes for all rows' look-ups no difference).  With its reading back 38.8: in the earlier
+// form four rows 37.0, two 39.2, three 37.7, four in shared memory by cp.async 39.0.  A single row 4.2 us.
 template <typename X, int ROWS, bool Q4>
-__global__ void __launch_bounds__(kAppendThreads, ROWS == 1 ? 16 : sizeof(X) == 2 ? 12 : 9) kv_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendParams p) {
   __shared__ int place_s[ROWS], pos_s[ROWS];           // cache row (-1: none), position
   pdl_wait();
   pdl_launch_dependents();
@@ -83,7 +82,7 @@ __global__ void __launch_bounds__(kAppendThreads, ROWS == 1 ? 16 : sizeof(X) == 
   if (warp < ROWS) {
     int place = -1, pos = 0;
     if (m0 + warp < p.s.rows) {
-      const PackedRow row = packed_row(p.s, m0 + warp, lane);
+      const PackedRow row = packed_row(p.s, m0 + warp, lane, p.err);
       int why = 0, page = 0, same = 0;
       if (row.seq >= 0) {
         const int refused = p.s.refused[row.seq];      // (on its way beside the page)
@@ -101,8 +100,10 @@ __global__ void __launch_bounds__(kAppendThreads, ROWS == 1 ? 16 : sizeof(X) == 
           if (same != 1 || refused != 0 || p.s.refs[page] != 1) why = DERR_PAGE_LIST;
         }
       }
-      if (why) place = -1;
-      if ((why || row.bad) && lane == 0 && blockIdx.y == 0) atomicCAS(p.err, 0, why ? why : (int)DERR_PAGE_LIST);
+      if (why) {
+        place = -1;
+        if (lane == 0 && blockIdx.y == 0) atomicCAS(p.err, 0, why);
+      }
     }
     if (lane == 0) {
       place_s[warp] = place;
@@ -191,7 +192,8 @@ struct ReadParams {
   int* err;
 };
 
-// A CTA takes ROWS rows: eight values a thread and turn, keys and then values.
+// A CTA takes ROWS rows: eight values a thread and turn, keys and then values.  5973 rows of 8 heads from 4 bits, 31 MB, 8.3 us (a single row 4.2): start, look-up, loads and
+// stores once each, too short for the memory's rate (4.8).
 template <bool Q4, int ROWS>
 __global__ void __launch_bounds__(kAppendThreads) kv_read_kernel(const ReadParams p) {
   __shared__ int place_s[ROWS];
@@ -201,12 +203,9 @@ __global__ void __launch_bounds__(kAppendThreads) kv_read_kernel(const ReadParam
   if (warp < ROWS) {
     int place = -1;
     if (m0 + warp < p.s.rows) {
-      const PackedRow row = packed_row(p.s, m0 + warp, lane);
+      const PackedRow row = packed_row(p.s, m0 + warp, lane, p.err);
       if (row.seq >= 0) place = page_row_of(p.s, row.seq, row.pos);
-      if (lane == 0) {
-        if (row.bad) atomicCAS(p.err, 0, (int)DERR_PAGE_LIST);
-        else if (row.seq >= 0 && place < 0) atomicCAS(p.err, 0, (int)DERR_POSITION);
-      }
+      if (row.seq >= 0 && place < 0 && lane == 0) atomicCAS(p.err, 0, (int)DERR_POSITION);
     }
     if (lane == 0) place_s[warp] = place;
   }

@@ -58,17 +58,18 @@ __device__ __forceinline__ int packed_seq(const PackedSeqs& p, int i) {
 // Where a packed row stands.
 struct PackedRow {
   int seq, pos;                        // of the pool (-1: nowhere), position
-  int i;                               // of the list
-  bool bad;                            // there is something to report: about this row, or the starts as a whole
 };
 // Starts need not be what they should be: they are the device's.  Rows seq_rows[i] .. seq_rows[i+1]-1 are sequence i's if no start before seq_rows[i] is larger (the first
 // one is 0) and they end neither before they begin nor behind the last row; such rows are never two sequences'.  Every kernel goes by that, whatever else the list
 // holds, so that a row which is appended is attended, and one which is not is left alone by all of them.
 //
-// Row m's, by a whole warp.  Rows behind the last sequence are nowhere, and that is nothing to report; a list with something to report need not be the row's fault.
-__device__ __forceinline__ PackedRow packed_row(const PackedSeqs& p, int m, int lane) {
-  PackedRow r{-1, 0, m, false};
-  int first = m, count = 1;
+// Row m's, by a whole warp, which reports what is wrong with it, or with the list.  Rows behind the last sequence are nowhere, and that is nothing to report.
+__device__ __forceinline__ PackedRow packed_row(const PackedSeqs& p, int m, int lane, int* err) {
+  const PackedRow nowhere{-1, 0};
+  auto report = [&] {
+    if (lane == 0) atomicCAS(err, 0, (int)DERR_PAGE_LIST);
+  };
+  int i = m, first = m, count = 1;
   if (p.seq_rows) {
     unsigned seen = 0;                 // starts at or before the row; from bit 16 on, those that are not what they should be
 #pragma unroll 4
@@ -77,27 +78,24 @@ __device__ __forceinline__ PackedRow packed_row(const PackedSeqs& p, int m, int 
       seen += (start <= m) + (start > next || (j == 0 && start != 0) ? 1u << 16 : 0u);
     }
     seen = __reduce_add_sync(0xffffffffu, seen);
-    int behind = seen & 0xFFFFu;       // the first start behind the row
-    r.bad = seen >> 16;
-    int largest = 0;                   // (of the starts before it: its neighbour, where they ascend)
-    if (r.bad) {
-      for (behind = 0; behind <= p.batch && p.seq_rows[behind] <= m; ++behind) largest = max(largest, p.seq_rows[behind]);
+    if (seen >> 16) {
+      report();
+      int largest = 0;                 // of the starts before the first one behind the row
+      for (seen = 0; (int)seen <= p.batch && p.seq_rows[seen] <= m; ++seen) largest = max(largest, p.seq_rows[seen]);
+      if (seen == 0 || (int)seen > p.batch) return nowhere;
+      if (p.seq_rows[seen - 1] != largest || (seen == 1 && largest != 0) || p.seq_rows[seen] > p.rows) return nowhere;
     }
-    if (behind > p.batch || behind == 0) return r;
-    r.i = behind - 1;
-    first = p.seq_rows[r.i];
-    const int end = p.seq_rows[behind];
-    count = end - first;
-    if (r.bad && (first != largest || (r.i == 0 && first != 0) || end > p.rows)) return r;
+    if ((int)seen > p.batch) return nowhere;
+    i = (int)seen - 1;
+    first = p.seq_rows[i];
+    count = p.seq_rows[i + 1] - first;
   }
-  const int s = packed_seq(p, r.i), len = s < 0 ? 0 : p.lens[s];
+  const int s = packed_seq(p, i), len = s < 0 ? 0 : p.lens[s];
   if (s < 0 || len < count || len > (long long)p.table_ld << p.page_shift) {
-    r.bad = true;
-    return r;
+    report();
+    return nowhere;
   }
-  r.seq = s;
-  r.pos = len - count + (m - first);
-  return r;
+  return PackedRow{s, len - count + (m - first)};
 }
 
 // Cache row of a position, the cache seen as one; -1 where the table names a page that does not exist.

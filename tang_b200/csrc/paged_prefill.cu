@@ -779,7 +779,7 @@ __global__ void __launch_bounds__(128) paged_prefill_join_kernel(const PackedPre
   if (i >= heads) return;
   // rows that nobody attended for are left as they are
   const int m = (int)(i / p.n_heads);
-  if (packed_row(p.s, m, lane).seq < 0) return;
+  if (packed_row(p.s, m, lane, p.err).seq < 0) return;
   const float2 ml = lane < p.parts ? *reinterpret_cast<const float2*>(p.part_ml + (lane * heads + i) * 2) : make_float2(-FLT_MAX, 0.f);
   const float top = warp_max(ml.x), w = ex2(ml.x - top), l = warp_sum(ml.y * w);
   float o[4] = {0.f, 0.f, 0.f, 0.f};
