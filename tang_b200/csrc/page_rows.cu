@@ -36,9 +36,9 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
   return r;
 }
 // The codes of eight values of a scale s, the first in the lowest four bits: 8 + x / s rounded to nearest even.  The quotient comes from the reciprocal with one
-// correction by its remainder, which fused operations have exactly (Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990): 2^-46 of it off before its last rounding.  s has 5 bits, a tie (k + 1/2) s nine at most, so
-// that the f32 numbers beside a tie are 2^-24 (1 + 2^-9) of it away and their quotients do not round to one.  (The compiler's division instead: 5800 rows of 1024
-// keys and values from bf16 41.8 us.)  Adding 1.5 * 2^23 + 8 leaves the code in the
+// correction by its remainder, which fused operations have exactly (Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990): 2^-46
+// of it off before its last rounding.  s has 5 bits, a tie (k + 1/2) s nine at most, so that the f32 numbers beside a tie are 2^-24 (1 + 2^-9) of it away and their
+// quotients do not round to one.  (The compiler's division instead: 5800 rows of 1024 keys and values from bf16 41.8 us.)  Adding 1.5 * 2^23 + 8 leaves the code in the
 // number's low bits, and what else is in them is the same for all.
 __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float s) {
   float inv;

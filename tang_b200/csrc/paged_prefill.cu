@@ -14,18 +14,20 @@
 // from tile to tile on their own: copies and scores of the next one run while the results of this one are stored (a tile a CTA: look-up, first copies and results
 // took 10000 of 21000 cycles for 8 blocks).  A weight is one bf16 number, and the sum that results are
 // divided by is that of the numbers as they entered: a row of a few keys, where the roundings do not average out, is then nearer (the largest weight need not
-// be 1 for that, so that the reference may lag: a row's sums are rescaled only when its maximum grew by more than 2^8.  It begins 2^8 above the maximum, so that weights
-// are 2^-8 to 1: sums hold what those of weights of at most 1 hold, and values of 2^-110 count.  What it costs is that the largest weight is rounded like the others:
-// errors against 64 bits of 1.70e-3 to 2.19e-3, and 1.70e-3 to 1.89e-3 with a reference that follows every maximum, for 176 instead of 149 us; the results' own rounding
-// is 1.57e-3 to 1.66e-3.  The sum over keys with a running reference is that of Milakov and Gimelshein, Online normalizer calculation for softmax, 2018).
+// be 1 for that, so that the reference may lag: a row's sums are rescaled only when its maximum grew by more than 2^8; sums with a running reference are those of
+// Milakov and Gimelshein, Online normalizer calculation for softmax, 2018).  It begins 2^8 above the maximum, so that weights are 2^-8 to 1: sums hold what those of
+// weights of at most 1 hold, and values of 2^-110 count.  What the lag costs is that the largest weight is rounded like the others: errors against 64 bits of 1.70e-3
+// to 2.19e-3, with a reference that follows every maximum 1.70e-3 to 1.89e-3, but one prompt of 4096 then takes 183 instead of 146 us; the results' own rounding is
+// 1.57e-3 to 1.66e-3.
 // Few rows: a tile's keys are cut into parts, a CTA each, and a second kernel joins the results.
 //
 // What bounds it: products of 128 x 64 x 16 take 48 cycles, the bytes of their operands (32 would do for the multiplications), of 128 x 128 x 16 from tensor memory
 // 64: 640 a block, 1280 for two CTAs' blocks, beside 1000 of a scheduler's special function unit and 900 of its issue slots.  One prompt of 4096 positions, 32 heads,
-// 8 KV heads, 118 us (1165 TFLOP/s; 141 us at the power limit, where a quarter of the weights as polynomials, to spare the special function unit, made it 149),
-// 13 prompts of up to 1237 80 us (94 at the power limit), 57 blocks and 8 tiles a CTA, where what lies between tiles is a quarter of the time.  Over 4 bits the same takes 1.35
-// to 1.45 times as long: one warp each unpacks keys and values, on the schedulers of two of the softmax warps.  A few rows are a chain of blocks of 0.8 to 1 us (64 behind 2000 keys 16.4 us, one block 8.2).  Scores
-// of 128 keys at a time, which cost the tensor core less, wait for the products of the tile before: 167 us.
+// 8 KV heads, 118 to 122 us (1140 TFLOP/s; 141 to 147 at the power limit, where a quarter of the weights as polynomials, to spare the special function unit, made 141
+// into 149), 13 prompts of up to 1237 80 us (94 to 97 at the power limit), 57 blocks and 8 tiles a CTA, where what lies between tiles is a quarter of the time.  Over 4
+// bits the same takes 1.35 to 1.45 times as long: one warp each unpacks keys and values, on the schedulers of two of the softmax warps.  A few rows are a chain of blocks of
+// 0.8 to 1 us (64 behind 2000 keys 16.4 us, one block 8.2).  Scores of 128 keys at a time, which cost the tensor core less, wait for the products of the tile before:
+// 167 us.
 #include <cfloat>
 #include <type_traits>
 
